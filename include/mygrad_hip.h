@@ -31,8 +31,8 @@ typedef enum {
   MG_ERR_NOT_INIT = -6     /* mg_init() has not succeeded */
 } mg_status;
 
-/* MG_F16 (IEEE binary16) is a storage type only: mg_cast and mg_accumulate take it, every other
- * entry point computes in float32 or float64 and refuses it (MG_ERR_UNSUPPORTED). */
+/* MG_F16 (IEEE binary16) is a storage type only: mg_cast, mg_accumulate, mg_attention_*, mg_cache_write and mg_head_norm_*
+ * take it (and sum in float32), every other entry point computes in float32 or float64 and refuses it (MG_ERR_UNSUPPORTED). */
 typedef enum { MG_F32 = 0, MG_F64 = 1, MG_F16 = 2 } mg_dtype;
 
 /* Shapes of one convolution  x:(N,C,X...) * w:(F,C,W...) -> out:(N,F,G...).
@@ -85,6 +85,41 @@ typedef struct {
   int64_t lead;
   int64_t X[MG_MAX_ND], W[MG_MAX_ND], S[MG_MAX_ND], D[MG_MAX_ND], G[MG_MAX_ND];
 } mg_window_desc;
+
+/* One attention: q:(B, TQ, HQ, D) over k, v:(B, TK, HK, D), out like q; HQ is a multiple of HK, query head h reads key head
+ * h / (HQ / HK).  1 <= D <= 256.  The pointers are device memory and may be null.
+ * Query i of item b stands at place p = i + n - TQ among the keys, n = lengths[b] (TK without lengths): the last query is at the last
+ * key.  It sees keys [0, n); of these with `starts` / `ends` those of [starts[b, p], ends[b, p]) only (p outside [0, n): none);
+ * with `causal` none behind p; with a window w none at p - w or before (and, not causal, at p + w or behind); with `prefix` also
+ * the first prefix[b] keys of its document, wherever it stands (not together with a window). */
+typedef struct {
+  int32_t dtype;           /* mg_dtype of q, k, v, out and their gradients */
+  int32_t causal;
+  int64_t B, TQ, TK, HQ, HK, D;
+  int64_t window;          /* 0: none; at most 2^30 */
+  double scale;            /* of the products */
+  double cap;              /* scores become cap * tanh(score / cap); 0: they stay */
+  const int32_t *lengths;  /* (B) keys in use, clamped to [0, TK] */
+  const int32_t *prefix;   /* (B) */
+  const int32_t *starts;   /* (B, TK) first key of the document that key j belongs to */
+  const int32_t *ends;     /* (B, TK) the key behind its last one */
+  const float *slopes;     /* (HQ): slopes[h] * |p - j| is taken off a score, after the cap */
+} mg_attention_desc;
+
+/* A norm for each head of x:(tokens, heads, D) and rotary positions: pair p of the first 2 * pairs values turns by the angle whose
+ * cos and sin are table[positions[token, axis_of[p]], p] (rows outside the table are clamped to it).  positions and axis_of are
+ * device memory, read where pairs > 0.  1 <= D <= 1024. */
+typedef struct {
+  int32_t dtype;             /* mg_dtype of x, weight, y and gradients; the table is float32 (float64 for MG_F64) */
+  int32_t norm;              /* 0: rotation only */
+  int32_t weight_heads;      /* 0: no weight, 1: (D) for all heads, heads: (heads, D) */
+  int32_t interleaved;       /* pairs (2p, 2p + 1); else (p, p + pairs) */
+  int32_t axes, reserved;
+  int64_t tokens, heads, D, pairs, table_rows;
+  double eps;                /* >= 0, added to the mean of the squares */
+  const int32_t *positions;  /* (tokens, axes) */
+  const uint8_t *axis_of;    /* (pairs) */
+} mg_head_norm_desc;
 
 typedef struct {
   char name[64];      /* hipDeviceProp_t::gcnArchName */
@@ -144,7 +179,8 @@ int mg_event_destroy(void *event);
  * 9 element-wise kernel, 10 whole-array sum, 11 - 14 batch norm (statistics, application, the
  * gradients' sums, their application), 15 and 16 repeat and its gradient, 17 window copy, 18 sum over
  * axes, 19 permutation, 20 batched product, 21 the single-precision filter gradient behind one on
- * three bf16 parts (which returns at once as a rule). */
+ * three bf16 parts (which returns at once as a rule), 22 attention, 23 - 25 its gradient (products of rows, dq, dk and dv),
+ * 26 tokens written to a cache, 27 and 28 the norm of heads and its gradient, 29 joining an attention that was split along its keys. */
 int mg_timing_enable(int on);
 int mg_timing_read(int32_t *tags, float *ms, int capacity, int *count);
 /* Suspends (1) or resumes (0) the recording without waiting for the stream and without
@@ -421,6 +457,31 @@ int mg_repeat_bwd(int dtype, int64_t outer, int64_t n, int64_t inner, int64_t re
  * sliding_window_view(x, W, S, D), src/mygrad/nnet/layers/utils.py:7-228 (the view itself is a
  * host-side stride trick and moves nothing). */
 int mg_window_gather(const mg_window_desc *desc, const void *x, void *out);
+
+/* ---- attention (no counterpart in the reference) ---- */
+
+/* out = softmax(scores) v over the keys each query sees; a query that sees none gets zeros.  lse:(B, HQ, TQ), float32 (float64 for
+ * MG_F64), receives the logarithm of each row's sum of exponentials (+infinity for a row without any weight), for mg_attention_bwd; it
+ * may be null.  Sums are carried in float32 (float64 for MG_F64).  What a query does not see does not touch its result, whatever it
+ * holds. */
+int mg_attention_fwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, void *out, void *lse);
+
+/* Gradients from grad (like out), `out` and `lse` of mg_attention_fwd.  dq, or dk and dv together, may be null (not wanted).  Fixed
+ * order of additions: run-to-run identical. */
+int mg_attention_bwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, const void *out, const void *lse,
+                     const void *grad, void *dq, void *dk, void *dv);
+
+/* keys, values:(B, capacity, row): token t of k, v:(B, T, row) goes to place lengths[b] - T + t of item b (lengths on the device); what
+ * falls outside [0, capacity) is left out.  `row` counts values of `dtype`. */
+int mg_cache_write(int dtype, int64_t B, int64_t T, int64_t capacity, int64_t row, const int32_t *lengths, const void *k, const void *v,
+                   void *keys, void *values);
+
+/* y = turn(weight * x / sqrt(mean(x^2) + eps)) for each head of each token; table:(table_rows, pairs, 2) holds cos and sin. */
+int mg_head_norm_fwd(const mg_head_norm_desc *desc, const void *x, const void *weight, const void *table, void *y);
+
+/* Its gradients; dx or dweight may be null (not wanted).  dweight is summed over tokens (and heads where they share it) in float64 over
+ * a fixed partition. */
+int mg_head_norm_bwd(const mg_head_norm_desc *desc, const void *x, const void *weight, const void *table, const void *grad, void *dx, void *dweight);
 
 #ifdef __cplusplus
 }

@@ -100,6 +100,46 @@ class WindowDesc(ctypes.Structure):
     ]
 
 
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("B", ctypes.c_int64),
+        ("TQ", ctypes.c_int64),
+        ("TK", ctypes.c_int64),
+        ("HQ", ctypes.c_int64),
+        ("HK", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("window", ctypes.c_int64),
+        ("scale", ctypes.c_double),
+        ("cap", ctypes.c_double),
+        ("lengths", ctypes.c_void_p),
+        ("prefix", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("ends", ctypes.c_void_p),
+        ("slopes", ctypes.c_void_p),
+    ]
+
+
+class HeadNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("weight_heads", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("pairs", ctypes.c_int64),
+        ("table_rows", ctypes.c_int64),
+        ("eps", ctypes.c_double),
+        ("positions", ctypes.c_void_p),
+        ("axis_of", ctypes.c_void_p),
+    ]
+
+
 class DeviceInfo(ctypes.Structure):
     _fields_ = [
         ("name", ctypes.c_char * 64),
@@ -176,6 +216,11 @@ _SIGNATURES = {
     "mg_window_gather": [ctypes.POINTER(WindowDesc), _vp, _vp],
     "mg_strided_copy": [ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64), ctypes.c_int64,
                         ctypes.c_int, _vp, _vp],
+    "mg_attention_fwd": [ctypes.POINTER(AttentionDesc)] + [_vp] * 5,
+    "mg_attention_bwd": [ctypes.POINTER(AttentionDesc)] + [_vp] * 9,
+    "mg_cache_write": [ctypes.c_int] + [ctypes.c_int64] * 4 + [_vp] * 5,
+    "mg_head_norm_fwd": [ctypes.POINTER(HeadNormDesc)] + [_vp] * 4,
+    "mg_head_norm_bwd": [ctypes.POINTER(HeadNormDesc)] + [_vp] * 6,
     "mg_permute": [ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int32), _vp, _vp],
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES) + ("mg_last_error", "mg_last_plan")
@@ -293,6 +338,14 @@ KERNEL_TAGS = {
     19: "permute",
     20: "batched_product",
     21: "gated",
+    22: "attention",
+    23: "attention_delta",
+    24: "attention_dq",
+    25: "attention_dkv",
+    26: "cache_write",
+    27: "head_norm",
+    28: "head_norm_bwd",
+    29: "attention_join",
 }
 
 
@@ -353,8 +406,8 @@ def dtype_code(dtype):
 
 
 def storage_code(dtype):
-    """``dtype_code`` for the two conversions (``mg_cast``, ``mg_accumulate``), which also take
-    float16: a type arrays are stored in, not one any kernel computes in."""
+    """``dtype_code`` for what also takes float16 (``mg_cast``, ``mg_accumulate``, attention and the norm
+    of heads): a type arrays are stored in, not one any kernel sums in."""
     import numpy as np
 
     return MG_F16 if np.dtype(dtype) == np.float16 else dtype_code(dtype)

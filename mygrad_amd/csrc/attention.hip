@@ -1,0 +1,379 @@
+// Attention with capped scores, a bias by distance and masks, and its gradient, for gfx950.
+//
+//   s_ij = scale * q_i . k_j                    s_ij = cap * tanh(s_ij / cap)   s_ij -= slope_h * |place_i - j|
+//   P_ij = exp(s_ij - lse_i), lse_i = log sum_j exp(s_ij)  over the keys j that row i sees
+//   out_i = sum_j P_ij v_j                      (a row that sees no key: zeros, and no gradient from it)
+//   dP_ij = g_i . v_j      D_i = g_i . out_i    dS_ij = P_ij (dP_ij - D_i) (1 - tanh^2) scale
+//   dq_i = sum_j dS_ij k_j      dk_j = sum_i dS_ij q_i      dv_j = sum_i P_ij g_i   (over the heads that share key head j)
+//
+// The kernels in this file take any type, head dimension up to 256 and mask: a wavefront per row of the result, keys (or
+// queries) over its lanes, sums in float32 (float64 for float64).  They serve double precision and what the kernels on the
+// matrix cores do not take.  What a row does not see never enters its sums, so infinities and NaN there stay where they are.
+#include "attention_device.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace mg {
+
+namespace {
+
+constexpr int kMaxDim = 256;
+constexpr int kParts = kMaxDim / 64;  // values of a row that a lane holds
+
+template <typename C>
+__device__ __forceinline__ C wave_sum(C v) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+template <typename C>
+__device__ __forceinline__ C wave_max(C v) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v = max(v, __shfl_xor(v, m));
+  return v;
+}
+
+// The score behind cap and bias; `through`: its derivative by the plain product.
+template <typename C>
+__device__ __forceinline__ C score(const Attention &p, C dot, C slope, int distance, C &through) {
+  const bool wide = sizeof(C) == 8;
+  const C scale = wide ? (C)p.scale64 : (C)p.scale, cap = wide ? (C)p.cap64 : (C)p.cap;
+  C s = dot * scale;
+  through = scale;
+  if (cap > 0) {
+    const C bent = tanh(s / cap);
+    s = cap * bent;
+    through *= 1 - bent * bent;
+  }
+  return s - slope * (C)(distance < 0 ? -distance : distance);
+}
+
+template <typename T, typename C>
+__device__ __forceinline__ C dot_row(const C *row, const T *other, int D) {
+  C sum = 0;
+  for (int d = 0; d < D; ++d) sum += row[d] * (C)other[d];
+  return sum;
+}
+
+struct Rows {
+  long long first;  // batch item * heads + head
+  int row;
+  bool in;
+};
+
+// A block takes four rows of one head: which of them is this wavefront's.
+__device__ __forceinline__ Rows row_of_wave(int tokens) {
+  const int tiles = (tokens + 3) / 4;
+  Rows r;
+  r.first = blockIdx.x / tiles;
+  r.row = (int)(blockIdx.x - r.first * tiles) * 4 + (threadIdx.x >> 6);
+  r.in = r.row < tokens;
+  return r;
+}
+
+template <typename T, typename C>
+__global__ void __launch_bounds__(256) attention_rows_kernel(Attention p, const T *__restrict__ q, const T *__restrict__ k,
+                                                             const T *__restrict__ v, T *__restrict__ out, C *__restrict__ lse) {
+  __shared__ C rows[4][kMaxDim];
+  const int lane = threadIdx.x & 63;
+  C *mine = rows[threadIdx.x >> 6];
+  const Rows r = row_of_wave(p.TQ);
+  const int b = (int)(r.first / p.HQ), h = (int)(r.first % p.HQ), i = r.row;
+  const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
+  if (r.in)
+    for (int d = lane; d < p.D; d += 64) mine[d] = (C)q[at + d];
+  __syncthreads();
+  if (!r.in) return;
+  const Span span = span_of(p, b, i);
+  const long long step = (long long)p.HK * p.D, head = ((long long)b * p.TK * p.HK + h / p.group) * p.D;
+  const C slope = p.slopes ? (C)p.slopes[h] : C(0);
+  C top = -INFINITY, total = 0, sum[kParts] = {};
+  for (int j0 = span.lo; j0 < span.hi; j0 += 64) {
+    const int j = j0 + lane, count = min(64, span.hi - j0);
+    C s = -INFINITY, through;
+    if (lane < count) s = score<C>(p, dot_row<T, C>(mine, k + head + j * step, p.D), slope, span.place - j, through);
+    const C now = max(top, wave_max(s)), base = now == -INFINITY ? C(0) : now;
+    const C back = exp(top - base);
+    const C e = lane < count ? exp(s - base) : C(0);
+    total = total * back + wave_sum(e);
+    top = now;
+#pragma unroll
+    for (int c = 0; c < kParts; ++c) sum[c] *= back;
+    for (int n = 0; n < count; ++n) {
+      const C weight = __shfl(e, n);
+      const T *row = v + head + (j0 + n) * step;
+#pragma unroll
+      for (int c = 0; c < kParts; ++c)
+        if (lane + 64 * c < p.D) sum[c] += weight * (C)row[lane + 64 * c];
+    }
+  }
+  const bool none = total == 0;
+#pragma unroll
+  for (int c = 0; c < kParts; ++c)
+    if (lane + 64 * c < p.D) out[at + lane + 64 * c] = (T)(none ? C(0) : sum[c] / total);
+  if (lse && lane == 0) lse[r.first * p.TQ + i] = none ? (C)INFINITY : top + log(total);  // no weight on any key
+}
+
+// D_i, a wavefront per row.
+template <typename T, typename C>
+__global__ void __launch_bounds__(256) attention_delta_kernel(Attention p, const T *__restrict__ out, const T *__restrict__ grad,
+                                                              C *__restrict__ delta) {
+  const int lane = threadIdx.x & 63;
+  const Rows r = row_of_wave(p.TQ);
+  if (!r.in) return;
+  const int b = (int)(r.first / p.HQ), h = (int)(r.first % p.HQ);
+  const long long at = (((long long)b * p.TQ + r.row) * p.HQ + h) * p.D;
+  C sum = 0;
+  for (int d = lane; d < p.D; d += 64) sum += (C)out[at + d] * (C)grad[at + d];
+  sum = wave_sum(sum);
+  if (lane == 0) delta[r.first * p.TQ + r.row] = sum;
+}
+
+template <typename T, typename C>
+__global__ void __launch_bounds__(256) attention_dq_rows_kernel(Attention p, const T *__restrict__ q, const T *__restrict__ k,
+                                                                const T *__restrict__ v, const T *__restrict__ grad,
+                                                                const C *__restrict__ lse, const C *__restrict__ delta,
+                                                                T *__restrict__ dq) {
+  __shared__ C rows[2][4][kMaxDim];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Rows r = row_of_wave(p.TQ);
+  const int b = (int)(r.first / p.HQ), h = (int)(r.first % p.HQ), i = r.row;
+  const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
+  if (r.in)
+    for (int d = lane; d < p.D; d += 64) rows[0][wave][d] = (C)q[at + d], rows[1][wave][d] = (C)grad[at + d];
+  __syncthreads();
+  if (!r.in) return;
+  const Span span = span_of(p, b, i);
+  const long long step = (long long)p.HK * p.D, head = ((long long)b * p.TK * p.HK + h / p.group) * p.D;
+  const C slope = p.slopes ? (C)p.slopes[h] : C(0);
+  const C norm = lse[r.first * p.TQ + i], mean = delta[r.first * p.TQ + i];
+  C sum[kParts] = {};
+  for (int j0 = span.lo; j0 < span.hi; j0 += 64) {
+    const int j = j0 + lane, count = min(64, span.hi - j0);
+    C ds = 0;
+    if (lane < count) {
+      C through;
+      const C s = score<C>(p, dot_row<T, C>(rows[0][wave], k + head + j * step, p.D), slope, span.place - j, through);
+      ds = exp(s - norm) * (dot_row<T, C>(rows[1][wave], v + head + j * step, p.D) - mean) * through;
+    }
+    for (int n = 0; n < count; ++n) {
+      const C weight = __shfl(ds, n);
+      const T *row = k + head + (j0 + n) * step;
+#pragma unroll
+      for (int c = 0; c < kParts; ++c)
+        if (lane + 64 * c < p.D) sum[c] += weight * (C)row[lane + 64 * c];
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kParts; ++c)
+    if (lane + 64 * c < p.D) dq[at + lane + 64 * c] = (T)sum[c];
+}
+
+// A wavefront per key and key head; queries over the lanes, the heads that share the key one after the other.
+template <typename T, typename C>
+__global__ void __launch_bounds__(256) attention_dkv_rows_kernel(Attention p, const T *__restrict__ q, const T *__restrict__ k,
+                                                                 const T *__restrict__ v, const T *__restrict__ grad,
+                                                                 const C *__restrict__ lse, const C *__restrict__ delta,
+                                                                 T *__restrict__ dk, T *__restrict__ dv) {
+  __shared__ C rows[2][4][kMaxDim];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Rows r = row_of_wave(p.TK);
+  const int b = (int)(r.first / p.HK), hk = (int)(r.first % p.HK), j = r.row;
+  const long long at = (((long long)b * p.TK + j) * p.HK + hk) * p.D;
+  if (r.in)
+    for (int d = lane; d < p.D; d += 64) rows[0][wave][d] = (C)k[at + d], rows[1][wave][d] = (C)v[at + d];
+  __syncthreads();
+  if (!r.in) return;
+  C sum_k[kParts] = {}, sum_v[kParts] = {};
+  const long long step = (long long)p.HQ * p.D;
+  for (int h = hk * p.group; h < (hk + 1) * p.group; ++h) {
+    const long long head = ((long long)b * p.TQ * p.HQ + h) * p.D, stats = ((long long)b * p.HQ + h) * p.TQ;
+    const C slope = p.slopes ? (C)p.slopes[h] : C(0);
+    for (int i0 = 0; i0 < p.TQ; i0 += 64) {
+      const int i = i0 + lane;
+      C weight = 0, ds = 0;
+      bool sees = false;
+      if (i < p.TQ) {
+        const Span span = span_of(p, b, i);
+        sees = j >= span.lo && j < span.hi;
+        if (sees) {
+          C through;
+          const C s = score<C>(p, dot_row<T, C>(rows[0][wave], q + head + i * step, p.D), slope, span.place - j, through);
+          weight = exp(s - lse[stats + i]);
+          ds = weight * (dot_row<T, C>(rows[1][wave], grad + head + i * step, p.D) - delta[stats + i]) * through;
+        }
+      }
+      for (unsigned long long left = __ballot(sees); left; left &= left - 1) {
+        const int n = __ffsll(left) - 1;
+        const C of_v = __shfl(weight, n), of_k = __shfl(ds, n);
+        const T *qr = q + head + (i0 + n) * step, *gr = grad + head + (i0 + n) * step;
+#pragma unroll
+        for (int c = 0; c < kParts; ++c)
+          if (lane + 64 * c < p.D) {
+            sum_k[c] += of_k * (C)qr[lane + 64 * c];
+            sum_v[c] += of_v * (C)gr[lane + 64 * c];
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kParts; ++c)
+    if (lane + 64 * c < p.D) dk[at + lane + 64 * c] = (T)sum_k[c], dv[at + lane + 64 * c] = (T)sum_v[c];
+}
+
+// Copies the t new tokens of each batch item to the places in the cache that end at its length, 16 bytes (or an element) a thread.
+template <typename V>
+__global__ void __launch_bounds__(256) cache_write_kernel(long long pieces, int row, int T, int capacity, const int32_t *__restrict__ lengths,
+                                                          const V *__restrict__ k, const V *__restrict__ v, V *__restrict__ keys,
+                                                          V *__restrict__ values) {
+  for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < pieces; n += (long long)gridDim.x * 256) {
+    const long long token = n / row;
+    const int b = (int)(token / T), place = lengths[b] - T + (int)(token - (long long)b * T);
+    if (place < 0 || place >= capacity) continue;
+    const long long to = ((long long)b * capacity + place) * row + (n - token * row);
+    keys[to] = k[n];
+    values[to] = v[n];
+  }
+}
+
+template <typename T, typename C>
+int forward_rows(const Attention &p, const void *q, const void *k, const void *v, void *out, void *lse) {
+  const long long blocks = (long long)p.B * p.HQ * ceil_div(p.TQ, 4);
+  ScopedTiming timed(TAG_ATTENTION);
+  attention_rows_kernel<T, C><<<dim3((unsigned)blocks), dim3(256), 0, runtime().stream>>>(p, (const T *)q, (const T *)k, (const T *)v, (T *)out, (C *)lse);
+  MG_HIP(hipGetLastError());
+  return MG_OK;
+}
+
+template <typename T, typename C>
+int backward_rows(const Attention &p, const void *q, const void *k, const void *v, const void *out, const void *lse, const void *grad,
+                  void *dq, void *dk, void *dv) {
+  hipStream_t s = runtime().stream;
+  const unsigned row_blocks = (unsigned)((long long)p.B * p.HQ * ceil_div(p.TQ, 4));
+  void *delta = nullptr;
+  const int rc = workspace((size_t)p.B * p.HQ * p.TQ * sizeof(C), &delta);
+  if (rc) return rc;
+  {
+    ScopedTiming timed(TAG_ATTENTION_DELTA);
+    attention_delta_kernel<T, C><<<dim3(row_blocks), dim3(256), 0, s>>>(p, (const T *)out, (const T *)grad, (C *)delta);
+  }
+  MG_HIP(hipGetLastError());
+  if (dq) {
+    ScopedTiming timed(TAG_ATTENTION_DQ);
+    attention_dq_rows_kernel<T, C><<<dim3(row_blocks), dim3(256), 0, s>>>(p, (const T *)q, (const T *)k, (const T *)v, (const T *)grad,
+                                                                          (const C *)lse, (const C *)delta, (T *)dq);
+    MG_HIP(hipGetLastError());
+  }
+  if (dk && p.TK) {
+    ScopedTiming timed(TAG_ATTENTION_DKV);
+    const unsigned key_blocks = (unsigned)((long long)p.B * p.HK * ceil_div(p.TK, 4));
+    attention_dkv_rows_kernel<T, C><<<dim3(key_blocks), dim3(256), 0, s>>>(p, (const T *)q, (const T *)k, (const T *)v, (const T *)grad,
+                                                                          (const C *)lse, (const C *)delta, (T *)dk, (T *)dv);
+    MG_HIP(hipGetLastError());
+  }
+  return MG_OK;
+}
+
+int check_attention(const mg_attention_desc *d, Attention *p, const char *who) {
+  if (!d) return fail(MG_ERR_BAD_ARG, "%s: null descriptor", who);
+  if (d->dtype != MG_F32 && d->dtype != MG_F64 && d->dtype != MG_F16) return fail(MG_ERR_UNSUPPORTED, "%s: dtype %d", who, d->dtype);
+  if (d->B < 0 || d->TQ < 0 || d->TK < 0 || d->HQ <= 0 || d->HK <= 0 || d->D <= 0 || d->HQ % d->HK != 0)
+    return fail(MG_ERR_BAD_ARG, "%s: batch %lld, %lld queries, %lld keys, %lld heads, %lld key heads, dim %lld", who, (long long)d->B,
+                (long long)d->TQ, (long long)d->TK, (long long)d->HQ, (long long)d->HK, (long long)d->D);
+  if (d->D > kMaxDim) return fail(MG_ERR_UNSUPPORTED, "%s: a head dimension of %lld (at most %d)", who, (long long)d->D, kMaxDim);
+  const int64_t most = 1 << 30;
+  if (d->TQ >= most || d->TK >= most || d->HQ >= most || d->B >= most || d->B * d->HQ >= most || d->B * d->HQ * ceil_div(d->TQ, 4) >= (1 << 24) ||
+      d->B * d->HK * ceil_div(d->TK, 4) >= (1 << 24))
+    return fail(MG_ERR_UNSUPPORTED, "%s: 2^26 rows of results or more", who);
+  if (d->window < 0 || d->window > most) return fail(MG_ERR_BAD_ARG, "%s: a window of %lld keys", who, (long long)d->window);
+  if (!std::isfinite(d->scale) || !std::isfinite(d->cap) || d->cap < 0) return fail(MG_ERR_BAD_ARG, "%s: scale %g, cap %g", who, d->scale, d->cap);
+  if (!d->starts != !d->ends) return fail(MG_ERR_BAD_ARG, "%s: starts of documents without their ends, or the other way round", who);
+  if (d->window && d->prefix) return fail(MG_ERR_BAD_ARG, "%s: a window and a prefix", who);
+  p->B = (int)d->B, p->TQ = (int)d->TQ, p->TK = (int)d->TK, p->HQ = (int)d->HQ, p->HK = (int)d->HK, p->D = (int)d->D;
+  p->group = p->HQ / p->HK;
+  p->causal = d->causal != 0, p->window = (int)d->window;
+  p->scale = (float)d->scale, p->cap = (float)d->cap, p->scale64 = d->scale, p->cap64 = d->cap;
+  p->lengths = d->lengths, p->prefix = d->prefix, p->starts = d->starts, p->ends = d->ends, p->slopes = d->slopes;
+  return MG_OK;
+}
+
+}  // namespace
+
+}  // namespace mg
+
+using namespace mg;
+
+extern "C" {
+
+int mg_attention_fwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, void *out, void *lse) {
+  std::lock_guard<std::recursive_mutex> guard(api_mutex());
+  MG_REQUIRE_INIT();
+  Attention p{};
+  const int rc = check_attention(desc, &p, "mg_attention_fwd");
+  if (rc) return rc;
+  if (p.B == 0 || p.TQ == 0) return MG_OK;
+  if (!q || !out || (p.TK && (!k || !v))) return fail(MG_ERR_BAD_ARG, "null pointer in mg_attention_fwd");
+  if (desc->dtype == MG_F64) return forward_rows<double, double>(p, q, k, v, out, lse);
+  if (desc->dtype == MG_F32) return forward_rows<float, float>(p, q, k, v, out, lse);
+  return forward_rows<_Float16, float>(p, q, k, v, out, lse);
+}
+
+int mg_attention_bwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, const void *out, const void *lse,
+                     const void *grad, void *dq, void *dk, void *dv) {
+  std::lock_guard<std::recursive_mutex> guard(api_mutex());
+  MG_REQUIRE_INIT();
+  Attention p{};
+  const int rc = check_attention(desc, &p, "mg_attention_bwd");
+  if (rc) return rc;
+  if (!dk != !dv) return fail(MG_ERR_BAD_ARG, "mg_attention_bwd: dk without dv, or the other way round");
+  const size_t size = desc->dtype == MG_F64 ? 8 : desc->dtype == MG_F32 ? 4 : 2;
+  if (p.B == 0 || p.TQ == 0) {
+    const size_t bytes = (size_t)p.B * p.TK * p.HK * p.D * size;
+    if (!dk || !bytes) return MG_OK;
+    const int zeroed = mg_memset_zero(dk, bytes);
+    return zeroed ? zeroed : mg_memset_zero(dv, bytes);
+  }
+  if (!q || !out || !lse || !grad || (p.TK && (!k || !v))) return fail(MG_ERR_BAD_ARG, "null pointer in mg_attention_bwd");
+  if (desc->dtype == MG_F64) return backward_rows<double, double>(p, q, k, v, out, lse, grad, dq, dk, dv);
+  if (desc->dtype == MG_F32) return backward_rows<float, float>(p, q, k, v, out, lse, grad, dq, dk, dv);
+  return backward_rows<_Float16, float>(p, q, k, v, out, lse, grad, dq, dk, dv);
+}
+
+int mg_cache_write(int dtype, int64_t B, int64_t T, int64_t capacity, int64_t row, const int32_t *lengths, const void *k, const void *v,
+                   void *keys, void *values) {
+  std::lock_guard<std::recursive_mutex> guard(api_mutex());
+  MG_REQUIRE_INIT();
+  if (dtype != MG_F32 && dtype != MG_F64 && dtype != MG_F16) return fail(MG_ERR_UNSUPPORTED, "mg_cache_write: dtype %d", dtype);
+  const int64_t most = 1 << 30;
+  if (B < 0 || T < 0 || capacity < 0 || row < 0 || B >= most || T >= most || capacity >= most || row >= most)
+    return fail(MG_ERR_BAD_ARG, "mg_cache_write: batch %lld, %lld tokens, capacity %lld, %lld values a token", (long long)B, (long long)T,
+                (long long)capacity, (long long)row);
+  if (B == 0 || T == 0 || row == 0) return MG_OK;
+  if (!lengths || !k || !v || !keys || !values) return fail(MG_ERR_BAD_ARG, "null pointer in mg_cache_write");
+  const int64_t size = dtype == MG_F64 ? 8 : dtype == MG_F32 ? 4 : 2;
+  const uintptr_t ends = (uintptr_t)k | (uintptr_t)v | (uintptr_t)keys | (uintptr_t)values;
+  const bool wide = row * size % 16 == 0 && ends % 16 == 0;
+  if (B * T >= (1ll << 40) / row) return fail(MG_ERR_UNSUPPORTED, "mg_cache_write: 2^40 values or more");
+  const int64_t piece = wide ? row * size / 16 : row, pieces = B * T * piece;
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(pieces, 256), 1 << 16)), block(256);
+  hipStream_t s = runtime().stream;
+  ScopedTiming timed(TAG_CACHE_WRITE);
+  auto launch = [&](auto one) {
+    using V = decltype(one);
+    cache_write_kernel<V><<<grid, block, 0, s>>>(pieces, (int)piece, (int)T, (int)capacity, lengths, (const V *)k, (const V *)v, (V *)keys, (V *)values);
+  };
+  if (wide)
+    launch(uint4{});
+  else if (size == 8)
+    launch(uint64_t{});
+  else if (size == 4)
+    launch(uint32_t{});
+  else
+    launch(uint16_t{});
+  MG_HIP(hipGetLastError());
+  return MG_OK;
+}
+
+}  // extern "C"

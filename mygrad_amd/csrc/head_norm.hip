@@ -1,0 +1,252 @@
+// A norm for each head with rotary positions in the same pass, and its gradient, for gfx950.
+//
+//   r = 1 / sqrt(mean(x^2) + eps)     z = w * x * r       (over the D values of one head of one token)
+//   y_a = z_a cos - z_b sin,  y_b = z_b cos + z_a sin     for the P pairs (a, b) = (p, p + P), or (2p, 2p + 1) interleaved
+//   u = the same turn backwards of grad                   dw = sum u x r       dx = r (w u - x r^2 mean(w u x))
+//
+// cos and sin of pair p lie in a table, at the row that the token's position along the pair's axis names.
+// Bandwidth-bound: x is read once forward, x and grad once backward; the table's rows are shared by a token's heads.
+#include "internal.h"
+
+#include <cmath>
+
+namespace mg {
+
+namespace {
+
+constexpr int kMaxDim = 1024;
+
+struct HeadNorm {
+  long long rows;  // tokens * heads
+  int heads, D, pairs, axes, table_rows, interleaved, norm, weight_heads;  // weight_heads: 0 no weight, 1 shared, else one for each head
+  double eps;
+  const int32_t *positions;  // (tokens, axes)
+  const uint8_t *axis_of;    // (pairs)
+};
+
+template <typename C>
+__device__ __forceinline__ C wave_sum(C v) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+// The place of a pair's first value and how far off the second one is.
+__device__ __forceinline__ int first_of(const HeadNorm &p, int pair) { return p.interleaved ? 2 * pair : pair; }
+__device__ __forceinline__ int apart(const HeadNorm &p) { return p.interleaved ? 1 : p.pairs; }
+
+template <typename C>
+__device__ __forceinline__ void turn_of(const HeadNorm &p, const C *table, long long token, int pair, C &cos, C &sin) {
+  const int row = p.positions[token * p.axes + p.axis_of[pair]];
+  const C *at = table + 2 * ((long long)min(max(row, 0), p.table_rows - 1) * p.pairs + pair);
+  cos = at[0], sin = at[1];
+}
+
+// A wavefront per row.
+template <typename T, typename C>
+__global__ void __launch_bounds__(256) head_norm_kernel(HeadNorm p, const T *__restrict__ x, const T *__restrict__ w, const C *__restrict__ table,
+                                                        T *__restrict__ y) {
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= p.rows) return;
+  const long long token = row / p.heads;
+  const int head = (int)(row - token * p.heads);
+  const T *xr = x + row * p.D, *wr = w + (p.weight_heads > 1 ? (long long)head * p.D : 0);
+  T *yr = y + row * p.D;
+  C r = 1;
+  if (p.norm) {
+    C sum = 0;
+    for (int d = lane; d < p.D; d += 64) sum += (C)xr[d] * (C)xr[d];
+    r = 1 / sqrt(wave_sum(sum) / p.D + (C)p.eps);
+  }
+  auto z = [&](int d) { return (C)xr[d] * r * (p.weight_heads ? (C)wr[d] : C(1)); };
+  for (int n = lane; n < p.pairs; n += 64) {
+    C cos, sin;
+    turn_of<C>(p, table, token, n, cos, sin);
+    const int a = first_of(p, n), b = a + apart(p);
+    const C za = z(a), zb = z(b);
+    yr[a] = (T)(za * cos - zb * sin);
+    yr[b] = (T)(zb * cos + za * sin);
+  }
+  for (int d = 2 * p.pairs + lane; d < p.D; d += 64) yr[d] = (T)z(d);
+}
+
+// A wavefront per row for dx; dw's terms go to `terms` (rows of a block of rows summed), see head_norm_weight_kernel.
+template <typename T, typename C>
+__global__ void __launch_bounds__(256) head_norm_dx_kernel(HeadNorm p, const T *__restrict__ x, const T *__restrict__ w, const C *__restrict__ table,
+                                                           const T *__restrict__ grad, T *__restrict__ dx) {
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= p.rows) return;
+  const long long token = row / p.heads;
+  const int head = (int)(row - token * p.heads);
+  const T *xr = x + row * p.D, *gr = grad + row * p.D, *wr = w + (p.weight_heads > 1 ? (long long)head * p.D : 0);
+  T *out = dx + row * p.D;
+  auto weight = [&](int d) { return p.weight_heads ? (C)wr[d] : C(1); };
+  C squares = 0, mix = 0;
+  auto add = [&](int d, C u) {
+    const C value = (C)xr[d];
+    squares += value * value;
+    mix += value * weight(d) * u;
+  };
+  for (int n = lane; n < p.pairs; n += 64) {
+    C cos, sin;
+    turn_of<C>(p, table, token, n, cos, sin);
+    const int a = first_of(p, n), b = a + apart(p);
+    const C ga = (C)gr[a], gb = (C)gr[b];
+    add(a, ga * cos + gb * sin);
+    add(b, gb * cos - ga * sin);
+  }
+  for (int d = 2 * p.pairs + lane; d < p.D; d += 64) add(d, (C)gr[d]);
+  C r = 1, m = 0;
+  if (p.norm) {
+    r = 1 / sqrt(wave_sum(squares) / p.D + (C)p.eps);
+    m = r * r * (wave_sum(mix) / p.D);
+  }
+  auto put = [&](int d, C u) { out[d] = (T)(r * (weight(d) * u - (C)xr[d] * m)); };
+  for (int n = lane; n < p.pairs; n += 64) {
+    C cos, sin;
+    turn_of<C>(p, table, token, n, cos, sin);
+    const int a = first_of(p, n), b = a + apart(p);
+    const C ga = (C)gr[a], gb = (C)gr[b];
+    put(a, ga * cos + gb * sin);
+    put(b, gb * cos - ga * sin);
+  }
+  for (int d = 2 * p.pairs + lane; d < p.D; d += 64) put(d, (C)gr[d]);
+}
+
+// Sums of u x r over the rows of one head (or of all) that block `blockIdx.y` takes, in double; a block's wavefronts go through them
+// in turn and are added in their order.
+template <typename T, typename C>
+__global__ void __launch_bounds__(256) head_norm_dw_kernel(HeadNorm p, long long per_block, const T *__restrict__ x, const C *__restrict__ table,
+                                                           const T *__restrict__ grad, double *__restrict__ parts) {
+  __shared__ double sums[4][kMaxDim];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.x;
+  const bool each = p.weight_heads > 1;
+  const long long count = each ? p.rows / p.heads : p.rows;
+  const long long from = blockIdx.y * per_block, to = min(count, from + per_block);
+  for (int d = lane; d < p.D; d += 64) sums[wave][d] = 0;
+  for (long long n = from + wave; n < to; n += 4) {
+    const long long row = each ? n * p.heads + head : n, token = row / p.heads;
+    const T *xr = x + row * p.D, *gr = grad + row * p.D;
+    C r = 1;
+    if (p.norm) {
+      C squares = 0;
+      for (int d = lane; d < p.D; d += 64) squares += (C)xr[d] * (C)xr[d];
+      r = 1 / sqrt(wave_sum(squares) / p.D + (C)p.eps);
+    }
+    for (int q = lane; q < p.pairs; q += 64) {
+      C cos, sin;
+      turn_of<C>(p, table, token, q, cos, sin);
+      const int a = first_of(p, q), b = a + apart(p);
+      const C ga = (C)gr[a], gb = (C)gr[b];
+      sums[wave][a] += (double)((ga * cos + gb * sin) * (C)xr[a] * r);
+      sums[wave][b] += (double)((gb * cos - ga * sin) * (C)xr[b] * r);
+    }
+    for (int d = 2 * p.pairs + lane; d < p.D; d += 64) sums[wave][d] += (double)((C)gr[d] * (C)xr[d] * r);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < p.D; d += 256)
+    parts[((long long)blockIdx.y * gridDim.x + head) * p.D + d] = sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d];
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) head_norm_dw_join_kernel(int values, int parts, const double *__restrict__ from, T *__restrict__ dw) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= values) return;
+  double sum = 0;
+  for (int part = 0; part < parts; ++part) sum += from[(long long)part * values + n];
+  dw[n] = (T)sum;
+}
+
+template <typename T, typename C>
+int forward(const HeadNorm &p, const void *x, const void *w, const void *table, void *y) {
+  ScopedTiming timed(TAG_HEAD_NORM);
+  head_norm_kernel<T, C><<<dim3((unsigned)ceil_div(p.rows, 4)), dim3(256), 0, runtime().stream>>>(p, (const T *)x, (const T *)w, (const C *)table, (T *)y);
+  MG_HIP(hipGetLastError());
+  return MG_OK;
+}
+
+template <typename T, typename C>
+int backward(const HeadNorm &p, const void *x, const void *w, const void *table, const void *grad, void *dx, void *dw) {
+  hipStream_t s = runtime().stream;
+  if (dx) {
+    ScopedTiming timed(TAG_HEAD_NORM_BWD);
+    head_norm_dx_kernel<T, C><<<dim3((unsigned)ceil_div(p.rows, 4)), dim3(256), 0, s>>>(p, (const T *)x, (const T *)w, (const C *)table, (const T *)grad, (T *)dx);
+    MG_HIP(hipGetLastError());
+  }
+  if (dw) {
+    const int heads = p.weight_heads;
+    const long long count = heads > 1 ? p.rows / p.heads : p.rows;
+    const long long per_block = ceil_div(count, 256), parts = ceil_div(count, per_block);
+    void *sums = nullptr;
+    const int rc = workspace((size_t)parts * heads * p.D * sizeof(double), &sums);
+    if (rc) return rc;
+    ScopedTiming timed(TAG_HEAD_NORM_BWD);
+    head_norm_dw_kernel<T, C><<<dim3((unsigned)heads, (unsigned)parts), dim3(256), 0, s>>>(p, per_block, (const T *)x, (const C *)table, (const T *)grad, (double *)sums);
+    MG_HIP(hipGetLastError());
+    head_norm_dw_join_kernel<T><<<dim3((unsigned)ceil_div(heads * p.D, 256)), dim3(256), 0, s>>>(heads * p.D, (int)parts, (const double *)sums, (T *)dw);
+    MG_HIP(hipGetLastError());
+  }
+  return MG_OK;
+}
+
+int check(const mg_head_norm_desc *d, HeadNorm *p, const char *who) {
+  if (!d) return fail(MG_ERR_BAD_ARG, "%s: null descriptor", who);
+  if (d->dtype != MG_F32 && d->dtype != MG_F64 && d->dtype != MG_F16) return fail(MG_ERR_UNSUPPORTED, "%s: dtype %d", who, d->dtype);
+  if (d->tokens < 0 || d->heads <= 0 || d->D <= 0 || d->pairs < 0 || 2 * d->pairs > d->D || d->eps < 0 || !std::isfinite(d->eps))
+    return fail(MG_ERR_BAD_ARG, "%s: %lld tokens, %lld heads, dim %lld, %lld pairs, eps %g", who, (long long)d->tokens, (long long)d->heads,
+                (long long)d->D, (long long)d->pairs, d->eps);
+  if (d->D > kMaxDim || d->heads > 65535 || d->tokens >= (1ll << 40) / d->heads || ceil_div(d->tokens * d->heads, 4) >= (1 << 24))
+    return fail(MG_ERR_UNSUPPORTED, "%s: %lld tokens, %lld heads, dim %lld (at most %d)", who, (long long)d->tokens, (long long)d->heads,
+                (long long)d->D, kMaxDim);
+  if (d->weight_heads != 0 && d->weight_heads != 1 && d->weight_heads != d->heads)
+    return fail(MG_ERR_BAD_ARG, "%s: weights of %d heads for %lld", who, d->weight_heads, (long long)d->heads);
+  if (d->pairs && (d->axes < 1 || d->axes > 255 || d->table_rows < 1 || d->table_rows >= (1 << 30) || !d->positions || !d->axis_of))
+    return fail(MG_ERR_BAD_ARG, "%s: %d axes, a table of %lld rows, or no positions", who, d->axes, (long long)d->table_rows);
+  p->rows = d->tokens * d->heads;
+  p->heads = (int)d->heads, p->D = (int)d->D, p->pairs = (int)d->pairs, p->axes = d->axes, p->table_rows = (int)d->table_rows;
+  p->interleaved = d->interleaved, p->norm = d->norm, p->weight_heads = d->weight_heads, p->eps = d->eps;
+  p->positions = d->positions, p->axis_of = d->axis_of;
+  return MG_OK;
+}
+
+}  // namespace
+
+}  // namespace mg
+
+using namespace mg;
+
+extern "C" {
+
+int mg_head_norm_fwd(const mg_head_norm_desc *desc, const void *x, const void *weight, const void *table, void *y) {
+  std::lock_guard<std::recursive_mutex> guard(api_mutex());
+  MG_REQUIRE_INIT();
+  HeadNorm p{};
+  const int rc = check(desc, &p, "mg_head_norm_fwd");
+  if (rc) return rc;
+  if (p.rows == 0) return MG_OK;
+  if (!x || !y || (p.weight_heads && !weight) || (p.pairs && !table)) return fail(MG_ERR_BAD_ARG, "null pointer in mg_head_norm_fwd");
+  if (desc->dtype == MG_F64) return forward<double, double>(p, x, weight, table, y);
+  if (desc->dtype == MG_F32) return forward<float, float>(p, x, weight, table, y);
+  return forward<_Float16, float>(p, x, weight, table, y);
+}
+
+int mg_head_norm_bwd(const mg_head_norm_desc *desc, const void *x, const void *weight, const void *table, const void *grad, void *dx, void *dweight) {
+  std::lock_guard<std::recursive_mutex> guard(api_mutex());
+  MG_REQUIRE_INIT();
+  HeadNorm p{};
+  const int rc = check(desc, &p, "mg_head_norm_bwd");
+  if (rc) return rc;
+  if (dweight && !p.weight_heads) return fail(MG_ERR_BAD_ARG, "mg_head_norm_bwd: a gradient of weights that there are none of");
+  if (p.rows == 0) {
+    const size_t size = desc->dtype == MG_F64 ? 8 : desc->dtype == MG_F32 ? 4 : 2;
+    return dweight ? mg_memset_zero(dweight, (size_t)p.weight_heads * p.D * size) : MG_OK;
+  }
+  if (!x || !grad || (p.weight_heads && !weight) || (p.pairs && !table)) return fail(MG_ERR_BAD_ARG, "null pointer in mg_head_norm_bwd");
+  if (desc->dtype == MG_F64) return backward<double, double>(p, x, weight, table, grad, dx, dweight);
+  if (desc->dtype == MG_F32) return backward<float, float>(p, x, weight, table, grad, dx, dweight);
+  return backward<_Float16, float>(p, x, weight, table, grad, dx, dweight);
+}
+
+}  // extern "C"

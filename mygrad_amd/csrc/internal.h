@@ -70,6 +70,14 @@ enum KernelTag {
   TAG_PERMUTE = 19,
   TAG_BATCHED_PRODUCT = 20,
   TAG_GATED = 21,  // the single-precision filter gradient behind one on parts: seldom anything to do
+  TAG_ATTENTION = 22,
+  TAG_ATTENTION_DELTA = 23,
+  TAG_ATTENTION_DQ = 24,
+  TAG_ATTENTION_DKV = 25,
+  TAG_CACHE_WRITE = 26,
+  TAG_HEAD_NORM = 27,
+  TAG_HEAD_NORM_BWD = 28,
+  TAG_ATTENTION_JOIN = 29,
 };
 void timing_begin(int tag);
 void timing_end();

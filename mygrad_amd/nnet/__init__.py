@@ -1,4 +1,4 @@
 from .activations import relu
-from .layers import batchnorm, conv_nd, max_pool
+from .layers import AttentionMask, KeyValueCache, RotaryTable, attention, batchnorm, conv_nd, head_norm, max_pool, rotate
 
-__all__ = ["batchnorm", "conv_nd", "max_pool", "relu"]
+__all__ = ["AttentionMask", "KeyValueCache", "RotaryTable", "attention", "batchnorm", "conv_nd", "head_norm", "max_pool", "relu", "rotate"]

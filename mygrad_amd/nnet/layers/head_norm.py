@@ -1,0 +1,204 @@
+"""A norm for each head and rotary positions in one pass on the MI355X, for the queries and keys of an attention.
+The reference has no counterpart; the operation keeps its ``Operation`` contract (``mygrad/operation_base.py:54-228``)."""
+
+from math import prod
+from numbers import Integral
+from typing import Optional
+
+import numpy as np
+
+from ... import _device, _hip
+from ...operation_base import Operation
+from ...tensor_base import Tensor
+
+__all__ = ["head_norm", "rotate", "HeadNorm", "RotaryTable", "RotaryPositions"]
+
+_DTYPES = (np.float16, np.float32, np.float64)
+
+
+class RotaryTable:
+    """cos and sin of the angles that rotary positions turn pairs of values by, made once.
+
+    Parameters
+    ----------
+    sections : int or sequence of ints
+        Pairs of a head's values that each axis of positions turns: ``dim // 2`` for the one axis of a text,
+        ``(16, 24, 24)``, say, for time, height and width.  What the pairs leave of a head stays as it is.
+    length : int
+        Positions lie in ``[0, length)``.
+    base : float
+        Pair ``m`` of the ``n`` of an axis turns by ``position * base ** (-m / n)``.
+    interleaved : bool
+        Pairs are values ``(2p, 2p + 1)``; otherwise ``(p, p + P)`` with ``P`` pairs in all.
+    """
+
+    def __init__(self, sections, length, *, base=10000.0, interleaved=False):
+        sections = (sections,) if isinstance(sections, Integral) else tuple(sections)
+        if not sections or len(sections) > 255 or not all(isinstance(n, Integral) and n >= 0 for n in sections) or not 1 <= sum(sections) <= 512:
+            raise ValueError(f"`sections` are pairs for each axis, 1 to 512 in all, got {sections}")
+        if not isinstance(length, Integral) or not 1 <= length < 1 << 30:
+            raise ValueError(f"`length` must be a whole number of 1 or more, got {length}")
+        if not base > 0 or not np.isfinite(base):
+            raise ValueError(f"`base` must be a positive number, got {base}")
+        if not isinstance(interleaved, (bool, np.bool_)):
+            raise TypeError(f"`interleaved` must be a boolean value, got: {interleaved}")
+        self.sections, self.length, self.interleaved = tuple(map(int, sections)), int(length), bool(interleaved)
+        self.pairs = sum(self.sections)
+        frequency = np.concatenate([float(base) ** (-np.arange(n) / n) if n else np.empty(0) for n in self.sections])
+        angle = np.arange(self.length)[:, None] * frequency
+        self._turns = np.stack((np.cos(angle), np.sin(angle)), -1)
+        self._axis_of = np.repeat(np.arange(len(self.sections)), self.sections).astype(np.uint8)
+        self._buffers = {}
+
+    def _buffer(self, what):
+        buf = self._buffers.get(what)
+        if buf is None:
+            arr = self._axis_of if what == "axis_of" else self._turns.astype(what)
+            buf = self._buffers[what] = _device.from_host(np.ascontiguousarray(arr)).buf
+        return buf
+
+    def at(self, positions):
+        """The table at the positions of some tokens, for any number of calls: ``positions`` are whole numbers of
+        shape ``(..., axes)`` whose leading axes broadcast to those of the tokens, or ``(tokens,)`` for one axis."""
+        return RotaryPositions(self, positions)
+
+
+class RotaryPositions:
+    """What :meth:`RotaryTable.at` gives."""
+
+    def __init__(self, table, positions):
+        arr = np.array(positions)
+        if arr.dtype.kind not in "iu":
+            raise TypeError(f"positions are whole numbers, got {arr.dtype}")
+        axes = len(table.sections)
+        if arr.ndim == 1 and axes == 1:
+            arr = arr[:, None]
+        if arr.ndim < 1 or arr.shape[-1] != axes:
+            raise ValueError(f"positions must have shape (..., {axes}) for {axes} axes, got {arr.shape}")
+        if arr.size and (arr.min() < 0 or arr.max() >= table.length):
+            raise ValueError(f"positions must lie in [0, {table.length}), got {arr.min()} to {arr.max()}")
+        self.table, self._positions, self._bound = table, arr.astype(np.int32), {}
+
+    def _check(self, lead):
+        try:
+            fits = np.broadcast_shapes(self._positions.shape[:-1], lead) == lead
+        except ValueError:
+            fits = False
+        if not fits:
+            raise ValueError(f"positions of shape {self._positions.shape} for tokens of shape {lead}")
+
+    def _buffer(self, lead):
+        buf = self._bound.get(lead)
+        if buf is None:
+            self._check(lead)
+            if len(self._bound) >= 16:
+                self._bound.clear()
+            spread = np.broadcast_to(self._positions, lead + self._positions.shape[-1:])
+            buf = self._bound[lead] = _device.from_host(np.ascontiguousarray(spread)).buf
+        return buf
+
+
+class HeadNorm(Operation):
+    """``x:(..., heads, dim)`` with ``weight:(dim,)`` or ``(heads, dim)``; an empty ``weight`` stands for none."""
+
+    takes_device_arrays = True
+
+    def __call__(self, x, weight, *, eps, rotary):
+        """``eps`` None: no norm."""
+        self.variables = (x, weight)
+        xd, wd = _device.value_of(x), _device.value_of(weight)
+        if xd.ndim < 2:
+            raise ValueError(f"`x` must have the axes (..., heads, dim), got shape {xd.shape}")
+        if xd.dtype not in _DTYPES:
+            raise TypeError(f"head_norm runs on the GPU in float16, float32 or float64, got {xd.dtype} (there is no CPU fallback)")
+        lead, (heads, dim) = xd.shape[:-2], xd.shape[-2:]
+        if not 1 <= dim <= 1024 or heads > 65535:
+            raise ValueError(f"heads have 1 to 1024 values and number at most 65535, got {xd.shape}")
+        self._weighted = wd.size > 0
+        if self._weighted:
+            if wd.shape not in ((dim,), (heads, dim)):
+                raise ValueError(f"`weight` must have shape ({dim},) or ({heads}, {dim}), got {wd.shape}")
+            if wd.dtype != xd.dtype:
+                raise TypeError(f"head_norm takes `weight` in the dtype of `x` ({xd.dtype}), got {wd.dtype}")
+        if eps is not None and not 0 <= eps < np.inf:
+            raise ValueError(f"`eps` must be a non-negative number, got {eps}")
+        if rotary is not None:
+            if not isinstance(rotary, RotaryPositions):
+                raise TypeError(f"`rotary` must come from RotaryTable.at, got {type(rotary).__name__}")
+            if 2 * rotary.table.pairs > dim:
+                raise ValueError(f"{rotary.table.pairs} pairs do not fit in {dim} values")
+            rotary._check(lead)
+        self._backed = None
+        if xd.size == 0:
+            return np.empty(xd.shape, dtype=xd.dtype)
+        self._rotary = rotary  # holds what the descriptor points to
+        self._table = None
+        desc = _hip.HeadNormDesc(_hip.storage_code(xd.dtype), eps is not None, wd.size // dim if self._weighted else 0, 0, 1, 0, prod(lead),
+                                 heads, dim, 0, 0, 0.0 if eps is None else eps, None, None)
+        if rotary is not None:
+            table = rotary.table
+            self._positions = rotary._buffer(lead)
+            self._table = table._buffer("f8" if xd.dtype == np.float64 else "f4").ptr
+            desc.interleaved, desc.axes, desc.pairs, desc.table_rows = table.interleaved, len(table.sections), table.pairs, table.length
+            desc.positions, desc.axis_of = self._positions.ptr, table._buffer("axis_of").ptr
+        self._desc = desc
+        xb = _device.to_device(xd)
+        wb = _device.to_device(wd) if self._weighted else None
+        out = _device.DeviceBuffer(xd.nbytes)
+        _hip.check(_hip.lib().mg_head_norm_fwd(desc, xb.ptr, None if wb is None else wb.ptr, self._table, out.ptr))
+        y = _device.download(out, xd.shape, xd.dtype)
+        _device.attach(y, out)
+        return y
+
+    def _run_backward(self, grad, want):
+        x, w = (_device.value_of(t) for t in self.variables)
+        if grad.shape != x.shape:
+            raise NotImplementedError(f"head_norm backward for gradient of shape {grad.shape} (no CPU fallback)")
+        xb, gb = _device.to_device(x), _device.to_device(grad, x.dtype)
+        wb = _device.to_device(w) if self._weighted else None
+        out = {i: _device.DeviceBuffer(a.nbytes) for i, a in enumerate((x, w)) if i in want}
+        _hip.check(_hip.lib().mg_head_norm_bwd(self._desc, xb.ptr, None if wb is None else wb.ptr, self._table, gb.ptr,
+                                               *(out[i].ptr if i in out else None for i in range(2))))
+        return {i: _device.download(buf, (x, w)[i].shape, x.dtype) for i, buf in out.items()}
+
+    def backward_var(self, grad, index, **kwargs):
+        value = _device.value_of(self.variables[index])
+        if _device.value_of(self.variables[0]).size == 0 or value.size == 0:
+            return np.zeros(value.shape, dtype=value.dtype)
+        # backward() asks for each variable in turn with the same `grad`: the first request computes all that are wanted
+        if self._backed is None or self._backed[0] is not grad or index not in self._backed[1]:
+            want = {index} | {i for i, var in enumerate(self.variables) if not var.constant and (i == 0 or self._weighted)}
+            self._backed = (grad, self._run_backward(grad, want))
+        out = self._backed[1].pop(index)
+        if not self._backed[1]:
+            self._backed = None
+        return out
+
+
+def head_norm(x, weight=None, *, eps: float, rotary: Optional[RotaryPositions] = None, constant: Optional[bool] = None) -> Tensor:
+    """Norm the values of each head of ``x:(..., heads, dim)`` on the GPU, and turn them by rotary positions::
+
+        y = turn(weight * x / sqrt(mean(x ** 2) + eps))
+
+    ``weight`` is ``(dim,)``, one for all heads, or ``(heads, dim)`` (so queries and keys of one projection take one call),
+    in the dtype of ``x`` (float16, float32 or float64), or None; ``eps`` is a non-negative number and has no default;
+    ``rotary`` comes from :meth:`RotaryTable.at`, None leaves the values where they are.  Sums and angles are carried in
+    float32 (float64 for float64), the result is rounded once.
+
+    >>> import mygrad_amd as mg
+    >>> from mygrad_amd.nnet import RotaryTable, head_norm
+    >>> table = RotaryTable(1, 8)
+    >>> head_norm(mg.Tensor([[[3.0, 4.0]], [[3.0, 4.0]]]), eps=0.0, rotary=table.at([0, 1])).data.round(3)
+    array([[[ 0.849,  1.131]],
+           [[-0.493,  1.325]]])
+    """
+    if eps is None:
+        raise TypeError("`eps` must be a non-negative number; without a norm use rotate()")
+    return Tensor._op(HeadNorm, x, np.array([]) if weight is None else weight, op_kwargs=dict(eps=eps, rotary=rotary), constant=constant)
+
+
+def rotate(x, rotary: RotaryPositions, *, constant: Optional[bool] = None) -> Tensor:
+    """Turn the values of each head of ``x:(..., heads, dim)`` by rotary positions (:func:`head_norm` without the norm)."""
+    if rotary is None:
+        raise TypeError("`rotary` must come from RotaryTable.at, got None")
+    return Tensor._op(HeadNorm, x, np.array([]), op_kwargs=dict(eps=None, rotary=rotary), constant=constant)

@@ -50,8 +50,8 @@ def device_tensor(x, *, dtype=None, constant=None):
             return Tensor(x, constant=constant, copy=False)
         x = x.data
     arr = np.ascontiguousarray(x, dtype=dtype)
-    if arr.dtype not in (np.float32, np.float64):
-        raise TypeError(f"device_tensor holds float32 or float64 values, got {arr.dtype}")
+    if arr.dtype not in (np.float32, np.float64, np.float16):
+        raise TypeError(f"device_tensor holds float32, float64 or float16 values, got {arr.dtype}")
     buf = _device.DeviceBuffer(max(arr.nbytes, 16))
     if arr.nbytes:
         buf.upload(arr)
@@ -293,7 +293,7 @@ class Tensor:
 
         if isinstance(grad, Tensor) and grad.on_device:
             grad = grad._value
-        if isinstance(grad, _device.DeviceArray) and grad.shape == self.shape and self.dtype in (np.float32, np.float64):
+        if isinstance(grad, _device.DeviceArray) and grad.shape == self.shape and self.dtype in (np.float32, np.float64, np.float16):
             seed = grad.astype(self.dtype)  # a gradient that is on the device already stays there
         elif grad is not None:
             seed = asarray(grad, dtype=self.dtype)
