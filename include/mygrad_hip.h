@@ -460,16 +460,17 @@ int mg_window_gather(const mg_window_desc *desc, const void *x, void *out);
 
 /* ---- attention (no counterpart in the reference) ---- */
 
-/* out = softmax(scores) v over the keys each query sees; a query that sees none gets zeros.  lse:(B, HQ, TQ), float32 (float64 for
- * MG_F64), receives the logarithm of each row's sum of exponentials (+infinity for a row without any weight), for mg_attention_bwd; it
- * may be null.  Sums are carried in float32 (float64 for MG_F64).  What a query does not see does not touch its result, whatever it
+/* out = softmax(scores) v over the keys each query sees; a query that sees none gets zeros.  For mg_attention_bwd, and null where
+ * there will be none: lse:(B, HQ, TQ), float32 (float64 for MG_F64), receives the logarithm of each row's sum of exponentials (+infinity
+ * for a row without any weight); rest, like out, receives with MG_F16 what rounding to float16 took off out, times 2^11 (the gradient of the
+ * scores takes products of out and grad off others of nearly the same size), and is not touched with other types.  Sums are carried in float32 (float64 for MG_F64).  What a query does not see does not touch its result, whatever it
  * holds. */
-int mg_attention_fwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, void *out, void *lse);
+int mg_attention_fwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, void *out, void *rest, void *lse);
 
-/* Gradients from grad (like out), `out` and `lse` of mg_attention_fwd.  dq, or dk and dv together, may be null (not wanted).  Fixed
+/* Gradients from grad (like out), `out`, `rest` and `lse` of mg_attention_fwd (rest may be null: out as it is rounded).  dq, or dk and dv together, may be null (not wanted).  Fixed
  * order of additions: run-to-run identical. */
-int mg_attention_bwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, const void *out, const void *lse,
-                     const void *grad, void *dq, void *dk, void *dv);
+int mg_attention_bwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, const void *out, const void *rest,
+                     const void *lse, const void *grad, void *dq, void *dk, void *dv);
 
 /* keys, values:(B, capacity, row): token t of k, v:(B, T, row) goes to place lengths[b] - T + t of item b (lengths on the device); what
  * falls outside [0, capacity) is left out.  `row` counts values of `dtype`. */

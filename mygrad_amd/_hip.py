@@ -216,8 +216,8 @@ _SIGNATURES = {
     "mg_window_gather": [ctypes.POINTER(WindowDesc), _vp, _vp],
     "mg_strided_copy": [ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64), ctypes.c_int64,
                         ctypes.c_int, _vp, _vp],
-    "mg_attention_fwd": [ctypes.POINTER(AttentionDesc)] + [_vp] * 5,
-    "mg_attention_bwd": [ctypes.POINTER(AttentionDesc)] + [_vp] * 9,
+    "mg_attention_fwd": [ctypes.POINTER(AttentionDesc)] + [_vp] * 6,
+    "mg_attention_bwd": [ctypes.POINTER(AttentionDesc)] + [_vp] * 10,
     "mg_cache_write": [ctypes.c_int] + [ctypes.c_int64] * 4 + [_vp] * 5,
     "mg_head_norm_fwd": [ctypes.POINTER(HeadNormDesc)] + [_vp] * 4,
     "mg_head_norm_bwd": [ctypes.POINTER(HeadNormDesc)] + [_vp] * 6,

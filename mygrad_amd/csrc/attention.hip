@@ -9,7 +9,7 @@
 // The kernels in this file take any type, head dimension up to 256 and mask: a wavefront per row of the result, keys (or
 // queries) over its lanes, sums in float32 (float64 for float64).  They serve double precision and what the kernels on the
 // matrix cores do not take.  What a row does not see never enters its sums, so infinities and NaN there stay where they are.
-#include "attention_device.h"
+#include "attention_rows.h"
 
 #include <algorithm>
 #include <cmath>
@@ -57,170 +57,191 @@ __device__ __forceinline__ C dot_row(const C *row, const T *other, int D) {
   return sum;
 }
 
+// A block takes `each` rows of one head, one after the other for each of its wavefronts; with `redo`, only where its entry there is set.
 struct Rows {
-  long long first;  // batch item * heads + head
-  int row;
-  bool in;
+  int each;
+  const int *redo;
 };
 
-// A block takes four rows of one head: which of them is this wavefront's.
-__device__ __forceinline__ Rows row_of_wave(int tokens) {
-  const int tiles = (tokens + 3) / 4;
-  Rows r;
-  r.first = blockIdx.x / tiles;
-  r.row = (int)(blockIdx.x - r.first * tiles) * 4 + (threadIdx.x >> 6);
-  r.in = r.row < tokens;
-  return r;
+struct Mine {
+  long long first;  // batch item * heads + head
+  int row, end;
+};
+
+__device__ __forceinline__ Mine rows_of_wave(const Rows &r, int tokens) {
+  const int tiles = (tokens + r.each - 1) / r.each;
+  Mine m;
+  m.first = blockIdx.x / tiles;
+  m.row = (int)(blockIdx.x - m.first * tiles) * r.each;
+  m.end = min(m.row + r.each, tokens);
+  m.row += threadIdx.x >> 6;
+  if (r.redo && !r.redo[blockIdx.x]) m.end = 0;
+  return m;
+}
+
+// What the lanes of a wavefront wrote to LDS is there for all of them.
+__device__ __forceinline__ void wave_sees() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) attention_rows_kernel(Attention p, const T *__restrict__ q, const T *__restrict__ k,
-                                                             const T *__restrict__ v, T *__restrict__ out, C *__restrict__ lse) {
+__global__ void __launch_bounds__(256) attention_rows_kernel(Attention p, Rows each, const T *__restrict__ q, const T *__restrict__ k,
+                                                             const T *__restrict__ v, T *__restrict__ out, _Float16 *__restrict__ rest,
+                                                             C *__restrict__ lse) {
   __shared__ C rows[4][kMaxDim];
   const int lane = threadIdx.x & 63;
   C *mine = rows[threadIdx.x >> 6];
-  const Rows r = row_of_wave(p.TQ);
-  const int b = (int)(r.first / p.HQ), h = (int)(r.first % p.HQ), i = r.row;
-  const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
-  if (r.in)
-    for (int d = lane; d < p.D; d += 64) mine[d] = (C)q[at + d];
-  __syncthreads();
-  if (!r.in) return;
-  const Span span = span_of(p, b, i);
+  const Mine r = rows_of_wave(each, p.TQ);
+  const int b = (int)(r.first / p.HQ), h = (int)(r.first % p.HQ);
   const long long step = (long long)p.HK * p.D, head = ((long long)b * p.TK * p.HK + h / p.group) * p.D;
   const C slope = p.slopes ? (C)p.slopes[h] : C(0);
-  C top = -INFINITY, total = 0, sum[kParts] = {};
-  for (int j0 = span.lo; j0 < span.hi; j0 += 64) {
-    const int j = j0 + lane, count = min(64, span.hi - j0);
-    C s = -INFINITY, through;
-    if (lane < count) s = score<C>(p, dot_row<T, C>(mine, k + head + j * step, p.D), slope, span.place - j, through);
-    const C now = max(top, wave_max(s)), base = now == -INFINITY ? C(0) : now;
-    const C back = exp(top - base);
-    const C e = lane < count ? exp(s - base) : C(0);
-    total = total * back + wave_sum(e);
-    top = now;
-#pragma unroll
-    for (int c = 0; c < kParts; ++c) sum[c] *= back;
-    for (int n = 0; n < count; ++n) {
-      const C weight = __shfl(e, n);
-      const T *row = v + head + (j0 + n) * step;
-#pragma unroll
-      for (int c = 0; c < kParts; ++c)
-        if (lane + 64 * c < p.D) sum[c] += weight * (C)row[lane + 64 * c];
+  for (int i = r.row; i < r.end; i += 4) {
+    const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
+    wave_sees();
+    for (int d = lane; d < p.D; d += 64) mine[d] = (C)q[at + d];
+    wave_sees();
+    const Span span = span_of(p, b, i);
+    C top = -INFINITY, total = 0, sum[kParts] = {};
+    for (int j0 = span.lo; j0 < span.hi; j0 += 64) {
+      const int j = j0 + lane, count = min(64, span.hi - j0);
+      C s = -INFINITY, through;
+      if (lane < count) s = score<C>(p, dot_row<T, C>(mine, k + head + j * step, p.D), slope, span.place - j, through);
+      const C now = max(top, wave_max(s)), base = now == -INFINITY ? C(0) : now;
+      const C back = exp(top - base);
+      const C e = lane < count ? exp(s - base) : C(0);
+      total = total * back + wave_sum(e);
+      top = now;
+  #pragma unroll
+      for (int c = 0; c < kParts; ++c) sum[c] *= back;
+      for (int n = 0; n < count; ++n) {
+        const C weight = __shfl(e, n);
+        const T *row = v + head + (j0 + n) * step;
+  #pragma unroll
+        for (int c = 0; c < kParts; ++c)
+          if (lane + 64 * c < p.D) sum[c] += weight * (C)row[lane + 64 * c];
+      }
     }
+    const bool none = total == 0;
+  #pragma unroll
+    for (int c = 0; c < kParts; ++c)
+      if (lane + 64 * c < p.D) {
+        const C value = none ? C(0) : sum[c] / total;
+        out[at + lane + 64 * c] = (T)value;
+        if (rest) rest[at + lane + 64 * c] = (_Float16)((value - (C)(T)value) * (C)kRest);
+      }
+    if (lse && lane == 0) lse[r.first * p.TQ + i] = none ? (C)INFINITY : top + log(total);  // no weight on any key
   }
-  const bool none = total == 0;
-#pragma unroll
-  for (int c = 0; c < kParts; ++c)
-    if (lane + 64 * c < p.D) out[at + lane + 64 * c] = (T)(none ? C(0) : sum[c] / total);
-  if (lse && lane == 0) lse[r.first * p.TQ + i] = none ? (C)INFINITY : top + log(total);  // no weight on any key
 }
 
 // D_i, a wavefront per row.
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) attention_delta_kernel(Attention p, const T *__restrict__ out, const T *__restrict__ grad,
-                                                              C *__restrict__ delta) {
+__global__ void __launch_bounds__(256) attention_delta_kernel(Attention p, Rows each, const T *__restrict__ out, const _Float16 *__restrict__ rest,
+                                                              const T *__restrict__ grad, C *__restrict__ delta) {
   const int lane = threadIdx.x & 63;
-  const Rows r = row_of_wave(p.TQ);
-  if (!r.in) return;
+  const Mine r = rows_of_wave(each, p.TQ);
   const int b = (int)(r.first / p.HQ), h = (int)(r.first % p.HQ);
-  const long long at = (((long long)b * p.TQ + r.row) * p.HQ + h) * p.D;
-  C sum = 0;
-  for (int d = lane; d < p.D; d += 64) sum += (C)out[at + d] * (C)grad[at + d];
-  sum = wave_sum(sum);
-  if (lane == 0) delta[r.first * p.TQ + r.row] = sum;
+  for (int i = r.row; i < r.end; i += 4) {
+    const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
+    C sum = 0;
+    for (int d = lane; d < p.D; d += 64) sum += ((C)out[at + d] + (rest ? (C)rest[at + d] / (C)kRest : C(0))) * (C)grad[at + d];
+    sum = wave_sum(sum);
+    if (lane == 0) delta[r.first * p.TQ + i] = sum;
+  }
 }
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) attention_dq_rows_kernel(Attention p, const T *__restrict__ q, const T *__restrict__ k,
+__global__ void __launch_bounds__(256) attention_dq_rows_kernel(Attention p, Rows each, const T *__restrict__ q, const T *__restrict__ k,
                                                                 const T *__restrict__ v, const T *__restrict__ grad,
                                                                 const C *__restrict__ lse, const C *__restrict__ delta,
                                                                 T *__restrict__ dq) {
   __shared__ C rows[2][4][kMaxDim];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Rows r = row_of_wave(p.TQ);
-  const int b = (int)(r.first / p.HQ), h = (int)(r.first % p.HQ), i = r.row;
-  const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
-  if (r.in)
-    for (int d = lane; d < p.D; d += 64) rows[0][wave][d] = (C)q[at + d], rows[1][wave][d] = (C)grad[at + d];
-  __syncthreads();
-  if (!r.in) return;
-  const Span span = span_of(p, b, i);
+  const Mine r = rows_of_wave(each, p.TQ);
+  const int b = (int)(r.first / p.HQ), h = (int)(r.first % p.HQ);
   const long long step = (long long)p.HK * p.D, head = ((long long)b * p.TK * p.HK + h / p.group) * p.D;
   const C slope = p.slopes ? (C)p.slopes[h] : C(0);
-  const C norm = lse[r.first * p.TQ + i], mean = delta[r.first * p.TQ + i];
-  C sum[kParts] = {};
-  for (int j0 = span.lo; j0 < span.hi; j0 += 64) {
-    const int j = j0 + lane, count = min(64, span.hi - j0);
-    C ds = 0;
-    if (lane < count) {
-      C through;
-      const C s = score<C>(p, dot_row<T, C>(rows[0][wave], k + head + j * step, p.D), slope, span.place - j, through);
-      ds = exp(s - norm) * (dot_row<T, C>(rows[1][wave], v + head + j * step, p.D) - mean) * through;
+  for (int i = r.row; i < r.end; i += 4) {
+    const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
+    wave_sees();
+    for (int d = lane; d < p.D; d += 64) rows[0][wave][d] = (C)q[at + d], rows[1][wave][d] = (C)grad[at + d];
+    wave_sees();
+    const Span span = span_of(p, b, i);
+    const C norm = lse[r.first * p.TQ + i], mean = delta[r.first * p.TQ + i];
+    C sum[kParts] = {};
+    for (int j0 = span.lo; j0 < span.hi; j0 += 64) {
+      const int j = j0 + lane, count = min(64, span.hi - j0);
+      C ds = 0;
+      if (lane < count) {
+        C through;
+        const C s = score<C>(p, dot_row<T, C>(rows[0][wave], k + head + j * step, p.D), slope, span.place - j, through);
+        ds = exp(s - norm) * (dot_row<T, C>(rows[1][wave], v + head + j * step, p.D) - mean) * through;
+      }
+      for (int n = 0; n < count; ++n) {
+        const C weight = __shfl(ds, n);
+        const T *row = k + head + (j0 + n) * step;
+  #pragma unroll
+        for (int c = 0; c < kParts; ++c)
+          if (lane + 64 * c < p.D) sum[c] += weight * (C)row[lane + 64 * c];
+      }
     }
-    for (int n = 0; n < count; ++n) {
-      const C weight = __shfl(ds, n);
-      const T *row = k + head + (j0 + n) * step;
-#pragma unroll
-      for (int c = 0; c < kParts; ++c)
-        if (lane + 64 * c < p.D) sum[c] += weight * (C)row[lane + 64 * c];
-    }
+  #pragma unroll
+    for (int c = 0; c < kParts; ++c)
+      if (lane + 64 * c < p.D) dq[at + lane + 64 * c] = (T)sum[c];
   }
-#pragma unroll
-  for (int c = 0; c < kParts; ++c)
-    if (lane + 64 * c < p.D) dq[at + lane + 64 * c] = (T)sum[c];
 }
 
 // A wavefront per key and key head; queries over the lanes, the heads that share the key one after the other.
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) attention_dkv_rows_kernel(Attention p, const T *__restrict__ q, const T *__restrict__ k,
+__global__ void __launch_bounds__(256) attention_dkv_rows_kernel(Attention p, Rows each, const T *__restrict__ q, const T *__restrict__ k,
                                                                  const T *__restrict__ v, const T *__restrict__ grad,
                                                                  const C *__restrict__ lse, const C *__restrict__ delta,
                                                                  T *__restrict__ dk, T *__restrict__ dv) {
   __shared__ C rows[2][4][kMaxDim];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Rows r = row_of_wave(p.TK);
-  const int b = (int)(r.first / p.HK), hk = (int)(r.first % p.HK), j = r.row;
-  const long long at = (((long long)b * p.TK + j) * p.HK + hk) * p.D;
-  if (r.in)
-    for (int d = lane; d < p.D; d += 64) rows[0][wave][d] = (C)k[at + d], rows[1][wave][d] = (C)v[at + d];
-  __syncthreads();
-  if (!r.in) return;
-  C sum_k[kParts] = {}, sum_v[kParts] = {};
+  const Mine r = rows_of_wave(each, p.TK);
+  const int b = (int)(r.first / p.HK), hk = (int)(r.first % p.HK);
   const long long step = (long long)p.HQ * p.D;
-  for (int h = hk * p.group; h < (hk + 1) * p.group; ++h) {
-    const long long head = ((long long)b * p.TQ * p.HQ + h) * p.D, stats = ((long long)b * p.HQ + h) * p.TQ;
-    const C slope = p.slopes ? (C)p.slopes[h] : C(0);
-    for (int i0 = 0; i0 < p.TQ; i0 += 64) {
-      const int i = i0 + lane;
-      C weight = 0, ds = 0;
-      bool sees = false;
-      if (i < p.TQ) {
-        const Span span = span_of(p, b, i);
-        sees = j >= span.lo && j < span.hi;
-        if (sees) {
-          C through;
-          const C s = score<C>(p, dot_row<T, C>(rows[0][wave], q + head + i * step, p.D), slope, span.place - j, through);
-          weight = exp(s - lse[stats + i]);
-          ds = weight * (dot_row<T, C>(rows[1][wave], grad + head + i * step, p.D) - delta[stats + i]) * through;
+  for (int j = r.row; j < r.end; j += 4) {
+    const long long at = (((long long)b * p.TK + j) * p.HK + hk) * p.D;
+    wave_sees();
+    for (int d = lane; d < p.D; d += 64) rows[0][wave][d] = (C)k[at + d], rows[1][wave][d] = (C)v[at + d];
+    wave_sees();
+    C sum_k[kParts] = {}, sum_v[kParts] = {};
+    for (int h = hk * p.group; h < (hk + 1) * p.group; ++h) {
+      const long long head = ((long long)b * p.TQ * p.HQ + h) * p.D, stats = ((long long)b * p.HQ + h) * p.TQ;
+      const C slope = p.slopes ? (C)p.slopes[h] : C(0);
+      for (int i0 = 0; i0 < p.TQ; i0 += 64) {
+        const int i = i0 + lane;
+        C weight = 0, ds = 0;
+        bool sees = false;
+        if (i < p.TQ) {
+          const Span span = span_of(p, b, i);
+          sees = j >= span.lo && j < span.hi;
+          if (sees) {
+            C through;
+            const C s = score<C>(p, dot_row<T, C>(rows[0][wave], q + head + i * step, p.D), slope, span.place - j, through);
+            weight = exp(s - lse[stats + i]);
+            ds = weight * (dot_row<T, C>(rows[1][wave], grad + head + i * step, p.D) - delta[stats + i]) * through;
+          }
+        }
+        for (unsigned long long left = __ballot(sees); left; left &= left - 1) {
+          const int n = __ffsll(left) - 1;
+          const C of_v = __shfl(weight, n), of_k = __shfl(ds, n);
+          const T *qr = q + head + (i0 + n) * step, *gr = grad + head + (i0 + n) * step;
+  #pragma unroll
+          for (int c = 0; c < kParts; ++c)
+            if (lane + 64 * c < p.D) {
+              sum_k[c] += of_k * (C)qr[lane + 64 * c];
+              sum_v[c] += of_v * (C)gr[lane + 64 * c];
+            }
         }
       }
-      for (unsigned long long left = __ballot(sees); left; left &= left - 1) {
-        const int n = __ffsll(left) - 1;
-        const C of_v = __shfl(weight, n), of_k = __shfl(ds, n);
-        const T *qr = q + head + (i0 + n) * step, *gr = grad + head + (i0 + n) * step;
-#pragma unroll
-        for (int c = 0; c < kParts; ++c)
-          if (lane + 64 * c < p.D) {
-            sum_k[c] += of_k * (C)qr[lane + 64 * c];
-            sum_v[c] += of_v * (C)gr[lane + 64 * c];
-          }
-      }
     }
+  #pragma unroll
+    for (int c = 0; c < kParts; ++c)
+      if (lane + 64 * c < p.D) dk[at + lane + 64 * c] = (T)sum_k[c], dv[at + lane + 64 * c] = (T)sum_v[c];
   }
-#pragma unroll
-  for (int c = 0; c < kParts; ++c)
-    if (lane + 64 * c < p.D) dk[at + lane + 64 * c] = (T)sum_k[c], dv[at + lane + 64 * c] = (T)sum_v[c];
 }
 
 // Copies the t new tokens of each batch item to the places in the cache that end at its length, 16 bytes (or an element) a thread.
@@ -238,18 +259,21 @@ __global__ void __launch_bounds__(256) cache_write_kernel(long long pieces, int 
   }
 }
 
+constexpr Rows kFour{4, nullptr};
+
 template <typename T, typename C>
-int forward_rows(const Attention &p, const void *q, const void *k, const void *v, void *out, void *lse) {
-  const long long blocks = (long long)p.B * p.HQ * ceil_div(p.TQ, 4);
-  ScopedTiming timed(TAG_ATTENTION);
-  attention_rows_kernel<T, C><<<dim3((unsigned)blocks), dim3(256), 0, runtime().stream>>>(p, (const T *)q, (const T *)k, (const T *)v, (T *)out, (C *)lse);
+int forward_rows(const Attention &p, Rows each, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
+  const long long blocks = (long long)p.B * p.HQ * ceil_div(p.TQ, each.each);
+  ScopedTiming timed(each.redo ? TAG_GATED : TAG_ATTENTION);
+  attention_rows_kernel<T, C><<<dim3((unsigned)blocks), dim3(256), 0, runtime().stream>>>(p, each, (const T *)q, (const T *)k, (const T *)v, (T *)out,
+                                                                                          (_Float16 *)rest, (C *)lse);
   MG_HIP(hipGetLastError());
   return MG_OK;
 }
 
 template <typename T, typename C>
-int backward_rows(const Attention &p, const void *q, const void *k, const void *v, const void *out, const void *lse, const void *grad,
-                  void *dq, void *dk, void *dv) {
+int backward_rows(const Attention &p, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
+                  const void *grad, void *dq, void *dk, void *dv) {
   hipStream_t s = runtime().stream;
   const unsigned row_blocks = (unsigned)((long long)p.B * p.HQ * ceil_div(p.TQ, 4));
   void *delta = nullptr;
@@ -257,20 +281,20 @@ int backward_rows(const Attention &p, const void *q, const void *k, const void *
   if (rc) return rc;
   {
     ScopedTiming timed(TAG_ATTENTION_DELTA);
-    attention_delta_kernel<T, C><<<dim3(row_blocks), dim3(256), 0, s>>>(p, (const T *)out, (const T *)grad, (C *)delta);
+    attention_delta_kernel<T, C><<<dim3(row_blocks), dim3(256), 0, s>>>(p, kFour, (const T *)out, (const _Float16 *)rest, (const T *)grad, (C *)delta);
   }
   MG_HIP(hipGetLastError());
   if (dq) {
     ScopedTiming timed(TAG_ATTENTION_DQ);
-    attention_dq_rows_kernel<T, C><<<dim3(row_blocks), dim3(256), 0, s>>>(p, (const T *)q, (const T *)k, (const T *)v, (const T *)grad,
+    attention_dq_rows_kernel<T, C><<<dim3(row_blocks), dim3(256), 0, s>>>(p, kFour, (const T *)q, (const T *)k, (const T *)v, (const T *)grad,
                                                                           (const C *)lse, (const C *)delta, (T *)dq);
     MG_HIP(hipGetLastError());
   }
   if (dk && p.TK) {
     ScopedTiming timed(TAG_ATTENTION_DKV);
     const unsigned key_blocks = (unsigned)((long long)p.B * p.HK * ceil_div(p.TK, 4));
-    attention_dkv_rows_kernel<T, C><<<dim3(key_blocks), dim3(256), 0, s>>>(p, (const T *)q, (const T *)k, (const T *)v, (const T *)grad,
-                                                                          (const C *)lse, (const C *)delta, (T *)dk, (T *)dv);
+    attention_dkv_rows_kernel<T, C><<<dim3(key_blocks), dim3(256), 0, s>>>(p, kFour, (const T *)q, (const T *)k, (const T *)v, (const T *)grad,
+                                                                           (const C *)lse, (const C *)delta, (T *)dk, (T *)dv);
     MG_HIP(hipGetLastError());
   }
   return MG_OK;
@@ -301,13 +325,20 @@ int check_attention(const mg_attention_desc *d, Attention *p, const char *who) {
 
 }  // namespace
 
+int forward_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse,
+                       const int *redo, int rows) {
+  const Rows each{rows, redo};
+  return dtype == MG_F16 ? forward_rows<_Float16, float>(p, each, q, k, v, out, rest, lse) : forward_rows<float, float>(p, each, q, k, v, out, rest, lse);
+}
+
 }  // namespace mg
 
 using namespace mg;
 
 extern "C" {
 
-int mg_attention_fwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, void *out, void *lse) {
+int mg_attention_fwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, void *out, void *rest,
+                     void *lse) {
   std::lock_guard<std::recursive_mutex> guard(api_mutex());
   MG_REQUIRE_INIT();
   Attention p{};
@@ -315,13 +346,16 @@ int mg_attention_fwd(const mg_attention_desc *desc, const void *q, const void *k
   if (rc) return rc;
   if (p.B == 0 || p.TQ == 0) return MG_OK;
   if (!q || !out || (p.TK && (!k || !v))) return fail(MG_ERR_BAD_ARG, "null pointer in mg_attention_fwd");
-  if (desc->dtype == MG_F64) return forward_rows<double, double>(p, q, k, v, out, lse);
-  if (desc->dtype == MG_F32) return forward_rows<float, float>(p, q, k, v, out, lse);
-  return forward_rows<_Float16, float>(p, q, k, v, out, lse);
+  if (desc->dtype != MG_F16) rest = nullptr;
+  if (desc->dtype == MG_F64) return forward_rows<double, double>(p, kFour, q, k, v, out, rest, lse);
+  const uintptr_t ends = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)rest;
+  if (p.TK && tiles_take(p, desc->dtype == MG_F16 ? 2 : 4, ends)) return forward_tiles(p, desc->dtype, q, k, v, out, rest, lse);
+  if (desc->dtype == MG_F32) return forward_rows<float, float>(p, kFour, q, k, v, out, rest, lse);
+  return forward_rows<_Float16, float>(p, kFour, q, k, v, out, rest, lse);
 }
 
-int mg_attention_bwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, const void *out, const void *lse,
-                     const void *grad, void *dq, void *dk, void *dv) {
+int mg_attention_bwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, const void *out, const void *rest,
+                     const void *lse, const void *grad, void *dq, void *dk, void *dv) {
   std::lock_guard<std::recursive_mutex> guard(api_mutex());
   MG_REQUIRE_INIT();
   Attention p{};
@@ -336,9 +370,10 @@ int mg_attention_bwd(const mg_attention_desc *desc, const void *q, const void *k
     return zeroed ? zeroed : mg_memset_zero(dv, bytes);
   }
   if (!q || !out || !lse || !grad || (p.TK && (!k || !v))) return fail(MG_ERR_BAD_ARG, "null pointer in mg_attention_bwd");
-  if (desc->dtype == MG_F64) return backward_rows<double, double>(p, q, k, v, out, lse, grad, dq, dk, dv);
-  if (desc->dtype == MG_F32) return backward_rows<float, float>(p, q, k, v, out, lse, grad, dq, dk, dv);
-  return backward_rows<_Float16, float>(p, q, k, v, out, lse, grad, dq, dk, dv);
+  if (desc->dtype != MG_F16) rest = nullptr;
+  if (desc->dtype == MG_F64) return backward_rows<double, double>(p, q, k, v, out, rest, lse, grad, dq, dk, dv);
+  if (desc->dtype == MG_F32) return backward_rows<float, float>(p, q, k, v, out, rest, lse, grad, dq, dk, dv);
+  return backward_rows<_Float16, float>(p, q, k, v, out, rest, lse, grad, dq, dk, dv);
 }
 
 int mg_cache_write(int dtype, int64_t B, int64_t T, int64_t capacity, int64_t row, const int32_t *lengths, const void *k, const void *v,

@@ -1,0 +1,20 @@
+// The two ways to compute an attention: on tiles (attention_tiles.hip), and a row at a time (attention.hip).
+#pragma once
+
+#include "attention_device.h"
+
+namespace mg {
+
+// What a float16 result leaves out is kept as this times it, in float16: 2^11, so that it is about as large as the result.
+constexpr float kRest = 2048.0f;
+
+bool tiles_take(const Attention &p, int size, uintptr_t ends);
+int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse);
+
+// Computes the rows of those blocks again, `rows` at a time, whose entry of redo[(batch item, head, block)] is not zero: the tiles'
+// products multiply what a row does not see by weights of zero, which an infinity or a NaN there turns into NaN.  Few blocks
+// as a rule have anything to do.
+int forward_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse,
+                       const int *redo, int rows);
+
+}  // namespace mg

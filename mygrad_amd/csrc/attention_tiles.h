@@ -1,0 +1,247 @@
+// Operands of attention on the matrix cores: tiles of rows in LDS, fragments, and the deal of blocks.
+//
+// All products run as D(32x32) += A(32xk) B(kx32), one wavefront each.  Lane l = 32 h + c (h = 0, 1) holds column c of D, at rows
+// 8 (r / 4) + 4 h + r % 4 for r = 0..15.  A fragment holds eight values along k for row (of A) or column (of B) c, and the two halves
+// of the wavefront hold sixteen between them.  The order of k is free as long as A and B agree:
+//   over the head dimension: value j of half h is d = 16 step + 8 h + j, eight neighbours in memory;
+//   over rows of a product's result: the registers 8 (step % 2) + j of a lane as they are, row 16 step + 8 (j / 4) + 4 h + j % 4 --
+//   so weights and their gradients go from the accumulators of one product into the next one without a move between lanes.
+// Float16 takes a fragment in one v_mfma_f32_32x32x16_f16, float32 in eight v_mfma_f32_32x32x2_f32.
+#pragma once
+
+#include "attention_device.h"
+
+namespace mg {
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+#define MG_LDS __attribute__((address_space(3)))
+
+constexpr unsigned kBeyond = 0x80000000u;  // a byte offset past the end of any buffer: reads as zero
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+template <typename T>
+struct Fragment;
+
+template <>
+struct Fragment<_Float16> {
+  typedef f16x8 V;
+  static __device__ __forceinline__ f32x16 mma(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+template <>
+struct Fragment<float> {
+  typedef f32x8 V;
+  static __device__ __forceinline__ f32x16 mma(V a, V b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// ROWS rows of DP values in LDS, in pieces of 16 bytes.  A row's pieces are permuted by the row's number, so that neither sixteen
+// rows at one piece (fragments along the head dimension) nor four rows at four neighbouring pieces (fragments along rows) fall on
+// the same banks twice.
+template <typename T, int DP, int ROWS>
+struct TileOf {
+  static constexpr int kPieces = DP * (int)sizeof(T) / 16;  // of a row
+  static constexpr int kRowBytes = DP * (int)sizeof(T);
+  static constexpr int kBytes = ROWS * kRowBytes;
+  typedef typename Fragment<T>::V V;
+
+  static __device__ __forceinline__ int turn(int row) {
+    if (sizeof(T) == 2) {
+      if (kPieces == 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+      if (kPieces == 8) return ((row & 2) << 1) | ((row >> 2) & 3);
+      return (row >> 2) & 3;  // 4 or 12
+    }
+    if (kPieces % 16 == 0) return ((row & 4) << 1) | ((row & 8) >> 1) | (row & 3);
+    return (row >> 1) & 7;  // 8 or 24
+  }
+
+  // Rows [0, ROWS) from `base` on, `stride` bytes apart, straight into LDS; pieces of rows outside [first, last) and behind the `dim`
+  // bytes of a row are zeros.  The block's 256 threads take part; `lds` is the tile's place in bytes.
+  static __device__ __forceinline__ void load(const char *base, unsigned stride, int first, int last, unsigned dim, unsigned lds) {
+    typedef MG_LDS void *LdsPointer;
+    const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0x7fffffff, 0x00020000);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int n = 0; n < ROWS * kPieces; n += 256) {
+      const int slot = n + (int)threadIdx.x;
+      if (ROWS * kPieces % 256 == 0 || n + wave * 64 < ROWS * kPieces) {
+        const int row = slot / kPieces, piece = (slot % kPieces) ^ turn(row);
+        const unsigned at = row >= first && row < last && (unsigned)piece * 16u < dim ? (unsigned)row * stride + (unsigned)piece * 16u : kBeyond;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (LdsPointer)(unsigned long long)(lds + (unsigned)(n + wave * 64) * 16u), 16, (int)at, 0, 0, 0);
+      }
+    }
+  }
+
+  // Fragment `step` along the head dimension of row `row`.
+  static __device__ __forceinline__ V along(unsigned lds, int row, int step, int h) {
+    const unsigned at = lds + (unsigned)row * kRowBytes;
+    const int turned = turn(row);
+    if constexpr (sizeof(T) == 2) {
+      return *(MG_LDS const f16x8 *)(unsigned long long)(at + (unsigned)((2 * step) ^ h ^ turned) * 16u);
+    } else {
+      const f32x4 a = *(MG_LDS const f32x4 *)(unsigned long long)(at + (unsigned)((4 * step) ^ (2 * h) ^ turned) * 16u);
+      const f32x4 b = *(MG_LDS const f32x4 *)(unsigned long long)(at + (unsigned)((4 * step) ^ (2 * h) ^ 1 ^ turned) * 16u);
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+
+  // Fragment `step` along the rows, for values 32 part .. 32 part + 31 of the head dimension (a value for each lane of a half).
+  static __device__ __forceinline__ V across(unsigned lds, int part, int step, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      // each sixteen lanes hand four rows of sixteen values to one another: lane 4 r + n reads row r at 4 n, lane m gets column m
+      const int row = 4 * h + ((lane & 15) >> 2), piece = 2 * ((lane & 31) >> 4) + ((lane & 3) >> 1);
+      V v;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int at = 16 * step + 8 * n + row;
+        const s16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (MG_LDS s16x4 *)(unsigned long long)(lds + (unsigned)at * kRowBytes + (unsigned)((4 * part) ^ piece ^ turn(at)) * 16u + (unsigned)(lane & 1) * 8u));
+        const f16x4 f = __builtin_bit_cast(f16x4, q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * n + j] = f[j];
+      }
+      return v;
+    } else {
+      V v;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = 16 * step + 8 * (j >> 2) + 4 * h + (j & 3), piece = (lane & 31) >> 2;
+        v[j] = *(MG_LDS const float *)(unsigned long long)(lds + (unsigned)at * kRowBytes + (unsigned)((8 * part) ^ piece ^ turn(at)) * 16u +
+                                                           (unsigned)(lane & 3) * 4u);
+      }
+      return v;
+    }
+  }
+};
+
+// Every load of this wave into LDS has landed and its LDS reads are done; then all waves of the block are here.
+__device__ __forceinline__ void all_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// What the two halves of the wavefront hold for a column: lane c's value and lane 32 + c's, in both lanes.
+struct Halves {
+  float low, high;
+};
+
+__device__ __forceinline__ Halves halves_of(float v) {
+  // The builtin's two results come out as one and the same in this compiler; the instruction wants two wait states behind what wrote its
+  // operands, which nobody puts there for an asm statement.
+  float low = v, high = v;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(low), "+v"(high));
+  return Halves{low, high};
+}
+
+__device__ __forceinline__ float larger_half(float v) {
+  const Halves both = halves_of(v);
+  return __builtin_fmaxf(both.low, both.high);
+}
+
+__device__ __forceinline__ float sum_halves(float v) {
+  const Halves both = halves_of(v);
+  return both.low + both.high;
+}
+
+// Of 32 rows of queries, a row for each lane of a half: the keys that any of them sees [lo, hi), and those that all of them see
+// [all_lo, all_hi) (rows beyond the last query count as seeing everything there, and nothing before).  The same in every lane.
+struct Reach {
+  int lo, hi, all_lo, all_hi;
+};
+
+__device__ __forceinline__ Reach reach_of(Span s, bool in) {
+  const bool some = in && s.hi > s.lo;
+  Reach r{some ? s.lo : 0x7fffffff, some ? s.hi : 0, in ? s.lo : 0, in ? s.hi : 0x7fffffff};
+#pragma unroll
+  for (int m = 16; m; m >>= 1) {
+    r.lo = min(r.lo, __shfl_xor(r.lo, m));
+    r.hi = max(r.hi, __shfl_xor(r.hi, m));
+    r.all_lo = max(r.all_lo, __shfl_xor(r.all_lo, m));
+    r.all_hi = min(r.all_hi, __shfl_xor(r.all_hi, m));
+  }
+  return Reach{__builtin_amdgcn_readfirstlane(r.lo), __builtin_amdgcn_readfirstlane(r.hi), __builtin_amdgcn_readfirstlane(r.all_lo),
+               __builtin_amdgcn_readfirstlane(r.all_hi)};
+}
+
+// Eight values of a row in memory as a fragment: zeros where the row or the piece is none.
+template <typename T>
+__device__ __forceinline__ typename Fragment<T>::V fragment_of(const T *row, int at, int dim, bool in) {
+  typename Fragment<T>::V v = {};
+  if (in && at < dim) v = *reinterpret_cast<const typename Fragment<T>::V *>(row + at);
+  return v;
+}
+
+// Rows of a tile of results as the registers of a lane hold them.
+__device__ __forceinline__ int row_of(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+__device__ __forceinline__ f32x16 zeros() { return f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}; }
+
+// Registers 8 n .. 8 n + 7 as a fragment along the rows.
+template <typename T>
+__device__ __forceinline__ typename Fragment<T>::V rows_of(const f32x16 &v, int n) {
+  f32x8 part;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) part[j] = v[8 * n + j];
+  return __builtin_convertvector(part, typename Fragment<T>::V);
+}
+
+// tanh: an odd polynomial for |x| < 1/4 (what the series leaves out is below 2^-31 of x), an exponential beyond (where the
+// difference from 1 costs no digits that count).  tanh_of_all() takes the polynomial alone where all values of a wavefront are small.
+__device__ __forceinline__ float tanh_small(float x) {
+  const float y = x * x;
+  float s = -0.00886323553f;       // -1382 / 155925
+  s = s * y + 0.0218694885f;       // 62 / 2835
+  s = s * y - 0.0539682540f;       // -17 / 315
+  s = s * y + 0.133333333f;
+  s = s * y - 0.333333333f;
+  return x + x * (s * y);
+}
+
+__device__ __forceinline__ float tanh_any(float x) {
+  const float e = __builtin_amdgcn_exp2f(x * (2 * kLog2e));  // infinity and 0 give +-1
+  const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+  return __builtin_fabsf(x) < 0.25f ? tanh_small(x) : far;
+}
+
+__device__ __forceinline__ void tanh_of_all(f32x16 &x) {
+  float most = 0;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) most = __builtin_fmaxf(most, __builtin_fabsf(x[r]));
+  if (__any(!(most < 0.25f))) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = tanh_any(x[r]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = tanh_small(x[r]);
+  }
+}
+
+// How the blocks of a launch are dealt out: `pairs` of a batch item and a key head, each with `heads` query heads and `tiles` row tiles.
+// Blocks go to the eight XCDs in turn, so with a multiple of eight pairs each pair stays on one XCD and is read through one L2.  The
+// last tiles, which see most where the mask is causal, come first.
+struct Deal {
+  int pairs, heads, tiles;
+};
+
+struct Dealt {
+  int pair, head, tile;
+};
+
+__device__ __forceinline__ Dealt dealt(const Deal &d, int block) {
+  const int each = d.heads * d.tiles;
+  if (d.pairs % 8 == 0) {
+    const int turn = block >> 3, pair = turn / each, rest = turn - pair * each;
+    return Dealt{pair * 8 + (block & 7), rest % d.heads, d.tiles - 1 - rest / d.heads};
+  }
+  const int many = d.pairs * d.heads, tile = block / many, rest = block - tile * many;
+  return Dealt{rest / d.heads, rest % d.heads, d.tiles - 1 - tile};
+}
+
+}  // namespace mg

@@ -203,11 +203,14 @@ class Attention(Operation):
         self._desc, self._slopes = _describe(qd.shape, kd.shape, qd.dtype, scale, cap, slopes, mask)
         qb, kb, vb = (_device.to_device(a) for a in (qd, kd, vd))
         self._out = _device.DeviceBuffer(qd.nbytes)
-        self._lse = None
+        self._lse = self._rest = None
         if _graph.TRACK_GRAPH and not (q.constant and k.constant and v.constant):
             wide = 8 if qd.dtype == np.float64 else 4
             self._lse = _device.DeviceBuffer(qd.size // qd.shape[3] * wide)
-        _hip.check(_hip.lib().mg_attention_fwd(self._desc, qb.ptr, kb.ptr, vb.ptr, self._out.ptr, None if self._lse is None else self._lse.ptr))
+            if qd.dtype == np.float16:
+                self._rest = _device.DeviceBuffer(qd.nbytes)
+        rest, lse = (None if b is None else b.ptr for b in (self._rest, self._lse))
+        _hip.check(_hip.lib().mg_attention_fwd(self._desc, qb.ptr, kb.ptr, vb.ptr, self._out.ptr, rest, lse))
         out = _device.download(self._out, qd.shape, qd.dtype)
         _device.attach(out, self._out)
         return out
@@ -223,7 +226,8 @@ class Attention(Operation):
         gb = _device.to_device(grad, q.dtype)
         indices = ({0} if 0 in want else set()) | ({1, 2} if want & {1, 2} else set())
         out = {i: _device.DeviceBuffer(max(arrays[i].nbytes, 16)) for i in indices}
-        _hip.check(_hip.lib().mg_attention_bwd(self._desc, *(b.ptr for b in held), self._out.ptr, self._lse.ptr, gb.ptr,
+        _hip.check(_hip.lib().mg_attention_bwd(self._desc, *(b.ptr for b in held), self._out.ptr,
+                                               None if self._rest is None else self._rest.ptr, self._lse.ptr, gb.ptr,
                                                *(out[i].ptr if i in out else None for i in range(3))))
         return {i: _device.download(out[i], arrays[i].shape, q.dtype) for i in want}
 
@@ -344,5 +348,5 @@ class KeyValueCache:
             return Tensor(np.zeros(qd.shape, dtype=qd.dtype), constant=True, copy=False)
         desc, held = _describe(qd.shape, self.shape, qd.dtype, scale, cap, slopes, mask)
         qb, out = _device.to_device(qd), _device.DeviceBuffer(qd.nbytes)
-        _hip.check(_hip.lib().mg_attention_fwd(desc, qb.ptr, self._keys.ptr, self._values.ptr, out.ptr, None))
+        _hip.check(_hip.lib().mg_attention_fwd(desc, qb.ptr, self._keys.ptr, self._values.ptr, out.ptr, None, None))
         return Tensor(_device.DeviceArray(out, qd.shape, qd.dtype), constant=True, copy=False)

@@ -352,12 +352,12 @@ def test_entry_points_refuse_bad_descriptors():
                            (-2, dict(B=1 << 20, TQ=1 << 20)), (-1, dict(window=-1)), (-1, dict(scale=float("nan"))), (-1, dict(cap=-1.0)),
                            (-1, dict(starts=buf.ptr)), (-1, dict(window=2, prefix=buf.ptr))):
         desc = _hip.AttentionDesc(**{**good, **change})
-        assert lib.mg_attention_fwd(desc, *[buf.ptr] * 5) == status, change
-        assert lib.mg_attention_bwd(desc, *[buf.ptr] * 9) == status, change
+        assert lib.mg_attention_fwd(desc, *[buf.ptr] * 6) == status, change
+        assert lib.mg_attention_bwd(desc, *[buf.ptr] * 10) == status, change
     desc = _hip.AttentionDesc(**good)
-    assert lib.mg_attention_fwd(desc, None, *[buf.ptr] * 4) == -1
-    assert lib.mg_attention_fwd(None, *[buf.ptr] * 5) == -1
-    assert lib.mg_attention_bwd(desc, *[buf.ptr] * 8, None) == -1  # dk without dv
+    assert lib.mg_attention_fwd(desc, None, *[buf.ptr] * 5) == -1
+    assert lib.mg_attention_fwd(None, *[buf.ptr] * 6) == -1
+    assert lib.mg_attention_bwd(desc, *[buf.ptr] * 9, None) == -1  # dk without dv
     assert lib.mg_cache_write(5, 1, 1, 1, 1, *[buf.ptr] * 5) == -2
     assert lib.mg_cache_write(0, 1, -1, 1, 1, *[buf.ptr] * 5) == -1
     assert lib.mg_cache_write(0, 1, 1, 1, 1, None, *[buf.ptr] * 4) == -1
