@@ -272,32 +272,41 @@ int forward_rows(const Attention &p, Rows each, const void *q, const void *k, co
 }
 
 template <typename T, typename C>
+int dq_rows(const Attention &p, Rows each, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad, void *dq) {
+  const unsigned blocks = (unsigned)((long long)p.B * p.HQ * ceil_div(p.TQ, each.each));
+  ScopedTiming timed(each.redo ? TAG_GATED : TAG_ATTENTION_DQ);
+  attention_dq_rows_kernel<T, C><<<dim3(blocks), dim3(256), 0, runtime().stream>>>(p, each, (const T *)q, (const T *)k, (const T *)v, (const T *)grad,
+                                                                                   (const C *)lse, (const C *)delta, (T *)dq);
+  MG_HIP(hipGetLastError());
+  return MG_OK;
+}
+
+template <typename T, typename C>
+int dkv_rows(const Attention &p, Rows each, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad, void *dk,
+             void *dv) {
+  const unsigned blocks = (unsigned)((long long)p.B * p.HK * ceil_div(p.TK, each.each));
+  ScopedTiming timed(each.redo ? TAG_GATED : TAG_ATTENTION_DKV);
+  attention_dkv_rows_kernel<T, C><<<dim3(blocks), dim3(256), 0, runtime().stream>>>(p, each, (const T *)q, (const T *)k, (const T *)v, (const T *)grad,
+                                                                                    (const C *)lse, (const C *)delta, (T *)dk, (T *)dv);
+  MG_HIP(hipGetLastError());
+  return MG_OK;
+}
+
+template <typename T, typename C>
 int backward_rows(const Attention &p, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
                   const void *grad, void *dq, void *dk, void *dv) {
-  hipStream_t s = runtime().stream;
-  const unsigned row_blocks = (unsigned)((long long)p.B * p.HQ * ceil_div(p.TQ, 4));
   void *delta = nullptr;
-  const int rc = workspace((size_t)p.B * p.HQ * p.TQ * sizeof(C), &delta);
+  int rc = workspace((size_t)p.B * p.HQ * p.TQ * sizeof(C), &delta);
   if (rc) return rc;
   {
     ScopedTiming timed(TAG_ATTENTION_DELTA);
-    attention_delta_kernel<T, C><<<dim3(row_blocks), dim3(256), 0, s>>>(p, kFour, (const T *)out, (const _Float16 *)rest, (const T *)grad, (C *)delta);
+    attention_delta_kernel<T, C><<<dim3((unsigned)((long long)p.B * p.HQ * ceil_div(p.TQ, 4))), dim3(256), 0, runtime().stream>>>(
+        p, kFour, (const T *)out, (const _Float16 *)rest, (const T *)grad, (C *)delta);
   }
   MG_HIP(hipGetLastError());
-  if (dq) {
-    ScopedTiming timed(TAG_ATTENTION_DQ);
-    attention_dq_rows_kernel<T, C><<<dim3(row_blocks), dim3(256), 0, s>>>(p, kFour, (const T *)q, (const T *)k, (const T *)v, (const T *)grad,
-                                                                          (const C *)lse, (const C *)delta, (T *)dq);
-    MG_HIP(hipGetLastError());
-  }
-  if (dk && p.TK) {
-    ScopedTiming timed(TAG_ATTENTION_DKV);
-    const unsigned key_blocks = (unsigned)((long long)p.B * p.HK * ceil_div(p.TK, 4));
-    attention_dkv_rows_kernel<T, C><<<dim3(key_blocks), dim3(256), 0, s>>>(p, kFour, (const T *)q, (const T *)k, (const T *)v, (const T *)grad,
-                                                                           (const C *)lse, (const C *)delta, (T *)dk, (T *)dv);
-    MG_HIP(hipGetLastError());
-  }
-  return MG_OK;
+  if (dq) rc = dq_rows<T, C>(p, kFour, q, k, v, lse, delta, grad, dq);
+  if (!rc && dk && p.TK) rc = dkv_rows<T, C>(p, kFour, q, k, v, lse, delta, grad, dk, dv);
+  return rc;
 }
 
 int check_attention(const mg_attention_desc *d, Attention *p, const char *who) {
@@ -329,6 +338,19 @@ int forward_rows_again(const Attention &p, int dtype, const void *q, const void 
                        const int *redo, int rows) {
   const Rows each{rows, redo};
   return dtype == MG_F16 ? forward_rows<_Float16, float>(p, each, q, k, v, out, rest, lse) : forward_rows<float, float>(p, each, q, k, v, out, rest, lse);
+}
+
+int dq_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad,
+                  void *dq, const int *redo, int rows) {
+  const Rows each{rows, redo};
+  return dtype == MG_F16 ? dq_rows<_Float16, float>(p, each, q, k, v, lse, delta, grad, dq) : dq_rows<float, float>(p, each, q, k, v, lse, delta, grad, dq);
+}
+
+int dkv_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad,
+                   void *dk, void *dv, const int *redo, int rows) {
+  const Rows each{rows, redo};
+  return dtype == MG_F16 ? dkv_rows<_Float16, float>(p, each, q, k, v, lse, delta, grad, dk, dv)
+                         : dkv_rows<float, float>(p, each, q, k, v, lse, delta, grad, dk, dv);
 }
 
 }  // namespace mg
@@ -372,6 +394,9 @@ int mg_attention_bwd(const mg_attention_desc *desc, const void *q, const void *k
   if (!q || !out || !lse || !grad || (p.TK && (!k || !v))) return fail(MG_ERR_BAD_ARG, "null pointer in mg_attention_bwd");
   if (desc->dtype != MG_F16) rest = nullptr;
   if (desc->dtype == MG_F64) return backward_rows<double, double>(p, q, k, v, out, rest, lse, grad, dq, dk, dv);
+  const uintptr_t ends = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)rest | (uintptr_t)grad | (uintptr_t)dq | (uintptr_t)dk |
+                         (uintptr_t)dv;
+  if (p.TK && tiles_take(p, desc->dtype == MG_F16 ? 2 : 4, ends)) return backward_tiles(p, desc->dtype, q, k, v, out, rest, lse, grad, dq, dk, dv);
   if (desc->dtype == MG_F32) return backward_rows<float, float>(p, q, k, v, out, rest, lse, grad, dq, dk, dv);
   return backward_rows<_Float16, float>(p, q, k, v, out, rest, lse, grad, dq, dk, dv);
 }

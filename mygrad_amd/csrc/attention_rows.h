@@ -17,4 +17,11 @@ int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, c
 int forward_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse,
                        const int *redo, int rows);
 
+int backward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
+                   const void *grad, void *dq, void *dk, void *dv);
+int dq_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad,
+                  void *dq, const int *redo, int rows);
+int dkv_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad,
+                   void *dk, void *dv, const int *redo, int rows);
+
 }  // namespace mg

@@ -166,6 +166,21 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
   if (threadIdx.x == 0) redo[((long long)b * p.HQ + hq) * deal.tiles + at.tile] = bad[0] | bad[1] | bad[2] | bad[3];
 }
 
+// Four neighbouring values of a result, registers r .. r + 3 times `by`; true if one is no number.
+template <typename T>
+__device__ __forceinline__ bool put_four(T *to, const f32x16 &from, int r, float by) {
+  f32x4 value;
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    value[j] = from[r + j] * by;
+    odd |= !(__builtin_fabsf(value[j]) < INFINITY);
+  }
+  typedef T V __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<V *>(to) = __builtin_convertvector(value, V);
+  return odd;
+}
+
 template <typename T, int DP, int KEYS>
 void launch_forward(const Attention &p, const void *q, const void *k, const void *v, void *out, void *rest, void *lse, int *redo) {
   const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
@@ -174,11 +189,433 @@ void launch_forward(const Attention &p, const void *q, const void *k, const void
                                                                                         (_Float16 *)rest, (float *)lse, redo);
 }
 
+// ---- gradient ----------------------------------------------------------------------------------------------------------------
+// What the two kernels of the gradient need of each row, made in one pass over out, grad and v:
+//   level_i = lse_i log2(e) - shift     exp2(s_i - level_i) = 2^shift P_i
+//   delta_i = grad_i . out_i            (with what the rounding of out took off)
+//   spans of the rows, and for each chunk of `rows` rows their union and intersection
+constexpr float kShift = 14.0f;  // 2^14 P in float16: whole down to 2^-28
+
+struct Stats {
+  float *level, *delta;  // (B, HQ, TQ)
+  int *lo, *hi;          // (B, TQ)
+  Reach *reach;          // (B, chunks of queries)
+  int rows, chunks;
+};
+
+template <typename T>
+__device__ __forceinline__ f32x8 eight(const T *from) {
+  return __builtin_convertvector(*reinterpret_cast<const typename Fragment<T>::V *>(from), f32x8);
+}
+
+// Sixteen lanes a row, eight values each.
+__device__ __forceinline__ float sum16(float v) {
+#pragma unroll
+  for (int m = 8; m; m >>= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) attention_stats_kernel(Attention p, Stats stats, const T *__restrict__ out, const _Float16 *__restrict__ rest,
+                                                              const float *__restrict__ lse, const T *__restrict__ grad) {
+  const int lane = threadIdx.x & 15, group = threadIdx.x >> 4, d = lane * 8;
+  const int bh = blockIdx.x / stats.chunks, chunk = blockIdx.x % stats.chunks, b = bh / p.HQ, h = bh % p.HQ;
+  for (int n = group; n < stats.rows; n += 16) {
+    const int i = chunk * stats.rows + n;
+    float dot = 0;
+    if (i < p.TQ && d < p.D) {
+      const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D + d;
+      const f32x8 g = eight(grad + at);
+      f32x8 o = eight(out + at);
+      if (rest) o += eight(rest + at) * (1.0f / kRest);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dot += g[j] * o[j];
+    }
+    dot = sum16(dot);
+    if (i < p.TQ && lane == 0) {
+      const long long at = (long long)bh * p.TQ + i;
+      stats.level[at] = lse[at] * kLog2e - (sizeof(T) == 2 ? kShift : 0.0f);
+      stats.delta[at] = dot;
+    }
+  }
+  if (h != 0 || threadIdx.x >= 64) return;
+  Reach r{0x7fffffff, 0, 0, 0x7fffffff};
+  for (int n = threadIdx.x; n < stats.rows; n += 64) {
+    const int i = chunk * stats.rows + n;
+    const bool in = i < p.TQ;
+    const Span s = in ? span_of(p, b, i) : Span{0, 0, 0};
+    if (in) stats.lo[(long long)b * p.TQ + i] = s.lo, stats.hi[(long long)b * p.TQ + i] = s.hi;
+    if (s.hi > s.lo) r.lo = min(r.lo, s.lo), r.hi = max(r.hi, s.hi);
+    r.all_lo = max(r.all_lo, s.lo), r.all_hi = min(r.all_hi, s.hi);  // a chunk with rows beyond the last query is never whole
+  }
+#pragma unroll
+  for (int m = 32; m; m >>= 1) {
+    r.lo = min(r.lo, __shfl_xor(r.lo, m)), r.hi = max(r.hi, __shfl_xor(r.hi, m));
+    r.all_lo = max(r.all_lo, __shfl_xor(r.all_lo, m)), r.all_hi = min(r.all_hi, __shfl_xor(r.all_hi, m));
+  }
+  if (threadIdx.x == 0) stats.reach[(long long)b * stats.chunks + chunk] = r;
+}
+
+// Gradients of scores in float16: a lane's column is held at a power of two of its own, which follows its largest value so far (in both
+// halves of the wavefront) and leaves that 2^8 of room, so that values down to 2^-21 of it keep all their digits and the sums are seldom
+// scaled.  Float32 needs none of this.
+struct Unit {
+  float by = 0x1p100f;  // nothing seen yet
+};
+
+template <typename T, int PARTS>
+__device__ __forceinline__ void in_units(Unit &unit, f32x16 &ds, f32x16 (&sums)[PARTS]) {
+  if constexpr (sizeof(T) == 2) {
+    float most = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) most = __builtin_fmaxf(most, __builtin_fabsf(ds[r]));
+    most = larger_half(most);
+    const bool over = most * unit.by > 0x1p15f;
+    if (__any(over)) {
+      const int e = min(max(261 - (int)(__builtin_bit_cast(unsigned, most) >> 23), 1), 254);  // 2^7 / 2^e of the largest
+      const float now = over ? __builtin_bit_cast(float, e << 23) : unit.by, back = now / unit.by;
+      unit.by = now;
+#pragma unroll
+      for (int n = 0; n < PARTS; ++n) sums[n] *= back;
+    }
+    ds *= unit.by;
+  }
+}
+
+// The weight and, but for (dP - delta), the gradient of a tile's scores; `away`: place of the query less the key's, as they differ along r.
+// On return s holds 2^shift P and `through` what the cap lets pass.
+template <bool ROW_IS_KEY>
+__device__ __forceinline__ void weights_of(const Attention &p, f32x16 &s, f32x16 &through, const f32x16 &level, float bend, float factor, float slope,
+                                           float away) {
+  if (p.cap > 0) {
+    s *= bend;
+    tanh_of_all(s);
+    through = 1.0f - s * s;
+  }
+  s *= factor;
+  if (p.slopes) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] -= slope * __builtin_fabsf(ROW_IS_KEY ? away - (float)row_of(r, 0) : away + (float)row_of(r, 0));
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - level[r]);
+}
+
+// dq^T = K^T dS^T: as the forward pass, with the queries' rows of grad beside those of q.
+template <typename T, int DP, int KEYS>
+__global__ void __launch_bounds__(256, 2) attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
+                                                              const T *__restrict__ v, const T *__restrict__ grad, T *__restrict__ dq,
+                                                              int *__restrict__ redo) {
+  typedef TileOf<T, DP, KEYS> Tile;
+  typedef typename Fragment<T>::V V;
+  constexpr int kSteps = DP / 16, kParts = DP / 32, kSubs = KEYS / 32;
+  __shared__ __attribute__((aligned(1024))) char tiles[4 * Tile::kBytes];
+  __shared__ int edges[2][4];
+  __shared__ int bad[4];
+  const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)tiles;
+  const Dealt at = dealt(deal, blockIdx.x);
+  const int b = at.pair / p.HK, hk = at.pair % p.HK, hq = hk * p.group + at.head;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+  const int i = at.tile * kBlockRows + wave * 32 + c;
+  const bool in = i < p.TQ;
+  const Span span = in ? span_of(p, b, i) : Span{0, 0, 0};
+  const Reach reach = reach_of(span, in);
+  if (lane == 0) edges[0][wave] = reach.lo, edges[1][wave] = reach.hi;
+
+  V rows[kSteps], grads[kSteps];
+  const long long row = (((long long)b * p.TQ + (in ? i : 0)) * p.HQ + hq) * p.D;
+#pragma unroll
+  for (int n = 0; n < kSteps; ++n) {
+    rows[n] = fragment_of(q + row, 16 * n + 8 * h, p.D, in);
+    grads[n] = fragment_of(grad + row, 16 * n + 8 * h, p.D, in);
+  }
+  const long long stat = ((long long)b * p.HQ + hq) * p.TQ + (in ? i : 0);
+  const float own_level = in ? stats.level[stat] : INFINITY, delta = in ? stats.delta[stat] : 0.0f;
+  Unit unit;
+
+  __syncthreads();
+  const int lo = __builtin_amdgcn_readfirstlane(min(min(edges[0][0], edges[0][1]), min(edges[0][2], edges[0][3])));
+  const int hi = __builtin_amdgcn_readfirstlane(max(max(edges[1][0], edges[1][1]), max(edges[1][2], edges[1][3])));
+  const int count = hi > lo ? (hi - lo + KEYS - 1) / KEYS : 0;
+  const unsigned stride = (unsigned)(p.HK * p.D) * (unsigned)sizeof(T), dim = (unsigned)p.D * (unsigned)sizeof(T);
+  const long long head = (((long long)b * p.TK + lo) * p.HK + hk) * p.D * (long long)sizeof(T);
+  const char *kb = (const char *)k + head, *vb = (const char *)v + head;
+  auto stage = [&](int t) {
+    const long long from = (long long)t * KEYS * stride;
+    const int last = hi - lo - t * KEYS;
+    const unsigned to = lds + (unsigned)(t & 1) * (2 * Tile::kBytes);
+    Tile::load(kb + from, stride, 0, last, dim, to);
+    Tile::load(vb + from, stride, 0, last, dim, to + Tile::kBytes);
+  };
+
+  f32x16 sums[kParts], level;
+#pragma unroll
+  for (int n = 0; n < kParts; ++n) sums[n] = zeros();
+#pragma unroll
+  for (int r = 0; r < 16; ++r) level[r] = own_level;
+  const float bend = p.cap > 0 ? p.scale / p.cap : 0.0f, factor = (p.cap > 0 ? p.cap : p.scale) * kLog2e;
+  const float slope = p.slopes ? p.slopes[hq] * kLog2e : 0.0f;
+
+  if (count) stage(0);
+  all_landed();
+  for (int t = 0; t < count; ++t) {
+    if (t + 1 < count) stage(t + 1);
+    const int key0 = lo + t * KEYS;
+    const unsigned keys = lds + (unsigned)(t & 1) * (2 * Tile::kBytes), values = keys + Tile::kBytes;
+#pragma unroll
+    for (int n = 0; n < kSubs; ++n) {
+      const int from = key0 + 32 * n;
+      if (from >= reach.hi || from + 32 <= reach.lo) continue;
+      f32x16 s = zeros(), dp = zeros(), through;
+#pragma unroll
+      for (int m = 0; m < kSteps; ++m) {
+        s = Fragment<T>::mma(Tile::along(keys, 32 * n + c, m, h), rows[m], s);
+        dp = Fragment<T>::mma(Tile::along(values, 32 * n + c, m, h), grads[m], dp);
+      }
+      weights_of<true>(p, s, through, level, bend, factor, slope, (float)(span.place - from - 4 * h));
+      s *= dp - delta;
+      if (p.cap > 0) s *= through;
+      if (from < reach.all_lo || from + 32 > reach.all_hi) {
+        const unsigned seen = (unsigned)(span.hi - span.lo);
+        const int first = from + 4 * h - span.lo;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = (unsigned)(first + row_of(r, 0)) < seen ? s[r] : 0.0f;
+      }
+      in_units<T>(unit, s, sums);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const V ds = rows_of<T>(s, m);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) sums[part] = Fragment<T>::mma(Tile::across(keys, part, 2 * n + m, lane), ds, sums[part]);
+      }
+    }
+    all_landed();
+  }
+
+  const float by = sizeof(T) == 2 ? p.scale / unit.by * 0x1p-14f : p.scale;  // 2^-kShift
+  bool odd = false;
+  if (in) {
+#pragma unroll
+    for (int n = 0; n < kParts; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int d = 32 * n + row_of(r, h);
+        if (d < p.D) odd |= put_four(dq + row + d, sums[n], r, by);
+      }
+  }
+  odd = __any(odd);
+  if (lane == 0) bad[wave] = odd;
+  __syncthreads();
+  if (threadIdx.x == 0) redo[((long long)b * p.HQ + hq) * deal.tiles + at.tile] = bad[0] | bad[1] | bad[2] | bad[3];
+}
+
+// dv^T = grad^T P and dk^T = q^T dS: a block keeps 128 keys, 32 for each wavefront in its lanes' columns, and goes through the chunks of queries
+// that see any of them, head by head of those that share the keys.
+template <typename T, int DP, int ROWS>
+__global__ void __launch_bounds__(256, 1) attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
+                                                               const T *__restrict__ v, const T *__restrict__ grad, T *__restrict__ dk,
+                                                               T *__restrict__ dv, int *__restrict__ redo) {
+  typedef TileOf<T, DP, ROWS> Tile;
+  typedef typename Fragment<T>::V V;
+  constexpr int kSteps = DP / 16, kParts = DP / 32, kSubs = ROWS / 32;
+  constexpr int kBuffer = 2 * Tile::kBytes + 4 * 256;  // rows of q and grad; level, delta, lo, hi of each
+  __shared__ __attribute__((aligned(1024))) char tiles[2 * kBuffer];
+  __shared__ int bad[4];
+  const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)tiles;
+  const Dealt at = dealt(deal, blockIdx.x);
+  const int b = at.pair / p.HK, hk = at.pair % p.HK, tile = deal.tiles - 1 - at.tile;  // the first keys are seen by most
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+  const int block0 = tile * kBlockRows, key0 = block0 + wave * 32, j = key0 + c;
+  const bool in = j < p.TK;
+
+  V rows[kSteps], values[kSteps];
+  const long long row = (((long long)b * p.TK + (in ? j : 0)) * p.HK + hk) * p.D;
+#pragma unroll
+  for (int n = 0; n < kSteps; ++n) {
+    rows[n] = fragment_of(k + row, 16 * n + 8 * h, p.D, in);
+    values[n] = fragment_of(v + row, 16 * n + 8 * h, p.D, in);
+  }
+  Unit unit;
+  const int n_keys = p.lengths ? min(max(p.lengths[b], 0), p.TK) : p.TK;
+
+  f32x16 sum_k[kParts], sum_v[kParts];
+#pragma unroll
+  for (int n = 0; n < kParts; ++n) sum_k[n] = sum_v[n] = zeros();
+  const float bend = p.cap > 0 ? p.scale / p.cap : 0.0f, factor = (p.cap > 0 ? p.cap : p.scale) * kLog2e;
+
+  const unsigned stride = (unsigned)(p.HQ * p.D) * (unsigned)sizeof(T), dim = (unsigned)p.D * (unsigned)sizeof(T);
+  const int every = p.group * stats.chunks;
+  const Reach *reaches = stats.reach + (long long)b * stats.chunks;
+  // the next chunk, of this head or a later one, with a query that sees a key of the block
+  auto next = [&](int at) {
+    for (; at < every; ++at) {
+      const Reach r = reaches[at % stats.chunks];
+      if (r.lo < block0 + kBlockRows && r.hi > block0) break;
+    }
+    return __builtin_amdgcn_readfirstlane(at);
+  };
+  auto stage = [&](int at, unsigned to) {
+    const int head = hk * p.group + at / stats.chunks, first = at % stats.chunks * ROWS;
+    const long long from = (((long long)b * p.TQ + first) * p.HQ + head) * p.D * (long long)sizeof(T);
+    Tile::load((const char *)q + from, stride, 0, p.TQ - first, dim, to);
+    Tile::load((const char *)grad + from, stride, 0, p.TQ - first, dim, to + Tile::kBytes);
+    const long long stat = ((long long)b * p.HQ + head) * p.TQ + first, span = (long long)b * p.TQ + first;
+    const char *from_stats = wave == 0 ? (const char *)(stats.level + stat) : wave == 1 ? (const char *)(stats.delta + stat)
+                           : wave == 2 ? (const char *)(stats.lo + span) : (const char *)(stats.hi + span);
+    const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(from_stats), 0, 0x7fffffff, 0x00020000);
+    typedef MG_LDS void *LdsPointer;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (LdsPointer)(unsigned long long)(to + 2 * Tile::kBytes + (unsigned)wave * 256u), 4,
+                                             (int)(lane < ROWS && first + lane < p.TQ ? (unsigned)lane * 4u : kBeyond), 0, 0, 0);
+  };
+
+  int at_chunk = next(0);
+  unsigned side = 0;
+  if (at_chunk < every) stage(at_chunk, lds);
+  all_landed();
+  while (at_chunk < every) {
+    const int then = next(at_chunk + 1);
+    if (then < every) stage(then, lds + (side ^ 1) * kBuffer);
+    const Reach reach = reaches[at_chunk % stats.chunks];
+    const unsigned queries = lds + side * kBuffer, grads = queries + Tile::kBytes, levels = grads + Tile::kBytes;
+    if (reach.lo < key0 + 32 && reach.hi > key0) {
+      const int hq = hk * p.group + at_chunk / stats.chunks, first = at_chunk % stats.chunks * ROWS;
+      const float slope = p.slopes ? p.slopes[hq] * kLog2e : 0.0f;
+      const bool whole = key0 >= reach.all_lo && key0 + 32 <= reach.all_hi;
+#pragma unroll
+      for (int n = 0; n < kSubs; ++n) {
+        f32x16 s = zeros(), dp = zeros(), through, level, delta;
+#pragma unroll
+        for (int m = 0; m < kSteps; ++m) {
+          s = Fragment<T>::mma(Tile::along(queries, 32 * n + c, m, h), rows[m], s);
+          dp = Fragment<T>::mma(Tile::along(grads, 32 * n + c, m, h), values[m], dp);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const unsigned from = levels + (unsigned)(32 * n + row_of(r, h)) * 4u;
+          const f32x4 a = *(MG_LDS const f32x4 *)(unsigned long long)from, d = *(MG_LDS const f32x4 *)(unsigned long long)(from + 256u);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) level[r + m] = a[m], delta[r + m] = d[m];
+        }
+        weights_of<false>(p, s, through, level, bend, factor, slope, (float)(first + 32 * n + 4 * h + n_keys - p.TQ - j));
+        f32x16 ds = s * (dp - delta);
+        if (p.cap > 0) ds *= through;
+        if (!whole) {
+#pragma unroll
+          for (int r = 0; r < 16; r += 4) {
+            typedef int s32x4 __attribute__((ext_vector_type(4)));
+            const unsigned from = levels + 512u + (unsigned)(32 * n + row_of(r, h)) * 4u;
+            const s32x4 los = *(MG_LDS const s32x4 *)(unsigned long long)from, his = *(MG_LDS const s32x4 *)(unsigned long long)(from + 256u);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              const bool sees = j >= los[m] && j < his[m];
+              s[r + m] = sees ? s[r + m] : 0.0f;
+              ds[r + m] = sees ? ds[r + m] : 0.0f;
+            }
+          }
+        }
+        in_units<T>(unit, ds, sum_k);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const V weights = rows_of<T>(s, m), back = rows_of<T>(ds, m);
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) {
+            sum_v[part] = Fragment<T>::mma(Tile::across(grads, part, 2 * n + m, lane), weights, sum_v[part]);
+            sum_k[part] = Fragment<T>::mma(Tile::across(queries, part, 2 * n + m, lane), back, sum_k[part]);
+          }
+        }
+      }
+    }
+    all_landed();
+    at_chunk = then;
+    side ^= 1;
+  }
+
+  const float lift = sizeof(T) == 2 ? 0x1p-14f : 1.0f, by = sizeof(T) == 2 ? p.scale / unit.by * lift : p.scale;  // 2^-kShift
+  bool odd = false;
+  if (in) {
+#pragma unroll
+    for (int n = 0; n < kParts; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int d = 32 * n + row_of(r, h);
+        if (d >= p.D) continue;
+        odd |= put_four(dk + row + d, sum_k[n], r, by);
+        odd |= put_four(dv + row + d, sum_v[n], r, lift);
+      }
+  }
+  odd = __any(odd);
+  if (lane == 0) bad[wave] = odd;
+  __syncthreads();
+  if (threadIdx.x == 0) redo[((long long)b * p.HK + hk) * deal.tiles + tile] = bad[0] | bad[1] | bad[2] | bad[3];
+}
+
+template <typename T, int DP, int ROWS>
+void launch_dq(const Attention &p, const Stats &stats, const void *q, const void *k, const void *v, const void *grad, void *dq, int *redo) {
+  const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
+  attention_dq_kernel<T, DP, ROWS><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, runtime().stream>>>(
+      p, deal, stats, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (T *)dq, redo);
+}
+
+template <typename T, int DP, int ROWS>
+void launch_dkv(const Attention &p, const Stats &stats, const void *q, const void *k, const void *v, const void *grad, void *dk, void *dv, int *redo) {
+  const Deal deal{p.B * p.HK, 1, (int)ceil_div(p.TK, kBlockRows)};
+  attention_dkv_kernel<T, DP, ROWS><<<dim3((unsigned)(deal.pairs * deal.tiles)), dim3(256), 0, runtime().stream>>>(
+      p, deal, stats, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (T *)dk, (T *)dv, redo);
+}
+
+template <typename T, int ROWS>
+int backward_of(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
+                const void *grad, void *dq, void *dk, void *dv) {
+  Stats stats{};
+  stats.rows = ROWS, stats.chunks = (int)ceil_div(p.TQ, ROWS);
+  const size_t rows = (size_t)p.B * p.TQ, all = rows * p.HQ;
+  const size_t blocks_q = (size_t)p.B * p.HQ * ceil_div(p.TQ, kBlockRows), blocks_k = (size_t)p.B * p.HK * ceil_div(p.TK, kBlockRows);
+  const size_t chunks = (size_t)p.B * stats.chunks;
+  void *space = nullptr;
+  int rc = workspace(sizeof(Reach) * chunks + 4 * (2 * all + 2 * rows + blocks_q + blocks_k), &space);
+  if (rc) return rc;
+  stats.reach = (Reach *)space;
+  stats.level = (float *)(stats.reach + chunks);
+  stats.delta = stats.level + all;
+  stats.lo = (int *)(stats.delta + all);
+  stats.hi = stats.lo + rows;
+  int *redo_q = stats.hi + rows, *redo_k = redo_q + blocks_q;
+  {
+    ScopedTiming timed(TAG_ATTENTION_DELTA);
+    attention_stats_kernel<T><<<dim3((unsigned)(p.B * p.HQ * stats.chunks)), dim3(256), 0, runtime().stream>>>(
+        p, stats, (const T *)out, (const _Float16 *)rest, (const float *)lse, (const T *)grad);
+    MG_HIP(hipGetLastError());
+  }
+  const int parts = (p.D + 31) / 32;
+  if (dq) {
+    {
+      ScopedTiming timed(TAG_ATTENTION_DQ);
+      if (parts == 1) launch_dq<T, 32, ROWS>(p, stats, q, k, v, grad, dq, redo_q);
+      if (parts == 2) launch_dq<T, 64, ROWS>(p, stats, q, k, v, grad, dq, redo_q);
+      if (parts == 3) launch_dq<T, 96, ROWS>(p, stats, q, k, v, grad, dq, redo_q);
+      if (parts == 4) launch_dq<T, 128, ROWS>(p, stats, q, k, v, grad, dq, redo_q);
+      MG_HIP(hipGetLastError());
+    }
+    rc = dq_rows_again(p, dtype, q, k, v, lse, stats.delta, grad, dq, redo_q, kBlockRows);
+    if (rc) return rc;
+  }
+  if (!dk) return MG_OK;
+  {
+    ScopedTiming timed(TAG_ATTENTION_DKV);
+    if (parts == 1) launch_dkv<T, 32, ROWS>(p, stats, q, k, v, grad, dk, dv, redo_k);
+    if (parts == 2) launch_dkv<T, 64, ROWS>(p, stats, q, k, v, grad, dk, dv, redo_k);
+    if (parts == 3) launch_dkv<T, 96, ROWS>(p, stats, q, k, v, grad, dk, dv, redo_k);
+    if (parts == 4) launch_dkv<T, 128, ROWS>(p, stats, q, k, v, grad, dk, dv, redo_k);
+    MG_HIP(hipGetLastError());
+  }
+  return dkv_rows_again(p, dtype, q, k, v, lse, stats.delta, grad, dk, dv, redo_k, kBlockRows);
+}
+
 }  // namespace
 
-// Head dimensions up to 128 in whole pieces of 16 bytes, from buffers that start on one, rows of a tile within reach of 32 bits.
+// Head dimensions up to 128 in whole fragments, from buffers that start on 16 bytes, rows of a tile within reach of 32 bits.
 bool tiles_take(const Attention &p, int size, uintptr_t ends) {
-  return p.D <= 128 && p.D * size % 16 == 0 && ends % 16 == 0 && (long long)p.HQ * p.D * size * 128 < (1ll << 31) &&
+  return p.D <= 128 && p.D % 8 == 0 && ends % 16 == 0 && (long long)p.HQ * p.D * size * 128 < (1ll << 31) &&
          (long long)p.B * p.HQ * ceil_div(p.TQ, 32) < (1 << 24) && (long long)p.B * p.HK * ceil_div(p.TK, 32) < (1 << 24);
 }
 
@@ -204,6 +641,12 @@ int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, c
     MG_HIP(hipGetLastError());
   }
   return forward_rows_again(p, dtype, q, k, v, out, rest, lse, redo, kBlockRows);
+}
+
+int backward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
+                   const void *grad, void *dq, void *dk, void *dv) {
+  return dtype == MG_F16 ? backward_of<_Float16, 64>(p, dtype, q, k, v, out, rest, lse, grad, dq, dk, dv)
+                         : backward_of<float, 32>(p, dtype, q, k, v, out, rest, lse, grad, dq, dk, dv);
 }
 
 }  // namespace mg
