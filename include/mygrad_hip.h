@@ -99,6 +99,7 @@ typedef struct {
   int64_t window;          /* 0: none; at most 2^30 */
   double scale;            /* of the products */
   double cap;              /* scores become cap * tanh(score / cap); 0: they stay */
+  int64_t longest;         /* lengths are at most this, or else taken as this; 0: at most TK.  What a launch is planned by */
   const int32_t *lengths;  /* (B) keys in use, clamped to [0, TK] */
   const int32_t *prefix;   /* (B) */
   const int32_t *starts;   /* (B, TK) first key of the document that key j belongs to */
@@ -461,7 +462,7 @@ int mg_window_gather(const mg_window_desc *desc, const void *x, void *out);
 /* ---- attention (no counterpart in the reference) ---- */
 
 /* out = softmax(scores) v over the keys each query sees; a query that sees none gets zeros.  For mg_attention_bwd, and null where
- * there will be none: lse:(B, HQ, TQ), float32 (float64 for MG_F64), receives the logarithm of each row's sum of exponentials (+infinity
+ * there will be none: lse:(B, HQ, TQ), float32 (float64 for MG_F64), receives the base-2 logarithm of each row's sum of exponentials (+infinity
  * for a row without any weight); rest, like out, receives with MG_F16 what rounding to float16 took off out, times 2^11 (the gradient of the
  * scores takes products of out and grad off others of nearly the same size), and is not touched with other types.  Sums are carried in float32 (float64 for MG_F64).  What a query does not see does not touch its result, whatever it
  * holds. */

@@ -1,7 +1,7 @@
 // Attention with capped scores, a bias by distance and masks, and its gradient, for gfx950.
 //
 //   s_ij = scale * q_i . k_j                    s_ij = cap * tanh(s_ij / cap)   s_ij -= slope_h * |place_i - j|
-//   P_ij = exp(s_ij - lse_i), lse_i = log sum_j exp(s_ij)  over the keys j that row i sees
+//   P_ij = exp(s_ij) / sum_j exp(s_ij)  over the keys j that row i sees; lse_i = log2 of that sum is kept for the gradient
 //   out_i = sum_j P_ij v_j                      (a row that sees no key: zeros, and no gradient from it)
 //   dP_ij = g_i . v_j      D_i = g_i . out_i    dS_ij = P_ij (dP_ij - D_i) (1 - tanh^2) scale
 //   dq_i = sum_j dS_ij k_j      dk_j = sum_i dS_ij q_i      dv_j = sum_i P_ij g_i   (over the heads that share key head j)
@@ -9,6 +9,7 @@
 // The kernels in this file take any type, head dimension up to 256 and mask: a wavefront per row of the result, keys (or
 // queries) over its lanes, sums in float32 (float64 for float64).  They serve double precision and what the kernels on the
 // matrix cores do not take.  What a row does not see never enters its sums, so infinities and NaN there stay where they are.
+#include "attention_row.h"
 #include "attention_rows.h"
 
 #include <algorithm>
@@ -17,45 +18,6 @@
 namespace mg {
 
 namespace {
-
-constexpr int kMaxDim = 256;
-constexpr int kParts = kMaxDim / 64;  // values of a row that a lane holds
-
-template <typename C>
-__device__ __forceinline__ C wave_sum(C v) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
-  return v;
-}
-
-template <typename C>
-__device__ __forceinline__ C wave_max(C v) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v = max(v, __shfl_xor(v, m));
-  return v;
-}
-
-// The score behind cap and bias; `through`: its derivative by the plain product.
-template <typename C>
-__device__ __forceinline__ C score(const Attention &p, C dot, C slope, int distance, C &through) {
-  const bool wide = sizeof(C) == 8;
-  const C scale = wide ? (C)p.scale64 : (C)p.scale, cap = wide ? (C)p.cap64 : (C)p.cap;
-  C s = dot * scale;
-  through = scale;
-  if (cap > 0) {
-    const C bent = tanh(s / cap);
-    s = cap * bent;
-    through *= 1 - bent * bent;
-  }
-  return s - slope * (C)(distance < 0 ? -distance : distance);
-}
-
-template <typename T, typename C>
-__device__ __forceinline__ C dot_row(const C *row, const T *other, int D) {
-  C sum = 0;
-  for (int d = 0; d < D; ++d) sum += row[d] * (C)other[d];
-  return sum;
-}
 
 // A block takes `each` rows of one head, one after the other for each of its wavefronts; with `redo`, only where its entry there is set.
 struct Rows {
@@ -79,59 +41,14 @@ __device__ __forceinline__ Mine rows_of_wave(const Rows &r, int tokens) {
   return m;
 }
 
-// What the lanes of a wavefront wrote to LDS is there for all of them.
-__device__ __forceinline__ void wave_sees() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 template <typename T, typename C>
 __global__ void __launch_bounds__(256) attention_rows_kernel(Attention p, Rows each, const T *__restrict__ q, const T *__restrict__ k,
                                                              const T *__restrict__ v, T *__restrict__ out, _Float16 *__restrict__ rest,
                                                              C *__restrict__ lse) {
   __shared__ C rows[4][kMaxDim];
-  const int lane = threadIdx.x & 63;
-  C *mine = rows[threadIdx.x >> 6];
   const Mine r = rows_of_wave(each, p.TQ);
-  const int b = (int)(r.first / p.HQ), h = (int)(r.first % p.HQ);
-  const long long step = (long long)p.HK * p.D, head = ((long long)b * p.TK * p.HK + h / p.group) * p.D;
-  const C slope = p.slopes ? (C)p.slopes[h] : C(0);
-  for (int i = r.row; i < r.end; i += 4) {
-    const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
-    wave_sees();
-    for (int d = lane; d < p.D; d += 64) mine[d] = (C)q[at + d];
-    wave_sees();
-    const Span span = span_of(p, b, i);
-    C top = -INFINITY, total = 0, sum[kParts] = {};
-    for (int j0 = span.lo; j0 < span.hi; j0 += 64) {
-      const int j = j0 + lane, count = min(64, span.hi - j0);
-      C s = -INFINITY, through;
-      if (lane < count) s = score<C>(p, dot_row<T, C>(mine, k + head + j * step, p.D), slope, span.place - j, through);
-      const C now = max(top, wave_max(s)), base = now == -INFINITY ? C(0) : now;
-      const C back = exp(top - base);
-      const C e = lane < count ? exp(s - base) : C(0);
-      total = total * back + wave_sum(e);
-      top = now;
-  #pragma unroll
-      for (int c = 0; c < kParts; ++c) sum[c] *= back;
-      for (int n = 0; n < count; ++n) {
-        const C weight = __shfl(e, n);
-        const T *row = v + head + (j0 + n) * step;
-  #pragma unroll
-        for (int c = 0; c < kParts; ++c)
-          if (lane + 64 * c < p.D) sum[c] += weight * (C)row[lane + 64 * c];
-      }
-    }
-    const bool none = total == 0;
-  #pragma unroll
-    for (int c = 0; c < kParts; ++c)
-      if (lane + 64 * c < p.D) {
-        const C value = none ? C(0) : sum[c] / total;
-        out[at + lane + 64 * c] = (T)value;
-        if (rest) rest[at + lane + 64 * c] = (_Float16)((value - (C)(T)value) * (C)kRest);
-      }
-    if (lse && lane == 0) lse[r.first * p.TQ + i] = none ? (C)INFINITY : top + log(total);  // no weight on any key
-  }
+  for (int i = r.row; i < r.end; i += 4)
+    attend_row<T, C>(p, (int)(r.first / p.HQ), (int)(r.first % p.HQ), i, rows[threadIdx.x >> 6], q, k, v, out, rest, lse);
 }
 
 // D_i, a wavefront per row.
@@ -175,17 +92,17 @@ __global__ void __launch_bounds__(256) attention_dq_rows_kernel(Attention p, Row
       if (lane < count) {
         C through;
         const C s = score<C>(p, dot_row<T, C>(rows[0][wave], k + head + j * step, p.D), slope, span.place - j, through);
-        ds = exp(s - norm) * (dot_row<T, C>(rows[1][wave], v + head + j * step, p.D) - mean) * through;
+        ds = exp2(s * (C)kLog2e64 - norm) * (dot_row<T, C>(rows[1][wave], v + head + j * step, p.D) - mean) * through;
       }
       for (int n = 0; n < count; ++n) {
         const C weight = __shfl(ds, n);
         const T *row = k + head + (j0 + n) * step;
-  #pragma unroll
+#pragma unroll
         for (int c = 0; c < kParts; ++c)
           if (lane + 64 * c < p.D) sum[c] += weight * (C)row[lane + 64 * c];
       }
     }
-  #pragma unroll
+#pragma unroll
     for (int c = 0; c < kParts; ++c)
       if (lane + 64 * c < p.D) dq[at + lane + 64 * c] = (T)sum[c];
   }
@@ -221,7 +138,7 @@ __global__ void __launch_bounds__(256) attention_dkv_rows_kernel(Attention p, Ro
           if (sees) {
             C through;
             const C s = score<C>(p, dot_row<T, C>(rows[0][wave], q + head + i * step, p.D), slope, span.place - j, through);
-            weight = exp(s - lse[stats + i]);
+            weight = exp2(s * (C)kLog2e64 - lse[stats + i]);
             ds = weight * (dot_row<T, C>(rows[1][wave], grad + head + i * step, p.D) - delta[stats + i]) * through;
           }
         }
@@ -229,7 +146,7 @@ __global__ void __launch_bounds__(256) attention_dkv_rows_kernel(Attention p, Ro
           const int n = __ffsll(left) - 1;
           const C of_v = __shfl(weight, n), of_k = __shfl(ds, n);
           const T *qr = q + head + (i0 + n) * step, *gr = grad + head + (i0 + n) * step;
-  #pragma unroll
+#pragma unroll
           for (int c = 0; c < kParts; ++c)
             if (lane + 64 * c < p.D) {
               sum_k[c] += of_k * (C)qr[lane + 64 * c];
@@ -238,7 +155,7 @@ __global__ void __launch_bounds__(256) attention_dkv_rows_kernel(Attention p, Ro
         }
       }
     }
-  #pragma unroll
+#pragma unroll
     for (int c = 0; c < kParts; ++c)
       if (lane + 64 * c < p.D) dk[at + lane + 64 * c] = (T)sum_k[c], dv[at + lane + 64 * c] = (T)sum_v[c];
   }
@@ -320,12 +237,14 @@ int check_attention(const mg_attention_desc *d, Attention *p, const char *who) {
   if (d->TQ >= most || d->TK >= most || d->HQ >= most || d->B >= most || d->B * d->HQ >= most || d->B * d->HQ * ceil_div(d->TQ, 4) >= (1 << 24) ||
       d->B * d->HK * ceil_div(d->TK, 4) >= (1 << 24))
     return fail(MG_ERR_UNSUPPORTED, "%s: 2^26 rows of results or more", who);
+  if (d->longest < 0) return fail(MG_ERR_BAD_ARG, "%s: a longest length of %lld", who, (long long)d->longest);
   if (d->window < 0 || d->window > most) return fail(MG_ERR_BAD_ARG, "%s: a window of %lld keys", who, (long long)d->window);
   if (!std::isfinite(d->scale) || !std::isfinite(d->cap) || d->cap < 0) return fail(MG_ERR_BAD_ARG, "%s: scale %g, cap %g", who, d->scale, d->cap);
   if (!d->starts != !d->ends) return fail(MG_ERR_BAD_ARG, "%s: starts of documents without their ends, or the other way round", who);
   if (d->window && d->prefix) return fail(MG_ERR_BAD_ARG, "%s: a window and a prefix", who);
   p->B = (int)d->B, p->TQ = (int)d->TQ, p->TK = (int)d->TK, p->HQ = (int)d->HQ, p->HK = (int)d->HK, p->D = (int)d->D;
   p->group = p->HQ / p->HK;
+  p->longest = d->longest ? (int)std::min(d->longest, d->TK) : p->TK;
   p->causal = d->causal != 0, p->window = (int)d->window;
   p->scale = (float)d->scale, p->cap = (float)d->cap, p->scale64 = d->scale, p->cap64 = d->cap;
   p->lengths = d->lengths, p->prefix = d->prefix, p->starts = d->starts, p->ends = d->ends, p->slopes = d->slopes;
@@ -371,7 +290,8 @@ int mg_attention_fwd(const mg_attention_desc *desc, const void *q, const void *k
   if (desc->dtype != MG_F16) rest = nullptr;
   if (desc->dtype == MG_F64) return forward_rows<double, double>(p, kFour, q, k, v, out, rest, lse);
   const uintptr_t ends = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)rest;
-  if (p.TK && tiles_take(p, desc->dtype == MG_F16 ? 2 : 4, ends)) return forward_tiles(p, desc->dtype, q, k, v, out, rest, lse);
+  if (p.TK && tiles_take(p, desc->dtype == MG_F16 ? 2 : 4, ends))
+    return p.TQ <= kFewQueries ? forward_few(p, desc->dtype, q, k, v, out, rest, lse) : forward_tiles(p, desc->dtype, q, k, v, out, rest, lse);
   if (desc->dtype == MG_F32) return forward_rows<float, float>(p, kFour, q, k, v, out, rest, lse);
   return forward_rows<_Float16, float>(p, kFour, q, k, v, out, rest, lse);
 }

@@ -10,6 +10,7 @@ struct Attention {
   int B, TQ, TK, HQ, HK, D;
   int group;  // query heads that share a key head
   int causal, window;
+  int longest;            // no item has more keys in use
   float scale, cap;       // cap 0: scores as they are
   double scale64, cap64;  // the same for double precision
   const int32_t *lengths, *prefix, *starts, *ends;
@@ -23,7 +24,7 @@ struct Span {
 };
 
 __device__ __forceinline__ Span span_of(const Attention &p, int b, int i) {
-  const int n = p.lengths ? min(max(p.lengths[b], 0), p.TK) : p.TK;
+  const int n = p.lengths ? min(max(p.lengths[b], 0), p.longest) : p.TK;
   Span s{0, n, i + n - p.TQ};
   if (p.starts) {
     if (s.place < 0 || s.place >= n) return Span{0, 0, s.place};

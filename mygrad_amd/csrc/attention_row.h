@@ -1,0 +1,98 @@
+// One row of an attention by one wavefront, keys over its lanes: any type, head dimension up to 256 and mask.  What the row does not see never
+// enters its sums.
+#pragma once
+
+#include "attention_rows.h"
+
+namespace mg {
+
+constexpr int kMaxDim = 256;
+constexpr double kLog2e64 = 1.44269504088896340736;
+constexpr int kParts = kMaxDim / 64;  // values of a row that a lane holds
+
+template <typename C>
+__device__ __forceinline__ C wave_sum(C v) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+template <typename C>
+__device__ __forceinline__ C wave_max(C v) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v = max(v, __shfl_xor(v, m));
+  return v;
+}
+
+// The score behind cap and bias; `through`: its derivative by the plain product.
+template <typename C>
+__device__ __forceinline__ C score(const Attention &p, C dot, C slope, int distance, C &through) {
+  const bool wide = sizeof(C) == 8;
+  const C scale = wide ? (C)p.scale64 : (C)p.scale, cap = wide ? (C)p.cap64 : (C)p.cap;
+  C s = dot * scale;
+  through = scale;
+  if (cap > 0) {
+    const C bent = tanh(s / cap);
+    s = cap * bent;
+    through *= 1 - bent * bent;
+  }
+  return s - slope * (C)(distance < 0 ? -distance : distance);
+}
+
+template <typename T, typename C>
+__device__ __forceinline__ C dot_row(const C *row, const T *other, int D) {
+  C sum = 0;
+  for (int d = 0; d < D; ++d) sum += row[d] * (C)other[d];
+  return sum;
+}
+
+// What the lanes of a wavefront wrote to LDS is there for all of them.
+__device__ __forceinline__ void wave_sees() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Row i of head h of batch item b; `mine`: LDS of this wavefront for the row's D values.
+template <typename T, typename C>
+__device__ __forceinline__ void attend_row(const Attention &p, int b, int h, int i, C *mine, const T *__restrict__ q, const T *__restrict__ k,
+                                           const T *__restrict__ v, T *__restrict__ out, _Float16 *__restrict__ rest, C *__restrict__ lse) {
+  const int lane = threadIdx.x & 63;
+  const long long step = (long long)p.HK * p.D, head = ((long long)b * p.TK * p.HK + h / p.group) * p.D;
+  const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
+  const C slope = p.slopes ? (C)p.slopes[h] : C(0);
+  wave_sees();
+  for (int d = lane; d < p.D; d += 64) mine[d] = (C)q[at + d];
+  wave_sees();
+  const Span span = span_of(p, b, i);
+  C top = -INFINITY, total = 0, sum[kParts] = {};
+  for (int j0 = span.lo; j0 < span.hi; j0 += 64) {
+    const int j = j0 + lane, count = min(64, span.hi - j0);
+    C s = -INFINITY, through;
+    if (lane < count) s = score<C>(p, dot_row<T, C>(mine, k + head + j * step, p.D), slope, span.place - j, through);
+    const C now = max(top, wave_max(s)), base = now == -INFINITY ? C(0) : now;
+    const C back = exp(top - base);
+    const C e = lane < count ? exp(s - base) : C(0);
+    total = total * back + wave_sum(e);
+    top = now;
+#pragma unroll
+    for (int c = 0; c < kParts; ++c) sum[c] *= back;
+    for (int n = 0; n < count; ++n) {
+      const C weight = __shfl(e, n);
+      const T *row = v + head + (j0 + n) * step;
+#pragma unroll
+      for (int c = 0; c < kParts; ++c)
+        if (lane + 64 * c < p.D) sum[c] += weight * (C)row[lane + 64 * c];
+    }
+  }
+  const bool none = total == 0;
+#pragma unroll
+  for (int c = 0; c < kParts; ++c)
+    if (lane + 64 * c < p.D) {
+      const C value = none ? C(0) : sum[c] / total;
+      out[at + lane + 64 * c] = (T)value;
+      if (rest) rest[at + lane + 64 * c] = (_Float16)((value - (C)(T)value) * (C)kRest);
+    }
+  if (lse && lane == 0) lse[((long long)b * p.HQ + h) * p.TQ + i] = none ? (C)INFINITY : top * (C)kLog2e64 + log2(total);  // no weight on any key
+}
+
+}  // namespace mg

@@ -1,4 +1,5 @@
-// The two ways to compute an attention: on tiles (attention_tiles.hip), and a row at a time (attention.hip).
+// The ways to compute an attention: on tiles (attention_tiles.hip), for few queries along split keys (attention_few.hip), and a row at a time
+// (attention.hip).
 #pragma once
 
 #include "attention_device.h"
@@ -17,6 +18,9 @@ int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, c
 int forward_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse,
                        const int *redo, int rows);
 
+// Worth it up to so many queries: beyond, a wavefront's 32 columns are filled by the queries of one head.
+constexpr int kFewQueries = 32;
+int forward_few(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse);
 int backward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
                    const void *grad, void *dq, void *dk, void *dv);
 int dq_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad,

@@ -23,7 +23,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 #define MG_LDS __attribute__((address_space(3)))
 
 constexpr unsigned kBeyond = 0x80000000u;  // a byte offset past the end of any buffer: reads as zero
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
 
 template <typename T>
 struct Fragment;
@@ -64,18 +64,18 @@ struct TileOf {
     return (row >> 1) & 7;  // 8 or 24
   }
 
-  // Rows [0, ROWS) from `base` on, `stride` bytes apart, straight into LDS; pieces of rows outside [first, last) and behind the `dim`
-  // bytes of a row are zeros.  The block's 256 threads take part; `lds` is the tile's place in bytes.
-  static __device__ __forceinline__ void load(const char *base, unsigned stride, int first, int last, unsigned dim, unsigned lds) {
+  // Rows [0, ROWS) from `base` on, `stride` bytes apart, straight into LDS; pieces of rows from `last` on and behind the `dim` bytes
+  // of a row are zeros.  THREADS threads (a wavefront, or the block) take part; `lds` is the tile's place in bytes.
+  template <int THREADS>
+  static __device__ __forceinline__ void load(const char *base, unsigned stride, int last, unsigned dim, unsigned lds) {
     typedef MG_LDS void *LdsPointer;
     const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0x7fffffff, 0x00020000);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = THREADS == 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
 #pragma unroll
-    for (int n = 0; n < ROWS * kPieces; n += 256) {
-      const int slot = n + (int)threadIdx.x;
-      if (ROWS * kPieces % 256 == 0 || n + wave * 64 < ROWS * kPieces) {
-        const int row = slot / kPieces, piece = (slot % kPieces) ^ turn(row);
-        const unsigned at = row >= first && row < last && (unsigned)piece * 16u < dim ? (unsigned)row * stride + (unsigned)piece * 16u : kBeyond;
+    for (int n = 0; n < ROWS * kPieces; n += THREADS) {
+      if (ROWS * kPieces % THREADS == 0 || n + wave * 64 < ROWS * kPieces) {
+        const int slot = n + wave * 64 + lane, row = slot / kPieces, piece = (slot % kPieces) ^ turn(row);
+        const unsigned at = row < last && (unsigned)piece * 16u < dim ? (unsigned)row * stride + (unsigned)piece * 16u : kBeyond;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (LdsPointer)(unsigned long long)(lds + (unsigned)(n + wave * 64) * 16u), 16, (int)at, 0, 0, 0);
       }
     }
@@ -222,6 +222,101 @@ __device__ __forceinline__ void tanh_of_all(f32x16 &x) {
     for (int r = 0; r < 16; ++r) x[r] = tanh_small(x[r]);
   }
 }
+
+// Weights are kept as 2^kLift times exp2(score - top): in float16 they are whole down to 2^-29 of the row's largest then.  `top` follows the
+// row's maximum only when that has grown by more than kSlack, so the sums are seldom scaled; 2^(kLift + kSlack) stays below 65504.
+constexpr float kLift = 7.0f, kSlack = 8.0f;
+
+// How scores are made of products, for one query head: factor * (tanh(bend * product), or the product) - slope * distance, in powers of two.
+struct Scores {
+  float bend, factor, slope;
+};
+
+__device__ __forceinline__ Scores scores_of(const Attention &p, int head) {
+  return Scores{p.cap > 0 ? p.scale / p.cap : 0.0f, (p.cap > 0 ? p.cap : p.scale) * kLog2e, p.slopes ? p.slopes[head] * kLog2e : 0.0f};
+}
+
+// 32 queries, one in each lane's column (in both halves), on their way through tiles of SUBS times 32 keys: S^T = K Q^T has a query's scores in
+// its lane (and the partner in the other half), so maximum and sum need no exchange but that one, and the weights are the right operand of
+// out^T = V^T P^T as they lie.
+template <typename T, int DP, int SUBS>
+struct Running {
+  typedef TileOf<T, DP, 32 * SUBS> Tile;
+  typedef typename Fragment<T>::V V;
+  static constexpr int kSteps = DP / 16, kParts = DP / 32;
+
+  f32x16 sums[kParts];
+  float top = -INFINITY, total = 0;  // `total`: of this half's keys
+
+  __device__ __forceinline__ void begin() {
+#pragma unroll
+    for (int n = 0; n < kParts; ++n) sums[n] = zeros();
+  }
+
+  // Keys from `key0` on; `whole`: all columns see all of them.
+  __device__ __forceinline__ void take(const Attention &p, const Scores &how, unsigned keys, unsigned values, const V (&rows)[kSteps], const Span &span,
+                                       int key0, bool whole, int lane) {
+    const int h = lane >> 5, c = lane & 31;
+    f32x16 s[SUBS];
+#pragma unroll
+    for (int n = 0; n < SUBS; ++n) s[n] = zeros();
+#pragma unroll
+    for (int m = 0; m < kSteps; ++m)
+#pragma unroll
+      for (int n = 0; n < SUBS; ++n) s[n] = Fragment<T>::mma(Tile::along(keys, 32 * n + c, m, h), rows[m], s[n]);
+    if (p.cap > 0) {
+#pragma unroll
+      for (int n = 0; n < SUBS; ++n) {
+        s[n] *= how.bend;
+        tanh_of_all(s[n]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < SUBS; ++n) s[n] *= how.factor;
+    if (p.slopes) {
+      const float away = (float)(span.place - key0 - 4 * h);
+#pragma unroll
+      for (int n = 0; n < SUBS; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[n][r] -= how.slope * __builtin_fabsf(away - (float)(32 * n + row_of(r, 0)));
+    }
+    if (!whole) {
+      const unsigned seen = (unsigned)(span.hi - span.lo);
+      const int from = key0 + 4 * h - span.lo;
+#pragma unroll
+      for (int n = 0; n < SUBS; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[n][r] = (unsigned)(from + 32 * n + row_of(r, 0)) < seen ? s[n][r] : -INFINITY;
+    }
+    float most = s[0][0];
+#pragma unroll
+    for (int n = 0; n < SUBS; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) most = __builtin_fmaxf(most, s[n][r]);
+    most = larger_half(most);
+    if (__any(most > top + kSlack)) {  // also the first keys that a column sees
+      const float now = __builtin_fmaxf(top, most), back = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+      top = now;
+      total *= back;
+#pragma unroll
+      for (int n = 0; n < kParts; ++n) sums[n] *= back;
+    }
+    const float base = top == -INFINITY ? 0.0f : top - kLift;
+#pragma unroll
+    for (int n = 0; n < SUBS; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - base);
+        total += s[n][r];
+      }
+#pragma unroll
+    for (int m = 0; m < 2 * SUBS; ++m) {
+      const V weights = rows_of<T>(s[m >> 1], m & 1);
+#pragma unroll
+      for (int n = 0; n < kParts; ++n) sums[n] = Fragment<T>::mma(Tile::across(values, n, m, lane), weights, sums[n]);
+    }
+  }
+};
 
 // How the blocks of a launch are dealt out: `pairs` of a batch item and a key head, each with `heads` query heads and `tiles` row tiles.
 // Blocks go to the eight XCDs in turn, so with a multiple of eight pairs each pair stays on one XCD and is read through one L2.  The

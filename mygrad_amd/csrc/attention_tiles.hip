@@ -10,19 +10,13 @@ namespace {
 
 constexpr int kBlockRows = 128;  // queries of a block: 32 for each of its four wavefronts
 
-// Weights are kept as 2^kLift times exp2(score - top): in float16 they are whole down to 2^-29 of the row's largest then.  `top` follows the
-// row's maximum only when that has grown by more than kSlack, so the sums are seldom scaled; 2^(kLift + kSlack) stays below 65504.
-constexpr float kLift = 7.0f, kSlack = 8.0f;
-
-// S^T = K Q^T has a query in each lane's column, so a row's maximum and sum are taken within a lane (and its partner in the other half),
-// and the weights are the right operand of out^T = V^T P^T as they lie.
 template <typename T, int DP, int KEYS>
 __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T *__restrict__ k,
                                                                  const T *__restrict__ v, T *__restrict__ out, _Float16 *__restrict__ rest,
                                                                  float *__restrict__ lse, int *__restrict__ redo) {
   typedef TileOf<T, DP, KEYS> Tile;
   typedef typename Fragment<T>::V V;
-  constexpr int kSteps = DP / 16, kParts = DP / 32, kSubs = KEYS / 32;
+  constexpr int kSteps = DP / 16, kParts = DP / 32;
   __shared__ __attribute__((aligned(1024))) char tiles[4 * Tile::kBytes];
   __shared__ int edges[2][4];
   __shared__ int bad[4];
@@ -52,88 +46,26 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
     const long long from = (long long)t * KEYS * stride;
     const int last = hi - lo - t * KEYS;
     const unsigned to = lds + (unsigned)(t & 1) * (2 * Tile::kBytes);
-    Tile::load(kb + from, stride, 0, last, dim, to);
-    Tile::load(vb + from, stride, 0, last, dim, to + Tile::kBytes);
+    Tile::template load<256>(kb + from, stride, last, dim, to);
+    Tile::template load<256>(vb + from, stride, last, dim, to + Tile::kBytes);
   };
 
-  f32x16 sums[kParts];
-#pragma unroll
-  for (int n = 0; n < kParts; ++n) sums[n] = zeros();
-  float top = -INFINITY, total = 0;
-  const float bend = p.cap > 0 ? p.scale / p.cap : 0.0f, factor = (p.cap > 0 ? p.cap : p.scale) * kLog2e;
-  const float slope = p.slopes ? p.slopes[hq] * kLog2e : 0.0f;
-
+  Running<T, DP, KEYS / 32> run;
+  run.begin();
+  const Scores how = scores_of(p, hq);
   if (count) stage(0);
   all_landed();
   for (int t = 0; t < count; ++t) {
     if (t + 1 < count) stage(t + 1);
     const int key0 = lo + t * KEYS;
     if (key0 < reach.hi && key0 + KEYS > reach.lo) {
-      const unsigned keys = lds + (unsigned)(t & 1) * (2 * Tile::kBytes), values = keys + Tile::kBytes;
-      f32x16 s[kSubs];
-#pragma unroll
-      for (int n = 0; n < kSubs; ++n) s[n] = zeros();
-#pragma unroll
-      for (int m = 0; m < kSteps; ++m)
-#pragma unroll
-        for (int n = 0; n < kSubs; ++n) s[n] = Fragment<T>::mma(Tile::along(keys, 32 * n + c, m, h), rows[m], s[n]);
-
-      if (p.cap > 0) {
-#pragma unroll
-        for (int n = 0; n < kSubs; ++n) {
-          s[n] *= bend;
-          tanh_of_all(s[n]);
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < kSubs; ++n) s[n] *= factor;
-      if (p.slopes) {
-        const float away = (float)(span.place - key0 - 4 * h);
-#pragma unroll
-        for (int n = 0; n < kSubs; ++n)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[n][r] -= slope * __builtin_fabsf(away - (float)(32 * n + row_of(r, 0)));
-      }
-      if (key0 < reach.all_lo || key0 + KEYS > reach.all_hi) {
-        const unsigned seen = (unsigned)(span.hi - span.lo);
-        const int from = key0 + 4 * h - span.lo;
-#pragma unroll
-        for (int n = 0; n < kSubs; ++n)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[n][r] = (unsigned)(from + 32 * n + row_of(r, 0)) < seen ? s[n][r] : -INFINITY;
-      }
-      float most = s[0][0];
-#pragma unroll
-      for (int n = 0; n < kSubs; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) most = __builtin_fmaxf(most, s[n][r]);
-      most = larger_half(most);
-      if (__any(most > top + kSlack)) {  // also the first keys that a row sees
-        const float now = __builtin_fmaxf(top, most), back = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
-        top = now;
-        total *= back;
-#pragma unroll
-        for (int n = 0; n < kParts; ++n) sums[n] *= back;
-      }
-      const float base = top == -INFINITY ? 0.0f : top - kLift;
-#pragma unroll
-      for (int n = 0; n < kSubs; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - base);
-          total += s[n][r];
-        }
-#pragma unroll
-      for (int m = 0; m < 2 * kSubs; ++m) {
-        const V weights = rows_of<T>(s[m >> 1], m & 1);
-#pragma unroll
-        for (int n = 0; n < kParts; ++n) sums[n] = Fragment<T>::mma(Tile::across(values, n, m, lane), weights, sums[n]);
-      }
+      const unsigned keys = lds + (unsigned)(t & 1) * (2 * Tile::kBytes);
+      run.take(p, how, keys, keys + Tile::kBytes, rows, span, key0, key0 >= reach.all_lo && key0 + KEYS <= reach.all_hi, lane);
     }
     all_landed();
   }
 
-  total = sum_halves(total);
+  const float total = sum_halves(run.total);
   const float by = total > 0 ? 1.0f / total : total == 0 ? 0.0f : NAN;
   bool odd = !(__builtin_fabsf(by) < INFINITY);
   if (in) {
@@ -147,7 +79,7 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
         f32x4 value;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          value[j] = sums[n][r + j] * by;
+          value[j] = run.sums[n][r + j] * by;
           odd |= !(__builtin_fabsf(value[j]) < INFINITY);
         }
         if constexpr (sizeof(T) == 2) {
@@ -158,7 +90,7 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
           *reinterpret_cast<f32x4 *>(out + to + d) = value;
         }
       }
-    if (lse && h == 0) lse[((long long)b * p.HQ + hq) * p.TQ + i] = total == 0 ? INFINITY : (top + __builtin_log2f(total) - kLift) * kLn2;
+    if (lse && h == 0) lse[((long long)b * p.HQ + hq) * p.TQ + i] = total == 0 ? INFINITY : run.top + __builtin_log2f(total) - kLift;
   }
   odd = __any(in && odd);
   if (lane == 0) bad[wave] = odd;
@@ -191,7 +123,7 @@ void launch_forward(const Attention &p, const void *q, const void *k, const void
 
 // ---- gradient ----------------------------------------------------------------------------------------------------------------
 // What the two kernels of the gradient need of each row, made in one pass over out, grad and v:
-//   level_i = lse_i log2(e) - shift     exp2(s_i - level_i) = 2^shift P_i
+//   level_i = lse_i - shift             exp2(s_i - level_i) = 2^shift P_i
 //   delta_i = grad_i . out_i            (with what the rounding of out took off)
 //   spans of the rows, and for each chunk of `rows` rows their union and intersection
 constexpr float kShift = 14.0f;  // 2^14 P in float16: whole down to 2^-28
@@ -234,7 +166,7 @@ __global__ void __launch_bounds__(256) attention_stats_kernel(Attention p, Stats
     dot = sum16(dot);
     if (i < p.TQ && lane == 0) {
       const long long at = (long long)bh * p.TQ + i;
-      stats.level[at] = lse[at] * kLog2e - (sizeof(T) == 2 ? kShift : 0.0f);
+      stats.level[at] = lse[at] - (sizeof(T) == 2 ? kShift : 0.0f);
       stats.delta[at] = dot;
     }
   }
@@ -285,17 +217,16 @@ __device__ __forceinline__ void in_units(Unit &unit, f32x16 &ds, f32x16 (&sums)[
 // The weight and, but for (dP - delta), the gradient of a tile's scores; `away`: place of the query less the key's, as they differ along r.
 // On return s holds 2^shift P and `through` what the cap lets pass.
 template <bool ROW_IS_KEY>
-__device__ __forceinline__ void weights_of(const Attention &p, f32x16 &s, f32x16 &through, const f32x16 &level, float bend, float factor, float slope,
-                                           float away) {
+__device__ __forceinline__ void weights_of(const Attention &p, f32x16 &s, f32x16 &through, const f32x16 &level, const Scores &how, float away) {
   if (p.cap > 0) {
-    s *= bend;
+    s *= how.bend;
     tanh_of_all(s);
     through = 1.0f - s * s;
   }
-  s *= factor;
+  s *= how.factor;
   if (p.slopes) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] -= slope * __builtin_fabsf(ROW_IS_KEY ? away - (float)row_of(r, 0) : away + (float)row_of(r, 0));
+    for (int r = 0; r < 16; ++r) s[r] -= how.slope * __builtin_fabsf(ROW_IS_KEY ? away - (float)row_of(r, 0) : away + (float)row_of(r, 0));
   }
 #pragma unroll
   for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - level[r]);
@@ -344,8 +275,8 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(Attention p, Deal 
     const long long from = (long long)t * KEYS * stride;
     const int last = hi - lo - t * KEYS;
     const unsigned to = lds + (unsigned)(t & 1) * (2 * Tile::kBytes);
-    Tile::load(kb + from, stride, 0, last, dim, to);
-    Tile::load(vb + from, stride, 0, last, dim, to + Tile::kBytes);
+    Tile::template load<256>(kb + from, stride, last, dim, to);
+    Tile::template load<256>(vb + from, stride, last, dim, to + Tile::kBytes);
   };
 
   f32x16 sums[kParts], level;
@@ -353,9 +284,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(Attention p, Deal 
   for (int n = 0; n < kParts; ++n) sums[n] = zeros();
 #pragma unroll
   for (int r = 0; r < 16; ++r) level[r] = own_level;
-  const float bend = p.cap > 0 ? p.scale / p.cap : 0.0f, factor = (p.cap > 0 ? p.cap : p.scale) * kLog2e;
-  const float slope = p.slopes ? p.slopes[hq] * kLog2e : 0.0f;
-
+  const Scores how = scores_of(p, hq);
   if (count) stage(0);
   all_landed();
   for (int t = 0; t < count; ++t) {
@@ -372,7 +301,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(Attention p, Deal 
         s = Fragment<T>::mma(Tile::along(keys, 32 * n + c, m, h), rows[m], s);
         dp = Fragment<T>::mma(Tile::along(values, 32 * n + c, m, h), grads[m], dp);
       }
-      weights_of<true>(p, s, through, level, bend, factor, slope, (float)(span.place - from - 4 * h));
+      weights_of<true>(p, s, through, level, how, (float)(span.place - from - 4 * h));
       s *= dp - delta;
       if (p.cap > 0) s *= through;
       if (from < reach.all_lo || from + 32 > reach.all_hi) {
@@ -436,13 +365,11 @@ __global__ void __launch_bounds__(256, 1) attention_dkv_kernel(Attention p, Deal
     values[n] = fragment_of(v + row, 16 * n + 8 * h, p.D, in);
   }
   Unit unit;
-  const int n_keys = p.lengths ? min(max(p.lengths[b], 0), p.TK) : p.TK;
+  const int n_keys = p.lengths ? min(max(p.lengths[b], 0), p.longest) : p.TK;
 
   f32x16 sum_k[kParts], sum_v[kParts];
 #pragma unroll
   for (int n = 0; n < kParts; ++n) sum_k[n] = sum_v[n] = zeros();
-  const float bend = p.cap > 0 ? p.scale / p.cap : 0.0f, factor = (p.cap > 0 ? p.cap : p.scale) * kLog2e;
-
   const unsigned stride = (unsigned)(p.HQ * p.D) * (unsigned)sizeof(T), dim = (unsigned)p.D * (unsigned)sizeof(T);
   const int every = p.group * stats.chunks;
   const Reach *reaches = stats.reach + (long long)b * stats.chunks;
@@ -457,8 +384,8 @@ __global__ void __launch_bounds__(256, 1) attention_dkv_kernel(Attention p, Deal
   auto stage = [&](int at, unsigned to) {
     const int head = hk * p.group + at / stats.chunks, first = at % stats.chunks * ROWS;
     const long long from = (((long long)b * p.TQ + first) * p.HQ + head) * p.D * (long long)sizeof(T);
-    Tile::load((const char *)q + from, stride, 0, p.TQ - first, dim, to);
-    Tile::load((const char *)grad + from, stride, 0, p.TQ - first, dim, to + Tile::kBytes);
+    Tile::template load<256>((const char *)q + from, stride, p.TQ - first, dim, to);
+    Tile::template load<256>((const char *)grad + from, stride, p.TQ - first, dim, to + Tile::kBytes);
     const long long stat = ((long long)b * p.HQ + head) * p.TQ + first, span = (long long)b * p.TQ + first;
     const char *from_stats = wave == 0 ? (const char *)(stats.level + stat) : wave == 1 ? (const char *)(stats.delta + stat)
                            : wave == 2 ? (const char *)(stats.lo + span) : (const char *)(stats.hi + span);
@@ -479,7 +406,7 @@ __global__ void __launch_bounds__(256, 1) attention_dkv_kernel(Attention p, Deal
     const unsigned queries = lds + side * kBuffer, grads = queries + Tile::kBytes, levels = grads + Tile::kBytes;
     if (reach.lo < key0 + 32 && reach.hi > key0) {
       const int hq = hk * p.group + at_chunk / stats.chunks, first = at_chunk % stats.chunks * ROWS;
-      const float slope = p.slopes ? p.slopes[hq] * kLog2e : 0.0f;
+      const Scores how = scores_of(p, hq);
       const bool whole = key0 >= reach.all_lo && key0 + 32 <= reach.all_hi;
 #pragma unroll
       for (int n = 0; n < kSubs; ++n) {
@@ -496,7 +423,7 @@ __global__ void __launch_bounds__(256, 1) attention_dkv_kernel(Attention p, Deal
 #pragma unroll
           for (int m = 0; m < 4; ++m) level[r + m] = a[m], delta[r + m] = d[m];
         }
-        weights_of<false>(p, s, through, level, bend, factor, slope, (float)(first + 32 * n + 4 * h + n_keys - p.TQ - j));
+        weights_of<false>(p, s, through, level, how, (float)(first + 32 * n + 4 * h + n_keys - p.TQ - j));
         f32x16 ds = s * (dp - delta);
         if (p.cap > 0) ds *= through;
         if (!whole) {

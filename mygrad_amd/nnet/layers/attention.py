@@ -161,6 +161,7 @@ def _describe(q_shape, k_shape, dtype, scale, cap, slopes, mask):
     pointers = mask._bind(batch, queries, keys)
     held = _slopes_on_device(slopes, heads)
     return _hip.AttentionDesc(_hip.storage_code(dtype), mask.causal, batch, queries, keys, heads, kv_heads, dim, mask.window, scale, cap,
+                              0 if mask._lengths is None else max(mask.longest, 1),
                               *pointers, None if held is None else held.ptr), held
 
 
