@@ -14,6 +14,8 @@ namespace mg {
 
 namespace {
 
+constexpr int kMostSplits = 2048;
+
 struct Split {
   int splits;   // blocks along the keys
   int columns;  // query heads of a key head times queries
@@ -116,7 +118,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split split, const float *__restrict__ sums, const float2 *__restrict__ ends,
                                                              const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
                                                              T *__restrict__ out, _Float16 *__restrict__ rest, float *__restrict__ lse) {
-  __shared__ float parts[4][128], totals[4], mine[kMaxDim];
+  __shared__ float parts[4][128], totals[4], mine[kMaxDim], weights[kMostSplits];
   __shared__ int odd[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int hq = blockIdx.x % p.HQ, i = blockIdx.x / p.HQ % p.TQ, b = blockIdx.x / p.HQ / p.TQ;
@@ -125,14 +127,21 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split 
   for (int n = lane; n < split.splits; n += 64) top = __builtin_fmaxf(top, ends[first + (long long)n * split.columns].x);
   top = wave_max(top);
   float total = 0, sum0 = 0, sum1 = 0;
+  for (int n = threadIdx.x; n < split.splits; n += 256) {
+    const float2 end = ends[first + (long long)n * split.columns];
+    weights[n] = end.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(end.x - top);
+    total += end.y * weights[n];
+  }
+  total = wave_sum(total);
+  __syncthreads();
+  const float *from = sums + first * p.D + (lane < p.D ? lane : 0);
+  const long long step = (long long)split.columns * p.D;
+  const int second = lane + 64 < p.D ? 64 : 0;
+#pragma unroll 8
   for (int n = wave; n < split.splits; n += 4) {
-    const long long at = first + (long long)n * split.columns;
-    const float2 end = ends[at];
-    if (end.x == -INFINITY) continue;
-    const float by = __builtin_amdgcn_exp2f(end.x - top);
-    total += end.y * by;
-    if (lane < p.D) sum0 += sums[at * p.D + lane] * by;
-    if (lane + 64 < p.D) sum1 += sums[at * p.D + lane + 64] * by;
+    const float by = weights[n];
+    sum0 += from[n * step] * by;
+    sum1 += from[n * step + second] * by;
   }
   parts[wave][lane] = sum0, parts[wave][lane + 64] = sum1;
   if (lane == 0) totals[wave] = total;
@@ -169,7 +178,7 @@ int few_of(const Attention &p, const void *q, const void *k, const void *v, void
   split.panels = (int)ceil_div(split.columns, 32);
   // A block for each 128 keys (a tile for each wavefront) while there are fewer than fill the device eight times over: a batch of ragged lengths
   // evens out over that many.
-  const int pairs = p.B * p.HK * split.panels, most = std::max(1, 8 * runtime().props.multiProcessorCount / pairs);
+  const int pairs = p.B * p.HK * split.panels, most = std::min(kMostSplits, std::max(1, 8 * runtime().props.multiProcessorCount / pairs));
   split.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, ceil_div(p.longest, 128)));
   const size_t rows = (size_t)p.B * p.HK * split.splits * split.columns;
   void *space = nullptr;

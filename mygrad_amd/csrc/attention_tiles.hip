@@ -214,14 +214,14 @@ __device__ __forceinline__ void in_units(Unit &unit, f32x16 &ds, f32x16 (&sums)[
   }
 }
 
-// The weight and, but for (dP - delta), the gradient of a tile's scores; `away`: place of the query less the key's, as they differ along r.
-// On return s holds 2^shift P and `through` what the cap lets pass.
-template <bool ROW_IS_KEY>
-__device__ __forceinline__ void weights_of(const Attention &p, f32x16 &s, f32x16 &through, const f32x16 &level, const Scores &how, float away) {
+// From products s = q.k and dp = grad.v - delta of a tile to s = 2^shift P and dp = 2^shift dS / scale; `away`: place of the query less the key's,
+// as they differ along r.  level(r): of registers r .. r + 3.
+template <bool ROW_IS_KEY, typename Level>
+__device__ __forceinline__ void gradients_of(const Attention &p, f32x16 &s, f32x16 &dp, const Scores &how, float away, Level level) {
   if (p.cap > 0) {
     s *= how.bend;
     tanh_of_all(s);
-    through = 1.0f - s * s;
+    dp *= 1.0f - s * s;
   }
   s *= how.factor;
   if (p.slopes) {
@@ -229,12 +229,17 @@ __device__ __forceinline__ void weights_of(const Attention &p, f32x16 &s, f32x16
     for (int r = 0; r < 16; ++r) s[r] -= how.slope * __builtin_fabsf(ROW_IS_KEY ? away - (float)row_of(r, 0) : away + (float)row_of(r, 0));
   }
 #pragma unroll
-  for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - level[r]);
+  for (int r = 0; r < 16; r += 4) {
+    const f32x4 from = level(r);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[r + j] = __builtin_amdgcn_exp2f(s[r + j] - from[j]);
+  }
+  dp *= s;
 }
 
 // dq^T = K^T dS^T: as the forward pass, with the queries' rows of grad beside those of q.
 template <typename T, int DP, int KEYS>
-__global__ void __launch_bounds__(256, 2) attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
                                                               const T *__restrict__ v, const T *__restrict__ grad, T *__restrict__ dq,
                                                               int *__restrict__ redo) {
   typedef TileOf<T, DP, KEYS> Tile;
@@ -279,11 +284,9 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(Attention p, Deal 
     Tile::template load<256>(vb + from, stride, last, dim, to + Tile::kBytes);
   };
 
-  f32x16 sums[kParts], level;
+  f32x16 sums[kParts];
 #pragma unroll
   for (int n = 0; n < kParts; ++n) sums[n] = zeros();
-#pragma unroll
-  for (int r = 0; r < 16; ++r) level[r] = own_level;
   const Scores how = scores_of(p, hq);
   if (count) stage(0);
   all_landed();
@@ -295,25 +298,24 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(Attention p, Deal 
     for (int n = 0; n < kSubs; ++n) {
       const int from = key0 + 32 * n;
       if (from >= reach.hi || from + 32 <= reach.lo) continue;
-      f32x16 s = zeros(), dp = zeros(), through;
+      f32x16 s = zeros(), dp = zeros();
 #pragma unroll
       for (int m = 0; m < kSteps; ++m) {
         s = Fragment<T>::mma(Tile::along(keys, 32 * n + c, m, h), rows[m], s);
         dp = Fragment<T>::mma(Tile::along(values, 32 * n + c, m, h), grads[m], dp);
       }
-      weights_of<true>(p, s, through, level, how, (float)(span.place - from - 4 * h));
-      s *= dp - delta;
-      if (p.cap > 0) s *= through;
+      dp -= delta;
+      gradients_of<true>(p, s, dp, how, (float)(span.place - from - 4 * h), [&](int) { return f32x4{own_level, own_level, own_level, own_level}; });
       if (from < reach.all_lo || from + 32 > reach.all_hi) {
         const unsigned seen = (unsigned)(span.hi - span.lo);
         const int first = from + 4 * h - span.lo;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = (unsigned)(first + row_of(r, 0)) < seen ? s[r] : 0.0f;
+        for (int r = 0; r < 16; ++r) dp[r] = (unsigned)(first + row_of(r, 0)) < seen ? dp[r] : 0.0f;
       }
-      in_units<T>(unit, s, sums);
+      in_units<T>(unit, dp, sums);
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const V ds = rows_of<T>(s, m);
+        const V ds = rows_of<T>(dp, m);
 #pragma unroll
         for (int part = 0; part < kParts; ++part) sums[part] = Fragment<T>::mma(Tile::across(keys, part, 2 * n + m, lane), ds, sums[part]);
       }
@@ -341,7 +343,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(Attention p, Deal 
 // dv^T = grad^T P and dk^T = q^T dS: a block keeps 128 keys, 32 for each wavefront in its lanes' columns, and goes through the chunks of queries
 // that see any of them, head by head of those that share the keys.
 template <typename T, int DP, int ROWS>
-__global__ void __launch_bounds__(256, 1) attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
                                                                const T *__restrict__ v, const T *__restrict__ grad, T *__restrict__ dk,
                                                                T *__restrict__ dv, int *__restrict__ redo) {
   typedef TileOf<T, DP, ROWS> Tile;
@@ -410,40 +412,38 @@ __global__ void __launch_bounds__(256, 1) attention_dkv_kernel(Attention p, Deal
       const bool whole = key0 >= reach.all_lo && key0 + 32 <= reach.all_hi;
 #pragma unroll
       for (int n = 0; n < kSubs; ++n) {
-        f32x16 s = zeros(), dp = zeros(), through, level, delta;
+        f32x16 s = zeros(), dp = zeros();
 #pragma unroll
         for (int m = 0; m < kSteps; ++m) {
           s = Fragment<T>::mma(Tile::along(queries, 32 * n + c, m, h), rows[m], s);
           dp = Fragment<T>::mma(Tile::along(grads, 32 * n + c, m, h), values[m], dp);
         }
+        const unsigned stats_at = levels + (unsigned)(32 * n + 4 * h) * 4u;  // registers r .. r + 3 are rows r * 2 and on
+        auto stat = [&](int which, int r) { return *(MG_LDS const f32x4 *)(unsigned long long)(stats_at + (unsigned)(which * 256 + r * 8)); };
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
-          const unsigned from = levels + (unsigned)(32 * n + row_of(r, h)) * 4u;
-          const f32x4 a = *(MG_LDS const f32x4 *)(unsigned long long)from, d = *(MG_LDS const f32x4 *)(unsigned long long)(from + 256u);
+          const f32x4 delta = stat(1, r);
 #pragma unroll
-          for (int m = 0; m < 4; ++m) level[r + m] = a[m], delta[r + m] = d[m];
+          for (int m = 0; m < 4; ++m) dp[r + m] -= delta[m];
         }
-        weights_of<false>(p, s, through, level, how, (float)(first + 32 * n + 4 * h + n_keys - p.TQ - j));
-        f32x16 ds = s * (dp - delta);
-        if (p.cap > 0) ds *= through;
+        gradients_of<false>(p, s, dp, how, (float)(first + 32 * n + 4 * h + n_keys - p.TQ - j), [&](int r) { return stat(0, r); });
         if (!whole) {
 #pragma unroll
           for (int r = 0; r < 16; r += 4) {
             typedef int s32x4 __attribute__((ext_vector_type(4)));
-            const unsigned from = levels + 512u + (unsigned)(32 * n + row_of(r, h)) * 4u;
-            const s32x4 los = *(MG_LDS const s32x4 *)(unsigned long long)from, his = *(MG_LDS const s32x4 *)(unsigned long long)(from + 256u);
+            const s32x4 los = __builtin_bit_cast(s32x4, stat(2, r)), his = __builtin_bit_cast(s32x4, stat(3, r));
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
               const bool sees = j >= los[m] && j < his[m];
               s[r + m] = sees ? s[r + m] : 0.0f;
-              ds[r + m] = sees ? ds[r + m] : 0.0f;
+              dp[r + m] = sees ? dp[r + m] : 0.0f;
             }
           }
         }
-        in_units<T>(unit, ds, sum_k);
+        in_units<T>(unit, dp, sum_k);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          const V weights = rows_of<T>(s, m), back = rows_of<T>(ds, m);
+          const V weights = rows_of<T>(s, m), back = rows_of<T>(dp, m);
 #pragma unroll
           for (int part = 0; part < kParts; ++part) {
             sum_v[part] = Fragment<T>::mma(Tile::across(grads, part, 2 * n + m, lane), weights, sum_v[part]);
