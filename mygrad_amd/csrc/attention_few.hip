@@ -48,19 +48,21 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
 
   const int tiles = reach.hi > reach.lo ? (reach.hi - reach.lo + 31) / 32 : 0;
   const int first = (int)((long long)tiles * part / split.splits), last = (int)((long long)tiles * (part + 1) / split.splits);
-  const unsigned stride = (unsigned)(p.HK * p.D) * (unsigned)sizeof(T), dim = (unsigned)p.D * (unsigned)sizeof(T);
+  const unsigned stride = (unsigned)(p.HK * p.D) * (unsigned)sizeof(T);
+  const typename Tile::template Loader<64> load(stride, (unsigned)p.D * (unsigned)sizeof(T));
   const long long head = (((long long)b * p.TK + reach.lo) * p.HK + hk) * p.D * (long long)sizeof(T);
   const char *kb = (const char *)k + head, *vb = (const char *)v + head;
   const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)space + (unsigned)wave * (STAGES * 2 * Tile::kBytes);
   auto stage = [&](int t, int side) {
     const long long from = (long long)t * 32 * stride;
     const unsigned to = lds + (unsigned)side * (2 * Tile::kBytes);
-    Tile::template load<64>(kb + from, stride, reach.hi - reach.lo - t * 32, dim, to);
-    Tile::template load<64>(vb + from, stride, reach.hi - reach.lo - t * 32, dim, to + Tile::kBytes);
+    load(kb + from, stride, reach.hi - reach.lo - t * 32, to);
+    load(vb + from, stride, reach.hi - reach.lo - t * 32, to + Tile::kBytes);
   };
 
   Running<T, DP, 1> run;
   run.begin();
+  const typename Tile::Place place = Tile::place(lane);
   int side = 0;
   if (first + wave < last) stage(first + wave, 0);
   for (int t = first + wave; t < last; t += 4) {
@@ -69,7 +71,7 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
     if (STAGES == 2 && more) stage(t + 4, side ^ 1);
     const int key0 = reach.lo + t * 32;
     const unsigned keys = lds + (unsigned)side * (2 * Tile::kBytes);
-    run.take(p, how, keys, keys + Tile::kBytes, rows, span, key0, key0 >= reach.all_lo && key0 + 32 <= reach.all_hi, lane);
+    run.take(p, how, keys, keys + Tile::kBytes, rows, span, key0, key0 >= reach.all_lo && key0 + 32 <= reach.all_hi, place, h);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (STAGES == 2)
       side ^= 1;

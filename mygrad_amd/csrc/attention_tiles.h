@@ -64,63 +64,118 @@ struct TileOf {
     return (row >> 1) & 7;  // 8 or 24
   }
 
-  // Rows [0, ROWS) from `base` on, `stride` bytes apart, straight into LDS; pieces of rows from `last` on and behind the `dim` bytes
-  // of a row are zeros.  THREADS threads (a wavefront, or the block) take part; `lds` is the tile's place in bytes.
+  // Brings rows that lie `stride` bytes apart straight into LDS, 16 bytes a lane; THREADS threads (a wavefront, or the block) take part.  A
+  // thread's pieces of all rounds that begin a multiple of sixteen rows apart are permuted alike: one offset serves them.
   template <int THREADS>
-  static __device__ __forceinline__ void load(const char *base, unsigned stride, int last, unsigned dim, unsigned lds) {
-    typedef MG_LDS void *LdsPointer;
-    const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0x7fffffff, 0x00020000);
-    const int wave = THREADS == 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  struct Loader {
+    static constexpr int kRounds = (ROWS * kPieces + THREADS - 1) / THREADS;
+    static constexpr int repeat() {
+      for (int m = 1; m < kRounds; ++m)
+        if (m * THREADS % (16 * kPieces) == 0) return m;
+      return kRounds;
+    }
+    static constexpr int kOffsets = repeat();
+    unsigned at[kOffsets];
+
+    static __device__ __forceinline__ int slot(int round) { return round * THREADS + (int)(THREADS == 64 ? threadIdx.x & 63 : threadIdx.x); }
+
+    // Pieces behind the `dim` bytes of a row are zeros.
+    __device__ __forceinline__ Loader(unsigned stride, unsigned dim) {
 #pragma unroll
-    for (int n = 0; n < ROWS * kPieces; n += THREADS) {
-      if (ROWS * kPieces % THREADS == 0 || n + wave * 64 < ROWS * kPieces) {
-        const int slot = n + wave * 64 + lane, row = slot / kPieces, piece = (slot % kPieces) ^ turn(row);
-        const unsigned at = row < last && (unsigned)piece * 16u < dim ? (unsigned)row * stride + (unsigned)piece * 16u : kBeyond;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (LdsPointer)(unsigned long long)(lds + (unsigned)(n + wave * 64) * 16u), 16, (int)at, 0, 0, 0);
+      for (int n = 0; n < kOffsets; ++n) {
+        const int row = slot(n) / kPieces, piece = (slot(n) % kPieces) ^ turn(row);
+        at[n] = (unsigned)piece * 16u < dim ? (unsigned)row * stride + (unsigned)piece * 16u : kBeyond;
       }
     }
+
+    // Rows [0, ROWS) from `base` on to the tile at byte `lds`; rows from `last` on are zeros.
+    __device__ __forceinline__ void operator()(const char *base, unsigned stride, int last, unsigned lds) const {
+      if (last >= ROWS)
+        rounds<false>(base, stride, last, lds);
+      else
+        rounds<true>(base, stride, last, lds);
+    }
+
+   private:
+    template <bool CUT>
+    __device__ __forceinline__ void rounds(const char *base, unsigned stride, int last, unsigned lds) const {
+      typedef MG_LDS void *LdsPointer;
+      const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0x7fffffff, 0x00020000);
+      const int wave = THREADS == 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+      for (int n = 0; n < kRounds; ++n) {
+        if (ROWS * kPieces % THREADS != 0 && n * THREADS + wave * 64 >= ROWS * kPieces) continue;
+        unsigned from = at[n % kOffsets];
+        if (CUT && slot(n) / kPieces >= last) from = kBeyond;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (LdsPointer)(unsigned long long)(lds + (unsigned)(n * THREADS + wave * 64) * 16u), 16, (int)from,
+                                                 (int)((unsigned)(n / kOffsets * kOffsets * THREADS / kPieces) * stride), 0, 0);
+      }
+    }
+  };
+
+  // Where a lane's fragments lie in a tile, but for what is the same in all lanes: pieces are permuted within groups of kGroup of a row, so
+  // a step to another piece is an exclusive or within the group's bytes and an offset from group to group.
+  static constexpr int kGroup = sizeof(T) == 2 ? (kPieces % 8 ? 4 : kPieces) : (kPieces % 16 ? 8 : 16);
+  struct Place {
+    unsigned along, across[sizeof(T) == 2 ? 2 : 8];
+  };
+
+  static __device__ __forceinline__ Place place(int lane) {
+    const int h = lane >> 5, c = lane & 31;
+    Place at;
+    at.along = (unsigned)(c * kRowBytes + (((sizeof(T) == 2 ? h : 2 * h) ^ turn(c)) & (kGroup - 1)) * 16);
+    if constexpr (sizeof(T) == 2) {
+      // each sixteen lanes hand four rows of sixteen values to one another: lane 4 r + n reads row r at 4 n, lane m gets column m
+      const int piece = 2 * ((lane & 31) >> 4) + ((lane & 3) >> 1);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int row = 8 * n + 4 * h + ((lane & 15) >> 2);
+        at.across[n] = (unsigned)(row * kRowBytes + ((piece ^ turn(row)) & (kGroup - 1)) * 16 + (lane & 1) * 8);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = 8 * (j >> 2) + 4 * h + (j & 3);
+        at.across[j] = (unsigned)(row * kRowBytes + (((c >> 2) ^ turn(row)) & (kGroup - 1)) * 16 + (c & 3) * 4);
+      }
+    }
+    return at;
   }
 
-  // Fragment `step` along the head dimension of row `row`.
-  static __device__ __forceinline__ V along(unsigned lds, int row, int step, int h) {
-    const unsigned at = lds + (unsigned)row * kRowBytes;
-    const int turned = turn(row);
+  static __device__ __forceinline__ unsigned moved(unsigned at, int pieces) {
+    return (at ^ (unsigned)(pieces % kGroup) * 16u) + (unsigned)(pieces / kGroup * kGroup) * 16u;
+  }
+
+  // Fragment `step` along the head dimension of the lane's row of rows 32 sub .. 32 sub + 31.  Tiles start on multiples of 1024 bytes; a
+  // tile that lies a constant `beyond` another shares its addresses.
+  static __device__ __forceinline__ V along(unsigned tile, const Place &place, int sub, int step, unsigned beyond = 0) {
+    const unsigned at = tile + place.along, more = (unsigned)(32 * sub) * kRowBytes + beyond;
     if constexpr (sizeof(T) == 2) {
-      return *(MG_LDS const f16x8 *)(unsigned long long)(at + (unsigned)((2 * step) ^ h ^ turned) * 16u);
+      return *(MG_LDS const f16x8 *)(unsigned long long)(moved(at, 2 * step) + more);
     } else {
-      const f32x4 a = *(MG_LDS const f32x4 *)(unsigned long long)(at + (unsigned)((4 * step) ^ (2 * h) ^ turned) * 16u);
-      const f32x4 b = *(MG_LDS const f32x4 *)(unsigned long long)(at + (unsigned)((4 * step) ^ (2 * h) ^ 1 ^ turned) * 16u);
+      const f32x4 a = *(MG_LDS const f32x4 *)(unsigned long long)(moved(at, 4 * step) + more);
+      const f32x4 b = *(MG_LDS const f32x4 *)(unsigned long long)(moved(at, 4 * step + 1) + more);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
 
   // Fragment `step` along the rows, for values 32 part .. 32 part + 31 of the head dimension (a value for each lane of a half).
-  static __device__ __forceinline__ V across(unsigned lds, int part, int step, int lane) {
-    const int h = lane >> 5;
+  static __device__ __forceinline__ V across(unsigned tile, const Place &place, int part, int step, unsigned beyond = 0) {
+    const unsigned more = (unsigned)(16 * step) * kRowBytes + beyond;
+    V v;
     if constexpr (sizeof(T) == 2) {
-      // each sixteen lanes hand four rows of sixteen values to one another: lane 4 r + n reads row r at 4 n, lane m gets column m
-      const int row = 4 * h + ((lane & 15) >> 2), piece = 2 * ((lane & 31) >> 4) + ((lane & 3) >> 1);
-      V v;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const int at = 16 * step + 8 * n + row;
-        const s16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (MG_LDS s16x4 *)(unsigned long long)(lds + (unsigned)at * kRowBytes + (unsigned)((4 * part) ^ piece ^ turn(at)) * 16u + (unsigned)(lane & 1) * 8u));
+        const s16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4 *)(unsigned long long)(moved(tile + place.across[n], 4 * part) + more));
         const f16x4 f = __builtin_bit_cast(f16x4, q);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[4 * n + j] = f[j];
       }
-      return v;
     } else {
-      V v;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int at = 16 * step + 8 * (j >> 2) + 4 * h + (j & 3), piece = (lane & 31) >> 2;
-        v[j] = *(MG_LDS const float *)(unsigned long long)(lds + (unsigned)at * kRowBytes + (unsigned)((8 * part) ^ piece ^ turn(at)) * 16u +
-                                                           (unsigned)(lane & 3) * 4u);
-      }
-      return v;
+      for (int j = 0; j < 8; ++j) v[j] = *(MG_LDS const float *)(unsigned long long)(moved(tile + place.across[j], 8 * part) + more);
     }
+    return v;
   }
 };
 
@@ -206,8 +261,8 @@ __device__ __forceinline__ float tanh_small(float x) {
 
 __device__ __forceinline__ float tanh_any(float x) {
   const float e = __builtin_amdgcn_exp2f(x * (2 * kLog2e));  // infinity and 0 give +-1
-  const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
-  return __builtin_fabsf(x) < 0.25f ? tanh_small(x) : far;
+  const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f), near = tanh_small(x);
+  return __builtin_fabsf(x) < 0.25f ? near : far;
 }
 
 __device__ __forceinline__ void tanh_of_all(f32x16 &x) {
@@ -216,10 +271,16 @@ __device__ __forceinline__ void tanh_of_all(f32x16 &x) {
   for (int r = 0; r < 16; ++r) most = __builtin_fmaxf(most, __builtin_fabsf(x[r]));
   if (__any(!(most < 0.25f))) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = tanh_any(x[r]);
+    for (int r = 0; r < 16; ++r) {
+      x[r] = tanh_any(x[r]);
+      if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // sixteen at once take too many registers
+    }
   } else {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = tanh_small(x[r]);
+    for (int r = 0; r < 16; ++r) {
+      x[r] = tanh_small(x[r]);
+      if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
   }
 }
 
@@ -255,15 +316,14 @@ struct Running {
 
   // Keys from `key0` on; `whole`: all columns see all of them.
   __device__ __forceinline__ void take(const Attention &p, const Scores &how, unsigned keys, unsigned values, const V (&rows)[kSteps], const Span &span,
-                                       int key0, bool whole, int lane) {
-    const int h = lane >> 5, c = lane & 31;
+                                       int key0, bool whole, const typename Tile::Place &place, int h) {
     f32x16 s[SUBS];
 #pragma unroll
     for (int n = 0; n < SUBS; ++n) s[n] = zeros();
 #pragma unroll
     for (int m = 0; m < kSteps; ++m)
 #pragma unroll
-      for (int n = 0; n < SUBS; ++n) s[n] = Fragment<T>::mma(Tile::along(keys, 32 * n + c, m, h), rows[m], s[n]);
+      for (int n = 0; n < SUBS; ++n) s[n] = Fragment<T>::mma(Tile::along(keys, place, n, m), rows[m], s[n]);
     if (p.cap > 0) {
 #pragma unroll
       for (int n = 0; n < SUBS; ++n) {
@@ -309,12 +369,13 @@ struct Running {
         s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - base);
         total += s[n][r];
       }
+    V weights[2 * SUBS];
 #pragma unroll
-    for (int m = 0; m < 2 * SUBS; ++m) {
-      const V weights = rows_of<T>(s[m >> 1], m & 1);
+    for (int m = 0; m < 2 * SUBS; ++m) weights[m] = rows_of<T>(s[m >> 1], m & 1);
 #pragma unroll
-      for (int n = 0; n < kParts; ++n) sums[n] = Fragment<T>::mma(Tile::across(values, n, m, lane), weights, sums[n]);
-    }
+    for (int n = 0; n < kParts; ++n)
+#pragma unroll
+      for (int m = 0; m < 2 * SUBS; ++m) sums[n] = Fragment<T>::mma(Tile::across(values, place, n, m), weights[m], sums[n]);
   }
 };
 

@@ -39,19 +39,21 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
   const int lo = __builtin_amdgcn_readfirstlane(min(min(edges[0][0], edges[0][1]), min(edges[0][2], edges[0][3])));
   const int hi = __builtin_amdgcn_readfirstlane(max(max(edges[1][0], edges[1][1]), max(edges[1][2], edges[1][3])));
   const int count = hi > lo ? (hi - lo + KEYS - 1) / KEYS : 0;
-  const unsigned stride = (unsigned)(p.HK * p.D) * (unsigned)sizeof(T), dim = (unsigned)p.D * (unsigned)sizeof(T);
+  const unsigned stride = (unsigned)(p.HK * p.D) * (unsigned)sizeof(T);
+  const typename Tile::template Loader<256> load(stride, (unsigned)p.D * (unsigned)sizeof(T));
   const long long head = (((long long)b * p.TK + lo) * p.HK + hk) * p.D * (long long)sizeof(T);
   const char *kb = (const char *)k + head, *vb = (const char *)v + head;
   auto stage = [&](int t) {
     const long long from = (long long)t * KEYS * stride;
     const int last = hi - lo - t * KEYS;
     const unsigned to = lds + (unsigned)(t & 1) * (2 * Tile::kBytes);
-    Tile::template load<256>(kb + from, stride, last, dim, to);
-    Tile::template load<256>(vb + from, stride, last, dim, to + Tile::kBytes);
+    load(kb + from, stride, last, to);
+    load(vb + from, stride, last, to + Tile::kBytes);
   };
 
   Running<T, DP, KEYS / 32> run;
   run.begin();
+  const typename Tile::Place place = Tile::place(lane);
   const Scores how = scores_of(p, hq);
   if (count) stage(0);
   all_landed();
@@ -60,7 +62,7 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
     const int key0 = lo + t * KEYS;
     if (key0 < reach.hi && key0 + KEYS > reach.lo) {
       const unsigned keys = lds + (unsigned)(t & 1) * (2 * Tile::kBytes);
-      run.take(p, how, keys, keys + Tile::kBytes, rows, span, key0, key0 >= reach.all_lo && key0 + KEYS <= reach.all_hi, lane);
+      run.take(p, how, keys, keys + Tile::kBytes, rows, span, key0, key0 >= reach.all_lo && key0 + KEYS <= reach.all_hi, place, h);
     }
     all_landed();
   }
@@ -273,27 +275,29 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
   const int lo = __builtin_amdgcn_readfirstlane(min(min(edges[0][0], edges[0][1]), min(edges[0][2], edges[0][3])));
   const int hi = __builtin_amdgcn_readfirstlane(max(max(edges[1][0], edges[1][1]), max(edges[1][2], edges[1][3])));
   const int count = hi > lo ? (hi - lo + KEYS - 1) / KEYS : 0;
-  const unsigned stride = (unsigned)(p.HK * p.D) * (unsigned)sizeof(T), dim = (unsigned)p.D * (unsigned)sizeof(T);
+  const unsigned stride = (unsigned)(p.HK * p.D) * (unsigned)sizeof(T);
+  const typename Tile::template Loader<256> load(stride, (unsigned)p.D * (unsigned)sizeof(T));
   const long long head = (((long long)b * p.TK + lo) * p.HK + hk) * p.D * (long long)sizeof(T);
   const char *kb = (const char *)k + head, *vb = (const char *)v + head;
   auto stage = [&](int t) {
     const long long from = (long long)t * KEYS * stride;
     const int last = hi - lo - t * KEYS;
     const unsigned to = lds + (unsigned)(t & 1) * (2 * Tile::kBytes);
-    Tile::template load<256>(kb + from, stride, last, dim, to);
-    Tile::template load<256>(vb + from, stride, last, dim, to + Tile::kBytes);
+    load(kb + from, stride, last, to);
+    load(vb + from, stride, last, to + Tile::kBytes);
   };
 
   f32x16 sums[kParts];
 #pragma unroll
   for (int n = 0; n < kParts; ++n) sums[n] = zeros();
+  const typename Tile::Place place = Tile::place(lane);
   const Scores how = scores_of(p, hq);
   if (count) stage(0);
   all_landed();
   for (int t = 0; t < count; ++t) {
     if (t + 1 < count) stage(t + 1);
     const int key0 = lo + t * KEYS;
-    const unsigned keys = lds + (unsigned)(t & 1) * (2 * Tile::kBytes), values = keys + Tile::kBytes;
+    const unsigned keys = lds + (unsigned)(t & 1) * (2 * Tile::kBytes);  // and values behind them
 #pragma unroll
     for (int n = 0; n < kSubs; ++n) {
       const int from = key0 + 32 * n;
@@ -301,8 +305,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
       f32x16 s = zeros(), dp = zeros();
 #pragma unroll
       for (int m = 0; m < kSteps; ++m) {
-        s = Fragment<T>::mma(Tile::along(keys, 32 * n + c, m, h), rows[m], s);
-        dp = Fragment<T>::mma(Tile::along(values, 32 * n + c, m, h), grads[m], dp);
+        s = Fragment<T>::mma(Tile::along(keys, place, n, m), rows[m], s);
+        dp = Fragment<T>::mma(Tile::along(keys, place, n, m, Tile::kBytes), grads[m], dp);
       }
       dp -= delta;
       gradients_of<true>(p, s, dp, how, (float)(span.place - from - 4 * h), [&](int) { return f32x4{own_level, own_level, own_level, own_level}; });
@@ -313,12 +317,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
         for (int r = 0; r < 16; ++r) dp[r] = (unsigned)(first + row_of(r, 0)) < seen ? dp[r] : 0.0f;
       }
       in_units<T>(unit, dp, sums);
+      const V ds[2] = {rows_of<T>(dp, 0), rows_of<T>(dp, 1)};
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const V ds = rows_of<T>(dp, m);
+      for (int part = 0; part < kParts; ++part)
 #pragma unroll
-        for (int part = 0; part < kParts; ++part) sums[part] = Fragment<T>::mma(Tile::across(keys, part, 2 * n + m, lane), ds, sums[part]);
-      }
+        for (int m = 0; m < 2; ++m) sums[part] = Fragment<T>::mma(Tile::across(keys, place, part, 2 * n + m), ds[m], sums[part]);
     }
     all_landed();
   }
@@ -342,7 +345,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
 
 // dv^T = grad^T P and dk^T = q^T dS: a block keeps 128 keys, 32 for each wavefront in its lanes' columns, and goes through the chunks of queries
 // that see any of them, head by head of those that share the keys.
-template <typename T, int DP, int ROWS>
+// With VALUES the keys' values lie in LDS instead of registers: at 128 values of float16 a head the two results and k take 160 of a lane's 256,
+// and with v's 32 as well the scores would not fit.
+template <typename T, int DP, int ROWS, bool VALUES>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
                                                                const T *__restrict__ v, const T *__restrict__ grad, T *__restrict__ dk,
                                                                T *__restrict__ dv, int *__restrict__ redo) {
@@ -350,7 +355,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
   typedef typename Fragment<T>::V V;
   constexpr int kSteps = DP / 16, kParts = DP / 32, kSubs = ROWS / 32;
   constexpr int kBuffer = 2 * Tile::kBytes + 4 * 256;  // rows of q and grad; level, delta, lo, hi of each
-  __shared__ __attribute__((aligned(1024))) char tiles[2 * kBuffer];
+  typedef TileOf<T, DP, kBlockRows> Whole;
+  __shared__ __attribute__((aligned(1024))) char tiles[2 * kBuffer + (VALUES ? Whole::kBytes : 0)];
   __shared__ int bad[4];
   const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)tiles;
   const Dealt at = dealt(deal, blockIdx.x);
@@ -359,12 +365,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
   const int block0 = tile * kBlockRows, key0 = block0 + wave * 32, j = key0 + c;
   const bool in = j < p.TK;
 
-  V rows[kSteps], values[kSteps];
+  V rows[kSteps], values[VALUES ? 1 : kSteps];
   const long long row = (((long long)b * p.TK + (in ? j : 0)) * p.HK + hk) * p.D;
 #pragma unroll
   for (int n = 0; n < kSteps; ++n) {
     rows[n] = fragment_of(k + row, 16 * n + 8 * h, p.D, in);
-    values[n] = fragment_of(v + row, 16 * n + 8 * h, p.D, in);
+    if constexpr (!VALUES) values[n] = fragment_of(v + row, 16 * n + 8 * h, p.D, in);
   }
   Unit unit;
   const int n_keys = p.lengths ? min(max(p.lengths[b], 0), p.longest) : p.TK;
@@ -372,7 +378,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
   f32x16 sum_k[kParts], sum_v[kParts];
 #pragma unroll
   for (int n = 0; n < kParts; ++n) sum_k[n] = sum_v[n] = zeros();
-  const unsigned stride = (unsigned)(p.HQ * p.D) * (unsigned)sizeof(T), dim = (unsigned)p.D * (unsigned)sizeof(T);
+  const typename Tile::Place place = Tile::place(lane);
+  const unsigned stride = (unsigned)(p.HQ * p.D) * (unsigned)sizeof(T);
+  const typename Tile::template Loader<256> load(stride, (unsigned)p.D * (unsigned)sizeof(T));
   const int every = p.group * stats.chunks;
   const Reach *reaches = stats.reach + (long long)b * stats.chunks;
   // the next chunk, of this head or a later one, with a query that sees a key of the block
@@ -386,8 +394,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
   auto stage = [&](int at, unsigned to) {
     const int head = hk * p.group + at / stats.chunks, first = at % stats.chunks * ROWS;
     const long long from = (((long long)b * p.TQ + first) * p.HQ + head) * p.D * (long long)sizeof(T);
-    Tile::template load<256>((const char *)q + from, stride, p.TQ - first, dim, to);
-    Tile::template load<256>((const char *)grad + from, stride, p.TQ - first, dim, to + Tile::kBytes);
+    load((const char *)q + from, stride, p.TQ - first, to);
+    load((const char *)grad + from, stride, p.TQ - first, to + Tile::kBytes);
     const long long stat = ((long long)b * p.HQ + head) * p.TQ + first, span = (long long)b * p.TQ + first;
     const char *from_stats = wave == 0 ? (const char *)(stats.level + stat) : wave == 1 ? (const char *)(stats.delta + stat)
                            : wave == 2 ? (const char *)(stats.lo + span) : (const char *)(stats.hi + span);
@@ -397,6 +405,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
                                              (int)(lane < ROWS && first + lane < p.TQ ? (unsigned)lane * 4u : kBeyond), 0, 0, 0);
   };
 
+  const unsigned whole_values = lds + 2 * kBuffer;
+  if constexpr (VALUES) {
+    const unsigned key_stride = (unsigned)(p.HK * p.D) * (unsigned)sizeof(T);
+    const typename Whole::template Loader<256> load_values(key_stride, (unsigned)p.D * (unsigned)sizeof(T));
+    load_values((const char *)v + (((long long)b * p.TK + block0) * p.HK + hk) * p.D * (long long)sizeof(T), key_stride, p.TK - block0, whole_values);
+  }
   int at_chunk = next(0);
   unsigned side = 0;
   if (at_chunk < every) stage(at_chunk, lds);
@@ -405,18 +419,19 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
     const int then = next(at_chunk + 1);
     if (then < every) stage(then, lds + (side ^ 1) * kBuffer);
     const Reach reach = reaches[at_chunk % stats.chunks];
-    const unsigned queries = lds + side * kBuffer, grads = queries + Tile::kBytes, levels = grads + Tile::kBytes;
+    const unsigned queries = lds + side * kBuffer, levels = queries + 2 * Tile::kBytes;  // grads between them
     if (reach.lo < key0 + 32 && reach.hi > key0) {
       const int hq = hk * p.group + at_chunk / stats.chunks, first = at_chunk % stats.chunks * ROWS;
       const Scores how = scores_of(p, hq);
       const bool whole = key0 >= reach.all_lo && key0 + 32 <= reach.all_hi;
-#pragma unroll
+#pragma unroll 1
       for (int n = 0; n < kSubs; ++n) {
         f32x16 s = zeros(), dp = zeros();
 #pragma unroll
         for (int m = 0; m < kSteps; ++m) {
-          s = Fragment<T>::mma(Tile::along(queries, 32 * n + c, m, h), rows[m], s);
-          dp = Fragment<T>::mma(Tile::along(grads, 32 * n + c, m, h), values[m], dp);
+          s = Fragment<T>::mma(Tile::along(queries, place, n, m), rows[m], s);
+          const V value = VALUES ? Tile::along(whole_values + (unsigned)(wave * 32) * Tile::kRowBytes, place, 0, m) : values[VALUES ? 0 : m];
+          dp = Fragment<T>::mma(Tile::along(queries, place, n, m, Tile::kBytes), value, dp);
         }
         const unsigned stats_at = levels + (unsigned)(32 * n + 4 * h) * 4u;  // registers r .. r + 3 are rows r * 2 and on
         auto stat = [&](int which, int r) { return *(MG_LDS const f32x4 *)(unsigned long long)(stats_at + (unsigned)(which * 256 + r * 8)); };
@@ -441,15 +456,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
           }
         }
         in_units<T>(unit, dp, sum_k);
+        const V weights[2] = {rows_of<T>(s, 0), rows_of<T>(s, 1)}, back[2] = {rows_of<T>(dp, 0), rows_of<T>(dp, 1)};
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const V weights = rows_of<T>(s, m), back = rows_of<T>(dp, m);
+        for (int part = 0; part < kParts; ++part)
 #pragma unroll
-          for (int part = 0; part < kParts; ++part) {
-            sum_v[part] = Fragment<T>::mma(Tile::across(grads, part, 2 * n + m, lane), weights, sum_v[part]);
-            sum_k[part] = Fragment<T>::mma(Tile::across(queries, part, 2 * n + m, lane), back, sum_k[part]);
+          for (int m = 0; m < 2; ++m) {
+            sum_k[part] = Fragment<T>::mma(Tile::across(queries, place, part, 2 * n + m), back[m], sum_k[part]);
+            sum_v[part] = Fragment<T>::mma(Tile::across(queries, place, part, 2 * n + m, Tile::kBytes), weights[m], sum_v[part]);
           }
-        }
       }
     }
     all_landed();
@@ -483,10 +497,10 @@ void launch_dq(const Attention &p, const Stats &stats, const void *q, const void
       p, deal, stats, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (T *)dq, redo);
 }
 
-template <typename T, int DP, int ROWS>
+template <typename T, int DP, int ROWS, bool VALUES>
 void launch_dkv(const Attention &p, const Stats &stats, const void *q, const void *k, const void *v, const void *grad, void *dk, void *dv, int *redo) {
   const Deal deal{p.B * p.HK, 1, (int)ceil_div(p.TK, kBlockRows)};
-  attention_dkv_kernel<T, DP, ROWS><<<dim3((unsigned)(deal.pairs * deal.tiles)), dim3(256), 0, runtime().stream>>>(
+  attention_dkv_kernel<T, DP, ROWS, VALUES><<<dim3((unsigned)(deal.pairs * deal.tiles)), dim3(256), 0, runtime().stream>>>(
       p, deal, stats, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (T *)dk, (T *)dv, redo);
 }
 
@@ -494,7 +508,7 @@ template <typename T, int ROWS>
 int backward_of(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
                 const void *grad, void *dq, void *dk, void *dv) {
   Stats stats{};
-  stats.rows = ROWS, stats.chunks = (int)ceil_div(p.TQ, ROWS);
+  stats.rows = sizeof(T) == 2 && p.D > 96 ? 32 : ROWS, stats.chunks = (int)ceil_div(p.TQ, stats.rows);
   const size_t rows = (size_t)p.B * p.TQ, all = rows * p.HQ;
   const size_t blocks_q = (size_t)p.B * p.HQ * ceil_div(p.TQ, kBlockRows), blocks_k = (size_t)p.B * p.HK * ceil_div(p.TK, kBlockRows);
   const size_t chunks = (size_t)p.B * stats.chunks;
@@ -529,10 +543,10 @@ int backward_of(const Attention &p, int dtype, const void *q, const void *k, con
   if (!dk) return MG_OK;
   {
     ScopedTiming timed(TAG_ATTENTION_DKV);
-    if (parts == 1) launch_dkv<T, 32, ROWS>(p, stats, q, k, v, grad, dk, dv, redo_k);
-    if (parts == 2) launch_dkv<T, 64, ROWS>(p, stats, q, k, v, grad, dk, dv, redo_k);
-    if (parts == 3) launch_dkv<T, 96, ROWS>(p, stats, q, k, v, grad, dk, dv, redo_k);
-    if (parts == 4) launch_dkv<T, 128, ROWS>(p, stats, q, k, v, grad, dk, dv, redo_k);
+    if (parts == 1) launch_dkv<T, 32, ROWS, false>(p, stats, q, k, v, grad, dk, dv, redo_k);
+    if (parts == 2) launch_dkv<T, 64, ROWS, false>(p, stats, q, k, v, grad, dk, dv, redo_k);
+    if (parts == 3) launch_dkv<T, 96, ROWS, false>(p, stats, q, k, v, grad, dk, dv, redo_k);
+    if (parts == 4) launch_dkv<T, 128, sizeof(T) == 2 ? 32 : ROWS, sizeof(T) == 2>(p, stats, q, k, v, grad, dk, dv, redo_k);
     MG_HIP(hipGetLastError());
   }
   return dkv_rows_again(p, dtype, q, k, v, lse, stats.delta, grad, dk, dv, redo_k, kBlockRows);
