@@ -23,7 +23,7 @@ struct Split {
 };
 
 // Column n of a panel is query n / group, head n % group.
-template <typename T, int DP, int STAGES>
+template <typename T, int DP, int STAGES, bool BENT>
 __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split split, const T *__restrict__ q, const T *__restrict__ k,
                                                             const T *__restrict__ v, float *__restrict__ sums, float2 *__restrict__ ends) {
   typedef TileOf<T, DP, 32> Tile;
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
     load(vb + from, stride, reach.hi - reach.lo - t * 32, to + Tile::kBytes);
   };
 
-  Running<T, DP, 1> run;
+  Running<T, DP, 1, BENT> run;
   run.begin();
   const typename Tile::Place place = Tile::place(lane);
   int side = 0;
@@ -166,12 +166,6 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split 
   if (wave == 0 && (odd[0] | odd[1] | odd[2] | odd[3])) attend_row<T, float>(p, b, hq, i, mine, q, k, v, out, rest, lse);
 }
 
-template <typename T, int DP, int STAGES>
-void launch_few(const Attention &p, const Split &split, const void *q, const void *k, const void *v, float *sums, float2 *ends) {
-  const unsigned blocks = (unsigned)(p.B * p.HK * split.panels * split.splits);
-  attention_few_kernel<T, DP, STAGES><<<dim3(blocks), dim3(256), 0, runtime().stream>>>(p, split, (const T *)q, (const T *)k, (const T *)v, sums, ends);
-}
-
 template <typename T>
 int few_of(const Attention &p, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
   constexpr int kStages = sizeof(T) == 2 ? 2 : 1;  // as many as four wavefronts have room for at 128 values a head
@@ -190,11 +184,10 @@ int few_of(const Attention &p, const void *q, const void *k, const void *v, void
   float2 *ends = (float2 *)(sums + rows * p.D);
   {
     ScopedTiming timed(TAG_ATTENTION);
-    const int parts = (p.D + 31) / 32;
-    if (parts == 1) launch_few<T, 32, kStages>(p, split, q, k, v, sums, ends);
-    if (parts == 2) launch_few<T, 64, kStages>(p, split, q, k, v, sums, ends);
-    if (parts == 3) launch_few<T, 96, kStages>(p, split, q, k, v, sums, ends);
-    if (parts == 4) launch_few<T, 128, kStages>(p, split, q, k, v, sums, ends);
+    const dim3 grid((unsigned)(p.B * p.HK * split.panels * split.splits));
+    with_shape(p, [&](auto dim, auto bent) {
+      attention_few_kernel<T, dim, kStages, bent><<<grid, dim3(256), 0, runtime().stream>>>(p, split, (const T *)q, (const T *)k, (const T *)v, sums, ends);
+    });
     MG_HIP(hipGetLastError());
   }
   ScopedTiming timed(TAG_ATTENTION_JOIN);

@@ -9,6 +9,8 @@
 // Float16 takes a fragment in one v_mfma_f32_32x32x16_f16, float32 in eight v_mfma_f32_32x32x2_f32.
 #pragma once
 
+#include <type_traits>
+
 #include "attention_device.h"
 
 namespace mg {
@@ -247,39 +249,46 @@ __device__ __forceinline__ typename Fragment<T>::V rows_of(const f32x16 &v, int 
   return __builtin_convertvector(part, typename Fragment<T>::V);
 }
 
-// tanh: an odd polynomial for |x| < 1/4 (what the series leaves out is below 2^-31 of x), an exponential beyond (where the
-// difference from 1 costs no digits that count).  tanh_of_all() takes the polynomial alone where all values of a wavefront are small.
+// tanh of a lane's sixteen values.  Where all of the wavefront's are below 1/4, an odd polynomial (what float32's leaves out is below
+// 2^-31 of x; float16's, two terms shorter, below 2^-19), which takes no quarter-rate instruction.  Else 1 - 2 / (e^2x + 1), which is off by
+// 2^-24 where |x| is small: that is nothing next to weights in float16, float32 takes the polynomial there.
+template <typename T>
 __device__ __forceinline__ float tanh_small(float x) {
   const float y = x * x;
-  float s = -0.00886323553f;       // -1382 / 155925
-  s = s * y + 0.0218694885f;       // 62 / 2835
-  s = s * y - 0.0539682540f;       // -17 / 315
+  float s = -0.0539682540f;                             // -17 / 315
+  if (sizeof(T) == 4) {
+    s = -0.00886323553f;                                // -1382 / 155925
+    s = s * y + 0.0218694885f;                          // 62 / 2835
+    s = s * y - 0.0539682540f;
+  }
   s = s * y + 0.133333333f;
   s = s * y - 0.333333333f;
   return x + x * (s * y);
 }
 
+template <typename T>
 __device__ __forceinline__ float tanh_any(float x) {
   const float e = __builtin_amdgcn_exp2f(x * (2 * kLog2e));  // infinity and 0 give +-1
-  const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f), near = tanh_small(x);
+  const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+  if (sizeof(T) == 2) return far;
+  const float near = tanh_small<T>(x);
   return __builtin_fabsf(x) < 0.25f ? near : far;
 }
 
+template <typename T>
 __device__ __forceinline__ void tanh_of_all(f32x16 &x) {
   float most = 0;
 #pragma unroll
   for (int r = 0; r < 16; ++r) most = __builtin_fmaxf(most, __builtin_fabsf(x[r]));
-  if (__any(!(most < 0.25f))) {
+  const bool small = !__any(!(most < 0.25f));
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      x[r] = tanh_any(x[r]);
-      if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // sixteen at once take too many registers
-    }
-  } else {
+  for (int r = 0; r < 16; r += 4) {  // sixteen at once would take too many registers
+    if (small) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      x[r] = tanh_small(x[r]);
-      if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      for (int j = 0; j < 4; ++j) x[r + j] = tanh_small<T>(x[r + j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[r + j] = tanh_any<T>(x[r + j]);
     }
   }
 }
@@ -299,8 +308,8 @@ __device__ __forceinline__ Scores scores_of(const Attention &p, int head) {
 
 // 32 queries, one in each lane's column (in both halves), on their way through tiles of SUBS times 32 keys: S^T = K Q^T has a query's scores in
 // its lane (and the partner in the other half), so maximum and sum need no exchange but that one, and the weights are the right operand of
-// out^T = V^T P^T as they lie.
-template <typename T, int DP, int SUBS>
+// out^T = V^T P^T as they lie.  BENT: scores have a cap (whose registers the others do without).
+template <typename T, int DP, int SUBS, bool BENT>
 struct Running {
   typedef TileOf<T, DP, 32 * SUBS> Tile;
   typedef typename Fragment<T>::V V;
@@ -324,11 +333,11 @@ struct Running {
     for (int m = 0; m < kSteps; ++m)
 #pragma unroll
       for (int n = 0; n < SUBS; ++n) s[n] = Fragment<T>::mma(Tile::along(keys, place, n, m), rows[m], s[n]);
-    if (p.cap > 0) {
+    if constexpr (BENT) {
 #pragma unroll
       for (int n = 0; n < SUBS; ++n) {
         s[n] *= how.bend;
-        tanh_of_all(s[n]);
+        tanh_of_all<T>(s[n]);
       }
     }
 #pragma unroll
@@ -378,6 +387,20 @@ struct Running {
       for (int m = 0; m < 2 * SUBS; ++m) sums[n] = Fragment<T>::mma(Tile::across(values, place, n, m), weights[m], sums[n]);
   }
 };
+
+// f(head dimension in whole parts of 32, whether scores are bent), both known to the compiler.
+template <typename F>
+void with_shape(const Attention &p, F f) {
+  auto with_dim = [&](auto bent) {
+    switch ((p.D + 31) / 32) {
+      case 1: return f(std::integral_constant<int, 32>{}, bent);
+      case 2: return f(std::integral_constant<int, 64>{}, bent);
+      case 3: return f(std::integral_constant<int, 96>{}, bent);
+      default: return f(std::integral_constant<int, 128>{}, bent);
+    }
+  };
+  p.cap > 0 ? with_dim(std::true_type{}) : with_dim(std::false_type{});
+}
 
 // How the blocks of a launch are dealt out: `pairs` of a batch item and a key head, each with `heads` query heads and `tiles` row tiles.
 // Blocks go to the eight XCDs in turn, so with a multiple of eight pairs each pair stays on one XCD and is read through one L2.  The

@@ -4,13 +4,15 @@
 
 #include "attention_rows.h"
 
+#include <algorithm>
+
 namespace mg {
 
 namespace {
 
 constexpr int kBlockRows = 128;  // queries of a block: 32 for each of its four wavefronts
 
-template <typename T, int DP, int KEYS>
+template <typename T, int DP, int KEYS, bool BENT>
 __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T *__restrict__ k,
                                                                  const T *__restrict__ v, T *__restrict__ out, _Float16 *__restrict__ rest,
                                                                  float *__restrict__ lse, int *__restrict__ redo) {
@@ -51,7 +53,7 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
     load(vb + from, stride, last, to + Tile::kBytes);
   };
 
-  Running<T, DP, KEYS / 32> run;
+  Running<T, DP, KEYS / 32, BENT> run;
   run.begin();
   const typename Tile::Place place = Tile::place(lane);
   const Scores how = scores_of(p, hq);
@@ -113,14 +115,6 @@ __device__ __forceinline__ bool put_four(T *to, const f32x16 &from, int r, float
   typedef T V __attribute__((ext_vector_type(4)));
   *reinterpret_cast<V *>(to) = __builtin_convertvector(value, V);
   return odd;
-}
-
-template <typename T, int DP, int KEYS>
-void launch_forward(const Attention &p, const void *q, const void *k, const void *v, void *out, void *rest, void *lse, int *redo) {
-  const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
-  const unsigned blocks = (unsigned)(deal.pairs * deal.heads * deal.tiles);
-  attention_tiles_kernel<T, DP, KEYS><<<dim3(blocks), dim3(256), 0, runtime().stream>>>(p, deal, (const T *)q, (const T *)k, (const T *)v, (T *)out,
-                                                                                        (_Float16 *)rest, (float *)lse, redo);
 }
 
 // ---- gradient ----------------------------------------------------------------------------------------------------------------
@@ -218,12 +212,14 @@ __device__ __forceinline__ void in_units(Unit &unit, f32x16 &ds, f32x16 (&sums)[
 
 // From products s = q.k and dp = grad.v - delta of a tile to s = 2^shift P and dp = 2^shift dS / scale; `away`: place of the query less the key's,
 // as they differ along r.  level(r): of registers r .. r + 3.
-template <bool ROW_IS_KEY, typename Level>
+template <typename T, bool ROW_IS_KEY, bool BENT, typename Level>
 __device__ __forceinline__ void gradients_of(const Attention &p, f32x16 &s, f32x16 &dp, const Scores &how, float away, Level level) {
-  if (p.cap > 0) {
+  if constexpr (BENT) {
     s *= how.bend;
-    tanh_of_all(s);
+    tanh_of_all<T>(s);
+    __builtin_amdgcn_sched_barrier(0);  // what follows, mixed with this, would not fit in the registers
     dp *= 1.0f - s * s;
+    __builtin_amdgcn_sched_barrier(0);
   }
   s *= how.factor;
   if (p.slopes) {
@@ -240,7 +236,7 @@ __device__ __forceinline__ void gradients_of(const Attention &p, f32x16 &s, f32x
 }
 
 // dq^T = K^T dS^T: as the forward pass, with the queries' rows of grad beside those of q.
-template <typename T, int DP, int KEYS>
+template <typename T, int DP, int KEYS, bool BENT>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
                                                               const T *__restrict__ v, const T *__restrict__ grad, T *__restrict__ dq,
                                                               int *__restrict__ redo) {
@@ -298,7 +294,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
     if (t + 1 < count) stage(t + 1);
     const int key0 = lo + t * KEYS;
     const unsigned keys = lds + (unsigned)(t & 1) * (2 * Tile::kBytes);  // and values behind them
-#pragma unroll
+#pragma unroll BENT ? 1 : kSubs
     for (int n = 0; n < kSubs; ++n) {
       const int from = key0 + 32 * n;
       if (from >= reach.hi || from + 32 <= reach.lo) continue;
@@ -309,7 +305,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
         dp = Fragment<T>::mma(Tile::along(keys, place, n, m, Tile::kBytes), grads[m], dp);
       }
       dp -= delta;
-      gradients_of<true>(p, s, dp, how, (float)(span.place - from - 4 * h), [&](int) { return f32x4{own_level, own_level, own_level, own_level}; });
+      gradients_of<T, true, BENT>(p, s, dp, how, (float)(span.place - from - 4 * h), [&](int) { return f32x4{own_level, own_level, own_level, own_level}; });
       if (from < reach.all_lo || from + 32 > reach.all_hi) {
         const unsigned seen = (unsigned)(span.hi - span.lo);
         const int first = from + 4 * h - span.lo;
@@ -344,13 +340,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
 }
 
 // dv^T = grad^T P and dk^T = q^T dS: a block keeps 128 keys, 32 for each wavefront in its lanes' columns, and goes through the chunks of queries
-// that see any of them, head by head of those that share the keys.
+// that see any of them, head by head of those that share the keys.  Where there are few blocks they are cut: each of `cuts` takes an equal share
+// of the chunks and leaves its sums in float32, which attention_dkv_join_kernel adds up in order.
 // With VALUES the keys' values lie in LDS instead of registers: at 128 values of float16 a head the two results and k take 160 of a lane's 256,
 // and with v's 32 as well the scores would not fit.
-template <typename T, int DP, int ROWS, bool VALUES>
+template <typename T, int DP, int ROWS, bool VALUES, bool BENT>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
                                                                const T *__restrict__ v, const T *__restrict__ grad, T *__restrict__ dk,
-                                                               T *__restrict__ dv, int *__restrict__ redo) {
+                                                               T *__restrict__ dv, int *__restrict__ redo, int cuts, float *__restrict__ parts) {
   typedef TileOf<T, DP, ROWS> Tile;
   typedef typename Fragment<T>::V V;
   constexpr int kSteps = DP / 16, kParts = DP / 32, kSubs = ROWS / 32;
@@ -359,7 +356,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
   __shared__ __attribute__((aligned(1024))) char tiles[2 * kBuffer + (VALUES ? Whole::kBytes : 0)];
   __shared__ int bad[4];
   const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)tiles;
-  const Dealt at = dealt(deal, blockIdx.x);
+  const Dealt at = dealt(deal, blockIdx.x);  // its head is the cut
   const int b = at.pair / p.HK, hk = at.pair % p.HK, tile = deal.tiles - 1 - at.tile;  // the first keys are seen by most
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
   const int block0 = tile * kBlockRows, key0 = block0 + wave * 32, j = key0 + c;
@@ -381,18 +378,44 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
   const typename Tile::Place place = Tile::place(lane);
   const unsigned stride = (unsigned)(p.HQ * p.D) * (unsigned)sizeof(T);
   const typename Tile::template Loader<256> load(stride, (unsigned)p.D * (unsigned)sizeof(T));
-  const int every = p.group * stats.chunks;
   const Reach *reaches = stats.reach + (long long)b * stats.chunks;
-  // the next chunk, of this head or a later one, with a query that sees a key of the block
-  auto next = [&](int at) {
-    for (; at < every; ++at) {
-      const Reach r = reaches[at % stats.chunks];
-      if (r.lo < block0 + kBlockRows && r.hi > block0) break;
+  // of chunks base .. base + 63, those with a query that sees a key of the block
+  auto seeing = [&](int base) -> unsigned long long {
+    bool sees = false;
+    if (base + lane < stats.chunks) {
+      const Reach r = reaches[base + lane];
+      sees = r.lo < block0 + kBlockRows && r.hi > block0;
     }
-    return __builtin_amdgcn_readfirstlane(at);
+    return __ballot(sees);
   };
-  auto stage = [&](int at, unsigned to) {
-    const int head = hk * p.group + at / stats.chunks, first = at % stats.chunks * ROWS;
+  int of_head = 0;
+  for (int base = 0; base < stats.chunks; base += 64) of_head += __popcll(seeing(base));
+  const long long every = (long long)of_head * p.group;
+  const int from = (int)(every * at.head / cuts), count = (int)(every * (at.head + 1) / cuts) - from;
+  int head = hk * p.group, base = 0;
+  unsigned long long left = 0;
+  if (count) {
+    head += from / of_head;
+    left = seeing(0);
+    for (int skip = from % of_head; skip > 0;) {
+      const int here = __popcll(left);
+      if (here <= skip) {
+        skip -= here;
+        left = seeing(base += 64);
+      } else {
+        for (; skip > 0; --skip) left &= left - 1;
+      }
+    }
+  }
+  auto find = [&] {  // the next chunk, of this head or a later one; only where there is one
+    while (!left) {
+      base += 64;
+      if (base >= stats.chunks) base = 0, ++head;
+      left = seeing(base);
+    }
+  };
+  auto stage = [&](int chunk, unsigned to) {
+    const int first = chunk * ROWS;
     const long long from = (((long long)b * p.TQ + first) * p.HQ + head) * p.D * (long long)sizeof(T);
     load((const char *)q + from, stride, p.TQ - first, to);
     load((const char *)grad + from, stride, p.TQ - first, to + Tile::kBytes);
@@ -411,18 +434,26 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
     const typename Whole::template Loader<256> load_values(key_stride, (unsigned)p.D * (unsigned)sizeof(T));
     load_values((const char *)v + (((long long)b * p.TK + block0) * p.HK + hk) * p.D * (long long)sizeof(T), key_stride, p.TK - block0, whole_values);
   }
-  int at_chunk = next(0);
   unsigned side = 0;
-  if (at_chunk < every) stage(at_chunk, lds);
+  int chunk = 0, hq = 0;
+  if (count) {
+    find();
+    chunk = base + __ffsll(left) - 1, hq = head;
+    stage(chunk, lds);
+  }
   all_landed();
-  while (at_chunk < every) {
-    const int then = next(at_chunk + 1);
-    if (then < every) stage(then, lds + (side ^ 1) * kBuffer);
-    const Reach reach = reaches[at_chunk % stats.chunks];
+  for (int n = 0; n < count; ++n) {
+    const int first = chunk * ROWS, this_hq = hq;
+    const Reach reach = reaches[chunk];
+    if (n + 1 < count) {
+      left &= left - 1;
+      find();
+      chunk = base + __ffsll(left) - 1, hq = head;
+      stage(chunk, lds + (side ^ 1) * kBuffer);
+    }
     const unsigned queries = lds + side * kBuffer, levels = queries + 2 * Tile::kBytes;  // grads between them
     if (reach.lo < key0 + 32 && reach.hi > key0) {
-      const int hq = hk * p.group + at_chunk / stats.chunks, first = at_chunk % stats.chunks * ROWS;
-      const Scores how = scores_of(p, hq);
+      const Scores how = scores_of(p, this_hq);
       const bool whole = key0 >= reach.all_lo && key0 + 32 <= reach.all_hi;
 #pragma unroll 1
       for (int n = 0; n < kSubs; ++n) {
@@ -441,7 +472,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
 #pragma unroll
           for (int m = 0; m < 4; ++m) dp[r + m] -= delta[m];
         }
-        gradients_of<false>(p, s, dp, how, (float)(first + 32 * n + 4 * h + n_keys - p.TQ - j), [&](int r) { return stat(0, r); });
+        gradients_of<T, false, BENT>(p, s, dp, how, (float)(first + 32 * n + 4 * h + n_keys - p.TQ - j), [&](int r) { return stat(0, r); });
         if (!whole) {
 #pragma unroll
           for (int r = 0; r < 16; r += 4) {
@@ -467,7 +498,6 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
       }
     }
     all_landed();
-    at_chunk = then;
     side ^= 1;
   }
 
@@ -480,28 +510,56 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
       for (int r = 0; r < 16; r += 4) {
         const int d = 32 * n + row_of(r, h);
         if (d >= p.D) continue;
-        odd |= put_four(dk + row + d, sum_k[n], r, by);
-        odd |= put_four(dv + row + d, sum_v[n], r, lift);
+        if (cuts == 1) {
+          odd |= put_four(dk + row + d, sum_k[n], r, by);
+          odd |= put_four(dv + row + d, sum_v[n], r, lift);
+        } else {
+          const long long all = (long long)p.B * p.TK * p.HK * p.D;
+          put_four(parts + at.head * all + row + d, sum_k[n], r, by);
+          put_four(parts + (cuts + at.head) * all + row + d, sum_v[n], r, lift);
+        }
       }
   }
+  if (cuts > 1) return;
   odd = __any(odd);
   if (lane == 0) bad[wave] = odd;
   __syncthreads();
   if (threadIdx.x == 0) redo[((long long)b * p.HK + hk) * deal.tiles + tile] = bad[0] | bad[1] | bad[2] | bad[3];
 }
 
-template <typename T, int DP, int ROWS>
-void launch_dq(const Attention &p, const Stats &stats, const void *q, const void *k, const void *v, const void *grad, void *dq, int *redo) {
-  const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
-  attention_dq_kernel<T, DP, ROWS><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, runtime().stream>>>(
-      p, deal, stats, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (T *)dq, redo);
+// Adds the cuts' sums in their order, four values a thread; a block takes 128 keys of one head, as the tiles do.
+template <typename T>
+__global__ void __launch_bounds__(256) attention_dkv_join_kernel(Attention p, int tiles, int cuts, const float *__restrict__ parts, T *__restrict__ dk,
+                                                                 T *__restrict__ dv, int *__restrict__ redo) {
+  __shared__ int bad[4];
+  const int pair = blockIdx.x / tiles, tile = blockIdx.x % tiles, b = pair / p.HK, hk = pair % p.HK, of_row = p.D / 4;
+  const long long all = (long long)p.B * p.TK * p.HK * p.D;
+  bool odd = false;
+  for (int n = threadIdx.x; n < 2 * kBlockRows * of_row; n += 256) {
+    const int which = n / (kBlockRows * of_row), rest = n - which * kBlockRows * of_row, j = tile * kBlockRows + rest / of_row;
+    if (j >= p.TK) continue;
+    const long long at = (((long long)b * p.TK + j) * p.HK + hk) * p.D + rest % of_row * 4;
+    f32x4 sum = *(const f32x4 *)(parts + which * cuts * all + at);
+    for (int m = 1; m < cuts; ++m) sum += *(const f32x4 *)(parts + (which * cuts + m) * all + at);
+    typedef T V __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<V *>((which ? dv : dk) + at) = __builtin_convertvector(sum, V);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) odd |= !(__builtin_fabsf(sum[m]) < INFINITY);
+  }
+  odd = __any(odd);
+  if ((threadIdx.x & 63) == 0) bad[threadIdx.x >> 6] = odd;
+  __syncthreads();
+  if (threadIdx.x == 0) redo[blockIdx.x] = bad[0] | bad[1] | bad[2] | bad[3];
 }
 
-template <typename T, int DP, int ROWS, bool VALUES>
-void launch_dkv(const Attention &p, const Stats &stats, const void *q, const void *k, const void *v, const void *grad, void *dk, void *dv, int *redo) {
-  const Deal deal{p.B * p.HK, 1, (int)ceil_div(p.TK, kBlockRows)};
-  attention_dkv_kernel<T, DP, ROWS, VALUES><<<dim3((unsigned)(deal.pairs * deal.tiles)), dim3(256), 0, runtime().stream>>>(
-      p, deal, stats, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (T *)dk, (T *)dv, redo);
+// How many cuts the blocks of attention_dkv_kernel are made in.  All blocks of an unmasked problem take as long, those of a causal one up to twice
+// the mean: one for each compute unit will do, or four.  A cut writes and reads 16 bytes for each value of k, which takes as long as the products
+// with some 250 queries (50 in float32): it is worth it at four times that.  Measured at 4 x 2048 tokens, 16 heads over 4, causal, float16: 604 us
+// in one piece, 460 in two, 355 in four; 3 x 12 heads, 1531 queries, 997 keys: 110 in one, 121 in two.
+int cuts_of(const Attention &p, int blocks, int size) {
+  const int cus = runtime().props.multiProcessorCount, enough = p.causal ? 4 * cus : cus;
+  const long long worth = (long long)p.group * p.TQ / (size == 2 ? 1000 : 200);
+  return (int)std::max(1ll, std::min({(long long)ceil_div(enough, blocks), worth, 8ll}));
 }
 
 template <typename T, int ROWS>
@@ -511,11 +569,13 @@ int backward_of(const Attention &p, int dtype, const void *q, const void *k, con
   stats.rows = sizeof(T) == 2 && p.D > 96 ? 32 : ROWS, stats.chunks = (int)ceil_div(p.TQ, stats.rows);
   const size_t rows = (size_t)p.B * p.TQ, all = rows * p.HQ;
   const size_t blocks_q = (size_t)p.B * p.HQ * ceil_div(p.TQ, kBlockRows), blocks_k = (size_t)p.B * p.HK * ceil_div(p.TK, kBlockRows);
-  const size_t chunks = (size_t)p.B * stats.chunks;
+  const size_t chunks = (size_t)p.B * stats.chunks, keys = (size_t)p.B * p.TK * p.HK * p.D;
+  const int cuts = dk ? cuts_of(p, (int)blocks_k, sizeof(T)) : 1;
   void *space = nullptr;
-  int rc = workspace(sizeof(Reach) * chunks + 4 * (2 * all + 2 * rows + blocks_q + blocks_k), &space);
+  int rc = workspace((cuts > 1 ? 8 * cuts * keys : 0) + sizeof(Reach) * chunks + 4 * (2 * all + 2 * rows + blocks_q + blocks_k), &space);
   if (rc) return rc;
-  stats.reach = (Reach *)space;
+  float *partial = (float *)space;  // whole pieces of 16 bytes: dim is a multiple of 8
+  stats.reach = (Reach *)(partial + (cuts > 1 ? 2 * cuts * keys : 0));
   stats.level = (float *)(stats.reach + chunks);
   stats.delta = stats.level + all;
   stats.lo = (int *)(stats.delta + all);
@@ -527,14 +587,14 @@ int backward_of(const Attention &p, int dtype, const void *q, const void *k, con
         p, stats, (const T *)out, (const _Float16 *)rest, (const float *)lse, (const T *)grad);
     MG_HIP(hipGetLastError());
   }
-  const int parts = (p.D + 31) / 32;
   if (dq) {
     {
       ScopedTiming timed(TAG_ATTENTION_DQ);
-      if (parts == 1) launch_dq<T, 32, ROWS>(p, stats, q, k, v, grad, dq, redo_q);
-      if (parts == 2) launch_dq<T, 64, ROWS>(p, stats, q, k, v, grad, dq, redo_q);
-      if (parts == 3) launch_dq<T, 96, ROWS>(p, stats, q, k, v, grad, dq, redo_q);
-      if (parts == 4) launch_dq<T, 128, ROWS>(p, stats, q, k, v, grad, dq, redo_q);
+      const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
+      with_shape(p, [&](auto dim, auto bent) {
+        attention_dq_kernel<T, dim, ROWS, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, runtime().stream>>>(
+            p, deal, stats, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (T *)dq, redo_q);
+      });
       MG_HIP(hipGetLastError());
     }
     rc = dq_rows_again(p, dtype, q, k, v, lse, stats.delta, grad, dq, redo_q, kBlockRows);
@@ -543,11 +603,18 @@ int backward_of(const Attention &p, int dtype, const void *q, const void *k, con
   if (!dk) return MG_OK;
   {
     ScopedTiming timed(TAG_ATTENTION_DKV);
-    if (parts == 1) launch_dkv<T, 32, ROWS, false>(p, stats, q, k, v, grad, dk, dv, redo_k);
-    if (parts == 2) launch_dkv<T, 64, ROWS, false>(p, stats, q, k, v, grad, dk, dv, redo_k);
-    if (parts == 3) launch_dkv<T, 96, ROWS, false>(p, stats, q, k, v, grad, dk, dv, redo_k);
-    if (parts == 4) launch_dkv<T, 128, sizeof(T) == 2 ? 32 : ROWS, sizeof(T) == 2>(p, stats, q, k, v, grad, dk, dv, redo_k);
+    const Deal deal{p.B * p.HK, cuts, (int)ceil_div(p.TK, kBlockRows)};
+    with_shape(p, [&](auto dim, auto bent) {
+      constexpr bool wide = sizeof(T) == 2 && dim == 128;
+      attention_dkv_kernel<T, dim, wide ? 32 : ROWS, wide, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, runtime().stream>>>(
+          p, deal, stats, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (T *)dk, (T *)dv, redo_k, cuts, partial);
+    });
     MG_HIP(hipGetLastError());
+    if (cuts > 1) {
+      attention_dkv_join_kernel<T><<<dim3((unsigned)(deal.pairs * deal.tiles)), dim3(256), 0, runtime().stream>>>(p, deal.tiles, cuts, partial, (T *)dk,
+                                                                                                                (T *)dv, redo_k);
+      MG_HIP(hipGetLastError());
+    }
   }
   return dkv_rows_again(p, dtype, q, k, v, lse, stats.delta, grad, dk, dv, redo_k, kBlockRows);
 }
@@ -567,18 +634,16 @@ int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, c
   int *redo = (int *)space;
   {
     ScopedTiming timed(TAG_ATTENTION);
-    const int parts = (p.D + 31) / 32;
-    if (dtype == MG_F16) {
-      if (parts == 1) launch_forward<_Float16, 32, 64>(p, q, k, v, out, rest, lse, redo);
-      if (parts == 2) launch_forward<_Float16, 64, 64>(p, q, k, v, out, rest, lse, redo);
-      if (parts == 3) launch_forward<_Float16, 96, 64>(p, q, k, v, out, rest, lse, redo);
-      if (parts == 4) launch_forward<_Float16, 128, 64>(p, q, k, v, out, rest, lse, redo);
-    } else {
-      if (parts == 1) launch_forward<float, 32, 32>(p, q, k, v, out, rest, lse, redo);
-      if (parts == 2) launch_forward<float, 64, 32>(p, q, k, v, out, rest, lse, redo);
-      if (parts == 3) launch_forward<float, 96, 32>(p, q, k, v, out, rest, lse, redo);
-      if (parts == 4) launch_forward<float, 128, 32>(p, q, k, v, out, rest, lse, redo);
-    }
+    const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
+    const dim3 grid((unsigned)(deal.pairs * deal.heads * deal.tiles));
+    auto launch = [&](auto zero) {
+      using T = decltype(zero);
+      with_shape(p, [&](auto dim, auto bent) {
+        attention_tiles_kernel<T, dim, sizeof(T) == 2 ? 64 : 32, bent><<<grid, dim3(256), 0, runtime().stream>>>(
+            p, deal, (const T *)q, (const T *)k, (const T *)v, (T *)out, (_Float16 *)rest, (float *)lse, redo);
+      });
+    };
+    dtype == MG_F16 ? launch(_Float16(0)) : launch(0.0f);
     MG_HIP(hipGetLastError());
   }
   return forward_rows_again(p, dtype, q, k, v, out, rest, lse, redo, kBlockRows);
