@@ -8,7 +8,9 @@
 // Bandwidth-bound: x is read once forward, x and grad once backward; the table's rows are shared by a token's heads.
 #include "internal.h"
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace mg {
 
@@ -150,18 +152,202 @@ __global__ void __launch_bounds__(256) head_norm_dw_kernel(HeadNorm p, long long
     parts[((long long)blockIdx.y * gridDim.x + head) * p.D + d] = sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d];
 }
 
+// A wavefront per value: its lanes take the parts in turn and are added as a tree.
 template <typename T>
 __global__ void __launch_bounds__(256) head_norm_dw_join_kernel(int values, int parts, const double *__restrict__ from, T *__restrict__ dw) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
+  const int lane = threadIdx.x & 63, n = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= values) return;
   double sum = 0;
-  for (int part = 0; part < parts; ++part) sum += from[(long long)part * values + n];
-  dw[n] = (T)sum;
+  for (int part = lane; part < parts; part += 64) sum += from[(long long)part * values + n];
+  sum = wave_sum(sum);
+  if (lane == 0) dw[n] = (T)sum;
+}
+
+// What the lanes of a wavefront wrote to LDS is there for all of them.
+__device__ __forceinline__ void wave_sees() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// ---- rows in whole pieces ----------------------------------------------------------------------------------------------------
+// A lane holds V neighbouring values (16 bytes where the head dimension allows) of a row and LANES = 2^k lanes a row; the wavefront keeps to
+// a token, whose cos and sin stay in registers, while it goes through the heads.  A value's partner in its pair lies in another lane or
+// not, wherever sections and layout put it: rows are handed over through LDS, a wavefront's own.
+// Bound by memory; float16, 16384 tokens of 32 heads of 128 values (134 MB a tensor): see launch_pieces.
+template <typename T, typename C, int V>
+struct Pieces {
+  typedef T Held __attribute__((ext_vector_type(V)));
+  C cos[V], sin[V];  // sin with the sign that the partner's value takes
+  int partner[V];
+
+  // What each of the lane's values turns with.
+  __device__ __forceinline__ void find(const HeadNorm &p, int d0) {
+#pragma unroll
+    for (int n = 0; n < V; ++n) {
+      const int d = d0 + n, pair = pair_of(p, d);
+      const bool first = p.interleaved ? d % 2 == 0 : d < p.pairs;
+      partner[n] = pair < 0 ? d : first ? d + apart(p) : d - apart(p);
+      cos[n] = 1, sin[n] = 0;
+    }
+  }
+
+  static __device__ __forceinline__ int pair_of(const HeadNorm &p, int d) {
+    return d >= 2 * p.pairs ? -1 : p.interleaved ? d / 2 : d < p.pairs ? d : d - p.pairs;
+  }
+
+  __device__ __forceinline__ void turn_at(const HeadNorm &p, const C *table, long long token, int d0) {
+#pragma unroll
+    for (int n = 0; n < V; ++n) {
+      const int d = d0 + n, pair = pair_of(p, d);
+      if (pair < 0) continue;
+      turn_of<C>(p, table, token, pair, cos[n], sin[n]);
+      if (partner[n] > d) sin[n] = -sin[n];
+    }
+  }
+};
+
+template <typename T, typename C, int V, bool BACK>
+__global__ void __launch_bounds__(256) head_norm_pieces_kernel(HeadNorm p, int lanes, bool neighbours, const T *__restrict__ x, const T *__restrict__ w,
+                                                               const C *__restrict__ table, const T *__restrict__ grad, T *__restrict__ out,
+                                                               double *__restrict__ parts) {
+  typedef Pieces<T, C, V> P;
+  typedef typename P::Held Held;
+  typedef C Wide __attribute__((ext_vector_type(V)));
+  __shared__ __attribute__((aligned(64))) char space[4 * 64 * V * sizeof(double)];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (lanes - 1), g = lane / lanes, groups = 64 / lanes;
+  const int d0 = l * V;
+  const bool in = d0 < p.D, each = p.weight_heads > 1;
+  C *row = (C *)space + wave * 64 * V + g * lanes * V;
+  P piece;
+  piece.find(p, in ? d0 : 0);
+  // The groups take heads of one token side by side, of several tokens where these have few.  With weights for each head and their gradient
+  // wanted, a group keeps to one head.
+  const bool keep = BACK && parts && each;
+  const int side = keep ? 1 : min(groups, p.heads), tokens_at_once = keep ? 1 : groups / side;
+  const int first_head = keep ? blockIdx.y * groups + g : g % side, rounds = keep ? 1 : (p.heads + side - 1) / side;
+  const bool mine = in && (keep || g / side < tokens_at_once);
+  const long long tokens = p.rows / p.heads, stride = (long long)gridDim.x * 4 * tokens_at_once;
+
+  Wide weight;
+#pragma unroll
+  for (int n = 0; n < V; ++n) weight[n] = 1;
+  if (p.weight_heads == 1 && in) weight = __builtin_convertvector(*reinterpret_cast<const Held *>(w + d0), Wide);
+  double sums[BACK ? V : 1] = {};
+  for (long long first = ((long long)blockIdx.x * 4 + wave) * tokens_at_once; first < tokens; first += stride) {
+    const long long token = first + (keep ? 0 : g / side);
+    const bool here = mine && token < tokens;
+    if (here && p.pairs) piece.turn_at(p, table, token, d0);
+    for (int round = 0; round < rounds; ++round) {
+      const int head = first_head + round * side;
+      const bool take = here && head < p.heads;
+      const long long at = (token * p.heads + head) * p.D + d0;
+      Wide value{}, other{};
+      if (take) {
+        value = __builtin_convertvector(*reinterpret_cast<const Held *>(x + at), Wide);
+        if (BACK) other = __builtin_convertvector(*reinterpret_cast<const Held *>(grad + at), Wide);
+        if (each) weight = __builtin_convertvector(*reinterpret_cast<const Held *>(w + (long long)head * p.D + d0), Wide);
+      }
+      C squares = 0;
+#pragma unroll
+      for (int n = 0; n < V; ++n) squares += value[n] * value[n];
+      C r = 1;
+      if (p.norm) {
+        for (int m = lanes >> 1; m; m >>= 1) squares += __shfl_xor(squares, m);
+        r = 1 / sqrt(squares / p.D + (C)p.eps);
+      }
+      Wide z = BACK ? other : value * r * weight;
+      if (p.pairs) {
+        wave_sees();
+        *reinterpret_cast<Wide *>(row + l * V) = z;
+        wave_sees();
+        Wide there;
+        if (neighbours) {  // partners of neighbours are neighbours, from a whole piece on
+          there = *reinterpret_cast<const Wide *>(row + piece.partner[0]);
+        } else {
+#pragma unroll
+          for (int n = 0; n < V; ++n) there[n] = row[piece.partner[n]];
+        }
+#pragma unroll
+        for (int n = 0; n < V; ++n) z[n] = z[n] * piece.cos[n] + there[n] * (BACK ? -piece.sin[n] : piece.sin[n]);
+      }
+      if constexpr (BACK) {
+        if (take && parts) {
+#pragma unroll
+          for (int n = 0; n < V; ++n) sums[n] += (double)(z[n] * value[n] * r);
+        }
+        z *= weight;
+        C mean = 0;
+        if (p.norm) {
+#pragma unroll
+          for (int n = 0; n < V; ++n) mean += z[n] * value[n];
+          for (int m = lanes >> 1; m; m >>= 1) mean += __shfl_xor(mean, m);
+          mean *= r * r / p.D;
+        }
+        z = (z - value * mean) * r;
+      }
+      if (take && out) *reinterpret_cast<Held *>(out + at) = __builtin_convertvector(z, Held);
+    }
+  }
+  if constexpr (BACK) {
+    if (!parts) return;
+    // the block's sums: of the groups that share a weight (all of them, but where each head has its own), then of its wavefronts
+    if (!each) {
+      for (int m = lanes; m < 64; m <<= 1)
+#pragma unroll
+        for (int n = 0; n < V; ++n) sums[n] += __shfl_xor(sums[n], m);
+    }
+    __syncthreads();
+    double *all = (double *)space;
+#pragma unroll
+    for (int n = 0; n < V; ++n) all[(wave * 64 + lane) * V + n] = sums[n];
+    __syncthreads();
+    const int held = each ? 64 * V : lanes * V;
+    for (int n = threadIdx.x; n < held; n += 256) {
+      const int head = each ? blockIdx.y * groups + n / (lanes * V) : 0, d = n % (lanes * V);
+      if (d >= p.D || head >= p.weight_heads) continue;
+      parts[((long long)blockIdx.x * p.weight_heads + head) * p.D + d] = all[n] + all[64 * V + n] + all[128 * V + n] + all[192 * V + n];
+    }
+  }
+}
+
+// Values a lane holds: as many as 16 bytes have, fewer where rows start elsewhere or 64 lanes do not suffice the other way round; 0: no way.
+int values_of(const HeadNorm &p, int size, uintptr_t ends) {
+  for (int v = 16 / size; v >= 1; v /= 2)
+    if (p.D % v == 0 && ends % (v * size) == 0) return p.D <= 64 * v ? v : 0;
+  return 0;
+}
+
+template <typename T, typename C, bool BACK>
+int launch_pieces(const HeadNorm &p, int values, const void *x, const void *w, const void *table, const void *grad, void *out, double *parts, int blocks) {
+  int lanes = 1;
+  while (lanes * values < p.D) lanes *= 2;
+  const bool each = BACK && parts && p.weight_heads > 1;
+  const bool neighbours = !p.interleaved && p.pairs % values == 0;
+  const dim3 grid((unsigned)blocks, each ? (unsigned)ceil_div(p.heads, 64 / lanes) : 1u);
+  auto run = [&](auto v) {
+    head_norm_pieces_kernel<T, C, v, BACK><<<grid, dim3(256), 0, runtime().stream>>>(p, lanes, neighbours, (const T *)x, (const T *)w, (const C *)table,
+                                                                                     (const T *)grad, (T *)out, parts);
+  };
+  if (values == 1) run(std::integral_constant<int, 1>{});
+  if (values == 2) run(std::integral_constant<int, 2>{});
+  if constexpr (sizeof(T) <= 4)
+    if (values == 4) run(std::integral_constant<int, 4>{});
+  if constexpr (sizeof(T) == 2)
+    if (values == 8) run(std::integral_constant<int, 8>{});
+  MG_HIP(hipGetLastError());
+  return MG_OK;
+}
+
+// Blocks whose wavefronts go through all tokens: up to eight a compute unit.
+int blocks_of(const HeadNorm &p) {
+  return (int)std::min<long long>(ceil_div(p.rows / p.heads, 4), 8 * runtime().props.multiProcessorCount);
 }
 
 template <typename T, typename C>
 int forward(const HeadNorm &p, const void *x, const void *w, const void *table, void *y) {
   ScopedTiming timed(TAG_HEAD_NORM);
+  const int values = values_of(p, sizeof(T), (uintptr_t)x | (uintptr_t)y | (uintptr_t)w);
+  if (values) return launch_pieces<T, C, false>(p, values, x, w, table, nullptr, y, nullptr, blocks_of(p));
   head_norm_kernel<T, C><<<dim3((unsigned)ceil_div(p.rows, 4)), dim3(256), 0, runtime().stream>>>(p, (const T *)x, (const T *)w, (const C *)table, (T *)y);
   MG_HIP(hipGetLastError());
   return MG_OK;
@@ -170,6 +356,22 @@ int forward(const HeadNorm &p, const void *x, const void *w, const void *table, 
 template <typename T, typename C>
 int backward(const HeadNorm &p, const void *x, const void *w, const void *table, const void *grad, void *dx, void *dw) {
   hipStream_t s = runtime().stream;
+  const int values = values_of(p, sizeof(T), (uintptr_t)x | (uintptr_t)dx | (uintptr_t)w | (uintptr_t)grad);
+  if (values) {  // both gradients in one pass
+    // with weights for each head a block keeps to some heads: fewer along the tokens
+    const int blocks = dw && p.weight_heads > 1 ? std::max(1, blocks_of(p) / 8) : blocks_of(p);
+    void *sums = nullptr;
+    if (dw) {
+      const int rc = workspace((size_t)blocks * p.weight_heads * p.D * sizeof(double), &sums);
+      if (rc) return rc;
+    }
+    ScopedTiming timed(TAG_HEAD_NORM_BWD);
+    const int rc = launch_pieces<T, C, true>(p, values, x, w, table, grad, dx, (double *)sums, blocks);
+    if (rc || !dw) return rc;
+    head_norm_dw_join_kernel<T><<<dim3((unsigned)ceil_div(p.weight_heads * p.D, 4)), dim3(256), 0, s>>>(p.weight_heads * p.D, blocks, (const double *)sums, (T *)dw);
+    MG_HIP(hipGetLastError());
+    return MG_OK;
+  }
   if (dx) {
     ScopedTiming timed(TAG_HEAD_NORM_BWD);
     head_norm_dx_kernel<T, C><<<dim3((unsigned)ceil_div(p.rows, 4)), dim3(256), 0, s>>>(p, (const T *)x, (const T *)w, (const C *)table, (const T *)grad, (T *)dx);
@@ -185,7 +387,7 @@ int backward(const HeadNorm &p, const void *x, const void *w, const void *table,
     ScopedTiming timed(TAG_HEAD_NORM_BWD);
     head_norm_dw_kernel<T, C><<<dim3((unsigned)heads, (unsigned)parts), dim3(256), 0, s>>>(p, per_block, (const T *)x, (const C *)table, (const T *)grad, (double *)sums);
     MG_HIP(hipGetLastError());
-    head_norm_dw_join_kernel<T><<<dim3((unsigned)ceil_div(heads * p.D, 256)), dim3(256), 0, s>>>(heads * p.D, (int)parts, (const double *)sums, (T *)dw);
+    head_norm_dw_join_kernel<T><<<dim3((unsigned)ceil_div(heads * p.D, 4)), dim3(256), 0, s>>>(heads * p.D, (int)parts, (const double *)sums, (T *)dw);
     MG_HIP(hipGetLastError());
   }
   return MG_OK;
