@@ -174,45 +174,86 @@ __device__ __forceinline__ void wave_sees() {
 // a token, whose cos and sin stay in registers, while it goes through the heads.  A value's partner in its pair lies in another lane or
 // not, wherever sections and layout put it: rows are handed over through LDS, a wavefront's own.
 // Bound by memory; float16, 16384 tokens of 32 heads of 128 values (134 MB a tensor): see launch_pieces.
-template <typename T, typename C, int V>
+// NEAR: a lane's values turn with neighbours, a whole piece of them (halves of a row that are whole pieces); it then needs one place.
+template <typename T, typename C, int V, bool NEAR>
 struct Pieces {
   typedef T Held __attribute__((ext_vector_type(V)));
-  C cos[V], sin[V];  // sin with the sign that the partner's value takes
-  int partner[V];
-
-  // What each of the lane's values turns with.
-  __device__ __forceinline__ void find(const HeadNorm &p, int d0) {
-#pragma unroll
-    for (int n = 0; n < V; ++n) {
-      const int d = d0 + n, pair = pair_of(p, d);
-      const bool first = p.interleaved ? d % 2 == 0 : d < p.pairs;
-      partner[n] = pair < 0 ? d : first ? d + apart(p) : d - apart(p);
-      cos[n] = 1, sin[n] = 0;
-    }
-  }
+  typedef C Wide __attribute__((ext_vector_type(V)));
+  Wide cos, sin;  // sin with the sign that the partner's value takes
+  int partner[NEAR ? 1 : V];
 
   static __device__ __forceinline__ int pair_of(const HeadNorm &p, int d) {
     return d >= 2 * p.pairs ? -1 : p.interleaved ? d / 2 : d < p.pairs ? d : d - p.pairs;
   }
 
+  // What each of the lane's values turns with.
+  __device__ __forceinline__ void find(const HeadNorm &p, int d0) {
+#pragma unroll
+    for (int n = 0; n < (NEAR ? 1 : V); ++n) {
+      const int d = d0 + n;
+      const bool first = p.interleaved ? d % 2 == 0 : d < p.pairs;
+      partner[n] = pair_of(p, d) < 0 ? d : first ? d + apart(p) : d - apart(p);
+    }
+#pragma unroll
+    for (int n = 0; n < V; ++n) cos[n] = 1, sin[n] = 0;
+  }
+
   __device__ __forceinline__ void turn_at(const HeadNorm &p, const C *table, long long token, int d0) {
+    if (NEAR && p.axes == 1) {  // a run of the table's row
+      const int pair = pair_of(p, d0);
+      if (pair < 0) return;
+      typedef C Both __attribute__((ext_vector_type(2)));
+      const int row = min(max(p.positions[token], 0), p.table_rows - 1);
+      const Both *at = reinterpret_cast<const Both *>(table) + ((long long)row * p.pairs + pair);
+      const C sign = partner[0] > d0 ? -1 : 1;
+#pragma unroll
+      for (int n = 0; n < V; ++n) {
+        const Both both = at[n];
+        cos[n] = both[0], sin[n] = both[1] * sign;
+      }
+      return;
+    }
 #pragma unroll
     for (int n = 0; n < V; ++n) {
       const int d = d0 + n, pair = pair_of(p, d);
       if (pair < 0) continue;
-      turn_of<C>(p, table, token, pair, cos[n], sin[n]);
-      if (partner[n] > d) sin[n] = -sin[n];
+      C c, s;
+      turn_of<C>(p, table, token, pair, c, s);
+      cos[n] = c, sin[n] = partner[NEAR ? 0 : n] > d0 + (NEAR ? 0 : n) ? -s : s;
     }
   }
 };
 
-template <typename T, typename C, int V, bool BACK>
-__global__ void __launch_bounds__(256) head_norm_pieces_kernel(HeadNorm p, int lanes, bool neighbours, const T *__restrict__ x, const T *__restrict__ w,
+// The sum over each run of `lanes` lanes, a power of two: sixteen are added by moves within a row of lanes, more through LDS.
+template <int CONTROL>
+__device__ __forceinline__ float moved(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CONTROL, 0xf, 0xf, true));
+}
+template <int CONTROL>
+__device__ __forceinline__ double moved(double v) {
+  typedef int Two __attribute__((ext_vector_type(2)));
+  Two q = __builtin_bit_cast(Two, v);
+  q[0] = __builtin_amdgcn_mov_dpp(q[0], CONTROL, 0xf, 0xf, true), q[1] = __builtin_amdgcn_mov_dpp(q[1], CONTROL, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, q);
+}
+template <typename C>
+__device__ __forceinline__ C sum_of_lanes(C v, int lanes) {
+  if (lanes > 1) v += moved<0xb1>(v);   // lanes 1 0 3 2 of four
+  if (lanes > 2) v += moved<0x4e>(v);   // 2 3 0 1
+  if (lanes > 4) v += moved<0x141>(v);  // eight from behind
+  if (lanes > 8) v += moved<0x140>(v);  // sixteen from behind
+  if (lanes > 16) v += __shfl_xor(v, 16);
+  if (lanes > 32) v += __shfl_xor(v, 32);
+  return v;
+}
+
+template <typename T, typename C, int V, bool BACK, bool NEAR>
+__global__ void __launch_bounds__(256) head_norm_pieces_kernel(HeadNorm p, int lanes, const T *__restrict__ x, const T *__restrict__ w,
                                                                const C *__restrict__ table, const T *__restrict__ grad, T *__restrict__ out,
                                                                double *__restrict__ parts) {
-  typedef Pieces<T, C, V> P;
+  typedef Pieces<T, C, V, NEAR> P;
   typedef typename P::Held Held;
-  typedef C Wide __attribute__((ext_vector_type(V)));
+  typedef typename P::Wide Wide;
   __shared__ __attribute__((aligned(64))) char space[4 * 64 * V * sizeof(double)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (lanes - 1), g = lane / lanes, groups = 64 / lanes;
   const int d0 = l * V;
@@ -252,7 +293,7 @@ __global__ void __launch_bounds__(256) head_norm_pieces_kernel(HeadNorm p, int l
       for (int n = 0; n < V; ++n) squares += value[n] * value[n];
       C r = 1;
       if (p.norm) {
-        for (int m = lanes >> 1; m; m >>= 1) squares += __shfl_xor(squares, m);
+        squares = sum_of_lanes(squares, lanes);
         r = 1 / sqrt(squares / p.D + (C)p.eps);
       }
       Wide z = BACK ? other : value * r * weight;
@@ -261,14 +302,13 @@ __global__ void __launch_bounds__(256) head_norm_pieces_kernel(HeadNorm p, int l
         *reinterpret_cast<Wide *>(row + l * V) = z;
         wave_sees();
         Wide there;
-        if (neighbours) {  // partners of neighbours are neighbours, from a whole piece on
+        if constexpr (NEAR) {
           there = *reinterpret_cast<const Wide *>(row + piece.partner[0]);
         } else {
 #pragma unroll
           for (int n = 0; n < V; ++n) there[n] = row[piece.partner[n]];
         }
-#pragma unroll
-        for (int n = 0; n < V; ++n) z[n] = z[n] * piece.cos[n] + there[n] * (BACK ? -piece.sin[n] : piece.sin[n]);
+        z = z * piece.cos + there * (BACK ? -piece.sin : piece.sin);
       }
       if constexpr (BACK) {
         if (take && parts) {
@@ -280,8 +320,7 @@ __global__ void __launch_bounds__(256) head_norm_pieces_kernel(HeadNorm p, int l
         if (p.norm) {
 #pragma unroll
           for (int n = 0; n < V; ++n) mean += z[n] * value[n];
-          for (int m = lanes >> 1; m; m >>= 1) mean += __shfl_xor(mean, m);
-          mean *= r * r / p.D;
+          mean = sum_of_lanes(mean, lanes) * (r * r / p.D);
         }
         z = (z - value * mean) * r;
       }
@@ -322,11 +361,11 @@ int launch_pieces(const HeadNorm &p, int values, const void *x, const void *w, c
   int lanes = 1;
   while (lanes * values < p.D) lanes *= 2;
   const bool each = BACK && parts && p.weight_heads > 1;
-  const bool neighbours = !p.interleaved && p.pairs % values == 0;
+  const bool near = !p.interleaved && p.pairs % values == 0;
   const dim3 grid((unsigned)blocks, each ? (unsigned)ceil_div(p.heads, 64 / lanes) : 1u);
   auto run = [&](auto v) {
-    head_norm_pieces_kernel<T, C, v, BACK><<<grid, dim3(256), 0, runtime().stream>>>(p, lanes, neighbours, (const T *)x, (const T *)w, (const C *)table,
-                                                                                     (const T *)grad, (T *)out, parts);
+    auto kernel = near ? head_norm_pieces_kernel<T, C, v, BACK, true> : head_norm_pieces_kernel<T, C, v, BACK, false>;
+    kernel<<<grid, dim3(256), 0, runtime().stream>>>(p, lanes, (const T *)x, (const T *)w, (const C *)table, (const T *)grad, (T *)out, parts);
   };
   if (values == 1) run(std::integral_constant<int, 1>{});
   if (values == 2) run(std::integral_constant<int, 2>{});
