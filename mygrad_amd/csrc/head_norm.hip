@@ -251,9 +251,13 @@ template <typename T, typename C, int V, bool BACK, bool NEAR>
 __global__ void __launch_bounds__(256) head_norm_pieces_kernel(HeadNorm p, int lanes, const T *__restrict__ x, const T *__restrict__ w,
                                                                const C *__restrict__ table, const T *__restrict__ grad, T *__restrict__ out,
                                                                double *__restrict__ parts) {
+  // Rounds whose values are on their way together: forward and in float16 two take 55 us where one takes 61; backward (108 against 98) and in
+  // float32 (2 x 7128 tokens of 16 heads of 72: 37 against 31) the registers for two cost more waves than they gain.
+  constexpr int kAtOnce = !BACK && sizeof(T) == 2 ? 2 : 1;
   typedef Pieces<T, C, V, NEAR> P;
   typedef typename P::Held Held;
   typedef typename P::Wide Wide;
+  typedef std::conditional_t<(kAtOnce > 1), Held, Wide> Kept;
   __shared__ __attribute__((aligned(64))) char space[4 * 64 * V * sizeof(double)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (lanes - 1), g = lane / lanes, groups = 64 / lanes;
   const int d0 = l * V;
@@ -265,7 +269,9 @@ __global__ void __launch_bounds__(256) head_norm_pieces_kernel(HeadNorm p, int l
   // wanted, a group keeps to one head.
   const bool keep = BACK && parts && each;
   const int side = keep ? 1 : min(groups, p.heads), tokens_at_once = keep ? 1 : groups / side;
-  const int first_head = keep ? blockIdx.y * groups + g : g % side, rounds = keep ? 1 : (p.heads + side - 1) / side;
+  const int all_rounds = (p.heads + side - 1) / side, share = (all_rounds + gridDim.y - 1) / gridDim.y;  // blockIdx.y takes a share of the heads
+  const int first_head = keep ? blockIdx.y * groups + g : g % side + blockIdx.y * share * side;
+  const int rounds = keep ? 1 : min(share, all_rounds - (int)blockIdx.y * share);
   const bool mine = in && (keep || g / side < tokens_at_once);
   const long long tokens = p.rows / p.heads, stride = (long long)gridDim.x * 4 * tokens_at_once;
 
@@ -278,53 +284,63 @@ __global__ void __launch_bounds__(256) head_norm_pieces_kernel(HeadNorm p, int l
     const long long token = first + (keep ? 0 : g / side);
     const bool here = mine && token < tokens;
     if (here && p.pairs) piece.turn_at(p, table, token, d0);
-    for (int round = 0; round < rounds; ++round) {
-      const int head = first_head + round * side;
-      const bool take = here && head < p.heads;
-      const long long at = (token * p.heads + head) * p.D + d0;
-      Wide value{}, other{};
-      if (take) {
-        value = __builtin_convertvector(*reinterpret_cast<const Held *>(x + at), Wide);
-        if (BACK) other = __builtin_convertvector(*reinterpret_cast<const Held *>(grad + at), Wide);
-        if (each) weight = __builtin_convertvector(*reinterpret_cast<const Held *>(w + (long long)head * p.D + d0), Wide);
-      }
-      C squares = 0;
+    for (int round = 0; round < rounds; round += kAtOnce) {
+      Kept values[kAtOnce] = {}, others[BACK ? kAtOnce : 1] = {};
 #pragma unroll
-      for (int n = 0; n < V; ++n) squares += value[n] * value[n];
-      C r = 1;
-      if (p.norm) {
-        squares = sum_of_lanes(squares, lanes);
-        r = 1 / sqrt(squares / p.D + (C)p.eps);
-      }
-      Wide z = BACK ? other : value * r * weight;
-      if (p.pairs) {
-        wave_sees();
-        *reinterpret_cast<Wide *>(row + l * V) = z;
-        wave_sees();
-        Wide there;
-        if constexpr (NEAR) {
-          there = *reinterpret_cast<const Wide *>(row + piece.partner[0]);
-        } else {
-#pragma unroll
-          for (int n = 0; n < V; ++n) there[n] = row[piece.partner[n]];
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int head = first_head + (round + u) * side;
+        if (here && head < p.heads && round + u < rounds) {
+          const long long at = (token * p.heads + head) * p.D + d0;
+          values[u] = __builtin_convertvector(*reinterpret_cast<const Held *>(x + at), Kept);
+          if constexpr (BACK) others[u] = __builtin_convertvector(*reinterpret_cast<const Held *>(grad + at), Kept);
+          if (each && kAtOnce == 1) weight = __builtin_convertvector(*reinterpret_cast<const Held *>(w + (long long)head * p.D + d0), Wide);
         }
-        z = z * piece.cos + there * (BACK ? -piece.sin : piece.sin);
       }
-      if constexpr (BACK) {
-        if (take && parts) {
 #pragma unroll
-          for (int n = 0; n < V; ++n) sums[n] += (double)(z[n] * value[n] * r);
-        }
-        z *= weight;
-        C mean = 0;
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int head = first_head + (round + u) * side;
+        const bool take = here && head < p.heads && round + u < rounds;
+        const long long at = (token * p.heads + head) * p.D + d0;
+        const Wide value = __builtin_convertvector(values[u], Wide), other = __builtin_convertvector(others[BACK ? u : 0], Wide);
+        if (each && kAtOnce > 1 && take) weight = __builtin_convertvector(*reinterpret_cast<const Held *>(w + (long long)head * p.D + d0), Wide);
+        C squares = 0;
+#pragma unroll
+        for (int n = 0; n < V; ++n) squares += value[n] * value[n];
+        C r = 1;
         if (p.norm) {
-#pragma unroll
-          for (int n = 0; n < V; ++n) mean += z[n] * value[n];
-          mean = sum_of_lanes(mean, lanes) * (r * r / p.D);
+          squares = sum_of_lanes(squares, lanes);
+          r = 1 / sqrt(squares / p.D + (C)p.eps);
         }
-        z = (z - value * mean) * r;
+        Wide z = BACK ? other : value * r * weight;
+        if (p.pairs) {
+          wave_sees();
+          *reinterpret_cast<Wide *>(row + l * V) = z;
+          wave_sees();
+          Wide there;
+          if constexpr (NEAR) {
+            there = *reinterpret_cast<const Wide *>(row + piece.partner[0]);
+          } else {
+#pragma unroll
+            for (int n = 0; n < V; ++n) there[n] = row[piece.partner[n]];
+          }
+          z = z * piece.cos + there * (BACK ? -piece.sin : piece.sin);
+        }
+        if constexpr (BACK) {
+          if (take && parts) {
+#pragma unroll
+            for (int n = 0; n < V; ++n) sums[n] += (double)(z[n] * value[n] * r);
+          }
+          z *= weight;
+          C mean = 0;
+          if (p.norm) {
+#pragma unroll
+            for (int n = 0; n < V; ++n) mean += z[n] * value[n];
+            mean = sum_of_lanes(mean, lanes) * (r * r / p.D);
+          }
+          z = (z - value * mean) * r;
+        }
+        if (take && out) *reinterpret_cast<Held *>(out + at) = __builtin_convertvector(z, Held);
       }
-      if (take && out) *reinterpret_cast<Held *>(out + at) = __builtin_convertvector(z, Held);
     }
   }
   if constexpr (BACK) {
@@ -344,7 +360,7 @@ __global__ void __launch_bounds__(256) head_norm_pieces_kernel(HeadNorm p, int l
     for (int n = threadIdx.x; n < held; n += 256) {
       const int head = each ? blockIdx.y * groups + n / (lanes * V) : 0, d = n % (lanes * V);
       if (d >= p.D || head >= p.weight_heads) continue;
-      parts[((long long)blockIdx.x * p.weight_heads + head) * p.D + d] = all[n] + all[64 * V + n] + all[128 * V + n] + all[192 * V + n];
+      parts[((each ? (long long)blockIdx.x : (long long)blockIdx.y * gridDim.x + blockIdx.x) * p.weight_heads + head) * p.D + d] = all[n] + all[64 * V + n] + all[128 * V + n] + all[192 * V + n];
     }
   }
 }
@@ -356,16 +372,35 @@ int values_of(const HeadNorm &p, int size, uintptr_t ends) {
   return 0;
 }
 
+struct Grid {
+  int lanes, blocks, shares;  // blocks along the tokens and along the heads
+};
+
+// Blocks whose wavefronts go through all tokens, up to eight a compute unit; where tokens are few, several share a token's heads.  With weights
+// for each head and their gradient a group keeps to a head, and blocks along the tokens are the fewer.
+Grid grid_of(const HeadNorm &p, int values, bool keep) {
+  Grid grid{1, 1, 1};
+  while (grid.lanes * values < p.D) grid.lanes *= 2;
+  const int cus = runtime().props.multiProcessorCount, groups = 64 / grid.lanes;
+  const long long blocks = ceil_div(p.rows / p.heads, 4);
+  grid.blocks = (int)std::min<long long>(blocks, 8 * cus);
+  if (keep) {
+    grid.shares = (int)ceil_div(p.heads, groups);
+    grid.blocks = std::max(1, std::min(grid.blocks, (int)ceil_div(8 * cus, grid.shares)));
+  } else if (groups < p.heads) {
+    grid.shares = (int)std::min<long long>(ceil_div(p.heads, groups), ceil_div(8 * cus, blocks));
+  }
+  return grid;
+}
+
 template <typename T, typename C, bool BACK>
-int launch_pieces(const HeadNorm &p, int values, const void *x, const void *w, const void *table, const void *grad, void *out, double *parts, int blocks) {
-  int lanes = 1;
-  while (lanes * values < p.D) lanes *= 2;
-  const bool each = BACK && parts && p.weight_heads > 1;
+int launch_pieces(const HeadNorm &p, const Grid &shape, int values, const void *x, const void *w, const void *table, const void *grad, void *out,
+                  double *parts) {
   const bool near = !p.interleaved && p.pairs % values == 0;
-  const dim3 grid((unsigned)blocks, each ? (unsigned)ceil_div(p.heads, 64 / lanes) : 1u);
+  const dim3 grid((unsigned)shape.blocks, (unsigned)shape.shares);
   auto run = [&](auto v) {
     auto kernel = near ? head_norm_pieces_kernel<T, C, v, BACK, true> : head_norm_pieces_kernel<T, C, v, BACK, false>;
-    kernel<<<grid, dim3(256), 0, runtime().stream>>>(p, lanes, (const T *)x, (const T *)w, (const C *)table, (const T *)grad, (T *)out, parts);
+    kernel<<<grid, dim3(256), 0, runtime().stream>>>(p, shape.lanes, (const T *)x, (const T *)w, (const C *)table, (const T *)grad, (T *)out, parts);
   };
   if (values == 1) run(std::integral_constant<int, 1>{});
   if (values == 2) run(std::integral_constant<int, 2>{});
@@ -377,16 +412,11 @@ int launch_pieces(const HeadNorm &p, int values, const void *x, const void *w, c
   return MG_OK;
 }
 
-// Blocks whose wavefronts go through all tokens: up to eight a compute unit.
-int blocks_of(const HeadNorm &p) {
-  return (int)std::min<long long>(ceil_div(p.rows / p.heads, 4), 8 * runtime().props.multiProcessorCount);
-}
-
 template <typename T, typename C>
 int forward(const HeadNorm &p, const void *x, const void *w, const void *table, void *y) {
   ScopedTiming timed(TAG_HEAD_NORM);
   const int values = values_of(p, sizeof(T), (uintptr_t)x | (uintptr_t)y | (uintptr_t)w);
-  if (values) return launch_pieces<T, C, false>(p, values, x, w, table, nullptr, y, nullptr, blocks_of(p));
+  if (values) return launch_pieces<T, C, false>(p, grid_of(p, values, false), values, x, w, table, nullptr, y, nullptr);
   head_norm_kernel<T, C><<<dim3((unsigned)ceil_div(p.rows, 4)), dim3(256), 0, runtime().stream>>>(p, (const T *)x, (const T *)w, (const C *)table, (T *)y);
   MG_HIP(hipGetLastError());
   return MG_OK;
@@ -397,17 +427,18 @@ int backward(const HeadNorm &p, const void *x, const void *w, const void *table,
   hipStream_t s = runtime().stream;
   const int values = values_of(p, sizeof(T), (uintptr_t)x | (uintptr_t)dx | (uintptr_t)w | (uintptr_t)grad);
   if (values) {  // both gradients in one pass
-    // with weights for each head a block keeps to some heads: fewer along the tokens
-    const int blocks = dw && p.weight_heads > 1 ? std::max(1, blocks_of(p) / 8) : blocks_of(p);
+    const bool keep = dw && p.weight_heads > 1;
+    const Grid grid = grid_of(p, values, keep);
+    const int parts = keep ? grid.blocks : grid.blocks * grid.shares;
     void *sums = nullptr;
     if (dw) {
-      const int rc = workspace((size_t)blocks * p.weight_heads * p.D * sizeof(double), &sums);
+      const int rc = workspace((size_t)parts * p.weight_heads * p.D * sizeof(double), &sums);
       if (rc) return rc;
     }
     ScopedTiming timed(TAG_HEAD_NORM_BWD);
-    const int rc = launch_pieces<T, C, true>(p, values, x, w, table, grad, dx, (double *)sums, blocks);
+    const int rc = launch_pieces<T, C, true>(p, grid, values, x, w, table, grad, dx, (double *)sums);
     if (rc || !dw) return rc;
-    head_norm_dw_join_kernel<T><<<dim3((unsigned)ceil_div(p.weight_heads * p.D, 4)), dim3(256), 0, s>>>(p.weight_heads * p.D, blocks, (const double *)sums, (T *)dw);
+    head_norm_dw_join_kernel<T><<<dim3((unsigned)ceil_div(p.weight_heads * p.D, 4)), dim3(256), 0, s>>>(p.weight_heads * p.D, parts, (const double *)sums, (T *)dw);
     MG_HIP(hipGetLastError());
     return MG_OK;
   }
