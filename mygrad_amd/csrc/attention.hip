@@ -19,146 +19,60 @@ namespace mg {
 
 namespace {
 
-// A block takes `each` rows of one head, one after the other for each of its wavefronts; with `redo`, only where its entry there is set.
-struct Rows {
-  int each;
-  const int *redo;
-};
-
 struct Mine {
   long long first;  // batch item * heads + head
-  int row, end;
+  int row;
+  bool in;
 };
 
-__device__ __forceinline__ Mine rows_of_wave(const Rows &r, int tokens) {
-  const int tiles = (tokens + r.each - 1) / r.each;
+// A block takes four rows of one head: which of them is this wavefront's.
+__device__ __forceinline__ Mine row_of_wave(int tokens) {
+  const int tiles = (tokens + 3) / 4;
   Mine m;
   m.first = blockIdx.x / tiles;
-  m.row = (int)(blockIdx.x - m.first * tiles) * r.each;
-  m.end = min(m.row + r.each, tokens);
-  m.row += threadIdx.x >> 6;
-  if (r.redo && !r.redo[blockIdx.x]) m.end = 0;
+  m.row = (int)(blockIdx.x - m.first * tiles) * 4 + (threadIdx.x >> 6);
+  m.in = m.row < tokens;
   return m;
 }
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) attention_rows_kernel(Attention p, Rows each, const T *__restrict__ q, const T *__restrict__ k,
-                                                             const T *__restrict__ v, T *__restrict__ out, _Float16 *__restrict__ rest,
-                                                             C *__restrict__ lse) {
+__global__ void __launch_bounds__(256) attention_rows_kernel(Attention p, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                                                             T *__restrict__ out, _Float16 *__restrict__ rest, C *__restrict__ lse) {
   __shared__ C rows[4][kMaxDim];
-  const Mine r = rows_of_wave(each, p.TQ);
-  for (int i = r.row; i < r.end; i += 4)
-    attend_row<T, C>(p, (int)(r.first / p.HQ), (int)(r.first % p.HQ), i, rows[threadIdx.x >> 6], q, k, v, out, rest, lse);
+  const Mine r = row_of_wave(p.TQ);
+  if (r.in) attend_row<T, C>(p, (int)(r.first / p.HQ), (int)(r.first % p.HQ), r.row, rows[threadIdx.x >> 6], q, k, v, out, rest, lse);
 }
 
 // D_i, a wavefront per row.
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) attention_delta_kernel(Attention p, Rows each, const T *__restrict__ out, const _Float16 *__restrict__ rest,
+__global__ void __launch_bounds__(256) attention_delta_kernel(Attention p, const T *__restrict__ out, const _Float16 *__restrict__ rest,
                                                               const T *__restrict__ grad, C *__restrict__ delta) {
   const int lane = threadIdx.x & 63;
-  const Mine r = rows_of_wave(each, p.TQ);
-  const int b = (int)(r.first / p.HQ), h = (int)(r.first % p.HQ);
-  for (int i = r.row; i < r.end; i += 4) {
-    const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
-    C sum = 0;
-    for (int d = lane; d < p.D; d += 64) sum += ((C)out[at + d] + (rest ? (C)rest[at + d] / (C)kRest : C(0))) * (C)grad[at + d];
-    sum = wave_sum(sum);
-    if (lane == 0) delta[r.first * p.TQ + i] = sum;
-  }
+  const Mine r = row_of_wave(p.TQ);
+  if (!r.in) return;
+  const long long at = ((r.first / p.HQ * p.TQ + r.row) * p.HQ + r.first % p.HQ) * p.D;
+  C sum = 0;
+  for (int d = lane; d < p.D; d += 64) sum += ((C)out[at + d] + (rest ? (C)rest[at + d] / (C)kRest : C(0))) * (C)grad[at + d];
+  sum = wave_sum(sum);
+  if (lane == 0) delta[r.first * p.TQ + r.row] = sum;
 }
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) attention_dq_rows_kernel(Attention p, Rows each, const T *__restrict__ q, const T *__restrict__ k,
-                                                                const T *__restrict__ v, const T *__restrict__ grad,
-                                                                const C *__restrict__ lse, const C *__restrict__ delta,
+__global__ void __launch_bounds__(256) attention_dq_rows_kernel(Attention p, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                                                                const T *__restrict__ grad, const C *__restrict__ lse, const C *__restrict__ delta,
                                                                 T *__restrict__ dq) {
-  __shared__ C rows[2][4][kMaxDim];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Mine r = rows_of_wave(each, p.TQ);
-  const int b = (int)(r.first / p.HQ), h = (int)(r.first % p.HQ);
-  const long long step = (long long)p.HK * p.D, head = ((long long)b * p.TK * p.HK + h / p.group) * p.D;
-  const C slope = p.slopes ? (C)p.slopes[h] : C(0);
-  for (int i = r.row; i < r.end; i += 4) {
-    const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
-    wave_sees();
-    for (int d = lane; d < p.D; d += 64) rows[0][wave][d] = (C)q[at + d], rows[1][wave][d] = (C)grad[at + d];
-    wave_sees();
-    const Span span = span_of(p, b, i);
-    const C norm = lse[r.first * p.TQ + i], mean = delta[r.first * p.TQ + i];
-    C sum[kParts] = {};
-    for (int j0 = span.lo; j0 < span.hi; j0 += 64) {
-      const int j = j0 + lane, count = min(64, span.hi - j0);
-      C ds = 0;
-      if (lane < count) {
-        C through;
-        const C s = score<C>(p, dot_row<T, C>(rows[0][wave], k + head + j * step, p.D), slope, span.place - j, through);
-        ds = exp2(s * (C)kLog2e64 - norm) * (dot_row<T, C>(rows[1][wave], v + head + j * step, p.D) - mean) * through;
-      }
-      for (int n = 0; n < count; ++n) {
-        const C weight = __shfl(ds, n);
-        const T *row = k + head + (j0 + n) * step;
-#pragma unroll
-        for (int c = 0; c < kParts; ++c)
-          if (lane + 64 * c < p.D) sum[c] += weight * (C)row[lane + 64 * c];
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < kParts; ++c)
-      if (lane + 64 * c < p.D) dq[at + lane + 64 * c] = (T)sum[c];
-  }
+  __shared__ C rows[4][2 * kMaxDim];
+  const Mine r = row_of_wave(p.TQ);
+  if (r.in) dq_row<T, C>(p, (int)(r.first / p.HQ), (int)(r.first % p.HQ), r.row, rows[threadIdx.x >> 6], q, k, v, grad, lse, delta, dq);
 }
 
-// A wavefront per key and key head; queries over the lanes, the heads that share the key one after the other.
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) attention_dkv_rows_kernel(Attention p, Rows each, const T *__restrict__ q, const T *__restrict__ k,
-                                                                 const T *__restrict__ v, const T *__restrict__ grad,
-                                                                 const C *__restrict__ lse, const C *__restrict__ delta,
+__global__ void __launch_bounds__(256) attention_dkv_rows_kernel(Attention p, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                                                                 const T *__restrict__ grad, const C *__restrict__ lse, const C *__restrict__ delta,
                                                                  T *__restrict__ dk, T *__restrict__ dv) {
-  __shared__ C rows[2][4][kMaxDim];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Mine r = rows_of_wave(each, p.TK);
-  const int b = (int)(r.first / p.HK), hk = (int)(r.first % p.HK);
-  const long long step = (long long)p.HQ * p.D;
-  for (int j = r.row; j < r.end; j += 4) {
-    const long long at = (((long long)b * p.TK + j) * p.HK + hk) * p.D;
-    wave_sees();
-    for (int d = lane; d < p.D; d += 64) rows[0][wave][d] = (C)k[at + d], rows[1][wave][d] = (C)v[at + d];
-    wave_sees();
-    C sum_k[kParts] = {}, sum_v[kParts] = {};
-    for (int h = hk * p.group; h < (hk + 1) * p.group; ++h) {
-      const long long head = ((long long)b * p.TQ * p.HQ + h) * p.D, stats = ((long long)b * p.HQ + h) * p.TQ;
-      const C slope = p.slopes ? (C)p.slopes[h] : C(0);
-      for (int i0 = 0; i0 < p.TQ; i0 += 64) {
-        const int i = i0 + lane;
-        C weight = 0, ds = 0;
-        bool sees = false;
-        if (i < p.TQ) {
-          const Span span = span_of(p, b, i);
-          sees = j >= span.lo && j < span.hi;
-          if (sees) {
-            C through;
-            const C s = score<C>(p, dot_row<T, C>(rows[0][wave], q + head + i * step, p.D), slope, span.place - j, through);
-            weight = exp2(s * (C)kLog2e64 - lse[stats + i]);
-            ds = weight * (dot_row<T, C>(rows[1][wave], grad + head + i * step, p.D) - delta[stats + i]) * through;
-          }
-        }
-        for (unsigned long long left = __ballot(sees); left; left &= left - 1) {
-          const int n = __ffsll(left) - 1;
-          const C of_v = __shfl(weight, n), of_k = __shfl(ds, n);
-          const T *qr = q + head + (i0 + n) * step, *gr = grad + head + (i0 + n) * step;
-#pragma unroll
-          for (int c = 0; c < kParts; ++c)
-            if (lane + 64 * c < p.D) {
-              sum_k[c] += of_k * (C)qr[lane + 64 * c];
-              sum_v[c] += of_v * (C)gr[lane + 64 * c];
-            }
-        }
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < kParts; ++c)
-      if (lane + 64 * c < p.D) dk[at + lane + 64 * c] = (T)sum_k[c], dv[at + lane + 64 * c] = (T)sum_v[c];
-  }
+  __shared__ C rows[4][2 * kMaxDim];
+  const Mine r = row_of_wave(p.TK);
+  if (r.in) dkv_row<T, C>(p, (int)(r.first / p.HK), (int)(r.first % p.HK), r.row, rows[threadIdx.x >> 6], q, k, v, grad, lse, delta, dk, dv);
 }
 
 // Copies the t new tokens of each batch item to the places in the cache that end at its length, 16 bytes (or an element) a thread.
@@ -176,35 +90,11 @@ __global__ void __launch_bounds__(256) cache_write_kernel(long long pieces, int 
   }
 }
 
-constexpr Rows kFour{4, nullptr};
-
 template <typename T, typename C>
-int forward_rows(const Attention &p, Rows each, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
-  const long long blocks = (long long)p.B * p.HQ * ceil_div(p.TQ, each.each);
-  ScopedTiming timed(each.redo ? TAG_GATED : TAG_ATTENTION);
-  attention_rows_kernel<T, C><<<dim3((unsigned)blocks), dim3(256), 0, runtime().stream>>>(p, each, (const T *)q, (const T *)k, (const T *)v, (T *)out,
-                                                                                          (_Float16 *)rest, (C *)lse);
-  MG_HIP(hipGetLastError());
-  return MG_OK;
-}
-
-template <typename T, typename C>
-int dq_rows(const Attention &p, Rows each, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad, void *dq) {
-  const unsigned blocks = (unsigned)((long long)p.B * p.HQ * ceil_div(p.TQ, each.each));
-  ScopedTiming timed(each.redo ? TAG_GATED : TAG_ATTENTION_DQ);
-  attention_dq_rows_kernel<T, C><<<dim3(blocks), dim3(256), 0, runtime().stream>>>(p, each, (const T *)q, (const T *)k, (const T *)v, (const T *)grad,
-                                                                                   (const C *)lse, (const C *)delta, (T *)dq);
-  MG_HIP(hipGetLastError());
-  return MG_OK;
-}
-
-template <typename T, typename C>
-int dkv_rows(const Attention &p, Rows each, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad, void *dk,
-             void *dv) {
-  const unsigned blocks = (unsigned)((long long)p.B * p.HK * ceil_div(p.TK, each.each));
-  ScopedTiming timed(each.redo ? TAG_GATED : TAG_ATTENTION_DKV);
-  attention_dkv_rows_kernel<T, C><<<dim3(blocks), dim3(256), 0, runtime().stream>>>(p, each, (const T *)q, (const T *)k, (const T *)v, (const T *)grad,
-                                                                                    (const C *)lse, (const C *)delta, (T *)dk, (T *)dv);
+int forward_rows(const Attention &p, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
+  ScopedTiming timed(TAG_ATTENTION);
+  attention_rows_kernel<T, C><<<dim3((unsigned)((long long)p.B * p.HQ * ceil_div(p.TQ, 4))), dim3(256), 0, runtime().stream>>>(
+      p, (const T *)q, (const T *)k, (const T *)v, (T *)out, (_Float16 *)rest, (C *)lse);
   MG_HIP(hipGetLastError());
   return MG_OK;
 }
@@ -212,18 +102,29 @@ int dkv_rows(const Attention &p, Rows each, const void *q, const void *k, const 
 template <typename T, typename C>
 int backward_rows(const Attention &p, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
                   const void *grad, void *dq, void *dk, void *dv) {
+  hipStream_t s = runtime().stream;
+  const dim3 rows((unsigned)((long long)p.B * p.HQ * ceil_div(p.TQ, 4))), keys((unsigned)((long long)p.B * p.HK * ceil_div(p.TK, 4)));
   void *delta = nullptr;
-  int rc = workspace((size_t)p.B * p.HQ * p.TQ * sizeof(C), &delta);
+  const int rc = workspace((size_t)p.B * p.HQ * p.TQ * sizeof(C), &delta);
   if (rc) return rc;
   {
     ScopedTiming timed(TAG_ATTENTION_DELTA);
-    attention_delta_kernel<T, C><<<dim3((unsigned)((long long)p.B * p.HQ * ceil_div(p.TQ, 4))), dim3(256), 0, runtime().stream>>>(
-        p, kFour, (const T *)out, (const _Float16 *)rest, (const T *)grad, (C *)delta);
+    attention_delta_kernel<T, C><<<rows, dim3(256), 0, s>>>(p, (const T *)out, (const _Float16 *)rest, (const T *)grad, (C *)delta);
+    MG_HIP(hipGetLastError());
   }
-  MG_HIP(hipGetLastError());
-  if (dq) rc = dq_rows<T, C>(p, kFour, q, k, v, lse, delta, grad, dq);
-  if (!rc && dk && p.TK) rc = dkv_rows<T, C>(p, kFour, q, k, v, lse, delta, grad, dk, dv);
-  return rc;
+  if (dq) {
+    ScopedTiming timed(TAG_ATTENTION_DQ);
+    attention_dq_rows_kernel<T, C><<<rows, dim3(256), 0, s>>>(p, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (const C *)lse,
+                                                              (const C *)delta, (T *)dq);
+    MG_HIP(hipGetLastError());
+  }
+  if (dk && p.TK) {
+    ScopedTiming timed(TAG_ATTENTION_DKV);
+    attention_dkv_rows_kernel<T, C><<<keys, dim3(256), 0, s>>>(p, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (const C *)lse,
+                                                               (const C *)delta, (T *)dk, (T *)dv);
+    MG_HIP(hipGetLastError());
+  }
+  return MG_OK;
 }
 
 int check_attention(const mg_attention_desc *d, Attention *p, const char *who) {
@@ -253,25 +154,6 @@ int check_attention(const mg_attention_desc *d, Attention *p, const char *who) {
 
 }  // namespace
 
-int forward_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse,
-                       const int *redo, int rows) {
-  const Rows each{rows, redo};
-  return dtype == MG_F16 ? forward_rows<_Float16, float>(p, each, q, k, v, out, rest, lse) : forward_rows<float, float>(p, each, q, k, v, out, rest, lse);
-}
-
-int dq_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad,
-                  void *dq, const int *redo, int rows) {
-  const Rows each{rows, redo};
-  return dtype == MG_F16 ? dq_rows<_Float16, float>(p, each, q, k, v, lse, delta, grad, dq) : dq_rows<float, float>(p, each, q, k, v, lse, delta, grad, dq);
-}
-
-int dkv_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad,
-                   void *dk, void *dv, const int *redo, int rows) {
-  const Rows each{rows, redo};
-  return dtype == MG_F16 ? dkv_rows<_Float16, float>(p, each, q, k, v, lse, delta, grad, dk, dv)
-                         : dkv_rows<float, float>(p, each, q, k, v, lse, delta, grad, dk, dv);
-}
-
 }  // namespace mg
 
 using namespace mg;
@@ -288,12 +170,12 @@ int mg_attention_fwd(const mg_attention_desc *desc, const void *q, const void *k
   if (p.B == 0 || p.TQ == 0) return MG_OK;
   if (!q || !out || (p.TK && (!k || !v))) return fail(MG_ERR_BAD_ARG, "null pointer in mg_attention_fwd");
   if (desc->dtype != MG_F16) rest = nullptr;
-  if (desc->dtype == MG_F64) return forward_rows<double, double>(p, kFour, q, k, v, out, rest, lse);
+  if (desc->dtype == MG_F64) return forward_rows<double, double>(p, q, k, v, out, rest, lse);
   const uintptr_t ends = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)rest;
   if (p.TK && tiles_take(p, desc->dtype == MG_F16 ? 2 : 4, ends))
     return p.TQ <= kFewQueries ? forward_few(p, desc->dtype, q, k, v, out, rest, lse) : forward_tiles(p, desc->dtype, q, k, v, out, rest, lse);
-  if (desc->dtype == MG_F32) return forward_rows<float, float>(p, kFour, q, k, v, out, rest, lse);
-  return forward_rows<_Float16, float>(p, kFour, q, k, v, out, rest, lse);
+  if (desc->dtype == MG_F32) return forward_rows<float, float>(p, q, k, v, out, rest, lse);
+  return forward_rows<_Float16, float>(p, q, k, v, out, rest, lse);
 }
 
 int mg_attention_bwd(const mg_attention_desc *desc, const void *q, const void *k, const void *v, const void *out, const void *rest,

@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split 
   if (lse && threadIdx.x == 0) lse[((long long)b * p.HQ + hq) * p.TQ + i] = total == 0 ? INFINITY : top + __builtin_log2f(total) - kLift;
   bad = __any(bad);
   if (lane == 0) odd[wave] = bad;
-  __syncthreads();
+  all_landed();  // what is stored, too: it may be written again
   if (wave == 0 && (odd[0] | odd[1] | odd[2] | odd[3])) attend_row<T, float>(p, b, hq, i, mine, q, k, v, out, rest, lse);
 }
 

@@ -95,4 +95,86 @@ __device__ __forceinline__ void attend_row(const Attention &p, int b, int h, int
   if (lse && lane == 0) lse[((long long)b * p.HQ + h) * p.TQ + i] = none ? (C)INFINITY : top * (C)kLog2e64 + log2(total);  // no weight on any key
 }
 
+// Row i of dq; `mine`: LDS of this wavefront for twice D values.
+template <typename T, typename C>
+__device__ __forceinline__ void dq_row(const Attention &p, int b, int h, int i, C *mine, const T *__restrict__ q, const T *__restrict__ k,
+                                       const T *__restrict__ v, const T *__restrict__ grad, const C *__restrict__ lse, const C *__restrict__ delta,
+                                       T *__restrict__ dq) {
+  const int lane = threadIdx.x & 63;
+  const long long step = (long long)p.HK * p.D, head = ((long long)b * p.TK * p.HK + h / p.group) * p.D;
+  const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D, stat = ((long long)b * p.HQ + h) * p.TQ + i;
+  const C slope = p.slopes ? (C)p.slopes[h] : C(0);
+  wave_sees();
+  for (int d = lane; d < p.D; d += 64) mine[d] = (C)q[at + d], mine[p.D + d] = (C)grad[at + d];
+  wave_sees();
+  const Span span = span_of(p, b, i);
+  const C norm = lse[stat], mean = delta[stat];
+  C sum[kParts] = {};
+  for (int j0 = span.lo; j0 < span.hi; j0 += 64) {
+    const int j = j0 + lane, count = min(64, span.hi - j0);
+    C ds = 0;
+    if (lane < count) {
+      C through;
+      const C s = score<C>(p, dot_row<T, C>(mine, k + head + j * step, p.D), slope, span.place - j, through);
+      ds = exp2(s * (C)kLog2e64 - norm) * (dot_row<T, C>(mine + p.D, v + head + j * step, p.D) - mean) * through;
+    }
+    for (int n = 0; n < count; ++n) {
+      const C weight = __shfl(ds, n);
+      const T *row = k + head + (j0 + n) * step;
+#pragma unroll
+      for (int c = 0; c < kParts; ++c)
+        if (lane + 64 * c < p.D) sum[c] += weight * (C)row[lane + 64 * c];
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kParts; ++c)
+    if (lane + 64 * c < p.D) dq[at + lane + 64 * c] = (T)sum[c];
+}
+
+// Row j of dk and dv: queries over the lanes, the heads that share the key one after the other; `mine` as for dq_row.
+template <typename T, typename C>
+__device__ __forceinline__ void dkv_row(const Attention &p, int b, int hk, int j, C *mine, const T *__restrict__ q, const T *__restrict__ k,
+                                        const T *__restrict__ v, const T *__restrict__ grad, const C *__restrict__ lse, const C *__restrict__ delta,
+                                        T *__restrict__ dk, T *__restrict__ dv) {
+  const int lane = threadIdx.x & 63;
+  const long long at = (((long long)b * p.TK + j) * p.HK + hk) * p.D, step = (long long)p.HQ * p.D;
+  wave_sees();
+  for (int d = lane; d < p.D; d += 64) mine[d] = (C)k[at + d], mine[p.D + d] = (C)v[at + d];
+  wave_sees();
+  C sum_k[kParts] = {}, sum_v[kParts] = {};
+  for (int h = hk * p.group; h < (hk + 1) * p.group; ++h) {
+    const long long head = ((long long)b * p.TQ * p.HQ + h) * p.D, stats = ((long long)b * p.HQ + h) * p.TQ;
+    const C slope = p.slopes ? (C)p.slopes[h] : C(0);
+    for (int i0 = 0; i0 < p.TQ; i0 += 64) {
+      const int i = i0 + lane;
+      C weight = 0, ds = 0;
+      bool sees = false;
+      if (i < p.TQ) {
+        const Span span = span_of(p, b, i);
+        sees = j >= span.lo && j < span.hi;
+        if (sees) {
+          C through;
+          const C s = score<C>(p, dot_row<T, C>(mine, q + head + i * step, p.D), slope, span.place - j, through);
+          weight = exp2(s * (C)kLog2e64 - lse[stats + i]);
+          ds = weight * (dot_row<T, C>(mine + p.D, grad + head + i * step, p.D) - delta[stats + i]) * through;
+        }
+      }
+      for (unsigned long long left = __ballot(sees); left; left &= left - 1) {
+        const int n = __ffsll(left) - 1;
+        const C of_v = __shfl(weight, n), of_k = __shfl(ds, n);
+        const T *qr = q + head + (i0 + n) * step, *gr = grad + head + (i0 + n) * step;
+#pragma unroll
+        for (int c = 0; c < kParts; ++c)
+          if (lane + 64 * c < p.D) {
+            sum_k[c] += of_k * (C)qr[lane + 64 * c];
+            sum_v[c] += of_v * (C)gr[lane + 64 * c];
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kParts; ++c)
+    if (lane + 64 * c < p.D) dk[at + lane + 64 * c] = (T)sum_k[c], dv[at + lane + 64 * c] = (T)sum_v[c];
+}
+
 }  // namespace mg

@@ -12,20 +12,10 @@ constexpr float kRest = 2048.0f;
 bool tiles_take(const Attention &p, int size, uintptr_t ends);
 int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse);
 
-// Computes the rows of those blocks again, `rows` at a time, whose entry of redo[(batch item, head, block)] is not zero: the tiles'
-// products multiply what a row does not see by weights of zero, which an infinity or a NaN there turns into NaN.  Few blocks
-// as a rule have anything to do.
-int forward_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse,
-                       const int *redo, int rows);
-
 // Worth it up to so many queries: beyond, a wavefront's 32 columns are filled by the queries of one head.
 constexpr int kFewQueries = 32;
 int forward_few(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse);
 int backward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
                    const void *grad, void *dq, void *dk, void *dv);
-int dq_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad,
-                  void *dq, const int *redo, int rows);
-int dkv_rows_again(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *lse, const void *delta, const void *grad,
-                   void *dk, void *dv, const int *redo, int rows);
 
 }  // namespace mg

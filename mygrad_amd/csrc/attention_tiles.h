@@ -181,7 +181,7 @@ struct TileOf {
   }
 };
 
-// Every load of this wave into LDS has landed and its LDS reads are done; then all waves of the block are here.
+// Every load of this wave into LDS has landed, its LDS accesses and its stores are done; then all waves of the block are here.
 __device__ __forceinline__ void all_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // What the two halves of the wavefront hold for a column: lane c's value and lane 32 + c's, in both lanes.

@@ -1,8 +1,11 @@
 // Attention of float16 and float32 on the matrix cores: tiles of queries against tiles of keys, one pass with the running maximum
 // and sum of the softmax, nothing of the scores in memory.
+//
+// The tiles' products multiply what a row does not see by weights of zero, which an infinity or a NaN there turns into NaN.  So a block
+// whose results hold one that is no number computes its rows once more, a row at a time (attention_row.h); few have to.
 #include "attention_tiles.h"
 
-#include "attention_rows.h"
+#include "attention_row.h"
 
 #include <algorithm>
 
@@ -15,7 +18,7 @@ constexpr int kBlockRows = 128;  // queries of a block: 32 for each of its four 
 template <typename T, int DP, int KEYS, bool BENT>
 __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T *__restrict__ k,
                                                                  const T *__restrict__ v, T *__restrict__ out, _Float16 *__restrict__ rest,
-                                                                 float *__restrict__ lse, int *__restrict__ redo) {
+                                                                 float *__restrict__ lse) {
   typedef TileOf<T, DP, KEYS> Tile;
   typedef typename Fragment<T>::V V;
   constexpr int kSteps = DP / 16, kParts = DP / 32;
@@ -98,8 +101,10 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
   }
   odd = __any(in && odd);
   if (lane == 0) bad[wave] = odd;
-  __syncthreads();
-  if (threadIdx.x == 0) redo[((long long)b * p.HQ + hq) * deal.tiles + at.tile] = bad[0] | bad[1] | bad[2] | bad[3];
+  all_landed();  // what is stored, too: other wavefronts may write it again
+  if (bad[0] | bad[1] | bad[2] | bad[3])
+    for (int again = at.tile * kBlockRows + wave; again < min(p.TQ, (at.tile + 1) * kBlockRows); again += 4)
+      attend_row<T, float>(p, b, hq, again, (float *)tiles + wave * kMaxDim, q, k, v, out, rest, lse);
 }
 
 // Four neighbouring values of a result, registers r .. r + 3 times `by`; true if one is no number.
@@ -238,8 +243,8 @@ __device__ __forceinline__ void gradients_of(const Attention &p, f32x16 &s, f32x
 // dq^T = K^T dS^T: as the forward pass, with the queries' rows of grad beside those of q.
 template <typename T, int DP, int KEYS, bool BENT>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
-                                                              const T *__restrict__ v, const T *__restrict__ grad, T *__restrict__ dq,
-                                                              int *__restrict__ redo) {
+                                                              const T *__restrict__ v, const T *__restrict__ grad, const float *__restrict__ lse,
+                                                              T *__restrict__ dq) {
   typedef TileOf<T, DP, KEYS> Tile;
   typedef typename Fragment<T>::V V;
   constexpr int kSteps = DP / 16, kParts = DP / 32, kSubs = KEYS / 32;
@@ -335,8 +340,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
   }
   odd = __any(odd);
   if (lane == 0) bad[wave] = odd;
-  __syncthreads();
-  if (threadIdx.x == 0) redo[((long long)b * p.HQ + hq) * deal.tiles + at.tile] = bad[0] | bad[1] | bad[2] | bad[3];
+  all_landed();  // what is stored, too: other wavefronts may write it again
+  if (bad[0] | bad[1] | bad[2] | bad[3])
+    for (int again = at.tile * kBlockRows + wave; again < min(p.TQ, (at.tile + 1) * kBlockRows); again += 4)
+      dq_row<T, float>(p, b, hq, again, (float *)tiles + wave * 2 * kMaxDim, q, k, v, grad, lse, stats.delta, dq);
 }
 
 // dv^T = grad^T P and dk^T = q^T dS: a block keeps 128 keys, 32 for each wavefront in its lanes' columns, and goes through the chunks of queries
@@ -346,8 +353,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
 // and with v's 32 as well the scores would not fit.
 template <typename T, int DP, int ROWS, bool VALUES, bool BENT>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
-                                                               const T *__restrict__ v, const T *__restrict__ grad, T *__restrict__ dk,
-                                                               T *__restrict__ dv, int *__restrict__ redo, int cuts, float *__restrict__ parts) {
+                                                               const T *__restrict__ v, const T *__restrict__ grad, const float *__restrict__ lse,
+                                                               T *__restrict__ dk, T *__restrict__ dv, int cuts, float *__restrict__ parts) {
   typedef TileOf<T, DP, ROWS> Tile;
   typedef typename Fragment<T>::V V;
   constexpr int kSteps = DP / 16, kParts = DP / 32, kSubs = ROWS / 32;
@@ -523,15 +530,20 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
   if (cuts > 1) return;
   odd = __any(odd);
   if (lane == 0) bad[wave] = odd;
-  __syncthreads();
-  if (threadIdx.x == 0) redo[((long long)b * p.HK + hk) * deal.tiles + tile] = bad[0] | bad[1] | bad[2] | bad[3];
+  all_landed();  // what is stored, too: other wavefronts may write it again
+  if (bad[0] | bad[1] | bad[2] | bad[3])
+    for (int again = block0 + wave; again < min(p.TK, block0 + kBlockRows); again += 4)
+      dkv_row<T, float>(p, b, hk, again, (float *)tiles + wave * 2 * kMaxDim, q, k, v, grad, lse, stats.delta, dk, dv);
 }
 
 // Adds the cuts' sums in their order, four values a thread; a block takes 128 keys of one head, as the tiles do.
 template <typename T>
-__global__ void __launch_bounds__(256) attention_dkv_join_kernel(Attention p, int tiles, int cuts, const float *__restrict__ parts, T *__restrict__ dk,
-                                                                 T *__restrict__ dv, int *__restrict__ redo) {
+__global__ void __launch_bounds__(256) attention_dkv_join_kernel(Attention p, Stats stats, int tiles, int cuts, const float *__restrict__ parts,
+                                                                 const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                                                                 const T *__restrict__ grad, const float *__restrict__ lse, T *__restrict__ dk,
+                                                                 T *__restrict__ dv) {
   __shared__ int bad[4];
+  __shared__ float mine[4][2 * kMaxDim];
   const int pair = blockIdx.x / tiles, tile = blockIdx.x % tiles, b = pair / p.HK, hk = pair % p.HK, of_row = p.D / 4;
   const long long all = (long long)p.B * p.TK * p.HK * p.D;
   bool odd = false;
@@ -548,8 +560,11 @@ __global__ void __launch_bounds__(256) attention_dkv_join_kernel(Attention p, in
   }
   odd = __any(odd);
   if ((threadIdx.x & 63) == 0) bad[threadIdx.x >> 6] = odd;
-  __syncthreads();
-  if (threadIdx.x == 0) redo[blockIdx.x] = bad[0] | bad[1] | bad[2] | bad[3];
+  all_landed();
+  const int wave = threadIdx.x >> 6;
+  if (bad[0] | bad[1] | bad[2] | bad[3])
+    for (int again = tile * kBlockRows + wave; again < min(p.TK, (tile + 1) * kBlockRows); again += 4)
+      dkv_row<T, float>(p, b, hk, again, mine[wave], q, k, v, grad, lse, stats.delta, dk, dv);
 }
 
 // How many cuts the blocks of attention_dkv_kernel are made in.  All blocks of an unmasked problem take as long, those of a causal one up to twice
@@ -563,16 +578,14 @@ int cuts_of(const Attention &p, int blocks, int size) {
 }
 
 template <typename T, int ROWS>
-int backward_of(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
+int backward_of(const Attention &p, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
                 const void *grad, void *dq, void *dk, void *dv) {
   Stats stats{};
   stats.rows = sizeof(T) == 2 && p.D > 96 ? 32 : ROWS, stats.chunks = (int)ceil_div(p.TQ, stats.rows);
-  const size_t rows = (size_t)p.B * p.TQ, all = rows * p.HQ;
-  const size_t blocks_q = (size_t)p.B * p.HQ * ceil_div(p.TQ, kBlockRows), blocks_k = (size_t)p.B * p.HK * ceil_div(p.TK, kBlockRows);
-  const size_t chunks = (size_t)p.B * stats.chunks, keys = (size_t)p.B * p.TK * p.HK * p.D;
-  const int cuts = dk ? cuts_of(p, (int)blocks_k, sizeof(T)) : 1;
+  const size_t rows = (size_t)p.B * p.TQ, all = rows * p.HQ, chunks = (size_t)p.B * stats.chunks, keys = (size_t)p.B * p.TK * p.HK * p.D;
+  const int key_tiles = (int)ceil_div(p.TK, kBlockRows), cuts = dk ? cuts_of(p, p.B * p.HK * key_tiles, sizeof(T)) : 1;
   void *space = nullptr;
-  int rc = workspace((cuts > 1 ? 8 * cuts * keys : 0) + sizeof(Reach) * chunks + 4 * (2 * all + 2 * rows + blocks_q + blocks_k), &space);
+  int rc = workspace((cuts > 1 ? 8 * cuts * keys : 0) + sizeof(Reach) * chunks + 4 * (2 * all + 2 * rows), &space);
   if (rc) return rc;
   float *partial = (float *)space;  // whole pieces of 16 bytes: dim is a multiple of 8
   stats.reach = (Reach *)(partial + (cuts > 1 ? 2 * cuts * keys : 0));
@@ -580,43 +593,40 @@ int backward_of(const Attention &p, int dtype, const void *q, const void *k, con
   stats.delta = stats.level + all;
   stats.lo = (int *)(stats.delta + all);
   stats.hi = stats.lo + rows;
-  int *redo_q = stats.hi + rows, *redo_k = redo_q + blocks_q;
+  hipStream_t s = runtime().stream;
+  const T *tq = (const T *)q, *tk = (const T *)k, *tv = (const T *)v, *tg = (const T *)grad;
+  const float *tl = (const float *)lse;
   {
     ScopedTiming timed(TAG_ATTENTION_DELTA);
-    attention_stats_kernel<T><<<dim3((unsigned)(p.B * p.HQ * stats.chunks)), dim3(256), 0, runtime().stream>>>(
-        p, stats, (const T *)out, (const _Float16 *)rest, (const float *)lse, (const T *)grad);
+    attention_stats_kernel<T><<<dim3((unsigned)(p.B * p.HQ * stats.chunks)), dim3(256), 0, s>>>(p, stats, (const T *)out, (const _Float16 *)rest, tl, tg);
     MG_HIP(hipGetLastError());
   }
   if (dq) {
-    {
-      ScopedTiming timed(TAG_ATTENTION_DQ);
-      const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
-      with_shape(p, [&](auto dim, auto bent) {
-        attention_dq_kernel<T, dim, ROWS, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, runtime().stream>>>(
-            p, deal, stats, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (T *)dq, redo_q);
-      });
-      MG_HIP(hipGetLastError());
-    }
-    rc = dq_rows_again(p, dtype, q, k, v, lse, stats.delta, grad, dq, redo_q, kBlockRows);
-    if (rc) return rc;
+    ScopedTiming timed(TAG_ATTENTION_DQ);
+    const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
+    with_shape(p, [&](auto dim, auto bent) {
+      attention_dq_kernel<T, dim, ROWS, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, s>>>(p, deal, stats, tq, tk, tv, tg, tl,
+                                                                                                                       (T *)dq);
+    });
+    MG_HIP(hipGetLastError());
   }
   if (!dk) return MG_OK;
   {
     ScopedTiming timed(TAG_ATTENTION_DKV);
-    const Deal deal{p.B * p.HK, cuts, (int)ceil_div(p.TK, kBlockRows)};
+    const Deal deal{p.B * p.HK, cuts, key_tiles};
     with_shape(p, [&](auto dim, auto bent) {
       constexpr bool wide = sizeof(T) == 2 && dim == 128;
-      attention_dkv_kernel<T, dim, wide ? 32 : ROWS, wide, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, runtime().stream>>>(
-          p, deal, stats, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (T *)dk, (T *)dv, redo_k, cuts, partial);
+      attention_dkv_kernel<T, dim, wide ? 32 : ROWS, wide, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, s>>>(
+          p, deal, stats, tq, tk, tv, tg, tl, (T *)dk, (T *)dv, cuts, partial);
     });
     MG_HIP(hipGetLastError());
-    if (cuts > 1) {
-      attention_dkv_join_kernel<T><<<dim3((unsigned)(deal.pairs * deal.tiles)), dim3(256), 0, runtime().stream>>>(p, deal.tiles, cuts, partial, (T *)dk,
-                                                                                                                (T *)dv, redo_k);
-      MG_HIP(hipGetLastError());
-    }
   }
-  return dkv_rows_again(p, dtype, q, k, v, lse, stats.delta, grad, dk, dv, redo_k, kBlockRows);
+  if (cuts == 1) return MG_OK;
+  ScopedTiming timed(TAG_ATTENTION_JOIN);
+  attention_dkv_join_kernel<T><<<dim3((unsigned)(p.B * p.HK * key_tiles)), dim3(256), 0, s>>>(p, stats, key_tiles, cuts, partial, tq, tk, tv, tg, tl, (T *)dk,
+                                                                                            (T *)dv);
+  MG_HIP(hipGetLastError());
+  return MG_OK;
 }
 
 }  // namespace
@@ -628,31 +638,25 @@ bool tiles_take(const Attention &p, int size, uintptr_t ends) {
 }
 
 int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
-  void *space = nullptr;
-  const int rc = workspace((size_t)p.B * p.HQ * ceil_div(p.TQ, kBlockRows) * sizeof(int), &space);
-  if (rc) return rc;
-  int *redo = (int *)space;
-  {
-    ScopedTiming timed(TAG_ATTENTION);
-    const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
-    const dim3 grid((unsigned)(deal.pairs * deal.heads * deal.tiles));
-    auto launch = [&](auto zero) {
-      using T = decltype(zero);
-      with_shape(p, [&](auto dim, auto bent) {
-        attention_tiles_kernel<T, dim, sizeof(T) == 2 ? 64 : 32, bent><<<grid, dim3(256), 0, runtime().stream>>>(
-            p, deal, (const T *)q, (const T *)k, (const T *)v, (T *)out, (_Float16 *)rest, (float *)lse, redo);
-      });
-    };
-    dtype == MG_F16 ? launch(_Float16(0)) : launch(0.0f);
-    MG_HIP(hipGetLastError());
-  }
-  return forward_rows_again(p, dtype, q, k, v, out, rest, lse, redo, kBlockRows);
+  ScopedTiming timed(TAG_ATTENTION);
+  const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
+  const dim3 grid((unsigned)(deal.pairs * deal.heads * deal.tiles));
+  auto launch = [&](auto zero) {
+    using T = decltype(zero);
+    with_shape(p, [&](auto dim, auto bent) {
+      attention_tiles_kernel<T, dim, sizeof(T) == 2 ? 64 : 32, bent><<<grid, dim3(256), 0, runtime().stream>>>(
+          p, deal, (const T *)q, (const T *)k, (const T *)v, (T *)out, (_Float16 *)rest, (float *)lse);
+    });
+  };
+  dtype == MG_F16 ? launch(_Float16(0)) : launch(0.0f);
+  MG_HIP(hipGetLastError());
+  return MG_OK;
 }
 
 int backward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
                    const void *grad, void *dq, void *dk, void *dv) {
-  return dtype == MG_F16 ? backward_of<_Float16, 64>(p, dtype, q, k, v, out, rest, lse, grad, dq, dk, dv)
-                         : backward_of<float, 32>(p, dtype, q, k, v, out, rest, lse, grad, dq, dk, dv);
+  return dtype == MG_F16 ? backward_of<_Float16, 64>(p, q, k, v, out, rest, lse, grad, dq, dk, dv)
+                         : backward_of<float, 32>(p, q, k, v, out, rest, lse, grad, dq, dk, dv);
 }
 
 }  // namespace mg

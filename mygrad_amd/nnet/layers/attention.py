@@ -65,7 +65,7 @@ class AttentionMask:
             self.shortest, self.longest = (int(f(self._lengths)) if self._lengths.size else 0 for f in (np.min, np.max))
         if documents is not None:
             self._starts, self._ends = _runs(np.atleast_2d(_integers(documents, "numbers of documents", (1, 2))))
-        self._bound = {}
+        self._bound, self._described = {}, {}
 
     @staticmethod
     def _counts(values, what):
@@ -95,8 +95,6 @@ class AttentionMask:
             self._check(batch, queries, keys)
             buffers = [None if arr is None else _uploaded(np.broadcast_to(arr, shape)) for arr, shape in (
                 (self._lengths, (batch,)), (self._prefix, (batch,)), (self._starts, (batch, keys)), (self._ends, (batch, keys)))]
-            if len(self._bound) >= 16:
-                self._bound.clear()
             held = self._bound[batch, queries, keys] = tuple(None if b is None else b.ptr for b in buffers), buffers
         return held[0]
 
@@ -154,15 +152,31 @@ def _slopes_on_device(slopes, heads):
 _UNMASKED = AttentionMask()
 
 
-def _describe(q_shape, k_shape, dtype, scale, cap, slopes, mask):
-    """The descriptor, and the buffers that have to outlive it."""
-    batch, queries, heads, dim = q_shape
-    keys, kv_heads = k_shape[1:3]
-    pointers = mask._bind(batch, queries, keys)
-    held = _slopes_on_device(slopes, heads)
-    return _hip.AttentionDesc(_hip.storage_code(dtype), mask.causal, batch, queries, keys, heads, kv_heads, dim, mask.window, scale, cap,
-                              0 if mask._lengths is None else max(mask.longest, 1),
-                              *pointers, None if held is None else held.ptr), held
+def _describe(q, k, v, scale, cap, slopes, mask):
+    """The descriptor, checked once for each mask and set of shapes and types (nothing writes to it), and the slopes' buffer, which has
+    to outlive it."""
+    if mask is None:
+        mask = _UNMASKED
+    elif not isinstance(mask, AttentionMask):
+        raise TypeError(f"`mask` must be an AttentionMask, got {type(mask).__name__}")
+    held = _slopes_on_device(slopes, q.shape[2]) if slopes is not None and q.ndim == 4 else None
+    key = q.shape, k.shape, v.shape, q.dtype, k.dtype, v.dtype, scale, cap, None if held is None else held.ptr
+    desc = mask._described.get(key)
+    if desc is None:
+        _check_operands(q, k, v)
+        scale, cap = _check_scores(scale, cap, q.shape[3])
+        (batch, queries, heads, dim), (keys, kv_heads) = q.shape, k.shape[1:3]
+        mask._check(batch, queries, keys)
+        if not q.size:
+            return None, held  # nothing to compute, nothing to upload
+        pointers = mask._bind(batch, queries, keys)
+        longest = 0 if mask._lengths is None else max(mask.longest, 1)
+        desc = _hip.AttentionDesc(_hip.storage_code(q.dtype), mask.causal, batch, queries, keys, heads, kv_heads, dim, mask.window, scale, cap, longest,
+                                  *pointers, key[-1])
+        if len(mask._described) >= 64:
+            mask._described.clear()
+        mask._described[key] = desc
+    return desc, held
 
 
 def _check_operands(q, k, v):
@@ -191,17 +205,11 @@ class Attention(Operation):
     def __call__(self, q, k, v, *, scale=None, cap=None, slopes=None, mask=None):
         self.variables = (q, k, v)
         qd, kd, vd = (_device.value_of(t) for t in (q, k, v))
-        _check_operands(qd, kd, vd)
-        scale, cap = _check_scores(scale, cap, qd.shape[3])
-        mask = _UNMASKED if mask is None else mask
-        if not isinstance(mask, AttentionMask):
-            raise TypeError(f"`mask` must be an AttentionMask, got {type(mask).__name__}")
-        mask._check(qd.shape[0], qd.shape[1], kd.shape[1])
         self._backed = None
-        if qd.size == 0:
-            return np.zeros(qd.shape, dtype=qd.dtype)
         self._mask = mask  # holds what the descriptor points to
-        self._desc, self._slopes = _describe(qd.shape, kd.shape, qd.dtype, scale, cap, slopes, mask)
+        self._desc, self._slopes = _describe(qd, kd, vd, scale, cap, slopes, mask)
+        if self._desc is None:
+            return np.zeros(qd.shape, dtype=qd.dtype)
         qb, kb, vb = (_device.to_device(a) for a in (qd, kd, vd))
         self._out = _device.DeviceBuffer(qd.nbytes)
         self._lse = self._rest = None
@@ -340,14 +348,11 @@ class KeyValueCache:
 
     def attend(self, q, *, mask, scale=None, cap=None, slopes=None):
         """:func:`attention` of ``q:(batch, queries, query heads, dim)`` over what the cache holds up to ``mask.lengths``; a constant."""
-        qd = self._operand(q, "q")
-        if qd.shape[2] == 0 or qd.shape[2] % self.shape[2]:
-            raise ValueError(f"the query heads must be a multiple of the cache's {self.shape[2]}, got {qd.shape[2]}")
-        scale, cap = _check_scores(scale, cap, qd.shape[3])
-        self._masked(mask)._check(self.shape[0], qd.shape[1], self.shape[1])
-        if qd.size == 0:
+        qd, mask = self._operand(q, "q"), self._masked(mask)
+        keys = self.keys
+        desc, held = _describe(qd, keys, keys, scale, cap, slopes, mask)
+        if desc is None:
             return Tensor(np.zeros(qd.shape, dtype=qd.dtype), constant=True, copy=False)
-        desc, held = _describe(qd.shape, self.shape, qd.dtype, scale, cap, slopes, mask)
         qb, out = _device.to_device(qd), _device.DeviceBuffer(qd.nbytes)
         _hip.check(_hip.lib().mg_attention_fwd(desc, qb.ptr, self._keys.ptr, self._values.ptr, out.ptr, None, None))
         return Tensor(_device.DeviceArray(out, qd.shape, qd.dtype), constant=True, copy=False)

@@ -77,7 +77,8 @@ class RotaryPositions:
             raise ValueError(f"positions must have shape (..., {axes}) for {axes} axes, got {arr.shape}")
         if arr.size and (arr.min() < 0 or arr.max() >= table.length):
             raise ValueError(f"positions must lie in [0, {table.length}), got {arr.min()} to {arr.max()}")
-        self.table, self._positions, self._bound = table, arr.astype(np.int32), {}
+        self.table, self._positions = table, arr.astype(np.int32)
+        self._bound, self._described = {}, {}
 
     def _check(self, lead):
         try:
@@ -91,11 +92,12 @@ class RotaryPositions:
         buf = self._bound.get(lead)
         if buf is None:
             self._check(lead)
-            if len(self._bound) >= 16:
-                self._bound.clear()
             spread = np.broadcast_to(self._positions, lead + self._positions.shape[-1:])
             buf = self._bound[lead] = _device.from_host(np.ascontiguousarray(spread)).buf
         return buf
+
+
+_described = {}  # descriptors of norms without positions
 
 
 class HeadNorm(Operation):
@@ -107,48 +109,60 @@ class HeadNorm(Operation):
         """``eps`` None: no norm."""
         self.variables = (x, weight)
         xd, wd = _device.value_of(x), _device.value_of(weight)
-        if xd.ndim < 2:
-            raise ValueError(f"`x` must have the axes (..., heads, dim), got shape {xd.shape}")
-        if xd.dtype not in _DTYPES:
-            raise TypeError(f"head_norm runs on the GPU in float16, float32 or float64, got {xd.dtype} (there is no CPU fallback)")
-        lead, (heads, dim) = xd.shape[:-2], xd.shape[-2:]
-        if not 1 <= dim <= 1024 or heads > 65535:
-            raise ValueError(f"heads have 1 to 1024 values and number at most 65535, got {xd.shape}")
-        self._weighted = wd.size > 0
-        if self._weighted:
-            if wd.shape not in ((dim,), (heads, dim)):
-                raise ValueError(f"`weight` must have shape ({dim},) or ({heads}, {dim}), got {wd.shape}")
-            if wd.dtype != xd.dtype:
-                raise TypeError(f"head_norm takes `weight` in the dtype of `x` ({xd.dtype}), got {wd.dtype}")
-        if eps is not None and not 0 <= eps < np.inf:
-            raise ValueError(f"`eps` must be a non-negative number, got {eps}")
-        if rotary is not None:
-            if not isinstance(rotary, RotaryPositions):
-                raise TypeError(f"`rotary` must come from RotaryTable.at, got {type(rotary).__name__}")
-            if 2 * rotary.table.pairs > dim:
-                raise ValueError(f"{rotary.table.pairs} pairs do not fit in {dim} values")
-            rotary._check(lead)
+        if rotary is not None and not isinstance(rotary, RotaryPositions):
+            raise TypeError(f"`rotary` must come from RotaryTable.at, got {type(rotary).__name__}")
         self._backed = None
-        if xd.size == 0:
-            return np.empty(xd.shape, dtype=xd.dtype)
         self._rotary = rotary  # holds what the descriptor points to
-        self._table = None
-        desc = _hip.HeadNormDesc(_hip.storage_code(xd.dtype), eps is not None, wd.size // dim if self._weighted else 0, 0, 1, 0, prod(lead),
-                                 heads, dim, 0, 0, 0.0 if eps is None else eps, None, None)
-        if rotary is not None:
-            table = rotary.table
-            self._positions = rotary._buffer(lead)
-            self._table = table._buffer("f8" if xd.dtype == np.float64 else "f4").ptr
-            desc.interleaved, desc.axes, desc.pairs, desc.table_rows = table.interleaved, len(table.sections), table.pairs, table.length
-            desc.positions, desc.axis_of = self._positions.ptr, table._buffer("axis_of").ptr
-        self._desc = desc
+        self._weighted = wd.size > 0
+        described = _described if rotary is None else rotary._described
+        key = xd.shape, xd.dtype, wd.shape, wd.dtype, eps
+        found = described.get(key)
+        if found is None:
+            found = self._describe(xd, wd, eps, rotary)
+            if xd.size == 0:
+                return np.empty(xd.shape, dtype=xd.dtype)
+            if len(described) >= 64:
+                described.clear()
+            described[key] = found
+        self._desc, self._table = found
         xb = _device.to_device(xd)
         wb = _device.to_device(wd) if self._weighted else None
         out = _device.DeviceBuffer(xd.nbytes)
-        _hip.check(_hip.lib().mg_head_norm_fwd(desc, xb.ptr, None if wb is None else wb.ptr, self._table, out.ptr))
+        _hip.check(_hip.lib().mg_head_norm_fwd(self._desc, xb.ptr, None if wb is None else wb.ptr, self._table, out.ptr))
         y = _device.download(out, xd.shape, xd.dtype)
         _device.attach(y, out)
         return y
+
+    def _describe(self, x, w, eps, rotary):
+        """The checked descriptor (nothing writes to it) and the table's address."""
+        if x.ndim < 2:
+            raise ValueError(f"`x` must have the axes (..., heads, dim), got shape {x.shape}")
+        if x.dtype not in _DTYPES:
+            raise TypeError(f"head_norm runs on the GPU in float16, float32 or float64, got {x.dtype} (there is no CPU fallback)")
+        lead, (heads, dim) = x.shape[:-2], x.shape[-2:]
+        if not 1 <= dim <= 1024 or heads > 65535:
+            raise ValueError(f"heads have 1 to 1024 values and number at most 65535, got {x.shape}")
+        if self._weighted:
+            if w.shape not in ((dim,), (heads, dim)):
+                raise ValueError(f"`weight` must have shape ({dim},) or ({heads}, {dim}), got {w.shape}")
+            if w.dtype != x.dtype:
+                raise TypeError(f"head_norm takes `weight` in the dtype of `x` ({x.dtype}), got {w.dtype}")
+        if eps is not None and not 0 <= eps < np.inf:
+            raise ValueError(f"`eps` must be a non-negative number, got {eps}")
+        table = None if rotary is None else rotary.table
+        if table is not None:
+            if 2 * table.pairs > dim:
+                raise ValueError(f"{table.pairs} pairs do not fit in {dim} values")
+            rotary._check(lead)
+        if x.size == 0:
+            return None
+        desc = _hip.HeadNormDesc(_hip.storage_code(x.dtype), eps is not None, w.size // dim if self._weighted else 0, 0, 1, 0, prod(lead),
+                                 heads, dim, 0, 0, 0.0 if eps is None else eps, None, None)
+        if table is None:
+            return desc, None
+        desc.interleaved, desc.axes, desc.pairs, desc.table_rows = table.interleaved, len(table.sections), table.pairs, table.length
+        desc.positions, desc.axis_of = rotary._buffer(lead).ptr, table._buffer("axis_of").ptr
+        return desc, table._buffer("f8" if x.dtype == np.float64 else "f4").ptr
 
     def _run_backward(self, grad, want):
         x, w = (_device.value_of(t) for t in self.variables)
