@@ -173,7 +173,7 @@ int mg_attention_fwd(const mg_attention_desc *desc, const void *q, const void *k
   if (desc->dtype == MG_F64) return forward_rows<double, double>(p, q, k, v, out, rest, lse);
   const uintptr_t ends = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)rest;
   if (p.TK && tiles_take(p, desc->dtype == MG_F16 ? 2 : 4, ends))
-    return p.TQ <= kFewQueries ? forward_few(p, desc->dtype, q, k, v, out, rest, lse) : forward_tiles(p, desc->dtype, q, k, v, out, rest, lse);
+    return few_take(p, desc->dtype == MG_F16 ? 2 : 4) ? forward_few(p, desc->dtype, q, k, v, out, rest, lse) : forward_tiles(p, desc->dtype, q, k, v, out, rest, lse);
   if (desc->dtype == MG_F32) return forward_rows<float, float>(p, q, k, v, out, rest, lse);
   return forward_rows<_Float16, float>(p, q, k, v, out, rest, lse);
 }

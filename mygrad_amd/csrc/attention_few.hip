@@ -1,9 +1,10 @@
-// Attention of few queries over many keys: the tokens of a step of generation over a cache.
+// Attention of few queries, or of few blocks of them: 32 queries x heads that share a key head make up the 32 columns of a block (a group of
+// eight heads and four tokens, say), its four wavefronts take every fourth tile of 32 keys, each with a running softmax (or sums of a
+// gradient) of its own over tiles that it brings into LDS for itself, without a barrier; they are joined through LDS at the end.  Where
+// that makes few blocks still, the keys are split among blocks, which are joined by a second launch.
 //
-// Bound by reading keys and values once: 32 queries x heads that share a key head make up the 32 columns of a wavefront (a group of eight
-// heads and four tokens, say), so the sixteen products of a tile of 32 keys wait for the tile's bytes even where most columns are empty.
-// Each wavefront keeps a running softmax of its own over tiles that it brings into LDS for itself, without a barrier; the four of a block
-// are joined through LDS, blocks that split one sequence's keys by a second launch.
+// With a step of generation over a cache this is bound by reading keys and values once: the sixteen products of a tile (128 values a head, float16)
+// wait for its bytes even where most columns are empty.
 #include "attention_tiles.h"
 
 #include "attention_row.h"
@@ -22,96 +23,170 @@ struct Split {
   int panels;   // of 32 columns
 };
 
-// Column n of a panel is query n / group, head n % group.
-template <typename T, int DP, int STAGES, bool BENT>
-__global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split split, const T *__restrict__ q, const T *__restrict__ k,
-                                                            const T *__restrict__ v, float *__restrict__ sums, float2 *__restrict__ ends) {
-  typedef TileOf<T, DP, 32> Tile;
-  typedef typename Fragment<T>::V V;
-  constexpr int kSteps = DP / 16, kPitch = DP + 4;
-  constexpr int kTiles = 4 * STAGES * 2 * Tile::kBytes, kJoin = 4 * 32 * kPitch * 4;
-  __shared__ __attribute__((aligned(1024))) char space[kTiles > kJoin ? kTiles : kJoin];
-  __shared__ float tops[4][32], totals[4][32];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
-  const int part = blockIdx.x % split.splits, rest = blockIdx.x / split.splits, panel = rest % split.panels, pair = rest / split.panels;
-  const int b = pair / p.HK, hk = pair % p.HK;
-  const int column = panel * 32 + c, i = column / p.group, hq = hk * p.group + column % p.group;
-  const bool in = column < split.columns;
-  const Span span = in ? span_of(p, b, i) : Span{0, 0, 0};
-  const Reach reach = reach_of(span, in);
+// What a lane has to know of its column, and the block of its keys.  Column n of a pair of batch item and key head is query n / group, head
+// n % group.
+struct Panel {
+  int part, pair, b, hk, first_column, columns;
+  int i, hq;
+  bool in;
+  Span span;
+  Reach reach;
+  int first, last;  // tiles of 32 keys from reach.lo on
+};
 
-  V rows[kSteps];
-  const T *row = q + (((long long)b * p.TQ + (in ? i : 0)) * p.HQ + hq) * p.D;
-#pragma unroll
-  for (int n = 0; n < kSteps; ++n) rows[n] = fragment_of(row, 16 * n + 8 * h, p.D, in);
-  const Scores how = scores_of(p, hq);
+__device__ __forceinline__ Panel panel_of(const Attention &p, const Split &split, int c) {
+  Panel at;
+  at.part = blockIdx.x % split.splits;
+  const int rest = blockIdx.x / split.splits, panel = split.panels - 1 - rest % split.panels;  // the last see most where the mask is causal
+  at.pair = rest / split.panels;
+  at.b = at.pair / p.HK, at.hk = at.pair % p.HK;
+  at.first_column = panel * 32, at.columns = min(32, split.columns - panel * 32);
+  const int column = at.first_column + c;
+  at.i = column / p.group, at.hq = at.hk * p.group + column % p.group;
+  at.in = c < at.columns;
+  at.span = at.in ? span_of(p, at.b, at.i) : Span{0, 0, 0};
+  at.reach = reach_of(at.span, at.in);
+  const int tiles = at.reach.hi > at.reach.lo ? (at.reach.hi - at.reach.lo + 31) / 32 : 0;
+  at.first = (int)((long long)tiles * at.part / split.splits), at.last = (int)((long long)tiles * (at.part + 1) / split.splits);
+  return at;
+}
 
-  const int tiles = reach.hi > reach.lo ? (reach.hi - reach.lo + 31) / 32 : 0;
-  const int first = (int)((long long)tiles * part / split.splits), last = (int)((long long)tiles * (part + 1) / split.splits);
+// A wavefront's every fourth tile: brings keys and values into its own part of LDS, one tile ahead where there is room (STAGES 2), and calls
+// f(the tile's place, its first key, whether all columns see all of it).
+template <typename T, typename Tile, int STAGES, typename F>
+__device__ __forceinline__ void each_tile(const Attention &p, const Panel &at, const void *k, const void *v, unsigned lds, int wave, F f) {
   const unsigned stride = (unsigned)(p.HK * p.D) * (unsigned)sizeof(T);
   const typename Tile::template Loader<64> load(stride, (unsigned)p.D * (unsigned)sizeof(T));
-  const long long head = (((long long)b * p.TK + reach.lo) * p.HK + hk) * p.D * (long long)sizeof(T);
+  const long long head = (((long long)at.b * p.TK + at.reach.lo) * p.HK + at.hk) * p.D * (long long)sizeof(T);
   const char *kb = (const char *)k + head, *vb = (const char *)v + head;
-  const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)space + (unsigned)wave * (STAGES * 2 * Tile::kBytes);
   auto stage = [&](int t, int side) {
     const long long from = (long long)t * 32 * stride;
     const unsigned to = lds + (unsigned)side * (2 * Tile::kBytes);
-    load(kb + from, stride, reach.hi - reach.lo - t * 32, to);
-    load(vb + from, stride, reach.hi - reach.lo - t * 32, to + Tile::kBytes);
+    load(kb + from, stride, at.reach.hi - at.reach.lo - t * 32, to);
+    load(vb + from, stride, at.reach.hi - at.reach.lo - t * 32, to + Tile::kBytes);
   };
-
-  Running<T, DP, 1, BENT> run;
-  run.begin();
-  const typename Tile::Place place = Tile::place(lane);
   int side = 0;
-  if (first + wave < last) stage(first + wave, 0);
-  for (int t = first + wave; t < last; t += 4) {
+  if (at.first + wave < at.last) stage(at.first + wave, 0);
+  for (int t = at.first + wave; t < at.last; t += 4) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const bool more = t + 4 < last;
+    const bool more = t + 4 < at.last;
     if (STAGES == 2 && more) stage(t + 4, side ^ 1);
-    const int key0 = reach.lo + t * 32;
-    const unsigned keys = lds + (unsigned)side * (2 * Tile::kBytes);
-    run.take(p, how, keys, keys + Tile::kBytes, rows, span, key0, key0 >= reach.all_lo && key0 + 32 <= reach.all_hi, place, h);
+    const int key0 = at.reach.lo + t * 32;
+    f(lds + (unsigned)side * (2 * Tile::kBytes), key0, key0 >= at.reach.all_lo && key0 + 32 <= at.reach.all_hi);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (STAGES == 2)
       side ^= 1;
     else if (more)
       stage(t + 4, 0);
   }
+}
 
-  // the block's four: sums at a common top, one after the other's space
+// The four wavefronts' sums, times `by`, side by side in LDS: wavefront, column, value.
+template <int DP>
+struct Joined {
+  static constexpr int kPitch = DP + 4, kBytes = 4 * 32 * kPitch * 4;
+
+  static __device__ __forceinline__ void put(float *space, const f32x16 (&sums)[DP / 32], float by, int wave, int c, int h) {
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *(f32x4 *)(space + (wave * 32 + c) * kPitch + 32 * n + row_of(r, h)) = f32x4{sums[n][r], sums[n][r + 1], sums[n][r + 2], sums[n][r + 3]} * by;
+  }
+
+  static __device__ __forceinline__ f32x4 sum(const float *space, int column, int d) {
+    f32x4 sum = *(const f32x4 *)(space + column * kPitch + d);
+#pragma unroll
+    for (int w = 1; w < 4; ++w) sum += *(const f32x4 *)(space + (w * 32 + column) * kPitch + d);
+    return sum;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ bool put_value(T *to, f32x4 value) {
+  typedef T V __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<V *>(to) = __builtin_convertvector(value, V);
+  bool odd = false;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) odd |= !(__builtin_fabsf(value[n]) < INFINITY);
+  return odd;
+}
+
+// With one split the result itself; else sums at the block's own top, and that with the total.
+template <typename T, int DP, int STAGES, bool BENT>
+__global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split split, const T *__restrict__ q, const T *__restrict__ k,
+                                                            const T *__restrict__ v, T *__restrict__ out, _Float16 *__restrict__ remains,
+                                                            float *__restrict__ lse, float *__restrict__ sums, float2 *__restrict__ ends) {
+  typedef TileOf<T, DP, 32> Tile;
+  typedef typename Fragment<T>::V V;
+  typedef Joined<DP> Join;
+  constexpr int kSteps = DP / 16, kTiles = 4 * STAGES * 2 * Tile::kBytes;
+  __shared__ __attribute__((aligned(1024))) char space[kTiles > Join::kBytes ? kTiles : Join::kBytes];
+  __shared__ float tops[4][32], totals[4][32];
+  __shared__ int bad[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+  const Panel at = panel_of(p, split, c);
+
+  V rows[kSteps];
+  const T *row = q + (((long long)at.b * p.TQ + (at.in ? at.i : 0)) * p.HQ + at.hq) * p.D;
+#pragma unroll
+  for (int n = 0; n < kSteps; ++n) rows[n] = fragment_of(row, 16 * n + 8 * h, p.D, at.in);
+  const Scores how = scores_of(p, at.hq);
+
+  Running<T, DP, 1, BENT> run;
+  run.begin();
+  const typename Tile::Place place = Tile::place(lane);
+  const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)space + (unsigned)wave * (STAGES * 2 * Tile::kBytes);
+  each_tile<T, Tile, STAGES>(p, at, k, v, lds, wave, [&](unsigned keys, int key0, bool whole) {
+    run.take(p, how, keys, keys + Tile::kBytes, rows, at.span, key0, whole, place, h);
+  });
+
   const float total = sum_halves(run.total);
   if (h == 0) tops[wave][c] = run.top, totals[wave][c] = total;
   __syncthreads();
   float top = -INFINITY;
 #pragma unroll
   for (int n = 0; n < 4; ++n) top = __builtin_fmaxf(top, tops[n][c]);
-  const float by = run.top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(run.top - top);
   float *join = (float *)space;
+  Join::put(join, run.sums, run.top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(run.top - top), wave, c, h);
+  float all = 0;
 #pragma unroll
-  for (int n = 0; n < DP / 32; ++n)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4)
-      *(f32x4 *)(join + (wave * 32 + c) * kPitch + 32 * n + row_of(r, h)) =
-          f32x4{run.sums[n][r], run.sums[n][r + 1], run.sums[n][r + 2], run.sums[n][r + 3]} * by;
+  for (int w = 0; w < 4; ++w)
+    if (tops[w][c] != -INFINITY) all += totals[w][c] * __builtin_amdgcn_exp2f(tops[w][c] - top);
   __syncthreads();
-  const int columns = min(32, split.columns - panel * 32);
-  const long long base = ((long long)pair * split.splits + part) * split.columns + panel * 32;
-  for (int n = threadIdx.x; n < columns * (DP / 4); n += 256) {
-    const int column = n / (DP / 4), d = n % (DP / 4) * 4;
+  const long long base = ((long long)at.pair * split.splits + at.part) * split.columns + at.first_column;
+  if (split.splits > 1) {
+    for (int n = threadIdx.x; n < at.columns * (DP / 4); n += 256) {
+      const int column = n / (DP / 4), d = n % (DP / 4) * 4;
+      if (d < p.D) *(f32x4 *)(sums + (base + column) * p.D + d) = Join::sum(join, column, d);
+    }
+    if ((int)threadIdx.x < at.columns) ends[base + c] = make_float2(top, all);
+    return;
+  }
+  if (wave == 0 && h == 0) {
+    tops[0][c] = all > 0 ? 1.0f / all : all == 0 ? 0.0f : NAN;
+    if (lse && at.in) lse[((long long)at.b * p.HQ + at.hq) * p.TQ + at.i] = all == 0 ? INFINITY : top + __builtin_log2f(all) - kLift;
+  }
+  __syncthreads();
+  bool odd = false;
+  for (int n = threadIdx.x; n < at.columns * (DP / 4); n += 256) {
+    const int column = n / (DP / 4), d = n % (DP / 4) * 4, all_columns = at.first_column + column;
     if (d >= p.D) continue;
-    f32x4 sum = *(const f32x4 *)(join + column * kPitch + d);
-#pragma unroll
-    for (int w = 1; w < 4; ++w) sum += *(const f32x4 *)(join + (w * 32 + column) * kPitch + d);
-    *(f32x4 *)(sums + (base + column) * p.D + d) = sum;
+    const f32x4 value = Join::sum(join, column, d) * tops[0][column];
+    const long long to = (((long long)at.b * p.TQ + all_columns / p.group) * p.HQ + at.hk * p.group + all_columns % p.group) * p.D + d;
+    odd |= put_value(out + to, value);
+    if constexpr (sizeof(T) == 2) {
+      if (remains)
+        *reinterpret_cast<f16x4 *>(remains + to) =
+            __builtin_convertvector((value - __builtin_convertvector(__builtin_convertvector(value, f16x4), f32x4)) * kRest, f16x4);
+    }
   }
-  if ((int)threadIdx.x < columns) {
-    float all = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-      if (tops[w][c] != -INFINITY) all += totals[w][c] * __builtin_amdgcn_exp2f(tops[w][c] - top);
-    ends[base + c] = make_float2(top, all);
-  }
+  odd = __any(odd);
+  if (lane == 0) bad[wave] = odd;
+  all_landed();  // what is stored, too: other wavefronts may write it again
+  if (bad[0] | bad[1] | bad[2] | bad[3])
+    for (int column = at.first_column + wave; column < at.first_column + at.columns; column += 4)
+      attend_row<T, float>(p, at.b, at.hk * p.group + column % p.group, column / p.group, (float *)space + wave * kMaxDim, q, k, v, out, remains, lse);
 }
 
 // A block per row of the result: the splits' sums at a common top, in their order.  A row that comes out as no number is computed once more, so
@@ -166,17 +241,107 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split 
   if (wave == 0 && (odd[0] | odd[1] | odd[2] | odd[3])) attend_row<T, float>(p, b, hq, i, mine, q, k, v, out, rest, lse);
 }
 
+// dq of a panel's columns; with one split the result itself.
+template <typename T, int DP, int STAGES, bool BENT>
+__global__ void __launch_bounds__(256) attention_few_dq_kernel(Attention p, Split split, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
+                                                               const T *__restrict__ v, const T *__restrict__ grad, const float *__restrict__ lse,
+                                                               T *__restrict__ dq, float *__restrict__ sums) {
+  typedef TileOf<T, DP, 32> Tile;
+  typedef typename Fragment<T>::V V;
+  typedef Joined<DP> Join;
+  constexpr int kSteps = DP / 16, kTiles = 4 * STAGES * 2 * Tile::kBytes;
+  __shared__ __attribute__((aligned(1024))) char space[kTiles > Join::kBytes ? kTiles : Join::kBytes];
+  __shared__ int bad[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+  const Panel at = panel_of(p, split, c);
+
+  V rows[kSteps], grads[kSteps];
+  const long long row = (((long long)at.b * p.TQ + (at.in ? at.i : 0)) * p.HQ + at.hq) * p.D;
+#pragma unroll
+  for (int n = 0; n < kSteps; ++n) {
+    rows[n] = fragment_of(q + row, 16 * n + 8 * h, p.D, at.in);
+    grads[n] = fragment_of(grad + row, 16 * n + 8 * h, p.D, at.in);
+  }
+  const long long stat = ((long long)at.b * p.HQ + at.hq) * p.TQ + (at.in ? at.i : 0);
+  const float level = at.in ? stats.level[stat] : INFINITY, delta = at.in ? stats.delta[stat] : 0.0f;
+  const Scores how = scores_of(p, at.hq);
+
+  Pulled<T, DP, 32, BENT> run;
+  run.begin();
+  const typename Tile::Place place = Tile::place(lane);
+  const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)space + (unsigned)wave * (STAGES * 2 * Tile::kBytes);
+  each_tile<T, Tile, STAGES>(p, at, k, v, lds, wave, [&](unsigned keys, int key0, bool whole) {
+    run.take(p, how, keys, 0, rows, grads, level, delta, at.span, key0, whole, place, h);
+  });
+
+  __syncthreads();
+  float *join = (float *)space;
+  Join::put(join, run.sums, run.by(p), wave, c, h);
+  __syncthreads();
+  const long long base = ((long long)at.pair * split.splits + at.part) * split.columns + at.first_column;
+  bool odd = false;
+  for (int n = threadIdx.x; n < at.columns * (DP / 4); n += 256) {
+    const int column = n / (DP / 4), d = n % (DP / 4) * 4, all_columns = at.first_column + column;
+    if (d >= p.D) continue;
+    const f32x4 value = Join::sum(join, column, d);
+    if (split.splits > 1)
+      *(f32x4 *)(sums + (base + column) * p.D + d) = value;
+    else
+      odd |= put_value(dq + (((long long)at.b * p.TQ + all_columns / p.group) * p.HQ + at.hk * p.group + all_columns % p.group) * p.D + d, value);
+  }
+  if (split.splits > 1) return;
+  odd = __any(odd);
+  if (lane == 0) bad[wave] = odd;
+  all_landed();  // what is stored, too: other wavefronts may write it again
+  if (bad[0] | bad[1] | bad[2] | bad[3])
+    for (int column = at.first_column + wave; column < at.first_column + at.columns; column += 4)
+      dq_row<T, float>(p, at.b, at.hk * p.group + column % p.group, column / p.group, (float *)space + wave * 2 * kMaxDim, q, k, v, grad, lse, stats.delta, dq);
+}
+
+// A wavefront per row of dq.
 template <typename T>
-int few_of(const Attention &p, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
-  constexpr int kStages = sizeof(T) == 2 ? 2 : 1;  // as many as four wavefronts have room for at 128 values a head
+__global__ void __launch_bounds__(256) attention_dq_join_kernel(Attention p, Split split, Stats stats, const float *__restrict__ sums,
+                                                                const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                                                                const T *__restrict__ grad, const float *__restrict__ lse, T *__restrict__ dq) {
+  __shared__ float mine[4][2 * kMaxDim];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long long at_row = (long long)blockIdx.x * 4 + wave;
+  if (at_row >= (long long)p.B * p.TQ * p.HQ) return;
+  const int hq = (int)(at_row % p.HQ), i = (int)(at_row / p.HQ % p.TQ), b = (int)(at_row / p.HQ / p.TQ);
+  const long long first = ((long long)b * p.HK + hq / p.group) * split.splits * split.columns + i * p.group + hq % p.group;
+  const float *from = sums + first * p.D + (lane < p.D ? lane : 0);
+  const long long step = (long long)split.columns * p.D;
+  const int second = lane + 64 < p.D ? 64 : 0;
+  float sum0 = 0, sum1 = 0;
+#pragma unroll 8
+  for (int n = 0; n < split.splits; ++n) sum0 += from[n * step], sum1 += from[n * step + second];
+  T *to = dq + at_row * p.D + lane;
+  if (lane < p.D) to[0] = (T)sum0;
+  if (second) to[64] = (T)sum1;
+  if (__any(!(__builtin_fabsf(sum0) < INFINITY) || !(__builtin_fabsf(sum1) < INFINITY))) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    dq_row<T, float>(p, b, hq, i, mine[wave], q, k, v, grad, lse, stats.delta, dq);
+  }
+}
+
+template <typename T>
+constexpr int stages_of() { return sizeof(T) == 2 ? 2 : 1; }  // as many as four wavefronts have room for at 128 values a head
+
+// A block for each 128 keys (a tile for each wavefront) while there are fewer than fill the device eight times over: a batch of ragged lengths evens
+// out over that many.  With more queries the products count and not the bytes, and twice over will do.
+Split split_of(const Attention &p) {
   Split split;
   split.columns = p.TQ * p.group;
   split.panels = (int)ceil_div(split.columns, 32);
-  // A block for each 128 keys (a tile for each wavefront) while there are fewer than fill the device eight times over: a batch of ragged lengths
-  // evens out over that many.
-  const int pairs = p.B * p.HK * split.panels, most = std::min(kMostSplits, std::max(1, 8 * runtime().props.multiProcessorCount / pairs));
-  split.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, ceil_div(p.longest, 128)));
-  const size_t rows = (size_t)p.B * p.HK * split.splits * split.columns;
+  const long long pairs = (long long)p.B * p.HK * split.panels, blocks = (p.TQ <= 32 ? 8 : 2) * runtime().props.multiProcessorCount;
+  split.splits = (int)std::min<int64_t>(std::min<int64_t>(kMostSplits, std::max<int64_t>(1, blocks / pairs)), std::max<int64_t>(1, ceil_div(p.longest, 128)));
+  return split;
+}
+
+template <typename T>
+int few_of(const Attention &p, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
+  const Split split = split_of(p);
+  const size_t rows = split.splits > 1 ? (size_t)p.B * p.HK * split.splits * split.columns : 0;
   void *space = nullptr;
   const int rc = workspace(rows * (sizeof(float2) + p.D * sizeof(float)), &space);
   if (rc) return rc;
@@ -186,13 +351,35 @@ int few_of(const Attention &p, const void *q, const void *k, const void *v, void
     ScopedTiming timed(TAG_ATTENTION);
     const dim3 grid((unsigned)(p.B * p.HK * split.panels * split.splits));
     with_shape(p, [&](auto dim, auto bent) {
-      attention_few_kernel<T, dim, kStages, bent><<<grid, dim3(256), 0, runtime().stream>>>(p, split, (const T *)q, (const T *)k, (const T *)v, sums, ends);
+      attention_few_kernel<T, dim, stages_of<T>(), bent><<<grid, dim3(256), 0, runtime().stream>>>(
+          p, split, (const T *)q, (const T *)k, (const T *)v, (T *)out, (_Float16 *)rest, (float *)lse, sums, ends);
     });
     MG_HIP(hipGetLastError());
   }
+  if (split.splits == 1) return MG_OK;
   ScopedTiming timed(TAG_ATTENTION_JOIN);
   attention_join_kernel<T><<<dim3((unsigned)(p.B * p.TQ * p.HQ)), dim3(256), 0, runtime().stream>>>(
       p, split, sums, ends, (const T *)q, (const T *)k, (const T *)v, (T *)out, (_Float16 *)rest, (float *)lse);
+  MG_HIP(hipGetLastError());
+  return MG_OK;
+}
+
+template <typename T>
+int few_dq_of(const Attention &p, const Stats &stats, const void *q, const void *k, const void *v, const void *grad, const void *lse, void *dq, float *sums) {
+  const Split split = split_of(p);
+  {
+    ScopedTiming timed(TAG_ATTENTION_DQ);
+    const dim3 grid((unsigned)(p.B * p.HK * split.panels * split.splits));
+    with_shape(p, [&](auto dim, auto bent) {
+      attention_few_dq_kernel<T, dim, stages_of<T>(), bent><<<grid, dim3(256), 0, runtime().stream>>>(
+          p, split, stats, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (const float *)lse, (T *)dq, sums);
+    });
+    MG_HIP(hipGetLastError());
+  }
+  if (split.splits == 1) return MG_OK;
+  ScopedTiming timed(TAG_ATTENTION_JOIN);
+  attention_dq_join_kernel<T><<<dim3((unsigned)ceil_div((int64_t)p.B * p.TQ * p.HQ, 4)), dim3(256), 0, runtime().stream>>>(
+      p, split, stats, sums, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (const float *)lse, (T *)dq);
   MG_HIP(hipGetLastError());
   return MG_OK;
 }
@@ -201,6 +388,16 @@ int few_of(const Attention &p, const void *q, const void *k, const void *v, void
 
 int forward_few(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
   return dtype == MG_F16 ? few_of<_Float16>(p, q, k, v, out, rest, lse) : few_of<float>(p, q, k, v, out, rest, lse);
+}
+
+size_t few_dq_bytes(const Attention &p) {
+  const Split split = split_of(p);
+  return split.splits > 1 ? (size_t)p.B * p.HK * split.splits * split.columns * p.D * sizeof(float) : 0;
+}
+
+int dq_few(const Attention &p, const Stats &stats, int dtype, const void *q, const void *k, const void *v, const void *grad, const void *lse, void *dq,
+           float *sums) {
+  return dtype == MG_F16 ? few_dq_of<_Float16>(p, stats, q, k, v, grad, lse, dq, sums) : few_dq_of<float>(p, stats, q, k, v, grad, lse, dq, sums);
 }
 
 }  // namespace mg

@@ -12,9 +12,14 @@ constexpr float kRest = 2048.0f;
 bool tiles_take(const Attention &p, int size, uintptr_t ends);
 int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse);
 
-// Worth it up to so many queries: beyond, a wavefront's 32 columns are filled by the queries of one head.
-constexpr int kFewQueries = 32;
+// Whether the forward pass and dq go 32 columns a block instead of 128 queries.
+bool few_take(const Attention &p, int size);
 int forward_few(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse);
+
+struct Stats;
+size_t few_dq_bytes(const Attention &p);  // of workspace for dq_few
+int dq_few(const Attention &p, const Stats &stats, int dtype, const void *q, const void *k, const void *v, const void *grad, const void *lse, void *dq,
+           float *sums);
 int backward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, const void *out, const void *rest, const void *lse,
                    const void *grad, void *dq, void *dk, void *dv);
 

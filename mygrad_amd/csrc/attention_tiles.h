@@ -388,6 +388,129 @@ struct Running {
   }
 };
 
+// Four neighbouring values of a result, registers r .. r + 3 times `by`; true if one is no number.
+template <typename T>
+__device__ __forceinline__ bool put_four(T *to, const f32x16 &from, int r, float by) {
+  f32x4 value;
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    value[j] = from[r + j] * by;
+    odd |= !(__builtin_fabsf(value[j]) < INFINITY);
+  }
+  typedef T V __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<V *>(to) = __builtin_convertvector(value, V);
+  return odd;
+}
+
+// What the two kernels of the gradient need of each row, made in one pass over out, grad and v:
+//   level_i = lse_i - shift             exp2(s_i - level_i) = 2^shift P_i
+//   delta_i = grad_i . out_i            (with what the rounding of out took off)
+//   spans of the rows, and for each chunk of `rows` rows their union and intersection
+constexpr float kShift = 14.0f;  // 2^14 P in float16: whole down to 2^-28
+
+struct Stats {
+  float *level, *delta;  // (B, HQ, TQ)
+  int *lo, *hi;          // (B, TQ)
+  Reach *reach;          // (B, chunks of queries)
+  int rows, chunks;
+};
+
+// Gradients of scores in float16: a lane's column is held at a power of two of its own, which follows its largest value so far (in both
+// halves of the wavefront) and leaves that 2^8 of room, so that values down to 2^-21 of it keep all their digits and the sums are seldom
+// scaled.  Float32 needs none of this.
+struct Unit {
+  float by = 0x1p100f;  // nothing seen yet
+};
+
+template <typename T, int PARTS>
+__device__ __forceinline__ void in_units(Unit &unit, f32x16 &ds, f32x16 (&sums)[PARTS]) {
+  if constexpr (sizeof(T) == 2) {
+    float most = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) most = __builtin_fmaxf(most, __builtin_fabsf(ds[r]));
+    most = larger_half(most);
+    const bool over = most * unit.by > 0x1p15f;
+    if (__any(over)) {
+      const int e = min(max(261 - (int)(__builtin_bit_cast(unsigned, most) >> 23), 1), 254);  // 2^7 / 2^e of the largest
+      const float now = over ? __builtin_bit_cast(float, e << 23) : unit.by, back = now / unit.by;
+      unit.by = now;
+#pragma unroll
+      for (int n = 0; n < PARTS; ++n) sums[n] *= back;
+    }
+    ds *= unit.by;
+  }
+}
+
+// From products s = q.k and dp = grad.v - delta of a tile to s = 2^shift P and dp = 2^shift dS / scale; `away`: place of the query less the key's,
+// as they differ along r.  level(r): of registers r .. r + 3.
+template <typename T, bool ROW_IS_KEY, bool BENT, typename Level>
+__device__ __forceinline__ void gradients_of(const Attention &p, f32x16 &s, f32x16 &dp, const Scores &how, float away, Level level) {
+  if constexpr (BENT) {
+    s *= how.bend;
+    tanh_of_all<T>(s);
+    __builtin_amdgcn_sched_barrier(0);  // what follows, mixed with this, would not fit in the registers
+    dp *= 1.0f - s * s;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  s *= how.factor;
+  if (p.slopes) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] -= how.slope * __builtin_fabsf(ROW_IS_KEY ? away - (float)row_of(r, 0) : away + (float)row_of(r, 0));
+  }
+#pragma unroll
+  for (int r = 0; r < 16; r += 4) {
+    const f32x4 from = level(r);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[r + j] = __builtin_amdgcn_exp2f(s[r + j] - from[j]);
+  }
+  dp *= s;
+}
+
+// Products of 32 queries' gradients with 32 keys, summed into dq^T = K^T dS^T: a query in each lane's column.
+template <typename T, int DP, int ROWS, bool BENT>
+struct Pulled {
+  typedef TileOf<T, DP, ROWS> Tile;
+  typedef typename Fragment<T>::V V;
+  static constexpr int kSteps = DP / 16, kParts = DP / 32;
+
+  f32x16 sums[kParts];
+  Unit unit;
+
+  __device__ __forceinline__ void begin() {
+#pragma unroll
+    for (int n = 0; n < kParts; ++n) sums[n] = zeros();
+  }
+
+  // Keys `from` .. from + 31, rows 32 sub on of the tile at `keys`; their values lie a tile behind.
+  __device__ __forceinline__ void take(const Attention &p, const Scores &how, unsigned keys, int sub, const V (&rows)[kSteps], const V (&grads)[kSteps],
+                                       float level, float delta, const Span &span, int from, bool whole, const typename Tile::Place &place, int h) {
+    f32x16 s = zeros(), dp = zeros();
+#pragma unroll
+    for (int m = 0; m < kSteps; ++m) {
+      s = Fragment<T>::mma(Tile::along(keys, place, sub, m), rows[m], s);
+      dp = Fragment<T>::mma(Tile::along(keys, place, sub, m, Tile::kBytes), grads[m], dp);
+    }
+    dp -= delta;
+    gradients_of<T, true, BENT>(p, s, dp, how, (float)(span.place - from - 4 * h), [&](int) { return f32x4{level, level, level, level}; });
+    if (!whole) {
+      const unsigned seen = (unsigned)(span.hi - span.lo);
+      const int first = from + 4 * h - span.lo;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = (unsigned)(first + row_of(r, 0)) < seen ? dp[r] : 0.0f;
+    }
+    in_units<T>(unit, dp, sums);
+    const V ds[2] = {rows_of<T>(dp, 0), rows_of<T>(dp, 1)};
+#pragma unroll
+    for (int part = 0; part < kParts; ++part)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) sums[part] = Fragment<T>::mma(Tile::across(keys, place, part, 2 * sub + m), ds[m], sums[part]);
+  }
+
+  // What the sums are to be multiplied by.
+  __device__ __forceinline__ float by(const Attention &p) const { return sizeof(T) == 2 ? p.scale / unit.by * 0x1p-14f : p.scale; }  // 2^-kShift
+};
+
 // f(head dimension in whole parts of 32, whether scores are bent), both known to the compiler.
 template <typename F>
 void with_shape(const Attention &p, F f) {

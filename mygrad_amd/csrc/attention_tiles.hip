@@ -107,35 +107,7 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
       attend_row<T, float>(p, b, hq, again, (float *)tiles + wave * kMaxDim, q, k, v, out, rest, lse);
 }
 
-// Four neighbouring values of a result, registers r .. r + 3 times `by`; true if one is no number.
-template <typename T>
-__device__ __forceinline__ bool put_four(T *to, const f32x16 &from, int r, float by) {
-  f32x4 value;
-  bool odd = false;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    value[j] = from[r + j] * by;
-    odd |= !(__builtin_fabsf(value[j]) < INFINITY);
-  }
-  typedef T V __attribute__((ext_vector_type(4)));
-  *reinterpret_cast<V *>(to) = __builtin_convertvector(value, V);
-  return odd;
-}
-
 // ---- gradient ----------------------------------------------------------------------------------------------------------------
-// What the two kernels of the gradient need of each row, made in one pass over out, grad and v:
-//   level_i = lse_i - shift             exp2(s_i - level_i) = 2^shift P_i
-//   delta_i = grad_i . out_i            (with what the rounding of out took off)
-//   spans of the rows, and for each chunk of `rows` rows their union and intersection
-constexpr float kShift = 14.0f;  // 2^14 P in float16: whole down to 2^-28
-
-struct Stats {
-  float *level, *delta;  // (B, HQ, TQ)
-  int *lo, *hi;          // (B, TQ)
-  Reach *reach;          // (B, chunks of queries)
-  int rows, chunks;
-};
-
 template <typename T>
 __device__ __forceinline__ f32x8 eight(const T *from) {
   return __builtin_convertvector(*reinterpret_cast<const typename Fragment<T>::V *>(from), f32x8);
@@ -189,57 +161,6 @@ __global__ void __launch_bounds__(256) attention_stats_kernel(Attention p, Stats
   if (threadIdx.x == 0) stats.reach[(long long)b * stats.chunks + chunk] = r;
 }
 
-// Gradients of scores in float16: a lane's column is held at a power of two of its own, which follows its largest value so far (in both
-// halves of the wavefront) and leaves that 2^8 of room, so that values down to 2^-21 of it keep all their digits and the sums are seldom
-// scaled.  Float32 needs none of this.
-struct Unit {
-  float by = 0x1p100f;  // nothing seen yet
-};
-
-template <typename T, int PARTS>
-__device__ __forceinline__ void in_units(Unit &unit, f32x16 &ds, f32x16 (&sums)[PARTS]) {
-  if constexpr (sizeof(T) == 2) {
-    float most = 0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) most = __builtin_fmaxf(most, __builtin_fabsf(ds[r]));
-    most = larger_half(most);
-    const bool over = most * unit.by > 0x1p15f;
-    if (__any(over)) {
-      const int e = min(max(261 - (int)(__builtin_bit_cast(unsigned, most) >> 23), 1), 254);  // 2^7 / 2^e of the largest
-      const float now = over ? __builtin_bit_cast(float, e << 23) : unit.by, back = now / unit.by;
-      unit.by = now;
-#pragma unroll
-      for (int n = 0; n < PARTS; ++n) sums[n] *= back;
-    }
-    ds *= unit.by;
-  }
-}
-
-// From products s = q.k and dp = grad.v - delta of a tile to s = 2^shift P and dp = 2^shift dS / scale; `away`: place of the query less the key's,
-// as they differ along r.  level(r): of registers r .. r + 3.
-template <typename T, bool ROW_IS_KEY, bool BENT, typename Level>
-__device__ __forceinline__ void gradients_of(const Attention &p, f32x16 &s, f32x16 &dp, const Scores &how, float away, Level level) {
-  if constexpr (BENT) {
-    s *= how.bend;
-    tanh_of_all<T>(s);
-    __builtin_amdgcn_sched_barrier(0);  // what follows, mixed with this, would not fit in the registers
-    dp *= 1.0f - s * s;
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  s *= how.factor;
-  if (p.slopes) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] -= how.slope * __builtin_fabsf(ROW_IS_KEY ? away - (float)row_of(r, 0) : away + (float)row_of(r, 0));
-  }
-#pragma unroll
-  for (int r = 0; r < 16; r += 4) {
-    const f32x4 from = level(r);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s[r + j] = __builtin_amdgcn_exp2f(s[r + j] - from[j]);
-  }
-  dp *= s;
-}
-
 // dq^T = K^T dS^T: as the forward pass, with the queries' rows of grad beside those of q.
 template <typename T, int DP, int KEYS, bool BENT>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
@@ -270,7 +191,6 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
   }
   const long long stat = ((long long)b * p.HQ + hq) * p.TQ + (in ? i : 0);
   const float own_level = in ? stats.level[stat] : INFINITY, delta = in ? stats.delta[stat] : 0.0f;
-  Unit unit;
 
   __syncthreads();
   const int lo = __builtin_amdgcn_readfirstlane(min(min(edges[0][0], edges[0][1]), min(edges[0][2], edges[0][3])));
@@ -288,46 +208,25 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
     load(vb + from, stride, last, to + Tile::kBytes);
   };
 
-  f32x16 sums[kParts];
-#pragma unroll
-  for (int n = 0; n < kParts; ++n) sums[n] = zeros();
+  Pulled<T, DP, KEYS, BENT> run;
+  run.begin();
   const typename Tile::Place place = Tile::place(lane);
   const Scores how = scores_of(p, hq);
   if (count) stage(0);
   all_landed();
   for (int t = 0; t < count; ++t) {
     if (t + 1 < count) stage(t + 1);
-    const int key0 = lo + t * KEYS;
     const unsigned keys = lds + (unsigned)(t & 1) * (2 * Tile::kBytes);  // and values behind them
 #pragma unroll BENT ? 1 : kSubs
     for (int n = 0; n < kSubs; ++n) {
-      const int from = key0 + 32 * n;
-      if (from >= reach.hi || from + 32 <= reach.lo) continue;
-      f32x16 s = zeros(), dp = zeros();
-#pragma unroll
-      for (int m = 0; m < kSteps; ++m) {
-        s = Fragment<T>::mma(Tile::along(keys, place, n, m), rows[m], s);
-        dp = Fragment<T>::mma(Tile::along(keys, place, n, m, Tile::kBytes), grads[m], dp);
-      }
-      dp -= delta;
-      gradients_of<T, true, BENT>(p, s, dp, how, (float)(span.place - from - 4 * h), [&](int) { return f32x4{own_level, own_level, own_level, own_level}; });
-      if (from < reach.all_lo || from + 32 > reach.all_hi) {
-        const unsigned seen = (unsigned)(span.hi - span.lo);
-        const int first = from + 4 * h - span.lo;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] = (unsigned)(first + row_of(r, 0)) < seen ? dp[r] : 0.0f;
-      }
-      in_units<T>(unit, dp, sums);
-      const V ds[2] = {rows_of<T>(dp, 0), rows_of<T>(dp, 1)};
-#pragma unroll
-      for (int part = 0; part < kParts; ++part)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) sums[part] = Fragment<T>::mma(Tile::across(keys, place, part, 2 * n + m), ds[m], sums[part]);
+      const int from = lo + t * KEYS + 32 * n;
+      if (from < reach.hi && from + 32 > reach.lo)
+        run.take(p, how, keys, n, rows, grads, own_level, delta, span, from, from >= reach.all_lo && from + 32 <= reach.all_hi, place, h);
     }
     all_landed();
   }
 
-  const float by = sizeof(T) == 2 ? p.scale / unit.by * 0x1p-14f : p.scale;  // 2^-kShift
+  const float by = run.by(p);
   bool odd = false;
   if (in) {
 #pragma unroll
@@ -335,7 +234,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const int d = 32 * n + row_of(r, h);
-        if (d < p.D) odd |= put_four(dq + row + d, sums[n], r, by);
+        if (d < p.D) odd |= put_four(dq + row + d, run.sums[n], r, by);
       }
   }
   odd = __any(odd);
@@ -536,7 +435,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
       dkv_row<T, float>(p, b, hk, again, (float *)tiles + wave * 2 * kMaxDim, q, k, v, grad, lse, stats.delta, dk, dv);
 }
 
-// Adds the cuts' sums in their order, four values a thread; a block takes 128 keys of one head, as the tiles do.
+constexpr int kJoinKeys = 16;
+
+// Adds the cuts' sums in their order, four values a thread; a block takes sixteen keys of one head.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_dkv_join_kernel(Attention p, Stats stats, int tiles, int cuts, const float *__restrict__ parts,
                                                                  const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
@@ -547,8 +448,8 @@ __global__ void __launch_bounds__(256) attention_dkv_join_kernel(Attention p, St
   const int pair = blockIdx.x / tiles, tile = blockIdx.x % tiles, b = pair / p.HK, hk = pair % p.HK, of_row = p.D / 4;
   const long long all = (long long)p.B * p.TK * p.HK * p.D;
   bool odd = false;
-  for (int n = threadIdx.x; n < 2 * kBlockRows * of_row; n += 256) {
-    const int which = n / (kBlockRows * of_row), rest = n - which * kBlockRows * of_row, j = tile * kBlockRows + rest / of_row;
+  for (int n = threadIdx.x; n < 2 * kJoinKeys * of_row; n += 256) {
+    const int which = n / (kJoinKeys * of_row), rest = n - which * kJoinKeys * of_row, j = tile * kJoinKeys + rest / of_row;
     if (j >= p.TK) continue;
     const long long at = (((long long)b * p.TK + j) * p.HK + hk) * p.D + rest % of_row * 4;
     f32x4 sum = *(const f32x4 *)(parts + which * cuts * all + at);
@@ -563,18 +464,27 @@ __global__ void __launch_bounds__(256) attention_dkv_join_kernel(Attention p, St
   all_landed();
   const int wave = threadIdx.x >> 6;
   if (bad[0] | bad[1] | bad[2] | bad[3])
-    for (int again = tile * kBlockRows + wave; again < min(p.TK, (tile + 1) * kBlockRows); again += 4)
+    for (int again = tile * kJoinKeys + wave; again < min(p.TK, (tile + 1) * kJoinKeys); again += 4)
       dkv_row<T, float>(p, b, hk, again, mine[wave], q, k, v, grad, lse, stats.delta, dk, dv);
 }
 
-// How many cuts the blocks of attention_dkv_kernel are made in.  All blocks of an unmasked problem take as long, those of a causal one up to twice
-// the mean: one for each compute unit will do, or four.  A cut writes and reads 16 bytes for each value of k, which takes as long as the products
-// with some 250 queries (50 in float32): it is worth it at four times that.  Measured at 4 x 2048 tokens, 16 heads over 4, causal, float16: 604 us
-// in one piece, 460 in two, 355 in four; 3 x 12 heads, 1531 queries, 997 keys: 110 in one, 121 in two.
-int cuts_of(const Attention &p, int blocks, int size) {
-  const int cus = runtime().props.multiProcessorCount, enough = p.causal ? 4 * cus : cus;
-  const long long worth = (long long)p.group * p.TQ / (size == 2 ? 1000 : 200);
-  return (int)std::max(1ll, std::min({(long long)ceil_div(enough, blocks), worth, 8ll}));
+// How many cuts the blocks of attention_dkv_kernel are made in: as many as make the estimate of the time least.  A block takes `chunk` for each
+// chunk of queries it goes through, while two of them on a compute unit run beside each other in float16 (in float32 one keeps the matrix cores
+// four fifths busy), and the first keys of a causal mask are seen by all queries, twice the mean.  Joining takes a launch and 16 bytes written
+// and read for each value of k and cut.  Measured at 4 x 2048 tokens, 16 heads over 4, causal, float16: 604 us in one piece, 415 in two, 285 in four;
+// 4 x 75 tokens, 32 heads over 4: 60 in one, 26 in eight.
+int cuts_of(const Attention &p, const Stats &stats, int size, int blocks) {
+  const double at_once = (size == 2 ? 2.0 : 1.25) * runtime().props.multiProcessorCount, every = (double)p.group * stats.chunks;
+  const double chunk = 1e-6 + stats.rows * 128.0 * ((p.D + 31) / 32 * 32) * 8 / (size == 2 ? 3.0e12 : 0.5e12);
+  const double bytes = 16.0 * p.B * p.TK * p.HK * p.D;
+  int best = 1;
+  double least = 0;
+  for (int cuts = 1; cuts <= 32 && cuts <= every; cuts *= 2) {
+    const double turns = std::max(blocks * every * (p.causal ? 0.5 : 1.0) / at_once, every / cuts);
+    const double time = turns * chunk + (cuts > 1 ? 5e-6 + cuts * bytes / 3e12 : 0.0);
+    if (cuts == 1 || time < least) best = cuts, least = time;
+  }
+  return best;
 }
 
 template <typename T, int ROWS>
@@ -583,12 +493,15 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
   Stats stats{};
   stats.rows = sizeof(T) == 2 && p.D > 96 ? 32 : ROWS, stats.chunks = (int)ceil_div(p.TQ, stats.rows);
   const size_t rows = (size_t)p.B * p.TQ, all = rows * p.HQ, chunks = (size_t)p.B * stats.chunks, keys = (size_t)p.B * p.TK * p.HK * p.D;
-  const int key_tiles = (int)ceil_div(p.TK, kBlockRows), cuts = dk ? cuts_of(p, p.B * p.HK * key_tiles, sizeof(T)) : 1;
+  const int key_tiles = (int)ceil_div(p.TK, kBlockRows), cuts = dk ? cuts_of(p, stats, sizeof(T), p.B * p.HK * key_tiles) : 1;
+  const bool few = dq && few_take(p, sizeof(T));
+  // sums of splits of dq and of cuts of dk and dv: one after the other
+  const size_t sums = std::max(cuts > 1 ? 8 * cuts * keys : 0, few ? few_dq_bytes(p) : 0);
   void *space = nullptr;
-  int rc = workspace((cuts > 1 ? 8 * cuts * keys : 0) + sizeof(Reach) * chunks + 4 * (2 * all + 2 * rows), &space);
+  int rc = workspace(sums + sizeof(Reach) * chunks + 4 * (2 * all + 2 * rows), &space);
   if (rc) return rc;
   float *partial = (float *)space;  // whole pieces of 16 bytes: dim is a multiple of 8
-  stats.reach = (Reach *)(partial + (cuts > 1 ? 2 * cuts * keys : 0));
+  stats.reach = (Reach *)((char *)space + sums);
   stats.level = (float *)(stats.reach + chunks);
   stats.delta = stats.level + all;
   stats.lo = (int *)(stats.delta + all);
@@ -601,7 +514,10 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
     attention_stats_kernel<T><<<dim3((unsigned)(p.B * p.HQ * stats.chunks)), dim3(256), 0, s>>>(p, stats, (const T *)out, (const _Float16 *)rest, tl, tg);
     MG_HIP(hipGetLastError());
   }
-  if (dq) {
+  if (few) {
+    rc = dq_few(p, stats, sizeof(T) == 2 ? MG_F16 : MG_F32, q, k, v, grad, lse, dq, partial);
+    if (rc) return rc;
+  } else if (dq) {
     ScopedTiming timed(TAG_ATTENTION_DQ);
     const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
     with_shape(p, [&](auto dim, auto bent) {
@@ -623,7 +539,7 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
   }
   if (cuts == 1) return MG_OK;
   ScopedTiming timed(TAG_ATTENTION_JOIN);
-  attention_dkv_join_kernel<T><<<dim3((unsigned)(p.B * p.HK * key_tiles)), dim3(256), 0, s>>>(p, stats, key_tiles, cuts, partial, tq, tk, tv, tg, tl, (T *)dk,
+  attention_dkv_join_kernel<T><<<dim3((unsigned)(p.B * p.HK * ceil_div(p.TK, kJoinKeys))), dim3(256), 0, s>>>(p, stats, (int)ceil_div(p.TK, kJoinKeys), cuts, partial, tq, tk, tv, tg, tl, (T *)dk,
                                                                                             (T *)dv);
   MG_HIP(hipGetLastError());
   return MG_OK;
@@ -635,6 +551,14 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
 bool tiles_take(const Attention &p, int size, uintptr_t ends) {
   return p.D <= 128 && p.D % 8 == 0 && ends % 16 == 0 && (long long)p.HQ * p.D * size * 128 < (1ll << 31) &&
          (long long)p.B * p.HQ * ceil_div(p.TQ, 32) < (1 << 24) && (long long)p.B * p.HK * ceil_div(p.TK, 32) < (1 << 24);
+}
+
+// Up to 32 queries one head would not fill a wavefront's columns.  Float32 products take so long that a few blocks of 128 queries, each on
+// a compute unit of its own, are slower than four times as many of 32 columns: 1 x 559 tokens of 4 heads 63 us against 25, 3 x 84 of 16 21 against
+// 13 -- until there are blocks for half the units (3 x 565 of 6: 37 against 33; 4 x 1024 of 8: 100 against 107).  In float16 they are no faster
+// (2 x 769 of 4 heads: 25 us against 44).
+bool few_take(const Attention &p, int size) {
+  return p.TQ <= 32 || (size == 4 && 2 * (long long)p.B * p.HQ * ceil_div(p.TQ, kBlockRows) < runtime().props.multiProcessorCount);
 }
 
 int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
