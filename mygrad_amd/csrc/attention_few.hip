@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
   for (int n = 0; n < kSteps; ++n) rows[n] = fragment_of(row, 16 * n + 8 * h, p.D, at.in);
   const Scores how = scores_of(p, at.hq);
 
-  Running<T, DP, 1, BENT> run;
+  Running<T, DP, 1, BENT, true> run;
   run.begin();
   const typename Tile::Place place = Tile::place(lane);
   const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)space + (unsigned)wave * (STAGES * 2 * Tile::kBytes);

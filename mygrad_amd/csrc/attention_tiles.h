@@ -240,13 +240,34 @@ __device__ __forceinline__ int row_of(int r, int h) { return 8 * (r >> 2) + 4 * 
 
 __device__ __forceinline__ f32x16 zeros() { return f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}; }
 
-// Registers 8 n .. 8 n + 7 as a fragment along the rows.
+// Registers 8 n .. 8 n + 7 as a fragment along the rows, and what rounding took off them as another.
 template <typename T>
 __device__ __forceinline__ typename Fragment<T>::V rows_of(const f32x16 &v, int n) {
   f32x8 part;
 #pragma unroll
   for (int j = 0; j < 8; ++j) part[j] = v[8 * n + j];
   return __builtin_convertvector(part, typename Fragment<T>::V);
+}
+
+template <typename T>
+__device__ __forceinline__ typename Fragment<T>::V rows_of(const f32x16 &v, int n, typename Fragment<T>::V &more) {
+  f32x8 part;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) part[j] = v[8 * n + j];
+  const auto near = __builtin_convertvector(part, typename Fragment<T>::V);
+  if constexpr (sizeof(T) == 2) more = __builtin_convertvector(part - __builtin_convertvector(near, f32x8), typename Fragment<T>::V);
+  return near;
+}
+
+// a times both: a float32 value in two of float16 keeps 22 bits (one is all of it in float32).  Gradients of scores are multiplied so: rounded to 11
+// bits they would make dq and dk off by half as much again as the rounding of the results does, which costs a fifth of dq's time and a
+// fourteenth of dk's and dv's (8192 packed tokens: 161 against 192 us, 291 against 315).  Weights are rounded once where products are the bound
+// (a block of 128 queries: results are off by 1.2 to 1.4 times their own rounding), and kept in two where bytes are.
+template <typename T>
+__device__ __forceinline__ f32x16 mma_of_two(typename Fragment<T>::V a, typename Fragment<T>::V b, typename Fragment<T>::V more, f32x16 c) {
+  c = Fragment<T>::mma(a, b, c);
+  if constexpr (sizeof(T) == 2) c = Fragment<T>::mma(a, more, c);
+  return c;
 }
 
 // tanh of a lane's sixteen values.  Where all of the wavefront's are below 1/4, an odd polynomial (what float32's leaves out is below
@@ -308,8 +329,9 @@ __device__ __forceinline__ Scores scores_of(const Attention &p, int head) {
 
 // 32 queries, one in each lane's column (in both halves), on their way through tiles of SUBS times 32 keys: S^T = K Q^T has a query's scores in
 // its lane (and the partner in the other half), so maximum and sum need no exchange but that one, and the weights are the right operand of
-// out^T = V^T P^T as they lie.  BENT: scores have a cap (whose registers the others do without).
-template <typename T, int DP, int SUBS, bool BENT>
+// out^T = V^T P^T as they lie.  BENT: scores have a cap (whose registers the others do
+// without).  FINE: float16 takes weights in two.
+template <typename T, int DP, int SUBS, bool BENT, bool FINE>
 struct Running {
   typedef TileOf<T, DP, 32 * SUBS> Tile;
   typedef typename Fragment<T>::V V;
@@ -378,13 +400,16 @@ struct Running {
         s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - base);
         total += s[n][r];
       }
-    V weights[2 * SUBS];
+    V weights[2 * SUBS], more[FINE ? 2 * SUBS : 1];
 #pragma unroll
-    for (int m = 0; m < 2 * SUBS; ++m) weights[m] = rows_of<T>(s[m >> 1], m & 1);
+    for (int m = 0; m < 2 * SUBS; ++m) weights[m] = FINE ? rows_of<T>(s[m >> 1], m & 1, more[FINE ? m : 0]) : rows_of<T>(s[m >> 1], m & 1);
 #pragma unroll
     for (int n = 0; n < kParts; ++n)
 #pragma unroll
-      for (int m = 0; m < 2 * SUBS; ++m) sums[n] = Fragment<T>::mma(Tile::across(values, place, n, m), weights[m], sums[n]);
+      for (int m = 0; m < 2 * SUBS; ++m) {
+        const V value = Tile::across(values, place, n, m);
+        sums[n] = FINE ? mma_of_two<T>(value, weights[m], more[FINE ? m : 0], sums[n]) : Fragment<T>::mma(value, weights[m], sums[n]);
+      }
   }
 };
 
@@ -500,11 +525,13 @@ struct Pulled {
       for (int r = 0; r < 16; ++r) dp[r] = (unsigned)(first + row_of(r, 0)) < seen ? dp[r] : 0.0f;
     }
     in_units<T>(unit, dp, sums);
-    const V ds[2] = {rows_of<T>(dp, 0), rows_of<T>(dp, 1)};
+    V ds[2], more[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) ds[m] = rows_of<T>(dp, m, more[m]);
 #pragma unroll
     for (int part = 0; part < kParts; ++part)
 #pragma unroll
-      for (int m = 0; m < 2; ++m) sums[part] = Fragment<T>::mma(Tile::across(keys, place, part, 2 * sub + m), ds[m], sums[part]);
+      for (int m = 0; m < 2; ++m) sums[part] = mma_of_two<T>(Tile::across(keys, place, part, 2 * sub + m), ds[m], more[m], sums[part]);
   }
 
   // What the sums are to be multiplied by.

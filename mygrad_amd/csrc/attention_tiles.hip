@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
     load(vb + from, stride, last, to + Tile::kBytes);
   };
 
-  Running<T, DP, KEYS / 32, BENT> run;
+  Running<T, DP, KEYS / 32, BENT, false> run;
   run.begin();
   const typename Tile::Place place = Tile::place(lane);
   const Scores how = scores_of(p, hq);
@@ -393,12 +393,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
           }
         }
         in_units<T>(unit, dp, sum_k);
-        const V weights[2] = {rows_of<T>(s, 0), rows_of<T>(s, 1)}, back[2] = {rows_of<T>(dp, 0), rows_of<T>(dp, 1)};
+        V weights[2], back[2], more[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) weights[m] = rows_of<T>(s, m), back[m] = rows_of<T>(dp, m, more[m]);
 #pragma unroll
         for (int part = 0; part < kParts; ++part)
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
-            sum_k[part] = Fragment<T>::mma(Tile::across(queries, place, part, 2 * n + m), back[m], sum_k[part]);
+            sum_k[part] = mma_of_two<T>(Tile::across(queries, place, part, 2 * n + m), back[m], more[m], sum_k[part]);
             sum_v[part] = Fragment<T>::mma(Tile::across(queries, place, part, 2 * n + m, Tile::kBytes), weights[m], sum_v[part]);
           }
       }
