@@ -127,7 +127,7 @@ int backward_rows(const Attention &p, const void *q, const void *k, const void *
   return MG_OK;
 }
 
-int check_attention(const mg_attention_desc *d, Attention *p, const char *who) {
+int check_attention(const mg_attention_desc *d, Attention *p, const char *who, bool gradient) {
   if (!d) return fail(MG_ERR_BAD_ARG, "%s: null descriptor", who);
   if (d->dtype != MG_F32 && d->dtype != MG_F64 && d->dtype != MG_F16) return fail(MG_ERR_UNSUPPORTED, "%s: dtype %d", who, d->dtype);
   if (d->B < 0 || d->TQ < 0 || d->TK < 0 || d->HQ <= 0 || d->HK <= 0 || d->D <= 0 || d->HQ % d->HK != 0)
@@ -136,7 +136,7 @@ int check_attention(const mg_attention_desc *d, Attention *p, const char *who) {
   if (d->D > kMaxDim) return fail(MG_ERR_UNSUPPORTED, "%s: a head dimension of %lld (at most %d)", who, (long long)d->D, kMaxDim);
   const int64_t most = 1 << 30;
   if (d->TQ >= most || d->TK >= most || d->HQ >= most || d->B >= most || d->B * d->HQ >= most || d->B * d->HQ * ceil_div(d->TQ, 4) >= (1 << 24) ||
-      d->B * d->HK * ceil_div(d->TK, 4) >= (1 << 24))
+      (gradient && d->B * d->HK * ceil_div(d->TK, 4) >= (1 << 24)))  // a wavefront per row
     return fail(MG_ERR_UNSUPPORTED, "%s: 2^26 rows of results or more", who);
   if (d->longest < 0) return fail(MG_ERR_BAD_ARG, "%s: a longest length of %lld", who, (long long)d->longest);
   if (d->window < 0 || d->window > most) return fail(MG_ERR_BAD_ARG, "%s: a window of %lld keys", who, (long long)d->window);
@@ -165,7 +165,7 @@ int mg_attention_fwd(const mg_attention_desc *desc, const void *q, const void *k
   std::lock_guard<std::recursive_mutex> guard(api_mutex());
   MG_REQUIRE_INIT();
   Attention p{};
-  const int rc = check_attention(desc, &p, "mg_attention_fwd");
+  const int rc = check_attention(desc, &p, "mg_attention_fwd", false);
   if (rc) return rc;
   if (p.B == 0 || p.TQ == 0) return MG_OK;
   if (!q || !out || (p.TK && (!k || !v))) return fail(MG_ERR_BAD_ARG, "null pointer in mg_attention_fwd");
@@ -183,7 +183,7 @@ int mg_attention_bwd(const mg_attention_desc *desc, const void *q, const void *k
   std::lock_guard<std::recursive_mutex> guard(api_mutex());
   MG_REQUIRE_INIT();
   Attention p{};
-  const int rc = check_attention(desc, &p, "mg_attention_bwd");
+  const int rc = check_attention(desc, &p, "mg_attention_bwd", true);
   if (rc) return rc;
   if (!dk != !dv) return fail(MG_ERR_BAD_ARG, "mg_attention_bwd: dk without dv, or the other way round");
   const size_t size = desc->dtype == MG_F64 ? 8 : desc->dtype == MG_F32 ? 4 : 2;

@@ -62,8 +62,8 @@ __device__ __forceinline__ void each_tile(const Attention &p, const Panel &at, c
   auto stage = [&](int t, int side) {
     const long long from = (long long)t * 32 * stride;
     const unsigned to = lds + (unsigned)side * (2 * Tile::kBytes);
-    load(kb + from, stride, at.reach.hi - at.reach.lo - t * 32, to);
-    load(vb + from, stride, at.reach.hi - at.reach.lo - t * 32, to + Tile::kBytes);
+    load(kb + from, at.reach.hi - at.reach.lo - t * 32, to);
+    load(vb + from, at.reach.hi - at.reach.lo - t * 32, to + Tile::kBytes);
   };
   int side = 0;
   if (at.first + wave < at.last) stage(at.first + wave, 0);
@@ -101,16 +101,6 @@ struct Joined {
     return sum;
   }
 };
-
-template <typename T>
-__device__ __forceinline__ bool put_value(T *to, f32x4 value) {
-  typedef T V __attribute__((ext_vector_type(4)));
-  *reinterpret_cast<V *>(to) = __builtin_convertvector(value, V);
-  bool odd = false;
-#pragma unroll
-  for (int n = 0; n < 4; ++n) odd |= !(__builtin_fabsf(value[n]) < INFINITY);
-  return odd;
-}
 
 // With one split the result itself; else sums at the block's own top, and that with the total.
 template <typename T, int DP, int STAGES, bool BENT>
@@ -151,8 +141,8 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
   Join::put(join, run.sums, run.top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(run.top - top), wave, c, h);
   float all = 0;
 #pragma unroll
-  for (int w = 0; w < 4; ++w)
-    if (tops[w][c] != -INFINITY) all += totals[w][c] * __builtin_amdgcn_exp2f(tops[w][c] - top);
+  for (int w = 0; w < 4; ++w)  // without a top the total is 0, or no number where no score is one
+    all += totals[w][c] * (tops[w][c] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(tops[w][c] - top));
   __syncthreads();
   const long long base = ((long long)at.pair * split.splits + at.part) * split.columns + at.first_column;
   if (split.splits > 1) {
@@ -174,11 +164,9 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
     if (d >= p.D) continue;
     const f32x4 value = Join::sum(join, column, d) * tops[0][column];
     const long long to = (((long long)at.b * p.TQ + all_columns / p.group) * p.HQ + at.hk * p.group + all_columns % p.group) * p.D + d;
-    odd |= put_value(out + to, value);
+    odd |= put_four(out + to, value);
     if constexpr (sizeof(T) == 2) {
-      if (remains)
-        *reinterpret_cast<f16x4 *>(remains + to) =
-            __builtin_convertvector((value - __builtin_convertvector(__builtin_convertvector(value, f16x4), f32x4)) * kRest, f16x4);
+      if (remains) put_four(remains + to, (value - __builtin_convertvector(__builtin_convertvector(value, f16x4), f32x4)) * kRest);
     }
   }
   odd = __any(odd);
@@ -191,11 +179,11 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
 
 // A block per row of the result: the splits' sums at a common top, in their order.  A row that comes out as no number is computed once more, so
 // that what it does not see leaves no mark (products with weights of zero do, where that is no number).
-template <typename T>
+template <typename T, int PARTS>
 __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split split, const float *__restrict__ sums, const float2 *__restrict__ ends,
                                                              const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
                                                              T *__restrict__ out, _Float16 *__restrict__ rest, float *__restrict__ lse) {
-  __shared__ float parts[4][128], totals[4], mine[kMaxDim], weights[kMostSplits];
+  __shared__ float parts[4][64 * PARTS], totals[4], mine[kMaxDim], weights[kMostSplits];
   __shared__ int odd[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int hq = blockIdx.x % p.HQ, i = blockIdx.x / p.HQ % p.TQ, b = blockIdx.x / p.HQ / p.TQ;
@@ -203,7 +191,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split 
   float top = -INFINITY;
   for (int n = lane; n < split.splits; n += 64) top = __builtin_fmaxf(top, ends[first + (long long)n * split.columns].x);
   top = wave_max(top);
-  float total = 0, sum0 = 0, sum1 = 0;
+  float total = 0, sum[PARTS] = {};
   for (int n = threadIdx.x; n < split.splits; n += 256) {
     const float2 end = ends[first + (long long)n * split.columns];
     weights[n] = end.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(end.x - top);
@@ -211,16 +199,19 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split 
   }
   total = wave_sum(total);
   __syncthreads();
-  const float *from = sums + first * p.D + (lane < p.D ? lane : 0);
+  const float *from = sums + first * p.D;
   const long long step = (long long)split.columns * p.D;
-  const int second = lane + 64 < p.D ? 64 : 0;
+  int at[PARTS];  // values that the row does not have repeat its first
+#pragma unroll
+  for (int m = 0; m < PARTS; ++m) at[m] = lane + 64 * m < p.D ? lane + 64 * m : 0;
 #pragma unroll 8
   for (int n = wave; n < split.splits; n += 4) {
     const float by = weights[n];
-    sum0 += from[n * step] * by;
-    sum1 += from[n * step + second] * by;
+#pragma unroll
+    for (int m = 0; m < PARTS; ++m) sum[m] += from[n * step + at[m]] * by;
   }
-  parts[wave][lane] = sum0, parts[wave][lane + 64] = sum1;
+#pragma unroll
+  for (int m = 0; m < PARTS; ++m) parts[wave][lane + 64 * m] = sum[m];
   if (lane == 0) totals[wave] = total;
   __syncthreads();
   total = totals[0] + totals[1] + totals[2] + totals[3];
@@ -287,7 +278,7 @@ __global__ void __launch_bounds__(256) attention_few_dq_kernel(Attention p, Spli
     if (split.splits > 1)
       *(f32x4 *)(sums + (base + column) * p.D + d) = value;
     else
-      odd |= put_value(dq + (((long long)at.b * p.TQ + all_columns / p.group) * p.HQ + at.hk * p.group + all_columns % p.group) * p.D + d, value);
+      odd |= put_four(dq + (((long long)at.b * p.TQ + all_columns / p.group) * p.HQ + at.hk * p.group + all_columns % p.group) * p.D + d, value);
   }
   if (split.splits > 1) return;
   odd = __any(odd);
@@ -299,7 +290,7 @@ __global__ void __launch_bounds__(256) attention_few_dq_kernel(Attention p, Spli
 }
 
 // A wavefront per row of dq.
-template <typename T>
+template <typename T, int PARTS>
 __global__ void __launch_bounds__(256) attention_dq_join_kernel(Attention p, Split split, Stats stats, const float *__restrict__ sums,
                                                                 const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
                                                                 const T *__restrict__ grad, const float *__restrict__ lse, T *__restrict__ dq) {
@@ -309,23 +300,40 @@ __global__ void __launch_bounds__(256) attention_dq_join_kernel(Attention p, Spl
   if (at_row >= (long long)p.B * p.TQ * p.HQ) return;
   const int hq = (int)(at_row % p.HQ), i = (int)(at_row / p.HQ % p.TQ), b = (int)(at_row / p.HQ / p.TQ);
   const long long first = ((long long)b * p.HK + hq / p.group) * split.splits * split.columns + i * p.group + hq % p.group;
-  const float *from = sums + first * p.D + (lane < p.D ? lane : 0);
+  const float *from = sums + first * p.D;
   const long long step = (long long)split.columns * p.D;
-  const int second = lane + 64 < p.D ? 64 : 0;
-  float sum0 = 0, sum1 = 0;
+  float sum[PARTS] = {};
+  int at[PARTS];  // values that the row does not have repeat its first
+#pragma unroll
+  for (int m = 0; m < PARTS; ++m) at[m] = lane + 64 * m < p.D ? lane + 64 * m : 0;
 #pragma unroll 8
-  for (int n = 0; n < split.splits; ++n) sum0 += from[n * step], sum1 += from[n * step + second];
-  T *to = dq + at_row * p.D + lane;
-  if (lane < p.D) to[0] = (T)sum0;
-  if (second) to[64] = (T)sum1;
-  if (__any(!(__builtin_fabsf(sum0) < INFINITY) || !(__builtin_fabsf(sum1) < INFINITY))) {
+  for (int n = 0; n < split.splits; ++n)
+#pragma unroll
+    for (int m = 0; m < PARTS; ++m) sum[m] += from[n * step + at[m]];
+  bool odd = false;
+#pragma unroll
+  for (int m = 0; m < PARTS; ++m)
+    if (lane + 64 * m < p.D) dq[at_row * p.D + lane + 64 * m] = (T)sum[m], odd |= !(__builtin_fabsf(sum[m]) < INFINITY);
+  if (__any(odd)) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     dq_row<T, float>(p, b, hq, i, mine[wave], q, k, v, grad, lse, stats.delta, dq);
   }
 }
 
+// f(values of a row that a lane of 64 holds)
+template <typename F>
+void with_parts(const Attention &p, F f) {
+  if (p.D <= 64)
+    f(std::integral_constant<int, 1>{});
+  else if (p.D <= 128)
+    f(std::integral_constant<int, 2>{});
+  else
+    f(std::integral_constant<int, 4>{});
+}
+
+// Tiles ahead of four wavefronts: as many as there is room for.
 template <typename T>
-constexpr int stages_of() { return sizeof(T) == 2 ? 2 : 1; }  // as many as four wavefronts have room for at 128 values a head
+constexpr int stages_of(int dim) { return sizeof(T) == 2 && dim <= 128 ? 2 : 1; }
 
 // A block for each 128 keys (a tile for each wavefront) while there are fewer than fill the device eight times over: a batch of ragged lengths evens
 // out over that many.  With more queries the products count and not the bytes, and twice over will do.
@@ -345,21 +353,23 @@ int few_of(const Attention &p, const void *q, const void *k, const void *v, void
   void *space = nullptr;
   const int rc = workspace(rows * (sizeof(float2) + p.D * sizeof(float)), &space);
   if (rc) return rc;
-  float *sums = (float *)space;  // D is a multiple of 8: what follows is aligned
+  float *sums = (float *)space;  // D is a multiple of 4: what follows is aligned
   float2 *ends = (float2 *)(sums + rows * p.D);
   {
     ScopedTiming timed(TAG_ATTENTION);
     const dim3 grid((unsigned)(p.B * p.HK * split.panels * split.splits));
-    with_shape(p, [&](auto dim, auto bent) {
-      attention_few_kernel<T, dim, stages_of<T>(), bent><<<grid, dim3(256), 0, runtime().stream>>>(
+    with_shape<T>(p, [&](auto dim, auto bent) {
+      attention_few_kernel<T, dim, stages_of<T>(dim), bent><<<grid, dim3(256), 0, runtime().stream>>>(
           p, split, (const T *)q, (const T *)k, (const T *)v, (T *)out, (_Float16 *)rest, (float *)lse, sums, ends);
     });
     MG_HIP(hipGetLastError());
   }
   if (split.splits == 1) return MG_OK;
   ScopedTiming timed(TAG_ATTENTION_JOIN);
-  attention_join_kernel<T><<<dim3((unsigned)(p.B * p.TQ * p.HQ)), dim3(256), 0, runtime().stream>>>(
-      p, split, sums, ends, (const T *)q, (const T *)k, (const T *)v, (T *)out, (_Float16 *)rest, (float *)lse);
+  with_parts(p, [&](auto parts) {
+    attention_join_kernel<T, parts><<<dim3((unsigned)(p.B * p.TQ * p.HQ)), dim3(256), 0, runtime().stream>>>(
+        p, split, sums, ends, (const T *)q, (const T *)k, (const T *)v, (T *)out, (_Float16 *)rest, (float *)lse);
+  });
   MG_HIP(hipGetLastError());
   return MG_OK;
 }
@@ -370,16 +380,18 @@ int few_dq_of(const Attention &p, const Stats &stats, const void *q, const void 
   {
     ScopedTiming timed(TAG_ATTENTION_DQ);
     const dim3 grid((unsigned)(p.B * p.HK * split.panels * split.splits));
-    with_shape(p, [&](auto dim, auto bent) {
-      attention_few_dq_kernel<T, dim, stages_of<T>(), bent><<<grid, dim3(256), 0, runtime().stream>>>(
+    with_shape<T>(p, [&](auto dim, auto bent) {
+      attention_few_dq_kernel<T, dim, stages_of<T>(dim), bent><<<grid, dim3(256), 0, runtime().stream>>>(
           p, split, stats, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (const float *)lse, (T *)dq, sums);
     });
     MG_HIP(hipGetLastError());
   }
   if (split.splits == 1) return MG_OK;
   ScopedTiming timed(TAG_ATTENTION_JOIN);
-  attention_dq_join_kernel<T><<<dim3((unsigned)ceil_div((int64_t)p.B * p.TQ * p.HQ, 4)), dim3(256), 0, runtime().stream>>>(
-      p, split, stats, sums, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (const float *)lse, (T *)dq);
+  with_parts(p, [&](auto parts) {
+    attention_dq_join_kernel<T, parts><<<dim3((unsigned)ceil_div((int64_t)p.B * p.TQ * p.HQ, 4)), dim3(256), 0, runtime().stream>>>(
+        p, split, stats, sums, (const T *)q, (const T *)k, (const T *)v, (const T *)grad, (const float *)lse, (T *)dq);
+  });
   MG_HIP(hipGetLastError());
   return MG_OK;
 }

@@ -77,12 +77,13 @@ struct TileOf {
       return kRounds;
     }
     static constexpr int kOffsets = repeat();
-    unsigned at[kOffsets];
+    unsigned at[kOffsets], stride, dim;
 
     static __device__ __forceinline__ int slot(int round) { return round * THREADS + (int)(THREADS == 64 ? threadIdx.x & 63 : threadIdx.x); }
 
-    // Pieces behind the `dim` bytes of a row are zeros.
-    __device__ __forceinline__ Loader(unsigned stride, unsigned dim) {
+    // Pieces behind the `dim` bytes of a row are zeros; the one that the row's end cuts goes on into what follows it, which meets zeros of the
+    // other operand (or lands in results that nobody stores).
+    __device__ __forceinline__ Loader(unsigned stride, unsigned dim) : stride(stride), dim(dim) {
 #pragma unroll
       for (int n = 0; n < kOffsets; ++n) {
         const int row = slot(n) / kPieces, piece = (slot(n) % kPieces) ^ turn(row);
@@ -90,27 +91,28 @@ struct TileOf {
       }
     }
 
-    // Rows [0, ROWS) from `base` on to the tile at byte `lds`; rows from `last` on are zeros.
-    __device__ __forceinline__ void operator()(const char *base, unsigned stride, int last, unsigned lds) const {
-      if (last >= ROWS)
-        rounds<false>(base, stride, last, lds);
+    // Rows [0, ROWS) from `base` on to the tile at byte `lds`; rows from `last` on are zeros, and the last one's end is that of what is read.
+    __device__ __forceinline__ void operator()(const char *base, int last, unsigned lds) const {
+      if (last >= ROWS + (dim % 16 ? 1 : 0))
+        rounds<false>(base, last, lds);
       else
-        rounds<true>(base, stride, last, lds);
+        rounds<true>(base, last, lds);
     }
 
    private:
     template <bool CUT>
-    __device__ __forceinline__ void rounds(const char *base, unsigned stride, int last, unsigned lds) const {
+    __device__ __forceinline__ void rounds(const char *base, int last, unsigned lds) const {
       typedef MG_LDS void *LdsPointer;
-      const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0x7fffffff, 0x00020000);
+      const int bytes = CUT ? last > 0 ? (last - 1) * (int)stride + (int)dim : 0 : 0x7fffffff;
+      const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, bytes, 0x00020000);
       const int wave = THREADS == 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
       for (int n = 0; n < kRounds; ++n) {
         if (ROWS * kPieces % THREADS != 0 && n * THREADS + wave * 64 >= ROWS * kPieces) continue;
-        unsigned from = at[n % kOffsets];
-        if (CUT && slot(n) / kPieces >= last) from = kBeyond;
+        unsigned from = at[n % kOffsets], more = (unsigned)(n / kOffsets * kOffsets * THREADS / kPieces) * stride;
+        if (CUT) from = slot(n) / kPieces < last && from != kBeyond ? from + more : kBeyond, more = 0;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (LdsPointer)(unsigned long long)(lds + (unsigned)(n * THREADS + wave * 64) * 16u), 16, (int)from,
-                                                 (int)((unsigned)(n / kOffsets * kOffsets * THREADS / kPieces) * stride), 0, 0);
+                                                 (int)more, 0, 0);
       }
     }
   };
@@ -227,13 +229,36 @@ __device__ __forceinline__ Reach reach_of(Span s, bool in) {
                __builtin_amdgcn_readfirstlane(r.all_hi)};
 }
 
-// Eight values of a row in memory as a fragment: zeros where the row or the piece is none.
+// Eight values of a row in memory as a fragment: zeros where the row or its values, whole fours, end.
 template <typename T>
 __device__ __forceinline__ typename Fragment<T>::V fragment_of(const T *row, int at, int dim, bool in) {
+  typedef T Eight __attribute__((ext_vector_type(8), aligned(4 * sizeof(T)))), Four __attribute__((ext_vector_type(4)));
   typename Fragment<T>::V v = {};
-  if (in && at < dim) v = *reinterpret_cast<const typename Fragment<T>::V *>(row + at);
+  if (in && at + 8 <= dim) {
+    const Eight held = *reinterpret_cast<const Eight *>(row + at);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = held[j];
+  }
+  if ((dim & 4) && in && at + 4 == dim) {
+    const Four held = *reinterpret_cast<const Four *>(row + at);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = held[j];
+  }
   return v;
 }
+
+// Four neighbouring values of a result to `to`; true if one of them is no number.
+template <typename T>
+__device__ __forceinline__ bool put_four(T *to, f32x4 value) {
+  typedef T V __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<V *>(to) = __builtin_convertvector(value, V);
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) odd |= !(__builtin_fabsf(value[j]) < INFINITY);
+  return odd;
+}
+
+__device__ __forceinline__ f32x4 four_of(const f32x16 &v, int r) { return f32x4{v[r], v[r + 1], v[r + 2], v[r + 3]}; }
 
 // Rows of a tile of results as the registers of a lane hold them.
 __device__ __forceinline__ int row_of(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
@@ -413,21 +438,6 @@ struct Running {
   }
 };
 
-// Four neighbouring values of a result, registers r .. r + 3 times `by`; true if one is no number.
-template <typename T>
-__device__ __forceinline__ bool put_four(T *to, const f32x16 &from, int r, float by) {
-  f32x4 value;
-  bool odd = false;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    value[j] = from[r + j] * by;
-    odd |= !(__builtin_fabsf(value[j]) < INFINITY);
-  }
-  typedef T V __attribute__((ext_vector_type(4)));
-  *reinterpret_cast<V *>(to) = __builtin_convertvector(value, V);
-  return odd;
-}
-
 // What the two kernels of the gradient need of each row, made in one pass over out, grad and v:
 //   level_i = lse_i - shift             exp2(s_i - level_i) = 2^shift P_i
 //   delta_i = grad_i . out_i            (with what the rounding of out took off)
@@ -538,15 +548,17 @@ struct Pulled {
   __device__ __forceinline__ float by(const Attention &p) const { return sizeof(T) == 2 ? p.scale / unit.by * 0x1p-14f : p.scale; }  // 2^-kShift
 };
 
-// f(head dimension in whole parts of 32, whether scores are bent), both known to the compiler.
-template <typename F>
+// f(head dimension in whole parts of 32, above 128 as 256 (float16 only), whether scores are bent), both known to the compiler.
+template <typename T, typename F>
 void with_shape(const Attention &p, F f) {
   auto with_dim = [&](auto bent) {
     switch ((p.D + 31) / 32) {
       case 1: return f(std::integral_constant<int, 32>{}, bent);
       case 2: return f(std::integral_constant<int, 64>{}, bent);
       case 3: return f(std::integral_constant<int, 96>{}, bent);
-      default: return f(std::integral_constant<int, 128>{}, bent);
+      case 4: return f(std::integral_constant<int, 128>{}, bent);
+      default:
+        if constexpr (sizeof(T) == 2) return f(std::integral_constant<int, 256>{}, bent);
     }
   };
   p.cap > 0 ? with_dim(std::true_type{}) : with_dim(std::false_type{});

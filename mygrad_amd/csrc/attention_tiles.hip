@@ -16,7 +16,7 @@ namespace {
 constexpr int kBlockRows = 128;  // queries of a block: 32 for each of its four wavefronts
 
 template <typename T, int DP, int KEYS, bool BENT>
-__global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T *__restrict__ k,
+__global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T *__restrict__ k,
                                                                  const T *__restrict__ v, T *__restrict__ out, _Float16 *__restrict__ rest,
                                                                  float *__restrict__ lse) {
   typedef TileOf<T, DP, KEYS> Tile;
@@ -52,8 +52,8 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
     const long long from = (long long)t * KEYS * stride;
     const int last = hi - lo - t * KEYS;
     const unsigned to = lds + (unsigned)(t & 1) * (2 * Tile::kBytes);
-    load(kb + from, stride, last, to);
-    load(vb + from, stride, last, to + Tile::kBytes);
+    load(kb + from, last, to);
+    load(vb + from, last, to + Tile::kBytes);
   };
 
   Running<T, DP, KEYS / 32, BENT, false> run;
@@ -83,19 +83,10 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
       for (int r = 0; r < 16; r += 4) {
         const int d = 32 * n + row_of(r, h);
         if (d >= p.D) continue;
-        f32x4 value;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          value[j] = run.sums[n][r + j] * by;
-          odd |= !(__builtin_fabsf(value[j]) < INFINITY);
-        }
-        if constexpr (sizeof(T) == 2) {
-          const f16x4 near = __builtin_convertvector(value, f16x4);
-          *reinterpret_cast<f16x4 *>(out + to + d) = near;
-          if (rest) *reinterpret_cast<f16x4 *>(rest + to + d) = __builtin_convertvector((value - __builtin_convertvector(near, f32x4)) * kRest, f16x4);
-        } else {
-          *reinterpret_cast<f32x4 *>(out + to + d) = value;
-        }
+        const f32x4 value = four_of(run.sums[n], r) * by;
+        odd |= put_four(out + to + d, value);
+        if constexpr (sizeof(T) == 2)
+          if (rest) put_four(rest + to + d, (value - __builtin_convertvector(__builtin_convertvector(value, f16x4), f32x4)) * kRest);
       }
     if (lse && h == 0) lse[((long long)b * p.HQ + hq) * p.TQ + i] = total == 0 ? INFINITY : run.top + __builtin_log2f(total) - kLift;
   }
@@ -108,11 +99,6 @@ __global__ void __launch_bounds__(256, 2) attention_tiles_kernel(Attention p, De
 }
 
 // ---- gradient ----------------------------------------------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ f32x8 eight(const T *from) {
-  return __builtin_convertvector(*reinterpret_cast<const typename Fragment<T>::V *>(from), f32x8);
-}
-
 // Sixteen lanes a row, eight values each.
 __device__ __forceinline__ float sum16(float v) {
 #pragma unroll
@@ -123,18 +109,20 @@ __device__ __forceinline__ float sum16(float v) {
 template <typename T>
 __global__ void __launch_bounds__(256) attention_stats_kernel(Attention p, Stats stats, const T *__restrict__ out, const _Float16 *__restrict__ rest,
                                                               const float *__restrict__ lse, const T *__restrict__ grad) {
-  const int lane = threadIdx.x & 15, group = threadIdx.x >> 4, d = lane * 8;
+  const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
   const int bh = blockIdx.x / stats.chunks, chunk = blockIdx.x % stats.chunks, b = bh / p.HQ, h = bh % p.HQ;
   for (int n = group; n < stats.rows; n += 16) {
     const int i = chunk * stats.rows + n;
     float dot = 0;
-    if (i < p.TQ && d < p.D) {
-      const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D + d;
-      const f32x8 g = eight(grad + at);
-      f32x8 o = eight(out + at);
-      if (rest) o += eight(rest + at) * (1.0f / kRest);
+    if (i < p.TQ) {
+      const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
+      for (int d = lane * 8; d < p.D; d += 128) {
+        const f32x8 g = __builtin_convertvector(fragment_of(grad + at, d, p.D, true), f32x8);
+        f32x8 o = __builtin_convertvector(fragment_of(out + at, d, p.D, true), f32x8);
+        if (rest) o += __builtin_convertvector(fragment_of(rest + at, d, p.D, true), f32x8) * (1.0f / kRest);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dot += g[j] * o[j];
+        for (int j = 0; j < 8; ++j) dot += g[j] * o[j];
+      }
     }
     dot = sum16(dot);
     if (i < p.TQ && lane == 0) {
@@ -163,7 +151,7 @@ __global__ void __launch_bounds__(256) attention_stats_kernel(Attention p, Stats
 
 // dq^T = K^T dS^T: as the forward pass, with the queries' rows of grad beside those of q.
 template <typename T, int DP, int KEYS, bool BENT>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
+__global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 64 : 128) ? 1 : 2) attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
                                                               const T *__restrict__ v, const T *__restrict__ grad, const float *__restrict__ lse,
                                                               T *__restrict__ dq) {
   typedef TileOf<T, DP, KEYS> Tile;
@@ -204,8 +192,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
     const long long from = (long long)t * KEYS * stride;
     const int last = hi - lo - t * KEYS;
     const unsigned to = lds + (unsigned)(t & 1) * (2 * Tile::kBytes);
-    load(kb + from, stride, last, to);
-    load(vb + from, stride, last, to + Tile::kBytes);
+    load(kb + from, last, to);
+    load(vb + from, last, to + Tile::kBytes);
   };
 
   Pulled<T, DP, KEYS, BENT> run;
@@ -234,7 +222,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const int d = 32 * n + row_of(r, h);
-        if (d < p.D) odd |= put_four(dq + row + d, run.sums[n], r, by);
+        if (d < p.D) odd |= put_four(dq + row + d, four_of(run.sums[n], r) * by);
       }
   }
   odd = __any(odd);
@@ -251,8 +239,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
 // With VALUES the keys' values lie in LDS instead of registers: at 128 values of float16 a head the two results and k take 160 of a lane's 256,
 // and with v's 32 as well the scores would not fit.
 template <typename T, int DP, int ROWS, bool VALUES, bool BENT>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
-                                                               const T *__restrict__ v, const T *__restrict__ grad, const float *__restrict__ lse,
+__global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 64 : 128) ? 1 : 2)
+attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const T *__restrict__ grad, const float *__restrict__ lse,
                                                                T *__restrict__ dk, T *__restrict__ dv, int cuts, float *__restrict__ parts) {
   typedef TileOf<T, DP, ROWS> Tile;
   typedef typename Fragment<T>::V V;
@@ -323,8 +311,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
   auto stage = [&](int chunk, unsigned to) {
     const int first = chunk * ROWS;
     const long long from = (((long long)b * p.TQ + first) * p.HQ + head) * p.D * (long long)sizeof(T);
-    load((const char *)q + from, stride, p.TQ - first, to);
-    load((const char *)grad + from, stride, p.TQ - first, to + Tile::kBytes);
+    load((const char *)q + from, p.TQ - first, to);
+    load((const char *)grad + from, p.TQ - first, to + Tile::kBytes);
     const long long stat = ((long long)b * p.HQ + head) * p.TQ + first, span = (long long)b * p.TQ + first;
     const char *from_stats = wave == 0 ? (const char *)(stats.level + stat) : wave == 1 ? (const char *)(stats.delta + stat)
                            : wave == 2 ? (const char *)(stats.lo + span) : (const char *)(stats.hi + span);
@@ -338,7 +326,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
   if constexpr (VALUES) {
     const unsigned key_stride = (unsigned)(p.HK * p.D) * (unsigned)sizeof(T);
     const typename Whole::template Loader<256> load_values(key_stride, (unsigned)p.D * (unsigned)sizeof(T));
-    load_values((const char *)v + (((long long)b * p.TK + block0) * p.HK + hk) * p.D * (long long)sizeof(T), key_stride, p.TK - block0, whole_values);
+    load_values((const char *)(v + (((long long)b * p.TK + block0) * p.HK + hk) * p.D), p.TK - block0, whole_values);
   }
   unsigned side = 0;
   int chunk = 0, hq = 0;
@@ -348,6 +336,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
     stage(chunk, lds);
   }
   all_landed();
+  if constexpr (VALUES)
+    if (p.D % 8 && h == 0)  // the second half of a row's last piece came from behind the row, and from behind the rows of grad there, too
+      *(MG_LDS unsigned long long *)(unsigned long long)(whole_values + (unsigned)(wave * 32 + c) * Whole::kRowBytes +
+                                                         (unsigned)((p.D / 8) ^ Whole::turn(c)) * 16u + 8u) = 0;
   for (int n = 0; n < count; ++n) {
     const int first = chunk * ROWS, this_hq = hq;
     const Reach reach = reaches[chunk];
@@ -419,12 +411,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
         const int d = 32 * n + row_of(r, h);
         if (d >= p.D) continue;
         if (cuts == 1) {
-          odd |= put_four(dk + row + d, sum_k[n], r, by);
-          odd |= put_four(dv + row + d, sum_v[n], r, lift);
+          odd |= put_four(dk + row + d, four_of(sum_k[n], r) * by);
+          odd |= put_four(dv + row + d, four_of(sum_v[n], r) * lift);
         } else {
           const long long all = (long long)p.B * p.TK * p.HK * p.D;
-          put_four(parts + at.head * all + row + d, sum_k[n], r, by);
-          put_four(parts + (cuts + at.head) * all + row + d, sum_v[n], r, lift);
+          put_four(parts + at.head * all + row + d, four_of(sum_k[n], r) * by);
+          put_four(parts + (cuts + at.head) * all + row + d, four_of(sum_v[n], r) * lift);
         }
       }
   }
@@ -454,12 +446,9 @@ __global__ void __launch_bounds__(256) attention_dkv_join_kernel(Attention p, St
     const int which = n / (kJoinKeys * of_row), rest = n - which * kJoinKeys * of_row, j = tile * kJoinKeys + rest / of_row;
     if (j >= p.TK) continue;
     const long long at = (((long long)b * p.TK + j) * p.HK + hk) * p.D + rest % of_row * 4;
-    f32x4 sum = *(const f32x4 *)(parts + which * cuts * all + at);
-    for (int m = 1; m < cuts; ++m) sum += *(const f32x4 *)(parts + (which * cuts + m) * all + at);
-    typedef T V __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<V *>((which ? dv : dk) + at) = __builtin_convertvector(sum, V);
-#pragma unroll
-    for (int m = 0; m < 4; ++m) odd |= !(__builtin_fabsf(sum[m]) < INFINITY);
+    f32x4 sum{};
+    for (int m = 0; m < cuts; ++m) sum += *(const f32x4 *)(parts + (which * cuts + m) * all + at);
+    odd |= put_four((which ? dv : dk) + at, sum);
   }
   odd = __any(odd);
   if ((threadIdx.x & 63) == 0) bad[threadIdx.x >> 6] = odd;
@@ -502,7 +491,7 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
   void *space = nullptr;
   int rc = workspace(sums + sizeof(Reach) * chunks + 4 * (2 * all + 2 * rows), &space);
   if (rc) return rc;
-  float *partial = (float *)space;  // whole pieces of 16 bytes: dim is a multiple of 8
+  float *partial = (float *)space;  // whole pieces of 16 bytes: dim is a multiple of 4
   stats.reach = (Reach *)((char *)space + sums);
   stats.level = (float *)(stats.reach + chunks);
   stats.delta = stats.level + all;
@@ -522,8 +511,8 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
   } else if (dq) {
     ScopedTiming timed(TAG_ATTENTION_DQ);
     const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
-    with_shape(p, [&](auto dim, auto bent) {
-      attention_dq_kernel<T, dim, ROWS, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, s>>>(p, deal, stats, tq, tk, tv, tg, tl,
+    with_shape<T>(p, [&](auto dim, auto bent) {
+      attention_dq_kernel<T, dim, dim <= 128 ? ROWS : 32, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, s>>>(p, deal, stats, tq, tk, tv, tg, tl,
                                                                                                                        (T *)dq);
     });
     MG_HIP(hipGetLastError());
@@ -532,8 +521,8 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
   {
     ScopedTiming timed(TAG_ATTENTION_DKV);
     const Deal deal{p.B * p.HK, cuts, key_tiles};
-    with_shape(p, [&](auto dim, auto bent) {
-      constexpr bool wide = sizeof(T) == 2 && dim == 128;
+    with_shape<T>(p, [&](auto dim, auto bent) {
+      constexpr bool wide = sizeof(T) == 2 && dim >= 128;
       attention_dkv_kernel<T, dim, wide ? 32 : ROWS, wide, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, s>>>(
           p, deal, stats, tq, tk, tv, tg, tl, (T *)dk, (T *)dv, cuts, partial);
     });
@@ -549,9 +538,10 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
 
 }  // namespace
 
-// Head dimensions up to 128 in whole fragments, from buffers that start on 16 bytes, rows of a tile within reach of 32 bits.
+// Head dimensions that are multiples of 4, up to 128 or, in float16, 256, in buffers that start on 16 bytes, rows of a tile within reach
+// of 32 bits.
 bool tiles_take(const Attention &p, int size, uintptr_t ends) {
-  return p.D <= 128 && p.D % 8 == 0 && ends % 16 == 0 && (long long)p.HQ * p.D * size * 128 < (1ll << 31) &&
+  return p.D <= (size == 2 ? 256 : 128) && p.D % 4 == 0 && ends % 16 == 0 && (long long)p.HQ * p.D * size * 128 < (1ll << 31) &&
          (long long)p.B * p.HQ * ceil_div(p.TQ, 32) < (1 << 24) && (long long)p.B * p.HK * ceil_div(p.TK, 32) < (1 << 24);
 }
 
@@ -569,8 +559,8 @@ int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, c
   const dim3 grid((unsigned)(deal.pairs * deal.heads * deal.tiles));
   auto launch = [&](auto zero) {
     using T = decltype(zero);
-    with_shape(p, [&](auto dim, auto bent) {
-      attention_tiles_kernel<T, dim, sizeof(T) == 2 ? 64 : 32, bent><<<grid, dim3(256), 0, runtime().stream>>>(
+    with_shape<T>(p, [&](auto dim, auto bent) {
+      attention_tiles_kernel<T, dim, sizeof(T) == 2 && dim <= 128 ? 64 : 32, bent><<<grid, dim3(256), 0, runtime().stream>>>(
           p, deal, (const T *)q, (const T *)k, (const T *)v, (T *)out, (_Float16 *)rest, (float *)lse);
     });
   };

@@ -97,6 +97,34 @@ def test_lengths_and_head_dimensions(dtype, TQ, TK, D):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("TQ,TK,D", [(3, 70, 4), (40, 300, 36), (130, 90, 100), (200, 200, 132), (70, 140, 160), (9, 900, 252), (300, 300, 256), (50, 50, 34)])
+def test_head_dimensions_that_fill_no_tile(dtype, TQ, TK, D):
+    _check(dtype, 1, TQ, TK, 2, 2, D)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("TQ,TK,HQ,HK,D,mask", [
+    (900, 900, 8, 1, 64, dict(causal=True)), (700, 700, 6, 2, 128, dict(causal=True, prefix=200)), (1000, 300, 2, 1, 32, dict()),
+    (60, 1500, 2, 1, 64, dict()), (100, 800, 4, 2, 96, dict(causal=True)), (640, 640, 4, 1, 256, dict(causal=True, window=100)),
+    (500, 500, 4, 1, 80, dict(documents=np.repeat([3, 1, 2, 0], [250, 3, 90, 157])))])
+def test_few_heads_over_long_rows(dtype, TQ, TK, HQ, HK, D, mask):
+    """Work is split along the keys, or the queries of one key, where there are few blocks of it."""
+    _check(dtype, 1, TQ, TK, HQ, HK, D, **mask)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_mask_for_several_shapes(dtype):
+    rng = np.random.default_rng(41)
+    mask = AttentionMask(causal=True, lengths=[40, 3])
+    for TQ, TK, HQ, HK, D in ((8, 50, 2, 1, 32), (50, 40, 4, 2, 64), (8, 50, 2, 1, 32)):
+        q, k, v = (rng.standard_normal(shape).astype(dtype) for shape in ((2, TQ, HQ, D), (2, TK, HK, D), (2, TK, HK, D)))
+        seen = ora.visible(2, TQ, TK, causal=True, lengths=[40, 3])
+        want, p, (s, bent) = ora.forward(q, k, v, seen, lengths=[40, 3])
+        bar = _bounds(dtype, q, k, v, None, p, s, bent, want, None, D**-0.5, None)[0]
+        assert (np.abs(attention(q, k, v, mask=mask).data.astype(np.float64) - want) <= bar).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("HQ,HK", [(1, 1), (3, 3), (6, 2), (8, 1)])
 def test_heads_that_share_keys(dtype, HQ, HK):
     _check(dtype, 3, 70, 70, HQ, HK, 64, causal=True)
@@ -206,6 +234,31 @@ def test_what_a_query_does_not_see_does_not_touch_it(dtype, bad, D):
             assert np.isfinite(dirty[n][where]).all(), n
             assert np.allclose(dirty[n][where], clean[n][where], rtol=4 * UNIT[dtype][1], atol=max(64 * UNIT[dtype][1], 1024 * UNIT[dtype][0]))
         assert not dirty[0][~seen.any(-1)].any()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("T,D", [(700, 36), (600, 128), (20, 64), (20, 100)])
+def test_documents_of_no_numbers_beside_others_where_work_is_split(dtype, T, D):
+    rng = np.random.default_rng([T, D])
+    HQ, HK = 4, 1
+    q, k, v, g = (rng.standard_normal((1, T, H, D)).astype(dtype) for H in (HQ, HK, HK, HQ))
+    middle = slice(T // 3, T // 2)
+    documents = np.zeros(T, dtype=np.int64)
+    documents[middle], documents[T // 2:] = 1, 2
+    results = []
+    for spoil in (False, True):
+        ops = [a.copy() for a in (q, k, v, g)]
+        if spoil:
+            for a in ops:
+                a[:, middle] = np.nan
+        tensors = [mg.device_tensor(a) for a in ops]
+        out = attention(*tensors[:3], mask=AttentionMask(causal=True, documents=documents))
+        out.backward(tensors[3])
+        results.append([out.data] + [t.grad for t in tensors[:3]])
+    rows = documents != 1
+    for clean, dirty in zip(*results):
+        assert np.isnan(dirty[0, ~rows]).any() and np.isfinite(dirty[0, rows]).all()
+        assert np.allclose(dirty[0, rows], clean[0, rows], rtol=4 * UNIT[dtype][1], atol=max(64 * UNIT[dtype][1], 1024 * UNIT[dtype][0]))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -318,6 +371,24 @@ def test_one_long_history_among_short_ones(dtype):
         want, p, (s, bent) = ora.forward(q[b:b + 1], k, v, seen)
         bar = _bounds(dtype, q[b:b + 1], k, v, None, p, s, bent, want, None, D**-0.5, None)[0]
         assert (np.abs(out[b:b + 1].astype(np.float64) - want) <= bar).all()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("HK,D", [(1, 128), (1, 7)])
+def test_offsets_beyond_32_bits(dtype, HK, D):
+    """The last tokens of a cache with more than 2^32 bytes and, at 128 values a head, 2^31 values."""
+    rng = np.random.default_rng(D)
+    capacity = (1 << 24) + 77 if D == 128 else (1 << 32) // (D * np.dtype(dtype).itemsize) + 1000
+    seen_tokens, T = 300, 2
+    cache = KeyValueCache(1, capacity, HK, D, dtype=dtype)
+    make = lambda *shape: rng.standard_normal(shape).astype(dtype)
+    k, v, q = make(1, seen_tokens, HK, D), make(1, seen_tokens, HK, D), make(1, T, 2 * HK, D)
+    cache.write(k, v, AttentionMask(causal=True, lengths=[capacity]))
+    out = cache.attend(q, mask=AttentionMask(causal=True, window=seen_tokens - T, lengths=[capacity])).data
+    seen = ora.visible(1, T, seen_tokens, causal=True, window=seen_tokens - T)
+    want, p, (s, bent) = ora.forward(q, k, v, seen)
+    bar = _bounds(dtype, q, k, v, None, p, s, bent, want, None, D**-0.5, None)[0]
+    assert (np.abs(out.astype(np.float64) - want) <= bar).all()
 
 
 def test_cache_refusals():
