@@ -160,7 +160,7 @@ def _describe(q, k, v, scale, cap, slopes, mask):
     elif not isinstance(mask, AttentionMask):
         raise TypeError(f"`mask` must be an AttentionMask, got {type(mask).__name__}")
     held = _slopes_on_device(slopes, q.shape[2]) if slopes is not None and q.ndim == 4 else None
-    key = q.shape, k.shape, v.shape, q.dtype, k.dtype, v.dtype, scale, cap, None if held is None else held.ptr
+    key = q.shape, k.shape, v.shape, q.dtype, k.dtype, v.dtype, scale, cap
     desc = mask._described.get(key)
     if desc is None:
         _check_operands(q, k, v)
@@ -172,10 +172,13 @@ def _describe(q, k, v, scale, cap, slopes, mask):
         pointers = mask._bind(batch, queries, keys)
         longest = 0 if mask._lengths is None else max(mask.longest, 1)
         desc = _hip.AttentionDesc(_hip.storage_code(q.dtype), mask.causal, batch, queries, keys, heads, kv_heads, dim, mask.window, scale, cap, longest,
-                                  *pointers, key[-1])
+                                  *pointers, None)
         if len(mask._described) >= 64:
             mask._described.clear()
         mask._described[key] = desc
+    if held is not None:
+        desc = _hip.AttentionDesc.from_buffer_copy(desc)
+        desc.slopes = held.ptr
     return desc, held
 
 
