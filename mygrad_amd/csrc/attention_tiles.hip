@@ -70,6 +70,8 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attention_tiles_kernel(
       run.take(p, how, keys, keys + Tile::kBytes, rows, span, key0, key0 >= reach.all_lo && key0 + KEYS <= reach.all_hi, place, h);
     }
     all_landed();
+#pragma unroll
+    for (int n = 0; n < kParts; ++n) asm volatile("" : "+v"(run.sums[n]));  // one set of registers, whichever way a round went
   }
 
   const float total = sum_halves(run.total);
