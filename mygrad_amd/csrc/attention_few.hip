@@ -4,7 +4,9 @@
 // that makes few blocks still, the keys are split among blocks, which are joined by a second launch.
 //
 // With a step of generation over a cache this is bound by reading keys and values once: the sixteen products of a tile (128 values a head, float16)
-// wait for its bytes even where most columns are empty.
+// wait for its bytes even where most columns are empty.  32 histories of 4000 to 8000 tokens, 32 heads over 8 of 128 in float16 (787 MB): 157 us and 7 to
+// join, 5.0 TB/s (a stream that only reads reaches 6.25, a copy 5.2); one history of 131001 tokens with a cap (537 MB): 128 and 12, 4.2 TB/s;
+// weights in two parts cost 4% of that.  A block holds 128 KB of tiles, one block a compute unit: four wavefronts with 16 KB each on the way.
 #include "attention_tiles.h"
 
 #include "attention_row.h"

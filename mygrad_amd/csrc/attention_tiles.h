@@ -286,7 +286,7 @@ __device__ __forceinline__ typename Fragment<T>::V rows_of(const f32x16 &v, int 
 
 // a times both: a float32 value in two of float16 keeps 22 bits (one is all of it in float32).  Gradients of scores are multiplied so: rounded to 11
 // bits they would make dq and dk off by half as much again as the rounding of the results does, which costs a fifth of dq's time and a
-// fourteenth of dk's and dv's (8192 packed tokens: 161 against 192 us, 291 against 315).  Weights are rounded once where products are the bound
+// fourteenth of dk's and dv's (8192 packed tokens: 161 us against 192, 291 against 315, as both were then).  Weights are rounded once where products are the bound
 // (a block of 128 queries: results are off by 1.2 to 1.4 times their own rounding), and kept in two where bytes are.
 template <typename T>
 __device__ __forceinline__ f32x16 mma_of_two(typename Fragment<T>::V a, typename Fragment<T>::V b, typename Fragment<T>::V more, f32x16 c) {
@@ -354,8 +354,7 @@ __device__ __forceinline__ Scores scores_of(const Attention &p, int head) {
 
 // 32 queries, one in each lane's column (in both halves), on their way through tiles of SUBS times 32 keys: S^T = K Q^T has a query's scores in
 // its lane (and the partner in the other half), so maximum and sum need no exchange but that one, and the weights are the right operand of
-// out^T = V^T P^T as they lie.  BENT: scores have a cap (whose registers the others do
-// without).  FINE: float16 takes weights in two.
+// out^T = V^T P^T as they lie.  BENT: scores have a cap (whose registers the others do without).  FINE: float16 takes weights in two.
 template <typename T, int DP, int SUBS, bool BENT, bool FINE>
 struct Running {
   typedef TileOf<T, DP, 32 * SUBS> Tile;
@@ -580,21 +579,35 @@ void with_shape(const Attention &p, F f) {
 }
 
 // How the blocks of a launch are dealt out: `pairs` of a batch item and a key head, each with `heads` query heads and `tiles` row tiles.
-// Blocks go to the eight XCDs in turn, so with a multiple of eight pairs each pair stays on one XCD and is read through one L2.  The
-// last tiles, which see most where the mask is causal, come first.
+// Blocks go to the eight XCDs in turn, so with a multiple of eight pairs each pair stays on one XCD and is read through one L2.  The last tiles,
+// which see most where the mask is causal, come first: of one pair after the other where one fills an XCD, else of as many as do.  Where all
+// blocks run at once, two on a compute unit, the second half comes the other way round, so that the unit with most of the first gets least of
+// it: 2 x 4096 causal tokens, 16 heads of 128 in float16, dk and dv 495 to 425 us, dq 327 to 303, forward 197 to 190; 4 x 1024 behind a prefix, 8
+// heads of 64 in float32, dk and dv 144 to 101.
 struct Deal {
   int pairs, heads, tiles;
+  int beside;  // pairs of an XCD whose tiles are dealt in turn
+  int folded;  // blocks, where all of them run at once; else 0
 };
 
 struct Dealt {
   int pair, head, tile;
 };
 
+inline Deal deal_of(int pairs, int heads, int tiles) {
+  const int units = runtime().props.multiProcessorCount, blocks = pairs * heads * tiles;
+  return Deal{pairs, heads, tiles, std::max(1, std::min(pairs / 8, (int)ceil_div(units / 4, heads * tiles))), blocks > units && blocks <= 2 * units ? blocks : 0};
+}
+
 __device__ __forceinline__ Dealt dealt(const Deal &d, int block) {
-  const int each = d.heads * d.tiles;
+  if (d.folded && block >= d.folded / 2) {  // in eights, as the XCDs take them
+    const int first = (d.folded / 2 + 7) / 8 * 8, last = d.folded / 8 * 8;
+    if (block >= first && block < last) block = first + (last - 8 - (block & ~7)) + (block & 7);
+  }
   if (d.pairs % 8 == 0) {
-    const int turn = block >> 3, pair = turn / each, rest = turn - pair * each;
-    return Dealt{pair * 8 + (block & 7), rest % d.heads, d.tiles - 1 - rest / d.heads};
+    const int each = d.heads * d.tiles, turn = block >> 3, of_group = d.beside * each, group = turn / of_group, rest = turn - group * of_group;
+    const int many = min(d.beside, d.pairs / 8 - group * d.beside) * d.heads, tile = rest / many, at = rest - tile * many;
+    return Dealt{(group * d.beside + at / d.heads) * 8 + (block & 7), at % d.heads, d.tiles - 1 - tile};
   }
   const int many = d.pairs * d.heads, tile = block / many, rest = block - tile * many;
   return Dealt{rest / d.heads, rest % d.heads, d.tiles - 1 - tile};

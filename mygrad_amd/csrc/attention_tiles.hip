@@ -15,10 +15,16 @@ namespace {
 
 constexpr int kBlockRows = 128;  // queries of a block: 32 for each of its four wavefronts
 
+// The forward pass: 4 D operations for each query and key, on the matrix cores with the softmax's exponentials beside them.  Four wavefronts of 32
+// queries share the tiles of keys and values, the next ones on their way while these are multiplied; 64 keys in two buffers are 64 KB at 128
+// values of float16, so two blocks share a compute unit and one's products run while the other takes exponentials (with half of the unit's
+// queries gone, as at the end of a causal launch, three fifths of the rate are left).  Float32's products take eight times as long: 32 keys do.
+// 2 x 4096 tokens, 16 heads of 128, float16: 314 us (875 TFLOP/s; a large product reaches 1168), causal 190 (720), with a cap 400 (687); of 64:
+// 188 (730).  2 x 2048, 8 heads of 128, float32: 303 (113; a large product 154).
 template <typename T, int DP, int KEYS, bool BENT>
-__global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T *__restrict__ k,
-                                                                 const T *__restrict__ v, T *__restrict__ out, _Float16 *__restrict__ rest,
-                                                                 float *__restrict__ lse) {
+__global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
+attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, T *__restrict__ out,
+                       _Float16 *__restrict__ rest, float *__restrict__ lse) {
   typedef TileOf<T, DP, KEYS> Tile;
   typedef typename Fragment<T>::V V;
   constexpr int kSteps = DP / 16, kParts = DP / 32;
@@ -101,13 +107,13 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attention_tiles_kernel(
 }
 
 // ---- gradient ----------------------------------------------------------------------------------------------------------------
-// Sixteen lanes a row, eight values each.
 __device__ __forceinline__ float sum16(float v) {
 #pragma unroll
   for (int m = 8; m; m >>= 1) v += __shfl_xor(v, m);
   return v;
 }
 
+// Sixteen lanes a row, eight values each at a time.  Bound by reading out, what it left over and grad: 100 MB in 20 us, 5 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_stats_kernel(Attention p, Stats stats, const T *__restrict__ out, const _Float16 *__restrict__ rest,
                                                               const float *__restrict__ lse, const T *__restrict__ grad) {
@@ -151,11 +157,14 @@ __global__ void __launch_bounds__(256) attention_stats_kernel(Attention p, Stats
   if (threadIdx.x == 0) stats.reach[(long long)b * stats.chunks + chunk] = r;
 }
 
-// dq^T = K^T dS^T: as the forward pass, with the queries' rows of grad beside those of q.
+// dq^T = K^T dS^T: as the forward pass, with the queries' rows of grad beside those of q; S and dP are formed again here and by the keys'
+// kernel, two of seven products more than one kernel would need, which would have to add to dq or to dk and dv across blocks, in no order.
+// Bound by the matrix cores: 2 x 4096 tokens, 16 heads of 128, float16: 530 us (1040 TFLOP/s, dS in two counted), causal 303; float32, 2 x 2048, 8
+// heads of 128: 430 (120 of 154).
 template <typename T, int DP, int KEYS, bool BENT>
-__global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 64 : 128) ? 1 : 2) attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
-                                                              const T *__restrict__ v, const T *__restrict__ grad, const float *__restrict__ lse,
-                                                              T *__restrict__ dq) {
+__global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 64 : 128) ? 1 : 2)
+attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                    const T *__restrict__ grad, const float *__restrict__ lse, T *__restrict__ dq) {
   typedef TileOf<T, DP, KEYS> Tile;
   typedef typename Fragment<T>::V V;
   constexpr int kSteps = DP / 16, kParts = DP / 32, kSubs = KEYS / 32;
@@ -238,12 +247,16 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 64 : 128) ? 1 : 2)
 // dv^T = grad^T P and dk^T = q^T dS: a block keeps 128 keys, 32 for each wavefront in its lanes' columns, and goes through the chunks of queries
 // that see any of them, head by head of those that share the keys.  Where there are few blocks they are cut: each of `cuts` takes an equal share
 // of the chunks and leaves its sums in float32, which attention_dkv_join_kernel adds up in order.
+// Bound by the matrix cores: 2 x 4096 tokens, 16 heads of 128, float16: 712 us (1160 TFLOP/s, dS in two counted), causal 425; float32, 2 x 2048,
+// 8 heads of 128: 620 (111 of 154).  Two causal halves that end at different times, and documents that do, leave units idle: 8192 tokens of five
+// documents, 16 heads of 128, take 297 us where even work would take 170; cut in two they would leave 134 MB of sums to be joined in 80 us.
 // With VALUES the keys' values lie in LDS instead of registers: at 128 values of float16 a head the two results and k take 160 of a lane's 256,
 // and with v's 32 as well the scores would not fit.
 template <typename T, int DP, int ROWS, bool VALUES, bool BENT>
 __global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 64 : 128) ? 1 : 2)
-attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const T *__restrict__ grad, const float *__restrict__ lse,
-                                                               T *__restrict__ dk, T *__restrict__ dv, int cuts, float *__restrict__ parts) {
+attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                     const T *__restrict__ grad, const float *__restrict__ lse, T *__restrict__ dk, T *__restrict__ dv, int cuts,
+                     float *__restrict__ parts) {
   typedef TileOf<T, DP, ROWS> Tile;
   typedef typename Fragment<T>::V V;
   constexpr int kSteps = DP / 16, kParts = DP / 32, kSubs = ROWS / 32;
@@ -433,7 +446,8 @@ attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ 
 
 constexpr int kJoinKeys = 16;
 
-// Adds the cuts' sums in their order, four values a thread; a block takes sixteen keys of one head.
+// Adds the cuts' sums in their order, four values a thread; a block takes sixteen keys of one head.  Bound by reading them: 4 x 2048 keys, 4 heads
+// of 128 in four cuts, 134 MB and 17 written, 29 us (5.2 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) attention_dkv_join_kernel(Attention p, Stats stats, int tiles, int cuts, const float *__restrict__ parts,
                                                                  const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
@@ -512,17 +526,17 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
     if (rc) return rc;
   } else if (dq) {
     ScopedTiming timed(TAG_ATTENTION_DQ);
-    const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
+    const Deal deal = deal_of(p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows));
     with_shape<T>(p, [&](auto dim, auto bent) {
-      attention_dq_kernel<T, dim, dim <= 128 ? ROWS : 32, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, s>>>(p, deal, stats, tq, tk, tv, tg, tl,
-                                                                                                                       (T *)dq);
+      attention_dq_kernel<T, dim, dim <= 128 ? ROWS : 32, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, s>>>(
+          p, deal, stats, tq, tk, tv, tg, tl, (T *)dq);
     });
     MG_HIP(hipGetLastError());
   }
   if (!dk) return MG_OK;
   {
     ScopedTiming timed(TAG_ATTENTION_DKV);
-    const Deal deal{p.B * p.HK, cuts, key_tiles};
+    const Deal deal = deal_of(p.B * p.HK, cuts, key_tiles);
     with_shape<T>(p, [&](auto dim, auto bent) {
       constexpr bool wide = sizeof(T) == 2 && dim >= 128;
       attention_dkv_kernel<T, dim, wide ? 32 : ROWS, wide, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, s>>>(
@@ -532,8 +546,9 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
   }
   if (cuts == 1) return MG_OK;
   ScopedTiming timed(TAG_ATTENTION_JOIN);
-  attention_dkv_join_kernel<T><<<dim3((unsigned)(p.B * p.HK * ceil_div(p.TK, kJoinKeys))), dim3(256), 0, s>>>(p, stats, (int)ceil_div(p.TK, kJoinKeys), cuts, partial, tq, tk, tv, tg, tl, (T *)dk,
-                                                                                            (T *)dv);
+  const int join_tiles = (int)ceil_div(p.TK, kJoinKeys);
+  attention_dkv_join_kernel<T><<<dim3((unsigned)(p.B * p.HK * join_tiles)), dim3(256), 0, s>>>(p, stats, join_tiles, cuts, partial, tq, tk, tv, tg, tl, (T *)dk,
+                                                                                               (T *)dv);
   MG_HIP(hipGetLastError());
   return MG_OK;
 }
@@ -541,7 +556,8 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
 }  // namespace
 
 // Head dimensions that are multiples of 4, up to 128 or, in float16, 256, in buffers that start on 16 bytes, rows of a tile within reach
-// of 32 bits.
+// of 32 bits.  Of 256 values a block has a compute unit to itself: 2048 causal tokens, 8 heads over 2, float16, 140 us forward, 255 dq, 259 dk and
+// dv (128 blocks; 3127, 3472 and 24976 us a row at a time).
 bool tiles_take(const Attention &p, int size, uintptr_t ends) {
   return p.D <= (size == 2 ? 256 : 128) && p.D % 4 == 0 && ends % 16 == 0 && (long long)p.HQ * p.D * size * 128 < (1ll << 31) &&
          (long long)p.B * p.HQ * ceil_div(p.TQ, 32) < (1 << 24) && (long long)p.B * p.HK * ceil_div(p.TK, 32) < (1 << 24);
@@ -557,7 +573,7 @@ bool few_take(const Attention &p, int size) {
 
 int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
   ScopedTiming timed(TAG_ATTENTION);
-  const Deal deal{p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows)};
+  const Deal deal = deal_of(p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows));
   const dim3 grid((unsigned)(deal.pairs * deal.heads * deal.tiles));
   auto launch = [&](auto zero) {
     using T = decltype(zero);
