@@ -35,7 +35,7 @@ attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T 
   const Dealt at = dealt(deal, blockIdx.x);
   const int b = at.pair / p.HK, hk = at.pair % p.HK, hq = hk * p.group + at.head;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
-  const int i = at.tile * kBlockRows + wave * 32 + c;
+  const int tile = tile_of_rank<false>(p, b, deal.tiles - 1 - at.tile, deal.tiles, kBlockRows), i = tile * kBlockRows + wave * 32 + c;
   const bool in = i < p.TQ;
   const Span span = in ? span_of(p, b, i) : Span{0, 0, 0};
   const Reach reach = reach_of(span, in);
@@ -102,7 +102,7 @@ attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T 
   if (lane == 0) bad[wave] = odd;
   all_landed();  // what is stored, too: other wavefronts may write it again
   if (bad[0] | bad[1] | bad[2] | bad[3])
-    for (int again = at.tile * kBlockRows + wave; again < min(p.TQ, (at.tile + 1) * kBlockRows); again += 4)
+    for (int again = tile * kBlockRows + wave; again < min(p.TQ, (tile + 1) * kBlockRows); again += 4)
       attend_row<T, float>(p, b, hq, again, (float *)tiles + wave * kMaxDim, q, k, v, out, rest, lse);
 }
 
@@ -175,7 +175,7 @@ attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q
   const Dealt at = dealt(deal, blockIdx.x);
   const int b = at.pair / p.HK, hk = at.pair % p.HK, hq = hk * p.group + at.head;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
-  const int i = at.tile * kBlockRows + wave * 32 + c;
+  const int tile = tile_of_rank<false>(p, b, deal.tiles - 1 - at.tile, deal.tiles, kBlockRows), i = tile * kBlockRows + wave * 32 + c;
   const bool in = i < p.TQ;
   const Span span = in ? span_of(p, b, i) : Span{0, 0, 0};
   const Reach reach = reach_of(span, in);
@@ -240,7 +240,7 @@ attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q
   if (lane == 0) bad[wave] = odd;
   all_landed();  // what is stored, too: other wavefronts may write it again
   if (bad[0] | bad[1] | bad[2] | bad[3])
-    for (int again = at.tile * kBlockRows + wave; again < min(p.TQ, (at.tile + 1) * kBlockRows); again += 4)
+    for (int again = tile * kBlockRows + wave; again < min(p.TQ, (tile + 1) * kBlockRows); again += 4)
       dq_row<T, float>(p, b, hq, again, (float *)tiles + wave * 2 * kMaxDim, q, k, v, grad, lse, stats.delta, dq);
 }
 
@@ -248,8 +248,8 @@ attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q
 // that see any of them, head by head of those that share the keys.  Where there are few blocks they are cut: each of `cuts` takes an equal share
 // of the chunks and leaves its sums in float32, which attention_dkv_join_kernel adds up in order.
 // Bound by the matrix cores: 2 x 4096 tokens, 16 heads of 128, float16: 712 us (1160 TFLOP/s, dS in two counted), causal 425; float32, 2 x 2048,
-// 8 heads of 128: 620 (111 of 154).  Two causal halves that end at different times, and documents that do, leave units idle: 8192 tokens of five
-// documents, 16 heads of 128, take 297 us where even work would take 170; cut in two they would leave 134 MB of sums to be joined in 80 us.
+// 8 heads of 128: 620 (111 of 154).  Documents end at different times, which leaves units idle: 8192 tokens of five of
+// them, 16 heads of 128, take 241 us where even work would take 170; cut in two they would leave 134 MB of sums to be joined in 80 us.
 // With VALUES the keys' values lie in LDS instead of registers: at 128 values of float16 a head the two results and k take 160 of a lane's 256,
 // and with v's 32 as well the scores would not fit.
 template <typename T, int DP, int ROWS, bool VALUES, bool BENT>
@@ -266,7 +266,8 @@ attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ 
   __shared__ int bad[4];
   const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)tiles;
   const Dealt at = dealt(deal, blockIdx.x);  // its head is the cut
-  const int b = at.pair / p.HK, hk = at.pair % p.HK, tile = deal.tiles - 1 - at.tile;  // the first keys are seen by most
+  const int b = at.pair / p.HK, hk = at.pair % p.HK;
+  const int tile = tile_of_rank<true>(p, b, deal.tiles - 1 - at.tile, deal.tiles, kBlockRows);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
   const int block0 = tile * kBlockRows, key0 = block0 + wave * 32, j = key0 + c;
   const bool in = j < p.TK;
@@ -526,7 +527,7 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
     if (rc) return rc;
   } else if (dq) {
     ScopedTiming timed(TAG_ATTENTION_DQ);
-    const Deal deal = deal_of(p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows));
+    const Deal deal = deal_of(p, p.group, (int)ceil_div(p.TQ, kBlockRows));
     with_shape<T>(p, [&](auto dim, auto bent) {
       attention_dq_kernel<T, dim, dim <= 128 ? ROWS : 32, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, s>>>(
           p, deal, stats, tq, tk, tv, tg, tl, (T *)dq);
@@ -536,7 +537,7 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
   if (!dk) return MG_OK;
   {
     ScopedTiming timed(TAG_ATTENTION_DKV);
-    const Deal deal = deal_of(p.B * p.HK, cuts, key_tiles);
+    const Deal deal = deal_of(p, cuts, key_tiles);
     with_shape<T>(p, [&](auto dim, auto bent) {
       constexpr bool wide = sizeof(T) == 2 && dim >= 128;
       attention_dkv_kernel<T, dim, wide ? 32 : ROWS, wide, bent><<<dim3((unsigned)(deal.pairs * deal.heads * deal.tiles)), dim3(256), 0, s>>>(
@@ -573,7 +574,7 @@ bool few_take(const Attention &p, int size) {
 
 int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
   ScopedTiming timed(TAG_ATTENTION);
-  const Deal deal = deal_of(p.B * p.HK, p.group, (int)ceil_div(p.TQ, kBlockRows));
+  const Deal deal = deal_of(p, p.group, (int)ceil_div(p.TQ, kBlockRows));
   const dim3 grid((unsigned)(deal.pairs * deal.heads * deal.tiles));
   auto launch = [&](auto zero) {
     using T = decltype(zero);
