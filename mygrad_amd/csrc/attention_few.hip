@@ -338,13 +338,15 @@ template <typename T>
 constexpr int stages_of(int dim) { return sizeof(T) == 2 && dim <= 128 ? 2 : 1; }
 
 // A block for each 128 keys (a tile for each wavefront) while there are fewer than fill the device eight times over: a batch of ragged lengths evens
-// out over that many.  With more queries the products count and not the bytes, and twice over will do.
+// out over that many.  With more queries the products count and not the bytes: a block a compute unit will do (4096 tokens of two heads of 128,
+// float16: forward and dq 131 us in one piece, 138 and two joins in two), and each join takes as long as 512 keys.
 Split split_of(const Attention &p) {
+  const bool single = p.TQ <= 32;
   Split split;
   split.columns = p.TQ * p.group;
   split.panels = (int)ceil_div(split.columns, 32);
-  const long long pairs = (long long)p.B * p.HK * split.panels, blocks = (p.TQ <= 32 ? 8 : 2) * runtime().props.multiProcessorCount;
-  split.splits = (int)std::min<int64_t>(std::min<int64_t>(kMostSplits, std::max<int64_t>(1, blocks / pairs)), std::max<int64_t>(1, ceil_div(p.longest, 128)));
+  const long long pairs = (long long)p.B * p.HK * split.panels, blocks = (single ? 8 : 1) * runtime().props.multiProcessorCount;
+  split.splits = (int)std::min<int64_t>({kMostSplits, std::max<int64_t>(1, blocks / pairs), std::max<int64_t>(1, ceil_div(p.longest, single ? 128 : 512))});
   return split;
 }
 

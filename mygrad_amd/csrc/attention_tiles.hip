@@ -564,12 +564,12 @@ bool tiles_take(const Attention &p, int size, uintptr_t ends) {
          (long long)p.B * p.HQ * ceil_div(p.TQ, 32) < (1 << 24) && (long long)p.B * p.HK * ceil_div(p.TK, 32) < (1 << 24);
 }
 
-// Up to 32 queries one head would not fill a wavefront's columns.  Float32 products take so long that a few blocks of 128 queries, each on
-// a compute unit of its own, are slower than four times as many of 32 columns: 1 x 559 tokens of 4 heads 63 us against 25, 3 x 84 of 16 21 against
-// 13 -- until there are blocks for half the units (3 x 565 of 6: 37 against 33; 4 x 1024 of 8: 100 against 107).  In float16 they are no faster
-// (2 x 769 of 4 heads: 25 us against 44).
+// Up to 32 queries one head would not fill a wavefront's columns.  And a few blocks of 128 queries, each on a compute unit of its own, are slower
+// than four times as many of 32 columns whose keys four wavefronts share, while that leaves half the units idle.  Forward and dq, microseconds on
+// tiles and here: float16, 4096 causal tokens of two heads of 128 228 against 115, 8192 of one 432 against 204, 2 x 769 of 4 of 64 45 against 29,
+// 1024 of 16 heads of 128 80 against 86, 4096 of 8 299 against 480; float32, 559 of 4 of 64 forward 63 against 25, 4 x 1024 of 8 100 against 107.
 bool few_take(const Attention &p, int size) {
-  return p.TQ <= 32 || (size == 4 && 2 * (long long)p.B * p.HQ * ceil_div(p.TQ, kBlockRows) < runtime().props.multiProcessorCount);
+  return p.TQ <= 32 || 2 * (long long)p.B * p.HQ * ceil_div(p.TQ, kBlockRows) <= runtime().props.multiProcessorCount;
 }
 
 int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
