@@ -618,17 +618,15 @@ __device__ __forceinline__ Dealt dealt(const Deal &d, int block) {
   return Dealt{rest / d.heads, rest % d.heads, d.tiles - 1 - tile};
 }
 
-// The tile of a batch item that is `rank`-th in work, where documents make that uneven; each wavefront finds it for itself, four tiles a
-// lane.  The work is an estimate by the tile's first and last row.  8192 tokens of five documents, 16 heads of 128, float16: dk and dv 301 to 241
-// us, dq 183 to 166, forward 119 to 117.
-template <bool KEYS>
+// The tile of a batch item that is `rank`-th in work, where documents make that uneven; each wavefront finds it for itself, a tile a lane or
+// four.  The work is an estimate by the tile's first and last row.  8192 tokens of five documents, 16 heads of 128, float16: dk and dv 301 to 240
+// us, dq 183 to 159, forward 119 to 113.
+template <bool KEYS, int EACH>
 __device__ __forceinline__ int tile_of_rank(const Attention &p, int b, int rank, int tiles, int rows) {
-  constexpr int kMost = kSorted / 64;
-  if (!p.starts || tiles > kSorted) return KEYS ? rank : tiles - 1 - rank;  // what is causal: the last see, the first are seen, most
   const int lane = threadIdx.x & 63, tokens = KEYS ? p.TK : p.TQ;
-  int work[kMost], before[kMost] = {};
+  int work[EACH], before[EACH] = {};
 #pragma unroll
-  for (int m = 0; m < kMost; ++m) {
+  for (int m = 0; m < EACH; ++m) {
     const int tile = tiles - 1 - lane - 64 * m, first = tile * rows, last = min(tokens, first + rows) - 1;
     work[m] = -1;
     if (tile < 0) continue;
@@ -641,21 +639,26 @@ __device__ __forceinline__ int tile_of_rank(const Attention &p, int b, int rank,
     }
     if (p.window) work[m] = min(work[m], (p.causal ? 1 : 2) * p.window + rows);
   }
-  for (int m = 0; m < kMost; ++m)
+#pragma unroll
+  for (int m = 0; m < EACH; ++m)
     for (int n = 0; n < min(64, tiles - 64 * m); ++n) {
-      int other = __builtin_amdgcn_readlane(work[0], n);
+      const int other = __builtin_amdgcn_readlane(work[m], n);
 #pragma unroll
-      for (int c = 1; c < kMost; ++c) other = m == c ? __builtin_amdgcn_readlane(work[c], n) : other;
-#pragma unroll
-      for (int c = 0; c < kMost; ++c) before[c] += other > work[c] || (other == work[c] && 64 * m + n < 64 * c + lane);
+      for (int c = 0; c < EACH; ++c) before[c] += other > work[c] || (other == work[c] && 64 * m + n < 64 * c + lane);
     }
   int found = 0;
 #pragma unroll
-  for (int m = 0; m < kMost; ++m) {
+  for (int m = 0; m < EACH; ++m) {
     const unsigned long long here = __ballot(before[m] == rank && lane + 64 * m < tiles);
     if (here) found = 64 * m + __ffsll(here) - 1;
   }
   return __builtin_amdgcn_readfirstlane(tiles - 1 - found);
+}
+
+template <bool KEYS>
+__device__ __forceinline__ int tile_of_rank(const Attention &p, int b, int rank, int tiles, int rows) {
+  if (!p.starts || tiles > kSorted) return KEYS ? rank : tiles - 1 - rank;  // what is causal: the last see, the first are seen, most
+  return tiles <= 64 ? tile_of_rank<KEYS, 1>(p, b, rank, tiles, rows) : tile_of_rank<KEYS, kSorted / 64>(p, b, rank, tiles, rows);
 }
 
 }  // namespace mg

@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(256) head_norm_dw_join_kernel(int values, int 
   const int lane = threadIdx.x & 63, n = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= values) return;
   double sum = 0;
+#pragma unroll 8  // as many loads on their way: 2048 parts take 10 us, 13 one by one
   for (int part = lane; part < parts; part += 64) sum += from[(long long)part * values + n];
   sum = wave_sum(sum);
   if (lane == 0) dw[n] = (T)sum;
@@ -173,8 +174,8 @@ __device__ __forceinline__ void wave_sees() {
 // A lane holds V neighbouring values (16 bytes where the head dimension allows) of a row and LANES = 2^k lanes a row; the wavefront keeps to
 // a token, whose cos and sin stay in registers, while it goes through the heads.  A value's partner in its pair lies in another lane or
 // not, wherever sections and layout put it: rows are handed over through LDS, a wavefront's own.
-// Bound by memory: float16, 16384 tokens of 32 heads of 128 values (134 MB a tensor), 58 us forward (4.6 TB/s; a copy reaches 5.2) and 104 back with dw
-// (3.9); float32, 14256 tokens of 16 heads of 72 (66 MB), 31 and 60 (4.3 and 3.3).  A wavefront per row took 1681 and 618 us for both passes.
+// Bound by memory: float16, 16384 tokens of 32 heads of 128 values (134 MB a tensor), 58 us forward (4.6 TB/s; a copy reaches 5.2) and 99 back with dw
+// (4.1); float32, 14256 tokens of 16 heads of 72 (66 MB), 31 and 55 (4.2 and 3.6).  A wavefront per row took 1681 and 618 us for both passes.
 // NEAR: a lane's values turn with neighbours, a whole piece of them (halves of a row that are whole pieces); it then needs one place.
 template <typename T, typename C, int V, bool NEAR>
 struct Pieces {
