@@ -99,7 +99,8 @@ typedef struct {
   int64_t window;          /* 0: none; at most 2^30 */
   double scale;            /* of the products */
   double cap;              /* scores become cap * tanh(score / cap); 0: they stay */
-  int64_t longest;         /* lengths are at most this, or else taken as this; 0: at most TK.  What a launch is planned by */
+  int64_t longest;         /* lengths are at most this, or else taken as this; 0: at most TK.  What a launch is planned by, with */
+  int64_t mean;            /* their mean, about; 0: all are as long as the longest */
   const int32_t *lengths;  /* (B) keys in use, clamped to [0, TK] */
   const int32_t *prefix;   /* (B) */
   const int32_t *starts;   /* (B, TK) first key of the document that key j belongs to */

@@ -114,6 +114,7 @@ class AttentionDesc(ctypes.Structure):
         ("scale", ctypes.c_double),
         ("cap", ctypes.c_double),
         ("longest", ctypes.c_int64),
+        ("mean", ctypes.c_int64),
         ("lengths", ctypes.c_void_p),
         ("prefix", ctypes.c_void_p),
         ("starts", ctypes.c_void_p),

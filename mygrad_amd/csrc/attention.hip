@@ -141,7 +141,7 @@ int check_attention(const mg_attention_desc *d, Attention *p, const char *who, b
   if (d->TQ >= most || d->TK >= most || d->HQ >= most || d->B >= most || d->B * d->HQ >= most || d->B * d->HQ * ceil_div(d->TQ, 4) >= (1 << 24) ||
       (gradient && d->B * d->HK * ceil_div(d->TK, 4) >= (1 << 24)))  // a wavefront per row
     return fail(MG_ERR_UNSUPPORTED, "%s: 2^26 rows of results or more", who);
-  if (d->longest < 0) return fail(MG_ERR_BAD_ARG, "%s: a longest length of %lld", who, (long long)d->longest);
+  if (d->longest < 0 || d->mean < 0) return fail(MG_ERR_BAD_ARG, "%s: a longest length of %lld, a mean of %lld", who, (long long)d->longest, (long long)d->mean);
   if (d->window < 0 || d->window > most) return fail(MG_ERR_BAD_ARG, "%s: a window of %lld keys", who, (long long)d->window);
   if (!std::isfinite(d->scale) || !std::isfinite(d->cap) || d->cap < 0) return fail(MG_ERR_BAD_ARG, "%s: scale %g, cap %g", who, d->scale, d->cap);
   if (!d->starts != !d->ends) return fail(MG_ERR_BAD_ARG, "%s: starts of documents without their ends, or the other way round", who);
@@ -149,6 +149,7 @@ int check_attention(const mg_attention_desc *d, Attention *p, const char *who, b
   p->B = (int)d->B, p->TQ = (int)d->TQ, p->TK = (int)d->TK, p->HQ = (int)d->HQ, p->HK = (int)d->HK, p->D = (int)d->D;
   p->group = p->HQ / p->HK;
   p->longest = d->longest ? (int)std::min(d->longest, d->TK) : p->TK;
+  p->mean = d->mean ? (int)std::min<int64_t>(d->mean, p->longest) : p->longest;
   p->causal = d->causal != 0, p->window = (int)d->window;
   p->scale = (float)d->scale, p->cap = (float)d->cap, p->scale64 = d->scale, p->cap64 = d->cap;
   p->lengths = d->lengths, p->prefix = d->prefix, p->starts = d->starts, p->ends = d->ends, p->slopes = d->slopes;

@@ -10,7 +10,7 @@ struct Attention {
   int B, TQ, TK, HQ, HK, D;
   int group;  // query heads that share a key head
   int causal, window;
-  int longest;            // no item has more keys in use
+  int longest, mean;      // keys in use of the item with most, and of all about
   float scale, cap;       // cap 0: scores as they are
   double scale64, cap64;  // the same for double precision
   const int32_t *lengths, *prefix, *starts, *ends;

@@ -4,9 +4,9 @@
 // that makes few blocks still, the keys are split among blocks, which are joined by a second launch.
 //
 // With a step of generation over a cache this is bound by reading keys and values once: the sixteen products of a tile (128 values a head, float16)
-// wait for its bytes even where most columns are empty.  32 histories of 4000 to 8000 tokens, 32 heads over 8 of 128 in float16 (787 MB): 157 us and 7 to
-// join, 5.0 TB/s (a stream that only reads reaches 6.25, a copy 5.2); one history of 131001 tokens with a cap (537 MB): 128 and 12, 4.2 TB/s;
-// weights in two parts cost 4% of that.  A block holds 128 KB of tiles, one block a compute unit: four wavefronts with 16 KB each on the way.
+// wait for its bytes even where most columns are empty.  32 histories of 4000 to 8000 tokens, 32 heads over 8 of 128 in float16 (787 MB): 154 us, 5.1
+// TB/s (a stream that only reads reaches 6.25, a copy 5.2); one history of 131001 tokens with a cap (537 MB): 105 and 6 to join, 4.8 TB/s; weights in
+// two parts cost 4% of that.  A block holds 128 KB of tiles, one block a compute unit: four wavefronts with two tiles of 16 KB each.
 #include "attention_tiles.h"
 
 #include "attention_row.h"
@@ -337,15 +337,16 @@ void with_parts(const Attention &p, F f) {
 template <typename T>
 constexpr int stages_of(int dim) { return sizeof(T) == 2 && dim <= 128 ? 2 : 1; }
 
-// A block for each 128 keys (a tile for each wavefront) while there are fewer than fill the device eight times over: a batch of ragged lengths evens
-// out over that many.  With more queries the products count and not the bytes: a block a compute unit will do (4096 tokens of two heads of 128,
-// float16: forward and dq 131 us in one piece, 138 and two joins in two), and each join takes as long as 512 keys.
+// Keys are split until there is a block for each compute unit, and no further: a block takes a unit's LDS to itself, so the next one's first tiles
+// wait for its last.  One history of 131001 tokens, 32 heads over 8 of 128, float16: 110 us with the join, 140 in eight times as many blocks; 32 of 4000
+// to 8000 tokens 156 in one piece, 170.  Where lengths differ, by as much more as the longest is longer than the mean.  Pieces are 128 keys (a tile for
+// each wavefront) or more; with more queries a join takes as long as 512.
 Split split_of(const Attention &p) {
   const bool single = p.TQ <= 32;
   Split split;
   split.columns = p.TQ * p.group;
   split.panels = (int)ceil_div(split.columns, 32);
-  const long long pairs = (long long)p.B * p.HK * split.panels, blocks = (single ? 8 : 1) * runtime().props.multiProcessorCount;
+  const long long pairs = (long long)p.B * p.HK * split.panels, blocks = (long long)runtime().props.multiProcessorCount * p.longest / std::max(p.mean, 1);
   split.splits = (int)std::min<int64_t>({kMostSplits, std::max<int64_t>(1, blocks / pairs), std::max<int64_t>(1, ceil_div(p.longest, single ? 128 : 512))});
   return split;
 }

@@ -62,7 +62,7 @@ class AttentionMask:
             self._prefix = self._counts(prefix, "keys of a prefix")
         if lengths is not None:
             self._lengths = self._counts(lengths, "lengths")
-            self.shortest, self.longest = (int(f(self._lengths)) if self._lengths.size else 0 for f in (np.min, np.max))
+            self.shortest, self._mean, self.longest = (int(f(self._lengths)) if self._lengths.size else 0 for f in (np.min, np.mean, np.max))
         if documents is not None:
             self._starts, self._ends = _runs(np.atleast_2d(_integers(documents, "numbers of documents", (1, 2))))
         self._bound, self._described = {}, {}
@@ -170,8 +170,8 @@ def _describe(q, k, v, scale, cap, slopes, mask):
         if not q.size:
             return None, held  # nothing to compute, nothing to upload
         pointers = mask._bind(batch, queries, keys)
-        longest = 0 if mask._lengths is None else max(mask.longest, 1)
-        desc = _hip.AttentionDesc(_hip.storage_code(q.dtype), mask.causal, batch, queries, keys, heads, kv_heads, dim, mask.window, scale, cap, longest,
+        longest, mean = (0, 0) if mask._lengths is None else (max(mask.longest, 1), mask._mean)
+        desc = _hip.AttentionDesc(_hip.storage_code(q.dtype), mask.causal, batch, queries, keys, heads, kv_heads, dim, mask.window, scale, cap, longest, mean,
                                   *pointers, None)
         if len(mask._described) >= 64:
             mask._described.clear()

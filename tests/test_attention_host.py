@@ -14,7 +14,7 @@ from oracle import attention as ora
 
 
 def test_descriptors_match_the_header():
-    assert ctypes.sizeof(_hip.AttentionDesc) == 8 + 7 * 8 + 2 * 8 + 6 * 8
+    assert ctypes.sizeof(_hip.AttentionDesc) == 8 + 7 * 8 + 2 * 8 + 7 * 8
     assert ctypes.sizeof(_hip.HeadNormDesc) == 6 * 4 + 5 * 8 + 8 + 2 * 8
 
 
