@@ -339,14 +339,14 @@ constexpr int stages_of(int dim) { return sizeof(T) == 2 && dim <= 128 ? 2 : 1; 
 
 // Keys are split until there is a block for each compute unit, and no further: a block takes a unit's LDS to itself, so the next one's first tiles
 // wait for its last.  One history of 131001 tokens, 32 heads over 8 of 128, float16: 110 us with the join, 140 in eight times as many blocks; 32 of 4000
-// to 8000 tokens 156 in one piece, 170.  Where lengths differ, by as much more as the longest is longer than the mean.  Pieces are 128 keys (a tile for
+// to 8000 tokens 156 in one piece, 170.  Where lengths differ, for as many times more as the longest has the mean.  Pieces are 128 keys (a tile for
 // each wavefront) or more; with more queries a join takes as long as 512.
 Split split_of(const Attention &p) {
   const bool single = p.TQ <= 32;
   Split split;
   split.columns = p.TQ * p.group;
   split.panels = (int)ceil_div(split.columns, 32);
-  const long long pairs = (long long)p.B * p.HK * split.panels, blocks = (long long)runtime().props.multiProcessorCount * p.longest / std::max(p.mean, 1);
+  const long long pairs = (long long)p.B * p.HK * split.panels, blocks = (long long)runtime().props.multiProcessorCount * std::max(1, p.longest / std::max(p.mean, 1));
   split.splits = (int)std::min<int64_t>({kMostSplits, std::max<int64_t>(1, blocks / pairs), std::max<int64_t>(1, ceil_div(p.longest, single ? 128 : 512))});
   return split;
 }
