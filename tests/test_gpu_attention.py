@@ -112,6 +112,43 @@ def test_few_heads_over_long_rows(dtype, TQ, TK, HQ, HK, D, mask):
     _check(dtype, 1, TQ, TK, HQ, HK, D, **mask)
 
 
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("mask,B,HQ,HK,D", [
+    ("causal", 9, 16, 4, 64), ("both-ways", 8, 12, 4, 100), ("prefix", 9, 16, 2, 128), ("documents", 9, 16, 16, 32),
+    ("documents-window", 7, 10, 5, 72), ("documents-prefix", 9, 16, 8, 160), ("documents-lengths", 9, 16, 4, 128), ("none", 5, 14, 2, 36)])
+def test_many_heads(dtype, mask, B, HQ, HK, D):
+    """Enough blocks of 128 queries for half the compute units, and more."""
+    how = {**MASKS, "none": {}}[mask]
+    if mask == "documents-lengths":
+        how = {**how, "lengths": [150 - 9 * b for b in range(B)]}
+    _check(dtype, B, 150, 150, HQ, HK, D, cap=4.0 if mask in ("prefix", "documents") else None, bias=mask == "both-ways", **how)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("B", [8, 9])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, "lowest"])
+def test_many_heads_beside_documents_of_no_numbers(dtype, B, bad):
+    bad = np.finfo(dtype).min if bad == "lowest" else bad
+    rng = np.random.default_rng(B)
+    T, H, D = 140, 16, 64
+    ops = [rng.standard_normal((B, T, H, D)).astype(dtype) for _ in range(4)]
+    documents = np.repeat([0, 1, 2], [50, 40, 50])
+    results = []
+    for spoil in (False, True):
+        if spoil:
+            ops = [a.copy() for a in ops]
+            for a in ops:
+                a[:, 50:90] = bad
+        tensors = [mg.device_tensor(a) for a in ops]
+        out = attention(*tensors[:3], mask=AttentionMask(causal=True, documents=documents))
+        out.backward(tensors[3])
+        results.append([out.data] + [t.grad for t in tensors[:3]])
+    rows = documents != 1
+    for clean, dirty in zip(*results):
+        assert np.isfinite(dirty[:, rows]).all()
+        assert np.allclose(dirty[:, rows], clean[:, rows], rtol=4 * UNIT[dtype][1], atol=max(64 * UNIT[dtype][1], 1024 * UNIT[dtype][0]))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_one_mask_for_several_shapes(dtype):
     rng = np.random.default_rng(41)
