@@ -26,7 +26,7 @@ struct Split {
 };
 
 // What a lane has to know of its column, and the block of its keys.  Column n of a pair of batch item and key head is query n / group, head
-// n % group.
+// n % group.  Panels with the last queries, which see most where the mask is causal, come first, of all pairs.
 struct Panel {
   int part, pair, b, hk, first_column, columns;
   int i, hq;
@@ -39,8 +39,8 @@ struct Panel {
 __device__ __forceinline__ Panel panel_of(const Attention &p, const Split &split, int c) {
   Panel at;
   at.part = blockIdx.x % split.splits;
-  const int rest = blockIdx.x / split.splits, panel = split.panels - 1 - rest % split.panels;  // the last see most where the mask is causal
-  at.pair = rest / split.panels;
+  const int rest = blockIdx.x / split.splits, pairs = p.B * p.HK, panel = split.panels - 1 - rest / pairs;
+  at.pair = rest % pairs;
   at.b = at.pair / p.HK, at.hk = at.pair % p.HK;
   at.first_column = panel * 32, at.columns = min(32, split.columns - panel * 32);
   const int column = at.first_column + c;

@@ -565,11 +565,12 @@ bool tiles_take(const Attention &p, int size, uintptr_t ends) {
 }
 
 // Up to 32 queries one head would not fill a wavefront's columns.  And a few blocks of 128 queries, each on a compute unit of its own, are slower
-// than four times as many of 32 columns whose keys four wavefronts share, while that leaves half the units idle.  Forward and dq, microseconds on
-// tiles and here: float16, 4096 causal tokens of two heads of 128 228 against 115, 8192 of one 432 against 204, 2 x 769 of 4 of 64 45 against 29,
-// 1024 of 16 heads of 128 80 against 86, 4096 of 8 299 against 480; float32, 559 of 4 of 64 forward 63 against 25, 4 x 1024 of 8 100 against 107.
+// than four times as many of 32 columns whose keys four wavefronts share: in float16 while that leaves half the units idle, in float32, whose
+// products take longer than the keys' way, up to a block a unit.  Forward and dq, microseconds on tiles and here: float16, 4096 causal tokens of two
+// heads of 128 228 against 115, 2 x 769 of 4 of 64 45 against 29, 1024 of 16 of 128 80 against 86, 4096 of 8 299 against 480; float32, 1500 causal
+// tokens of 12 heads of 128 508 against 236, 4 x 1024 of 8 of 64 217 against 147, 4 x 2048 of 8, with no mask, 749 against 774.
 bool few_take(const Attention &p, int size) {
-  return p.TQ <= 32 || 2 * (long long)p.B * p.HQ * ceil_div(p.TQ, kBlockRows) <= runtime().props.multiProcessorCount;
+  return p.TQ <= 32 || (size == 4 ? 1 : 2) * (long long)p.B * p.HQ * ceil_div(p.TQ, kBlockRows) <= runtime().props.multiProcessorCount;
 }
 
 int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse) {
