@@ -5,8 +5,7 @@
 //
 // With a step of generation over a cache this is bound by reading keys and values once: the sixteen products of a tile (128 values a head, float16)
 // wait for its bytes even where most columns are empty.  32 histories of 4000 to 8000 tokens, 32 heads over 8 of 128 in float16 (787 MB): 154 us, 5.1
-// TB/s (a stream that only reads reaches 6.25, a copy 5.2); one history of 131001 tokens with a cap (537 MB): 105 and 6 to join, 4.8 TB/s; weights in
-// two parts cost 4% of that.  A block holds 128 KB of tiles, one block a compute unit: four wavefronts with two tiles of 16 KB each.
+// TB/s (a stream that only reads reaches 6.25, a copy 5.2); one history of 131001 tokens with a cap (537 MB): 105 and 6 to join, 4.8 TB/s.  A block holds 128 KB of tiles, one block a compute unit: four wavefronts with two tiles of 16 KB each.
 #include "attention_tiles.h"
 
 #include "attention_row.h"
@@ -125,7 +124,7 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
   for (int n = 0; n < kSteps; ++n) rows[n] = fragment_of(row, 16 * n + 8 * h, p.D, at.in);
   const Scores how = scores_of(p, at.hq);
 
-  Running<T, DP, 1, BENT, true> run;
+  Running<T, DP, 1, BENT> run;
   run.begin();
   const typename Tile::Place place = Tile::place(lane);
   const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)space + (unsigned)wave * (STAGES * 2 * Tile::kBytes);

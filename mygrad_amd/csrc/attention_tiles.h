@@ -284,10 +284,10 @@ __device__ __forceinline__ typename Fragment<T>::V rows_of(const f32x16 &v, int 
   return near;
 }
 
-// a times both: a float32 value in two of float16 keeps 22 bits (one is all of it in float32).  Gradients of scores are multiplied so: rounded to 11
-// bits they would make dq and dk off by half as much again as the rounding of the results does, which costs a fifth of dq's time and a
-// fourteenth of dk's and dv's (8192 packed tokens: 161 us against 192, 291 against 315, as both were then).  Weights are rounded once where products are the bound
-// (a block of 128 queries: results are off by 1.2 to 1.4 times their own rounding), and kept in two where bytes are.
+// a times both: a float32 value in two of float16 keeps 22 bits (one is all of it in float32).  Weights and gradients of scores are multiplied so,
+// and a result in float16 is off by its own rounding and no more.  Rounded to 11 bits weights would make out and dv off by 1.3 to 1.4 times that
+// and, by what grad . out is off, dq and dk by 1.05 times; gradients of scores dq and dk by half as much again.  The third product of a tile forward and
+// the sixth of dk and dv cost a tenth of a step: 8192 packed tokens, 16 heads of 128, 515 us against 568, 4 x 2048 of 16 over 4 with a cap 614 against 674.
 template <typename T>
 __device__ __forceinline__ f32x16 mma_of_two(typename Fragment<T>::V a, typename Fragment<T>::V b, typename Fragment<T>::V more, f32x16 c) {
   c = Fragment<T>::mma(a, b, c);
@@ -354,8 +354,8 @@ __device__ __forceinline__ Scores scores_of(const Attention &p, int head) {
 
 // 32 queries, one in each lane's column (in both halves), on their way through tiles of SUBS times 32 keys: S^T = K Q^T has a query's scores in
 // its lane (and the partner in the other half), so maximum and sum need no exchange but that one, and the weights are the right operand of
-// out^T = V^T P^T as they lie.  BENT: scores have a cap (whose registers the others do without).  FINE: float16 takes weights in two.
-template <typename T, int DP, int SUBS, bool BENT, bool FINE>
+// out^T = V^T P^T as they lie.  BENT: scores have a cap (whose registers the others do without).
+template <typename T, int DP, int SUBS, bool BENT>
 struct Running {
   typedef TileOf<T, DP, 32 * SUBS> Tile;
   typedef typename Fragment<T>::V V;
@@ -424,16 +424,13 @@ struct Running {
         s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], factor, -base));
         total += s[n][r];
       }
-    V weights[2 * SUBS], more[FINE ? 2 * SUBS : 1];
+    V weights[2 * SUBS], more[2 * SUBS];
 #pragma unroll
-    for (int m = 0; m < 2 * SUBS; ++m) weights[m] = FINE ? rows_of<T>(s[m >> 1], m & 1, more[FINE ? m : 0]) : rows_of<T>(s[m >> 1], m & 1);
+    for (int m = 0; m < 2 * SUBS; ++m) weights[m] = rows_of<T>(s[m >> 1], m & 1, more[m]);
 #pragma unroll
     for (int n = 0; n < kParts; ++n)
 #pragma unroll
-      for (int m = 0; m < 2 * SUBS; ++m) {
-        const V value = Tile::across(values, place, n, m);
-        sums[n] = FINE ? mma_of_two<T>(value, weights[m], more[FINE ? m : 0], sums[n]) : Fragment<T>::mma(value, weights[m], sums[n]);
-      }
+      for (int m = 0; m < 2 * SUBS; ++m) sums[n] = mma_of_two<T>(Tile::across(values, place, n, m), weights[m], more[m], sums[n]);
   }
 };
 

@@ -62,7 +62,7 @@ attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T 
     load(vb + from, last, to + Tile::kBytes);
   };
 
-  Running<T, DP, KEYS / 32, BENT, false> run;
+  Running<T, DP, KEYS / 32, BENT> run;
   run.begin();
   const typename Tile::Place place = Tile::place(lane);
   const Scores how = scores_of(p, hq);
@@ -400,17 +400,20 @@ attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ 
             }
           }
         }
-        in_units<T>(unit, dp, sum_k);
         V weights[2], back[2], more[2];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) weights[m] = rows_of<T>(s, m), back[m] = rows_of<T>(dp, m, more[m]);
+        for (int m = 0; m < 2; ++m) weights[m] = rows_of<T>(s, m, more[m]);
 #pragma unroll
         for (int part = 0; part < kParts; ++part)
 #pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            sum_k[part] = mma_of_two<T>(Tile::across(queries, place, part, 2 * n + m), back[m], more[m], sum_k[part]);
-            sum_v[part] = Fragment<T>::mma(Tile::across(queries, place, part, 2 * n + m, Tile::kBytes), weights[m], sum_v[part]);
-          }
+          for (int m = 0; m < 2; ++m) sum_v[part] = mma_of_two<T>(Tile::across(queries, place, part, 2 * n + m, Tile::kBytes), weights[m], more[m], sum_v[part]);
+        in_units<T>(unit, dp, sum_k);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) back[m] = rows_of<T>(dp, m, more[m]);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part)
+#pragma unroll
+          for (int m = 0; m < 2; ++m) sum_k[part] = mma_of_two<T>(Tile::across(queries, place, part, 2 * n + m), back[m], more[m], sum_k[part]);
       }
     }
     all_landed();

@@ -1,0 +1,40 @@
+"""How near attention and its gradients come to their formulas in 64 bits."""
+
+import numpy as np
+import pytest
+
+import mygrad_amd as mg
+from mygrad_amd.nnet import AttentionMask, attention
+from oracle import attention as ora
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    if not mg.is_available():
+        pytest.fail("libmygrad_hip.so / gfx950 device not available: the GPU tests need both")
+
+
+def run(q, k, v, g, mask=None, **how):
+    """out, dq, dk and dv as host arrays."""
+    tensors = [mg.device_tensor(a) for a in (q, k, v)]
+    out = attention(*tensors, mask=None if mask is None else AttentionMask(**mask), **how)
+    out.backward(mg.device_tensor(g, constant=True))
+    return [out.data] + [t.grad for t in tensors]
+
+
+@pytest.mark.parametrize("B,TQ,TK,HQ,HK,D,cap,mask", [
+    (9, 150, 150, 16, 4, 64, None, dict(causal=True)), (9, 150, 150, 16, 16, 128, 20.0, dict()), (3, 300, 200, 16, 8, 72, None, dict()),
+    (5, 300, 300, 16, 2, 256, None, dict(causal=True)), (1, 700, 700, 4, 1, 128, None, dict(causal=True)), (2, 20, 900, 8, 2, 96, 20.0, dict())])
+def test_float16_results_are_rounded_once(B, TQ, TK, HQ, HK, D, cap, mask):
+    """A result is off by its own rounding to float16, e.  What else there is -- sums, exponentials and scores in 32 bits, weights and their
+    gradients in two parts of float16 -- is some 2^-16 of it or less next to e of 2^-12.3, and adds in squares: 1% of e; twice that is allowed."""
+    rng = np.random.default_rng([B, TQ, D])
+    q, k, v, g = (rng.standard_normal(shape).astype(np.float16) for shape in ((B, TQ, HQ, D), (B, TK, HK, D), (B, TK, HK, D), (B, TQ, HQ, D)))
+    seen = ora.visible(B, TQ, TK, **mask)
+    exact = ora.forward(q, k, v, seen, cap=cap)[0], *ora.backward(q, k, v, g, seen, cap=cap)
+    rms = lambda a: np.sqrt((a * a).mean())
+    for name, have, want in zip(("out", "dq", "dk", "dv"), run(q, k, v, g, mask, cap=cap), exact):
+        rounding = rms(want.astype(np.float16).astype(np.float64) - want)
+        assert rms(have.astype(np.float64) - want) <= 1.02 * rounding, (name, rms(have - want) / rounding)
