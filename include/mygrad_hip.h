@@ -105,7 +105,7 @@ typedef struct {
   const int32_t *prefix;   /* (B) */
   const int32_t *starts;   /* (B, TK) first key of the document that key j belongs to */
   const int32_t *ends;     /* (B, TK) the key behind its last one */
-  const float *slopes;     /* (HQ): slopes[h] * |p - j| is taken off a score, after the cap */
+  const void *slopes;      /* (HQ), float32 (float64 for MG_F64): slopes[h] * |p - j| is taken off a score, after the cap */
 } mg_attention_desc;
 
 /* A norm for each head of x:(tokens, heads, D) and rotary positions: pair p of the first 2 * pairs values turns by the angle whose

@@ -14,7 +14,7 @@ struct Attention {
   float scale, cap;       // cap 0: scores as they are
   double scale64, cap64;  // the same for double precision
   const int32_t *lengths, *prefix, *starts, *ends;
-  const float *slopes;
+  const void *slopes;  // float, double for double precision
 };
 
 // Keys [lo, hi) are visible to a query that stands at `place` among them.  Every mask is one interval for each row: what is causal

@@ -59,7 +59,7 @@ __device__ __forceinline__ void attend_row(const Attention &p, int b, int h, int
   const int lane = threadIdx.x & 63;
   const long long step = (long long)p.HK * p.D, head = ((long long)b * p.TK * p.HK + h / p.group) * p.D;
   const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D;
-  const C slope = p.slopes ? (C)p.slopes[h] : C(0);
+  const C slope = p.slopes ? ((const C *)p.slopes)[h] : C(0);
   wave_sees();
   for (int d = lane; d < p.D; d += 64) mine[d] = (C)q[at + d];
   wave_sees();
@@ -103,7 +103,7 @@ __device__ __forceinline__ void dq_row(const Attention &p, int b, int h, int i, 
   const int lane = threadIdx.x & 63;
   const long long step = (long long)p.HK * p.D, head = ((long long)b * p.TK * p.HK + h / p.group) * p.D;
   const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D, stat = ((long long)b * p.HQ + h) * p.TQ + i;
-  const C slope = p.slopes ? (C)p.slopes[h] : C(0);
+  const C slope = p.slopes ? ((const C *)p.slopes)[h] : C(0);
   wave_sees();
   for (int d = lane; d < p.D; d += 64) mine[d] = (C)q[at + d], mine[p.D + d] = (C)grad[at + d];
   wave_sees();
@@ -144,7 +144,7 @@ __device__ __forceinline__ void dkv_row(const Attention &p, int b, int hk, int j
   C sum_k[kParts] = {}, sum_v[kParts] = {};
   for (int h = hk * p.group; h < (hk + 1) * p.group; ++h) {
     const long long head = ((long long)b * p.TQ * p.HQ + h) * p.D, stats = ((long long)b * p.HQ + h) * p.TQ;
-    const C slope = p.slopes ? (C)p.slopes[h] : C(0);
+    const C slope = p.slopes ? ((const C *)p.slopes)[h] : C(0);
     for (int i0 = 0; i0 < p.TQ; i0 += 64) {
       const int i = i0 + lane;
       C weight = 0, ds = 0;

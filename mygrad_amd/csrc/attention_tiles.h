@@ -349,7 +349,7 @@ struct Scores {
 };
 
 __device__ __forceinline__ Scores scores_of(const Attention &p, int head) {
-  return Scores{p.cap > 0 ? p.scale / p.cap : 0.0f, (p.cap > 0 ? p.cap : p.scale) * kLog2e, p.slopes ? p.slopes[head] * kLog2e : 0.0f};
+  return Scores{p.cap > 0 ? p.scale / p.cap : 0.0f, (p.cap > 0 ? p.cap : p.scale) * kLog2e, p.slopes ? ((const float *)p.slopes)[head] * kLog2e : 0.0f};
 }
 
 // 32 queries, one in each lane's column (in both halves), on their way through tiles of SUBS times 32 keys: S^T = K Q^T has a query's scores in

@@ -133,7 +133,7 @@ def _check_scores(scale, cap, dim):
     return scale, cap
 
 
-def _slopes_on_device(slopes, heads):
+def _slopes_on_device(slopes, heads, dtype):
     if slopes is None:
         return None
     if isinstance(slopes, Tensor):
@@ -146,7 +146,7 @@ def _slopes_on_device(slopes, heads):
         raise ValueError(f"`slopes` must have shape ({heads},), one for each query head, got {slopes.shape}")
     if slopes.dtype.kind != "f":
         raise TypeError(f"`slopes` are floating-point numbers, got {slopes.dtype}")
-    return _device.to_device(slopes, np.float32)
+    return _device.to_device(slopes, np.float64 if dtype == np.float64 else np.float32)
 
 
 _UNMASKED = AttentionMask()
@@ -159,7 +159,7 @@ def _describe(q, k, v, scale, cap, slopes, mask):
         mask = _UNMASKED
     elif not isinstance(mask, AttentionMask):
         raise TypeError(f"`mask` must be an AttentionMask, got {type(mask).__name__}")
-    held = _slopes_on_device(slopes, q.shape[2]) if slopes is not None and q.ndim == 4 else None
+    held = _slopes_on_device(slopes, q.shape[2], q.dtype) if slopes is not None and q.ndim == 4 else None
     key = q.shape, k.shape, v.shape, q.dtype, k.dtype, v.dtype, scale, cap
     desc = mask._described.get(key)
     if desc is None:
@@ -270,7 +270,7 @@ def attention(q, k, v, *, scale=None, cap=None, slopes=None, mask=None, constant
     What a query does not see does not touch its result, infinities and NaN included.
 
     ``scale`` is ``dim ** -0.5`` unless given; ``cap`` and ``slopes`` (one for each query head, a constant) are left out
-    unless given; ``mask`` is an :class:`AttentionMask`, none for all keys.
+    unless given (slopes in float32, float64 for float64); ``mask`` is an :class:`AttentionMask`, none for all keys.
 
     >>> import numpy as np
     >>> from mygrad_amd.nnet import AttentionMask, attention

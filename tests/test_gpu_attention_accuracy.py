@@ -6,6 +6,7 @@ import pytest
 import mygrad_amd as mg
 from mygrad_amd.nnet import AttentionMask, attention
 from oracle import attention as ora
+from tests.attention_bars import formulas_and_bars
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +39,17 @@ def test_float16_results_are_rounded_once(B, TQ, TK, HQ, HK, D, cap, mask):
     for name, have, want in zip(("out", "dq", "dk", "dv"), run(q, k, v, g, mask, cap=cap), exact):
         rounding = rms(want.astype(np.float16).astype(np.float64) - want)
         assert rms(have.astype(np.float64) - want) <= 1.02 * rounding, (name, rms(have - want) / rounding)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32, np.float64])
+@pytest.mark.parametrize("as_tensor", [False, True])
+def test_slopes_that_are_no_powers_of_two(dtype, as_tensor):
+    """In float64 they keep their digits; the other types take them in float32."""
+    rng = np.random.default_rng(12)
+    q, k, v, g = (rng.standard_normal((1, 600, 12, 16)).astype(dtype) for _ in range(4))
+    slopes = 2.0 ** (-8.0 * np.arange(1, 13) / 12)
+    held = slopes if dtype == np.float64 else slopes.astype(np.float32)
+    seen = ora.visible(1, 600, 600, causal=True)
+    results = run(q, k, v, g, dict(causal=True), slopes=mg.tensor(slopes, constant=True) if as_tensor else slopes)
+    for have, (want, bar) in zip(results, formulas_and_bars(dtype, q, k, v, g, seen, slopes=held)):
+        assert (np.abs(have.astype(np.float64) - want) <= bar).all()
