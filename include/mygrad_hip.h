@@ -97,8 +97,8 @@ typedef struct {
   int32_t causal;
   int64_t B, TQ, TK, HQ, HK, D;
   int64_t window;          /* 0: none; at most 2^30 */
-  double scale;            /* of the products */
-  double cap;              /* scores become cap * tanh(score / cap); 0: they stay */
+  double scale;            /* of the products; at most 1e30 but for MG_F64 */
+  double cap;              /* scores become cap * tanh(score / cap); 0: they stay; 1e-30 to 1e30 but for MG_F64 */
   int64_t longest;         /* lengths are at most this, or else taken as this; 0: at most TK.  What a launch is planned by, with */
   int64_t mean;            /* their mean, about; 0: all are as long as the longest */
   const int32_t *lengths;  /* (B) keys in use, clamped to [0, TK] */

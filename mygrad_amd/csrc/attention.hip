@@ -144,6 +144,9 @@ int check_attention(const mg_attention_desc *d, Attention *p, const char *who, b
   if (d->longest < 0 || d->mean < 0) return fail(MG_ERR_BAD_ARG, "%s: a longest length of %lld, a mean of %lld", who, (long long)d->longest, (long long)d->mean);
   if (d->window < 0 || d->window > most) return fail(MG_ERR_BAD_ARG, "%s: a window of %lld keys", who, (long long)d->window);
   if (!std::isfinite(d->scale) || !std::isfinite(d->cap) || d->cap < 0) return fail(MG_ERR_BAD_ARG, "%s: scale %g, cap %g", who, d->scale, d->cap);
+  // in single precision quotients and products of the two stay numbers, and neither turns into zero or infinity
+  if (d->dtype != MG_F64 && (std::fabs(d->scale) > 1e30 || d->cap > 1e30 || (d->cap > 0 && d->cap < 1e-30)))
+    return fail(MG_ERR_UNSUPPORTED, "%s: scale %g, cap %g in single precision", who, d->scale, d->cap);
   if (!d->starts != !d->ends) return fail(MG_ERR_BAD_ARG, "%s: starts of documents without their ends, or the other way round", who);
   if (d->window && d->prefix) return fail(MG_ERR_BAD_ARG, "%s: a window and a prefix", who);
   p->B = (int)d->B, p->TQ = (int)d->TQ, p->TK = (int)d->TK, p->HQ = (int)d->HQ, p->HK = (int)d->HK, p->D = (int)d->D;

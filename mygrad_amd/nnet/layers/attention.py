@@ -123,13 +123,19 @@ def _runs(ids):
     return (np.where(padding, 0, a).astype(np.int32) for a in (starts, ends))
 
 
-def _check_scores(scale, cap, dim):
+_LARGEST = 1e30  # of scale and cap in single precision, and one over it the smallest cap: their quotients and products stay numbers there
+
+
+def _check_scores(scale, cap, dim, dtype):
     scale = dim ** -0.5 if scale is None else float(scale)
     if not np.isfinite(scale):
         raise ValueError(f"`scale` must be finite, got {scale}")
     cap = 0.0 if cap is None else float(cap)
     if cap < 0 or not np.isfinite(cap):
         raise ValueError(f"`cap` must be a positive number or None, got {cap}")
+    if dtype != np.float64 and (abs(scale) > _LARGEST or cap > _LARGEST or 0 < cap < 1 / _LARGEST):
+        raise ValueError(f"scores in single precision take a `scale` of at most {_LARGEST:g} and a `cap` of {1 / _LARGEST:g} to {_LARGEST:g}, "
+                         f"got {scale} and {cap or None}")
     return scale, cap
 
 
@@ -164,7 +170,7 @@ def _describe(q, k, v, scale, cap, slopes, mask):
     desc = mask._described.get(key)
     if desc is None:
         _check_operands(q, k, v)
-        scale, cap = _check_scores(scale, cap, q.shape[3])
+        scale, cap = _check_scores(scale, cap, q.shape[3], q.dtype)
         (batch, queries, heads, dim), (keys, kv_heads) = q.shape, k.shape[1:3]
         mask._check(batch, queries, keys)
         if not q.size:

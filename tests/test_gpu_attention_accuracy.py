@@ -53,3 +53,28 @@ def test_slopes_that_are_no_powers_of_two(dtype, as_tensor):
     results = run(q, k, v, g, dict(causal=True), slopes=mg.tensor(slopes, constant=True) if as_tensor else slopes)
     for have, (want, bar) in zip(results, formulas_and_bars(dtype, q, k, v, g, seen, slopes=held)):
         assert (np.abs(have.astype(np.float64) - want) <= bar).all()
+
+
+@pytest.mark.parametrize("dtype,TQ,cap,scale", [
+    (np.float64, 40, 1e-50, None), (np.float64, 40, 1e40, None), (np.float32, 300, 1e-30, None), (np.float16, 300, 1e-30, None), (np.float32, 9, 1e-30, 1e20),
+    (np.float32, 40, 1e30, None), (np.float16, 300, 1e30, None)])
+def test_smallest_and_largest_caps(dtype, TQ, cap, scale):
+    """Scores next to zero give the mean, behind the largest caps what no cap gives; rows of zeros among the queries."""
+    rng = np.random.default_rng(TQ)
+    q, k, v = (rng.standard_normal((9, TQ, 8, 32)).astype(dtype) for _ in range(3))
+    q[:, ::7] = 0
+    out = attention(q, k, v, cap=cap, scale=scale).data.astype(np.float64)
+    seen = ora.visible(9, TQ, TQ)
+    zeros = np.zeros_like(q)
+    want, bar = formulas_and_bars(dtype, zeros if cap < 1 else q, k, v, zeros, seen)[0]
+    assert (np.abs(out - want) <= bar).all()
+
+
+def test_entry_points_refuse_scores_beyond_single_precision():
+    from mygrad_amd import _device, _hip
+
+    lib, buf = _hip.lib(), _device.DeviceBuffer(1 << 16)
+    for dtype, status in ((0, -2), (2, -2), (1, 0)):
+        for how in (dict(scale=0.25, cap=1e-50), dict(scale=0.25, cap=1e39), dict(scale=1e39, cap=0.0)):
+            desc = _hip.AttentionDesc(dtype=dtype, B=1, TQ=4, TK=4, HQ=2, HK=1, D=16, **how)
+            assert lib.mg_attention_fwd(desc, buf.ptr, buf.ptr, buf.ptr, buf.ptr + 8192, None, None) == status, (dtype, how)
