@@ -188,13 +188,13 @@ struct Pieces {
     return d >= 2 * p.pairs ? -1 : p.interleaved ? d / 2 : d < p.pairs ? d : d - p.pairs;
   }
 
-  // What each of the lane's values turns with.
-  __device__ __forceinline__ void find(const HeadNorm &p, int d0) {
+  // What each of the lane's values turns with; those without a pair with a zero at `nothing` (an infinity times their sine of 0 would be no number).
+  __device__ __forceinline__ void find(const HeadNorm &p, int d0, int nothing) {
 #pragma unroll
     for (int n = 0; n < (NEAR ? 1 : V); ++n) {
       const int d = d0 + n;
       const bool first = p.interleaved ? d % 2 == 0 : d < p.pairs;
-      partner[n] = pair_of(p, d) < 0 ? d : first ? d + apart(p) : d - apart(p);
+      partner[n] = pair_of(p, d) < 0 ? nothing : first ? d + apart(p) : d - apart(p);
     }
 #pragma unroll
     for (int n = 0; n < V; ++n) cos[n] = 1, sin[n] = 0;
@@ -260,13 +260,15 @@ __global__ void __launch_bounds__(256) head_norm_pieces_kernel(HeadNorm p, int l
   typedef typename P::Held Held;
   typedef typename P::Wide Wide;
   typedef std::conditional_t<(kAtOnce > 1), Held, Wide> Kept;
-  __shared__ __attribute__((aligned(64))) char space[4 * 64 * V * sizeof(double)];
+  __shared__ __attribute__((aligned(64))) char space[(4 * 64 + 4) * V * sizeof(double)];  // rows of four wavefronts, or sums; a zero for each of them
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (lanes - 1), g = lane / lanes, groups = 64 / lanes;
   const int d0 = l * V;
   const bool in = d0 < p.D, each = p.weight_heads > 1;
   C *row = (C *)space + wave * 64 * V + g * lanes * V;
+  C *nothing = (C *)(space + 4 * 64 * V * sizeof(double)) + wave * V;
+  if (lane < V) nothing[lane] = 0;
   P piece;
-  piece.find(p, in ? d0 : 0);
+  piece.find(p, in ? d0 : 0, (int)(nothing - row));
   // The groups take heads of one token side by side, of several tokens where these have few.  With weights for each head and their gradient
   // wanted, a group keeps to one head.
   const bool keep = BACK && parts && each;

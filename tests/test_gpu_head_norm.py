@@ -140,3 +140,26 @@ def test_entry_points_refuse_bad_descriptors():
         assert lib.mg_head_norm_bwd(desc, *[buf.ptr] * 6) == status, change
     assert lib.mg_head_norm_fwd(_hip.HeadNormDesc(**good), buf.ptr, None, buf.ptr, buf.ptr) == -1
     assert lib.mg_head_norm_bwd(_hip.HeadNormDesc(**{**good, "weight_heads": 0}), *[buf.ptr] * 6) == -1
+
+
+KERNELS = [(64, (16,)), (64, (5, 6)), (72, (16, 9)), (130, (40,)), (7, (2,)), (1000, (300,))]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,sections", KERNELS)
+def test_infinities_behind_the_pairs_stay_as_they_are(dtype, interleaved, dim, sections):
+    """In each kernel: what a head's pairs leave over is handed on bit for bit, and so is its gradient."""
+    rng = np.random.default_rng(dim)
+    pairs = sum(sections)
+    x, g = (rng.standard_normal((2, 9, 3, dim)).astype(dtype) for _ in range(2))
+    spoilt = [a.copy() for a in (x, g)]
+    for a in spoilt:
+        a[..., 2 * pairs:] = rng.choice(np.array([np.inf, -np.inf, 1.5, -0.25], dtype), a[..., 2 * pairs:].shape)
+    rotary = RotaryTable(sections, 50, interleaved=interleaved).at(rng.integers(0, 50, (2, 9, len(sections))))
+    t = mg.device_tensor(x)
+    y = rotate(t, rotary)
+    y.backward(mg.device_tensor(spoilt[1], constant=True))
+    for have, given in ((rotate(spoilt[0], rotary).data, spoilt[0]), (t.grad, spoilt[1])):
+        assert np.array_equal(have[..., 2 * pairs:], given[..., 2 * pairs:])
+        assert np.isfinite(have[..., :2 * pairs]).all()
