@@ -163,3 +163,18 @@ def test_infinities_behind_the_pairs_stay_as_they_are(dtype, interleaved, dim, s
     for have, given in ((rotate(spoilt[0], rotary).data, spoilt[0]), (t.grad, spoilt[1])):
         assert np.array_equal(have[..., 2 * pairs:], given[..., 2 * pairs:])
         assert np.isfinite(have[..., :2 * pairs]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,sections", KERNELS)
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_the_gradient_of_a_rotation_has_no_part_of_its_input(dtype, dim, sections, bad):
+    rng = np.random.default_rng(dim)
+    rotary = RotaryTable(sections, 50).at(rng.integers(0, 50, (2, 9, len(sections))))
+    g = rng.standard_normal((2, 9, 3, dim)).astype(dtype)
+    grads = []
+    for x in (np.ones_like(g), np.full_like(g, bad)):
+        t = mg.device_tensor(x)
+        rotate(t, rotary).backward(mg.device_tensor(g, constant=True))
+        grads.append(t.grad)
+    assert np.array_equal(*grads)
