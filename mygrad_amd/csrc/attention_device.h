@@ -43,4 +43,9 @@ __device__ __forceinline__ Span span_of(const Attention &p, int b, int i) {
   return s;
 }
 
+// How many keys a window lets some neighbouring rows see between them, at most: beyond 2^31 for the largest window both ways.
+__host__ __device__ constexpr unsigned window_of_rows(int window, int causal, int rows) {
+  return (causal ? 1u : 2u) * (unsigned)window + (unsigned)rows;
+}
+
 }  // namespace mg

@@ -637,7 +637,7 @@ __device__ __forceinline__ int tile_of_rank(const Attention &p, int b, int rank,
       const Span from = span_of(p, b, first), to = span_of(p, b, last);
       work[m] = max(max(to.hi, from.hi) - (from.hi ? from.lo : to.lo), 0);
     }
-    if (p.window) work[m] = min(work[m], (p.causal ? 1 : 2) * p.window + rows);
+    if (p.window) work[m] = (int)min((unsigned)work[m], window_of_rows(p.window, p.causal, rows));
   }
 #pragma unroll
   for (int m = 0; m < EACH; ++m)

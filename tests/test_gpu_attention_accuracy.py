@@ -78,3 +78,16 @@ def test_entry_points_refuse_scores_beyond_single_precision():
         for how in (dict(scale=0.25, cap=1e-50), dict(scale=0.25, cap=1e39), dict(scale=1e39, cap=0.0)):
             desc = _hip.AttentionDesc(dtype=dtype, B=1, TQ=4, TK=4, HQ=2, HK=1, D=16, **how)
             assert lib.mg_attention_fwd(desc, buf.ptr, buf.ptr, buf.ptr, buf.ptr + 8192, None, None) == status, (dtype, how)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("causal", [False, True])
+def test_the_largest_window_is_none(dtype, causal):
+    """With documents, whose tiles are sorted by an estimate of what they see."""
+    rng = np.random.default_rng(3)
+    q, k, v, g = (rng.standard_normal((9, 400, 16, 32)).astype(dtype) for _ in range(4))
+    documents = np.repeat([0, 1, 2], [150, 30, 220])
+    without = run(q, k, v, g, dict(causal=causal, documents=documents))
+    for window in (400, 1 << 30, 1 << 40):
+        for a, b in zip(without, run(q, k, v, g, dict(causal=causal, documents=documents, window=window))):
+            assert np.array_equal(a, b)
