@@ -14,6 +14,7 @@ __all__ = ["attention", "Attention", "AttentionMask", "KeyValueCache"]
 
 _DTYPES = (np.float16, np.float32, np.float64)
 _MOST_TOKENS = 1 << 30
+_MOST_SHAPES = 64  # that a mask keeps device copies and descriptors for; those in use are held by their users as well
 
 
 def _integers(values, what, ndim):
@@ -79,7 +80,7 @@ class AttentionMask:
         """Keys in use of each sequence, or None."""
         return None if self._lengths is None else self._lengths.copy()
 
-    def _check(self, batch, queries, keys):
+    def _check(self, batch, keys):
         for what, arr in (("lengths", self._lengths), ("prefix", self._prefix)):
             if arr is not None and arr.ndim and arr.shape != (batch,):
                 raise ValueError(f"`{what}` must have shape ({batch},) for a batch of {batch}, got {arr.shape}")
@@ -88,15 +89,16 @@ class AttentionMask:
         if self._starts is not None and (self._starts.shape[1] != keys or self._starts.shape[0] not in (1, batch)):
             raise ValueError(f"`documents` must have shape ({keys},) or ({batch}, {keys}), got {self._starts.shape}")
 
-    def _bind(self, batch, queries, keys):
-        """Device addresses (lengths, prefix, starts, ends) for a batch of that many queries and keys."""
-        held = self._bound.get((batch, queries, keys))
+    def _bind(self, batch, keys):
+        """Device buffers (lengths, prefix, starts, ends) for a batch of that many keys; whoever launches with them holds them."""
+        held = self._bound.get((batch, keys))
         if held is None:
-            self._check(batch, queries, keys)
-            buffers = [None if arr is None else _uploaded(np.broadcast_to(arr, shape)) for arr, shape in (
-                (self._lengths, (batch,)), (self._prefix, (batch,)), (self._starts, (batch, keys)), (self._ends, (batch, keys)))]
-            held = self._bound[batch, queries, keys] = tuple(None if b is None else b.ptr for b in buffers), buffers
-        return held[0]
+            self._check(batch, keys)
+            if len(self._bound) >= _MOST_SHAPES:
+                self._bound.clear()
+            held = self._bound[batch, keys] = tuple(None if arr is None else _uploaded(np.broadcast_to(arr, shape)) for arr, shape in (
+                (self._lengths, (batch,)), (self._prefix, (batch,)), (self._starts, (batch, keys)), (self._ends, (batch, keys))))
+        return held
 
 
 def _uploaded(arr):
@@ -159,33 +161,34 @@ _UNMASKED = AttentionMask()
 
 
 def _describe(q, k, v, scale, cap, slopes, mask):
-    """The descriptor, checked once for each mask and set of shapes and types (nothing writes to it), and the slopes' buffer, which has
-    to outlive it."""
+    """The descriptor, checked once for each mask and set of shapes and types (nothing writes to it), and the buffers that it points to,
+    which have to outlive it."""
     if mask is None:
         mask = _UNMASKED
     elif not isinstance(mask, AttentionMask):
         raise TypeError(f"`mask` must be an AttentionMask, got {type(mask).__name__}")
-    held = _slopes_on_device(slopes, q.shape[2], q.dtype) if slopes is not None and q.ndim == 4 else None
+    sloped = _slopes_on_device(slopes, q.shape[2], q.dtype) if slopes is not None and q.ndim == 4 else None
     key = q.shape, k.shape, v.shape, q.dtype, k.dtype, v.dtype, scale, cap
-    desc = mask._described.get(key)
-    if desc is None:
+    found = mask._described.get(key)
+    if found is None:
         _check_operands(q, k, v)
         scale, cap = _check_scores(scale, cap, q.shape[3], q.dtype)
         (batch, queries, heads, dim), (keys, kv_heads) = q.shape, k.shape[1:3]
-        mask._check(batch, queries, keys)
+        mask._check(batch, keys)
         if not q.size:
-            return None, held  # nothing to compute, nothing to upload
-        pointers = mask._bind(batch, queries, keys)
+            return None, None  # nothing to compute, nothing to upload
+        buffers = mask._bind(batch, keys)
         longest, mean = (0, 0) if mask._lengths is None else (max(mask.longest, 1), mask._mean)
         desc = _hip.AttentionDesc(_hip.storage_code(q.dtype), mask.causal, batch, queries, keys, heads, kv_heads, dim, mask.window, scale, cap, longest, mean,
-                                  *pointers, None)
-        if len(mask._described) >= 64:
+                                  *(None if b is None else b.ptr for b in buffers), None)
+        if len(mask._described) >= _MOST_SHAPES:
             mask._described.clear()
-        mask._described[key] = desc
-    if held is not None:
-        desc = _hip.AttentionDesc.from_buffer_copy(desc)
-        desc.slopes = held.ptr
-    return desc, held
+        found = mask._described[key] = desc, buffers
+    if sloped is None:
+        return found
+    desc = _hip.AttentionDesc.from_buffer_copy(found[0])
+    desc.slopes = sloped.ptr
+    return desc, (found[1], sloped)
 
 
 def _check_operands(q, k, v):
@@ -215,8 +218,7 @@ class Attention(Operation):
         self.variables = (q, k, v)
         qd, kd, vd = (_device.value_of(t) for t in (q, k, v))
         self._backed = None
-        self._mask = mask  # holds what the descriptor points to
-        self._desc, self._slopes = _describe(qd, kd, vd, scale, cap, slopes, mask)
+        self._desc, self._held = _describe(qd, kd, vd, scale, cap, slopes, mask)
         if self._desc is None:
             return np.zeros(qd.shape, dtype=qd.dtype)
         qb, kb, vb = (_device.to_device(a) for a in (qd, kd, vd))
@@ -346,13 +348,13 @@ class KeyValueCache:
         if kd.shape != vd.shape or kd.shape[2] != heads:
             raise ValueError(f"k and v must both have {heads} heads and as many tokens, got {kd.shape} and {vd.shape}")
         tokens = kd.shape[1]
-        pointers = self._masked(mask)._bind(batch, tokens, capacity)
+        lengths = self._masked(mask)._bind(batch, capacity)[0]
         if mask.shortest < tokens:
             raise ValueError(f"{tokens} tokens do not fit in a length of {mask.shortest}: lengths count the new tokens")
         if tokens == 0:
             return
         kb, vb = _device.to_device(kd), _device.to_device(vd)
-        _hip.check(_hip.lib().mg_cache_write(_hip.storage_code(self.dtype), batch, tokens, capacity, heads * dim, pointers[0], kb.ptr, vb.ptr,
+        _hip.check(_hip.lib().mg_cache_write(_hip.storage_code(self.dtype), batch, tokens, capacity, heads * dim, lengths.ptr, kb.ptr, vb.ptr,
                                              self._keys.ptr, self._values.ptr))
 
     def attend(self, q, *, mask, scale=None, cap=None, slopes=None):

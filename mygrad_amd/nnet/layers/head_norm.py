@@ -14,6 +14,7 @@ from ...tensor_base import Tensor
 __all__ = ["head_norm", "rotate", "HeadNorm", "RotaryTable", "RotaryPositions"]
 
 _DTYPES = (np.float16, np.float32, np.float64)
+_MOST_SHAPES = 64  # that positions keep device copies and descriptors for; those in use are held by their users as well
 
 
 class RotaryTable:
@@ -92,6 +93,8 @@ class RotaryPositions:
         buf = self._bound.get(lead)
         if buf is None:
             self._check(lead)
+            if len(self._bound) >= _MOST_SHAPES:
+                self._bound.clear()
             spread = np.broadcast_to(self._positions, lead + self._positions.shape[-1:])
             buf = self._bound[lead] = _device.from_host(np.ascontiguousarray(spread)).buf
         return buf
@@ -112,7 +115,6 @@ class HeadNorm(Operation):
         if rotary is not None and not isinstance(rotary, RotaryPositions):
             raise TypeError(f"`rotary` must come from RotaryTable.at, got {type(rotary).__name__}")
         self._backed = None
-        self._rotary = rotary  # holds what the descriptor points to
         self._weighted = wd.size > 0
         described = _described if rotary is None else rotary._described
         key = xd.shape, xd.dtype, wd.shape, wd.dtype, eps
@@ -121,10 +123,10 @@ class HeadNorm(Operation):
             found = self._describe(xd, wd, eps, rotary)
             if xd.size == 0:
                 return np.empty(xd.shape, dtype=xd.dtype)
-            if len(described) >= 64:
+            if len(described) >= _MOST_SHAPES:
                 described.clear()
             described[key] = found
-        self._desc, self._table = found
+        self._desc, self._table, self._held = found
         xb = _device.to_device(xd)
         wb = _device.to_device(wd) if self._weighted else None
         out = _device.DeviceBuffer(xd.nbytes)
@@ -134,7 +136,7 @@ class HeadNorm(Operation):
         return y
 
     def _describe(self, x, w, eps, rotary):
-        """The checked descriptor (nothing writes to it) and the table's address."""
+        """The checked descriptor (nothing writes to it), the table's address, and what holds the memory of both."""
         if x.ndim < 2:
             raise ValueError(f"`x` must have the axes (..., heads, dim), got shape {x.shape}")
         if x.dtype not in _DTYPES:
@@ -159,10 +161,11 @@ class HeadNorm(Operation):
         desc = _hip.HeadNormDesc(_hip.storage_code(x.dtype), eps is not None, w.size // dim if self._weighted else 0, 0, 1, 0, prod(lead),
                                  heads, dim, 0, 0, 0.0 if eps is None else eps, None, None)
         if table is None:
-            return desc, None
+            return desc, None, None
         desc.interleaved, desc.axes, desc.pairs, desc.table_rows = table.interleaved, len(table.sections), table.pairs, table.length
-        desc.positions, desc.axis_of = rotary._buffer(lead).ptr, table._buffer("axis_of").ptr
-        return desc, table._buffer("f8" if x.dtype == np.float64 else "f4").ptr
+        held = rotary._buffer(lead), table._buffer("axis_of"), table._buffer("f8" if x.dtype == np.float64 else "f4")
+        desc.positions, desc.axis_of = held[0].ptr, held[1].ptr
+        return desc, held[2].ptr, held
 
     def _run_backward(self, grad, want):
         x, w = (_device.value_of(t) for t in self.variables)

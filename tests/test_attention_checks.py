@@ -9,6 +9,7 @@ import numpy as np
 import pytest
 
 from mygrad_amd.nnet import attention
+from tests.test_host import run_on_standins
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
@@ -34,3 +35,30 @@ def test_rows_of_the_largest_window_see_no_fewer_keys_than_a_small_one_lets(tmp_
     for causal, each in ((1, 1), (0, 2)):
         for window in (1, 100, 1 << 29, 1 << 30):
             assert estimate(window, causal, 128) == each * window + 128
+
+
+def test_masks_and_positions_hold_memory_for_few_shapes(tmp_path):
+    """However many shapes pass through one mask, or through none; what a recorded operation points to stays for its gradient."""
+    program = """
+import numpy as np
+import mygrad_amd as mg
+from mygrad_amd.nnet import AttentionMask, KeyValueCache, RotaryTable, attention, rotate
+from mygrad_amd.nnet.layers.attention import _UNMASKED
+mask, positions = AttentionMask(True, lengths=3, prefix=2), RotaryTable(2, 8).at([1])
+x = lambda batch, tokens=4: mg.device_tensor(np.ones((batch, tokens, 1, 4), np.float32))
+first = [attention(x(2), x(2), x(2), slopes=np.ones(1, np.float32), mask=mask), rotate(x(2), positions)]
+for n in range(1, 200):
+    attention(x(n), x(n), x(n), mask=mask), attention(x(1, n), x(1, n), x(1, n)), rotate(x(n), positions)
+    cache = KeyValueCache(1, n + 3, 1, 4)
+    cache.write(x(1, 2), x(1, 2), mask), cache.attend(x(1, 2), mask=mask)
+for kept in (mask, _UNMASKED, positions):
+    assert len(kept._bound) <= 64 and len(kept._described) <= 64, (kept, len(kept._bound))
+for out in first:
+    operation, ours = out.creator, lambda held: sum(map(ours, held), []) if isinstance(held, tuple) else [] if held is None else [held]
+    buffers = ours(operation._held)
+    desc = operation._desc
+    pointers = {getattr(desc, name) for name in ("lengths", "prefix", "slopes", "positions", "axis_of") if hasattr(desc, name)}
+    assert buffers and all(b._owned for b in buffers) and pointers <= {b.ptr for b in buffers}
+print("held")
+"""
+    assert "held" in run_on_standins(tmp_path, program)
