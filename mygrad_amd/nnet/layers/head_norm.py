@@ -211,7 +211,11 @@ def head_norm(x, weight=None, *, eps: float, rotary: Optional[RotaryPositions] =
     """
     if eps is None:
         raise TypeError("`eps` must be a non-negative number; without a norm use rotate()")
-    return Tensor._op(HeadNorm, x, np.array([]) if weight is None else weight, op_kwargs=dict(eps=eps, rotary=rotary), constant=constant)
+    if weight is None:
+        weight = np.array([])
+    elif 0 in np.shape(weight) and np.shape(weight) != np.shape(x)[-2:]:  # to the operation an empty one is none
+        raise ValueError(f"`weight` of shape {np.shape(weight)} for heads of shape {np.shape(x)[-2:]}")
+    return Tensor._op(HeadNorm, x, weight, op_kwargs=dict(eps=eps, rotary=rotary), constant=constant)
 
 
 def rotate(x, rotary: RotaryPositions, *, constant: Optional[bool] = None) -> Tensor:

@@ -8,7 +8,8 @@ import subprocess
 import numpy as np
 import pytest
 
-from mygrad_amd.nnet import attention
+import mygrad_amd as mg
+from mygrad_amd.nnet import attention, head_norm
 from tests.test_host import run_on_standins
 
 
@@ -62,3 +63,12 @@ for out in first:
 print("held")
 """
     assert "held" in run_on_standins(tmp_path, program)
+
+
+@pytest.mark.parametrize("shape", [(0,), (4, 0), (0, 8), (1, 0)])
+def test_an_empty_weight_is_not_none(shape):
+    x = np.ones((2, 3, 4, 8), dtype=np.float32)
+    for weight in (np.ones(shape, dtype=np.float32), mg.tensor(np.ones(shape, dtype=np.float32))):
+        with pytest.raises(ValueError, match="weight"):
+            head_norm(x, weight, eps=1e-6)
+    assert head_norm(np.ones((2, 0, 8)), np.ones((0, 8)), eps=1e-6).shape == (2, 0, 8)
