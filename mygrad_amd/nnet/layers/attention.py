@@ -50,20 +50,20 @@ class AttentionMask:
     def __init__(self, causal=False, *, window=None, prefix=None, documents=None, lengths=None):
         if not isinstance(causal, (bool, np.bool_)):
             raise TypeError(f"`causal` must be a boolean value, got: {causal}")
-        self.causal = bool(causal)
-        self.window = 0
+        self._causal = bool(causal)
+        self._window = 0
         if window is not None:
             if _integers(window, "keys in a window", (0,)) < 1:
                 raise ValueError(f"a window holds one key or more, got {window}")
-            self.window = min(int(window), _MOST_TOKENS)
+            self._window = min(int(window), _MOST_TOKENS)
         self._lengths = self._prefix = self._starts = self._ends = None
         if prefix is not None:
-            if not self.causal or window is not None:
+            if not self._causal or window is not None:
                 raise ValueError("a prefix goes with a causal mask without a window")
             self._prefix = self._counts(prefix, "keys of a prefix")
         if lengths is not None:
             self._lengths = self._counts(lengths, "lengths")
-            self.shortest, self._mean, self.longest = (int(f(self._lengths)) if self._lengths.size else 0 for f in (np.min, np.mean, np.max))
+            self._shortest, self._mean, self._longest = (int(f(self._lengths)) if self._lengths.size else 0 for f in (np.min, np.mean, np.max))
         if documents is not None:
             self._starts, self._ends = _runs(np.atleast_2d(_integers(documents, "numbers of documents", (1, 2))))
         self._bound, self._described = {}, {}
@@ -75,6 +75,16 @@ class AttentionMask:
             raise ValueError(f"{what} lie in [0, 2**30), got {arr.min()} to {arr.max()}")
         return arr.astype(np.int32)
 
+    # Read only: descriptors that calls have made are not made again.
+    @property
+    def causal(self):
+        return self._causal
+
+    @property
+    def window(self):
+        """Keys of the window, 0 for none."""
+        return self._window
+
     @property
     def lengths(self):
         """Keys in use of each sequence, or None."""
@@ -84,8 +94,8 @@ class AttentionMask:
         for what, arr in (("lengths", self._lengths), ("prefix", self._prefix)):
             if arr is not None and arr.ndim and arr.shape != (batch,):
                 raise ValueError(f"`{what}` must have shape ({batch},) for a batch of {batch}, got {arr.shape}")
-        if self._lengths is not None and self.longest > keys:
-            raise ValueError(f"a length of {self.longest} among {keys} keys")
+        if self._lengths is not None and self._longest > keys:
+            raise ValueError(f"a length of {self._longest} among {keys} keys")
         if self._starts is not None and (self._starts.shape[1] != keys or self._starts.shape[0] not in (1, batch)):
             raise ValueError(f"`documents` must have shape ({keys},) or ({batch}, {keys}), got {self._starts.shape}")
 
@@ -178,8 +188,8 @@ def _describe(q, k, v, scale, cap, slopes, mask):
         if not q.size:
             return None, None  # nothing to compute, nothing to upload
         buffers = mask._bind(batch, keys)
-        longest, mean = (0, 0) if mask._lengths is None else (max(mask.longest, 1), mask._mean)
-        desc = _hip.AttentionDesc(_hip.storage_code(q.dtype), mask.causal, batch, queries, keys, heads, kv_heads, dim, mask.window, scale, cap, longest, mean,
+        longest, mean = (0, 0) if mask._lengths is None else (max(mask._longest, 1), mask._mean)
+        desc = _hip.AttentionDesc(_hip.storage_code(q.dtype), mask._causal, batch, queries, keys, heads, kv_heads, dim, mask._window, scale, cap, longest, mean,
                                   *(None if b is None else b.ptr for b in buffers), None)
         if len(mask._described) >= _MOST_SHAPES:
             mask._described.clear()
@@ -309,28 +319,37 @@ class KeyValueCache:
         shape = tuple(int(_integers(n, "extents of a cache", (0,))) for n in (batch, capacity, heads, dim))
         if min(shape) < 1 or shape[1] >= _MOST_TOKENS or shape[3] > 256:
             raise ValueError(f"a cache needs a batch, a capacity, heads and a dimension (at most 256) of one or more, got {shape}")
-        self.shape, self.dtype = shape, dtype
+        self._shape, self._dtype = shape, dtype
         nbytes = int(np.prod(shape, dtype=np.int64)) * dtype.itemsize
         self._keys, self._values = _device.DeviceBuffer(nbytes), _device.DeviceBuffer(nbytes)
         for buf in (self._keys, self._values):
             _hip.check(_hip.lib().mg_memset_zero(buf.ptr, nbytes))
 
     @property
+    def shape(self):
+        """Batch, capacity, heads and dimension."""
+        return self._shape
+
+    @property
+    def dtype(self):
+        return self._dtype
+
+    @property
     def keys(self):
         """``(batch, capacity, heads, dim)``, on the device; ``.host()`` copies what it holds now."""
-        return _device.DeviceArray(self._keys, self.shape, self.dtype)
+        return _device.DeviceArray(self._keys, self._shape, self._dtype)
 
     @property
     def values(self):
         """Like :attr:`keys`."""
-        return _device.DeviceArray(self._values, self.shape, self.dtype)
+        return _device.DeviceArray(self._values, self._shape, self._dtype)
 
     def _operand(self, x, name):
         value = _device.value_of(x) if isinstance(x, Tensor) else x if isinstance(x, _device.DeviceArray) else np.asarray(x)
-        if value.ndim != 4 or value.shape[0] != self.shape[0] or value.shape[3] != self.shape[3]:
-            raise ValueError(f"`{name}` must have shape ({self.shape[0]}, tokens, heads, {self.shape[3]}), got {value.shape}")
-        if value.dtype != self.dtype:
-            raise TypeError(f"a cache of {self.dtype} takes `{name}` in that dtype, got {value.dtype}")
+        if value.ndim != 4 or value.shape[0] != self._shape[0] or value.shape[3] != self._shape[3]:
+            raise ValueError(f"`{name}` must have shape ({self._shape[0]}, tokens, heads, {self._shape[3]}), got {value.shape}")
+        if value.dtype != self._dtype:
+            raise TypeError(f"a cache of {self._dtype} takes `{name}` in that dtype, got {value.dtype}")
         return value
 
     @staticmethod
@@ -344,17 +363,17 @@ class KeyValueCache:
     def write(self, k, v, mask):
         """Puts the tokens of ``k, v:(batch, tokens, heads, dim)`` at the places that end at ``mask.lengths``."""
         kd, vd = self._operand(k, "k"), self._operand(v, "v")
-        batch, capacity, heads, dim = self.shape
+        batch, capacity, heads, dim = self._shape
         if kd.shape != vd.shape or kd.shape[2] != heads:
             raise ValueError(f"k and v must both have {heads} heads and as many tokens, got {kd.shape} and {vd.shape}")
         tokens = kd.shape[1]
         lengths = self._masked(mask)._bind(batch, capacity)[0]
-        if mask.shortest < tokens:
-            raise ValueError(f"{tokens} tokens do not fit in a length of {mask.shortest}: lengths count the new tokens")
+        if mask._shortest < tokens:
+            raise ValueError(f"{tokens} tokens do not fit in a length of {mask._shortest}: lengths count the new tokens")
         if tokens == 0:
             return
         kb, vb = _device.to_device(kd), _device.to_device(vd)
-        _hip.check(_hip.lib().mg_cache_write(_hip.storage_code(self.dtype), batch, tokens, capacity, heads * dim, lengths.ptr, kb.ptr, vb.ptr,
+        _hip.check(_hip.lib().mg_cache_write(_hip.storage_code(self._dtype), batch, tokens, capacity, heads * dim, lengths.ptr, kb.ptr, vb.ptr,
                                              self._keys.ptr, self._values.ptr))
 
     def attend(self, q, *, mask, scale=None, cap=None, slopes=None):

@@ -43,13 +43,30 @@ class RotaryTable:
             raise ValueError(f"`base` must be a positive number, got {base}")
         if not isinstance(interleaved, (bool, np.bool_)):
             raise TypeError(f"`interleaved` must be a boolean value, got: {interleaved}")
-        self.sections, self.length, self.interleaved = tuple(map(int, sections)), int(length), bool(interleaved)
-        self.pairs = sum(self.sections)
+        self._sections, self._length, self._interleaved = tuple(map(int, sections)), int(length), bool(interleaved)
         frequency = np.concatenate([float(base) ** (-np.arange(n) / n) if n else np.empty(0) for n in self.sections])
         angle = np.arange(self.length)[:, None] * frequency
         self._turns = np.stack((np.cos(angle), np.sin(angle)), -1)
         self._axis_of = np.repeat(np.arange(len(self.sections)), self.sections).astype(np.uint8)
         self._buffers = {}
+
+    # Read only: the angles are made of them.
+    @property
+    def sections(self):
+        return self._sections
+
+    @property
+    def length(self):
+        return self._length
+
+    @property
+    def interleaved(self):
+        return self._interleaved
+
+    @property
+    def pairs(self):
+        """Of all axes."""
+        return sum(self._sections)
 
     def _buffer(self, what):
         buf = self._buffers.get(what)
@@ -78,8 +95,12 @@ class RotaryPositions:
             raise ValueError(f"positions must have shape (..., {axes}) for {axes} axes, got {arr.shape}")
         if arr.size and (arr.min() < 0 or arr.max() >= table.length):
             raise ValueError(f"positions must lie in [0, {table.length}), got {arr.min()} to {arr.max()}")
-        self.table, self._positions = table, arr.astype(np.int32)
+        self._table, self._positions = table, arr.astype(np.int32)
         self._bound, self._described = {}, {}
+
+    @property
+    def table(self):
+        return self._table
 
     def _check(self, lead):
         try:

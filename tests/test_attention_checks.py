@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 
 import mygrad_amd as mg
-from mygrad_amd.nnet import attention, head_norm
+from mygrad_amd.nnet import AttentionMask, RotaryTable, attention, head_norm
 from tests.test_host import run_on_standins
 
 
@@ -72,3 +72,15 @@ def test_an_empty_weight_is_not_none(shape):
         with pytest.raises(ValueError, match="weight"):
             head_norm(x, weight, eps=1e-6)
     assert head_norm(np.ones((2, 0, 8)), np.ones((0, 8)), eps=1e-6).shape == (2, 0, 8)
+
+
+def test_masks_and_tables_do_not_change():
+    """What a call has checked and sent to the device goes for the next one, too."""
+    mask, table = AttentionMask(causal=True, window=3, lengths=[2, 4]), RotaryTable((1, 2), 9)
+    for owner, name, value in ((mask, "causal", False), (mask, "window", 5), (mask, "lengths", [1, 1]), (table, "length", 20), (table, "sections", (2, 1)),
+                               (table, "interleaved", True), (table, "pairs", 2), (table.at([[0, 1]]), "table", table)):
+        with pytest.raises(AttributeError):
+            setattr(owner, name, value)
+    assert mask.causal and mask.window == 3 and table.pairs == 3 and table.length == 9 and table.sections == (1, 2) and not table.interleaved
+    mask.lengths[0] = 7
+    assert mask.lengths[0] == 2
