@@ -6,7 +6,7 @@ import pytest
 import mygrad_amd as mg
 from mygrad_amd.nnet import AttentionMask, attention
 from oracle import attention as ora
-from tests.attention_bars import formulas_and_bars
+from tests.attention_bars import CASES, Formulas, bars_of, formulas_and_bars, name_of, operands
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,16 @@ def test_the_largest_window_is_none(dtype, causal):
     for window in (400, 1 << 30, 1 << 40):
         for a, b in zip(without, run(q, k, v, g, dict(causal=causal, documents=documents, window=window))):
             assert np.array_equal(a, b)
+
+
+def arguments(case, how):
+    return {name: how[name] for name in ("scale", "cap", "slopes")}
+
+
+@pytest.mark.parametrize("case", CASES, ids=name_of)
+def test_results_within_their_bars(case):
+    arrays, seen, how = operands(case)
+    f = Formulas(*arrays, seen, **how)
+    for name, have, want, bar in zip(("out", "dq", "dk", "dv"), run(*arrays, case["mask"], **arguments(case, how)), f.results, bars_of(case["dtype"], f)):
+        over = np.abs(have.astype(np.float64) - want) - bar
+        assert have.dtype == case["dtype"] and (over <= 0).all(), (name, over.max(), np.unravel_index(over.argmax(), over.shape))
