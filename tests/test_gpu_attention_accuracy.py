@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import mygrad_amd as mg
-from mygrad_amd.nnet import AttentionMask, attention
+from mygrad_amd.nnet import AttentionMask, RotaryTable, attention, head_norm
 from oracle import attention as ora
 from tests.attention_bars import CASES, Formulas, bars_of, formulas_and_bars, name_of, operands
 
@@ -104,3 +104,41 @@ def test_results_within_their_bars(case):
     for name, have, want, bar in zip(("out", "dq", "dk", "dv"), run(*arrays, case["mask"], **arguments(case, how)), f.results, bars_of(case["dtype"], f)):
         over = np.abs(have.astype(np.float64) - want) - bar
         assert have.dtype == case["dtype"] and (over <= 0).all(), (name, over.max(), np.unravel_index(over.argmax(), over.shape))
+
+
+EACH_WAY = [(1, 700, 4, 1, 36), (1, 600, 4, 1, 128), (1, 20, 4, 1, 100), (2, 140, 2, 2, 192), (9, 140, 16, 16, 64), (8, 140, 16, 4, 72)]
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, "lowest"])
+@pytest.mark.parametrize("dtype,B,T,HQ,HK,D", [*((dtype, *shape) for dtype in (np.float16, np.float32) for shape in EACH_WAY),
+                                               *((np.float64, *shape) for shape in EACH_WAY[:4])])
+def test_beside_documents_of_no_numbers_results_are_within_their_bars(dtype, bad, B, T, HQ, HK, D):
+    """What other documents of the same tiles hold changes nothing: the bars are those of the operands that are seen."""
+    case = dict(dtype=dtype, shape=(B, T, T, HQ, HK, D), cap=None, bias=False, scale=None, grad_scale=1.0)
+    documents = np.repeat([0, 1, 2], [T // 3, T // 2 - T // 3, T - T // 2])
+    arrays, seen, how = operands(dict(case, mask=dict(causal=True, documents=documents)))
+    f = Formulas(*arrays, seen, **how)
+    spoilt = [a.copy() for a in arrays]
+    for a in spoilt:
+        a[:, documents == 1] = np.finfo(dtype).min if bad == "lowest" else bad
+    rows = documents != 1
+    for name, have, want, bar in zip(("out", "dq", "dk", "dv"), run(*spoilt, dict(causal=True, documents=documents)), f.results, bars_of(dtype, f)):
+        over = (np.abs(have.astype(np.float64) - want) - bar)[:, rows]
+        assert (over <= 0).all(), (name, np.nanmax(over), np.isnan(over).sum())
+
+
+def test_float16_through_other_operations():
+    """Bit for bit what the parts give one by one: a norm of heads before attention, one tensor in three places behind it."""
+    rng = np.random.default_rng(31)
+    x, w, g = (rng.standard_normal(shape).astype(np.float16) for shape in ((2, 40, 4, 32), (32,), (2, 40, 4, 32)))
+    rotary = RotaryTable(16, 40).at(np.arange(40))
+    tx, tw = mg.device_tensor(x), mg.device_tensor(w)
+    y = head_norm(tx, tw, eps=1e-6, rotary=rotary)
+    out = attention(y, y, y, mask=AttentionMask(causal=True))
+    out.backward(mg.device_tensor(g, constant=True))
+    leaf = y.data.copy()
+    alone, dq, dk, dv = run(leaf, leaf, leaf, g, dict(causal=True))
+    assert np.array_equal(out.data, alone)
+    ux, uw = mg.device_tensor(x), mg.device_tensor(w)
+    head_norm(ux, uw, eps=1e-6, rotary=rotary).backward(mg.device_tensor((dq + dk) + dv, constant=True))
+    assert tx.grad.dtype == np.float16 and np.array_equal(tx.grad, ux.grad) and np.array_equal(tw.grad, uw.grad)
