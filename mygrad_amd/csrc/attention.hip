@@ -13,6 +13,7 @@
 #include "attention_rows.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 namespace mg {
@@ -154,7 +155,9 @@ int check_attention(const mg_attention_desc *d, Attention *p, const char *who, b
   p->longest = d->longest ? (int)std::min(d->longest, d->TK) : p->TK;
   p->mean = d->mean ? (int)std::min<int64_t>(d->mean, p->longest) : p->longest;
   p->causal = d->causal != 0, p->window = (int)d->window;
-  p->scale = (float)d->scale, p->cap = (float)d->cap, p->scale64 = d->scale, p->cap64 = d->cap;
+  p->scale = (float)d->scale, p->cap = (float)d->cap;
+  p->bend = d->cap > 0 ? (float)std::max(-(double)FLT_MAX, std::min((double)FLT_MAX, d->scale / d->cap)) : 0.0f;
+  p->scale64 = d->scale, p->cap64 = d->cap;
   p->lengths = d->lengths, p->prefix = d->prefix, p->starts = d->starts, p->ends = d->ends, p->slopes = d->slopes;
   return MG_OK;
 }

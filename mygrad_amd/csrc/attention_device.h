@@ -11,7 +11,7 @@ struct Attention {
   int group;  // query heads that share a key head
   int causal, window;
   int longest, mean;      // keys in use of the item with most, and of all about
-  float scale, cap;       // cap 0: scores as they are
+  float scale, cap, bend;  // cap 0: scores as they are; bend: scale / cap, or float's largest (infinity times a product of zero is no number)
   double scale64, cap64;  // the same for double precision
   const int32_t *lengths, *prefix, *starts, *ends;
   const void *slopes;  // float, double for double precision

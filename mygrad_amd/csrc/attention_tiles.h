@@ -9,7 +9,6 @@
 // Float16 takes a fragment in one v_mfma_f32_32x32x16_f16, float32 in eight v_mfma_f32_32x32x2_f32.
 #pragma once
 
-#include <cfloat>
 #include <type_traits>
 
 #include "attention_device.h"
@@ -350,9 +349,7 @@ struct Scores {
 };
 
 __device__ __forceinline__ Scores scores_of(const Attention &p, int head) {
-  // a quotient beyond float's largest stays that: infinity times a product of zero would be no number
-  const float bend = p.cap > 0 ? __builtin_fminf(__builtin_fmaxf(p.scale / p.cap, -FLT_MAX), FLT_MAX) : 0.0f;
-  return Scores{bend, (p.cap > 0 ? p.cap : p.scale) * kLog2e, p.slopes ? ((const float *)p.slopes)[head] * kLog2e : 0.0f};
+  return Scores{p.bend, (p.cap > 0 ? p.cap : p.scale) * kLog2e, p.slopes ? ((const float *)p.slopes)[head] * kLog2e : 0.0f};
 }
 
 // 32 queries, one in each lane's column (in both halves), on their way through tiles of SUBS times 32 keys: S^T = K Q^T has a query's scores in
