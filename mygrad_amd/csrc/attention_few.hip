@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
   constexpr int kSteps = DP / 16, kTiles = 4 * STAGES * 2 * Tile::kBytes;
   __shared__ __attribute__((aligned(1024))) char space[kTiles > Join::kBytes ? kTiles : Join::kBytes];
   __shared__ float tops[4][32], totals[4][32];
-  __shared__ int bad[4];
+  __shared__ unsigned bad;  // columns to be computed again
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
   const Panel at = panel_of(p, split, c);
 
@@ -158,28 +158,30 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
     tops[0][c] = all > 0 ? 1.0f / all : all == 0 ? 0.0f : NAN;
     if (lse && at.in) lse[((long long)at.b * p.HQ + at.hq) * p.TQ + at.i] = all == 0 ? INFINITY : top + __builtin_log2f(all) - kLift;
   }
+  if (threadIdx.x == 0) bad = 0;
   __syncthreads();
-  bool odd = false;
   for (int n = threadIdx.x; n < at.columns * (DP / 4); n += 256) {
     const int column = n / (DP / 4), d = n % (DP / 4) * 4, all_columns = at.first_column + column;
     if (d >= p.D) continue;
-    const f32x4 value = Join::sum(join, column, d) * tops[0][column];
+    const float by = tops[0][column];
+    const f32x4 value = Join::sum(join, column, d) * by;
     const long long to = (((long long)at.b * p.TQ + all_columns / p.group) * p.HQ + at.hk * p.group + all_columns % p.group) * p.D + d;
-    odd |= put_four(out + to, value);
+    if (put_four(out + to, value) && (by == by || shares_pieces(p, sizeof(T)))) atomicOr(&bad, 1u << column);
     if constexpr (sizeof(T) == 2) {
       if (remains) put_four(remains + to, (value - __builtin_convertvector(__builtin_convertvector(value, f16x4), f32x4)) * kRest);
     }
   }
-  odd = __any(odd);
-  if (lane == 0) bad[wave] = odd;
   all_landed();  // what is stored, too: other wavefronts may write it again
-  if (bad[0] | bad[1] | bad[2] | bad[3])
-    for (int column = at.first_column + wave; column < at.first_column + at.columns; column += 4)
-      attend_row<T, float>(p, at.b, at.hk * p.group + column % p.group, column / p.group, (float *)space + wave * kMaxDim, q, k, v, out, remains, lse);
+  each_marked<1>(&bad, [&](int n) {
+    const int column = at.first_column + n;
+    const int hq = at.hk * p.group + column % p.group, i = column / p.group;
+    const float by = tops[0][n];
+    if (by == by || !out_stands(p, at.b, hq, i, q, k)) attend_row<T, float>(p, at.b, hq, i, (float *)space + wave * kMaxDim, q, k, v, out, remains, lse);
+  });
 }
 
-// A block per row of the result: the splits' sums at a common top, in their order.  A row that comes out as no number is computed once more, so
-// that what it does not see leaves no mark (products with weights of zero do, where that is no number).
+// A block per row of the result: the splits' sums at a common top, in their order.  A row that comes out as no number is computed once more, unless
+// its total is none, so that what it does not see leaves no mark (products with weights of zero do, where that is no number).
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split split, const float *__restrict__ sums, const float2 *__restrict__ ends,
                                                              const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
@@ -224,18 +226,19 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split 
     const T near = (T)value;
     out[to + d] = near;
     if (rest) rest[to + d] = (_Float16)((value - (float)near) * kRest);
-    bad |= !(__builtin_fabsf(value) < INFINITY);
+    bad |= no_number(value);
   }
   if (lse && threadIdx.x == 0) lse[((long long)b * p.HQ + hq) * p.TQ + i] = total == 0 ? INFINITY : top + __builtin_log2f(total) - kLift;
   bad = __any(bad);
   if (lane == 0) odd[wave] = bad;
   all_landed();  // what is stored, too: it may be written again
-  if (wave == 0 && (odd[0] | odd[1] | odd[2] | odd[3])) attend_row<T, float>(p, b, hq, i, mine, q, k, v, out, rest, lse);
+  if (wave == 0 && (odd[0] | odd[1] | odd[2] | odd[3]) && (total == total || !out_stands(p, b, hq, i, q, k))) attend_row<T, float>(p, b, hq, i, mine, q, k, v, out, rest, lse);
 }
 
-// dq of a panel's columns; with one split the result itself.
+// dq of a panel's columns; with one split the result itself.  Up to 64 values a head two blocks share a compute unit: 77 us for
+// 4 x 1024 tokens behind a prefix, 8 heads of 64 in float32, where registers for one block alone made it 94.
 template <typename T, int DP, int STAGES, bool BENT>
-__global__ void __launch_bounds__(256) attention_few_dq_kernel(Attention p, Split split, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
+__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_few_dq_kernel(Attention p, Split split, Stats stats, const T *__restrict__ q, const T *__restrict__ k,
                                                                const T *__restrict__ v, const T *__restrict__ grad, const float *__restrict__ lse,
                                                                T *__restrict__ dq, float *__restrict__ sums) {
   typedef TileOf<T, DP, 32> Tile;
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(256) attention_few_dq_kernel(Attention p, Spli
   typedef Joined<DP> Join;
   constexpr int kSteps = DP / 16, kTiles = 4 * STAGES * 2 * Tile::kBytes;
   __shared__ __attribute__((aligned(1024))) char space[kTiles > Join::kBytes ? kTiles : Join::kBytes];
-  __shared__ int bad[4];
+  __shared__ unsigned bad;  // columns to be computed again
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
   const Panel at = panel_of(p, split, c);
 
@@ -256,6 +259,7 @@ __global__ void __launch_bounds__(256) attention_few_dq_kernel(Attention p, Spli
   }
   const long long stat = ((long long)at.b * p.HQ + at.hq) * p.TQ + (at.in ? at.i : 0);
   const float level = at.in ? stats.level[stat] : INFINITY, delta = at.in ? stats.delta[stat] : 0.0f;
+  const unsigned stand = marks_of(dq_stands(at.span, level, delta));
   const Scores how = scores_of(p, at.hq);
 
   Pulled<T, DP, 32, BENT> run;
@@ -266,28 +270,28 @@ __global__ void __launch_bounds__(256) attention_few_dq_kernel(Attention p, Spli
     run.take(p, how, keys, 0, rows, grads, level, delta, at.span, key0, whole, place, h);
   });
 
+  if (threadIdx.x == 0) bad = 0;
   __syncthreads();
   float *join = (float *)space;
   Join::put(join, run.sums, run.by(p), wave, c, h);
   __syncthreads();
   const long long base = ((long long)at.pair * split.splits + at.part) * split.columns + at.first_column;
-  bool odd = false;
   for (int n = threadIdx.x; n < at.columns * (DP / 4); n += 256) {
     const int column = n / (DP / 4), d = n % (DP / 4) * 4, all_columns = at.first_column + column;
     if (d >= p.D) continue;
     const f32x4 value = Join::sum(join, column, d);
     if (split.splits > 1)
       *(f32x4 *)(sums + (base + column) * p.D + d) = value;
-    else
-      odd |= put_four(dq + (((long long)at.b * p.TQ + all_columns / p.group) * p.HQ + at.hk * p.group + all_columns % p.group) * p.D + d, value);
+    else if (put_four(dq + (((long long)at.b * p.TQ + all_columns / p.group) * p.HQ + at.hk * p.group + all_columns % p.group) * p.D + d, value) &&
+             !(stand >> column & 1))
+      atomicOr(&bad, 1u << column);
   }
   if (split.splits > 1) return;
-  odd = __any(odd);
-  if (lane == 0) bad[wave] = odd;
   all_landed();  // what is stored, too: other wavefronts may write it again
-  if (bad[0] | bad[1] | bad[2] | bad[3])
-    for (int column = at.first_column + wave; column < at.first_column + at.columns; column += 4)
-      dq_row<T, float>(p, at.b, at.hk * p.group + column % p.group, column / p.group, (float *)space + wave * 2 * kMaxDim, q, k, v, grad, lse, stats.delta, dq);
+  each_marked<1>(&bad, [&](int n) {
+    const int column = at.first_column + n;
+    dq_row<T, float>(p, at.b, at.hk * p.group + column % p.group, column / p.group, (float *)space + wave * 2 * kMaxDim, q, k, v, grad, lse, stats.delta, dq);
+  });
 }
 
 // A wavefront per row of dq.
@@ -315,7 +319,8 @@ __global__ void __launch_bounds__(256) attention_dq_join_kernel(Attention p, Spl
 #pragma unroll
   for (int m = 0; m < PARTS; ++m)
     if (lane + 64 * m < p.D) dq[at_row * p.D + lane + 64 * m] = (T)sum[m], odd |= !(__builtin_fabsf(sum[m]) < INFINITY);
-  if (__any(odd)) {
+  const long long stat = ((long long)b * p.HQ + hq) * p.TQ + i;
+  if (__any(odd) && !dq_stands(span_of(p, b, i), stats.level[stat], stats.delta[stat])) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     dq_row<T, float>(p, b, hq, i, mine[wave], q, k, v, grad, lse, stats.delta, dq);
   }

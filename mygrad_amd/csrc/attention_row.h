@@ -177,4 +177,80 @@ __device__ __forceinline__ void dkv_row(const Attention &p, int b, int hk, int j
     if (lane + 64 * c < p.D) dk[at + lane + 64 * c] = (T)sum_k[c], dv[at + lane + 64 * c] = (T)sum_v[c];
 }
 
+// ---- which rows to compute once more -------------------------------------------------------------------------------------------
+// A row of a result that is no number has to be computed again by the functions above only if what it does not see may have made it one.  It need
+// not where what it sees does, whatever stands elsewhere:
+//   out: the sum of the row's weights is no number (scores of unseen keys never enter it; where rows share pieces in LDS: and q_i or a key is none);
+//   dq:  lse_i or D_i of the row is none, which makes each of its dS_ij none (a row that sees nothing has no dS);
+//   dk, dv: the same of a query that sees the key, for all of dk and for dv where that query's grad is none (all of it where lse_i is).
+// So an upstream gradient that overflowed, or operands that are no numbers throughout, cost a step what numbers do.
+template <typename C>
+__device__ __forceinline__ bool no_number(C v) { return !(fabs(v) < INFINITY); }
+
+__device__ __forceinline__ bool dq_stands(const Span &span, float lse, float delta) { return span.hi > span.lo && (lse != lse || no_number(delta)); }
+
+// Whether row i of an attention, whose weights' sum is no number, stands; the same in every lane.  An infinity may give weights of zero: those are
+// computed again.
+template <typename T>
+__device__ __forceinline__ bool out_stands(const Attention &p, int b, int h, int i, const T *__restrict__ q, const T *__restrict__ k) {
+  if (!shares_pieces(p, sizeof(T))) return true;
+  const int lane = threadIdx.x & 63;
+  const Span span = span_of(p, b, i);
+  if (span.hi <= span.lo) return false;
+  const T *row = q + (((long long)b * p.TQ + i) * p.HQ + h) * p.D, *keys = k + ((long long)b * p.TK * p.HK + h / p.group) * p.D;
+  auto none = [&](const T *from) {
+    bool none = false;
+    for (int d = lane; d < p.D; d += 64) none |= from[d] != from[d];
+    return none;
+  };
+  if (__any(none(row))) return true;
+  for (int j = span.lo; j < span.hi; ++j)
+    if (__any(none(keys + (long long)j * p.HK * p.D))) return true;
+  return false;
+}
+
+// Whether row j of dk (`of_k`: it holds one that is no number) and dv (bit c of `of_v`: value lane + 64 c is none) stands; the same in every lane.
+template <typename T>
+__device__ __forceinline__ bool dkv_stands(const Attention &p, int b, int hk, int j, bool of_k, unsigned of_v, const T *__restrict__ grad,
+                                           const float *__restrict__ lse, const float *__restrict__ delta) {
+  const int lane = threadIdx.x & 63;
+  for (int h = hk * p.group; h < (hk + 1) * p.group; ++h) {
+    const long long head = ((long long)b * p.TQ * p.HQ + h) * p.D, step = (long long)p.HQ * p.D, stats = ((long long)b * p.HQ + h) * p.TQ;
+    for (int i0 = 0; i0 < p.TQ; i0 += 64) {
+      const int i = i0 + lane;
+      bool all = false, some = false;
+      if (i < p.TQ) {
+        const Span span = span_of(p, b, i);
+        if (j >= span.lo && j < span.hi) all = lse[stats + i] != lse[stats + i], some = no_number(delta[stats + i]);
+      }
+      if (__any(all)) return true;
+      for (unsigned long long left = __ballot(some); left; left &= left - 1) {
+        of_k = false;
+        const T *row = grad + head + (i0 + __ffsll(left) - 1) * step;
+#pragma unroll
+        for (int c = 0; c < kParts; ++c)
+          if ((of_v >> c & 1) && no_number((float)row[lane + 64 * c])) of_v &= ~(1u << c);
+        if (!__any(of_v)) return true;
+      }
+    }
+  }
+  return !of_k && !__any(of_v);
+}
+
+// The rows that lanes c and 32 + c of a wavefront mark, as bits.
+__device__ __forceinline__ unsigned marks_of(bool mark) {
+  const unsigned long long all = __ballot(mark);
+  return (unsigned)all | (unsigned)(all >> 32);
+}
+
+// f(row) for the rows marked in `words`, shared out among four wavefronts.
+template <int WORDS, typename F>
+__device__ __forceinline__ void each_marked(const unsigned *words, F f) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int turn = 0;
+  for (int w = 0; w < WORDS; ++w)
+    for (unsigned left = __builtin_amdgcn_readfirstlane(words[w]); left; left &= left - 1, ++turn)
+      if ((turn & 3) == wave) f(32 * w + __ffs(left) - 1);
+}
+
 }  // namespace mg

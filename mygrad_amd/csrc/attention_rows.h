@@ -9,6 +9,9 @@ namespace mg {
 // What a float16 result leaves out is kept as this times it, in float16: 2^11, so that it is about as large as the result.
 constexpr float kRest = 2048.0f;
 
+// In float16 the last piece of a row in LDS may hold values of the next one, which meet zeros: scores that come out as no number need not be.
+__device__ __forceinline__ bool shares_pieces(const Attention &p, int size) { return p.D * size % 16 != 0; }
+
 bool tiles_take(const Attention &p, int size, uintptr_t ends);
 int forward_tiles(const Attention &p, int dtype, const void *q, const void *k, const void *v, void *out, void *rest, void *lse);
 

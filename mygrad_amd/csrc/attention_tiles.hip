@@ -1,8 +1,8 @@
 // Attention of float16 and float32 on the matrix cores: tiles of queries against tiles of keys, one pass with the running maximum
 // and sum of the softmax, nothing of the scores in memory.
 //
-// The tiles' products multiply what a row does not see by weights of zero, which an infinity or a NaN there turns into NaN.  So a block
-// whose results hold one that is no number computes its rows once more, a row at a time (attention_row.h); few have to.
+// The tiles' products multiply what a row does not see by weights of zero, which an infinity or a NaN there turns into NaN.  So rows
+// whose results hold one that is no number are computed once more, a row at a time, unless what they see explains it (attention_row.h).
 #include "attention_tiles.h"
 
 #include "attention_row.h"
@@ -30,7 +30,7 @@ attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T 
   constexpr int kSteps = DP / 16, kParts = DP / 32;
   __shared__ __attribute__((aligned(1024))) char tiles[4 * Tile::kBytes];
   __shared__ int edges[2][4];
-  __shared__ int bad[4];
+  __shared__ unsigned bad[2][4];  // rows with one that is no number, and those whose weights' sum is none
   const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)tiles;
   const Dealt at = dealt(deal, blockIdx.x);
   const int b = at.pair / p.HK, hk = at.pair % p.HK, hq = hk * p.group + at.head;
@@ -82,7 +82,7 @@ attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T 
 
   const float total = sum_halves(run.total);
   const float by = total > 0 ? 1.0f / total : total == 0 ? 0.0f : NAN;
-  bool odd = !(__builtin_fabsf(by) < INFINITY);
+  bool odd = false;
   if (in) {
     const long long to = (((long long)b * p.TQ + i) * p.HQ + hq) * p.D;
 #pragma unroll
@@ -98,12 +98,14 @@ attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T 
       }
     if (lse && h == 0) lse[((long long)b * p.HQ + hq) * p.TQ + i] = total == 0 ? INFINITY : run.top + __builtin_log2f(total) - kLift;
   }
-  odd = __any(in && odd);
-  if (lane == 0) bad[wave] = odd;
+  const unsigned marks = marks_of(odd), none = marks_of(odd && total != total);
+  if (lane == 0) bad[0][wave] = marks, bad[1][wave] = none;
   all_landed();  // what is stored, too: other wavefronts may write it again
-  if (bad[0] | bad[1] | bad[2] | bad[3])
-    for (int again = tile * kBlockRows + wave; again < min(p.TQ, (tile + 1) * kBlockRows); again += 4)
+  each_marked<4>(bad[0], [&](int n) {
+    const int again = tile * kBlockRows + n;
+    if (!(bad[1][n >> 5] >> (n & 31) & 1) || !out_stands(p, b, hq, again, q, k))
       attend_row<T, float>(p, b, hq, again, (float *)tiles + wave * kMaxDim, q, k, v, out, rest, lse);
+  });
 }
 
 // ---- gradient ----------------------------------------------------------------------------------------------------------------
@@ -170,7 +172,7 @@ attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q
   constexpr int kSteps = DP / 16, kParts = DP / 32, kSubs = KEYS / 32;
   __shared__ __attribute__((aligned(1024))) char tiles[4 * Tile::kBytes];
   __shared__ int edges[2][4];
-  __shared__ int bad[4];
+  __shared__ unsigned bad[4];
   const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)tiles;
   const Dealt at = dealt(deal, blockIdx.x);
   const int b = at.pair / p.HK, hk = at.pair % p.HK, hq = hk * p.group + at.head;
@@ -190,6 +192,7 @@ attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q
   }
   const long long stat = ((long long)b * p.HQ + hq) * p.TQ + (in ? i : 0);
   const float own_level = in ? stats.level[stat] : INFINITY, delta = in ? stats.delta[stat] : 0.0f;
+  const bool stands = dq_stands(span, own_level, delta);
 
   __syncthreads();
   const int lo = __builtin_amdgcn_readfirstlane(min(min(edges[0][0], edges[0][1]), min(edges[0][2], edges[0][3])));
@@ -236,12 +239,12 @@ attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q
         if (d < p.D) odd |= put_four(dq + row + d, four_of(run.sums[n], r) * by);
       }
   }
-  odd = __any(odd);
-  if (lane == 0) bad[wave] = odd;
+  const unsigned marks = marks_of(odd && !stands);
+  if (lane == 0) bad[wave] = marks;
   all_landed();  // what is stored, too: other wavefronts may write it again
-  if (bad[0] | bad[1] | bad[2] | bad[3])
-    for (int again = tile * kBlockRows + wave; again < min(p.TQ, (tile + 1) * kBlockRows); again += 4)
-      dq_row<T, float>(p, b, hq, again, (float *)tiles + wave * 2 * kMaxDim, q, k, v, grad, lse, stats.delta, dq);
+  each_marked<4>(bad, [&](int n) {
+    dq_row<T, float>(p, b, hq, tile * kBlockRows + n, (float *)tiles + wave * 2 * kMaxDim, q, k, v, grad, lse, stats.delta, dq);
+  });
 }
 
 // dv^T = grad^T P and dk^T = q^T dS: a block keeps 128 keys, 32 for each wavefront in its lanes' columns, and goes through the chunks of queries
@@ -263,7 +266,7 @@ attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ 
   constexpr int kBuffer = 2 * Tile::kBytes + 4 * 256;  // rows of q and grad; level, delta, lo, hi of each
   typedef TileOf<T, DP, kBlockRows> Whole;
   __shared__ __attribute__((aligned(1024))) char tiles[2 * kBuffer + (VALUES ? Whole::kBytes : 0)];
-  __shared__ int bad[4];
+  __shared__ unsigned bad[2][4];  // rows with one that is no number in dk or dv, and in dk
   const unsigned lds = (unsigned)(unsigned long long)(MG_LDS char *)tiles;
   const Dealt at = dealt(deal, blockIdx.x);  // its head is the cut
   const int b = at.pair / p.HK, hk = at.pair % p.HK;
@@ -421,7 +424,7 @@ attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ 
   }
 
   const float lift = sizeof(T) == 2 ? 0x1p-14f : 1.0f, by = sizeof(T) == 2 ? p.scale / unit.by * lift : p.scale;  // 2^-kShift
-  bool odd = false;
+  bool odd_k = false, odd_v = false;
   if (in) {
 #pragma unroll
     for (int n = 0; n < kParts; ++n)
@@ -430,8 +433,8 @@ attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ 
         const int d = 32 * n + row_of(r, h);
         if (d >= p.D) continue;
         if (cuts == 1) {
-          odd |= put_four(dk + row + d, four_of(sum_k[n], r) * by);
-          odd |= put_four(dv + row + d, four_of(sum_v[n], r) * lift);
+          odd_k |= put_four(dk + row + d, four_of(sum_k[n], r) * by);
+          odd_v |= put_four(dv + row + d, four_of(sum_v[n], r) * lift);
         } else {
           const long long all = (long long)p.B * p.TK * p.HK * p.D;
           put_four(parts + at.head * all + row + d, four_of(sum_k[n], r) * by);
@@ -440,12 +443,27 @@ attention_dkv_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ 
       }
   }
   if (cuts > 1) return;
-  odd = __any(odd);
-  if (lane == 0) bad[wave] = odd;
+  const unsigned marks_k = marks_of(odd_k), marks = marks_k | marks_of(odd_v);
+  unsigned *which = (unsigned *)(tiles + 4 * 2 * kMaxDim * sizeof(float));  // a bit for each value of dv that is no number, behind what rows need
+  static_assert(4 * 2 * kMaxDim * sizeof(float) + kBlockRows * kParts * sizeof(unsigned) <= sizeof tiles, "marks do not fit");
+  if (marks) {
+#pragma unroll
+    for (int n = 0; n < kParts; ++n) {
+      unsigned bits = 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) bits |= no_number(sum_v[n][r] * lift) && 32 * n + row_of(r, h) < p.D ? 1u << row_of(r, h) : 0u;
+      bits |= __shfl_xor(bits, 32);
+      if (h == 0) which[(wave * 32 + c) * kParts + n] = bits;
+    }
+  }
+  if (lane == 0) bad[0][wave] = marks, bad[1][wave] = marks_k;
   all_landed();  // what is stored, too: other wavefronts may write it again
-  if (bad[0] | bad[1] | bad[2] | bad[3])
-    for (int again = block0 + wave; again < min(p.TK, block0 + kBlockRows); again += 4)
-      dkv_row<T, float>(p, b, hk, again, (float *)tiles + wave * 2 * kMaxDim, q, k, v, grad, lse, stats.delta, dk, dv);
+  each_marked<4>(bad[0], [&](int n) {
+    unsigned of_v = 0;
+    for (int m = lane >> 5; m < kParts; m += 2) of_v |= (which[n * kParts + m] >> (lane & 31) & 1) << (m >> 1);
+    if (!dkv_stands(p, b, hk, block0 + n, bad[1][n >> 5] >> (n & 31) & 1, of_v, grad, lse, stats.delta))
+      dkv_row<T, float>(p, b, hk, block0 + n, (float *)tiles + wave * 2 * kMaxDim, q, k, v, grad, lse, stats.delta, dk, dv);
+  });
 }
 
 constexpr int kJoinKeys = 16;
@@ -457,26 +475,36 @@ __global__ void __launch_bounds__(256) attention_dkv_join_kernel(Attention p, St
                                                                  const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
                                                                  const T *__restrict__ grad, const float *__restrict__ lse, T *__restrict__ dk,
                                                                  T *__restrict__ dv) {
-  __shared__ int bad[4];
+  __shared__ unsigned bad[2], which[kJoinKeys][kMaxDim / 32];  // rows as in attention_dkv_kernel, and a bit for each value of dv
   __shared__ float mine[4][2 * kMaxDim];
+  if (threadIdx.x < 2) bad[threadIdx.x] = 0;
+  if (threadIdx.x < kJoinKeys * (kMaxDim / 32)) which[0][threadIdx.x] = 0;
+  __syncthreads();
   const int pair = blockIdx.x / tiles, tile = blockIdx.x % tiles, b = pair / p.HK, hk = pair % p.HK, of_row = p.D / 4;
   const long long all = (long long)p.B * p.TK * p.HK * p.D;
-  bool odd = false;
   for (int n = threadIdx.x; n < 2 * kJoinKeys * of_row; n += 256) {
-    const int which = n / (kJoinKeys * of_row), rest = n - which * kJoinKeys * of_row, j = tile * kJoinKeys + rest / of_row;
+    const int of_v = n / (kJoinKeys * of_row), rest = n - of_v * kJoinKeys * of_row, row = rest / of_row, j = tile * kJoinKeys + row, d = rest % of_row * 4;
     if (j >= p.TK) continue;
-    const long long at = (((long long)b * p.TK + j) * p.HK + hk) * p.D + rest % of_row * 4;
+    const long long at = (((long long)b * p.TK + j) * p.HK + hk) * p.D + d;
     f32x4 sum{};
-    for (int m = 0; m < cuts; ++m) sum += *(const f32x4 *)(parts + (which * cuts + m) * all + at);
-    odd |= put_four((which ? dv : dk) + at, sum);
+    for (int m = 0; m < cuts; ++m) sum += *(const f32x4 *)(parts + (of_v * cuts + m) * all + at);
+    if (put_four((of_v ? dv : dk) + at, sum)) {
+      atomicOr(&bad[0], 1u << row);
+      if (!of_v) atomicOr(&bad[1], 1u << row);
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+        if (of_v && no_number(sum[m])) atomicOr(&which[row][d >> 5], 1u << ((d & 31) + m));
+    }
   }
-  odd = __any(odd);
-  if ((threadIdx.x & 63) == 0) bad[threadIdx.x >> 6] = odd;
   all_landed();
-  const int wave = threadIdx.x >> 6;
-  if (bad[0] | bad[1] | bad[2] | bad[3])
-    for (int again = tile * kJoinKeys + wave; again < min(p.TK, (tile + 1) * kJoinKeys); again += 4)
-      dkv_row<T, float>(p, b, hk, again, mine[wave], q, k, v, grad, lse, stats.delta, dk, dv);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  each_marked<1>(bad, [&](int n) {
+    unsigned of_v = 0;
+#pragma unroll
+    for (int c = 0; c < kParts; ++c) of_v |= (which[n][2 * c + (lane >> 5)] >> (lane & 31) & 1) << c;
+    if (!dkv_stands(p, b, hk, tile * kJoinKeys + n, bad[1] >> n & 1, of_v, grad, lse, stats.delta))
+      dkv_row<T, float>(p, b, hk, tile * kJoinKeys + n, mine[wave], q, k, v, grad, lse, stats.delta, dk, dv);
+  });
 }
 
 // How many cuts the blocks of attention_dkv_kernel are made in: as many as make the estimate of the time least.  A block takes `chunk` for each

@@ -1,9 +1,12 @@
 """How near attention and its gradients come to their formulas in 64 bits."""
 
+import time
+
 import numpy as np
 import pytest
 
 import mygrad_amd as mg
+from mygrad_amd import _hip
 from mygrad_amd.nnet import AttentionMask, RotaryTable, attention, head_norm
 from oracle import attention as ora
 from tests.attention_bars import CASES, Formulas, bars_of, formulas_and_bars, name_of, operands
@@ -71,7 +74,7 @@ def test_smallest_and_largest_caps(dtype, TQ, cap, scale):
 
 
 def test_entry_points_refuse_scores_beyond_single_precision():
-    from mygrad_amd import _device, _hip
+    from mygrad_amd import _device
 
     lib, buf = _hip.lib(), _device.DeviceBuffer(1 << 16)
     for dtype, status in ((0, -2), (2, -2), (1, 0)):
@@ -142,3 +145,56 @@ def test_float16_through_other_operations():
     ux, uw = mg.device_tensor(x), mg.device_tensor(w)
     head_norm(ux, uw, eps=1e-6, rotary=rotary).backward(mg.device_tensor((dq + dk) + dv, constant=True))
     assert tx.grad.dtype == np.float16 and np.array_equal(tx.grad, ux.grad) and np.array_equal(tw.grad, uw.grad)
+
+
+def milliseconds(operands, grad, mask):
+    """Shortest of four forward and backward passes."""
+    tensors, grad, best = [mg.device_tensor(a) for a in operands], mg.device_tensor(grad, constant=True), [np.inf, np.inf]
+    for _ in range(4):
+        at = []
+        for step in (lambda: None, lambda: attention(*tensors, mask=mask), lambda: out.backward(grad)):
+            out = step()
+            _hip.synchronize()
+            at.append(1e3 * time.perf_counter())
+        best = [min(b, t) for b, t in zip(best, np.diff(at))]
+    return best
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("B,T,HQ,HK,D", [(2, 2048, 8, 2, 64), (1, 700, 4, 1, 128), (2, 1500, 8, 8, 36)])
+def test_an_overflow_costs_a_step_what_numbers_do(dtype, B, T, HQ, HK, D):
+    """An upstream gradient of infinities (a scaled loss that overflowed), in all or in some values, and operands that are no numbers: every row
+    of a block is no number by what it sees.  A row at a time they took 30 to 260 times as long; a third of that ratio is allowed here."""
+    rng = np.random.default_rng(T)
+    q, k, v, g = (rng.standard_normal((B, T, heads, D)).astype(dtype) for heads in (HQ, HK, HK, HQ))
+    mask = AttentionMask(causal=True)
+
+    some = g.copy()
+    some[:, T // 2:, :, 3] = np.inf
+    clean = milliseconds((q, k, v), g, mask)
+    for operands, grad in (((q, k, v), np.full_like(g, np.inf)), ((q, k, v), some), ([np.full_like(a, np.nan) for a in (q, k, v)], g)):
+        for way, spoilt in zip(clean, milliseconds(operands, grad, mask)):
+            assert spoilt < 0.3 + 5 * way, (way, spoilt)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("B,T,HQ,HK,D", EACH_WAY)
+def test_infinite_gradients_of_some_queries_and_values(dtype, B, T, HQ, HK, D):
+    """dv of a key is no number where a query that sees it has none, and nowhere else; dk and dq wherever such a query has a part in them."""
+    case = dict(dtype=dtype, shape=(B, T, T, HQ, HK, D), mask=dict(causal=True), cap=None, bias=False, scale=None, grad_scale=1.0)
+    (q, k, v, g), seen, how = operands(case)
+    f = Formulas(q, k, v, g, seen, **how)
+    spoilt = g.copy()
+    at, heads = [2, T // 2, T // 2 + 1], slice(HQ - 1, HQ)
+    spoilt[:, at, heads, 1:3] = np.inf
+    out, dq, dk, dv = run(q, k, v, spoilt, case["mask"])
+    bars = bars_of(dtype, f)
+    finite_q = np.ones(q.shape, bool)
+    finite_q[:, at, heads] = False
+    finite_k, finite_v = np.ones(k.shape, bool), np.ones(k.shape, bool)
+    finite_k[:, :max(at) + 1, HK - 1] = False
+    finite_v[:, :max(at) + 1, HK - 1, 1:3] = False
+    for have, which, finite in ((out, 0, np.ones(q.shape, bool)), (dq, 1, finite_q), (dk, 2, finite_k), (dv, 3, finite_v)):
+        assert np.array_equal(np.isfinite(have), finite), which
+        over = np.abs(np.where(finite, have, 0).astype(np.float64) - np.where(finite, f.results[which], 0)) - bars[which]
+        assert (over <= 0).all(), (which, over.max())
