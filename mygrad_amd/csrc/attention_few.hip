@@ -5,7 +5,8 @@
 //
 // With a step of generation over a cache this is bound by reading keys and values once: the sixteen products of a tile (128 values a head, float16)
 // wait for its bytes even where most columns are empty.  32 histories of 4000 to 8000 tokens, 32 heads over 8 of 128 in float16 (787 MB): 154 us, 5.1
-// TB/s (a stream that only reads reaches 6.25, a copy 5.2); one history of 131001 tokens with a cap (537 MB): 105 and 6 to join, 4.8 TB/s.  A block holds 128 KB of tiles, one block a compute unit: four wavefronts with two tiles of 16 KB each.
+// TB/s (a stream that only reads reaches 6.25, a copy 5.2); one history of 131001 tokens with a cap (537 MB): 105 and 6 to join, 4.8 TB/s.  At 128 values a
+// head a block holds 128 KB of tiles, one block a compute unit: four wavefronts with two tiles of 16 KB each (float32 one of twice that).
 #include "attention_tiles.h"
 
 #include "attention_row.h"
@@ -341,8 +342,8 @@ void with_parts(const Attention &p, F f) {
 template <typename T>
 constexpr int stages_of(int dim) { return sizeof(T) == 2 && dim <= 128 ? 2 : 1; }
 
-// Keys are split until there is a block for each compute unit, and no further: a block takes a unit's LDS to itself, so the next one's first tiles
-// wait for its last.  One history of 131001 tokens, 32 heads over 8 of 128, float16: 110 us with the join, 140 in eight times as many blocks; 32 of 4000
+// Keys are split until there is a block for each compute unit, and no further: at 128 values a head, where this was measured, a block takes a unit's
+// LDS to itself, so the next one's first tiles wait for its last (at 64 two blocks would fit a unit).  One history of 131001 tokens, 32 heads over 8 of 128, float16: 110 us with the join, 140 in eight times as many blocks; 32 of 4000
 // to 8000 tokens 156 in one piece, 170.  Where lengths differ, for as many times more as the longest has the mean.  Pieces are 128 keys (a tile for
 // each wavefront) or more; with more queries a join takes as long as 512.
 Split split_of(const Attention &p) {

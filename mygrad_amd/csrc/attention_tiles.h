@@ -287,7 +287,7 @@ __device__ __forceinline__ typename Fragment<T>::V rows_of(const f32x16 &v, int 
 // a times both: a float32 value in two of float16 keeps 22 bits (one is all of it in float32).  Weights and gradients of scores are multiplied so,
 // and a result in float16 is off by its own rounding and no more.  Rounded to 11 bits weights would make out and dv off by 1.3 to 1.4 times that
 // and, by what grad . out is off, dq and dk by 1.05 times; gradients of scores dq and dk by half as much again.  The third product of a tile forward and
-// the sixth of dk and dv cost a tenth of a step: 8192 packed tokens, 16 heads of 128, 515 us against 568, 4 x 2048 of 16 over 4 with a cap 614 against 674.
+// the sixth of dk and dv cost a tenth of a step: 8192 packed tokens, 16 heads of 128, 515 us against 568, 4 x 2048 of 16 over 4 with a cap 614 against 668.
 template <typename T>
 __device__ __forceinline__ f32x16 mma_of_two(typename Fragment<T>::V a, typename Fragment<T>::V b, typename Fragment<T>::V more, f32x16 c) {
   c = Fragment<T>::mma(a, b, c);
@@ -339,7 +339,8 @@ __device__ __forceinline__ void tanh_of_all(f32x16 &x) {
   }
 }
 
-// Weights are kept as 2^kLift times exp2(score - top): in float16 they are whole down to 2^-29 of the row's largest then.  `top` follows the
+// Weights are kept as 2^kLift times exp2(score - top): in float16 they are whole down to 2^-21 of the row's largest then, down to 2^-29 as `top` lags
+// behind it, and their second parts down to 2^-31.  `top` follows the
 // row's maximum only when that has grown by more than kSlack, so the sums are seldom scaled; 2^(kLift + kSlack) stays below 65504.
 constexpr float kLift = 7.0f, kSlack = 8.0f;
 
@@ -577,10 +578,10 @@ void with_shape(const Attention &p, F f) {
 
 // How the blocks of a launch are dealt out: `pairs` of a batch item and a key head, each with `heads` query heads and `tiles` row tiles.
 // Blocks go to the eight XCDs in turn, so with a multiple of eight pairs each pair stays on one XCD and is read through one L2.  The last tiles,
-// which see most where the mask is causal, come first: of one pair after the other where one fills an XCD, else of as many as do.  Where all
-// blocks run at once, two on a compute unit, the second half comes the other way round, so that the unit with most of the first gets least of
-// it: 2 x 4096 causal tokens, 16 heads of 128 in float16, dk and dv 495 to 425 us, dq 327 to 303, forward 197 to 190; 4 x 1024 behind a prefix, 8
-// heads of 64 in float32, dk and dv 144 to 101.
+// which see most where the mask is causal, come first: of one pair after the other where one fills an XCD, else of as many as do.  2 x 4096 causal
+// tokens, 16 heads of 128 in float16, with the first tiles first and with the last: dk and dv 538 and 425 us, dq 326 and 274, forward 254 and 219.  Where
+// all blocks run at once, two on a compute unit, the second half comes the other way round, so that the unit with most of the first gets least of
+// it: 4 x 1024 behind a prefix, 8 heads of 64 in float32, dk and dv 112 to 100.
 struct Deal {
   int pairs, heads, tiles;
   int beside;  // pairs of an XCD whose tiles are dealt in turn
@@ -616,8 +617,8 @@ __device__ __forceinline__ Dealt dealt(const Deal &d, int block) {
 }
 
 // The tile of a batch item that is `rank`-th in work, where documents make that uneven; each wavefront finds it for itself, a tile a lane or
-// four.  The work is an estimate by the tile's first and last row.  8192 tokens of five documents, 16 heads of 128, float16: dk and dv 301 to 240
-// us, dq 183 to 159, forward 119 to 113.
+// four.  The work is an estimate by the tile's first and last row.  8192 tokens of five documents, 16 heads of 128, float16: dk and dv 313 to 275
+// us, dq 168 to 166, forward 136 to 135.
 template <bool KEYS, int EACH>
 __device__ __forceinline__ int tile_of_rank(const Attention &p, int b, int rank, int tiles, int rows) {
   const int lane = threadIdx.x & 63, tokens = KEYS ? p.TK : p.TQ;

@@ -19,8 +19,8 @@ constexpr int kBlockRows = 128;  // queries of a block: 32 for each of its four 
 // queries share the tiles of keys and values, the next ones on their way while these are multiplied; 64 keys in two buffers are 64 KB at 128
 // values of float16, so two blocks share a compute unit and one's products run while the other takes exponentials (with half of the unit's
 // queries gone, as at the end of a causal launch, three fifths of the rate are left).  Float32's products take eight times as long: 32 keys do.
-// 2 x 4096 tokens, 16 heads of 128, float16: 314 us (875 TFLOP/s; a large product reaches 1168), causal 190 (720), with a cap 400 (687); of 64:
-// 188 (730).  2 x 2048, 8 heads of 128, float32: 303 (113; a large product 154).
+// 2 x 4096 tokens, 16 heads of 128, float16: 382 us (1080 TFLOP/s of three products, as weights come in two parts; a large product reaches 1168), causal
+// 220 (940), with a cap 480 (860); of 64: 227 (910).  2 x 2048, 8 heads of 128, float32: 324 (106; a large product 154).
 template <typename T, int DP, int KEYS, bool BENT>
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
 attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, T *__restrict__ out,
@@ -161,8 +161,8 @@ __global__ void __launch_bounds__(256) attention_stats_kernel(Attention p, Stats
 
 // dq^T = K^T dS^T: as the forward pass, with the queries' rows of grad beside those of q; S and dP are formed again here and by the keys'
 // kernel, two of seven products more than one kernel would need, which would have to add to dq or to dk and dv across blocks, in no order.
-// Bound by the matrix cores: 2 x 4096 tokens, 16 heads of 128, float16: 530 us (1040 TFLOP/s, dS in two counted), causal 303; float32, 2 x 2048, 8
-// heads of 128: 430 (120 of 154).
+// Bound by the matrix cores: 2 x 4096 tokens, 16 heads of 128, float16: 500 us (1100 TFLOP/s of four products, dS in two counted), causal 276;
+// float32, 2 x 2048, 8 heads of 128: 455 (113 of 154).
 template <typename T, int DP, int KEYS, bool BENT>
 __global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 64 : 128) ? 1 : 2)
 attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
@@ -250,9 +250,9 @@ attention_dq_kernel(Attention p, Deal deal, Stats stats, const T *__restrict__ q
 // dv^T = grad^T P and dk^T = q^T dS: a block keeps 128 keys, 32 for each wavefront in its lanes' columns, and goes through the chunks of queries
 // that see any of them, head by head of those that share the keys.  Where there are few blocks they are cut: each of `cuts` takes an equal share
 // of the chunks and leaves its sums in float32, which attention_dkv_join_kernel adds up in order.
-// Bound by the matrix cores: 2 x 4096 tokens, 16 heads of 128, float16: 712 us (1160 TFLOP/s, dS in two counted), causal 425; float32, 2 x 2048,
-// 8 heads of 128: 620 (111 of 154).  Documents end at different times, which leaves units idle: 8192 tokens of five of
-// them, 16 heads of 128, take 241 us where even work would take 170; cut in two they would leave 134 MB of sums to be joined in 80 us.
+// Bound by the matrix cores: 2 x 4096 tokens, 16 heads of 128, float16: 775 us (1065 TFLOP/s of six products, P and dS in two counted), causal 425;
+// float32, 2 x 2048, 8 heads of 128: 582 (118 of 154).  Documents end at different times, which leaves units idle: 8192 tokens of five of them, 16
+// heads of 128, take 275 us where even work would take 200; cut in two they would leave 134 MB of sums to be joined in 80 us.
 // With VALUES the keys' values lie in LDS instead of registers: at 128 values of float16 a head the two results and k take 160 of a lane's 256,
 // and with v's 32 as well the scores would not fit.
 template <typename T, int DP, int ROWS, bool VALUES, bool BENT>
@@ -510,8 +510,8 @@ __global__ void __launch_bounds__(256) attention_dkv_join_kernel(Attention p, St
 // How many cuts the blocks of attention_dkv_kernel are made in: as many as make the estimate of the time least.  A block takes `chunk` for each
 // chunk of queries it goes through, while two of them on a compute unit run beside each other in float16 (in float32 one keeps the matrix cores
 // four fifths busy), and the first keys of a causal mask are seen by all queries, twice the mean.  Joining takes a launch and 16 bytes written
-// and read for each value of k and cut.  Measured at 4 x 2048 tokens, 16 heads over 4, causal, float16: 604 us in one piece, 415 in two, 285 in four;
-// 4 x 75 tokens, 32 heads over 4: 60 in one, 26 in eight.
+// and read for each value of k and cut.  Measured with the join at 4 x 2048 tokens, 16 heads over 4, causal, float16: 490 us in one piece, 297 in two, 258 in
+// four; 4 x 75 tokens, 32 heads over 4: 64 in one, 45 in two, 35 in eight.
 int cuts_of(const Attention &p, const Stats &stats, int size, int blocks) {
   const double at_once = (size == 2 ? 2.0 : 1.25) * runtime().props.multiProcessorCount, every = (double)p.group * stats.chunks;
   const double chunk = 1e-6 + stats.rows * 128.0 * ((p.D + 31) / 32 * 32) * 8 / (size == 2 ? 3.0e12 : 0.5e12);
@@ -588,8 +588,8 @@ int backward_of(const Attention &p, const void *q, const void *k, const void *v,
 }  // namespace
 
 // Head dimensions that are multiples of 4, up to 128 or, in float16, 256, in buffers that start on 16 bytes, rows of a tile within reach
-// of 32 bits.  Of 256 values a block has a compute unit to itself: 2048 causal tokens, 8 heads over 2, float16, 140 us forward, 255 dq, 259 dk and
-// dv (128 blocks; 3127, 3472 and 24976 us a row at a time).
+// of 32 bits.  Of 256 values a block has a compute unit to itself: 2048 causal tokens, 8 heads over 2, float16, 69 us forward and 102 dq (both 32
+// columns a block), 310 dk and dv and 44 to join them (3127, 3472 and 24976 us a row at a time).
 bool tiles_take(const Attention &p, int size, uintptr_t ends) {
   return p.D <= (size == 2 ? 256 : 128) && p.D % 4 == 0 && ends % 16 == 0 && (long long)p.HQ * p.D * size * 128 < (1ll << 31) &&
          (long long)p.B * p.HQ * ceil_div(p.TQ, 32) < (1 << 24) && (long long)p.B * p.HK * ceil_div(p.TK, 32) < (1 << 24);
@@ -598,8 +598,8 @@ bool tiles_take(const Attention &p, int size, uintptr_t ends) {
 // Up to 32 queries one head would not fill a wavefront's columns.  And a few blocks of 128 queries, each on a compute unit of its own, are slower
 // than four times as many of 32 columns whose keys four wavefronts share: in float16 while that leaves half the units idle, in float32, whose
 // products take longer than the keys' way, up to a block a unit.  Forward and dq, microseconds on tiles and here: float16, 4096 causal tokens of two
-// heads of 128 228 against 115, 2 x 769 of 4 of 64 45 against 29, 1024 of 16 of 128 80 against 86, 4096 of 8 299 against 480; float32, 1500 causal
-// tokens of 12 heads of 128 508 against 236, 4 x 1024 of 8 of 64 217 against 147, 4 x 2048 of 8, with no mask, 749 against 774.
+// heads of 128 249 against 109, 2 x 769 of 4 of 64 49 against 27, 1024 of 16 of 128 83 against 62, and beyond the rule 4096 of 8 258 against 238;
+// float32, 1500 causal tokens of 12 heads of 128 497 against 230, 4 x 1024 of 8 of 64, with no mask, 211 against 201, beyond it 4 x 2048 684 against 697.
 bool few_take(const Attention &p, int size) {
   return p.TQ <= 32 || (size == 4 ? 1 : 2) * (long long)p.B * p.HQ * ceil_div(p.TQ, kBlockRows) <= runtime().props.multiProcessorCount;
 }

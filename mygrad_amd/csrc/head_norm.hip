@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(256) head_norm_kernel(HeadNorm p, const T *__r
   for (int d = 2 * p.pairs + lane; d < p.D; d += 64) yr[d] = (T)z(d);
 }
 
-// A wavefront per row for dx; dw's terms go to `terms` (rows of a block of rows summed), see head_norm_weight_kernel.
+// A wavefront per row, for dx.
 template <typename T, typename C>
 __global__ void __launch_bounds__(256) head_norm_dx_kernel(HeadNorm p, const T *__restrict__ x, const T *__restrict__ w, const C *__restrict__ table,
                                                            const T *__restrict__ grad, T *__restrict__ dx) {
