@@ -86,6 +86,7 @@ class RotaryPositions:
 
     def __init__(self, table, positions):
         arr = np.array(positions)
+        whole = arr.shape == (len(table.sections),)  # one token's, or for one axis those of one token in a row of one
         if arr.dtype.kind not in "iu":
             raise TypeError(f"positions are whole numbers, got {arr.dtype}")
         axes = len(table.sections)
@@ -95,7 +96,7 @@ class RotaryPositions:
             raise ValueError(f"positions must have shape (..., {axes}) for {axes} axes, got {arr.shape}")
         if arr.size and (arr.min() < 0 or arr.max() >= table.length):
             raise ValueError(f"positions must lie in [0, {table.length}), got {arr.min()} to {arr.max()}")
-        self._table, self._positions = table, arr.astype(np.int32)
+        self._table, self._positions, self._whole = table, arr.astype(np.int32), whole
         self._bound, self._described = {}, {}
 
     @property
@@ -104,7 +105,7 @@ class RotaryPositions:
 
     def _check(self, lead):
         try:
-            fits = np.broadcast_shapes(self._positions.shape[:-1], lead) == lead
+            fits = lead == () and self._whole or np.broadcast_shapes(self._positions.shape[:-1], lead) == lead
         except ValueError:
             fits = False
         if not fits:
@@ -116,7 +117,7 @@ class RotaryPositions:
             self._check(lead)
             if len(self._bound) >= _MOST_SHAPES:
                 self._bound.clear()
-            spread = np.broadcast_to(self._positions, lead + self._positions.shape[-1:])
+            spread = self._positions if lead == () else np.broadcast_to(self._positions, lead + self._positions.shape[-1:])
             buf = self._bound[lead] = _device.from_host(np.ascontiguousarray(spread)).buf
         return buf
 

@@ -84,3 +84,20 @@ def test_masks_and_tables_do_not_change():
     assert mask.causal and mask.window == 3 and table.pairs == 3 and table.length == 9 and table.sections == (1, 2) and not table.interleaved
     mask.lengths[0] = 7
     assert mask.lengths[0] == 2
+
+
+def test_positions_of_one_token_without_axes_of_its_own(tmp_path):
+    """``(axes,)`` is ``(..., axes)`` for a token that is no row of tokens, for one axis, too."""
+    program = """
+import numpy as np
+from mygrad_amd.nnet import RotaryTable, rotate
+for sections, position in ((2, [5]), ((1, 1), [5, 3])):
+    at = RotaryTable(sections, 9).at(position)
+    assert rotate(np.ones((3, 4)), at).shape == (3, 4) and rotate(np.ones((1, 3, 4)), at).shape == (1, 3, 4)
+    assert rotate(np.ones((7, 3, 4)), at).shape == (7, 3, 4)
+try:
+    rotate(np.ones((3, 4)), RotaryTable(2, 9).at([5, 6]))
+except ValueError:
+    print("turned")
+"""
+    assert "turned" in run_on_standins(tmp_path, program)
