@@ -126,8 +126,17 @@ CASES = [
 ]
 
 
+_MASKS = [dict(), dict(causal=True), dict(causal=True, window=37), dict(window=20), dict(causal=True, window=1), dict(causal=True, prefix=50),
+          dict(causal=True, prefix=[0, 111]), dict(lengths=[130, 0]), dict(causal=True, lengths=[33, 97]), dict(documents=_DOCUMENTS[:130]),
+          dict(causal=True, documents=np.stack([_DOCUMENTS[:130], _DOCUMENTS[20:]])), dict(causal=True, window=16, documents=_DOCUMENTS[:130]),
+          dict(causal=True, prefix=20, documents=_DOCUMENTS[:130]), dict(causal=True, lengths=[100, 64], documents=_DOCUMENTS[:130])]
+# Each mask in 32 columns a block, and in 128 queries a block.
+CASES += [_case(dtype, 2, 130, 130, *heads, 32, mask=mask) for dtype in (np.float16, np.float32) for mask in _MASKS for heads in ((2, 1), (66, 22))]
+
+
 def name_of(case):
     shape, rest = "x".join(map(str, case["shape"])), [k for k in ("cap", "bias", "scale") if case[k]] + list(case["mask"])
+    rest += [str(v) for k, v in case["mask"].items() if k == "window"]
     return "-".join([np.dtype(case["dtype"]).name, shape, *rest, *(["small"] if case["grad_scale"] != 1 else [])])
 
 

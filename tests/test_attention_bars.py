@@ -33,8 +33,10 @@ def test_mistaken_results_exceed_the_bars(case):
     f = Formulas(*arrays, seen, **how)
     if f.q.size * f.shape[1] < 1 << 24:  # the same by other means, where that is quick
         for a, b in zip(f.results[1:], ora.backward(*arrays, seen, **how)):
-            assert np.allclose(a, b, rtol=1e-9, atol=1e-11 * np.abs(b).max())
+            assert np.allclose(a, b, rtol=1e-9, atol=1e-13 + 1e-11 * np.abs(b).max())
     bars = bars_of(case["dtype"], f)
     for name, which, values in _mistaken(f):
+        if seen.sum(-1).max() == 1 and (which in (1, 2) or name == "weights of equal size"):  # there is no dS, and weights are even
+            continue
         over = (np.abs(values - f.results[which]) > bars[which])[f.results[which] != 0]
         assert over.mean() > 0.05, (name, which, over.mean())
