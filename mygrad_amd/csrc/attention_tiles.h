@@ -267,14 +267,6 @@ __device__ __forceinline__ f32x16 zeros() { return f32x16{0, 0, 0, 0, 0, 0, 0, 0
 
 // Registers 8 n .. 8 n + 7 as a fragment along the rows, and what rounding took off them as another.
 template <typename T>
-__device__ __forceinline__ typename Fragment<T>::V rows_of(const f32x16 &v, int n) {
-  f32x8 part;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) part[j] = v[8 * n + j];
-  return __builtin_convertvector(part, typename Fragment<T>::V);
-}
-
-template <typename T>
 __device__ __forceinline__ typename Fragment<T>::V rows_of(const f32x16 &v, int n, typename Fragment<T>::V &more) {
   f32x8 part;
 #pragma unroll
