@@ -233,7 +233,8 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split 
   bad = __any(bad);
   if (lane == 0) odd[wave] = bad;
   all_landed();  // what is stored, too: it may be written again
-  if (wave == 0 && (odd[0] | odd[1] | odd[2] | odd[3]) && (total == total || !out_stands(p, b, hq, i, q, k))) attend_row<T, float>(p, b, hq, i, mine, q, k, v, out, rest, lse);
+  if (wave == 0 && (odd[0] | odd[1] | odd[2] | odd[3]) && (total == total || !out_stands(p, b, hq, i, q, k)))
+    attend_row<T, float>(p, b, hq, i, mine, q, k, v, out, rest, lse);
 }
 
 // dq of a panel's columns; with one split the result itself.  Up to 64 values a head two blocks share a compute unit: 77 us for
@@ -343,9 +344,9 @@ template <typename T>
 constexpr int stages_of(int dim) { return sizeof(T) == 2 && dim <= 128 ? 2 : 1; }
 
 // Keys are split until there is a block for each compute unit, and no further: at 128 values a head, where this was measured, a block takes a unit's
-// LDS to itself, so the next one's first tiles wait for its last (at 64 two blocks would fit a unit).  One history of 131001 tokens, 32 heads over 8 of 128, float16: 110 us with the join, 140 in eight times as many blocks; 32 of 4000
-// to 8000 tokens 156 in one piece, 170.  Where lengths differ, for as many times more as the longest has the mean.  Pieces are 128 keys (a tile for
-// each wavefront) or more; with more queries a join takes as long as 512.
+// LDS to itself, so the next one's first tiles wait for its last (at 64 two blocks would fit a unit).  One history of 131001 tokens, 32 heads over 8
+// of 128, float16: 110 us with the join, 140 in eight times as many blocks; 32 of 4000 to 8000 tokens 156 in one piece, 170.  Where lengths differ, for as
+// many times more as the longest has the mean.  Pieces are 128 keys (a tile for each wavefront) or more; with more queries a join takes as long as 512.
 Split split_of(const Attention &p) {
   const bool single = p.TQ <= 32;
   Split split;
