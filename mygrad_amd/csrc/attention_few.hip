@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
   constexpr int kSteps = DP / 16, kTiles = 4 * STAGES * 2 * Tile::kBytes;
   __shared__ __attribute__((aligned(1024))) char space[kTiles > Join::kBytes ? kTiles : Join::kBytes];
   __shared__ float tops[4][32], totals[4][32];
-  __shared__ unsigned bad;  // columns to be computed again
+  __shared__ unsigned bad, numbers;  // columns with one that is no number, and those of them whose total is one
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
   const Panel at = panel_of(p, split, c);
 
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
     tops[0][c] = all > 0 ? 1.0f / all : all == 0 ? 0.0f : NAN;
     if (lse && at.in) lse[((long long)at.b * p.HQ + at.hq) * p.TQ + at.i] = all == 0 ? INFINITY : top + __builtin_log2f(all) - kLift;
   }
-  if (threadIdx.x == 0) bad = 0;
+  if (threadIdx.x == 0) bad = numbers = 0;
   __syncthreads();
   for (int n = threadIdx.x; n < at.columns * (DP / 4); n += 256) {
     const int column = n / (DP / 4), d = n % (DP / 4) * 4, all_columns = at.first_column + column;
@@ -167,28 +167,34 @@ __global__ void __launch_bounds__(256) attention_few_kernel(Attention p, Split s
     const float by = tops[0][column];
     const f32x4 value = Join::sum(join, column, d) * by;
     const long long to = (((long long)at.b * p.TQ + all_columns / p.group) * p.HQ + at.hk * p.group + all_columns % p.group) * p.D + d;
-    if (put_four(out + to, value) && (by == by || shares_pieces(p, sizeof(T)))) atomicOr(&bad, 1u << column);
+    if (put_four(out + to, value)) {
+      atomicOr(&bad, 1u << column);
+      if (by == by) atomicOr(&numbers, 1u << column);
+    }
     if constexpr (sizeof(T) == 2) {
       if (remains) put_four(remains + to, (value - __builtin_convertvector(__builtin_convertvector(value, f16x4), f32x4)) * kRest);
     }
   }
   all_landed();  // what is stored, too: other wavefronts may write it again
+  OddValues &values = *(OddValues *)(space + 4 * kMaxDim * sizeof(float));  // behind what rows need
+  static_assert(4 * kMaxDim * sizeof(float) + sizeof values <= sizeof space, "no room for them");
+  if (numbers) values.find(p, at.b, at.hk, at.reach.lo, at.reach.hi, v);
   each_marked<1>(&bad, [&](int n) {
-    const int column = at.first_column + n;
-    const int hq = at.hk * p.group + column % p.group, i = column / p.group;
-    const float by = tops[0][n];
-    if (by == by || !out_stands(p, at.b, hq, i, q, k)) attend_row<T, float>(p, at.b, hq, i, (float *)space + wave * kMaxDim, q, k, v, out, remains, lse);
+    const int column = at.first_column + n, hq = at.hk * p.group + column % p.group, i = column / p.group;
+    if (numbers >> n & 1 ? !out_settled(p, at.b, hq, i, values, v, out, remains) : !out_stands(p, at.b, hq, i, q, k))
+      attend_row<T, float>(p, at.b, hq, i, (float *)space + wave * kMaxDim, q, k, v, out, remains, lse);
   });
 }
 
 // A block per row of the result: the splits' sums at a common top, in their order.  A row that comes out as no number is computed once more, unless
-// its total is none, so that what it does not see leaves no mark (products with weights of zero do, where that is no number).
+// what it sees explains it, so that what it does not see leaves no mark (products with weights of zero do, where that is no number).
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split split, const float *__restrict__ sums, const float2 *__restrict__ ends,
                                                              const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
                                                              T *__restrict__ out, _Float16 *__restrict__ rest, float *__restrict__ lse) {
   __shared__ float parts[4][64 * PARTS], totals[4], mine[kMaxDim], weights[kMostSplits];
   __shared__ int odd[4];
+  __shared__ OddValues values;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int hq = blockIdx.x % p.HQ, i = blockIdx.x / p.HQ % p.TQ, b = blockIdx.x / p.HQ / p.TQ;
   const long long first = ((long long)b * p.HK + hq / p.group) * split.splits * split.columns + i * p.group + hq % p.group;
@@ -233,7 +239,12 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Attention p, Split 
   bad = __any(bad);
   if (lane == 0) odd[wave] = bad;
   all_landed();  // what is stored, too: it may be written again
-  if (wave == 0 && (odd[0] | odd[1] | odd[2] | odd[3]) && (total == total || !out_stands(p, b, hq, i, q, k)))
+  if (!(odd[0] | odd[1] | odd[2] | odd[3])) return;
+  if (total == total) {
+    const Span span = span_of(p, b, i);
+    values.find(p, b, hq / p.group, span.lo, span.hi, v);
+  }
+  if (wave == 0 && (total == total ? !out_settled(p, b, hq, i, values, v, out, rest) : !out_stands(p, b, hq, i, q, k)))
     attend_row<T, float>(p, b, hq, i, mine, q, k, v, out, rest, lse);
 }
 

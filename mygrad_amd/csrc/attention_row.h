@@ -181,6 +181,7 @@ __device__ __forceinline__ void dkv_row(const Attention &p, int b, int hk, int j
 // A row of a result that is no number has to be computed again by the functions above only if what it does not see may have made it one.  It need
 // not where what it sees does, whatever stands elsewhere:
 //   out: the sum of the row's weights is no number (scores of unseen keys never enter it; where rows share pieces in LDS: and q_i or a key is none);
+//        else, where a value that it sees is no number or infinite, that value is what the row has there (weights are not zero);
 //   dq:  lse_i or D_i of the row is none, which makes each of its dS_ij none (a row that sees nothing has no dS);
 //   dk, dv: the same of a query that sees the key, for all of dk and for dv where that query's grad is none (all of it where lse_i is).
 // So an upstream gradient that overflowed, or operands that are no numbers throughout, cost a step what numbers do.
@@ -207,6 +208,78 @@ __device__ __forceinline__ bool out_stands(const Attention &p, int b, int h, int
   for (int j = span.lo; j < span.hi; ++j)
     if (__any(none(keys + (long long)j * p.HK * p.D))) return true;
   return false;
+}
+
+// The rows of a head's values among [lo, hi) that hold one that is no number, in no order; a block's four wavefronts find them together, eight
+// rows at a time each (2048 of 64 values: 40 us).
+struct OddValues {
+  static constexpr int kMost = 256;
+  int count, rows[kMost];  // more than kMost: they are not all here
+
+  template <typename T>
+  __device__ __forceinline__ void find(const Attention &p, int b, int hk, int lo, int hi, const T *__restrict__ v) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long step = (long long)p.HK * p.D;
+    const T *head = v + ((long long)b * p.TK * p.HK + hk) * p.D;
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    for (int j0 = lo < hi ? lo + 8 * wave : hi; j0 < hi; j0 += 32) {
+      bool odd[8] = {};
+#pragma unroll
+      for (int c = 0; c < kParts; ++c)
+        if (64 * c < p.D) {
+          T values[8];
+#pragma unroll
+          for (int n = 0; n < 8; ++n) values[n] = lane + 64 * c < p.D && j0 + n < hi ? head[(j0 + n) * step + lane + 64 * c] : T(0);
+#pragma unroll
+          for (int n = 0; n < 8; ++n) odd[n] |= no_number((float)values[n]);
+        }
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+        if (__any(odd[n]) && lane == 0) {
+          const int at = atomicAdd(&count, 1);
+          if (at < kMost) rows[at] = j0 + n;
+        }
+    }
+    __syncthreads();
+  }
+};
+
+// Puts into row i of `out` what the values that it sees make of those that are no number there; false if they do not explain all of them.
+template <typename T>
+__device__ __forceinline__ bool out_settled(const Attention &p, int b, int h, int i, const OddValues &odd, const T *__restrict__ v, T *__restrict__ out,
+                                            _Float16 *__restrict__ rest) {
+  const int lane = threadIdx.x & 63;
+  const long long at = (((long long)b * p.TQ + i) * p.HQ + h) * p.D, step = (long long)p.HK * p.D;
+  const T *head = v + ((long long)b * p.TK * p.HK + h / p.group) * p.D;
+  const Span span = span_of(p, b, i);
+  const bool listed = odd.count <= OddValues::kMost;
+  unsigned open = 0, up = 0, down = 0;  // bit c: value lane + 64 c is no number, with an infinity among what makes it, or one of the other sign
+#pragma unroll
+  for (int c = 0; c < kParts; ++c)
+    if (lane + 64 * c < p.D && no_number((float)out[at + lane + 64 * c])) open |= 1u << c;
+  const unsigned all = open;
+  const int last = listed ? odd.count : span.hi - span.lo;
+  for (int n = 0; n < last && __any(open & ~(up & down)); ++n) {
+    const int j = listed ? odd.rows[n] : span.lo + n;
+    if (j < span.lo || j >= span.hi) continue;
+#pragma unroll
+    for (int c = 0; c < kParts; ++c)
+      if (open >> c & 1) {
+        const float value = (float)head[j * step + lane + 64 * c];
+        if (no_number(value) && !(value < 0)) up |= 1u << c;
+        if (no_number(value) && !(value > 0)) down |= 1u << c;
+      }
+  }
+  if (__any(all & ~(up | down))) return false;
+#pragma unroll
+  for (int c = 0; c < kParts; ++c)
+    if (all >> c & 1) {
+      const float value = (up & down) >> c & 1 ? NAN : up >> c & 1 ? INFINITY : -INFINITY;
+      out[at + lane + 64 * c] = (T)value;
+      if (rest) rest[at + lane + 64 * c] = (_Float16)NAN;
+    }
+  return true;
 }
 
 // Whether row j of dk (`of_k`: it holds one that is no number) and dv (bit c of `of_v`: value lane + 64 c is none) stands; the same in every lane.

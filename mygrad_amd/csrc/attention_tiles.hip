@@ -101,9 +101,12 @@ attention_tiles_kernel(Attention p, Deal deal, const T *__restrict__ q, const T 
   const unsigned marks = marks_of(odd), none = marks_of(odd && total != total);
   if (lane == 0) bad[0][wave] = marks, bad[1][wave] = none;
   all_landed();  // what is stored, too: other wavefronts may write it again
+  OddValues &values = *(OddValues *)(tiles + 4 * kMaxDim * sizeof(float));  // behind what rows need
+  static_assert(4 * kMaxDim * sizeof(float) + sizeof values <= sizeof tiles, "no room for them");
+  if ((bad[0][0] & ~bad[1][0]) | (bad[0][1] & ~bad[1][1]) | (bad[0][2] & ~bad[1][2]) | (bad[0][3] & ~bad[1][3])) values.find(p, b, hk, lo, hi, v);
   each_marked<4>(bad[0], [&](int n) {
     const int again = tile * kBlockRows + n;
-    if (!(bad[1][n >> 5] >> (n & 31) & 1) || !out_stands(p, b, hq, again, q, k))
+    if (bad[1][n >> 5] >> (n & 31) & 1 ? !out_stands(p, b, hq, again, q, k) : !out_settled(p, b, hq, again, values, v, out, rest))
       attend_row<T, float>(p, b, hq, again, (float *)tiles + wave * kMaxDim, q, k, v, out, rest, lse);
   });
 }

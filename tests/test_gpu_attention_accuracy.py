@@ -163,8 +163,9 @@ def milliseconds(operands, grad, mask):
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
 @pytest.mark.parametrize("B,T,HQ,HK,D", [(2, 2048, 8, 2, 64), (1, 700, 4, 1, 128), (2, 1500, 8, 8, 36)])
 def test_an_overflow_costs_a_step_what_numbers_do(dtype, B, T, HQ, HK, D):
-    """An upstream gradient of infinities (a scaled loss that overflowed), in all or in some values, and operands that are no numbers: every row
-    of a block is no number by what it sees.  A row at a time they took 30 to 260 times as long; a third of that ratio is allowed here."""
+    """An upstream gradient of infinities (a scaled loss that overflowed), in all or in some values, operands that are no numbers, and a value of the
+    first key that is infinite: every row of a block is no number by what it sees.  A row at a time they took 30 to 260 times as long; five times
+    are allowed here."""
     rng = np.random.default_rng(T)
     q, k, v, g = (rng.standard_normal((B, T, heads, D)).astype(dtype) for heads in (HQ, HK, HK, HQ))
     mask = AttentionMask(causal=True)
@@ -172,7 +173,10 @@ def test_an_overflow_costs_a_step_what_numbers_do(dtype, B, T, HQ, HK, D):
     some = g.copy()
     some[:, T // 2:, :, 3] = np.inf
     clean = milliseconds((q, k, v), g, mask)
-    for operands, grad in (((q, k, v), np.full_like(g, np.inf)), ((q, k, v), some), ([np.full_like(a, np.nan) for a in (q, k, v)], g)):
+    one = v.copy()
+    one[:, 0, :, 5] = np.inf
+    for operands, grad in (((q, k, v), np.full_like(g, np.inf)), ((q, k, v), some), ([np.full_like(a, np.nan) for a in (q, k, v)], g), ((q, k, one), g),
+                           ((q, k, np.full_like(v, np.nan)), g)):
         for way, spoilt in zip(clean, milliseconds(operands, grad, mask)):
             assert spoilt < 0.3 + 5 * way, (way, spoilt)
 
@@ -198,3 +202,33 @@ def test_infinite_gradients_of_some_queries_and_values(dtype, B, T, HQ, HK, D):
         assert np.array_equal(np.isfinite(have), finite), which
         over = np.abs(np.where(finite, have, 0).astype(np.float64) - np.where(finite, f.results[which], 0)) - bars[which]
         assert (over <= 0).all(), (which, over.max())
+
+
+@pytest.mark.parametrize("dtype,B,T,HQ,HK,D", [*((dtype, *shape) for dtype in (np.float16, np.float32) for shape in EACH_WAY),
+                                               *((np.float64, *shape) for shape in EACH_WAY[:4])])
+@pytest.mark.parametrize("many", [False, True])
+def test_values_that_are_no_numbers_reach_the_rows_that_see_them(dtype, B, T, HQ, HK, D, many):
+    """In their places: an infinity as one, NaN or infinities of both signs as NaN; all others are as if those keys held numbers."""
+    case = dict(dtype=dtype, shape=(B, T, T, HQ, HK, D), mask=dict(causal=True), cap=None, bias=False, scale=None, grad_scale=1.0)
+    (q, k, v, g), seen, how = operands(case)
+    f = Formulas(q, k, v, g, seen, **how)
+    want, bar = f.results[0], bars_of(dtype, f)[0]
+    spoilt = v.copy()
+    if many:  # each key from a third of the row on, in some places
+        spoilt[:, T // 3:, HK - 1, 1] = np.inf
+        spoilt[:, T // 3::2, HK - 1, 2] = -np.inf
+        spoilt[:, T // 2, HK - 1, 2] = np.nan
+    else:
+        spoilt[:, T // 3, HK - 1, 1] = np.inf
+        spoilt[:, T // 3, HK - 1, 2] = -np.inf
+        spoilt[:, T // 2, HK - 1, 2:4] = np.nan, np.inf
+        spoilt[:, T // 2 + 1, HK - 1, 3] = -np.inf
+    held = np.where(np.isfinite(spoilt), 0, spoilt).astype(np.float64)
+    ups, downs = ((seen[:, :, :, None, None] & test[:, None]).any(2) for test in (~(held <= 0), ~(held >= 0)))
+    expected = np.repeat(np.where(ups & downs, np.nan, np.where(ups, np.inf, np.where(downs, -np.inf, 0))), HQ // HK, axis=2)
+    with mg.no_autodiff:
+        out = attention(q, k, spoilt, mask=AttentionMask(causal=True)).data
+    odd = expected != 0
+    assert np.array_equal(out[odd].astype(np.float64), expected[odd], equal_nan=True)
+    over = np.abs(np.where(odd, 0, out).astype(np.float64) - np.where(odd, 0, want)) - bar
+    assert (over <= 0).all(), over.max()
