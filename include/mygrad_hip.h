@@ -486,6 +486,44 @@ int mg_head_norm_fwd(const mg_head_norm_desc *desc, const void *x, const void *w
  * a fixed partition. */
 int mg_head_norm_bwd(const mg_head_norm_desc *desc, const void *x, const void *weight, const void *table, const void *grad, void *dx, void *dweight);
 
+/* ---- a language model's ends, and the norm between its blocks (no counterparts in the reference) ----
+ * dtype: MG_F16, MG_F32 or MG_F64.  Sums and statistics are float32 (float64 for MG_F64), and every result is rounded once.  Tokens
+ * are int32 on the device; a negative one stands for none. */
+
+/* y = weight * (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps) + bias over the D values of each row; weight and bias (D,) may be null. */
+int mg_layer_norm_fwd(int dtype, int64_t rows, int64_t D, double eps, const void *x, const void *weight, const void *bias, void *y);
+
+/* Its gradients, like x, weight and bias; any of dx, dweight, dbias may be null (not wanted), not all three.  Run-to-run identical. */
+int mg_layer_norm_bwd(int dtype, int64_t rows, int64_t D, double eps, const void *x, const void *weight, const void *grad, void *dx, void *dweight,
+                      void *dbias);
+
+/* out[n] = scale * weight[ids[n]], weight:(rows, D), out:(tokens, D); zeros for tokens that are none (or lie beyond the table). */
+int mg_embedding_fwd(int dtype, int64_t tokens, int64_t rows, int64_t D, double scale, const int32_t *ids, const void *weight, void *out);
+
+/* dweight[v] = scale * sum of the grad[n] with ids[n] = v: all rows of dweight:(rows, D) are written.  Run-to-run identical. */
+int mg_embedding_bwd(int dtype, int64_t tokens, int64_t rows, int64_t D, double scale, const int32_t *ids, const void *grad, void *dweight);
+
+/* Of logits:(rows, V): scores[r], the logarithm of the probability of token ids[r] (0 for none); entropy[r]; top_scores and
+ * top_ids:(rows, top), the likeliest tokens and the logarithms of their probabilities in falling order, the lowest token first among
+ * equals (top at most 128).  All but top_ids are float32 (float64 for MG_F64); scores, entropy and kept may be null (not wanted).
+ * kept:(rows, 3), of the same type, is for mg_log_probabilities_bwd. */
+int mg_log_probabilities_fwd(int dtype, int64_t rows, int64_t V, int top, const int32_t *ids, const void *logits, void *scores, void *entropy, void *kept,
+                             void *top_scores, int32_t *top_ids);
+
+/* dlogits, like logits, from the gradients of scores and entropy (one of them may be null). */
+int mg_log_probabilities_bwd(int dtype, int64_t rows, int64_t V, const int32_t *ids, const void *logits, const void *kept, const void *grad_scores,
+                             const void *grad_entropy, void *dlogits);
+
+/* loss[r] = sum over k of q_k (log q_k - log p(ids[r, k])): p = softmax(logits[r] / temperature), q = softmax(teacher[r] / temperature) over
+ * those of the K tokens (at most 256) that are there; 0 without any.  teacher:(rows, K) is of `dtype`, or float32 beside MG_F16.  loss,
+ * kept:(rows, 3) and shares:(rows, K), both for mg_distillation_bwd and null where there will be none, are float32 (float64 for MG_F64). */
+int mg_distillation_fwd(int dtype, int teacher_dtype, int64_t rows, int64_t V, int64_t K, double temperature, const void *logits, const int32_t *ids,
+                        const void *teacher, void *loss, void *kept, void *shares);
+
+/* dlogits, like logits, from grad:(rows), the gradient of loss. */
+int mg_distillation_bwd(int dtype, int64_t rows, int64_t V, int64_t K, double temperature, const void *logits, const int32_t *ids, const void *kept,
+                        const void *shares, const void *grad, void *dlogits);
+
 #ifdef __cplusplus
 }
 #endif

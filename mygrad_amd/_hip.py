@@ -223,6 +223,14 @@ _SIGNATURES = {
     "mg_cache_write": [ctypes.c_int] + [ctypes.c_int64] * 4 + [_vp] * 5,
     "mg_head_norm_fwd": [ctypes.POINTER(HeadNormDesc)] + [_vp] * 4,
     "mg_head_norm_bwd": [ctypes.POINTER(HeadNormDesc)] + [_vp] * 6,
+    "mg_layer_norm_fwd": [ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_double] + [_vp] * 4,
+    "mg_layer_norm_bwd": [ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_double] + [_vp] * 6,
+    "mg_embedding_fwd": [ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_double] + [_vp] * 3,
+    "mg_embedding_bwd": [ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_double] + [_vp] * 3,
+    "mg_log_probabilities_fwd": [ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_int] + [_vp] * 7,
+    "mg_log_probabilities_bwd": [ctypes.c_int] + [ctypes.c_int64] * 2 + [_vp] * 6,
+    "mg_distillation_fwd": [ctypes.c_int] * 2 + [ctypes.c_int64] * 3 + [ctypes.c_double] + [_vp] * 6,
+    "mg_distillation_bwd": [ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_double] + [_vp] * 6,
     "mg_permute": [ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int32), _vp, _vp],
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES) + ("mg_last_error", "mg_last_plan")
@@ -348,6 +356,14 @@ KERNEL_TAGS = {
     27: "head_norm",
     28: "head_norm_bwd",
     29: "attention_join",
+    30: "layer_norm",
+    31: "layer_norm_bwd",
+    32: "embedding",
+    33: "embedding_bwd",
+    34: "log_probabilities",
+    35: "log_probabilities_bwd",
+    36: "distillation",
+    37: "distillation_bwd",
 }
 
 
@@ -408,8 +424,8 @@ def dtype_code(dtype):
 
 
 def storage_code(dtype):
-    """``dtype_code`` for what also takes float16 (``mg_cast``, ``mg_accumulate``, attention and the norm
-    of heads): a type arrays are stored in, not one any kernel sums in."""
+    """``dtype_code`` for what also takes float16 (``mg_cast``, ``mg_accumulate``, attention, the norms,
+    embedding and what is made of logits): a type arrays are stored in, not one any kernel sums in."""
     import numpy as np
 
     return MG_F16 if np.dtype(dtype) == np.float16 else dtype_code(dtype)

@@ -78,6 +78,14 @@ enum KernelTag {
   TAG_HEAD_NORM = 27,
   TAG_HEAD_NORM_BWD = 28,
   TAG_ATTENTION_JOIN = 29,
+  TAG_LAYER_NORM = 30,
+  TAG_LAYER_NORM_BWD = 31,
+  TAG_EMBEDDING = 32,
+  TAG_EMBEDDING_BWD = 33,
+  TAG_SCORES = 34,
+  TAG_SCORES_BWD = 35,
+  TAG_DISTILLATION = 36,
+  TAG_DISTILLATION_BWD = 37,
 };
 void timing_begin(int tag);
 void timing_end();

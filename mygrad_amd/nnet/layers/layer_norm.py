@@ -1,0 +1,97 @@
+"""Layer norm on the MI355X.  The reference has no counterpart; the operation keeps its ``Operation`` contract
+(``mygrad/operation_base.py:54-228``)."""
+
+from math import prod
+from typing import Optional
+
+import numpy as np
+
+from ... import _device, _hip
+from ...operation_base import Operation
+from ...tensor_base import Tensor
+
+__all__ = ["LayerNorm", "layer_norm"]
+
+_DTYPES = (np.float16, np.float32, np.float64)
+
+
+class LayerNorm(Operation):
+    """``x:(..., dim)`` with ``weight:(dim,)`` and ``bias:(dim,)``; empty ones stand for none."""
+
+    takes_device_arrays = True
+
+    def __call__(self, x, weight, bias, *, eps):
+        self.variables = (x, weight, bias)
+        values = [_device.value_of(t) for t in self.variables]
+        xd = values[0]
+        if xd.ndim < 1:
+            raise ValueError(f"`x` must have the axes (..., dim), got shape {xd.shape}")
+        if xd.dtype not in _DTYPES:
+            raise TypeError(f"layer_norm runs on the GPU in float16, float32 or float64, got {xd.dtype} (there is no CPU fallback)")
+        dim = xd.shape[-1]
+        self._there = [True, values[1].size > 0, values[2].size > 0]
+        for name, value, there in zip(("weight", "bias"), values[1:], self._there[1:]):
+            if there and value.shape != (dim,):
+                raise ValueError(f"`{name}` must have shape ({dim},), got {value.shape}")
+            if there and value.dtype != xd.dtype:
+                raise TypeError(f"layer_norm takes `{name}` in the dtype of `x` ({xd.dtype}), got {value.dtype}")
+        if not 0 <= eps < np.inf:
+            raise ValueError(f"`eps` must be a non-negative number, got {eps}")
+        self._backed = None
+        if xd.size == 0:
+            return np.empty(xd.shape, dtype=xd.dtype)
+        self._call = _hip.storage_code(xd.dtype), prod(xd.shape[:-1]), dim, float(eps)
+        buffers = [_device.to_device(v) if there else None for v, there in zip(values, self._there)]
+        out = _device.DeviceBuffer(xd.nbytes)
+        _hip.check(_hip.lib().mg_layer_norm_fwd(*self._call, *(None if b is None else b.ptr for b in buffers), out.ptr))
+        y = _device.download(out, xd.shape, xd.dtype)
+        _device.attach(y, out)
+        return y
+
+    def _run_backward(self, grad, want):
+        values = [_device.value_of(t) for t in self.variables]
+        if grad.shape != values[0].shape:
+            raise NotImplementedError(f"layer_norm backward for gradient of shape {grad.shape} (no CPU fallback)")
+        xb, gb = _device.to_device(values[0]), _device.to_device(grad, values[0].dtype)
+        wb = _device.to_device(values[1]) if self._there[1] else None
+        out = {i: _device.DeviceBuffer(values[i].nbytes) for i in sorted(want)}
+        _hip.check(_hip.lib().mg_layer_norm_bwd(*self._call, xb.ptr, None if wb is None else wb.ptr, gb.ptr,
+                                                *(out[i].ptr if i in out else None for i in range(3))))
+        return {i: _device.download(buf, values[i].shape, values[i].dtype) for i, buf in out.items()}
+
+    def backward_var(self, grad, index, **kwargs):
+        value = _device.value_of(self.variables[index])
+        if _device.value_of(self.variables[0]).size == 0 or value.size == 0:
+            return np.zeros(value.shape, dtype=value.dtype)
+        # backward() asks for each variable in turn with the same `grad`: the first request computes all that are wanted
+        if self._backed is None or self._backed[0] is not grad or index not in self._backed[1]:
+            want = {index} | {i for i, var in enumerate(self.variables) if not var.constant and self._there[i]}
+            self._backed = (grad, self._run_backward(grad, want))
+        out = self._backed[1].pop(index)
+        if not self._backed[1]:
+            self._backed = None
+        return out
+
+
+def layer_norm(x, weight=None, bias=None, *, eps: float, constant: Optional[bool] = None) -> Tensor:
+    """Norm each row of ``x:(..., dim)`` on the GPU::
+
+        y = weight * (x - mean(x)) / sqrt(mean((x - mean(x)) ** 2) + eps) + bias
+
+    ``weight`` and ``bias`` are ``(dim,)`` in the dtype of ``x`` (float16, float32 or float64), or None; ``eps`` is a
+    non-negative number and has no default.  Sums are carried in float32 (float64 for float64), the gradients of
+    ``weight`` and ``bias`` are joined in float64, and each result is rounded once.
+
+    >>> import mygrad_amd as mg
+    >>> from mygrad_amd.nnet import layer_norm
+    >>> layer_norm(mg.Tensor([[1.0, 2.0, 3.0], [4.0, 4.0, 10.0]]), eps=0.0).data.round(3)
+    array([[-1.225,  0.   ,  1.225],
+           [-0.707, -0.707,  1.414]])
+    """
+    if eps is None:
+        raise TypeError("`eps` must be a non-negative number")
+    for name, value in (("weight", weight), ("bias", bias)):  # to the operation an empty one is none
+        if value is not None and 0 in np.shape(value) and np.shape(value) != np.shape(x)[-1:]:
+            raise ValueError(f"`{name}` of shape {np.shape(value)} for rows of shape {np.shape(x)[-1:]}")
+    none = np.array([])
+    return Tensor._op(LayerNorm, x, none if weight is None else weight, none if bias is None else bias, op_kwargs=dict(eps=eps), constant=constant)
