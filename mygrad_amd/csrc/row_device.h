@@ -1,9 +1,36 @@
-// What the kernels over rows (layer norm, log probabilities, distillation) share: sums over a block, and the types sums are carried in.
+// What the kernels over rows (embedding, layer norm, log probabilities, distillation) share: pieces of a row that a lane loads at once, and
+// sums over wavefronts and blocks.
 #pragma once
 
 #include "internal.h"
 
 namespace mg {
+
+// V neighbouring values of a row, 16 bytes.  Rows begin wherever their length puts them: the vector instructions take any address, and a
+// row of 50001 halves moves as fast as one of 50000.
+template <typename T>
+struct Piece {
+  static constexpr int V = 16 / sizeof(T);
+  typedef T Held __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+
+  // From `at` on, of which `count` values are there (as many as V or more: all of them); the others are `otherwise`.
+  static __device__ __forceinline__ Held load(const T *at, long long count, T otherwise) {
+    Held v;
+    if (count >= V) return *reinterpret_cast<const Held *>(at);
+#pragma unroll
+    for (int n = 0; n < V; ++n) v[n] = n < count ? at[n] : otherwise;
+    return v;
+  }
+  static __device__ __forceinline__ void store(T *at, long long count, const Held &v) {
+    if (count >= V) {
+      *reinterpret_cast<Held *>(at) = v;
+      return;
+    }
+#pragma unroll
+    for (int n = 0; n < V; ++n)
+      if (n < count) at[n] = v[n];
+  }
+};
 
 template <typename C>
 __device__ __forceinline__ C wave_add(C v) {
