@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace mg {
 
@@ -39,36 +40,6 @@ struct Row {
   C m, s, a;  // the largest logit (0 in a row without any), the sum of exponentials, the mean of t (distillation: 1, or 0 without a teacher's token)
 };
 
-template <typename C>
-__device__ __forceinline__ C block_max(C v, C *space) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-#pragma unroll
-  for (int k = 32; k; k >>= 1) v = max(v, __shfl_xor(v, k));
-  __syncthreads();
-  if (lane == 0) space[wave] = v;
-  __syncthreads();
-  for (int w = 0; w < waves; ++w) v = max(v, space[w]);
-  return v;
-}
-
-// m, s and a of a row that the whole block goes through.
-template <typename T, typename C>
-__device__ __forceinline__ Row<C> row_of(const Vocabulary &p, const T *z, bool with_mean, C *space) {
-  const C per = (C)p.per;
-  C most = -infinity<C>();
-  for (int j = threadIdx.x; j < p.V; j += blockDim.x) most = max(most, (C)z[j]);
-  most = block_max(most, space);
-  if (most == -infinity<C>()) most = 0;
-  C sums[2] = {0, 0};
-  for (int j = threadIdx.x; j < p.V; j += blockDim.x) {
-    const C t = ((C)z[j] - most) * per, e = exp(t);
-    sums[0] += e;
-    if (with_mean && e > 0) sums[1] += e * t;
-  }
-  block_add(sums, space);
-  return Row<C>{most, sums[0], sums[0] > 0 ? sums[1] / sums[0] : C(0)};
-}
-
 // The log probability of a token with logit z.
 template <typename C>
 __device__ __forceinline__ C log_probability(const Row<C> &row, C z, C per) {
@@ -85,134 +56,521 @@ __device__ __forceinline__ uint64_t order_of(double z) {
   return z != z ? ~0ull : bits >> 63 ? ~bits : bits | 1ull << 63;
 }
 
-// ---- log probabilities ----------------------------------------------------------------------------------------------------------
+// The exponential of a number that is not positive.  The result of float16 is rounded to 11 bits, so the instruction's own is enough
+// there: an argument rounded in single precision, |x| 2^-24 of the result.
+template <typename T>
+__device__ __forceinline__ float exponential(float x) {
+  return sizeof(T) == 2 ? __builtin_amdgcn_exp2f(x * 1.4426950408889634f) : expf(x);
+}
+template <typename T>
+__device__ __forceinline__ double exponential(double x) {
+  return exp(x);
+}
+
+// LANES threads that share a row: a wavefront, or a block of 256.  All of them call; `space` is 16 values of LDS for a block.
+template <int LANES, typename C>
+__device__ __forceinline__ C group_max(C v, C *space) {
+#pragma unroll
+  for (int k = 32; k; k >>= 1) v = max(v, __shfl_xor(v, k));
+  if (LANES == 64) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) space[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return max(max(space[0], space[1]), max(space[2], space[3]));
+}
+template <int LANES, typename C>
+__device__ __forceinline__ C group_add(C v, C *space) {
+  v = wave_add(v);
+  if (LANES == 64) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) space[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (space[0] + space[1]) + (space[2] + space[3]);
+}
+
+// ---- sums of a row in one pass --------------------------------------------------------------------------------------------------
+constexpr int kAtOnce = 4;  // pieces that a thread has on their way together
+
+// m: the largest logit so far (minus infinity: none); s = sum e^t and w = sum e^t t with t = (z - m) / T, none of them from a logit of minus infinity.
+template <typename C>
+struct Sums {
+  C m, s, w;
+};
+
+// A t of minus infinity times its exponential of 0 is no number; this is.
+template <typename C>
+__device__ __forceinline__ C bounded(C t) {
+  return max(t, (C)-1e30);
+}
+template <typename C>
+__device__ __forceinline__ C base_of(C m) {
+  return m == -infinity<C>() ? C(0) : m;
+}
+
+// As seen from a larger m.
+template <typename T, bool MEAN, typename C>
+__device__ __forceinline__ void move_to(Sums<C> &a, C m, C per) {
+  const C step = bounded((a.m - base_of(m)) * per), c = exponential<T>(step);
+  if (MEAN) a.w = c * (a.w + a.s * step);
+  a.s *= c;
+  a.m = m;
+}
+
+template <typename T, bool MEAN, typename C>
+__device__ __forceinline__ void add_pieces(Sums<C> &a, const typename Piece<T>::Held (&z)[kAtOnce], C per) {
+  constexpr int V = Piece<T>::V;
+  T most = z[0][0];  // a NaN is passed over: the sum shows it
+#pragma unroll
+  for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+    for (int n = 0; n < V; ++n) most = sizeof(T) == 2 ? (T)__builtin_fmaxf16((_Float16)most, (_Float16)z[u][n]) : (T)max((C)most, (C)z[u][n]);
+  move_to<T, MEAN>(a, max(a.m, (C)most), per);
+  const C base = base_of(a.m);
+  C s[kAtOnce] = {}, w[kAtOnce] = {};
+#pragma unroll
+  for (int n = 0; n < V; ++n)
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const C t = ((C)z[u][n] - base) * per, e = exponential<T>(t);
+      s[u] += e;
+      if (MEAN) w[u] += e * bounded(t);
+    }
+  a.s += (s[0] + s[1]) + (s[2] + s[3]);
+  if (MEAN) a.w += (w[0] + w[1]) + (w[2] + w[3]);
+}
+
+// Of all threads' sums.
+template <int LANES, typename T, bool MEAN, typename C>
+__device__ __forceinline__ Sums<C> join(Sums<C> a, C per, C *space) {
+  move_to<T, MEAN>(a, group_max<LANES>(a.m, space), per);
+  a.s = group_add<LANES>(a.s, space);
+  if (MEAN) a.w = group_add<LANES>(a.w, space);
+  return a;
+}
+
+template <typename C>
+__device__ __forceinline__ Row<C> row_of(const Sums<C> &a) {
+  return Row<C>{base_of(a.m), a.s, a.s == 0 ? C(0) : a.w / a.s};
+}
+
+// Pieces of a thread's from `at` on, LANES threads side by side.
+template <int LANES, typename T>
+__device__ __forceinline__ void load_pieces(typename Piece<T>::Held (&z)[kAtOnce], const T *row, long long at, long long end) {
+  constexpr int V = Piece<T>::V;
+#pragma unroll
+  for (int u = 0; u < kAtOnce; ++u) {
+    const long long d = at + (long long)u * LANES * V;
+    z[u] = Piece<T>::load(row + d, end - d, (T)-__builtin_inff());
+  }
+}
+
+// ---- the likeliest tokens ---------------------------------------------------------------------------------------------------------
+// The threads' own maxima bound the k-th largest logit from below: k of them are as large as the k-th of them.  What is not below that bound is
+// collected in LDS, which is little more than k, and ranked there by comparing all with all.  Ties can make it more: when the list is full, all
+// but the first k are dropped, and the last of those is the new bound.
+template <typename C>
+struct Candidate {
+  typedef decltype(order_of(C(0))) Order;
+  Order value;
+  int place;
+  __device__ __forceinline__ bool before(const Candidate &o) const { return value > o.value || (value == o.value && place < o.place); }
+};
+
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) scores_kernel(Vocabulary p, const int32_t *__restrict__ ids, const T *__restrict__ logits, C *__restrict__ scores,
-                                                     C *__restrict__ entropy, Row<C> *__restrict__ kept, C *__restrict__ top_scores,
-                                                     int32_t *__restrict__ top_ids) {
-  __shared__ C space[32];
-  const long long r = blockIdx.x;
-  const T *z = logits + r * p.V;
-  const Row<C> row = row_of(p, z, true, space);
-  if (threadIdx.x == 0) {
+struct Likeliest {
+  static constexpr int kStep = 256 * Piece<T>::V;  // that a block may add before it looks at the count
+  static constexpr int kRoom = 2 * kStep < 1024 ? 1024 : 2 * kStep;
+  typedef Candidate<C> Found;
+  typedef typename Found::Order Order;
+  Order values[kRoom];
+  int places[kRoom];
+  Found first[kMostTop];
+  int count;
+  Found bound;  // what does not come before it, and is not it, is not wanted
+
+  __device__ __forceinline__ Found at(int n) const { return Found{values[n], places[n]}; }
+
+  // The k-th of the threads' largest values (0: a thread has none).
+  __device__ __forceinline__ void begin(Order most, int k) {
+    values[threadIdx.x] = most;
+    if (threadIdx.x == 0) count = 0, bound = Found{0, 0x7fffffff};
+    __syncthreads();
+    int rank = 0;
+    for (int n = 0; n < 256; ++n) rank += values[n] > most || (values[n] == most && n < (int)threadIdx.x);
+    __syncthreads();
+    if (rank == k - 1 && most) bound = Found{most, 0x7fffffff};
+    __syncthreads();
+  }
+  __device__ __forceinline__ void add(const Found &f) {
+    const int n = atomicAdd(&count, 1);
+    values[n] = f.value, places[n] = f.place;
+  }
+  // The first k of the list, in order, in `first`; returns how many there are.  All threads call.
+  __device__ __forceinline__ int rank(int k) {
+    __syncthreads();
+    const int n = count;
+    for (int i = threadIdx.x; i < n; i += 256) {
+      const Found mine = at(i);
+      int better = 0;
+      for (int j = 0; j < n && better < k; ++j) better += at(j).before(mine);
+      if (better < k) first[better] = mine;
+    }
+    __syncthreads();
+    return min(n, k);
+  }
+  // Room for another step.  All threads call.
+  __device__ __forceinline__ void make_room(int k) {
+    __syncthreads();
+    const int held = count;
+    __syncthreads();  // nobody adds before all have seen the same count
+    if (held + kStep <= kRoom) return;
+    const int left = rank(k);
+    if ((int)threadIdx.x < left) values[threadIdx.x] = first[threadIdx.x].value, places[threadIdx.x] = first[threadIdx.x].place;
+    if (threadIdx.x == 0) count = left, bound = first[left - 1];
+    __syncthreads();
+  }
+};
+
+template <typename T, typename C>
+__device__ __forceinline__ void collect(Likeliest<T, C> &list, const typename Piece<T>::Held &z, long long d, long long end, int k) {
+  typedef Candidate<C> Found;
+  list.make_room(k);
+  const Found bound = list.bound;
+#pragma unroll
+  for (int n = 0; n < Piece<T>::V; ++n) {
+    const Found f{order_of((C)z[n]), (int)(d + n)};
+    if (f.value >= bound.value && d + n < end && !bound.before(f)) list.add(f);
+  }
+}
+
+// ---- log probabilities ----------------------------------------------------------------------------------------------------------
+// What is made of a row's sums.
+template <typename T, typename C>
+struct Scores {
+  const int32_t *ids;
+  const T *logits;
+  C *scores, *entropy;
+  Row<C> *kept;
+
+  template <int LANES>
+  __device__ __forceinline__ void end(const Vocabulary &p, long long r, int lane, const Sums<C> &sums, C *) const {
+    if (lane) return;
+    const Row<C> row = row_of(sums);
     if (kept) kept[r] = row;
     if (scores) {
       const int id = ids[r];
-      scores[r] = id < 0 || id >= p.V ? C(0) : log_probability<C>(row, (C)z[id], 1);
+      scores[r] = id < 0 || id >= p.V ? C(0) : log_probability<C>(row, (C)logits[r * p.V + id], 1);
     }
     if (entropy) entropy[r] = row.s == 0 ? C(0) : log(row.s) - row.a;
   }
-  typedef decltype(order_of(C(0))) Order;
-  __shared__ Order best_value[4];
-  __shared__ int best_place[4];
-  Order last = 0;
-  int after = -1;
-  for (int k = 0; k < p.top; ++k) {
-    Order value = 0;
-    int place = 0x7fffffff;
-    for (int j = threadIdx.x; j < p.V; j += 256) {
-      const Order o = order_of((C)z[j]);
-      const bool left = k == 0 || o < last || (o == last && j > after);
-      if (left && (place == 0x7fffffff || o > value)) value = o, place = j;
-    }
-    for (int m = 32; m; m >>= 1) {
-      const Order other = __shfl_xor(value, m);
-      const int where = __shfl_xor(place, m);
-      if (where != 0x7fffffff && (place == 0x7fffffff || other > value || (other == value && where < place))) value = other, place = where;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) best_value[threadIdx.x >> 6] = value, best_place[threadIdx.x >> 6] = place;
-    __syncthreads();
-    last = best_value[0], after = best_place[0];
-    for (int w = 1; w < 4; ++w)
-      if (best_place[w] != 0x7fffffff && (after == 0x7fffffff || best_value[w] > last || (best_value[w] == last && best_place[w] < after)))
-        last = best_value[w], after = best_place[w];
-    if (threadIdx.x == 0) {
-      top_ids[r * p.top + k] = after;
-      top_scores[r * p.top + k] = log_probability<C>(row, (C)z[after], 1);
-    }
-  }
-}
+};
 
-template <typename T, typename C>
-__global__ void __launch_bounds__(256) scores_bwd_kernel(Vocabulary p, const int32_t *__restrict__ ids, const T *__restrict__ logits,
-                                                         const Row<C> *__restrict__ kept, const C *__restrict__ grad_scores,
-                                                         const C *__restrict__ grad_entropy, T *__restrict__ dlogits) {
-  const long long r = blockIdx.x;
-  const T *z = logits + r * p.V;
-  T *out = dlogits + r * p.V;
-  const Row<C> row = kept[r];
-  int id = grad_scores ? ids[r] : -1;
-  if (id >= p.V) id = -1;
-  const C g = id < 0 ? C(0) : grad_scores[r], h = grad_entropy ? grad_entropy[r] : C(0), inverse = 1 / row.s;
-  const bool nothing = row.s == 0 || (id < 0 && !grad_entropy);
-  for (int j = threadIdx.x; j < p.V; j += 256) {
-    const C t = (C)z[j] - row.m, share = exp(t) * inverse;
-    C dz = -share * g;
-    if (grad_entropy) dz -= share * ((share > 0 ? t : C(0)) - row.a) * h;
-    out[j] = nothing ? (T)0 : (T)(j == id ? dz + g : dz);
-  }
-}
-
-// ---- distillation ---------------------------------------------------------------------------------------------------------------
-// Thread k takes the teacher's k-th token; q goes to memory for the backward pass.
+// Or of those and a teacher's logits: a thread (or each lane of a wavefront, in turns) takes one of them; q goes to memory for the backward pass.
 template <typename T, typename Y, typename C>
-__global__ void __launch_bounds__(256) distillation_kernel(Vocabulary p, const int32_t *__restrict__ ids, const T *__restrict__ logits,
-                                                           const Y *__restrict__ teacher, C *__restrict__ loss, Row<C> *__restrict__ kept,
-                                                           C *__restrict__ shares) {
-  __shared__ C space[32];
-  const long long r = blockIdx.x;
-  const T *z = logits + r * p.V;
-  const C per = (C)p.per;
-  Row<C> row = row_of(p, z, false, space);
-  const int k = threadIdx.x;
-  int id = k < p.top ? ids[r * p.top + k] : -1;
-  if (id >= p.V) id = -1;
-  const C y = id < 0 ? -infinity<C>() : (C)teacher[r * p.top + k];
-  C most = block_max(y, space);
-  if (most == -infinity<C>()) most = 0;
-  const C u = (y - most) * per;
-  C total[1] = {exp(u)};
-  block_add(total, space);
-  const C q = total[0] == 0 ? C(0) : exp(u) / total[0];
-  const C zk = id < 0 ? C(0) : (C)z[id];
-  C sum[1] = {q == 0 ? C(0) : q * ((u - log(total[0])) - log_probability<C>(row, zk, per))};
-  block_add(sum, space);
-  if (k < p.top && shares) shares[r * p.top + k] = q;
-  if (k == 0) {
-    loss[r] = sum[0];
-    row.a = total[0] == 0 ? C(0) : total[0] / total[0];  // 1, or NaN
+struct Distillation {
+  const int32_t *ids;
+  const T *logits;
+  const Y *teacher;
+  C *loss;
+  Row<C> *kept;
+  C *shares;
+
+  template <int LANES>
+  __device__ __forceinline__ void end(const Vocabulary &p, long long r, int lane, const Sums<C> &sums, C *space) const {
+    constexpr int TURNS = kMostTaught / LANES;
+    const C per = (C)p.per;
+    Row<C> row = row_of(sums);
+    int id[TURNS];
+    C y[TURNS], z[TURNS], most = -infinity<C>();
+#pragma unroll
+    for (int n = 0; n < TURNS; ++n) {
+      const int k = lane + n * LANES;
+      id[n] = k < p.top ? ids[r * p.top + k] : -1;
+      const bool there = id[n] >= 0 && id[n] < p.V;
+      y[n] = there ? (C)teacher[r * p.top + k] : -infinity<C>();
+      z[n] = there ? (C)logits[r * p.V + id[n]] : C(0);
+      most = max(most, y[n]);
+    }
+    const C base = base_of(group_max<LANES>(most, space));
+    C total = 0, f[TURNS];
+#pragma unroll
+    for (int n = 0; n < TURNS; ++n) {
+      y[n] = (y[n] - base) * per;
+      total += f[n] = exp(y[n]);
+    }
+    total = group_add<LANES>(total, space);
+    C sum = 0;
+#pragma unroll
+    for (int n = 0; n < TURNS; ++n) {
+      const int k = lane + n * LANES;
+      const C q = total == 0 ? C(0) : f[n] / total;
+      sum += q == 0 ? C(0) : q * ((y[n] - log(total)) - log_probability<C>(row, z[n], per));
+      if (k < p.top && shares) shares[r * p.top + k] = q;
+    }
+    sum = group_add<LANES>(sum, space);
+    if (lane) return;
+    loss[r] = sum;
+    row.a = total == 0 ? C(0) : total / total;  // 1, or NaN
     if (kept) kept[r] = row;
   }
+};
+
+struct Top {
+  int parts;      // of a row, each for a block
+  int part;       // logits in one
+  void *partial;  // sums of parts
+  void *values;   // and their candidates: (rows, parts, top) in the order of Candidate, and their places
+  int *places;
+  void *scores;
+  int32_t *ids;
+};
+
+// A wavefront per row (four to a block), or a block per part of a row.  Bound by memory, and in float16 nearly by the exponentials.
+template <typename T, typename C, int LANES, bool MEAN, bool TOP, typename End>
+__global__ void __launch_bounds__(256) row_kernel(Vocabulary p, Top w, const T *__restrict__ logits, End end) {
+  constexpr int V = Piece<T>::V, kStep = LANES * V * kAtOnce;
+  __shared__ C space[16];
+  typedef typename Candidate<C>::Order Order;
+  __shared__ std::conditional_t<TOP, Likeliest<T, C>, int> list;
+  const int lane = threadIdx.x & (LANES - 1);
+  const long long units = LANES == 64 ? (p.rows + 3) / 4 : p.rows * w.parts;
+  for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const long long r = LANES == 64 ? unit * 4 + (threadIdx.x >> 6) : unit / w.parts;
+    if (LANES == 64 && r >= p.rows) return;
+    const int part = LANES == 64 ? 0 : (int)(unit - r * w.parts);
+    const T *row = logits + r * p.V;
+    const long long from = (long long)part * w.part, to = min(from + w.part, (long long)p.V);
+    const C per = (C)p.per;
+    Sums<C> sums{-infinity<C>(), 0, 0};
+    typename Piece<T>::Held z[kAtOnce];
+    for (long long d = from + lane * V; d < to; d += kStep) {
+      load_pieces<LANES>(z, row, d, to);
+      add_pieces<T, MEAN>(sums, z, per);
+    }
+    const bool any = from + lane * V < to;
+    const C own = sums.m;
+    sums = join<LANES, T, MEAN>(sums, per, space);
+    if (LANES == 64 || w.parts == 1) end.template end<LANES>(p, r, lane, sums, space);
+    else if (lane == 0) ((Sums<C> *)w.partial)[unit] = sums;
+    if constexpr (TOP) {
+      __syncthreads();
+      list.begin(any ? order_of(own) : Order(0), p.top);
+      const bool held = to - from <= kStep;
+      for (long long d0 = from; d0 < to; d0 += kStep) {
+        const long long d = d0 + lane * V;
+        if (!held) load_pieces<LANES>(z, row, d, to);
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u)
+          if (d0 + u * LANES * V < to) collect<T, C>(list, z[u], d + u * LANES * V, to, p.top);
+      }
+      const int found = list.rank(p.top);
+      if ((int)threadIdx.x < p.top) {
+        const bool there = (int)threadIdx.x < found;
+        const Candidate<C> f = there ? list.first[threadIdx.x] : Candidate<C>{0, 0};
+        const long long at = unit * p.top + threadIdx.x;
+        if (w.parts == 1) {
+          w.ids[at] = f.place;
+          ((C *)w.scores)[at] = log_probability<C>(row_of(sums), (C)row[f.place], 1);
+        } else {
+          ((Order *)w.values)[at] = f.value;
+          w.places[at] = f.place;
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Joins the parts of a row.
+template <typename T, typename C, bool MEAN, bool TOP, typename End>
+__global__ void __launch_bounds__(256) row_join_kernel(Vocabulary p, Top w, const T *__restrict__ logits, End end) {
+  __shared__ C space[16];
+  typedef typename Candidate<C>::Order Order;
+  __shared__ std::conditional_t<TOP, Likeliest<T, C>, int> list;
+  for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    const C per = (C)p.per;
+    Sums<C> sums{-infinity<C>(), 0, 0};
+    for (int n = threadIdx.x; n < w.parts; n += 256) {
+      Sums<C> next = ((const Sums<C> *)w.partial)[r * w.parts + n];
+      const C m = max(sums.m, next.m);
+      move_to<T, MEAN>(sums, m, per);
+      move_to<T, MEAN>(next, m, per);
+      sums.s += next.s, sums.w += next.w;
+    }
+    sums = join<256, T, MEAN>(sums, per, space);
+    end.template end<256>(p, r, threadIdx.x, sums, space);
+    if constexpr (TOP) {
+      __syncthreads();
+      const Order *values = (const Order *)w.values + r * w.parts * p.top;
+      const int *places = w.places + r * w.parts * p.top;
+      // the largest of the parts' last ones bounds the row's
+      Order last = 0;
+      for (int n = threadIdx.x; n < w.parts; n += 256) last = max(last, values[(long long)n * p.top + p.top - 1]);
+      list.values[threadIdx.x] = last;
+      if (threadIdx.x == 0) list.count = 0;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        for (int n = 1; n < 256; ++n) last = max(last, list.values[n]);
+        list.bound = Candidate<C>{last, 0x7fffffff};
+      }
+      __syncthreads();
+      const int all = w.parts * p.top;
+      for (int n0 = 0; n0 < all; n0 += 256) {
+        list.make_room(p.top);
+        const Candidate<C> bound = list.bound;
+        if (n0 + (int)threadIdx.x < all) {
+          const Candidate<C> f{values[n0 + threadIdx.x], places[n0 + threadIdx.x]};
+          if (f.value && f.value >= bound.value && !bound.before(f)) list.add(f);
+        }
+      }
+      list.rank(p.top);
+      if ((int)threadIdx.x < p.top) {
+        const int place = list.first[threadIdx.x].place;
+        w.ids[r * p.top + threadIdx.x] = place;
+        ((C *)w.scores)[r * p.top + threadIdx.x] = log_probability<C>(row_of(sums), (C)logits[r * p.V + place], 1);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// How a pass over the rows is laid out.
+struct Plan {
+  bool wavefronts;  // a wavefront per row
+  int parts, part;
+  unsigned blocks;
+};
+
+// Rows that a wavefront takes in one step go four to a block.  Longer ones have a block each, or where that leaves compute units without
+// work, parts of a step or more.
+template <typename T>
+Plan plan_of(const Vocabulary &p, bool alone) {
+  constexpr int V = Piece<T>::V;
+  const long long most = 1 << 22;
+  if (!alone && p.V <= 64 * V * kAtOnce) return Plan{true, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 4), most)};
+  const long long wanted = ceil_div(4ll * runtime().props.multiProcessorCount, p.rows), step = 256 * V;
+  const long long parts = std::max<long long>(1, std::min<long long>(wanted, ceil_div(p.V, step)));
+  const long long part = ceil_div(ceil_div(p.V, parts), step) * step;
+  Plan plan{false, (int)ceil_div(p.V, part), (int)std::min<long long>(part, p.V), 0};
+  plan.blocks = (unsigned)std::min<long long>(p.rows * plan.parts, most);
+  return plan;
+}
+
+template <typename T, typename C, bool MEAN, bool TOP, typename End>
+int over_rows(const Vocabulary &p, const void *logits, const End &end, void *top_scores, int32_t *top_ids) {
+  typedef typename Candidate<C>::Order Order;
+  const Plan plan = plan_of<T>(p, TOP);
+  hipStream_t s = runtime().stream;
+  Top w{plan.parts, plan.part, nullptr, nullptr, nullptr, top_scores, top_ids};
+  if (plan.parts > 1) {
+    const size_t parts = (size_t)p.rows * plan.parts, sums = ceil_div(parts * sizeof(Sums<C>), 16) * 16, found = TOP ? parts * p.top : 0;
+    char *space = nullptr;
+    if (const int rc = workspace(sums + found * (sizeof(Order) + 4), (void **)&space)) return rc;
+    w.partial = space, w.values = space + sums, w.places = (int *)(space + sums + found * sizeof(Order));
+  }
+  if (plan.wavefronts) {
+    if constexpr (!TOP) row_kernel<T, C, 64, MEAN, false, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
+  } else {
+    row_kernel<T, C, 256, MEAN, TOP, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
+  }
+  MG_HIP(hipGetLastError());
+  if (plan.parts > 1) {
+    row_join_kernel<T, C, MEAN, TOP, End><<<dim3((unsigned)std::min<long long>(p.rows, 1 << 22)), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
+    MG_HIP(hipGetLastError());
+  }
+  return MG_OK;
+}
+
+// ---- gradients --------------------------------------------------------------------------------------------------------------------
+// As many pieces of a row as a block has on their way together, or a wavefront per row.
+template <typename T, typename C, int LANES, bool ENTROPY>
+__global__ void __launch_bounds__(256) scores_bwd_kernel(Vocabulary p, int parts, const int32_t *__restrict__ ids, const T *__restrict__ logits,
+                                                         const Row<C> *__restrict__ kept, const C *__restrict__ grad_scores,
+                                                         const C *__restrict__ grad_entropy, T *__restrict__ dlogits) {
+  typedef typename Piece<T>::Held Held;
+  constexpr int V = Piece<T>::V, kStep = LANES * V * kAtOnce;
+  const int lane = threadIdx.x & (LANES - 1);
+  const long long units = LANES == 64 ? (p.rows + 3) / 4 : p.rows * parts;
+  for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const long long r = LANES == 64 ? unit * 4 + (threadIdx.x >> 6) : unit / parts;
+    if (LANES == 64 && r >= p.rows) return;
+    const long long at = (LANES == 64 ? 0 : (unit - r * parts) * kStep) + lane * V;
+    const T *z = logits + r * p.V;
+    T *out = dlogits + r * p.V;
+    Held held[kAtOnce];
+    load_pieces<LANES>(held, z, at, p.V);
+    const Row<C> row = kept[r];
+    int id = grad_scores ? ids[r] : -1;
+    if (id >= p.V) id = -1;
+    const C g = id < 0 ? C(0) : grad_scores[r], h = ENTROPY ? grad_entropy[r] : C(0), inverse = 1 / row.s;
+    const bool nothing = row.s == 0 || (id < 0 && !ENTROPY);
+    // one value; the other way round, p (-g - h (t - a)), a row's own numbers would be formed for each
+    auto gradient = [&](T value) {
+      const C t = (C)value - row.m, share = exponential<T>(t) * inverse;
+      C dz = -share * g;
+      if (ENTROPY) dz -= share * ((share > 0 ? t : C(0)) - row.a) * h;
+      return dz;
+    };
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const long long d = at + (long long)u * LANES * V;
+      if (d >= p.V) break;
+      Held dz;
+#pragma unroll
+      for (int n = 0; n < V; ++n) dz[n] = nothing ? T(0) : (T)gradient(held[u][n]);
+      const long long own = id - d;  // the token's place among them
+      if (own >= 0 && own < V && !nothing) {
+#pragma unroll
+        for (int n = 0; n < V; ++n)
+          if (n == own) dz[n] = (T)(gradient(held[u][n]) + g);
+      }
+      Piece<T>::store(out + d, p.V - d, dz);
+    }
+  }
 }
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) distillation_bwd_kernel(Vocabulary p, const int32_t *__restrict__ ids, const T *__restrict__ logits,
+__global__ void __launch_bounds__(256) distillation_bwd_kernel(Vocabulary p, int parts, const int32_t *__restrict__ ids, const T *__restrict__ logits,
                                                                const Row<C> *__restrict__ kept, const C *__restrict__ shares,
                                                                const C *__restrict__ grad, T *__restrict__ dlogits) {
+  typedef typename Piece<T>::Held Held;
+  constexpr int V = Piece<T>::V, kStep = 256 * V * kAtOnce;
   __shared__ int taught[kMostTaught];
   __shared__ C share_of[kMostTaught];
-  const long long r = blockIdx.x;
-  const T *z = logits + r * p.V;
-  T *out = dlogits + r * p.V;
-  const Row<C> row = kept[r];
   const int k = threadIdx.x;
-  if (k < p.top) taught[k] = ids[r * p.top + k], share_of[k] = shares[r * p.top + k];
-  __syncthreads();
-  const C per = (C)p.per, g = grad[r] * per, inverse = row.a / row.s;
-  const bool nothing = row.s == 0 || row.a == 0;
-  for (int j = threadIdx.x; j < p.V; j += 256) out[j] = nothing ? (T)0 : (T)(g * exp(((C)z[j] - row.m) * per) * inverse);
-  __syncthreads();  // the teacher's tokens are written once more, each by the first thread that has it
-  if (k >= p.top || nothing) return;
-  const int id = taught[k];
-  if (id < 0 || id >= p.V) return;
-  C q = 0;
-  for (int n = 0; n < p.top; ++n)
-    if (taught[n] == id) {
-      if (n < k) return;
-      q += share_of[n];
+  for (long long unit = blockIdx.x; unit < p.rows * parts; unit += gridDim.x) {
+    const long long r = unit / parts, from = (unit - r * parts) * kStep, at = from + k * V;
+    const T *z = logits + r * p.V;
+    T *out = dlogits + r * p.V;
+    Held held[kAtOnce];
+    load_pieces<256>(held, z, at, p.V);
+    const Row<C> row = kept[r];
+    __syncthreads();
+    if (k < p.top) taught[k] = ids[r * p.top + k], share_of[k] = shares[r * p.top + k];
+    __syncthreads();
+    const C per = (C)p.per, g = grad[r] * per, inverse = row.a / row.s;
+    const bool nothing = row.s == 0 || row.a == 0;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const long long d = at + (long long)u * 256 * V;
+      if (d >= p.V) break;
+      Held dz;
+#pragma unroll
+      for (int n = 0; n < V; ++n) dz[n] = nothing ? T(0) : (T)(g * (exponential<T>(((C)held[u][n] - row.m) * per) * inverse));
+      Piece<T>::store(out + d, p.V - d, dz);
     }
-  out[id] = (T)(g * (exp(((C)z[id] - row.m) * per) * inverse - q));
+    __syncthreads();  // the teacher's tokens are written once more, each by the first thread that has it
+    const int id = k < p.top ? taught[k] : -1;
+    if (id < 0 || id >= p.V || id < from || id >= from + kStep || nothing) continue;
+    C q = 0;
+    bool first = true;
+    for (int n = 0; n < p.top; ++n)
+      if (taught[n] == id) {
+        first = first && n >= k;
+        q += share_of[n];
+      }
+    if (first) out[id] = (T)(g * (exponential<T>(((C)z[id] - row.m) * per) * inverse - q));
+  }
 }
 
 int check(int dtype, int64_t rows, int64_t V, const char *who) {
@@ -260,10 +618,11 @@ int mg_log_probabilities_fwd(int dtype, int64_t rows, int64_t V, int top, const 
     typedef std::remove_pointer_t<decltype(t)> T;
     typedef std::remove_pointer_t<decltype(c)> C;
     ScopedTiming timed(TAG_SCORES);
-    scores_kernel<T, C><<<dim3((unsigned)rows), dim3(256), 0, runtime().stream>>>(p, ids, (const T *)logits, (C *)scores, (C *)entropy, (Row<C> *)kept,
-                                                                                  (C *)top_scores, top_ids);
-    MG_HIP(hipGetLastError());
-    return (int)MG_OK;
+    const Scores<T, C> end{ids, (const T *)logits, (C *)scores, (C *)entropy, (Row<C> *)kept};
+    if (entropy && top) return over_rows<T, C, true, true>(p, logits, end, top_scores, top_ids);
+    if (entropy) return over_rows<T, C, true, false>(p, logits, end, nullptr, nullptr);
+    if (top) return over_rows<T, C, false, true>(p, logits, end, top_scores, top_ids);
+    return over_rows<T, C, false, false>(p, logits, end, nullptr, nullptr);
   });
 }
 
@@ -280,8 +639,17 @@ int mg_log_probabilities_bwd(int dtype, int64_t rows, int64_t V, const int32_t *
     typedef std::remove_pointer_t<decltype(t)> T;
     typedef std::remove_pointer_t<decltype(c)> C;
     ScopedTiming timed(TAG_SCORES_BWD);
-    scores_bwd_kernel<T, C><<<dim3((unsigned)rows), dim3(256), 0, runtime().stream>>>(p, ids, (const T *)logits, (const Row<C> *)kept,
-                                                                                      (const C *)grad_scores, (const C *)grad_entropy, (T *)dlogits);
+    auto run = [&](auto lanes, auto with_entropy) {
+      const long long parts = ceil_div(V, lanes * Piece<T>::V * kAtOnce), blocks = lanes == 64 ? ceil_div(rows, 4) : rows * parts;
+      scores_bwd_kernel<T, C, lanes, with_entropy><<<dim3((unsigned)std::min<long long>(blocks, 1 << 22)), dim3(256), 0, runtime().stream>>>(
+          p, (int)parts, ids, (const T *)logits, (const Row<C> *)kept, (const C *)grad_scores, (const C *)grad_entropy, (T *)dlogits);
+    };
+    auto by_length = [&](auto with_entropy) {
+      if (V <= 64 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 64>{}, with_entropy);
+      else run(std::integral_constant<int, 256>{}, with_entropy);
+    };
+    if (grad_entropy) by_length(std::true_type{});
+    else by_length(std::false_type{});
     MG_HIP(hipGetLastError());
     return (int)MG_OK;
   });
@@ -301,13 +669,9 @@ int mg_distillation_fwd(int dtype, int teacher_dtype, int64_t rows, int64_t V, i
     typedef std::remove_pointer_t<decltype(t)> T;
     typedef std::remove_pointer_t<decltype(c)> C;
     ScopedTiming timed(TAG_DISTILLATION);
-    const dim3 grid((unsigned)rows);
     if (teacher_dtype == dtype)
-      distillation_kernel<T, T, C><<<grid, dim3(256), 0, runtime().stream>>>(p, ids, (const T *)logits, (const T *)teacher, (C *)loss, (Row<C> *)kept, (C *)shares);
-    else
-      distillation_kernel<T, C, C><<<grid, dim3(256), 0, runtime().stream>>>(p, ids, (const T *)logits, (const C *)teacher, (C *)loss, (Row<C> *)kept, (C *)shares);
-    MG_HIP(hipGetLastError());
-    return (int)MG_OK;
+      return over_rows<T, C, false, false>(p, logits, Distillation<T, T, C>{ids, (const T *)logits, (const T *)teacher, (C *)loss, (Row<C> *)kept, (C *)shares}, nullptr, nullptr);
+    return over_rows<T, C, false, false>(p, logits, Distillation<T, C, C>{ids, (const T *)logits, (const C *)teacher, (C *)loss, (Row<C> *)kept, (C *)shares}, nullptr, nullptr);
   });
 }
 
@@ -323,8 +687,9 @@ int mg_distillation_bwd(int dtype, int64_t rows, int64_t V, int64_t K, double te
     typedef std::remove_pointer_t<decltype(t)> T;
     typedef std::remove_pointer_t<decltype(c)> C;
     ScopedTiming timed(TAG_DISTILLATION_BWD);
-    distillation_bwd_kernel<T, C><<<dim3((unsigned)rows), dim3(256), 0, runtime().stream>>>(p, ids, (const T *)logits, (const Row<C> *)kept,
-                                                                                            (const C *)shares, (const C *)grad, (T *)dlogits);
+    const long long parts = ceil_div(V, 256 * Piece<T>::V * kAtOnce);
+    distillation_bwd_kernel<T, C><<<dim3((unsigned)std::min<long long>(rows * parts, 1 << 22)), dim3(256), 0, runtime().stream>>>(
+        p, (int)parts, ids, (const T *)logits, (const Row<C> *)kept, (const C *)shares, (const C *)grad, (T *)dlogits);
     MG_HIP(hipGetLastError());
     return (int)MG_OK;
   });
