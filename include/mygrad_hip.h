@@ -490,12 +490,13 @@ int mg_head_norm_bwd(const mg_head_norm_desc *desc, const void *x, const void *w
  * dtype: MG_F16, MG_F32 or MG_F64.  Sums and statistics are float32 (float64 for MG_F64), and every result is rounded once.  Tokens
  * are int32 on the device; a negative one stands for none. */
 
-/* y = weight * (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps) + bias over the D values of each row; weight and bias (D,) may be null. */
-int mg_layer_norm_fwd(int dtype, int64_t rows, int64_t D, double eps, const void *x, const void *weight, const void *bias, void *y);
+/* y = weight * (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps) + bias over the D values of each row; weight and bias (D,) may be null.
+ * kept:(rows, 3), float32 (float64 for MG_F64), is for mg_layer_norm_bwd, and null where there will be none.  Fewer than 2^24 rows. */
+int mg_layer_norm_fwd(int dtype, int64_t rows, int64_t D, double eps, const void *x, const void *weight, const void *bias, void *y, void *kept);
 
 /* Its gradients, like x, weight and bias; any of dx, dweight, dbias may be null (not wanted), not all three.  Run-to-run identical. */
-int mg_layer_norm_bwd(int dtype, int64_t rows, int64_t D, double eps, const void *x, const void *weight, const void *grad, void *dx, void *dweight,
-                      void *dbias);
+int mg_layer_norm_bwd(int dtype, int64_t rows, int64_t D, const void *x, const void *weight, const void *kept, const void *grad, void *dx,
+                      void *dweight, void *dbias);
 
 /* out[n] = scale * weight[ids[n]], weight:(rows, D), out:(tokens, D); zeros for tokens that are none (or lie beyond the table). */
 int mg_embedding_fwd(int dtype, int64_t tokens, int64_t rows, int64_t D, double scale, const int32_t *ids, const void *weight, void *out);

@@ -223,8 +223,8 @@ _SIGNATURES = {
     "mg_cache_write": [ctypes.c_int] + [ctypes.c_int64] * 4 + [_vp] * 5,
     "mg_head_norm_fwd": [ctypes.POINTER(HeadNormDesc)] + [_vp] * 4,
     "mg_head_norm_bwd": [ctypes.POINTER(HeadNormDesc)] + [_vp] * 6,
-    "mg_layer_norm_fwd": [ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_double] + [_vp] * 4,
-    "mg_layer_norm_bwd": [ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_double] + [_vp] * 6,
+    "mg_layer_norm_fwd": [ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_double] + [_vp] * 5,
+    "mg_layer_norm_bwd": [ctypes.c_int] + [ctypes.c_int64] * 2 + [_vp] * 7,
     "mg_embedding_fwd": [ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_double] + [_vp] * 3,
     "mg_embedding_bwd": [ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_double] + [_vp] * 3,
     "mg_log_probabilities_fwd": [ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_int] + [_vp] * 7,

@@ -32,11 +32,33 @@ struct Piece {
   }
 };
 
+// What another lane of a row of sixteen has, by a move within the vector unit.
+template <int CONTROL>
+__device__ __forceinline__ float from_lane(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CONTROL, 0xf, 0xf, true));
+}
+template <int CONTROL>
+__device__ __forceinline__ double from_lane(double v) {
+  typedef int Two __attribute__((ext_vector_type(2)));
+  Two q = __builtin_bit_cast(Two, v);
+  q[0] = __builtin_amdgcn_mov_dpp(q[0], CONTROL, 0xf, 0xf, true), q[1] = __builtin_amdgcn_mov_dpp(q[1], CONTROL, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, q);
+}
+
+// The sum over each run of `lanes` lanes, a power of two, for all of them.
+template <typename C>
+__device__ __forceinline__ C lanes_add(C v, int lanes) {
+  if (lanes > 1) v += from_lane<0xb1>(v);   // lanes 1 0 3 2 of four
+  if (lanes > 2) v += from_lane<0x4e>(v);   // 2 3 0 1
+  if (lanes > 4) v += from_lane<0x141>(v);  // eight from behind
+  if (lanes > 8) v += from_lane<0x140>(v);  // sixteen from behind
+  if (lanes > 16) v += __shfl_xor(v, 16);
+  if (lanes > 32) v += __shfl_xor(v, 32);
+  return v;
+}
 template <typename C>
 __device__ __forceinline__ C wave_add(C v) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
-  return v;
+  return lanes_add(v, 64);
 }
 
 // The sums of N values over a block of up to 16 wavefronts, for all of its threads; `space` is N * 16 values of LDS.

@@ -40,10 +40,14 @@ class LayerNorm(Operation):
         self._backed = None
         if xd.size == 0:
             return np.empty(xd.shape, dtype=xd.dtype)
-        self._call = _hip.storage_code(xd.dtype), prod(xd.shape[:-1]), dim, float(eps)
+        self._call = _, rows, _ = _hip.storage_code(xd.dtype), prod(xd.shape[:-1]), dim
+        self._kept = None
+        if not all(t.constant for t in self.variables):  # two parts of the mean and 1 / sqrt for each row
+            self._kept = _device.DeviceBuffer(3 * rows * (8 if xd.dtype == np.float64 else 4))
         buffers = [_device.to_device(v) if there else None for v, there in zip(values, self._there)]
         out = _device.DeviceBuffer(xd.nbytes)
-        _hip.check(_hip.lib().mg_layer_norm_fwd(*self._call, *(None if b is None else b.ptr for b in buffers), out.ptr))
+        _hip.check(_hip.lib().mg_layer_norm_fwd(*self._call, eps, *(None if b is None else b.ptr for b in buffers), out.ptr,
+                                                None if self._kept is None else self._kept.ptr))
         y = _device.download(out, xd.shape, xd.dtype)
         _device.attach(y, out)
         return y
@@ -55,7 +59,7 @@ class LayerNorm(Operation):
         xb, gb = _device.to_device(values[0]), _device.to_device(grad, values[0].dtype)
         wb = _device.to_device(values[1]) if self._there[1] else None
         out = {i: _device.DeviceBuffer(values[i].nbytes) for i in sorted(want)}
-        _hip.check(_hip.lib().mg_layer_norm_bwd(*self._call, xb.ptr, None if wb is None else wb.ptr, gb.ptr,
+        _hip.check(_hip.lib().mg_layer_norm_bwd(*self._call, xb.ptr, None if wb is None else wb.ptr, self._kept.ptr, gb.ptr,
                                                 *(out[i].ptr if i in out else None for i in range(3))))
         return {i: _device.download(buf, values[i].shape, values[i].dtype) for i, buf in out.items()}
 
