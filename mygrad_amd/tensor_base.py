@@ -257,6 +257,10 @@ class Tensor:
 
         ref_f = ReferenceType(f)
         for v in tensor_vars:
+            # a tensor that is only ever read (a constant, weights that a model answers with) is never cleared: without this it would
+            # collect one dead reference per operation, which hash alike where the operations lie in the same memory one after another
+            if len(v._ops) >= 32:
+                v._ops = {ref for ref in v._ops if ref() is not None}
             v._ops.add(ref_f)
 
         out = cls(op_out, constant=constant, copy=False, _creator=f)

@@ -162,3 +162,21 @@ def test_the_oracle_of_rows_without_a_distribution():
     loss, dz = ora.distillation(z, [[0, 1]] * 3, np.zeros((3, 2)), 1.0, np.ones(3))
     assert np.isinf(loss[:2]).all() and loss[2] == 0 and not dz[0].any()
     assert ora.likeliest([[1.0, 2.0, 2.0, -np.inf]], 4).tolist() == [[1, 2, 0, 3]]
+
+
+def test_a_tensor_that_is_only_read_collects_no_dead_operations(tmp_path):
+    """Weights that answer and are never trained: what is gone is dropped, what lives is kept."""
+    program = """
+import numpy as np
+import mygrad_amd as mg
+from mygrad_amd.nnet import embedding
+weight = mg.device_tensor(np.ones((4, 8), np.float32))
+live = [embedding(weight, [n]) for n in range(3)]
+for n in range(500):
+    embedding(weight, [1])
+assert len(weight._ops) <= 40 and {out.creator for out in live} <= {ref() for ref in weight._ops}
+live[1].backward(mg.device_tensor(np.ones((1, 8), np.float32), constant=True))
+assert weight.grad.shape == (4, 8)
+print("dropped")
+"""
+    assert "dropped" in run_on_standins(tmp_path, program)
