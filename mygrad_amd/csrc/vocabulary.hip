@@ -186,19 +186,22 @@ struct Likeliest {
   int places[kRoom];
   Found first[kMostTop];
   int count;
+  unsigned long long least;
   Found bound;  // what does not come before it, and is not it, is not wanted
 
   __device__ __forceinline__ Found at(int n) const { return Found{values[n], places[n]}; }
 
-  // The k-th of the threads' largest values (0: a thread has none).
+  // The k-th of the threads' largest values (0: a thread has none): the smallest of those that fewer than k are larger than.
   __device__ __forceinline__ void begin(Order most, int k) {
     values[threadIdx.x] = most;
-    if (threadIdx.x == 0) count = 0, bound = Found{0, 0x7fffffff};
+    if (threadIdx.x == 0) count = 0, least = ~0ull, bound = Found{0, 0x7fffffff};
     __syncthreads();
-    int rank = 0;
-    for (int n = 0; n < 256; ++n) rank += values[n] > most || (values[n] == most && n < (int)threadIdx.x);
+    int larger = 0;
+#pragma unroll 16
+    for (int n = 0; n < 256; ++n) larger += values[n] > most;
+    if (larger < k) atomicMin((unsigned long long *)&least, (unsigned long long)most);
     __syncthreads();
-    if (rank == k - 1 && most) bound = Found{most, 0x7fffffff};
+    if (threadIdx.x == 0) bound.value = (Order)least;
     __syncthreads();
   }
   __device__ __forceinline__ void add(const Found &f) {
@@ -212,7 +215,8 @@ struct Likeliest {
     for (int i = threadIdx.x; i < n; i += 256) {
       const Found mine = at(i);
       int better = 0;
-      for (int j = 0; j < n && better < k; ++j) better += at(j).before(mine);
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) better += at(j).before(mine);
       if (better < k) first[better] = mine;
     }
     __syncthreads();
@@ -406,13 +410,12 @@ __global__ void __launch_bounds__(256) row_join_kernel(Vocabulary p, Top w, cons
       // the largest of the parts' last ones bounds the row's
       Order last = 0;
       for (int n = threadIdx.x; n < w.parts; n += 256) last = max(last, values[(long long)n * p.top + p.top - 1]);
-      list.values[threadIdx.x] = last;
-      if (threadIdx.x == 0) list.count = 0;
+#pragma unroll
+      for (int m = 32; m; m >>= 1) last = max(last, (Order)__shfl_xor(last, m));
+      if ((threadIdx.x & 63) == 0) list.values[threadIdx.x >> 6] = last;
       __syncthreads();
-      if (threadIdx.x == 0) {
-        for (int n = 1; n < 256; ++n) last = max(last, list.values[n]);
-        list.bound = Candidate<C>{last, 0x7fffffff};
-      }
+      if (threadIdx.x == 0)
+        list.count = 0, list.bound = Candidate<C>{max(max(list.values[0], list.values[1]), max(list.values[2], list.values[3])), 0x7fffffff};
       __syncthreads();
       const int all = w.parts * p.top;
       for (int n0 = 0; n0 < all; n0 += 256) {
@@ -441,14 +444,15 @@ struct Plan {
   unsigned blocks;
 };
 
-// Rows that a wavefront takes in one step go four to a block.  Longer ones have a block each, or where that leaves compute units without
-// work, parts of a step or more.
+// Rows that a wavefront takes in one step go four to a block.  Longer ones have a block each, or, where there are fewer than two for a
+// compute unit, parts of a step or more for four blocks a unit.  50001 halves a row, us with and without parts: 300 rows 12 + 4 and 14, 600
+// rows 19 + 4 and 18; one row of 131101 4 + 3 in parts.
 template <typename T>
 Plan plan_of(const Vocabulary &p, bool alone) {
   constexpr int V = Piece<T>::V;
   const long long most = 1 << 22;
   if (!alone && p.V <= 64 * V * kAtOnce) return Plan{true, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 4), most)};
-  const long long wanted = ceil_div(4ll * runtime().props.multiProcessorCount, p.rows), step = 256 * V;
+  const long long wanted = 4ll * runtime().props.multiProcessorCount / p.rows, step = 256 * V;
   const long long parts = std::max<long long>(1, std::min<long long>(wanted, ceil_div(p.V, step)));
   const long long part = ceil_div(ceil_div(p.V, parts), step) * step;
   Plan plan{false, (int)ceil_div(p.V, part), (int)std::min<long long>(part, p.V), 0};

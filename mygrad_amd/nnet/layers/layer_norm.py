@@ -13,6 +13,8 @@ from ...tensor_base import Tensor
 __all__ = ["LayerNorm", "layer_norm"]
 
 _DTYPES = (np.float16, np.float32, np.float64)
+_MOST_SHAPES = 64
+_described = {}  # what was checked of calls of the same shapes
 
 
 class LayerNorm(Operation):
@@ -22,50 +24,63 @@ class LayerNorm(Operation):
 
     def __call__(self, x, weight, bias, *, eps):
         self.variables = (x, weight, bias)
-        values = [_device.value_of(t) for t in self.variables]
-        xd = values[0]
-        if xd.ndim < 1:
-            raise ValueError(f"`x` must have the axes (..., dim), got shape {xd.shape}")
-        if xd.dtype not in _DTYPES:
-            raise TypeError(f"layer_norm runs on the GPU in float16, float32 or float64, got {xd.dtype} (there is no CPU fallback)")
-        dim = xd.shape[-1]
-        self._there = [True, values[1].size > 0, values[2].size > 0]
-        for name, value, there in zip(("weight", "bias"), values[1:], self._there[1:]):
-            if there and value.shape != (dim,):
-                raise ValueError(f"`{name}` must have shape ({dim},), got {value.shape}")
-            if there and value.dtype != xd.dtype:
-                raise TypeError(f"layer_norm takes `{name}` in the dtype of `x` ({xd.dtype}), got {value.dtype}")
-        if not 0 <= eps < np.inf:
-            raise ValueError(f"`eps` must be a non-negative number, got {eps}")
+        xd, wd, bd = values = [_device.value_of(t) for t in self.variables]
+        key = xd.shape, xd.dtype, wd.shape, wd.dtype, bd.shape, bd.dtype, eps
+        found = _described.get(key)
+        if found is None:
+            found = self._describe(values, eps)
+            if len(_described) >= _MOST_SHAPES:
+                _described.clear()
+            _described[key] = found
+        self._call, self._there, item = found
+        self._empty = self._call[1] * self._call[2] == 0
         self._backed = None
-        if xd.size == 0:
+        if self._empty:
             return np.empty(xd.shape, dtype=xd.dtype)
-        self._call = _, rows, _ = _hip.storage_code(xd.dtype), prod(xd.shape[:-1]), dim
         self._kept = None
-        if not all(t.constant for t in self.variables):  # two parts of the mean and 1 / sqrt for each row
-            self._kept = _device.DeviceBuffer(3 * rows * (8 if xd.dtype == np.float64 else 4))
-        buffers = [_device.to_device(v) if there else None for v, there in zip(values, self._there)]
+        if not (x.constant and weight.constant and bias.constant):  # two parts of the mean and 1 / sqrt for each row
+            self._kept = _device.DeviceBuffer(3 * self._call[1] * item)
+        xb, wb, bb = (_device.to_device(v) if there else None for v, there in zip(values, self._there))
         out = _device.DeviceBuffer(xd.nbytes)
-        _hip.check(_hip.lib().mg_layer_norm_fwd(*self._call, eps, *(None if b is None else b.ptr for b in buffers), out.ptr,
+        _hip.check(_hip.lib().mg_layer_norm_fwd(*self._call, eps, xb.ptr, None if wb is None else wb.ptr, None if bb is None else bb.ptr, out.ptr,
                                                 None if self._kept is None else self._kept.ptr))
         y = _device.download(out, xd.shape, xd.dtype)
         _device.attach(y, out)
         return y
 
+    @staticmethod
+    def _describe(values, eps):
+        """The checked arguments of the entry points, which of the operands there are, and the size of a statistic."""
+        x = values[0]
+        if x.ndim < 1:
+            raise ValueError(f"`x` must have the axes (..., dim), got shape {x.shape}")
+        if x.dtype not in _DTYPES:
+            raise TypeError(f"layer_norm runs on the GPU in float16, float32 or float64, got {x.dtype} (there is no CPU fallback)")
+        dim = x.shape[-1]
+        there = True, values[1].size > 0, values[2].size > 0
+        for name, value, given in zip(("weight", "bias"), values[1:], there[1:]):
+            if given and value.shape != (dim,):
+                raise ValueError(f"`{name}` must have shape ({dim},), got {value.shape}")
+            if given and value.dtype != x.dtype:
+                raise TypeError(f"layer_norm takes `{name}` in the dtype of `x` ({x.dtype}), got {value.dtype}")
+        if not 0 <= eps < np.inf:
+            raise ValueError(f"`eps` must be a non-negative number, got {eps}")
+        return (_hip.storage_code(x.dtype), prod(x.shape[:-1]), dim), there, 8 if x.dtype == np.float64 else 4
+
     def _run_backward(self, grad, want):
-        values = [_device.value_of(t) for t in self.variables]
-        if grad.shape != values[0].shape:
+        x, w, b = values = [_device.value_of(t) for t in self.variables]
+        if grad.shape != x.shape:
             raise NotImplementedError(f"layer_norm backward for gradient of shape {grad.shape} (no CPU fallback)")
-        xb, gb = _device.to_device(values[0]), _device.to_device(grad, values[0].dtype)
-        wb = _device.to_device(values[1]) if self._there[1] else None
-        out = {i: _device.DeviceBuffer(values[i].nbytes) for i in sorted(want)}
+        xb, gb = _device.to_device(x), _device.to_device(grad, x.dtype)
+        wb = _device.to_device(w) if self._there[1] else None
+        out = [_device.DeviceBuffer(v.nbytes) if i in want else None for i, v in enumerate(values)]
         _hip.check(_hip.lib().mg_layer_norm_bwd(*self._call, xb.ptr, None if wb is None else wb.ptr, self._kept.ptr, gb.ptr,
-                                                *(out[i].ptr if i in out else None for i in range(3))))
-        return {i: _device.download(buf, values[i].shape, values[i].dtype) for i, buf in out.items()}
+                                                *(None if buf is None else buf.ptr for buf in out)))
+        return {i: _device.download(out[i], values[i].shape, x.dtype) for i in want}
 
     def backward_var(self, grad, index, **kwargs):
-        value = _device.value_of(self.variables[index])
-        if _device.value_of(self.variables[0]).size == 0 or value.size == 0:
+        if self._empty or not self._there[index]:
+            value = _device.value_of(self.variables[index])
             return np.zeros(value.shape, dtype=value.dtype)
         # backward() asks for each variable in turn with the same `grad`: the first request computes all that are wanted
         if self._backed is None or self._backed[0] is not grad or index not in self._backed[1]:

@@ -10,13 +10,15 @@ import numpy as np
 from ... import _device, _graph, _hip
 from ...operation_base import Operation
 from ...tensor_base import Tensor
-from ..layers.embedding import as_tokens
+from ..layers.embedding import TokenIds, as_tokens
 from .log_probabilities import result_type
 
 __all__ = ["Distillation", "distillation"]
 
 _DTYPES = (np.float16, np.float32, np.float64)
 _MOST_TAUGHT = 256
+_MOST_SHAPES = 64
+_described = {}  # what was checked of calls of the same shapes
 
 
 class Distillation(Operation):
@@ -29,44 +31,56 @@ class Distillation(Operation):
         z, y = _device.value_of(logits), _device.value_of(teacher)
         if _graph.TRACK_GRAPH and not teacher.constant:
             raise ValueError("the teacher's logits have no gradient: they must be a constant")
+        tokens = self._tokens = tokens if isinstance(tokens, TokenIds) else TokenIds(tokens)
+        key = z.shape, z.dtype, y.shape, y.dtype, tokens.shape, temperature
+        found = _described.get(key)
+        if found is None:
+            found = self._describe(z, y, tokens, temperature)
+            if len(_described) >= _MOST_SHAPES:
+                _described.clear()
+            _described[key] = found
+        self._code, self._call, self._dtype, taught = found
+        rows, vocabulary, count, _ = self._call
+        as_tokens(tokens, vocabulary)
+        lead, item = z.shape[:-1], self._dtype.itemsize
+        self._empty = rows == 0
+        if self._empty:
+            return np.empty(lead, dtype=self._dtype)
+        yb = _device.to_device(y, None if taught == y.dtype else taught)
+        out = _device.DeviceBuffer(rows * item)
+        keep = not logits.constant
+        self._kept = _device.DeviceBuffer(3 * rows * item) if keep else None
+        self._shares = _device.DeviceBuffer(rows * count * item) if keep else None
+        _hip.check(_hip.lib().mg_distillation_fwd(self._code, _hip.storage_code(taught), *self._call, _device.to_device(z).ptr, tokens._buffer().ptr,
+                                                  yb.ptr, out.ptr, *((self._kept.ptr, self._shares.ptr) if keep else (None, None))))
+        loss = _device.download(out, lead, self._dtype)
+        _device.attach(loss, out)
+        return loss
+
+    @staticmethod
+    def _describe(z, y, tokens, temperature):
+        """The checked arguments of the entry points, the type of the loss and the one that the teacher's logits are taken in."""
         if z.ndim < 1 or z.shape[-1] == 0:
             raise ValueError(f"`logits` must have the axes (..., vocabulary), got shape {z.shape}")
         if z.dtype not in _DTYPES or y.dtype not in _DTYPES:
             raise TypeError(f"distillation runs on the GPU in float16, float32 or float64, got {z.dtype} and {y.dtype} (there is no CPU fallback)")
-        self._dtype = result_type(z.dtype)
-        if result_type(y.dtype) != self._dtype and y.dtype == np.float64:
+        dtype = result_type(z.dtype)
+        if y.dtype == np.float64 and dtype != np.float64:
             raise TypeError(f"a teacher in float64 for logits in {z.dtype}: its digits would be lost")
-        self._tokens = as_tokens(tokens, z.shape[-1])
-        if y.shape != self._tokens.shape or y.ndim < 1 or y.shape[:-1] != z.shape[:-1]:
-            raise ValueError(f"tokens of shape {self._tokens.shape} and teacher's logits of shape {y.shape} for logits of shape {z.shape}")
+        if y.shape != tokens.shape or y.ndim < 1 or y.shape[:-1] != z.shape[:-1]:
+            raise ValueError(f"tokens of shape {tokens.shape} and teacher's logits of shape {y.shape} for logits of shape {z.shape}")
         if not 1 <= y.shape[-1] <= _MOST_TAUGHT:
             raise ValueError(f"a row is taught by 1 to {_MOST_TAUGHT} tokens, got {y.shape[-1]}")
         if not isinstance(temperature, Real) or not 1e-30 <= temperature <= 1e30:
             raise ValueError(f"`temperature` must be a positive number (1e-30 to 1e30), got {temperature}")
-        lead = z.shape[:-1]
-        if z.size == 0:
-            return np.empty(lead, dtype=self._dtype)
-        rows, item = prod(lead), self._dtype.itemsize
-        self._call = rows, z.shape[-1], y.shape[-1], float(temperature)
-        self._code = _hip.storage_code(z.dtype)
-        as_it_is = y.dtype in (z.dtype, self._dtype)
-        yb = _device.to_device(y, None if as_it_is else self._dtype)
-        out = _device.DeviceBuffer(rows * item)
-        keep = not logits.constant
-        self._kept = _device.DeviceBuffer(3 * rows * item) if keep else None
-        self._shares = _device.DeviceBuffer(rows * y.shape[-1] * item) if keep else None
-        _hip.check(_hip.lib().mg_distillation_fwd(self._code, _hip.storage_code(y.dtype if as_it_is else self._dtype), *self._call,
-                                                  _device.to_device(z).ptr, self._tokens._buffer().ptr, yb.ptr, out.ptr,
-                                                  *((self._kept.ptr, self._shares.ptr) if keep else (None, None))))
-        loss = _device.download(out, lead, self._dtype)
-        _device.attach(loss, out)
-        return loss
+        call = prod(z.shape[:-1]), z.shape[-1], y.shape[-1], float(temperature)
+        return _hip.storage_code(z.dtype), call, dtype, y.dtype if y.dtype in (z.dtype, dtype) else dtype
 
     def backward_var(self, grad, index, **kwargs):
         z = _device.value_of(self.variables[0])
         if index != 0:
             raise NotImplementedError("the teacher's logits have no gradient")
-        if z.size == 0:
+        if self._empty:
             return np.zeros(z.shape, dtype=z.dtype)
         if grad.shape != z.shape[:-1]:
             raise NotImplementedError(f"distillation backward for gradient of shape {grad.shape} (no CPU fallback)")

@@ -24,10 +24,11 @@ def result_type(dtype):
     return np.dtype(np.float64 if dtype == np.float64 else np.float32)
 
 
-class _Scores:
-    """The checked arguments of one call, and its launch."""
+class _Plan:
+    """The checked arguments of calls of one kind, and their launch."""
 
-    def __init__(self, z, tokens, entropy, top):
+    def __init__(self, z, lead, entropy, top):
+        """``lead``: the shape of the tokens, None without them."""
         if z.ndim < 1:
             raise ValueError(f"`logits` must have the axes (..., vocabulary), got shape {z.shape}")
         if z.dtype not in _DTYPES:
@@ -38,39 +39,58 @@ class _Scores:
             raise TypeError(f"`entropy` must be a boolean value, got: {entropy}")
         if not isinstance(top, Integral) or isinstance(top, (bool, np.bool_)) or not 0 <= top <= min(_MOST_TOP, z.shape[-1]):
             raise ValueError(f"`top` must be a whole number up to {_MOST_TOP} and to the vocabulary of {z.shape[-1]}, got {top}")
-        if tokens is None and not entropy and not top:
+        if lead is None and not entropy and not top:
             raise TypeError("log_probabilities without tokens, entropies or alternatives has nothing to compute")
+        if lead is not None and lead != z.shape[:-1]:
+            raise ValueError(f"tokens of shape {lead} for logits of shape {z.shape}")
         self.lead, self.rows, self.vocabulary = z.shape[:-1], prod(z.shape[:-1]), z.shape[-1]
-        self.tokens = None if tokens is None else as_tokens(tokens, self.vocabulary)
-        if self.tokens is not None and self.tokens.shape != self.lead:
-            raise ValueError(f"tokens of shape {self.tokens.shape} for logits of shape {z.shape}")
-        self.entropy, self.top = bool(entropy), int(top)
+        self.tokens, self.entropy, self.top, self.empty = lead is not None, bool(entropy), int(top), z.size == 0
         self.code, self.dtype = _hip.storage_code(z.dtype), result_type(z.dtype)
-        self.shape = (2, *self.lead) if entropy and tokens is not None else self.lead  # of what has a gradient
-
-    def ids(self):
-        return None if self.tokens is None else self.tokens._buffer().ptr
+        self.shape = (2, *self.lead) if entropy and self.tokens else self.lead  # of what has a gradient
+        self.nbytes = prod(self.shape) * self.dtype.itemsize
+        self.kept_bytes = 3 * self.rows * self.dtype.itemsize
+        self.alternatives = (*self.lead, self.top)
 
     def planes(self, ptr):
         """Where log probabilities and entropies (or their gradients) lie."""
-        if self.tokens is None:
+        if not self.tokens:
             return None, ptr
-        return ptr, ptr + self.rows * self.dtype.itemsize if self.entropy else None
+        return ptr, ptr + self.nbytes // 2 if self.entropy else None
 
-    def run(self, z, keep):
+    def no_alternatives(self):
+        return np.empty(self.alternatives, dtype=self.dtype), np.empty(self.alternatives, dtype=np.int32)
+
+    def run(self, z, ids, keep):
         """The memory of the values that have a gradient and, if the gradient is to follow, of what it needs; the likeliest tokens."""
-        item = self.dtype.itemsize
-        out = _device.DeviceBuffer(prod(self.shape) * item) if self.tokens is not None or self.entropy else None
-        kept = _device.DeviceBuffer(3 * self.rows * item) if keep else None
-        scores, entropies = (None, None) if out is None else self.planes(out.ptr)
-        top = (None, None)
+        out = _device.DeviceBuffer(self.nbytes) if self.tokens or self.entropy else None
+        kept = _device.DeviceBuffer(self.kept_bytes) if keep else None
+        top = ()
         if self.top:
-            shape = (*self.lead, self.top)
-            top = _device.DeviceArray(_device.DeviceBuffer(prod(shape) * item), shape, self.dtype), _device.DeviceArray(
-                _device.DeviceBuffer(prod(shape) * 4), shape, np.int32)
-        _hip.check(_hip.lib().mg_log_probabilities_fwd(self.code, self.rows, self.vocabulary, self.top, self.ids(), _device.to_device(z).ptr, scores,
-                                                       entropies, None if kept is None else kept.ptr, *(None if a is None else a.buf.ptr for a in top)))
+            count = self.rows * self.top
+            top = (_device.DeviceArray(_device.DeviceBuffer(count * self.dtype.itemsize), self.alternatives, self.dtype),
+                   _device.DeviceArray(_device.DeviceBuffer(count * 4), self.alternatives, np.int32))
+        _hip.check(_hip.lib().mg_log_probabilities_fwd(self.code, self.rows, self.vocabulary, self.top, ids, _device.to_device(z).ptr,
+                                                       *((None, None) if out is None else self.planes(out.ptr)), None if kept is None else kept.ptr,
+                                                       *((top[0].buf.ptr, top[1].buf.ptr) if top else (None, None))))
         return out, kept, top
+
+
+_plans = {}
+_MOST_PLANS = 64
+
+
+def _plan(z, tokens, entropy, top):
+    """The plan of a call, whose tokens fit its vocabulary."""
+    key = z.shape, z.dtype, None if tokens is None else tokens.shape, entropy, top, type(entropy), type(top)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _Plan(z, key[2], entropy, top)
+        if len(_plans) >= _MOST_PLANS:
+            _plans.clear()
+        _plans[key] = plan
+    if tokens is not None:
+        as_tokens(tokens, plan.vocabulary)
+    return plan
 
 
 class LogProbabilities(Operation):
@@ -79,29 +99,31 @@ class LogProbabilities(Operation):
     takes_device_arrays = True
 
     def __call__(self, logits, *, tokens, entropy, top, alternatives):
-        """``alternatives``: a list that receives the likeliest tokens and their log probabilities."""
+        """``tokens``: TokenIds or None; ``alternatives``: a list that receives the likeliest tokens and their log probabilities."""
         self.variables = (logits,)
         z = _device.value_of(logits)
-        self._scores = scores = _Scores(z, tokens, entropy, top)
-        if z.size == 0:
-            alternatives += np.empty((*scores.lead, top), dtype=scores.dtype), np.empty((*scores.lead, top), dtype=np.int32)
-            return np.empty(scores.shape, dtype=scores.dtype)
-        out, self._kept, found = scores.run(z, not logits.constant)
+        plan = self._plan = _plan(z, tokens, entropy, top)
+        self._tokens = tokens
+        if plan.empty:
+            alternatives += plan.no_alternatives()
+            return np.empty(plan.shape, dtype=plan.dtype)
+        out, self._kept, found = plan.run(z, None if tokens is None else tokens._buffer().ptr, not logits.constant)
         alternatives += found
-        y = _device.download(out, scores.shape, scores.dtype)
+        y = _device.download(out, plan.shape, plan.dtype)
         _device.attach(y, out)
         return y
 
     def backward_var(self, grad, index, **kwargs):
-        scores, z = self._scores, _device.value_of(self.variables[index])
-        if z.size == 0:
+        plan, z = self._plan, _device.value_of(self.variables[index])
+        if plan.empty:
             return np.zeros(z.shape, dtype=z.dtype)
-        if grad.shape != scores.shape:
+        if grad.shape != plan.shape:
             raise NotImplementedError(f"log_probabilities backward for gradient of shape {grad.shape} (no CPU fallback)")
-        gb = _device.to_device(grad, scores.dtype)
+        gb = _device.to_device(grad, plan.dtype)
         out = _device.DeviceBuffer(z.nbytes)
-        _hip.check(_hip.lib().mg_log_probabilities_bwd(scores.code, scores.rows, scores.vocabulary, scores.ids(), _device.to_device(z).ptr, self._kept.ptr,
-                                                       *scores.planes(gb.ptr), out.ptr))
+        ids = None if self._tokens is None else self._tokens._buffer().ptr
+        _hip.check(_hip.lib().mg_log_probabilities_bwd(plan.code, plan.rows, plan.vocabulary, ids, _device.to_device(z).ptr, self._kept.ptr,
+                                                       *plan.planes(gb.ptr), out.ptr))
         return _device.download(out, z.shape, z.dtype)
 
 
@@ -150,17 +172,16 @@ def log_probabilities(logits, tokens=None, *, entropy: bool = False, top: int = 
            [0, 1]], dtype=int32)
     """
     alternatives = []
+    if tokens is not None and not isinstance(tokens, TokenIds):
+        tokens = TokenIds(tokens)
     if tokens is not None or entropy or not top:
         out = Tensor._op(LogProbabilities, logits, op_kwargs=dict(tokens=tokens, entropy=entropy, top=top, alternatives=alternatives), constant=constant)
         if not top:
             return out
     else:  # nothing that has a gradient
         z = _device.value_of(logits if isinstance(logits, Tensor) else Tensor(logits, constant=True, copy=False))
-        scores, out = _Scores(z, tokens, entropy, top), None
-        if z.size == 0:
-            alternatives += np.empty((*scores.lead, top), dtype=scores.dtype), np.empty((*scores.lead, top), dtype=np.int32)
-        else:
-            alternatives += scores.run(z, False)[2]
+        plan, out = _plan(z, None, entropy, top), None
+        alternatives += plan.no_alternatives() if plan.empty else plan.run(z, None, False)[2]
     likeliest, which = alternatives
     which = TokenIds._on_device(which, np.shape(logits)[-1]) if isinstance(which, _device.DeviceArray) else TokenIds(which)
     return out, Tensor(likeliest, constant=True, copy=False), which
