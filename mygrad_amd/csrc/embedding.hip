@@ -70,12 +70,6 @@ __global__ void __launch_bounds__(256) embedding_kernel(Embedding p, int lanes, 
 constexpr int kSorters = 16;
 constexpr int kMostBits = 10;
 
-// What the lanes of a wavefront wrote to LDS is there for all of them.
-__device__ __forceinline__ void wave_sees() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 struct Digit {
   int shift, bits;
   __device__ __forceinline__ int of(unsigned key) const { return (int)(key >> shift) & ((1 << bits) - 1); }

@@ -34,8 +34,12 @@ struct Piece {
 
 // What another lane of a row of sixteen has, by a move within the vector unit.
 template <int CONTROL>
+__device__ __forceinline__ int from_lane(int v) {
+  return __builtin_amdgcn_mov_dpp(v, CONTROL, 0xf, 0xf, true);
+}
+template <int CONTROL>
 __device__ __forceinline__ float from_lane(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CONTROL, 0xf, 0xf, true));
+  return __builtin_bit_cast(float, from_lane<CONTROL>(__builtin_bit_cast(int, v)));
 }
 template <int CONTROL>
 __device__ __forceinline__ double from_lane(double v) {
@@ -56,6 +60,12 @@ __device__ __forceinline__ C lanes_add(C v, int lanes) {
   if (lanes > 32) v += __shfl_xor(v, 32);
   return v;
 }
+// What the lanes of a wavefront wrote is there for all of them.
+__device__ __forceinline__ void wave_sees() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 template <typename C>
 __device__ __forceinline__ C wave_add(C v) {
   return lanes_add(v, 64);

@@ -269,7 +269,8 @@ struct Scores {
   }
 };
 
-// Or of those and a teacher's logits: a thread (or each lane of a wavefront, in turns) takes one of them; q goes to memory for the backward pass.
+// Or of those and a teacher's logits: a thread (or each lane of a wavefront, in turns) takes one of them.  q goes to memory for the backward
+// pass: that of all entries of a token where it stands first, and -1 for those that have nothing to add.
 template <typename T, typename Y, typename C>
 struct Distillation {
   const int32_t *ids;
@@ -306,12 +307,42 @@ struct Distillation {
     C sum = 0;
 #pragma unroll
     for (int n = 0; n < TURNS; ++n) {
-      const int k = lane + n * LANES;
-      const C q = total == 0 ? C(0) : f[n] / total;
-      sum += q == 0 ? C(0) : q * ((y[n] - log(total)) - log_probability<C>(row, z[n], per));
-      if (k < p.top && shares) shares[r * p.top + k] = q;
+      f[n] = total == 0 ? C(0) : f[n] / total;
+      sum += f[n] == 0 ? C(0) : f[n] * ((y[n] - log(total)) - log_probability<C>(row, z[n], per));
     }
     sum = group_add<LANES>(sum, space);
+    if (shares) {
+      __shared__ __attribute__((aligned(16))) int tokens[256 / LANES][kMostTaught];
+      __shared__ C q[256 / LANES][kMostTaught];
+      const int group = LANES == 64 ? threadIdx.x >> 6 : 0;
+#pragma unroll
+      for (int n = 0; n < TURNS; ++n) tokens[group][lane + n * LANES] = id[n] < p.V ? id[n] : -1, q[group][lane + n * LANES] = f[n];
+      if (LANES == 64) wave_sees();
+      else __syncthreads();
+#pragma unroll
+      for (int n = 0; n < TURNS; ++n) {
+        const int k = lane + n * LANES;
+        if (k >= p.top) break;
+        const int own = id[n] < p.V ? id[n] : -1;
+        int alike = 0;  // seldom more than one
+#pragma unroll 4
+        for (int j = 0; j < p.top; j += 4) {
+          typedef int Quad __attribute__((ext_vector_type(4)));
+          const Quad four = *reinterpret_cast<const Quad *>(&tokens[group][j]);
+          alike += (four[0] == own) + (four[1] == own) + (four[2] == own) + (four[3] == own);
+        }
+        C all = f[n];
+        bool adds = own >= 0;
+        if (adds && alike > 1) {
+          all = 0;
+          for (int j = 0; j < p.top; ++j)
+            if (tokens[group][j] == own) all += q[group][j], adds = adds && j >= k;
+        }
+        shares[r * p.top + k] = adds ? all : C(-1);
+      }
+      if (LANES == 64) wave_sees();
+      else __syncthreads();
+    }
     if (lane) return;
     loss[r] = sum;
     row.a = total == 0 ? C(0) : total / total;  // 1, or NaN
@@ -486,7 +517,9 @@ int over_rows(const Vocabulary &p, const void *logits, const End &end, void *top
 }
 
 // ---- gradients --------------------------------------------------------------------------------------------------------------------
-// As many pieces of a row as a block has on their way together, or a wavefront per row.
+// As many pieces of a row as a block has on their way together, or a wavefront per row.  The rows come in the order opposite to the forward
+// pass's: it has read the last of them last, and some of those are still near (4096 x 50000 halves, both passes 244 us and 246; distillation
+// over 32000 181 and 185).
 template <typename T, typename C, int LANES, bool ENTROPY>
 __global__ void __launch_bounds__(256) scores_bwd_kernel(Vocabulary p, int parts, const int32_t *__restrict__ ids, const T *__restrict__ logits,
                                                          const Row<C> *__restrict__ kept, const C *__restrict__ grad_scores,
@@ -496,9 +529,10 @@ __global__ void __launch_bounds__(256) scores_bwd_kernel(Vocabulary p, int parts
   const int lane = threadIdx.x & (LANES - 1);
   const long long units = LANES == 64 ? (p.rows + 3) / 4 : p.rows * parts;
   for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const long long r = LANES == 64 ? unit * 4 + (threadIdx.x >> 6) : unit / parts;
-    if (LANES == 64 && r >= p.rows) return;
-    const long long at = (LANES == 64 ? 0 : (unit - r * parts) * kStep) + lane * V;
+    const long long r0 = LANES == 64 ? unit * 4 + (threadIdx.x >> 6) : unit / parts;
+    if (LANES == 64 && r0 >= p.rows) return;
+    const long long r = p.rows - 1 - r0;
+    const long long at = (LANES == 64 ? 0 : (unit - r0 * parts) * kStep) + lane * V;
     const T *z = logits + r * p.V;
     T *out = dlogits + r * p.V;
     Held held[kAtOnce];
@@ -533,47 +567,45 @@ __global__ void __launch_bounds__(256) scores_bwd_kernel(Vocabulary p, int parts
   }
 }
 
-template <typename T, typename C>
+// Wavefronts write the teacher's tokens among their own values once more; nobody waits for another.
+template <typename T, typename C, int LANES>
 __global__ void __launch_bounds__(256) distillation_bwd_kernel(Vocabulary p, int parts, const int32_t *__restrict__ ids, const T *__restrict__ logits,
                                                                const Row<C> *__restrict__ kept, const C *__restrict__ shares,
                                                                const C *__restrict__ grad, T *__restrict__ dlogits) {
   typedef typename Piece<T>::Held Held;
-  constexpr int V = Piece<T>::V, kStep = 256 * V * kAtOnce;
-  __shared__ int taught[kMostTaught];
-  __shared__ C share_of[kMostTaught];
-  const int k = threadIdx.x;
-  for (long long unit = blockIdx.x; unit < p.rows * parts; unit += gridDim.x) {
-    const long long r = unit / parts, from = (unit - r * parts) * kStep, at = from + k * V;
+  constexpr int V = Piece<T>::V, kStep = LANES * V * kAtOnce;
+  const int lane = threadIdx.x & (LANES - 1);
+  const long long units = LANES == 64 ? (p.rows + 3) / 4 : p.rows * parts;
+  for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const long long nth = LANES == 64 ? unit * 4 + (threadIdx.x >> 6) : unit / parts;
+    if (LANES == 64 && nth >= p.rows) return;
+    const long long r = p.rows - 1 - nth, from = LANES == 64 ? 0 : (unit - nth * parts) * kStep, at = from + lane * V;
     const T *z = logits + r * p.V;
     T *out = dlogits + r * p.V;
     Held held[kAtOnce];
-    load_pieces<256>(held, z, at, p.V);
+    load_pieces<LANES>(held, z, at, p.V);
     const Row<C> row = kept[r];
-    __syncthreads();
-    if (k < p.top) taught[k] = ids[r * p.top + k], share_of[k] = shares[r * p.top + k];
-    __syncthreads();
     const C per = (C)p.per, g = grad[r] * per, inverse = row.a / row.s;
     const bool nothing = row.s == 0 || row.a == 0;
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
-      const long long d = at + (long long)u * 256 * V;
+      const long long d = at + (long long)u * LANES * V;
       if (d >= p.V) break;
       Held dz;
 #pragma unroll
       for (int n = 0; n < V; ++n) dz[n] = nothing ? T(0) : (T)(g * (exponential<T>(((C)held[u][n] - row.m) * per) * inverse));
       Piece<T>::store(out + d, p.V - d, dz);
     }
-    __syncthreads();  // the teacher's tokens are written once more, each by the first thread that has it
-    const int id = k < p.top ? taught[k] : -1;
-    if (id < 0 || id >= p.V || id < from || id >= from + kStep || nothing) continue;
-    C q = 0;
-    bool first = true;
-    for (int n = 0; n < p.top; ++n)
-      if (taught[n] == id) {
-        first = first && n >= k;
-        q += share_of[n];
-      }
-    if (first) out[id] = (T)(g * (exponential<T>(((C)z[id] - row.m) * per) * inverse - q));
+    if (nothing) continue;
+    wave_sees();  // the same memory again, by other lanes
+    for (int k = threadIdx.x & 63; k < p.top; k += 64) {
+      const int id = ids[r * p.top + k];
+      const C q = shares[r * p.top + k];
+      const long long place = id - from;
+      if (q < 0 || place < 0 || place >= kStep) continue;
+      if (LANES == 64 || (int)(place % (LANES * V)) / (64 * V) == (int)(threadIdx.x >> 6))
+        out[id] = (T)(g * (exponential<T>(((C)z[id] - row.m) * per) * inverse - q));
+    }
   }
 }
 
@@ -691,9 +723,13 @@ int mg_distillation_bwd(int dtype, int64_t rows, int64_t V, int64_t K, double te
     typedef std::remove_pointer_t<decltype(t)> T;
     typedef std::remove_pointer_t<decltype(c)> C;
     ScopedTiming timed(TAG_DISTILLATION_BWD);
-    const long long parts = ceil_div(V, 256 * Piece<T>::V * kAtOnce);
-    distillation_bwd_kernel<T, C><<<dim3((unsigned)std::min<long long>(rows * parts, 1 << 22)), dim3(256), 0, runtime().stream>>>(
-        p, (int)parts, ids, (const T *)logits, (const Row<C> *)kept, (const C *)shares, (const C *)grad, (T *)dlogits);
+    auto run = [&](auto lanes) {
+      const long long parts = ceil_div(V, lanes * Piece<T>::V * kAtOnce), blocks = lanes == 64 ? ceil_div(rows, 4) : rows * parts;
+      distillation_bwd_kernel<T, C, lanes><<<dim3((unsigned)std::min<long long>(blocks, 1 << 22)), dim3(256), 0, runtime().stream>>>(
+          p, (int)parts, ids, (const T *)logits, (const Row<C> *)kept, (const C *)shares, (const C *)grad, (T *)dlogits);
+    };
+    if (V <= 64 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 64>{});
+    else run(std::integral_constant<int, 256>{});
     MG_HIP(hipGetLastError());
     return (int)MG_OK;
   });
