@@ -18,73 +18,75 @@ _described = {}  # what was checked of calls of the same shapes
 
 
 class LayerNorm(Operation):
-    """``x:(..., dim)`` with ``weight:(dim,)`` and ``bias:(dim,)``; empty ones stand for none."""
+    """``x:(..., dim)``, and ``weight:(dim,)`` and ``bias:(dim,)`` where there are any: ``given`` names them."""
 
     takes_device_arrays = True
 
-    def __call__(self, x, weight, bias, *, eps):
-        self.variables = (x, weight, bias)
-        xd, wd, bd = values = [_device.value_of(t) for t in self.variables]
-        key = xd.shape, xd.dtype, wd.shape, wd.dtype, bd.shape, bd.dtype, eps
+    def __call__(self, x, *params, eps, given):
+        self.variables = (x, *params)
+        values = [_device.value_of(t) for t in self.variables]
+        xd = values[0]
+        key = tuple([(v.shape, v.dtype) for v in values]), given, eps
         found = _described.get(key)
         if found is None:
-            found = self._describe(values, eps)
+            found = self._describe(values, given, eps)
             if len(_described) >= _MOST_SHAPES:
                 _described.clear()
             _described[key] = found
-        self._call, self._there, item = found
+        self._call, self._places, item = found
         self._empty = self._call[1] * self._call[2] == 0
         self._backed = None
         if self._empty:
             return np.empty(xd.shape, dtype=xd.dtype)
         self._kept = None
-        if not (x.constant and weight.constant and bias.constant):  # two parts of the mean and 1 / sqrt for each row
+        if not all([t.constant for t in self.variables]):  # two parts of the mean and 1 / sqrt for each row
             self._kept = _device.DeviceBuffer(3 * self._call[1] * item)
-        xb, wb, bb = (_device.to_device(v) if there else None for v, there in zip(values, self._there))
+        held = [_device.to_device(v) for v in values]  # until the launch
         out = _device.DeviceBuffer(xd.nbytes)
-        _hip.check(_hip.lib().mg_layer_norm_fwd(*self._call, eps, xb.ptr, None if wb is None else wb.ptr, None if bb is None else bb.ptr, out.ptr,
-                                                None if self._kept is None else self._kept.ptr))
+        xp, wp, bp = (None if n is None else held[n].ptr for n in self._places)
+        _hip.check(_hip.lib().mg_layer_norm_fwd(*self._call, eps, xp, wp, bp, out.ptr, None if self._kept is None else self._kept.ptr))
         y = _device.download(out, xd.shape, xd.dtype)
         _device.attach(y, out)
         return y
 
     @staticmethod
-    def _describe(values, eps):
-        """The checked arguments of the entry points, which of the operands there are, and the size of a statistic."""
+    def _describe(values, given, eps):
+        """The checked arguments of the entry points, where x, weight and bias are among the variables, and the size of a statistic."""
         x = values[0]
         if x.ndim < 1:
             raise ValueError(f"`x` must have the axes (..., dim), got shape {x.shape}")
         if x.dtype not in _DTYPES:
             raise TypeError(f"layer_norm runs on the GPU in float16, float32 or float64, got {x.dtype} (there is no CPU fallback)")
         dim = x.shape[-1]
-        there = True, values[1].size > 0, values[2].size > 0
-        for name, value, given in zip(("weight", "bias"), values[1:], there[1:]):
-            if given and value.shape != (dim,):
+        for name, value in zip(given, values[1:]):
+            if value.shape != (dim,):
                 raise ValueError(f"`{name}` must have shape ({dim},), got {value.shape}")
-            if given and value.dtype != x.dtype:
+            if value.dtype != x.dtype:
                 raise TypeError(f"layer_norm takes `{name}` in the dtype of `x` ({x.dtype}), got {value.dtype}")
         if not 0 <= eps < np.inf:
             raise ValueError(f"`eps` must be a non-negative number, got {eps}")
-        return (_hip.storage_code(x.dtype), prod(x.shape[:-1]), dim), there, 8 if x.dtype == np.float64 else 4
+        places = 0, *(1 + given.index(name) if name in given else None for name in ("weight", "bias"))
+        return (_hip.storage_code(x.dtype), prod(x.shape[:-1]), dim), places, 8 if x.dtype == np.float64 else 4
 
     def _run_backward(self, grad, want):
-        x, w, b = values = [_device.value_of(t) for t in self.variables]
+        values = [_device.value_of(t) for t in self.variables]
+        x = values[0]
         if grad.shape != x.shape:
             raise NotImplementedError(f"layer_norm backward for gradient of shape {grad.shape} (no CPU fallback)")
         xb, gb = _device.to_device(x), _device.to_device(grad, x.dtype)
-        wb = _device.to_device(w) if self._there[1] else None
-        out = [_device.DeviceBuffer(v.nbytes) if i in want else None for i, v in enumerate(values)]
+        wb = None if self._places[1] is None else _device.to_device(values[self._places[1]])
+        out = {i: _device.DeviceBuffer(values[i].nbytes) for i in want}
         _hip.check(_hip.lib().mg_layer_norm_bwd(*self._call, xb.ptr, None if wb is None else wb.ptr, self._kept.ptr, gb.ptr,
-                                                *(None if buf is None else buf.ptr for buf in out)))
-        return {i: _device.download(out[i], values[i].shape, x.dtype) for i in want}
+                                                *(out[i].ptr if i in out else None for i in self._places)))
+        return {i: _device.download(buf, values[i].shape, x.dtype) for i, buf in out.items()}
 
     def backward_var(self, grad, index, **kwargs):
-        if self._empty or not self._there[index]:
+        if self._empty:
             value = _device.value_of(self.variables[index])
             return np.zeros(value.shape, dtype=value.dtype)
         # backward() asks for each variable in turn with the same `grad`: the first request computes all that are wanted
         if self._backed is None or self._backed[0] is not grad or index not in self._backed[1]:
-            want = {index} | {i for i, var in enumerate(self.variables) if not var.constant and self._there[i]}
+            want = {index} | {i for i, var in enumerate(self.variables) if not var.constant}
             self._backed = (grad, self._run_backward(grad, want))
         out = self._backed[1].pop(index)
         if not self._backed[1]:
@@ -109,8 +111,5 @@ def layer_norm(x, weight=None, bias=None, *, eps: float, constant: Optional[bool
     """
     if eps is None:
         raise TypeError("`eps` must be a non-negative number")
-    for name, value in (("weight", weight), ("bias", bias)):  # to the operation an empty one is none
-        if value is not None and 0 in np.shape(value) and np.shape(value) != np.shape(x)[-1:]:
-            raise ValueError(f"`{name}` of shape {np.shape(value)} for rows of shape {np.shape(x)[-1:]}")
-    none = np.array([])
-    return Tensor._op(LayerNorm, x, none if weight is None else weight, none if bias is None else bias, op_kwargs=dict(eps=eps), constant=constant)
+    given = [(name, value) for name, value in (("weight", weight), ("bias", bias)) if value is not None]
+    return Tensor._op(LayerNorm, x, *[value for _, value in given], op_kwargs=dict(eps=eps, given=tuple([name for name, _ in given])), constant=constant)

@@ -124,6 +124,8 @@ class Tensor:
             # graph, which is also what keeps the device buffer a valid copy of it
             _device.attach(arr, dev.buf)
             for op in holders:
+                if not op._guarded:
+                    finalize(op, _graph.release, op._guarded)
                 op._guarded.append(_graph.lock(arr))
             _device.drop_pending()
         return arr
@@ -277,7 +279,8 @@ class Tensor:
                     if len(t._guards) >= 32:
                         t._guards = [ref for ref in t._guards if ref() is not None]
                     t._guards.append(ref_f)
-            finalize(f, _graph.release, guarded)
+            if guarded:  # else nothing is to be released yet: what is read later sees to it (a finalizer costs 3 us)
+                finalize(f, _graph.release, guarded)
         _device.drop_pending()
         return out
 

@@ -180,3 +180,28 @@ assert weight.grad.shape == (4, 8)
 print("dropped")
 """
     assert "dropped" in run_on_standins(tmp_path, program)
+
+
+def test_arrays_read_from_a_live_graph_are_released_with_it(tmp_path):
+    """Where all operands lie on the device, nothing is held until somebody reads them; then until the operation is gone."""
+    program = """
+import numpy as np
+import mygrad_amd as mg
+from mygrad_amd import _graph
+from mygrad_amd.nnet import layer_norm
+x, w = mg.device_tensor(np.ones((2, 8), np.float32)), mg.device_tensor(np.ones(8, np.float32))
+y = layer_norm(x, w, eps=1e-5)
+z = layer_norm(y, eps=1e-5)
+assert _graph.held_count() == 0
+arrays = [t.data for t in (x, y, w, z)]
+assert _graph.held_count() == len(arrays) and not any(a.flags.writeable for a in arrays)
+z.backward(mg.device_tensor(np.ones((2, 8), np.float32), constant=True))
+assert _graph.held_count() == 0 and all(a.flags.writeable for a in arrays)
+y = layer_norm(mg.device_tensor(np.ones((2, 8), np.float32)), eps=1e-5)
+held = y.data
+assert not held.flags.writeable
+del y
+assert held.flags.writeable and _graph.held_count() == 0
+print("released")
+"""
+    assert "released" in run_on_standins(tmp_path, program)
