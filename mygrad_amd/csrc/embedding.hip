@@ -101,12 +101,13 @@ __device__ __forceinline__ void count_digits(Digit digit, const unsigned (&key)[
 // counts[w][d] becomes the number of tokens with digit d in wavefronts before w; the number in all is returned to thread d.
 __device__ __forceinline__ int over_wavefronts(int bins, unsigned short *counts) {
   int total = 0;
-  if ((int)threadIdx.x < bins)
-    for (int w = 0; w < kSorters; ++w) {
-      const int here = counts[w * bins + threadIdx.x];
-      counts[w * bins + threadIdx.x] = (unsigned short)total;
-      total += here;
-    }
+  if ((int)threadIdx.x < bins) {
+    int here[kSorters];
+#pragma unroll
+    for (int w = 0; w < kSorters; ++w) here[w] = counts[w * bins + threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < kSorters; ++w) counts[w * bins + threadIdx.x] = (unsigned short)total, total += here[w];
+  }
   return total;
 }
 
@@ -203,12 +204,13 @@ __global__ void __launch_bounds__(1024) order_kernel(Owners p) {
     }
     __syncthreads();
     int total = 0;
-    if (t < own)
-      for (int w = 0; w < kSorters; ++w) {
-        const int here = counts[w * own + t];
-        counts[w * own + t] = total;
-        total += here;
-      }
+    if (t < own) {
+      int here[kSorters];
+#pragma unroll
+      for (int w = 0; w < kSorters; ++w) here[w] = counts[w * own + t];
+#pragma unroll
+      for (int w = 0; w < kSorters; ++w) counts[w * own + t] = total, total += here[w];
+    }
     if (tile == 0) {
       if (p.tokens <= kOwnTile) all = total;
       block_add(less, space);

@@ -116,8 +116,9 @@ __device__ __forceinline__ void move_to(Sums<C> &a, C m, C per) {
   a.m = m;
 }
 
+// Returns the largest of the pieces' values, NaN passed over.
 template <typename T, bool MEAN, typename C>
-__device__ __forceinline__ void add_pieces(Sums<C> &a, const typename Piece<T>::Held (&z)[kAtOnce], C per) {
+__device__ __forceinline__ C add_pieces(Sums<C> &a, const typename Piece<T>::Held (&z)[kAtOnce], C per) {
   constexpr int V = Piece<T>::V;
   T most = z[0][0];  // a NaN is passed over: the sum shows it
 #pragma unroll
@@ -137,6 +138,7 @@ __device__ __forceinline__ void add_pieces(Sums<C> &a, const typename Piece<T>::
     }
   a.s += (s[0] + s[1]) + (s[2] + s[3]);
   if (MEAN) a.w += (w[0] + w[1]) + (w[2] + w[3]);
+  return (C)most;
 }
 
 // Of all threads' sums.
@@ -165,9 +167,10 @@ __device__ __forceinline__ void load_pieces(typename Piece<T>::Held (&z)[kAtOnce
 }
 
 // ---- the likeliest tokens ---------------------------------------------------------------------------------------------------------
-// The threads' own maxima bound the k-th largest logit from below: k of them are as large as the k-th of them.  What is not below that bound is
-// collected in LDS, which is little more than k, and ranked there by comparing all with all.  Ties can make it more: when the list is full, all
-// but the first k are dropped, and the last of those is the new bound.
+// The threads' own maxima in a block's first step bound the k-th largest logit from below: k of them are as large as the k-th of them.  What is
+// not below that bound is collected in LDS as the pass over the row goes on (k for each step, about) and ranked there at its end by comparing
+// all with all.  Where that is more than there is room for (ties, mostly), or logits are NaN, a second pass begins with the bound by all values and
+// drops all but the first k when the list is full; the last of those is the new bound.
 template <typename C>
 struct Candidate {
   typedef decltype(order_of(C(0))) Order;
@@ -206,7 +209,17 @@ struct Likeliest {
   }
   __device__ __forceinline__ void add(const Found &f) {
     const int n = atomicAdd(&count, 1);
-    values[n] = f.value, places[n] = f.place;
+    if (n < kRoom) values[n] = f.value, places[n] = f.place;
+  }
+  __device__ __forceinline__ void add_pieces(const typename Piece<T>::Held (&z)[kAtOnce], long long d, long long end) {
+    const Order least_of_all = bound.value;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+      for (int n = 0; n < Piece<T>::V; ++n) {
+        const Found f{order_of((C)z[u][n]), (int)(d + u * kStep + n)};
+        if (f.value >= least_of_all && d + u * kStep + n < end) add(f);
+      }
   }
   // The first k of the list, in order, in `first`; returns how many there are.  All threads call.
   __device__ __forceinline__ int rank(int k) {
@@ -378,25 +391,38 @@ __global__ void __launch_bounds__(256) row_kernel(Vocabulary p, Top w, const T *
     const C per = (C)p.per;
     Sums<C> sums{-infinity<C>(), 0, 0};
     typename Piece<T>::Held z[kAtOnce];
-    for (long long d = from + lane * V; d < to; d += kStep) {
-      load_pieces<LANES>(z, row, d, to);
-      add_pieces<T, MEAN>(sums, z, per);
+    if constexpr (TOP) {
+      __syncthreads();  // the list of the unit before has been read
+      for (long long d0 = from; d0 < to; d0 += kStep) {
+        const long long d = d0 + lane * V;
+        load_pieces<LANES>(z, row, d, to);
+        const C most = add_pieces<T, MEAN>(sums, z, per);
+        if (d0 == from) list.begin(d < to ? order_of(most) : Order(0), p.top);
+        if (order_of(most) >= list.bound.value) list.add_pieces(z, d, to);
+      }
+    } else {
+      for (long long d = from + lane * V; d < to; d += kStep) {
+        load_pieces<LANES>(z, row, d, to);
+        add_pieces<T, MEAN>(sums, z, per);
+      }
     }
-    const bool any = from + lane * V < to;
     const C own = sums.m;
     sums = join<LANES, T, MEAN>(sums, per, space);
     if (LANES == 64 || w.parts == 1) end.template end<LANES>(p, r, lane, sums, space);
     else if (lane == 0) ((Sums<C> *)w.partial)[unit] = sums;
     if constexpr (TOP) {
       __syncthreads();
-      list.begin(any ? order_of(own) : Order(0), p.top);
-      const bool held = to - from <= kStep;
-      for (long long d0 = from; d0 < to; d0 += kStep) {
-        const long long d = d0 + lane * V;
-        if (!held) load_pieces<LANES>(z, row, d, to);
+      const bool again = list.count > Likeliest<T, C>::kRoom || sums.s != sums.s;
+      if (again) {
+        __syncthreads();
+        list.begin(from + lane * V < to ? order_of(own) : Order(0), p.top);
+        for (long long d0 = from; d0 < to; d0 += kStep) {
+          const long long d = d0 + lane * V;
+          load_pieces<LANES>(z, row, d, to);
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u)
-          if (d0 + u * LANES * V < to) collect<T, C>(list, z[u], d + u * LANES * V, to, p.top);
+          for (int u = 0; u < kAtOnce; ++u)
+            if (d0 + u * LANES * V < to) collect<T, C>(list, z[u], d + u * LANES * V, to, p.top);
+        }
       }
       const int found = list.rank(p.top);
       if ((int)threadIdx.x < p.top) {
