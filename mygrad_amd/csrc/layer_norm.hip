@@ -120,8 +120,8 @@ __global__ void __launch_bounds__(1024) layer_norm_join_kernel(long long D, int 
 }
 
 // ---- rows in registers ------------------------------------------------------------------------------------------------------------
-// A row's pieces go to `lanes` threads, N for each: a part of a wavefront or one (WAVES = 1, 256 / lanes rows at once), or a whole block of
-// 4 or 16 wavefronts.
+// A row's pieces go to a part of a wavefront or one (WAVES = 1: `lanes` threads, 256 / lanes rows at once), or to a whole block of 2, 4 or 16
+// wavefronts, N pieces for each thread.
 template <int WAVES>
 constexpr int kThreads = WAVES == 1 ? 256 : WAVES * 64;
 
@@ -204,6 +204,8 @@ __global__ void __launch_bounds__(kThreads<WAVES>) layer_norm_rows_kernel(LayerN
   }
 }
 
+// With one or two pieces the next row is on its way during a row's sums, which registers for four do not allow: 2^27 bytes of x, us with and
+// without, 2048 pieces of float16 157 and 95, 512 pieces 85 and 91.
 template <typename T, typename C, int WAVES, int N>
 __global__ void __launch_bounds__(kThreads<WAVES>) layer_norm_rows_bwd_kernel(LayerNorm p, int lanes, const T *__restrict__ x, const T *__restrict__ w,
                                                                               const T *__restrict__ grad, const Moments<C> *__restrict__ kept,
@@ -214,10 +216,13 @@ __global__ void __launch_bounds__(kThreads<WAVES>) layer_norm_rows_bwd_kernel(La
   RowSums<WAVES, C> rows{space};
   const int lane = WAVES == 1 ? threadIdx.x & (lanes - 1) : threadIdx.x, groups = WAVES == 1 ? 256 / lanes : 1;
   const int group = WAVES == 1 ? threadIdx.x / lanes : 0, step = (WAVES == 1 ? lanes : kThreads<WAVES>) * V, d0 = lane * V;
+  constexpr bool AHEAD = N == 1 || (N == 2 && WAVES < 16), HELD = WAVES < 16 || N < 4;  // the next row is loaded early; the weight stays in registers
   Held weight[N];
+  auto load_weight = [&] {
 #pragma unroll
-  for (int u = 0; u < N; ++u)
-    if (w) weight[u] = Piece<T>::load(w + d0 + u * step, p.D - d0 - u * step, T(0));
+    for (int u = 0; u < N; ++u) weight[u] = w ? Piece<T>::load(w + d0 + u * step, p.D - d0 - u * step, T(0)) : Held{};
+  };
+  if (HELD) load_weight();
   C dw[N][V] = {}, db[N][V] = {};
   Held xs[N], gs[N];
   auto load = [&](long long row) {
@@ -229,33 +234,62 @@ __global__ void __launch_bounds__(kThreads<WAVES>) layer_norm_rows_bwd_kernel(La
     }
   };
   const long long stride = (long long)gridDim.x * groups;
-  load((long long)blockIdx.x * groups + group);
+  if (AHEAD) load((long long)blockIdx.x * groups + group);
   for (long long row0 = (long long)blockIdx.x * groups; row0 < p.rows; row0 += stride) {
     const long long row = row0 + group;
     const bool here = row < p.rows;
     const Moments<C> m = here ? kept[row] : Moments<C>{0, 0, 0};
-    C v[N][V], u_of[N][V], first = 0, second = 0;
+    C first = 0, second = 0;
+    if constexpr (AHEAD) {
+      C v[N][V], u_of[N][V];
 #pragma unroll
-    for (int u = 0; u < N; ++u)
+      for (int u = 0; u < N; ++u)
 #pragma unroll
-      for (int n = 0; n < V; ++n) {
-        const C g = (C)gs[u][n], t = ((C)xs[u][n] - m.shift - m.mean) * m.r;  // behind the row's end g is 0
-        v[u][n] = t;
-        u_of[u][n] = w ? g * (C)weight[u][n] : g;
-        first += u_of[u][n], second += u_of[u][n] * t;
-        dw[u][n] += g * t, db[u][n] += g;
+        for (int n = 0; n < V; ++n) {
+          const C g = (C)gs[u][n], t = ((C)xs[u][n] - m.shift - m.mean) * m.r;  // behind the row's end g is 0
+          v[u][n] = t;
+          u_of[u][n] = w ? g * (C)weight[u][n] : g;
+          first += u_of[u][n], second += u_of[u][n] * t;
+          dw[u][n] += g * t, db[u][n] += g;
+        }
+      load(row + stride);  // the next row is on its way during the sums
+      if (dx) {
+        rows.add(first, second, lanes);
+        first /= (C)p.D, second /= (C)p.D;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          Held out;
+#pragma unroll
+          for (int n = 0; n < V; ++n) out[n] = (T)(m.r * (u_of[u][n] - first - v[u][n] * second));
+          const int d = d0 + u * step;
+          if (here) Piece<T>::store(dx + row * p.D + d, p.D - d, out);
+        }
       }
-    load(row + stride);  // the next row is on its way during the sums
-    if (dx) {
-      rows.add(first, second, lanes);
-      first /= (C)p.D, second /= (C)p.D;
+    } else {
+      load(row);
+      if constexpr (!HELD) load_weight();
 #pragma unroll
-      for (int u = 0; u < N; ++u) {
-        Held out;
+      for (int u = 0; u < N; ++u)
 #pragma unroll
-        for (int n = 0; n < V; ++n) out[n] = (T)(m.r * (u_of[u][n] - first - v[u][n] * second));
-        const int d = d0 + u * step;
-        if (here) Piece<T>::store(dx + row * p.D + d, p.D - d, out);
+        for (int n = 0; n < V; ++n) {
+          const C g = (C)gs[u][n], t = ((C)xs[u][n] - m.shift - m.mean) * m.r, uw = w ? g * (C)weight[u][n] : g;
+          first += uw, second += uw * t;
+          dw[u][n] += g * t, db[u][n] += g;
+        }
+      if (dx) {
+        rows.add(first, second, lanes);
+        first /= (C)p.D, second /= (C)p.D;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          Held out;
+#pragma unroll
+          for (int n = 0; n < V; ++n) {
+            const C g = (C)gs[u][n], t = ((C)xs[u][n] - m.shift - m.mean) * m.r;
+            out[n] = (T)(m.r * ((w ? g * (C)weight[u][n] : g) - first - t * second));
+          }
+          const int d = d0 + u * step;
+          if (here) Piece<T>::store(dx + row * p.D + d, p.D - d, out);
+        }
       }
     }
   }
@@ -291,8 +325,8 @@ __global__ void __launch_bounds__(kThreads<WAVES>) layer_norm_rows_bwd_kernel(La
   }
 }
 
-// Threads and pieces for a row: as few threads as hold it with one piece each up to a wavefront, two pieces in a wavefront, then a block of
-// 256 with up to four, and one of 1024.  Longer rows do not stay in registers.
+// Threads and pieces for a row.  Two wavefronts with a piece each rather than one with two, which in float16 leaves three wavefronts a SIMD
+// (800 values, 2^27 bytes of x: 104 us back, 135).  Longer rows do not stay in registers.
 struct Shape {
   int waves, pieces, lanes;
 };
@@ -303,28 +337,36 @@ Shape shape_of(long long D) {
   if (pieces <= 64) {
     s = Shape{1, 1, 1};
     while (s.lanes < pieces) s.lanes *= 2;
-  } else if (pieces <= 128) {
-    s = Shape{1, 2, 64};
+  } else if (pieces <= 256) {
+    s = Shape{pieces <= 128 ? 2 : 4, 1, 64};
+  } else if (pieces <= 512) {
+    s = Shape{4, 2, 64};
   } else if (pieces <= 1024) {
-    s = Shape{4, pieces <= 256 ? 1 : pieces <= 512 ? 2 : 4, 256};
+    s = sizeof(T) == 2 ? Shape{16, 1, 64} : Shape{4, 4, 64};  // 85 us and 95 back in float16, 84 and 80 in float32
   } else if (pieces <= 4096) {
-    s = Shape{16, 4, 1024};
+    s = Shape{16, pieces <= 2048 ? 2 : 4, 64};
   }
   return s;
 }
 
 // Calls f with a Shape's numbers of wavefronts and pieces as constants.
-template <typename F>
+template <typename T, typename F>
 void with_shape(const Shape &s, F f) {
   typedef std::integral_constant<int, 1> One;
   typedef std::integral_constant<int, 2> Two;
   typedef std::integral_constant<int, 4> Four;
-  if (s.waves == 1 && s.pieces == 1) f(One{}, One{});
-  if (s.waves == 1 && s.pieces == 2) f(One{}, Two{});
+  typedef std::integral_constant<int, 16> Sixteen;
+  if (s.waves == 1) f(One{}, One{});
+  if (s.waves == 2) f(Two{}, One{});
   if (s.waves == 4 && s.pieces == 1) f(Four{}, One{});
   if (s.waves == 4 && s.pieces == 2) f(Four{}, Two{});
-  if (s.waves == 4 && s.pieces == 4) f(Four{}, Four{});
-  if (s.waves == 16) f(std::integral_constant<int, 16>{}, Four{});
+  if constexpr (sizeof(T) == 2) {
+    if (s.waves == 16 && s.pieces == 1) f(Sixteen{}, One{});
+  } else {
+    if (s.waves == 4 && s.pieces == 4) f(Four{}, Four{});
+  }
+  if (s.waves == 16 && s.pieces == 2) f(Sixteen{}, Two{});
+  if (s.waves == 16 && s.pieces == 4) f(Sixteen{}, Four{});
 }
 
 template <typename T, typename C>
@@ -333,9 +375,10 @@ int forward(const LayerNorm &p, const void *x, const void *w, const void *b, voi
   hipStream_t s = runtime().stream;
   const Shape shape = shape_of<T>(p.D);
   if (shape.waves) {
-    const int cus = runtime().props.multiProcessorCount;
-    const long long blocks = std::min<long long>(ceil_div(p.rows, shape.waves == 1 ? 256 / shape.lanes : 1), (shape.waves == 16 ? 2 : 8) * cus);
-    with_shape(shape, [&](auto waves, auto pieces) {
+    // eight blocks of 256 a compute unit, or as many threads in larger or smaller ones
+    const long long most = (shape.waves == 1 ? 8 : 32 / shape.waves) * runtime().props.multiProcessorCount;
+    const long long blocks = std::min<long long>(ceil_div(p.rows, shape.waves == 1 ? 256 / shape.lanes : 1), most);
+    with_shape<T>(shape, [&](auto waves, auto pieces) {
       layer_norm_rows_kernel<T, C, waves, pieces><<<dim3((unsigned)blocks), dim3(kThreads<waves>), 0, s>>>(p, shape.lanes, (const T *)x, (const T *)w,
                                                                                                           (const T *)b, (T *)y, (Moments<C> *)kept);
     });
@@ -353,14 +396,16 @@ int backward(const LayerNorm &p, const void *x, const void *w, const void *kept,
   const Shape shape = shape_of<T>(p.D);
   void *space = nullptr;
   if (shape.waves) {
-    // Each block's sums are written once and read once: two blocks a compute unit, more only where one would add up 256 rows or more.
-    const int groups = shape.waves == 1 ? 256 / shape.lanes : 1;
-    const long long most = std::max<long long>((shape.waves == 16 ? 1 : 2) * runtime().props.multiProcessorCount, ceil_div(p.rows, 256ll * groups));
+    // Each block's sums are written once and read once: four blocks of 256 a compute unit (or as many threads) where a thread has one piece, two
+    // where it has more, and more only where one would add up 256 rows or more.  256 pieces, us: four 85, two 96; 512 pieces 94 and 85.
+    const int groups = shape.waves == 1 ? 256 / shape.lanes : 1, wavefronts = shape.pieces == 1 ? 16 : 8;
+    const long long few = std::max(1, wavefronts / (shape.waves == 1 ? 4 : shape.waves)) * runtime().props.multiProcessorCount;
+    const long long most = std::max<long long>(few, ceil_div(p.rows, 256ll * groups));
     const long long blocks = std::min<long long>(ceil_div(p.rows, groups), most);
     if (columns)
       if (const int rc = workspace((size_t)(2 * blocks * p.D) * sizeof(C), &space)) return rc;
     ScopedTiming timed(TAG_LAYER_NORM_BWD);
-    with_shape(shape, [&](auto waves, auto pieces) {
+    with_shape<T>(shape, [&](auto waves, auto pieces) {
       layer_norm_rows_bwd_kernel<T, C, waves, pieces><<<dim3((unsigned)blocks), dim3(kThreads<waves>), 0, s>>>(
           p, shape.lanes, (const T *)x, (const T *)w, (const T *)grad, (const Moments<C> *)kept, (T *)dx, (C *)space);
     });
