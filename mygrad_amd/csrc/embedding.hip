@@ -3,8 +3,8 @@
 //   y[n] = scale W[ids[n]]  (zeros where ids[n] < 0)          dW[v] = scale * sum of grad[n] over the n with ids[n] = v, in their order
 //
 // Both are bound by memory.  The gradient sorts the tokens, so that the rows to be added lie in a run, whatever the text: a run is cut
-// into chunks of a few rows that are summed side by side, what a cut went through is joined in order, and rows that no token names are
-// filled with zeros by the same launch.  Nothing is added by atomics: the same bits every time.
+// into chunks of a few rows that are summed side by side, and what a cut went through is joined in order.  Rows that no token names are zeros, which
+// all rows are filled with first.  Nothing is added by atomics: the same bits every time.
 #include "row_device.h"
 
 #include <algorithm>
@@ -136,19 +136,36 @@ __device__ __forceinline__ unsigned key_of(const int32_t *ids, long long n, long
 // A block owns `own` rows of the table: it looks at all tokens, counts those of rows before its own, which is where its own tokens go, and puts
 // these in order by itself.  One launch, no block waits for another.  Tokens are taken 16384 at a time: threads look at 16 neighbours
 // each, what is the block's own goes into a queue in LDS as it stands, and wavefronts take a run of the queue each.
-// 16384 tokens of 50000 rows: 9 us; one block that sorts them by digits 46.
+// All that waits for loads and for LDS, so the blocks behind them fill the gradient with zeros meanwhile.
+// 16384 tokens of 50000 rows: 9 us (one block that sorts them by digits 46), 31 with 205 MB to fill, 6.6 TB/s.
 constexpr int kLook = 16;
 constexpr int kOwnMost = 1024;
 constexpr int kOwnTile = 1024 * kLook;
 
 struct Owners {
-  int tokens, rows, own;
+  int tokens, rows, own, owners;
   const int32_t *ids;
   unsigned *keys, *order;
-  unsigned long long *present;  // a bit for each row that has tokens
+  char *zeros;  // to be filled
+  unsigned long long bytes;
 };
 
+// Zeros by the part'th of `parts` blocks of 1024.
+__device__ __forceinline__ void fill_zeros(char *to, unsigned long long bytes, unsigned part, unsigned parts) {
+  const unsigned long long before = min((16 - (unsigned long long)to % 16) % 16, bytes), whole = (bytes - before) / 16, after = before + whole * 16;
+  uint4 *const at = reinterpret_cast<uint4 *>(to + before);
+  for (unsigned long long n = (unsigned long long)part * 1024 + threadIdx.x; n < whole; n += parts * 1024ull) at[n] = uint4{0, 0, 0, 0};
+  if (part == 0 && threadIdx.x < before) to[threadIdx.x] = 0;
+  if (part == 0 && threadIdx.x < bytes - after) to[after + threadIdx.x] = 0;
+}
+
+__global__ void __launch_bounds__(1024) fill_kernel(char *to, unsigned long long bytes) { fill_zeros(to, bytes, blockIdx.x, gridDim.x); }
+
 __global__ void __launch_bounds__(1024) order_kernel(Owners p) {
+  if ((int)blockIdx.x >= p.owners) {
+    fill_zeros(p.zeros, p.bytes, blockIdx.x - p.owners, gridDim.x - p.owners);
+    return;
+  }
   extern __shared__ __attribute__((aligned(16))) unsigned lds[];
   __shared__ int space[16], base[kOwnMost];
   unsigned *const queue = lds, *const counts = lds + kOwnTile;  // counts[w][d]: of wavefront w and row d
@@ -239,8 +256,6 @@ __global__ void __launch_bounds__(1024) order_kernel(Owners p) {
     }
     __syncthreads();
   }
-  const unsigned long long some = __ballot(all > 0);
-  if (t < own && lane == 0 && lo + t < p.rows) p.present[(lo + t) >> 6] = some;
   if (hi == p.rows) {  // tokens that are none come last
     __shared__ int end;
     if (t == own - 1) end = places;
@@ -316,19 +331,6 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(Tiles p, const unsigne
   }
 }
 
-// The rows that have tokens, by a search for each.
-__global__ void __launch_bounds__(256) present_kernel(long long tokens, int rows, const unsigned *__restrict__ keys, unsigned long long *__restrict__ present) {
-  const long long row = (long long)blockIdx.x * 256 + threadIdx.x;
-  long long lo = 0, hi = tokens;
-  while (lo < hi) {
-    const long long mid = (lo + hi) >> 1;
-    if ((long long)keys[mid] < row) lo = mid + 1;
-    else hi = mid;
-  }
-  const unsigned long long some = __ballot(lo < tokens && keys[lo] == row);
-  if ((threadIdx.x & 63) == 0 && row < rows) present[row >> 6] = some;
-}
-
 // ---- rows by runs of tokens ---------------------------------------------------------------------------------------------------------
 constexpr int kAtOnce = 16;  // tokens whose rows are on their way together
 
@@ -340,13 +342,12 @@ struct Runs {
   int lanes;          // threads for a row's pieces
   long long chunks;
   int chunk;          // tokens of a chunk
-  int sum_blocks;     // blocks that add (times those along a row); the others fill, 64 rows each
   const unsigned *keys, *order;
-  const unsigned long long *present;
 };
 
-// 16384 tokens of 50000 rows of 2048 halves (67 MB read, 205 written): 55 us, 4.9 TB/s where writes alone reach 6.8 and a copy 5.3; the join 8.  With
-// eight rows on their way, and chunks of 32, 70.  Stores past the caches: 22 us for 98 MB instead of 17.
+// 16384 tokens of 50000 rows of 2048 halves: 35 us (67 MB read and 24 written, while what was filled leaves the caches for memory), and 8 for
+// the join.  With eight rows on their way, and chunks of 32, it was half as much again.  Rows without tokens filled by this launch instead, from a
+// bit for each that the ordering left: 9 + 57 us where the two take 31 + 35, and 8 + 19 where they take 20 + 8 (1999 tokens of 32003 x 771 floats).
 //
 // A group of threads adds the rows of a chunk's tokens.  A run that lies in the chunk becomes a row of the table's gradient; of one that comes in from
 // the chunk before it, the part here goes to parts[2 chunk], and of one that begins here and goes on, to parts[2 chunk + 1].
@@ -354,20 +355,6 @@ template <typename T, typename C>
 __global__ void __launch_bounds__(256) embedding_runs_kernel(Runs p, const T *__restrict__ grad, T *__restrict__ dweight, C *__restrict__ parts) {
   typedef typename Piece<T>::Held Held;
   constexpr int V = Piece<T>::V;
-  if ((int)blockIdx.x >= p.sum_blocks) {
-    if (blockIdx.y) return;
-    const long long first = (long long)(blockIdx.x - p.sum_blocks) * 64;
-    const int count = (int)min(64ll, p.rows - first);
-    const unsigned long long present = p.present[first >> 6];
-    // a group of threads takes every so many of the rows
-    const int lane = threadIdx.x & (p.lanes - 1), groups = 256 / p.lanes;
-    for (int n = threadIdx.x / p.lanes; n < count; n += groups) {
-      if (present >> n & 1) continue;
-      T *to = dweight + (first + n) * p.D;
-      for (long long d = (long long)lane * V; d < p.D; d += (long long)p.lanes * V) Piece<T>::store(to + d, p.D - d, Held{});
-    }
-    return;
-  }
   const int lane = threadIdx.x & (p.lanes - 1), group = threadIdx.x / p.lanes, groups = 256 / p.lanes;
   const long long c = (long long)blockIdx.x * groups + group, d = ((long long)blockIdx.y * p.lanes + lane) * V;
   if (c >= p.chunks || d >= p.D) return;
@@ -490,20 +477,30 @@ int forward(const Embedding &p, const int32_t *ids, const void *weight, void *ou
   return MG_OK;
 }
 
-// The tokens in order, and where each came from, in `keys` and `order`, and the rows that have some: by blocks that own rows, or ...
-int order_by_owners(const Embedding &p, const int32_t *ids, unsigned *keys, unsigned *order, unsigned long long *present) {
+// The tokens in order, and where each came from, in `keys` and `order`, and `zeros` filled: by blocks that own rows, or ...
+int order_by_owners(const Embedding &p, const int32_t *ids, unsigned *keys, unsigned *order, void *zeros, size_t bytes) {
   const int own = std::max<int>(64, (int)ceil_div(ceil_div(p.rows, runtime().props.multiProcessorCount), 64) * 64);
   const int lds = (kOwnTile + kSorters * own) * 4;
   static const hipError_t allowed = hipFuncSetAttribute((const void *)order_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (kOwnTile + kSorters * kOwnMost) * 4);
   MG_HIP(allowed);
-  order_kernel<<<dim3((unsigned)ceil_div(p.rows, own)), dim3(1024), lds, runtime().stream>>>(Owners{(int)p.tokens, p.rows, own, ids, keys, order, present});
+  const int owners = (int)ceil_div(p.rows, own), fillers = (int)std::min<long long>(ceil_div((long long)bytes, 16 * 1024 * 4), 4 * runtime().props.multiProcessorCount);
+  order_kernel<<<dim3((unsigned)(owners + fillers)), dim3(1024), lds, runtime().stream>>>(
+      Owners{(int)p.tokens, p.rows, own, owners, ids, keys, order, (char *)zeros, bytes});
+  MG_HIP(hipGetLastError());
+  return MG_OK;
+}
+
+int fill(void *to, size_t bytes) {
+  const long long blocks = std::min<long long>(ceil_div((long long)bytes, 16 * 1024 * 4), 4 * runtime().props.multiProcessorCount);
+  fill_kernel<<<dim3((unsigned)blocks), dim3(1024), 0, runtime().stream>>>((char *)to, bytes);
   MG_HIP(hipGetLastError());
   return MG_OK;
 }
 
 // ... by digits; `other` has room for keys and order once more, `totals` for the counts.
 int order_by_digits(const Embedding &p, const int32_t *ids, unsigned *keys, unsigned *order, unsigned *other, unsigned *totals, int bits, int passes,
-                    unsigned long long *present) {
+                    void *zeros, size_t bytes) {
+  if (const int rc = fill(zeros, bytes)) return rc;
   const unsigned tiles = (unsigned)ceil_div(p.tokens, kTile);
   unsigned *from[2] = {nullptr, nullptr}, *to[2] = {keys, order}, *spare[2] = {other, other + p.tokens};
   if (passes % 2 == 0) std::swap(to, spare);  // the last digit's go to where they are wanted
@@ -516,19 +513,21 @@ int order_by_digits(const Embedding &p, const int32_t *ids, unsigned *keys, unsi
     from[0] = to[0], from[1] = to[1];
     std::swap(to, spare);
   }
-  present_kernel<<<dim3((unsigned)ceil_div(p.rows, 256)), dim3(256), 0, runtime().stream>>>(p.tokens, p.rows, keys, present);
-  MG_HIP(hipGetLastError());
   return MG_OK;
 }
 
 template <typename T, typename C>
 int backward(const Embedding &p, const int32_t *ids, const void *grad, void *dweight) {
-  if (p.tokens == 0) return mg_memset_zero(dweight, (size_t)p.rows * p.D * sizeof(T));
   int width = 1, passes = 1;
   while (width < 31 && (1ll << width) <= p.rows) ++width;  // digits of 0 to rows
   passes = (int)ceil_div(width, kMostBits);
   const int bits = (int)ceil_div(width, passes);
 
+  const size_t bytes = (size_t)p.rows * p.D * sizeof(T);
+  if (p.tokens == 0) {
+    ScopedTiming timed(TAG_EMBEDDING_BWD);
+    return fill(dweight, bytes);
+  }
   constexpr int V = Piece<T>::V;
   Runs r{};
   r.tokens = p.tokens, r.rows = p.rows, r.D = p.D, r.scale = p.scale;
@@ -538,22 +537,22 @@ int backward(const Embedding &p, const int32_t *ids, const void *grad, void *dwe
   const long long rounds = std::max((p.tokens / kAtOnce * r.lanes) >> 18, p.tokens >> 17);
   r.chunk = kAtOnce * (int)std::min<long long>(std::max<long long>(rounds, 1), 16);
   r.chunks = ceil_div(p.tokens, r.chunk);
-  r.sum_blocks = (int)ceil_div(r.chunks, 256 / r.lanes);
 
   // 50000 rows, us by owners and by digits: 16384 tokens 9 and 39, 65536 38 and 46, 131072 80 and 48.
   const bool owners = p.rows <= kOwnMost * runtime().props.multiProcessorCount && p.tokens <= 1 << 16;
   const long long tiles = owners ? 0 : ceil_div(p.tokens, kTile);
-  const size_t parts = (size_t)(2 * r.chunks * p.D) * sizeof(C), words = (size_t)ceil_div(p.rows, 64) * 8, places = (size_t)p.tokens * 4;
+  const size_t parts = (size_t)(2 * r.chunks * p.D) * sizeof(C), places = (size_t)p.tokens * 4;
   char *space = nullptr;
-  if (const int rc = workspace(ceil_div(parts, 8) * 8 + words + places * (owners ? 2 : 4) + (size_t)(tiles << bits) * 4, (void **)&space)) return rc;
-  unsigned long long *present = (unsigned long long *)(space + ceil_div(parts, 8) * 8);
-  unsigned *keys = (unsigned *)((char *)present + words), *order = keys + p.tokens, *other = order + p.tokens, *totals = other + 2 * p.tokens;
+  if (const int rc = workspace(parts + places * (owners ? 2 : 4) + (size_t)(tiles << bits) * 4, (void **)&space)) return rc;
+  unsigned *keys = (unsigned *)(space + parts), *order = keys + p.tokens, *other = order + p.tokens, *totals = other + 2 * p.tokens;
   hipStream_t s = runtime().stream;
   ScopedTiming timed(TAG_EMBEDDING_BWD);
-  if (const int rc = owners ? order_by_owners(p, ids, keys, order, present) : order_by_digits(p, ids, keys, order, other, totals, bits, passes, present)) return rc;
-  r.keys = keys, r.order = order, r.present = present;
+  if (const int rc = owners ? order_by_owners(p, ids, keys, order, dweight, bytes)
+                              : order_by_digits(p, ids, keys, order, other, totals, bits, passes, dweight, bytes))
+    return rc;
+  r.keys = keys, r.order = order;
   const unsigned along = (unsigned)ceil_div(pieces, r.lanes);
-  embedding_runs_kernel<T, C><<<dim3((unsigned)(r.sum_blocks + ceil_div(p.rows, 64)), along), dim3(256), 0, s>>>(r, (const T *)grad, (T *)dweight, (C *)space);
+  embedding_runs_kernel<T, C><<<dim3((unsigned)ceil_div(r.chunks, 256 / r.lanes), along), dim3(256), 0, s>>>(r, (const T *)grad, (T *)dweight, (C *)space);
   MG_HIP(hipGetLastError());
   if (r.chunks > 1) {
     embedding_join_kernel<T, C><<<dim3((unsigned)(r.chunks - 1), (unsigned)std::min<long long>(ceil_div(p.D, 256), 65535)), dim3(256), 0, s>>>(r, (const C *)space, (T *)dweight);

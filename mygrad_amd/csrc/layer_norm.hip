@@ -383,6 +383,7 @@ int forward(const LayerNorm &p, const void *x, const void *w, const void *b, voi
                                                                                                           (const T *)b, (T *)y, (Moments<C> *)kept);
     });
   } else {
+    if (p.rows >= 1 << 24) return fail(MG_ERR_UNSUPPORTED, "mg_layer_norm_fwd: %lld rows of %lld values", p.rows, p.D);  // a block each
     layer_norm_kernel<T, C><<<dim3((unsigned)p.rows), dim3(256), 0, s>>>(p, (const T *)x, (const T *)w, (const T *)b, (T *)y, (Moments<C> *)kept);
   }
   MG_HIP(hipGetLastError());
@@ -415,6 +416,7 @@ int backward(const LayerNorm &p, const void *x, const void *w, const void *kept,
     MG_HIP(hipGetLastError());
     return MG_OK;
   }
+  if (p.rows >= 1 << 24) return fail(MG_ERR_UNSUPPORTED, "mg_layer_norm_bwd: %lld rows of %lld values", p.rows, p.D);
   const long long share = std::max<long long>(ceil_div(p.rows, 256), 16), shares = ceil_div(p.rows, share);
   if (columns)
     if (const int rc = workspace((size_t)(2 * shares * p.D) * sizeof(double), &space)) return rc;
@@ -436,8 +438,7 @@ int check(int dtype, int64_t rows, int64_t D, double eps, const char *who) {
   if (dtype != MG_F32 && dtype != MG_F64 && dtype != MG_F16) return fail(MG_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
   if (rows < 0 || D <= 0 || !(eps >= 0) || !std::isfinite(eps))
     return fail(MG_ERR_BAD_ARG, "%s: %lld rows of %lld values, eps %g", who, (long long)rows, (long long)D, eps);
-  if (rows >= 1ll << 24 || D > 1 << 24)  // what the grids hold
-    return fail(MG_ERR_UNSUPPORTED, "%s: %lld rows of %lld values", who, (long long)rows, (long long)D);
+  if (rows > 0x7fffffff || D > 1 << 24) return fail(MG_ERR_UNSUPPORTED, "%s: %lld rows of %lld values", who, (long long)rows, (long long)D);
   return MG_OK;
 }
 

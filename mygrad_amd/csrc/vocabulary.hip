@@ -19,8 +19,8 @@ namespace mg {
 
 namespace {
 
-constexpr int kMostTop = 128;      // likeliest tokens that are looked for
-constexpr int kMostTaught = 256;   // a teacher's tokens for a row: a thread each
+constexpr int kMostTop = 128;     // likeliest tokens that are looked for
+constexpr int kMostTaught = 256;  // a teacher's tokens for a row: a thread of a block each
 
 struct Vocabulary {
   long long rows;
@@ -107,7 +107,6 @@ __device__ __forceinline__ C base_of(C m) {
   return m == -infinity<C>() ? C(0) : m;
 }
 
-// As seen from a larger m.
 // t and e^t as the sums take them.  In single precision t is held at -104 and above (a NaN stays one), where the exponential is less than half of
 // the smallest number, so zero.  With n = round(t log2 e), made by adding 1.5 2^23, 2^(t log2 e - n) is the instruction's, to a unit or two, and the
 // result is that times 2^n: nine instructions where the library's function has thirteen.  1021 x 32003 logits with entropies and alternatives take
@@ -133,6 +132,7 @@ __device__ __forceinline__ double term(double &t) {
   return e;
 }
 
+// As seen from a larger m.
 template <typename T, bool MEAN, typename C>
 __device__ __forceinline__ void move_to(Sums<C> &a, C m, C per) {
   const C step = bounded((a.m - base_of(m)) * per), c = exponential<T>(step);

@@ -44,7 +44,7 @@ class LayerNorm(Operation):
         held = [_device.to_device(v) for v in values]  # until the launch
         out = _device.DeviceBuffer(xd.nbytes)
         xp, wp, bp = (None if n is None else held[n].ptr for n in self._places)
-        _hip.check(_hip.lib().mg_layer_norm_fwd(*self._call, eps, xp, wp, bp, out.ptr, None if self._kept is None else self._kept.ptr))
+        _hip.check(_hip.lib().mg_layer_norm_fwd(*self._call, float(eps), xp, wp, bp, out.ptr, None if self._kept is None else self._kept.ptr))
         y = _device.download(out, xd.shape, xd.dtype)
         _device.attach(y, out)
         return y

@@ -196,6 +196,18 @@ def test_tokens_beyond_the_table_are_none_to_the_entry_points():
     assert np.array_equal(y, np.array([1, 0, 0, 0], np.float32)[:, None] * np.ones(8)) and np.array_equal(sums, np.array([0, 0, 1, 0, 0])[:, None] * np.ones(8))
 
 
+def test_no_tokens_leave_a_gradient_of_zeros():
+    from mygrad_amd import _device, _hip
+
+    for dtype in DTYPES:
+        for shift in (0, 1, 3):
+            held, item = np.full(16 + 7 * 33, 5, dtype), np.dtype(dtype).itemsize
+            buf = _device.from_host(held).buf
+            _hip.check(_hip.lib().mg_embedding_bwd(_hip.storage_code(dtype), 0, 7, 33, 1.0, None, None, buf.ptr + shift * item))
+            buf.download_into(held)
+            assert not held[shift:shift + 7 * 33].any() and (held[:shift] == 5).all() and (held[shift + 7 * 33:] == 5).all()
+
+
 def test_entry_points_refuse_bad_arguments():
     from mygrad_amd import _device, _hip
 

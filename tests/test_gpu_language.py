@@ -140,3 +140,13 @@ def test_what_float16_chains():
     # two roundings of float16 on the way, each of half a unit of its value and, where it falls the other way than here, one
     bar = 2.0**-10 * (np.abs(dt) + ora.embedding(table, ids, 1.0, np.abs(dx) + np.abs(dx).max(-1, keepdims=True))[1]) + 2.0**-24 * 12
     assert t.grad.dtype == np.float16 and (np.abs(t.grad - dt) <= bar).all()
+
+
+def test_numbers_of_numpys_types():
+    """``eps``, ``scale``, ``temperature`` and ``top`` as NumPy's scalars."""
+    x = np.random.default_rng(0).standard_normal((3, 8)).astype(np.float32)
+    assert np.array_equal(layer_norm(x, eps=np.float32(0.5)).data, layer_norm(x, eps=0.5).data)
+    assert np.array_equal(embedding(x, [0, 2], scale=np.float32(0.25)).data, embedding(x, [0, 2], scale=0.25).data)
+    assert np.array_equal(embedding(x, np.array([0, 2], np.uint8), scale=np.int64(2)).data, x[[0, 2]] * 2)
+    assert np.array_equal(log_probabilities(x, top=np.int64(2))[2].data, log_probabilities(x, top=2)[2].data)
+    assert np.array_equal(*(distillation(x, [[0], [1], [2]], x[:, :1], temperature=t).data for t in (np.float32(2), 2)))

@@ -210,6 +210,17 @@ def test_entry_points_refuse_bad_arguments():
     assert not held.any()
 
 
+def test_more_rows_than_a_grid_has_blocks():
+    rows = (1 << 24) + 1000
+    x = np.random.default_rng(0).integers(-8, 8, (rows, 2)).astype(np.float16)
+    x[:, 1] += x[:, 0] == x[:, 1]
+    t, b = mg.device_tensor(x), mg.device_tensor(np.zeros(2, np.float16))
+    y = layer_norm(t, None, b, eps=0.0)
+    y.backward(mg.device_tensor(np.full((rows, 2), 2.0**-14, np.float16), constant=True))
+    want = np.where(x == x.max(-1, keepdims=True), 1.0, -1.0)
+    assert np.array_equal(y.data, want) and not t.grad.any() and np.abs(b.grad / (rows * 2.0**-14) - 1).max() < 2.0**-10
+
+
 def test_empty_tensors():
     for shape in ((0, 8), (3, 0), (2, 0, 4)):
         x, w = mg.tensor(np.ones(shape, np.float32)), mg.tensor(np.ones(shape[-1], np.float32))

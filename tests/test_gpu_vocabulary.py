@@ -199,6 +199,30 @@ def test_the_same_bits_every_time(rows, vocabulary):
     assert all(np.array_equal(a, b) for run in runs[1:] for a, b in zip(run, runs[0]))
 
 
+def test_more_rows_than_a_grid_has_blocks():
+    rows = (1 << 22) + 1000
+    z = np.random.default_rng(0).integers(-8, 9, (rows, 3)).astype(np.float16)
+    ids = np.arange(rows) % 3
+    t = mg.device_tensor(z)
+    out, likeliest, which = log_probabilities(t, ids, top=1)
+    p = np.exp(z.astype(np.float64))
+    p /= p.sum(-1, keepdims=True)
+    assert np.array_equal(which.data[:, 0], z.argmax(-1)) and np.abs(out.data - np.log(p[np.arange(rows), ids])).max() < 1e-5
+    assert np.abs(likeliest.data[:, 0] - np.log(p.max(-1))).max() < 1e-5
+    out.backward()
+    p[np.arange(rows), ids] -= 1
+    assert np.abs(t.grad + p).max() < 2.0**-11 + 1e-6
+    rows = (1 << 24) + 1000  # four to a block
+    t = mg.device_tensor(np.ones((rows, 1), np.float16))
+    out = log_probabilities(t, np.zeros(rows, np.int32), entropy=True)
+    out.backward()
+    assert not out.data.any() and not t.grad.any()
+    t = mg.device_tensor(np.ones((rows, 1), np.float16))
+    loss = distillation(t, np.zeros((rows, 1), np.int32), np.ones((rows, 1), np.float16))
+    loss.backward()
+    assert not loss.data.any() and not t.grad.any()
+
+
 def test_leading_shapes():
     z = made(12, 50)
     flat = log_probabilities(z, np.arange(12), entropy=True, top=2)
