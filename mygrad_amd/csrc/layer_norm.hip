@@ -30,71 +30,103 @@ struct Moments {
   C shift, mean, r;  // x - shift - mean, times r
 };
 
+// Calls f with each of the block's values of a row, or of two side by side: a piece, the place of its first value and how many of its values are there.
+constexpr int kLong = 512;  // threads that share a long row
+template <typename T, typename F>
+__device__ __forceinline__ void over_row(const LayerNorm &p, F f) {
+  for (long long d = (long long)threadIdx.x * Piece<T>::V; d < p.D; d += kLong * Piece<T>::V) f(d, (int)min(p.D - d, (long long)Piece<T>::V));
+}
+
 // Of a row that the whole block goes through.
 template <typename T, typename C>
 __device__ __forceinline__ Moments<C> moments_of(const LayerNorm &p, const T *row, C *space) {
+  typedef typename Piece<T>::Held Held;
   C sum[1] = {0};
-  for (long long d = threadIdx.x; d < p.D; d += blockDim.x) sum[0] += (C)row[d];
+  over_row<T>(p, [&](long long d, int count) {
+    const Held v = Piece<T>::load(row + d, count, T(0));
+#pragma unroll
+    for (int n = 0; n < Piece<T>::V; ++n) sum[0] += (C)v[n];
+  });
   block_add(sum, space);
   const C shift = sum[0] / (C)p.D;
   C both[2] = {0, 0};
-  for (long long d = threadIdx.x; d < p.D; d += blockDim.x) {
-    const C v = (C)row[d] - shift;
-    both[0] += v, both[1] += v * v;
-  }
+  over_row<T>(p, [&](long long d, int count) {
+    const Held v = Piece<T>::load(row + d, count, T(0));
+#pragma unroll
+    for (int n = 0; n < Piece<T>::V; ++n) {
+      const C t = n < count ? (C)v[n] - shift : C(0);
+      both[0] += t, both[1] += t * t;
+    }
+  });
   block_add(both, space);
   const C mean = both[0] / (C)p.D;
   return Moments<C>{shift, mean, 1 / sqrt(max(both[1] / (C)p.D - mean * mean, C(0)) + (C)p.eps)};
 }
 
 // ---- a block per row, which it goes through three times ------------------------------------------------------------------------
+// Again from L2, mostly: rows of 40000 halves, 2^27 bytes of x, 79 us forward and 195 back (a copy of as many values 51; one value a thread at a time 226 and 367).
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) layer_norm_kernel(LayerNorm p, const T *__restrict__ x, const T *__restrict__ w, const T *__restrict__ b,
-                                                         T *__restrict__ y, Moments<C> *__restrict__ kept) {
+__global__ void __launch_bounds__(kLong) layer_norm_kernel(LayerNorm p, const T *__restrict__ x, const T *__restrict__ w, const T *__restrict__ b,
+                                                           T *__restrict__ y, Moments<C> *__restrict__ kept) {
+  typedef typename Piece<T>::Held Held;
   __shared__ C space[32];
   const T *row = x + blockIdx.x * p.D;
   T *out = y + blockIdx.x * p.D;
   const Moments<C> m = moments_of(p, row, space);
   if (kept && threadIdx.x == 0) kept[blockIdx.x] = m;
-  for (long long d = threadIdx.x; d < p.D; d += 256)
-    out[d] = (T)(((C)row[d] - m.shift - m.mean) * m.r * (w ? (C)w[d] : C(1)) + (b ? (C)b[d] : C(0)));
+  over_row<T>(p, [&](long long d, int count) {
+    Held v = Piece<T>::load(row + d, count, T(0));
+    const Held weight = w ? Piece<T>::load(w + d, count, T(0)) : Held{}, bias = b ? Piece<T>::load(b + d, count, T(0)) : Held{};
+#pragma unroll
+    for (int n = 0; n < Piece<T>::V; ++n) v[n] = (T)(((C)v[n] - m.shift - m.mean) * m.r * (w ? (C)weight[n] : C(1)) + (C)bias[n]);
+    Piece<T>::store(out + d, count, v);
+  });
 }
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) layer_norm_dx_kernel(LayerNorm p, const T *__restrict__ x, const T *__restrict__ w, const T *__restrict__ grad,
-                                                            const Moments<C> *__restrict__ kept, T *__restrict__ dx) {
+__global__ void __launch_bounds__(kLong) layer_norm_dx_kernel(LayerNorm p, const T *__restrict__ x, const T *__restrict__ w, const T *__restrict__ grad,
+                                                              const Moments<C> *__restrict__ kept, T *__restrict__ dx) {
+  typedef typename Piece<T>::Held Held;
   __shared__ C space[32];
   const T *row = x + blockIdx.x * p.D, *g = grad + blockIdx.x * p.D;
   const Moments<C> m = kept[blockIdx.x];
   C sums[2] = {0, 0};
-  for (long long d = threadIdx.x; d < p.D; d += 256) {
-    const C u = (C)g[d] * (w ? (C)w[d] : C(1));
-    sums[0] += u, sums[1] += u * (((C)row[d] - m.shift - m.mean) * m.r);
-  }
+  auto each = [&](long long d, int count, auto f) {  // behind the row's end g is 0
+    const Held xs = Piece<T>::load(row + d, count, T(0)), gs = Piece<T>::load(g + d, count, T(0));
+    const Held weight = w ? Piece<T>::load(w + d, count, T(0)) : Held{};
+#pragma unroll
+    for (int n = 0; n < Piece<T>::V; ++n) f(n, (C)gs[n] * (w ? (C)weight[n] : C(1)), ((C)xs[n] - m.shift - m.mean) * m.r);
+  };
+  over_row<T>(p, [&](long long d, int count) { each(d, count, [&](int, C u, C n) { sums[0] += u, sums[1] += u * n; }); });
   block_add(sums, space);
   const C first = sums[0] / (C)p.D, second = sums[1] / (C)p.D;
-  for (long long d = threadIdx.x; d < p.D; d += 256) {
-    const C n = ((C)row[d] - m.shift - m.mean) * m.r;
-    dx[blockIdx.x * p.D + d] = (T)(m.r * ((C)g[d] * (w ? (C)w[d] : C(1)) - first - n * second));
-  }
+  over_row<T>(p, [&](long long d, int count) {
+    Held out;
+    each(d, count, [&](int k, C u, C n) { out[k] = (T)(m.r * (u - first - n * second)); });
+    Piece<T>::store(dx + blockIdx.x * p.D + d, count, out);
+  });
 }
 
-// Sums over the rows of one share (blockIdx.y): a thread per column.
+// Sums over the rows of one share (blockIdx.y): a thread per piece of the columns.
 template <typename T, typename C>
 __global__ void __launch_bounds__(256) layer_norm_columns_kernel(LayerNorm p, long long share, const T *__restrict__ x, const T *__restrict__ grad,
-                                                                 const Moments<C> *__restrict__ moments, double *__restrict__ parts) {
-  const long long d = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (d >= p.D) return;
+                                                                 const Moments<C> *__restrict__ kept, double *__restrict__ parts) {
+  typedef typename Piece<T>::Held Held;
+  constexpr int V = Piece<T>::V;
+  const long long d = ((long long)blockIdx.x * 256 + threadIdx.x) * V, left = p.D - d;
+  if (left <= 0) return;
   const long long from = blockIdx.y * share, to = min(p.rows, from + share);
-  double dw = 0, db = 0;
+  double dw[V] = {}, db[V] = {};
+#pragma unroll 2
   for (long long row = from; row < to; ++row) {
-    const Moments<C> m = moments[row];
-    const C g = (C)grad[row * p.D + d];
-    dw += (double)(g * (((C)x[row * p.D + d] - m.shift - m.mean) * m.r));
-    db += (double)g;
+    const Moments<C> m = kept[row];
+    const Held xs = Piece<T>::load(x + row * p.D + d, left, T(0)), gs = Piece<T>::load(grad + row * p.D + d, left, T(0));
+#pragma unroll
+    for (int n = 0; n < V; ++n) dw[n] += (double)((C)gs[n] * (((C)xs[n] - m.shift - m.mean) * m.r)), db[n] += (double)(C)gs[n];
   }
-  parts[(2ll * blockIdx.y) * p.D + d] = dw;
-  parts[(2ll * blockIdx.y + 1) * p.D + d] = db;
+#pragma unroll
+  for (int n = 0; n < V; ++n)
+    if (n < left) parts[(2ll * blockIdx.y) * p.D + d + n] = dw[n], parts[(2ll * blockIdx.y + 1) * p.D + d + n] = db[n];
 }
 
 // Adds the parts of dw and db (blockIdx.y): 64 columns a block, whose 16 wavefronts take a share of the parts each.
@@ -331,7 +363,7 @@ struct Shape {
   int waves, pieces, lanes;
 };
 template <typename T>
-Shape shape_of(long long D) {
+Shape shape_of(long long D, bool back) {
   const long long pieces = ceil_div(D, Piece<T>::V);
   Shape s{0, 0, 64};
   if (pieces <= 64) {
@@ -343,7 +375,7 @@ Shape shape_of(long long D) {
     s = Shape{4, 2, 64};
   } else if (pieces <= 1024) {
     s = sizeof(T) == 2 ? Shape{16, 1, 64} : Shape{4, 4, 64};  // 85 us and 95 back in float16, 84 and 80 in float32
-  } else if (pieces <= 4096) {
+  } else if (pieces <= (back && sizeof(T) == 2 ? 2048 : 4096)) {  // four pieces' sums of float16 do not fit: 265 us back, 190 by the kernels for longer rows
     s = Shape{16, pieces <= 2048 ? 2 : 4, 64};
   }
   return s;
@@ -373,7 +405,7 @@ template <typename T, typename C>
 int forward(const LayerNorm &p, const void *x, const void *w, const void *b, void *y, void *kept) {
   ScopedTiming timed(TAG_LAYER_NORM);
   hipStream_t s = runtime().stream;
-  const Shape shape = shape_of<T>(p.D);
+  const Shape shape = shape_of<T>(p.D, false);
   if (shape.waves) {
     // eight blocks of 256 a compute unit, or as many threads in larger or smaller ones
     const long long most = (shape.waves == 1 ? 8 : 32 / shape.waves) * runtime().props.multiProcessorCount;
@@ -384,7 +416,7 @@ int forward(const LayerNorm &p, const void *x, const void *w, const void *b, voi
     });
   } else {
     if (p.rows >= 1 << 24) return fail(MG_ERR_UNSUPPORTED, "mg_layer_norm_fwd: %lld rows of %lld values", p.rows, p.D);  // a block each
-    layer_norm_kernel<T, C><<<dim3((unsigned)p.rows), dim3(256), 0, s>>>(p, (const T *)x, (const T *)w, (const T *)b, (T *)y, (Moments<C> *)kept);
+    layer_norm_kernel<T, C><<<dim3((unsigned)p.rows), dim3(kLong), 0, s>>>(p, (const T *)x, (const T *)w, (const T *)b, (T *)y, (Moments<C> *)kept);
   }
   MG_HIP(hipGetLastError());
   return MG_OK;
@@ -394,7 +426,7 @@ template <typename T, typename C>
 int backward(const LayerNorm &p, const void *x, const void *w, const void *kept, const void *grad, void *dx, void *dw, void *db) {
   hipStream_t s = runtime().stream;
   const bool columns = dw || db;
-  const Shape shape = shape_of<T>(p.D);
+  const Shape shape = shape_of<T>(p.D, true);
   void *space = nullptr;
   if (shape.waves) {
     // Each block's sums are written once and read once: four blocks of 256 a compute unit (or as many threads) where a thread has one piece, two
@@ -422,11 +454,11 @@ int backward(const LayerNorm &p, const void *x, const void *w, const void *kept,
     if (const int rc = workspace((size_t)(2 * shares * p.D) * sizeof(double), &space)) return rc;
   ScopedTiming timed(TAG_LAYER_NORM_BWD);
   if (dx) {
-    layer_norm_dx_kernel<T, C><<<dim3((unsigned)p.rows), dim3(256), 0, s>>>(p, (const T *)x, (const T *)w, (const T *)grad, (const Moments<C> *)kept, (T *)dx);
+    layer_norm_dx_kernel<T, C><<<dim3((unsigned)p.rows), dim3(kLong), 0, s>>>(p, (const T *)x, (const T *)w, (const T *)grad, (const Moments<C> *)kept, (T *)dx);
     MG_HIP(hipGetLastError());
   }
   if (!columns) return MG_OK;
-  layer_norm_columns_kernel<T, C><<<dim3((unsigned)ceil_div(p.D, 256), (unsigned)shares), dim3(256), 0, s>>>(p, share, (const T *)x, (const T *)grad,
+  layer_norm_columns_kernel<T, C><<<dim3((unsigned)ceil_div(p.D, 256 * Piece<T>::V), (unsigned)shares), dim3(256), 0, s>>>(p, share, (const T *)x, (const T *)grad,
                                                                                                           (const Moments<C> *)kept, (double *)space);
   MG_HIP(hipGetLastError());
   layer_norm_join_kernel<T, double><<<dim3((unsigned)ceil_div(p.D, 64), 2), dim3(1024), 0, s>>>(p.D, (int)shares, (const double *)space, (T *)dw, (T *)db);
