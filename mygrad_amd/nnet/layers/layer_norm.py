@@ -38,13 +38,15 @@ class LayerNorm(Operation):
         self._backed = None
         if self._empty:
             return np.empty(xd.shape, dtype=xd.dtype)
-        self._kept = None
-        if not all([t.constant for t in self.variables]):  # two parts of the mean and 1 / sqrt for each row
-            self._kept = _device.DeviceBuffer(3 * self._call[1] * item)
         held = [_device.to_device(v) for v in values]  # until the launch
-        out = _device.DeviceBuffer(xd.nbytes)
+        # behind the result, for the gradient: two parts of the mean and 1 / sqrt for each row
+        self._kept, behind = None, -(-xd.nbytes // 16) * 16
+        out = _device.DeviceBuffer(behind + 3 * self._call[1] * item)
+        if not all([t.constant for t in self.variables]):
+            self._kept = out.ptr + behind
+            self._result = out
         xp, wp, bp = (None if n is None else held[n].ptr for n in self._places)
-        _hip.check(_hip.lib().mg_layer_norm_fwd(*self._call, float(eps), xp, wp, bp, out.ptr, None if self._kept is None else self._kept.ptr))
+        _hip.check(_hip.lib().mg_layer_norm_fwd(*self._call, float(eps), xp, wp, bp, out.ptr, self._kept))
         y = _device.download(out, xd.shape, xd.dtype)
         _device.attach(y, out)
         return y
@@ -76,7 +78,7 @@ class LayerNorm(Operation):
         xb, gb = _device.to_device(x), _device.to_device(grad, x.dtype)
         wb = None if self._places[1] is None else _device.to_device(values[self._places[1]])
         out = {i: _device.DeviceBuffer(values[i].nbytes) for i in want}
-        _hip.check(_hip.lib().mg_layer_norm_bwd(*self._call, xb.ptr, None if wb is None else wb.ptr, self._kept.ptr, gb.ptr,
+        _hip.check(_hip.lib().mg_layer_norm_bwd(*self._call, xb.ptr, None if wb is None else wb.ptr, self._kept, gb.ptr,
                                                 *(out[i].ptr if i in out else None for i in self._places)))
         return {i: _device.download(buf, values[i].shape, x.dtype) for i, buf in out.items()}
 

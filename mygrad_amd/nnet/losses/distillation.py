@@ -48,14 +48,19 @@ class Distillation(Operation):
             return np.empty(lead, dtype=self._dtype)
         yb = _device.to_device(y, None if taught == y.dtype else taught)
         out = _device.DeviceBuffer(rows * item)
-        keep = not logits.constant
-        self._kept = _device.DeviceBuffer(3 * rows * item) if keep else None
-        self._shares = _device.DeviceBuffer(rows * count * item) if keep else None
+        # what the gradient needs of a row: three statistics and the shares of its tokens
+        self._kept = None if logits.constant else _device.DeviceBuffer((3 + count) * rows * item)
         _hip.check(_hip.lib().mg_distillation_fwd(self._code, _hip.storage_code(taught), *self._call, _device.to_device(z).ptr, tokens._buffer().ptr,
-                                                  yb.ptr, out.ptr, *((self._kept.ptr, self._shares.ptr) if keep else (None, None))))
+                                                  yb.ptr, out.ptr, *self._both()))
         loss = _device.download(out, lead, self._dtype)
         _device.attach(loss, out)
         return loss
+
+    def _both(self):
+        """Where the statistics and the shares lie."""
+        if self._kept is None:
+            return None, None
+        return self._kept.ptr, self._kept.ptr + 3 * self._call[0] * self._dtype.itemsize
 
     @staticmethod
     def _describe(z, y, tokens, temperature):
@@ -85,8 +90,8 @@ class Distillation(Operation):
         if grad.shape != z.shape[:-1]:
             raise NotImplementedError(f"distillation backward for gradient of shape {grad.shape} (no CPU fallback)")
         out = _device.DeviceBuffer(z.nbytes)
-        _hip.check(_hip.lib().mg_distillation_bwd(self._code, *self._call, _device.to_device(z).ptr, self._tokens._buffer().ptr, self._kept.ptr,
-                                                  self._shares.ptr, _device.to_device(grad, self._dtype).ptr, out.ptr))
+        _hip.check(_hip.lib().mg_distillation_bwd(self._code, *self._call, _device.to_device(z).ptr, self._tokens._buffer().ptr, *self._both(),
+                                                  _device.to_device(grad, self._dtype).ptr, out.ptr))
         return _device.download(out, z.shape, z.dtype)
 
 

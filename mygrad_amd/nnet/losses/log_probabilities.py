@@ -61,18 +61,18 @@ class _Plan:
         return np.empty(self.alternatives, dtype=self.dtype), np.empty(self.alternatives, dtype=np.int32)
 
     def run(self, z, ids, keep):
-        """The memory of the values that have a gradient and, if the gradient is to follow, of what it needs; the likeliest tokens."""
-        out = _device.DeviceBuffer(self.nbytes) if self.tokens or self.entropy else None
-        kept = _device.DeviceBuffer(self.kept_bytes) if keep else None
+        """The memory of the values that have a gradient (and, if it is to follow, of what it needs behind them), and the likeliest tokens."""
+        out = _device.DeviceBuffer(self.nbytes + (self.kept_bytes if keep else 0)) if self.tokens or self.entropy else None
+        kept = out.ptr + self.nbytes if keep else None  # behind the result
         top = ()
         if self.top:
             count = self.rows * self.top
             top = (_device.DeviceArray(_device.DeviceBuffer(count * self.dtype.itemsize), self.alternatives, self.dtype),
                    _device.DeviceArray(_device.DeviceBuffer(count * 4), self.alternatives, np.int32))
         _hip.check(_hip.lib().mg_log_probabilities_fwd(self.code, self.rows, self.vocabulary, self.top, ids, _device.to_device(z).ptr,
-                                                       *((None, None) if out is None else self.planes(out.ptr)), None if kept is None else kept.ptr,
+                                                       *((None, None) if out is None else self.planes(out.ptr)), kept,
                                                        *((top[0].buf.ptr, top[1].buf.ptr) if top else (None, None))))
-        return out, kept, top
+        return out, top
 
 
 _plans = {}
@@ -107,7 +107,8 @@ class LogProbabilities(Operation):
         if plan.empty:
             alternatives += plan.no_alternatives()
             return np.empty(plan.shape, dtype=plan.dtype)
-        out, self._kept, found = plan.run(z, None if tokens is None else tokens._buffer().ptr, not logits.constant)
+        out, found = plan.run(z, None if tokens is None else tokens._buffer().ptr, not logits.constant)
+        self._kept = None if logits.constant else out
         alternatives += found
         y = _device.download(out, plan.shape, plan.dtype)
         _device.attach(y, out)
@@ -122,7 +123,7 @@ class LogProbabilities(Operation):
         gb = _device.to_device(grad, plan.dtype)
         out = _device.DeviceBuffer(z.nbytes)
         ids = None if self._tokens is None else self._tokens._buffer().ptr
-        _hip.check(_hip.lib().mg_log_probabilities_bwd(plan.code, plan.rows, plan.vocabulary, ids, _device.to_device(z).ptr, self._kept.ptr,
+        _hip.check(_hip.lib().mg_log_probabilities_bwd(plan.code, plan.rows, plan.vocabulary, ids, _device.to_device(z).ptr, self._kept.ptr + plan.nbytes,
                                                        *plan.planes(gb.ptr), out.ptr))
         return _device.download(out, z.shape, z.dtype)
 
@@ -181,7 +182,7 @@ def log_probabilities(logits, tokens=None, *, entropy: bool = False, top: int = 
     else:  # nothing that has a gradient
         z = _device.value_of(logits if isinstance(logits, Tensor) else Tensor(logits, constant=True, copy=False))
         plan, out = _plan(z, None, entropy, top), None
-        alternatives += plan.no_alternatives() if plan.empty else plan.run(z, None, False)[2]
+        alternatives += plan.no_alternatives() if plan.empty else plan.run(z, None, False)[1]
     likeliest, which = alternatives
     which = TokenIds._on_device(which, np.shape(logits)[-1]) if isinstance(which, _device.DeviceArray) else TokenIds(which)
     return out, Tensor(likeliest, constant=True, copy=False), which
