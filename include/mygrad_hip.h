@@ -488,7 +488,7 @@ int mg_head_norm_bwd(const mg_head_norm_desc *desc, const void *x, const void *w
 
 /* ---- a language model's ends, and the norm between its blocks (no counterparts in the reference) ----
  * dtype: MG_F16, MG_F32 or MG_F64.  Sums and statistics are float32 (float64 for MG_F64), and every result is rounded once.  Tokens
- * are int32 on the device; a negative one stands for none. */
+ * are int32 on the device; a negative one stands for none.  Results do not overlap operands. */
 
 /* y = weight * (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps) + bias over the D values of each row; weight and bias (D,) may be null.
  * kept:(rows, 3), float32 (float64 for MG_F64), is for mg_layer_norm_bwd, and null where there will be none.  Fewer

@@ -67,12 +67,12 @@ __device__ __forceinline__ double exponential(double x) {
   return exp(x);
 }
 
-// LANES threads that share a row: a wavefront, or a block of 256.  All of them call; `space` is 16 values of LDS for a block.
+// LANES threads that share a row: eight, a wavefront, or a block of 256.  All of them call; `space` is 16 values of LDS for a block.
 template <int LANES, typename C>
 __device__ __forceinline__ C group_max(C v, C *space) {
 #pragma unroll
-  for (int k = 32; k; k >>= 1) v = max(v, __shfl_xor(v, k));
-  if (LANES == 64) return v;
+  for (int k = min(LANES, 64) / 2; k; k >>= 1) v = max(v, __shfl_xor(v, k));
+  if (LANES <= 64) return v;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) space[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -80,8 +80,8 @@ __device__ __forceinline__ C group_max(C v, C *space) {
 }
 template <int LANES, typename C>
 __device__ __forceinline__ C group_add(C v, C *space) {
-  v = wave_add(v);
-  if (LANES == 64) return v;
+  v = lanes_add(v, min(LANES, 64));
+  if (LANES <= 64) return v;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) space[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -142,12 +142,12 @@ __device__ __forceinline__ void move_to(Sums<C> &a, C m, C per) {
 }
 
 // Returns the largest of the pieces' values, NaN passed over.
-template <typename T, bool MEAN, typename C>
+template <typename T, bool MEAN, int PIECES, typename C>
 __device__ __forceinline__ C add_pieces(Sums<C> &a, const typename Piece<T>::Held (&z)[kAtOnce], C per) {
   constexpr int V = Piece<T>::V;
   T most = z[0][0];  // a NaN is passed over: the sum shows it
 #pragma unroll
-  for (int u = 0; u < kAtOnce; ++u)
+  for (int u = 0; u < PIECES; ++u)
 #pragma unroll
     for (int n = 0; n < V; ++n) most = sizeof(T) == 2 ? (T)__builtin_fmaxf16((_Float16)most, (_Float16)z[u][n]) : (T)max((C)most, (C)z[u][n]);
   move_to<T, MEAN>(a, max(a.m, (C)most), per);
@@ -156,7 +156,7 @@ __device__ __forceinline__ C add_pieces(Sums<C> &a, const typename Piece<T>::Hel
 #pragma unroll
   for (int n = 0; n < V; ++n)
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
+    for (int u = 0; u < PIECES; ++u) {
       C t = ((C)z[u][n] - base) * per;
       const C e = term<T>(t);
       s[u] += e;
@@ -165,6 +165,16 @@ __device__ __forceinline__ C add_pieces(Sums<C> &a, const typename Piece<T>::Hel
   a.s += (s[0] + s[1]) + (s[2] + s[3]);
   if (MEAN) a.w += (w[0] + w[1]) + (w[2] + w[3]);
   return (C)most;
+}
+
+// Of the first `pieces`, the same number for all threads that share a row: the others hold nothing.
+template <typename T, bool MEAN, typename C>
+__device__ __forceinline__ C add_pieces(Sums<C> &a, const typename Piece<T>::Held (&z)[kAtOnce], C per, long long pieces) {
+  static_assert(kAtOnce == 4);
+  if (pieces >= 4) return add_pieces<T, MEAN, 4>(a, z, per);
+  if (pieces == 1) return add_pieces<T, MEAN, 1>(a, z, per);
+  if (pieces == 2) return add_pieces<T, MEAN, 2>(a, z, per);
+  return add_pieces<T, MEAN, 3>(a, z, per);
 }
 
 // Of all threads' sums.
@@ -290,6 +300,7 @@ __device__ __forceinline__ void collect(Likeliest<T, C> &list, const typename Pi
 // What is made of a row's sums.
 template <typename T, typename C>
 struct Scores {
+  static constexpr bool kFew = true;  // eight threads can take a row
   const int32_t *ids;
   const T *logits;
   C *scores, *entropy;
@@ -312,6 +323,7 @@ struct Scores {
 // pass: that of all entries of a token where it stands first, and -1 for those that have nothing to add.
 template <typename T, typename Y, typename C>
 struct Distillation {
+  static constexpr bool kFew = false;
   const int32_t *ids;
   const T *logits;
   const Y *teacher;
@@ -399,7 +411,8 @@ struct Top {
   int32_t *ids;
 };
 
-// A wavefront per row (four to a block), or a block per part of a row.  Bound by memory, and in float16 nearly by the exponentials.
+// Eight threads or a wavefront per row (32 or four to a block), or a block per part of a row.  Bound by memory, and in float16 nearly by the
+// exponentials.
 template <typename T, typename C, int LANES, bool MEAN, bool TOP, typename End>
 __global__ void __launch_bounds__(256) row_kernel(Vocabulary p, Top w, const T *__restrict__ logits, End end) {
   constexpr int V = Piece<T>::V, kStep = LANES * V * kAtOnce;
@@ -407,11 +420,12 @@ __global__ void __launch_bounds__(256) row_kernel(Vocabulary p, Top w, const T *
   typedef typename Candidate<C>::Order Order;
   __shared__ std::conditional_t<TOP, Likeliest<T, C>, int> list;
   const int lane = threadIdx.x & (LANES - 1);
-  const long long units = LANES == 64 ? (p.rows + 3) / 4 : p.rows * w.parts;
+  constexpr bool SHARED = LANES < 256;  // rows share a block
+  const long long units = SHARED ? (p.rows + 256 / LANES - 1) / (256 / LANES) : p.rows * w.parts;
   for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const long long r = LANES == 64 ? unit * 4 + (threadIdx.x >> 6) : unit / w.parts;
-    if (LANES == 64 && r >= p.rows) return;
-    const int part = LANES == 64 ? 0 : (int)(unit - r * w.parts);
+    const long long r = SHARED ? unit * (256 / LANES) + threadIdx.x / LANES : unit / w.parts;
+    if (SHARED && r >= p.rows) return;
+    const int part = SHARED ? 0 : (int)(unit - r * w.parts);
     const T *row = logits + r * p.V;
     const long long from = (long long)part * w.part, to = min(from + w.part, (long long)p.V);
     const C per = (C)p.per;
@@ -422,19 +436,19 @@ __global__ void __launch_bounds__(256) row_kernel(Vocabulary p, Top w, const T *
       for (long long d0 = from; d0 < to; d0 += kStep) {
         const long long d = d0 + lane * V;
         load_pieces<LANES>(z, row, d, to);
-        const C most = add_pieces<T, MEAN>(sums, z, per);
+        const C most = add_pieces<T, MEAN>(sums, z, per, (to - d0 + LANES * V - 1) / (LANES * V));
         if (d0 == from) list.begin(d < to ? order_of(most) : Order(0), p.top);
         if (order_of(most) >= list.bound.value) list.add_pieces(z, d, to);
       }
     } else {
-      for (long long d = from + lane * V; d < to; d += kStep) {
-        load_pieces<LANES>(z, row, d, to);
-        add_pieces<T, MEAN>(sums, z, per);
+      for (long long d0 = from; d0 < to; d0 += kStep) {
+        load_pieces<LANES>(z, row, d0 + lane * V, to);
+        add_pieces<T, MEAN>(sums, z, per, (to - d0 + LANES * V - 1) / (LANES * V));
       }
     }
     const C own = sums.m;
     sums = join<LANES, T, MEAN>(sums, per, space);
-    if (LANES == 64 || w.parts == 1) end.template end<LANES>(p, r, lane, sums, space);
+    if (SHARED || w.parts == 1) end.template end<LANES>(p, r, lane, sums, space);
     else if (lane == 0) ((Sums<C> *)w.partial)[unit] = sums;
     if constexpr (TOP) {
       __syncthreads();
@@ -522,23 +536,24 @@ __global__ void __launch_bounds__(256) row_join_kernel(Vocabulary p, Top w, cons
 
 // How a pass over the rows is laid out.
 struct Plan {
-  bool wavefronts;  // a wavefront per row
+  int lanes;  // threads that share a row: 8, 64 or 256
   int parts, part;
   unsigned blocks;
 };
 
-// Rows that a wavefront takes in one step go four to a block.  Longer ones have a block each, or, where there are fewer than two for a
+// Rows that eight threads or a wavefront take in one step go 32 or four to a block.  Longer ones have a block each, or, where there are fewer than two for a
 // compute unit, parts of a step or more for four blocks a unit.  50001 halves a row, us with and without parts: 300 rows 12 + 4 and 14, 600
 // rows 19 + 4 and 18; one row of 131101 4 + 3 in parts.
 template <typename T>
-Plan plan_of(const Vocabulary &p, bool alone) {
+Plan plan_of(const Vocabulary &p, bool alone, bool few) {
   constexpr int V = Piece<T>::V;
   const long long most = 1 << 22;
-  if (!alone && p.V <= 64 * V * kAtOnce) return Plan{true, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 4), most)};
+  if (!alone && few && p.V <= 8 * V * kAtOnce) return Plan{8, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 32), most)};
+  if (!alone && p.V <= 64 * V * kAtOnce) return Plan{64, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 4), most)};
   const long long wanted = 4ll * runtime().props.multiProcessorCount / p.rows, step = 256 * V;
   const long long parts = std::max<long long>(1, std::min<long long>(wanted, ceil_div(p.V, step)));
   const long long part = ceil_div(ceil_div(p.V, parts), step) * step;
-  Plan plan{false, (int)ceil_div(p.V, part), (int)std::min<long long>(part, p.V), 0};
+  Plan plan{256, (int)ceil_div(p.V, part), (int)std::min<long long>(part, p.V), 0};
   plan.blocks = (unsigned)std::min<long long>(p.rows * plan.parts, most);
   return plan;
 }
@@ -546,7 +561,7 @@ Plan plan_of(const Vocabulary &p, bool alone) {
 template <typename T, typename C, bool MEAN, bool TOP, typename End>
 int over_rows(const Vocabulary &p, const void *logits, const End &end, void *top_scores, int32_t *top_ids) {
   typedef typename Candidate<C>::Order Order;
-  const Plan plan = plan_of<T>(p, TOP);
+  const Plan plan = plan_of<T>(p, TOP, End::kFew);
   hipStream_t s = runtime().stream;
   Top w{plan.parts, plan.part, nullptr, nullptr, nullptr, top_scores, top_ids};
   if (plan.parts > 1) {
@@ -555,7 +570,9 @@ int over_rows(const Vocabulary &p, const void *logits, const End &end, void *top
     if (const int rc = workspace(sums + found * (sizeof(Order) + 4), (void **)&space)) return rc;
     w.partial = space, w.values = space + sums, w.places = (int *)(space + sums + found * sizeof(Order));
   }
-  if (plan.wavefronts) {
+  if (plan.lanes == 8) {
+    if constexpr (!TOP && End::kFew) row_kernel<T, C, 8, MEAN, false, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
+  } else if (plan.lanes == 64) {
     if constexpr (!TOP) row_kernel<T, C, 64, MEAN, false, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
   } else {
     row_kernel<T, C, 256, MEAN, TOP, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
@@ -569,7 +586,7 @@ int over_rows(const Vocabulary &p, const void *logits, const End &end, void *top
 }
 
 // ---- gradients --------------------------------------------------------------------------------------------------------------------
-// As many pieces of a row as a block has on their way together, or a wavefront per row.  The rows come in the order opposite to the forward
+// As many pieces of a row as a block has on their way together, or eight threads or a wavefront per row.  The rows come in the order opposite to the forward
 // pass's: it has read the last of them last, and some of those are still near (4096 x 50000 halves, both passes 244 us and 246; distillation
 // over 32000 181 and 185).
 template <typename T, typename C, int LANES, bool ENTROPY>
@@ -579,12 +596,13 @@ __global__ void __launch_bounds__(256) scores_bwd_kernel(Vocabulary p, int parts
   typedef typename Piece<T>::Held Held;
   constexpr int V = Piece<T>::V, kStep = LANES * V * kAtOnce;
   const int lane = threadIdx.x & (LANES - 1);
-  const long long units = LANES == 64 ? (p.rows + 3) / 4 : p.rows * parts;
+  constexpr bool SHARED = LANES < 256;  // rows share a block
+  const long long units = SHARED ? (p.rows + 256 / LANES - 1) / (256 / LANES) : p.rows * parts;
   for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const long long r0 = LANES == 64 ? unit * 4 + (threadIdx.x >> 6) : unit / parts;
-    if (LANES == 64 && r0 >= p.rows) return;
-    const long long r = p.rows - 1 - r0;
-    const long long at = (LANES == 64 ? 0 : (unit - r0 * parts) * kStep) + lane * V;
+    const long long nth = SHARED ? unit * (256 / LANES) + threadIdx.x / LANES : unit / parts;
+    if (SHARED && nth >= p.rows) return;
+    const long long r = p.rows - 1 - nth;
+    const long long at = (SHARED ? 0 : (unit - nth * parts) * kStep) + lane * V;
     const T *z = logits + r * p.V;
     T *out = dlogits + r * p.V;
     Held held[kAtOnce];
@@ -728,12 +746,13 @@ int mg_log_probabilities_bwd(int dtype, int64_t rows, int64_t V, const int32_t *
     typedef std::remove_pointer_t<decltype(c)> C;
     ScopedTiming timed(TAG_SCORES_BWD);
     auto run = [&](auto lanes, auto with_entropy) {
-      const long long parts = ceil_div(V, lanes * Piece<T>::V * kAtOnce), blocks = lanes == 64 ? ceil_div(rows, 4) : rows * parts;
+      const long long parts = ceil_div(V, lanes * Piece<T>::V * kAtOnce), blocks = lanes < 256 ? ceil_div(rows, 256 / lanes) : rows * parts;
       scores_bwd_kernel<T, C, lanes, with_entropy><<<dim3((unsigned)std::min<long long>(blocks, 1 << 22)), dim3(256), 0, runtime().stream>>>(
           p, (int)parts, ids, (const T *)logits, (const Row<C> *)kept, (const C *)grad_scores, (const C *)grad_entropy, (T *)dlogits);
     };
     auto by_length = [&](auto with_entropy) {
-      if (V <= 64 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 64>{}, with_entropy);
+      if (V <= 8 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 8>{}, with_entropy);
+      else if (V <= 64 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 64>{}, with_entropy);
       else run(std::integral_constant<int, 256>{}, with_entropy);
     };
     if (grad_entropy) by_length(std::true_type{});
