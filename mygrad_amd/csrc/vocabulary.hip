@@ -67,7 +67,7 @@ __device__ __forceinline__ double exponential(double x) {
   return exp(x);
 }
 
-// LANES threads that share a row: eight, a wavefront, or a block of 256.  All of them call; `space` is 16 values of LDS for a block.
+// LANES threads that share a row: eight, sixteen, a wavefront, or a block of 256.  All of them call; `space` is 16 values of LDS for a block.
 template <int LANES, typename C>
 __device__ __forceinline__ C group_max(C v, C *space) {
 #pragma unroll
@@ -300,7 +300,7 @@ __device__ __forceinline__ void collect(Likeliest<T, C> &list, const typename Pi
 // What is made of a row's sums.
 template <typename T, typename C>
 struct Scores {
-  static constexpr bool kFew = true;  // eight threads can take a row
+  static constexpr bool kFew = true;  // less than a wavefront can take a row
   const int32_t *ids;
   const T *logits;
   C *scores, *entropy;
@@ -411,7 +411,7 @@ struct Top {
   int32_t *ids;
 };
 
-// Eight threads or a wavefront per row (32 or four to a block), or a block per part of a row.  Bound by memory, and in float16 nearly by the
+// Eight or sixteen threads or a wavefront per row, or a block per part of a row.  Bound by memory, and in float16 nearly by the
 // exponentials.
 template <typename T, typename C, int LANES, bool MEAN, bool TOP, typename End>
 __global__ void __launch_bounds__(256) row_kernel(Vocabulary p, Top w, const T *__restrict__ logits, End end) {
@@ -536,12 +536,14 @@ __global__ void __launch_bounds__(256) row_join_kernel(Vocabulary p, Top w, cons
 
 // How a pass over the rows is laid out.
 struct Plan {
-  int lanes;  // threads that share a row: 8, 64 or 256
+  int lanes;  // threads that share a row: 8, 16, 64 or 256
   int parts, part;
   unsigned blocks;
 };
 
-// Rows that eight threads or a wavefront take in one step go 32 or four to a block.  Longer ones have a block each, or, where there are fewer than two for a
+// Rows that eight or sixteen threads or a wavefront take in one step share a block; where there are enough for all wavefronts, also those that a
+// wavefront takes in four.  2^27 bytes of halves, us forward: rows of 64 by eight threads 58, by a wavefront 630; of 300 by sixteen 36, by a wavefront 111; of
+// 2100 by a wavefront 36, by a block 73; of 8000 29 either way.  Longer ones have a block each, or, where there are fewer than two for a
 // compute unit, parts of a step or more for four blocks a unit.  50001 halves a row, us with and without parts: 300 rows 12 + 4 and 14, 600
 // rows 19 + 4 and 18; one row of 131101 4 + 3 in parts.
 template <typename T>
@@ -549,7 +551,9 @@ Plan plan_of(const Vocabulary &p, bool alone, bool few) {
   constexpr int V = Piece<T>::V;
   const long long most = 1 << 22;
   if (!alone && few && p.V <= 8 * V * kAtOnce) return Plan{8, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 32), most)};
-  if (!alone && p.V <= 64 * V * kAtOnce) return Plan{64, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 4), most)};
+  if (!alone && few && p.V <= 16 * V * kAtOnce) return Plan{16, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 16), most)};
+  const int steps = p.rows >= 16ll * runtime().props.multiProcessorCount ? 4 : 1;
+  if (!alone && p.V <= 64 * V * kAtOnce * steps) return Plan{64, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 4), most)};
   const long long wanted = 4ll * runtime().props.multiProcessorCount / p.rows, step = 256 * V;
   const long long parts = std::max<long long>(1, std::min<long long>(wanted, ceil_div(p.V, step)));
   const long long part = ceil_div(ceil_div(p.V, parts), step) * step;
@@ -572,6 +576,8 @@ int over_rows(const Vocabulary &p, const void *logits, const End &end, void *top
   }
   if (plan.lanes == 8) {
     if constexpr (!TOP && End::kFew) row_kernel<T, C, 8, MEAN, false, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
+  } else if (plan.lanes == 16) {
+    if constexpr (!TOP && End::kFew) row_kernel<T, C, 16, MEAN, false, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
   } else if (plan.lanes == 64) {
     if constexpr (!TOP) row_kernel<T, C, 64, MEAN, false, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
   } else {
@@ -586,7 +592,7 @@ int over_rows(const Vocabulary &p, const void *logits, const End &end, void *top
 }
 
 // ---- gradients --------------------------------------------------------------------------------------------------------------------
-// As many pieces of a row as a block has on their way together, or eight threads or a wavefront per row.  The rows come in the order opposite to the forward
+// As many pieces of a row as a block has on their way together, or eight or sixteen threads or a wavefront per row.  The rows come in the order opposite to the forward
 // pass's: it has read the last of them last, and some of those are still near (4096 x 50000 halves, both passes 244 us and 246; distillation
 // over 32000 181 and 185).
 template <typename T, typename C, int LANES, bool ENTROPY>
@@ -752,6 +758,7 @@ int mg_log_probabilities_bwd(int dtype, int64_t rows, int64_t V, const int32_t *
     };
     auto by_length = [&](auto with_entropy) {
       if (V <= 8 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 8>{}, with_entropy);
+      else if (V <= 16 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 16>{}, with_entropy);
       else if (V <= 64 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 64>{}, with_entropy);
       else run(std::integral_constant<int, 256>{}, with_entropy);
     };

@@ -100,14 +100,15 @@ def some(rows, vocabulary, seed=0):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("vocabulary", [1, 2, 3, 7, 8, 63, 64, 65, 255, 1000, 1024, 2049, 4096, 8191, 8200, 32003, 50000, 131101])
+@pytest.mark.parametrize("vocabulary", [1, 2, 3, 7, 8, 31, 33, 63, 64, 65, 127, 129, 255, 257, 511, 513, 1000, 1024, 2049, 4096, 8191, 8200, 32003, 50000, 131101])
 def test_lengths_of_rows(dtype, vocabulary):
     check(dtype, made(3, vocabulary), some(3, vocabulary))
     check(dtype, made(3, vocabulary, 1), some(3, vocabulary, 1), entropy=True, top=min(7, vocabulary))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,vocabulary", [(1, 1000), (1, 70001), (40, 33), (257, 1001), (600, 5000), (3000, 640), (70000, 9)])
+@pytest.mark.parametrize("rows,vocabulary", [(1, 1000), (1, 70001), (40, 33), (257, 1001), (600, 5000), (3000, 640), (70000, 9), (4097, 2500), (4100, 1999),
+                                             (1001, 200), (999, 300)])
 def test_numbers_of_rows(dtype, rows, vocabulary):
     check(dtype, made(rows, vocabulary), some(rows, vocabulary), entropy=True)
     check(dtype, made(rows, vocabulary, 2), some(rows, vocabulary, 2), top=3)
@@ -294,7 +295,7 @@ def test_distillation_lengths_of_rows(dtype, vocabulary):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,vocabulary,count", [(1, 600, 1), (1, 5000, 256), (300, 300, 200), (700, 1999, 20), (20000, 17, 3), (2, 60000, 65)])
+@pytest.mark.parametrize("rows,vocabulary,count", [(1, 600, 1), (1, 5000, 256), (300, 300, 200), (700, 1999, 20), (20000, 17, 3), (2, 60000, 65), (4101, 2300, 70)])
 def test_distillation_numbers_of_rows_and_tokens(dtype, rows, vocabulary, count):
     check_distillation(dtype, made(rows, vocabulary), *lessons(rows, vocabulary, count))
 
