@@ -20,7 +20,8 @@ namespace mg {
 namespace {
 
 constexpr int kMostTop = 128;     // likeliest tokens that are looked for
-constexpr int kMostTaught = 256;  // a teacher's tokens for a row: a thread of a block each
+constexpr int kMostTaught = 256;  // a teacher's tokens for a row: a thread of a block each, or kTurns for each that shares a row otherwise
+constexpr int kTurns = 4;
 
 struct Vocabulary {
   long long rows;
@@ -300,7 +301,6 @@ __device__ __forceinline__ void collect(Likeliest<T, C> &list, const typename Pi
 // What is made of a row's sums.
 template <typename T, typename C>
 struct Scores {
-  static constexpr bool kFew = true;  // less than a wavefront can take a row
   const int32_t *ids;
   const T *logits;
   C *scores, *entropy;
@@ -319,11 +319,10 @@ struct Scores {
   }
 };
 
-// Or of those and a teacher's logits: a thread (or each lane of a wavefront, in turns) takes one of them.  q goes to memory for the backward
+// Or of those and a teacher's logits: a thread takes one of them, or up to four in turns.  q goes to memory for the backward
 // pass: that of all entries of a token where it stands first, and -1 for those that have nothing to add.
 template <typename T, typename Y, typename C>
 struct Distillation {
-  static constexpr bool kFew = false;
   const int32_t *ids;
   const T *logits;
   const Y *teacher;
@@ -333,7 +332,7 @@ struct Distillation {
 
   template <int LANES>
   __device__ __forceinline__ void end(const Vocabulary &p, long long r, int lane, const Sums<C> &sums, C *space) const {
-    constexpr int TURNS = kMostTaught / LANES;
+    constexpr int TURNS = LANES < 256 ? kTurns : 1, MOST = TURNS * LANES;
     const C per = (C)p.per;
     Row<C> row = row_of(sums);
     int id[TURNS];
@@ -363,12 +362,12 @@ struct Distillation {
     }
     sum = group_add<LANES>(sum, space);
     if (shares) {
-      __shared__ __attribute__((aligned(16))) int tokens[256 / LANES][kMostTaught];
-      __shared__ C q[256 / LANES][kMostTaught];
-      const int group = LANES == 64 ? threadIdx.x >> 6 : 0;
+      __shared__ __attribute__((aligned(16))) int tokens[256 / LANES][MOST];
+      __shared__ C q[256 / LANES][MOST];
+      const int group = threadIdx.x / LANES;
 #pragma unroll
       for (int n = 0; n < TURNS; ++n) tokens[group][lane + n * LANES] = id[n] < p.V ? id[n] : -1, q[group][lane + n * LANES] = f[n];
-      if (LANES == 64) wave_sees();
+      if (LANES <= 64) wave_sees();
       else __syncthreads();
 #pragma unroll
       for (int n = 0; n < TURNS; ++n) {
@@ -391,7 +390,7 @@ struct Distillation {
         }
         shares[r * p.top + k] = adds ? all : C(-1);
       }
-      if (LANES == 64) wave_sees();
+      if (LANES <= 64) wave_sees();
       else __syncthreads();
     }
     if (lane) return;
@@ -543,15 +542,16 @@ struct Plan {
 
 // Rows that eight or sixteen threads or a wavefront take in one step share a block; where there are enough for all wavefronts, also those that a
 // wavefront takes in four.  2^27 bytes of halves, us forward: rows of 64 by eight threads 58, by a wavefront 630; of 300 by sixteen 36, by a wavefront 111; of
-// 2100 by a wavefront 36, by a block 73; of 8000 29 either way.  Longer ones have a block each, or, where there are fewer than two for a
+// 2100 by a wavefront 36, by a block 73; of 8000 29 either way; distillation with 8 of 64 tokens, both passes, 207 by eight threads a row, 1342 by
+// a wavefront.  Longer ones have a block each, or, where there are fewer than two for a
 // compute unit, parts of a step or more for four blocks a unit.  50001 halves a row, us with and without parts: 300 rows 12 + 4 and 14, 600
 // rows 19 + 4 and 18; one row of 131101 4 + 3 in parts.
 template <typename T>
-Plan plan_of(const Vocabulary &p, bool alone, bool few) {
+Plan plan_of(const Vocabulary &p, bool alone) {
   constexpr int V = Piece<T>::V;
   const long long most = 1 << 22;
-  if (!alone && few && p.V <= 8 * V * kAtOnce) return Plan{8, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 32), most)};
-  if (!alone && few && p.V <= 16 * V * kAtOnce) return Plan{16, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 16), most)};
+  if (!alone && p.top <= 8 * kTurns && p.V <= 8 * V * kAtOnce) return Plan{8, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 32), most)};
+  if (!alone && p.top <= 16 * kTurns && p.V <= 16 * V * kAtOnce) return Plan{16, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 16), most)};
   const int steps = p.rows >= 16ll * runtime().props.multiProcessorCount ? 4 : 1;
   if (!alone && p.V <= 64 * V * kAtOnce * steps) return Plan{64, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 4), most)};
   const long long wanted = 4ll * runtime().props.multiProcessorCount / p.rows, step = 256 * V;
@@ -565,7 +565,7 @@ Plan plan_of(const Vocabulary &p, bool alone, bool few) {
 template <typename T, typename C, bool MEAN, bool TOP, typename End>
 int over_rows(const Vocabulary &p, const void *logits, const End &end, void *top_scores, int32_t *top_ids) {
   typedef typename Candidate<C>::Order Order;
-  const Plan plan = plan_of<T>(p, TOP, End::kFew);
+  const Plan plan = plan_of<T>(p, TOP);
   hipStream_t s = runtime().stream;
   Top w{plan.parts, plan.part, nullptr, nullptr, nullptr, top_scores, top_ids};
   if (plan.parts > 1) {
@@ -575,9 +575,9 @@ int over_rows(const Vocabulary &p, const void *logits, const End &end, void *top
     w.partial = space, w.values = space + sums, w.places = (int *)(space + sums + found * sizeof(Order));
   }
   if (plan.lanes == 8) {
-    if constexpr (!TOP && End::kFew) row_kernel<T, C, 8, MEAN, false, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
+    if constexpr (!TOP) row_kernel<T, C, 8, MEAN, false, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
   } else if (plan.lanes == 16) {
-    if constexpr (!TOP && End::kFew) row_kernel<T, C, 16, MEAN, false, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
+    if constexpr (!TOP) row_kernel<T, C, 16, MEAN, false, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
   } else if (plan.lanes == 64) {
     if constexpr (!TOP) row_kernel<T, C, 64, MEAN, false, End><<<dim3(plan.blocks), dim3(256), 0, s>>>(p, w, (const T *)logits, end);
   } else {
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(256) scores_bwd_kernel(Vocabulary p, int parts
   }
 }
 
-// Wavefronts write the teacher's tokens among their own values once more; nobody waits for another.
+// The threads that share a row, or those of each wavefront, write the teacher's tokens among their own values once more; nobody waits for another.
 template <typename T, typename C, int LANES>
 __global__ void __launch_bounds__(256) distillation_bwd_kernel(Vocabulary p, int parts, const int32_t *__restrict__ ids, const T *__restrict__ logits,
                                                                const Row<C> *__restrict__ kept, const C *__restrict__ shares,
@@ -651,11 +651,12 @@ __global__ void __launch_bounds__(256) distillation_bwd_kernel(Vocabulary p, int
   typedef typename Piece<T>::Held Held;
   constexpr int V = Piece<T>::V, kStep = LANES * V * kAtOnce;
   const int lane = threadIdx.x & (LANES - 1);
-  const long long units = LANES == 64 ? (p.rows + 3) / 4 : p.rows * parts;
+  constexpr bool SHARED = LANES < 256;  // rows share a block
+  const long long units = SHARED ? (p.rows + 256 / LANES - 1) / (256 / LANES) : p.rows * parts;
   for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const long long nth = LANES == 64 ? unit * 4 + (threadIdx.x >> 6) : unit / parts;
-    if (LANES == 64 && nth >= p.rows) return;
-    const long long r = p.rows - 1 - nth, from = LANES == 64 ? 0 : (unit - nth * parts) * kStep, at = from + lane * V;
+    const long long nth = SHARED ? unit * (256 / LANES) + threadIdx.x / LANES : unit / parts;
+    if (SHARED && nth >= p.rows) return;
+    const long long r = p.rows - 1 - nth, from = SHARED ? 0 : (unit - nth * parts) * kStep, at = from + lane * V;
     const T *z = logits + r * p.V;
     T *out = dlogits + r * p.V;
     Held held[kAtOnce];
@@ -674,12 +675,12 @@ __global__ void __launch_bounds__(256) distillation_bwd_kernel(Vocabulary p, int
     }
     if (nothing) continue;
     wave_sees();  // the same memory again, by other lanes
-    for (int k = threadIdx.x & 63; k < p.top; k += 64) {
+    for (int k = lane & 63; k < p.top; k += min(LANES, 64)) {
       const int id = ids[r * p.top + k];
       const C q = shares[r * p.top + k];
       const long long place = id - from;
       if (q < 0 || place < 0 || place >= kStep) continue;
-      if (LANES == 64 || (int)(place % (LANES * V)) / (64 * V) == (int)(threadIdx.x >> 6))
+      if (SHARED || (int)(place % (LANES * V)) / (64 * V) == (int)(threadIdx.x >> 6))
         out[id] = (T)(g * (exponential<T>(((C)z[id] - row.m) * per) * inverse - q));
     }
   }
@@ -802,11 +803,13 @@ int mg_distillation_bwd(int dtype, int64_t rows, int64_t V, int64_t K, double te
     typedef std::remove_pointer_t<decltype(c)> C;
     ScopedTiming timed(TAG_DISTILLATION_BWD);
     auto run = [&](auto lanes) {
-      const long long parts = ceil_div(V, lanes * Piece<T>::V * kAtOnce), blocks = lanes == 64 ? ceil_div(rows, 4) : rows * parts;
+      const long long parts = ceil_div(V, lanes * Piece<T>::V * kAtOnce), blocks = lanes < 256 ? ceil_div(rows, 256 / lanes) : rows * parts;
       distillation_bwd_kernel<T, C, lanes><<<dim3((unsigned)std::min<long long>(blocks, 1 << 22)), dim3(256), 0, runtime().stream>>>(
           p, (int)parts, ids, (const T *)logits, (const Row<C> *)kept, (const C *)shares, (const C *)grad, (T *)dlogits);
     };
-    if (V <= 64 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 64>{});
+    if (K <= 8 * kTurns && V <= 8 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 8>{});
+    else if (K <= 16 * kTurns && V <= 16 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 16>{});
+    else if (V <= 64 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 64>{});
     else run(std::integral_constant<int, 256>{});
     MG_HIP(hipGetLastError());
     return (int)MG_OK;

@@ -301,6 +301,17 @@ def test_distillation_numbers_of_rows_and_tokens(dtype, rows, vocabulary, count)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocabulary", [50, 120, 250, 500, 520])
+@pytest.mark.parametrize("rows,count", [(67, 32), (35, 33), (19, 64), (17, 65), (5, 256)])
+def test_distillation_of_short_rows(dtype, vocabulary, rows, count):
+    z, (ids, teacher) = made(rows, vocabulary), lessons(rows, max(vocabulary, count), count)
+    ids %= vocabulary
+    ids[rows // 2, ::3] = ids[rows // 2, 0]  # the same token again and again
+    ids[rows // 3] = -1  # a row without a teacher
+    check_distillation(dtype, z, ids, teacher, temperature=1.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("vocabulary", [40, 9000, 70001])
 def test_distillation_with_lists_of_all_kinds(dtype, vocabulary):
     ids, teacher = lessons(8, vocabulary, 16)
