@@ -43,23 +43,61 @@ __device__ __forceinline__ float from_lane(float v) {
 }
 template <int CONTROL>
 __device__ __forceinline__ double from_lane(double v) {
-  typedef int Two __attribute__((ext_vector_type(2)));
-  Two q = __builtin_bit_cast(Two, v);
+  typedef int Words __attribute__((ext_vector_type(2)));
+  Words q = __builtin_bit_cast(Words, v);
   q[0] = __builtin_amdgcn_mov_dpp(q[0], CONTROL, 0xf, 0xf, true), q[1] = __builtin_amdgcn_mov_dpp(q[1], CONTROL, 0xf, 0xf, true);
   return __builtin_bit_cast(double, q);
 }
 
-// The sum over each run of `lanes` lanes, a power of two, for all of them.
+// Of the two lanes of a wavefront that lie 16 (32) apart both values, the lower lane's first, by a move within the vector unit.
 template <typename C>
-__device__ __forceinline__ C lanes_add(C v, int lanes) {
-  if (lanes > 1) v += from_lane<0xb1>(v);   // lanes 1 0 3 2 of four
-  if (lanes > 2) v += from_lane<0x4e>(v);   // 2 3 0 1
-  if (lanes > 4) v += from_lane<0x141>(v);  // eight from behind
-  if (lanes > 8) v += from_lane<0x140>(v);  // sixteen from behind
-  if (lanes > 16) v += __shfl_xor(v, 16);
-  if (lanes > 32) v += __shfl_xor(v, 32);
+struct Two {
+  C low, high;
+};
+template <int APART>
+__device__ __forceinline__ Two<int> pair_of(int v) {
+  const auto both = APART == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return {(int)both[0], (int)both[1]};
+}
+template <int APART>
+__device__ __forceinline__ Two<float> pair_of(float v) {
+  const Two<int> both = pair_of<APART>(__builtin_bit_cast(int, v));
+  return {__builtin_bit_cast(float, both.low), __builtin_bit_cast(float, both.high)};
+}
+template <int APART>
+__device__ __forceinline__ Two<double> pair_of(double v) {
+  typedef int Words __attribute__((ext_vector_type(2)));
+  const Words words = __builtin_bit_cast(Words, v);
+  const Two<int> first = pair_of<APART>(words[0]), second = pair_of<APART>(words[1]);
+  return {__builtin_bit_cast(double, Words{first.low, second.low}), __builtin_bit_cast(double, Words{first.high, second.high})};
+}
+
+// `over` of each run of `lanes` lanes, a power of two, for all of them.
+template <typename C, typename Over>
+__device__ __forceinline__ C lanes_over(C v, int lanes, Over over) {
+  if (lanes > 1) v = over(v, from_lane<0xb1>(v));   // lanes 1 0 3 2 of four
+  if (lanes > 2) v = over(v, from_lane<0x4e>(v));   // 2 3 0 1
+  if (lanes > 4) v = over(v, from_lane<0x141>(v));  // eight from behind
+  if (lanes > 8) v = over(v, from_lane<0x140>(v));  // sixteen from behind
+  if (lanes > 16) {
+    const Two<C> both = pair_of<16>(v);
+    v = over(both.low, both.high);
+  }
+  if (lanes > 32) {
+    const Two<C> both = pair_of<32>(v);
+    v = over(both.low, both.high);
+  }
   return v;
 }
+template <typename C>
+__device__ __forceinline__ C lanes_add(C v, int lanes) {
+  return lanes_over(v, lanes, [](C a, C b) { return a + b; });
+}
+template <typename C>
+__device__ __forceinline__ C lanes_max(C v, int lanes) {
+  return lanes_over(v, lanes, [](C a, C b) { return max(a, b); });
+}
+
 // What the lanes of a wavefront wrote is there for all of them.
 __device__ __forceinline__ void wave_sees() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
