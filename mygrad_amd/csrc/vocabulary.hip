@@ -587,20 +587,23 @@ struct Plan {
 // Rows that eight or sixteen threads or a wavefront take in one step share a block; where there are enough for all wavefronts, also those that a
 // wavefront takes in four.  2^27 bytes of halves, us forward: rows of 64 by eight threads 58, by a wavefront 630; of 300 by sixteen 36, by a wavefront 111; of
 // 2100 by a wavefront 36, by a block 73; of 8000 29 either way; distillation with 8 of 64 tokens, both passes, 207 by eight threads a row, 1342 by
-// a wavefront.  Longer ones have a block each, or, where there are fewer than two for a
-// compute unit, parts of a step or more for four blocks a unit.  50001 halves a row, us with and without parts: 300 rows 12 + 4 and 14, 600
-// rows 19 + 4 and 18; one row of 131101 4 + 3 in parts.
+// a wavefront.  Longer ones have a block each, or, where there are few, parts for four blocks a compute unit and a launch that joins
+// them, if that saves a block five steps (three where likeliest tokens are looked for, whose list a block waits for in each step; then two parts are
+// worth it, otherwise three).  us in parts and without: 4 rows of 32003 halves 7.0 and 7.0, of 50001 7.1 and 9.9, of 131101 7.2 and 19.6;
+// 257 of 16001 8.2 and 5.9, of 50001 13.0 and 12.9, of 131101 22.8 and 30.7; 500 of 131101 floats 47.7 and 42.2.  With 8 alternatives 4
+// rows of 16001 halves 9.3 and 9.1, of 32003 9.5 and 13.6, 257 of 50001 19.6 and 22.6, 500 of them 27.0 and 27.4.
 template <typename T>
-Plan plan_of(const Vocabulary &p, bool alone) {
+Plan plan_of(const Vocabulary &p, bool top) {
   constexpr int V = Piece<T>::V;
   const long long most = 1 << 22;
-  if (!alone && p.top <= 8 * kTurns && p.V <= 8 * V * kAtOnce) return Plan{8, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 32), most)};
-  if (!alone && p.top <= 16 * kTurns && p.V <= 16 * V * kAtOnce) return Plan{16, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 16), most)};
+  if (!top && p.top <= 8 * kTurns && p.V <= 8 * V * kAtOnce) return Plan{8, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 32), most)};
+  if (!top && p.top <= 16 * kTurns && p.V <= 16 * V * kAtOnce) return Plan{16, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 16), most)};
   const int steps = p.rows >= 16ll * runtime().props.multiProcessorCount ? 4 : 1;
-  if (!alone && p.V <= 64 * V * kAtOnce * steps) return Plan{64, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 4), most)};
-  const long long wanted = 4ll * runtime().props.multiProcessorCount / p.rows, step = 256 * V;
-  const long long parts = std::max<long long>(1, std::min<long long>(wanted, ceil_div(p.V, step)));
-  const long long part = ceil_div(ceil_div(p.V, parts), step) * step;
+  if (!top && p.V <= 64 * V * kAtOnce * steps) return Plan{64, 1, p.V, (unsigned)std::min<long long>(ceil_div(p.rows, 4), most)};
+  const long long wanted = 4ll * runtime().props.multiProcessorCount / p.rows, piece = 256 * V, step = piece * kAtOnce;
+  const long long parts = std::max<long long>(1, std::min<long long>(wanted, ceil_div(p.V, piece)));
+  long long part = ceil_div(ceil_div(p.V, parts), piece) * piece;
+  if (parts < (top ? 2 : 3) || ceil_div(p.V, step) - ceil_div(part, step) <= (top ? 2 : 4)) part = p.V;
   Plan plan{256, (int)ceil_div(p.V, part), (int)std::min<long long>(part, p.V), 0};
   plan.blocks = (unsigned)std::min<long long>(p.rows * plan.parts, most);
   return plan;
