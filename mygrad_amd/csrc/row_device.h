@@ -21,9 +21,12 @@ struct Piece {
     for (int n = 0; n < V; ++n) v[n] = n < count ? at[n] : otherwise;
     return v;
   }
+  // PAST: whole pieces do not stay in the last-level cache.
+  template <bool PAST = false>
   static __device__ __forceinline__ void store(T *at, long long count, const Held &v) {
     if (count >= V) {
-      *reinterpret_cast<Held *>(at) = v;
+      if (PAST) __builtin_nontemporal_store(v, reinterpret_cast<Held *>(at));
+      else *reinterpret_cast<Held *>(at) = v;
       return;
     }
 #pragma unroll

@@ -639,9 +639,18 @@ int over_rows(const Vocabulary &p, const void *logits, const End &end, void *top
 
 // ---- gradients --------------------------------------------------------------------------------------------------------------------
 // As many pieces of a row as a block has on their way together, or eight or sixteen threads or a wavefront per row.  The rows come in the order opposite to the forward
-// pass's: it has read the last of them last, and some of those are still near (4096 x 50000 halves, both passes 244 us and 246; distillation
-// over 32000 181 and 185).
-template <typename T, typename C, int LANES, bool ENTROPY>
+// pass's: it has read the last of them last, and some of those are still near (4096 x 50000 halves, both passes 214 us and 231; distillation
+// over 32000 144 and 153).
+//
+// PAST: a gradient that with its logits is more than the last-level cache (256 MB) holds is stored past it: what is stored there would have to go before
+// the next kernel's reads come in.  us of both passes, and with a pass over the gradient behind them: 262 MB of halves 155 and 212, past it 127 and 190;
+// 160 MB 84 and 123, 81 and 121; 128 MB 68 and 97, 66 and 99; 64 MB 37 and 52, 36 and 53.
+template <typename T>
+bool stores_past(const Vocabulary &p) {
+  return (double)p.rows * p.V * sizeof(T) > 1.5e8;
+}
+
+template <typename T, typename C, int LANES, bool ENTROPY, bool PAST>
 __global__ void __launch_bounds__(256) scores_bwd_kernel(Vocabulary p, int parts, const int32_t *__restrict__ ids, const T *__restrict__ logits,
                                                          const Row<C> *__restrict__ kept, const C *__restrict__ grad_scores,
                                                          const C *__restrict__ grad_entropy, T *__restrict__ dlogits) {
@@ -684,13 +693,13 @@ __global__ void __launch_bounds__(256) scores_bwd_kernel(Vocabulary p, int parts
         for (int n = 0; n < V; ++n)
           if (n == own) dz[n] = (T)(gradient(held[u][n]) + g);
       }
-      Piece<T>::store(out + d, p.V - d, dz);
+      Piece<T>::template store<PAST>(out + d, p.V - d, dz);
     }
   }
 }
 
 // The threads that share a row, or those of each wavefront, write the teacher's tokens among their own values once more; nobody waits for another.
-template <typename T, typename C, int LANES>
+template <typename T, typename C, int LANES, bool PAST>
 __global__ void __launch_bounds__(256) distillation_bwd_kernel(Vocabulary p, int parts, const int32_t *__restrict__ ids, const T *__restrict__ logits,
                                                                const Row<C> *__restrict__ kept, const C *__restrict__ shares,
                                                                const C *__restrict__ grad, T *__restrict__ dlogits) {
@@ -717,7 +726,7 @@ __global__ void __launch_bounds__(256) distillation_bwd_kernel(Vocabulary p, int
       Held dz;
 #pragma unroll
       for (int n = 0; n < V; ++n) dz[n] = nothing ? T(0) : (T)(g * (exponential<T>(((C)held[u][n] - row.m) * per) * inverse));
-      Piece<T>::store(out + d, p.V - d, dz);
+      Piece<T>::template store<PAST>(out + d, p.V - d, dz);
     }
     if (nothing) continue;
     wave_sees();  // the same memory again, by other lanes
@@ -753,6 +762,21 @@ int with_types(int dtype, F f) {
   if (dtype == MG_F64) return f((double *)nullptr, (double *)nullptr);
   if (dtype == MG_F32) return f((float *)nullptr, (float *)nullptr);
   return f((_Float16 *)nullptr, (float *)nullptr);
+}
+
+// Calls f with the number of threads that share a row of a gradient, of whose tokens a teacher names K.
+template <typename T, typename F>
+void with_lanes(int64_t V, int64_t K, F f) {
+  constexpr int one = Piece<T>::V * kAtOnce;
+  if (K <= 8 * kTurns && V <= 8 * one) f(std::integral_constant<int, 8>{});
+  else if (K <= 16 * kTurns && V <= 16 * one) f(std::integral_constant<int, 16>{});
+  else if (V <= 64 * one) f(std::integral_constant<int, 64>{});
+  else f(std::integral_constant<int, 256>{});
+}
+template <typename F>
+void with_bool(bool value, F f) {
+  if (value) f(std::true_type{});
+  else f(std::false_type{});
 }
 
 }  // namespace
@@ -798,19 +822,14 @@ int mg_log_probabilities_bwd(int dtype, int64_t rows, int64_t V, const int32_t *
     typedef std::remove_pointer_t<decltype(t)> T;
     typedef std::remove_pointer_t<decltype(c)> C;
     ScopedTiming timed(TAG_SCORES_BWD);
-    auto run = [&](auto lanes, auto with_entropy) {
+    auto run = [&](auto lanes, auto with_entropy, auto past) {
       const long long parts = ceil_div(V, lanes * Piece<T>::V * kAtOnce), blocks = lanes < 256 ? ceil_div(rows, 256 / lanes) : rows * parts;
-      scores_bwd_kernel<T, C, lanes, with_entropy><<<dim3((unsigned)std::min<long long>(blocks, 1 << 22)), dim3(256), 0, runtime().stream>>>(
+      scores_bwd_kernel<T, C, lanes, with_entropy, past><<<dim3((unsigned)std::min<long long>(blocks, 1 << 22)), dim3(256), 0, runtime().stream>>>(
           p, (int)parts, ids, (const T *)logits, (const Row<C> *)kept, (const C *)grad_scores, (const C *)grad_entropy, (T *)dlogits);
     };
-    auto by_length = [&](auto with_entropy) {
-      if (V <= 8 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 8>{}, with_entropy);
-      else if (V <= 16 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 16>{}, with_entropy);
-      else if (V <= 64 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 64>{}, with_entropy);
-      else run(std::integral_constant<int, 256>{}, with_entropy);
-    };
-    if (grad_entropy) by_length(std::true_type{});
-    else by_length(std::false_type{});
+    with_lanes<T>(V, 0, [&](auto lanes) {
+      with_bool(grad_entropy != nullptr, [&](auto with_entropy) { with_bool(stores_past<T>(p), [&](auto past) { run(lanes, with_entropy, past); }); });
+    });
     MG_HIP(hipGetLastError());
     return (int)MG_OK;
   });
@@ -848,15 +867,12 @@ int mg_distillation_bwd(int dtype, int64_t rows, int64_t V, int64_t K, double te
     typedef std::remove_pointer_t<decltype(t)> T;
     typedef std::remove_pointer_t<decltype(c)> C;
     ScopedTiming timed(TAG_DISTILLATION_BWD);
-    auto run = [&](auto lanes) {
+    auto run = [&](auto lanes, auto past) {
       const long long parts = ceil_div(V, lanes * Piece<T>::V * kAtOnce), blocks = lanes < 256 ? ceil_div(rows, 256 / lanes) : rows * parts;
-      distillation_bwd_kernel<T, C, lanes><<<dim3((unsigned)std::min<long long>(blocks, 1 << 22)), dim3(256), 0, runtime().stream>>>(
+      distillation_bwd_kernel<T, C, lanes, past><<<dim3((unsigned)std::min<long long>(blocks, 1 << 22)), dim3(256), 0, runtime().stream>>>(
           p, (int)parts, ids, (const T *)logits, (const Row<C> *)kept, (const C *)shares, (const C *)grad, (T *)dlogits);
     };
-    if (K <= 8 * kTurns && V <= 8 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 8>{});
-    else if (K <= 16 * kTurns && V <= 16 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 16>{});
-    else if (V <= 64 * Piece<T>::V * kAtOnce) run(std::integral_constant<int, 64>{});
-    else run(std::integral_constant<int, 256>{});
+    with_lanes<T>(V, K, [&](auto lanes) { with_bool(stores_past<T>(p), [&](auto past) { run(lanes, past); }); });
     MG_HIP(hipGetLastError());
     return (int)MG_OK;
   });

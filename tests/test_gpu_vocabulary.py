@@ -386,6 +386,22 @@ def test_a_teacher_on_the_device():
     assert np.abs(loss.data - want).max() < 1e-5 and np.abs(t.grad - dz).max() < 1e-6
 
 
+@pytest.mark.parametrize("vocabulary", [250, 1000, 40001])
+def test_gradients_of_many_logits_are_those_of_their_rows(vocabulary):
+    rows = 84_000_000 // vocabulary  # half of them are less than 150 MB
+    z = made(1000, vocabulary).astype(np.float16)[np.arange(rows) % 1000]
+    ids, (lists, teacher) = some(rows, vocabulary), lessons(1000, vocabulary, 7)
+    lists, teacher = lists[np.arange(rows) % 1000], teacher[np.arange(rows) % 1000].astype(np.float16)
+    for loss in (lambda t, at: log_probabilities(t, ids[at]), lambda t, at: distillation(t, lists[at], teacher[at])):
+        found = []
+        for at in (slice(None), slice(0, rows // 2), slice(rows // 2, None)):
+            t = mg.device_tensor(z[at])
+            loss(t, at).backward()
+            found.append(t.grad)
+        assert np.abs(found[0]).max() > 0
+        assert np.array_equal(found[0][: rows // 2], found[1]) and np.array_equal(found[0][rows // 2 :], found[2])
+
+
 def test_distillation_leading_shapes_and_empty_rows():
     z, (ids, teacher) = made(12, 50), lessons(12, 50, 4)
     flat = distillation(z, ids, teacher).data
