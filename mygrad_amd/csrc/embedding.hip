@@ -34,8 +34,10 @@ int lanes_of(long long pieces) {
   return lanes;
 }
 
-// A group of threads takes AT_ONCE tokens, whose rows are on their way together.
-template <typename T, int AT_ONCE>
+// A group of threads takes AT_ONCE tokens, whose rows are on their way together.  Where they are more than 60 MB they are stored past the last-level
+// cache (PAST), which the table has a better use for.  A table of 205 MB of halves, us alone, with a pass over the rows behind it, and with the gradient and passes
+// over both: 16384 rows of 2048 15, 32 and 155, past it 13, 32 and 150; 100000 rows 83, 213 and 459, 64, 165 and 411; 2000 rows 12, 22 and 95 either way.
+template <typename T, int AT_ONCE, bool PAST>
 __global__ void __launch_bounds__(256) embedding_kernel(Embedding p, int lanes, const int32_t *__restrict__ ids, const T *__restrict__ weight,
                                                         T *__restrict__ out) {
   typedef typename Piece<T>::Held Held;
@@ -57,7 +59,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(Embedding p, int lanes, 
       if (first + u >= p.tokens) break;
 #pragma unroll
       for (int n = 0; n < V; ++n) v[u][n] = id[u] < 0 ? T(0) : (T)((Scaled<T>)v[u][n] * (Scaled<T>)p.scale);
-      Piece<T>::store(out + (first + u) * p.D + d, p.D - d, v[u]);
+      Piece<T>::template store<PAST>(out + (first + u) * p.D + d, p.D - d, v[u]);
     }
   }
 }
@@ -471,7 +473,9 @@ int forward(const Embedding &p, const int32_t *ids, const void *weight, void *ou
   const int lanes = lanes_of(ceil_div(p.D, Piece<T>::V)), groups = 256 / lanes;
   // several rows a group where that leaves eight blocks a compute unit
   const bool many = p.tokens >= 4ll * groups * 8 * runtime().props.multiProcessorCount;
-  auto kernel = many ? embedding_kernel<T, 4> : embedding_kernel<T, 1>;
+  const bool past = (double)p.tokens * p.D * sizeof(T) > 6e7;
+  auto kernel = many ? past ? embedding_kernel<T, 4, true> : embedding_kernel<T, 4, false>
+                     : past ? embedding_kernel<T, 1, true> : embedding_kernel<T, 1, false>;
   kernel<<<dim3((unsigned)ceil_div(p.tokens, groups * (many ? 4 : 1))), dim3(256), 0, runtime().stream>>>(p, lanes, ids, (const T *)weight, (T *)out);
   MG_HIP(hipGetLastError());
   return MG_OK;

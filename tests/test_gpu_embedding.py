@@ -118,6 +118,16 @@ def test_rows_that_are_no_numbers_stay_alone(dtype):
     assert np.isinf(t.grad[4]).all() and np.array_equal(t.grad[:4], np.array([2, 0, 0, 2], dtype)[:, None] * np.ones(8, dtype))
 
 
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("count,dim", [(30011, 1001), (150001, 200), (1500, 20003), (4_000_001, 7)])
+def test_more_rows_than_caches_hold(dtype, count, dim):
+    rng = np.random.default_rng(dim)
+    weight, ids = rng.standard_normal((301, dim)).astype(dtype), rng.integers(-1, 301, count)
+    y = embedding(mg.device_tensor(weight, constant=True), ids).data
+    assert y.nbytes > 5e7 and np.array_equal(y[ids < 0], np.zeros_like(y[ids < 0]))
+    assert np.array_equal(y[ids >= 0], weight[ids[ids >= 0]])
+
+
 @pytest.mark.parametrize("count,vocabulary", [(3000, 50), (20000, 700)])
 def test_the_same_bits_every_time(count, vocabulary):
     rng = np.random.default_rng(0)
