@@ -35,7 +35,7 @@ int lanes_of(long long pieces) {
 }
 
 // A group of threads takes AT_ONCE tokens, whose rows are on their way together.  Where they are more than 60 MB they are stored past the last-level
-// cache (PAST), which the table has a better use for.  A table of 205 MB of halves, us alone, with a pass over the rows behind it, and with the gradient and passes
+// cache (PAST), which the table has a better use for.  The same table of 205 MB of halves each time, us alone, with a pass over the rows behind it, and with the gradient and passes
 // over both: 16384 rows of 2048 15, 32 and 155, past it 13, 32 and 150; 100000 rows 83, 213 and 459, 64, 165 and 411; 2000 rows 12, 22 and 95 either way.
 template <typename T, int AT_ONCE, bool PAST>
 __global__ void __launch_bounds__(256) embedding_kernel(Embedding p, int lanes, const int32_t *__restrict__ ids, const T *__restrict__ weight,
@@ -347,7 +347,7 @@ struct Runs {
   const unsigned *keys, *order;
 };
 
-// 16384 tokens of 50000 rows of 2048 halves: 35 us (67 MB read and 24 written, while what was filled leaves the caches for memory), and 8 for
+// 16384 tokens of 50000 rows of 2048 halves: 28 us (67 MB read and 24 written, while what was filled leaves the caches for memory), and 9 for
 // the join.  With eight rows on their way, and chunks of 32, it was half as much again.  Rows without tokens filled by this launch instead, from a
 // bit for each that the ordering left: 9 + 57 us where the two take 31 + 35, and 8 + 19 where they take 20 + 8 (1999 tokens of 32003 x 771 floats).
 //
