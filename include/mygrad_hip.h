@@ -492,15 +492,15 @@ int mg_head_norm_bwd(const mg_head_norm_desc *desc, const void *x, const void *w
 
 /* y = weight * (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps) + bias over the D values of each row; weight and bias (D,) may be null.
  * kept:(rows, 3), float32 (float64 for MG_F64), is for mg_layer_norm_bwd, and null where there will be none.  Fewer
- * than 2^31 rows, 2^24 where a row has more than 65536 bytes. */
+ * than 2^31 rows, 2^23 where a row has more than 65536 bytes. */
 int mg_layer_norm_fwd(int dtype, int64_t rows, int64_t D, double eps, const void *x, const void *weight, const void *bias, void *y, void *kept);
 
 /* Its gradients, like x, weight and bias; any of dx, dweight, dbias may be null (not wanted), not all three.  Run-to-run identical. */
 int mg_layer_norm_bwd(int dtype, int64_t rows, int64_t D, const void *x, const void *weight, const void *kept, const void *grad, void *dx,
                       void *dweight, void *dbias);
 
-/* out[n] = scale * weight[ids[n]], weight:(rows, D), out:(tokens, D); zeros for tokens that are none (or lie beyond the table).  At most
- * 2^26 tokens, 2^29 rows, 2^24 values a row; |scale| at most 1e30. */
+/* out[n] = scale * weight[ids[n]], weight:(rows, D), out:(tokens, D); zeros for tokens that are none (or lie beyond the table).  Fewer than
+ * 2^26 tokens, at most 2^29 rows, 2^24 values a row; |scale| at most 1e30. */
 int mg_embedding_fwd(int dtype, int64_t tokens, int64_t rows, int64_t D, double scale, const int32_t *ids, const void *weight, void *out);
 
 /* dweight[v] = scale * sum of the grad[n] with ids[n] = v: all rows of dweight:(rows, D) are written.  Run-to-run identical. */

@@ -462,7 +462,7 @@ int check(int dtype, int64_t tokens, int64_t rows, int64_t D, double scale, cons
   if (tokens < 0 || rows < 0 || D < 0 || !(std::fabs(scale) <= 1e30))  // single precision holds it
     return fail(MG_ERR_BAD_ARG, "%s: %lld tokens, a table of %lld rows of %lld values, scale %g", who, (long long)tokens, (long long)rows, (long long)D,
                 scale);
-  if (tokens > 1 << 26 || rows > 1 << 29 || D > 1 << 24)  // what the grids hold
+  if (tokens >= 1 << 26 || rows > 1 << 29 || D > 1 << 24)  // what the grids hold
     return fail(MG_ERR_UNSUPPORTED, "%s: %lld tokens, a table of %lld rows of %lld values", who, (long long)tokens, (long long)rows, (long long)D);
   return MG_OK;
 }

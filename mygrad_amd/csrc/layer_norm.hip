@@ -415,7 +415,7 @@ int forward(const LayerNorm &p, const void *x, const void *w, const void *b, voi
                                                                                                           (const T *)b, (T *)y, (Moments<C> *)kept);
     });
   } else {
-    if (p.rows >= 1 << 24) return fail(MG_ERR_UNSUPPORTED, "mg_layer_norm_fwd: %lld rows of %lld values", p.rows, p.D);  // a block each
+    if (p.rows >= 1 << 23) return fail(MG_ERR_UNSUPPORTED, "mg_layer_norm_fwd: %lld rows of %lld values", p.rows, p.D);  // a block each
     layer_norm_kernel<T, C><<<dim3((unsigned)p.rows), dim3(kLong), 0, s>>>(p, (const T *)x, (const T *)w, (const T *)b, (T *)y, (Moments<C> *)kept);
   }
   MG_HIP(hipGetLastError());
@@ -448,7 +448,7 @@ int backward(const LayerNorm &p, const void *x, const void *w, const void *kept,
     MG_HIP(hipGetLastError());
     return MG_OK;
   }
-  if (p.rows >= 1 << 24) return fail(MG_ERR_UNSUPPORTED, "mg_layer_norm_bwd: %lld rows of %lld values", p.rows, p.D);
+  if (p.rows >= 1 << 23) return fail(MG_ERR_UNSUPPORTED, "mg_layer_norm_bwd: %lld rows of %lld values", p.rows, p.D);
   const long long share = std::max<long long>(ceil_div(p.rows, 256), 16), shares = ceil_div(p.rows, share);
   if (columns)
     if (const int rc = workspace((size_t)(2 * shares * p.D) * sizeof(double), &space)) return rc;

@@ -223,7 +223,7 @@ def test_entry_points_refuse_bad_arguments():
 
     lib, p = _hip.lib(), _device.DeviceBuffer(1 << 16).ptr
     for status, (dtype, tokens, rows, dim, scale) in ((-2, (7, 2, 3, 8, 1.0)), (-1, (0, -1, 3, 8, 1.0)), (-1, (0, 2, -3, 8, 1.0)), (-1, (0, 2, 3, -8, 1.0)),
-                                                      (-1, (0, 2, 3, 8, float("inf"))), (-1, (0, 2, 3, 8, float("nan"))), (-2, (0, 1 << 31, 3, 8, 1.0)),
+                                                      (-1, (0, 2, 3, 8, float("inf"))), (-1, (0, 2, 3, 8, float("nan"))), (-2, (0, 1 << 31, 3, 8, 1.0)), (-2, (0, 1 << 26, 3, 8, 1.0)),
                                                       (-2, (0, 2, 1 << 31, 8, 1.0)), (-2, (0, 2, 3, 1 << 31, 1.0))):
         assert lib.mg_embedding_fwd(dtype, tokens, rows, dim, scale, p, p, p) == status
         assert lib.mg_embedding_bwd(dtype, tokens, rows, dim, scale, p, p, p) == status

@@ -150,3 +150,46 @@ def test_numbers_of_numpys_types():
     assert np.array_equal(embedding(x, np.array([0, 2], np.uint8), scale=np.int64(2)).data, x[[0, 2]] * 2)
     assert np.array_equal(log_probabilities(x, top=np.int64(2))[2].data, log_probabilities(x, top=2)[2].data)
     assert np.array_equal(*(distillation(x, [[0], [1], [2]], x[:, :1], temperature=t).data for t in (np.float32(2), 2)))
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32, np.float64])
+def test_arrays_of_any_order(dtype):
+    rng = np.random.default_rng(0)
+    whole, ids, lists = rng.standard_normal((14, 22)).astype(dtype), rng.integers(0, 11, (7, 2)), rng.integers(0, 11, (14, 5))
+    params, teacher = rng.standard_normal((11, 4)).astype(dtype), rng.standard_normal((14, 5)).astype(dtype)
+    views = [(whole[::2, ::-2], ids[:, 1], params[:, 1], params[:, 2], lists[::-2, 1:3], teacher[1::2, ::3]),
+             (np.asfortranarray(whole[:7, :11]), ids.T[0], params[::-1, 3], params[:, 0], np.asfortranarray(lists[:7]), np.asfortranarray(teacher[7:]))]
+    for x, tokens, w, b, which, taught in views:
+        for f in (lambda x, tokens, w, b, which, taught: layer_norm(x, w, b, eps=1e-3),
+                  lambda x, tokens, w, b, which, taught: embedding(x, tokens % 7),
+                  lambda x, tokens, w, b, which, taught: log_probabilities(x, tokens, entropy=True),
+                  lambda x, tokens, w, b, which, taught: distillation(x, which, taught, temperature=2.0)):
+            found = []
+            for arrays in ((x, tokens, w, b, which, taught), tuple(np.ascontiguousarray(a) for a in (x, tokens, w, b, which, taught))):
+                t, tw, tb = (mg.Tensor(arrays[n], copy=False) for n in (0, 2, 3))
+                y = f(t, arrays[1], tw, tb, *arrays[4:])
+                g = rng.standard_normal(y.shape).astype(y.dtype) if not found else found[-1]
+                y.backward(np.asfortranarray(g))
+                found += [[y.data] + [p.grad for p in (t, tw, tb) if p.grad is not None], g]
+            assert len(found[0]) == len(found[2]) and all(np.array_equal(a, c) for a, c in zip(found[0], found[2]))
+
+
+def test_one_tensor_in_several_places():
+    """Its gradients are added up: those of a row that is its own weight and bias, and those of a table that is looked up, normed and scored."""
+    rng = np.random.default_rng(1)
+    x, g = rng.standard_normal(33), rng.standard_normal(33)
+    t = mg.Tensor(x)
+    layer_norm(t, t, t, eps=1e-2).backward(g)
+    parts = ora.layer_norm(x, x, x, 1e-2, g)
+    assert np.abs(t.grad - (parts[1] + parts[2] + parts[3])).max() < 1e-12
+    table, ids = rng.standard_normal((9, 9)), rng.integers(0, 9, 6)
+    t = mg.Tensor(table)
+    log_probabilities(layer_norm(embedding(t, ids), t_row := mg.Tensor(table[0]), t_row, eps=1e-2), ids).backward()
+    first = t.grad.copy()
+    for n in range(9):
+        moved = []
+        for step in (1e-6, -1e-6):
+            other = table.copy()
+            other[ids[0], n] += step
+            moved.append(log_probabilities(layer_norm(embedding(other, ids), table[0], table[0], eps=1e-2), ids).data.sum())
+        assert abs((moved[0] - moved[1]) / 2e-6 - first[ids[0], n]) < 1e-7
