@@ -33,14 +33,14 @@ class LayerNorm(Operation):
             if len(_described) >= _MOST_SHAPES:
                 _described.clear()
             _described[key] = found
-        self._call, self._places, item = found
+        self._call, self._places, self._sizes, item = found
         self._empty = self._call[1] * self._call[2] == 0
         self._backed = None
         if self._empty:
             return np.empty(xd.shape, dtype=xd.dtype)
         held = [_device.to_device(v) for v in values]  # until the launch
         # behind the result, for the gradient: two parts of the mean and 1 / sqrt for each row
-        self._kept, behind = None, -(-xd.nbytes // 16) * 16
+        self._kept, behind = None, -(-self._sizes[0] // 16) * 16
         out = _device.DeviceBuffer(behind + 3 * self._call[1] * item)
         if not all([t.constant for t in self.variables]):
             self._kept = out.ptr + behind
@@ -53,7 +53,7 @@ class LayerNorm(Operation):
 
     @staticmethod
     def _describe(values, given, eps):
-        """The checked arguments of the entry points, where x, weight and bias are among the variables, and the size of a statistic."""
+        """The checked arguments of the entry points, where x, weight and bias are among the variables, the variables' bytes, and those of a statistic."""
         x = values[0]
         if x.ndim < 1:
             raise ValueError(f"`x` must have the axes (..., dim), got shape {x.shape}")
@@ -68,7 +68,7 @@ class LayerNorm(Operation):
         if not 0 <= eps < np.inf:
             raise ValueError(f"`eps` must be a non-negative number, got {eps}")
         places = 0, *(1 + given.index(name) if name in given else None for name in ("weight", "bias"))
-        return (_hip.storage_code(x.dtype), prod(x.shape[:-1]), dim), places, 8 if x.dtype == np.float64 else 4
+        return (_hip.storage_code(x.dtype), prod(x.shape[:-1]), dim), places, [v.nbytes for v in values], 8 if x.dtype == np.float64 else 4
 
     def _run_backward(self, grad, want):
         values = [_device.value_of(t) for t in self.variables]
@@ -77,7 +77,7 @@ class LayerNorm(Operation):
             raise NotImplementedError(f"layer_norm backward for gradient of shape {grad.shape} (no CPU fallback)")
         xb, gb = _device.to_device(x), _device.to_device(grad, x.dtype)
         wb = None if self._places[1] is None else _device.to_device(values[self._places[1]])
-        out = {i: _device.DeviceBuffer(values[i].nbytes) for i in want}
+        out = {i: _device.DeviceBuffer(self._sizes[i]) for i in want}
         _hip.check(_hip.lib().mg_layer_norm_bwd(*self._call, xb.ptr, None if wb is None else wb.ptr, self._kept, gb.ptr,
                                                 *(out[i].ptr if i in out else None for i in self._places)))
         return {i: _device.download(buf, values[i].shape, x.dtype) for i, buf in out.items()}

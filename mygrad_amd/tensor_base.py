@@ -67,7 +67,7 @@ class Tensor:
     def __init__(self, x, *, dtype=None, constant=None, copy=True, ndmin=0, _creator=None, _base=None):
         if constant is not None and not isinstance(constant, bool):
             raise TypeError(f"`constant` must be a boolean value, got: {constant}")
-        if not isinstance(ndmin, Integral):
+        if ndmin.__class__ is not int and not isinstance(ndmin, Integral):  # the second asks an abstract class
             raise TypeError(f"'{type(ndmin)}' object cannot be interpreted as an integer")
         if isinstance(x, Tensor):
             x = x._value if copy is False else x.data
@@ -227,9 +227,7 @@ class Tensor:
         until the operation is released; the result array is wrapped, not
         copied (reference: tensor_base.py:1086-1212).
         """
-        tensor_vars = tuple(
-            var if isinstance(var, Tensor) else cls(var, constant=True, copy=False) for var in input_vars
-        )
+        tensor_vars = tuple([var if isinstance(var, Tensor) else cls(var, constant=True, copy=False) for var in input_vars])
         _device.drop_pending()  # an offer left by an operation that was called directly has lapsed
         guarded = []
         guard = _graph.TRACK_GRAPH and _graph.MEM_GUARD
@@ -255,7 +253,11 @@ class Tensor:
                 v._grad = None  # a tensor that enters a new graph starts without a gradient
 
         if constant is None:
-            constant = None if any(not v.constant for v in tensor_vars) else True
+            constant = True
+            for v in tensor_vars:
+                if not v.constant:
+                    constant = None
+                    break
 
         ref_f = ReferenceType(f)
         for v in tensor_vars:
@@ -273,7 +275,7 @@ class Tensor:
             # values that are still on the device have no host array to lock yet: the tensor
             # remembers who holds it, and locks the array on their behalf when it is read
             for t in (*tensor_vars, out):
-                if t.on_device:
+                if isinstance(t._value, _device.DeviceArray):
                     # a device tensor that is never read on the host (a weight in a training loop)
                     # would collect one dead reference per operation: drop them as the list grows
                     if len(t._guards) >= 32:
