@@ -133,9 +133,9 @@ class Embedding(Operation):
         shape = self._tokens.shape + w.shape[1:]
         if 0 in shape:
             return np.empty(shape, dtype=w.dtype)
-        out = _device.DeviceBuffer(prod(shape) * w.dtype.itemsize)
+        out, wb = _device.DeviceBuffer(prod(shape) * w.dtype.itemsize), _device.to_device(w)  # until the launch
         _hip.check(_hip.lib().mg_embedding_fwd(_hip.storage_code(w.dtype), self._tokens.size, *w.shape, self._scale, self._tokens._buffer().ptr,
-                                               _device.to_device(w).ptr, out.ptr))
+                                               wb.ptr, out.ptr))
         y = _device.download(out, shape, w.dtype)
         _device.attach(y, out)
         return y
@@ -146,9 +146,9 @@ class Embedding(Operation):
             return np.zeros(w.shape, dtype=w.dtype)
         if grad.shape != self._tokens.shape + w.shape[1:]:
             raise NotImplementedError(f"embedding backward for gradient of shape {grad.shape} (no CPU fallback)")
-        out = _device.DeviceBuffer(w.nbytes)
+        out, gb = _device.DeviceBuffer(w.nbytes), _device.to_device(grad, w.dtype)
         _hip.check(_hip.lib().mg_embedding_bwd(_hip.storage_code(w.dtype), self._tokens.size, *w.shape, self._scale, self._tokens._buffer().ptr,
-                                               _device.to_device(grad, w.dtype).ptr, out.ptr))
+                                               gb.ptr, out.ptr))
         return _device.download(out, w.shape, w.dtype)
 
 

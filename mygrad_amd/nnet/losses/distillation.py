@@ -46,11 +46,11 @@ class Distillation(Operation):
         self._empty = rows == 0
         if self._empty:
             return np.empty(lead, dtype=self._dtype)
-        yb = _device.to_device(y, None if taught == y.dtype else taught)
+        zb, yb = _device.to_device(z), _device.to_device(y, None if taught == y.dtype else taught)  # until the launch
         out = _device.DeviceBuffer(rows * item)
         # what the gradient needs of a row: three statistics and the shares of its tokens
         self._kept = None if logits.constant else _device.DeviceBuffer((3 + count) * rows * item)
-        _hip.check(_hip.lib().mg_distillation_fwd(self._code, _hip.storage_code(taught), *self._call, _device.to_device(z).ptr, tokens._buffer().ptr,
+        _hip.check(_hip.lib().mg_distillation_fwd(self._code, _hip.storage_code(taught), *self._call, zb.ptr, tokens._buffer().ptr,
                                                   yb.ptr, out.ptr, *self._both()))
         loss = _device.download(out, lead, self._dtype)
         _device.attach(loss, out)
@@ -89,9 +89,9 @@ class Distillation(Operation):
             return np.zeros(z.shape, dtype=z.dtype)
         if grad.shape != z.shape[:-1]:
             raise NotImplementedError(f"distillation backward for gradient of shape {grad.shape} (no CPU fallback)")
-        out = _device.DeviceBuffer(z.nbytes)
-        _hip.check(_hip.lib().mg_distillation_bwd(self._code, *self._call, _device.to_device(z).ptr, self._tokens._buffer().ptr, *self._both(),
-                                                  _device.to_device(grad, self._dtype).ptr, out.ptr))
+        out, zb, gb = _device.DeviceBuffer(z.nbytes), _device.to_device(z), _device.to_device(grad, self._dtype)
+        _hip.check(_hip.lib().mg_distillation_bwd(self._code, *self._call, zb.ptr, self._tokens._buffer().ptr, *self._both(),
+                                                  gb.ptr, out.ptr))
         return _device.download(out, z.shape, z.dtype)
 
 

@@ -69,7 +69,8 @@ class _Plan:
             count = self.rows * self.top
             top = (_device.DeviceArray(_device.DeviceBuffer(count * self.dtype.itemsize), self.alternatives, self.dtype),
                    _device.DeviceArray(_device.DeviceBuffer(count * 4), self.alternatives, np.int32))
-        _hip.check(_hip.lib().mg_log_probabilities_fwd(self.code, self.rows, self.vocabulary, self.top, ids, _device.to_device(z).ptr,
+        zb = _device.to_device(z)  # until the launch
+        _hip.check(_hip.lib().mg_log_probabilities_fwd(self.code, self.rows, self.vocabulary, self.top, ids, zb.ptr,
                                                        *((None, None) if out is None else self.planes(out.ptr)), kept,
                                                        *((top[0].buf.ptr, top[1].buf.ptr) if top else (None, None))))
         return out, top
@@ -120,10 +121,10 @@ class LogProbabilities(Operation):
             return np.zeros(z.shape, dtype=z.dtype)
         if grad.shape != plan.shape:
             raise NotImplementedError(f"log_probabilities backward for gradient of shape {grad.shape} (no CPU fallback)")
-        gb = _device.to_device(grad, plan.dtype)
+        zb, gb = _device.to_device(z), _device.to_device(grad, plan.dtype)
         out = _device.DeviceBuffer(z.nbytes)
         ids = None if self._tokens is None else self._tokens._buffer().ptr
-        _hip.check(_hip.lib().mg_log_probabilities_bwd(plan.code, plan.rows, plan.vocabulary, ids, _device.to_device(z).ptr, self._kept.ptr + plan.nbytes,
+        _hip.check(_hip.lib().mg_log_probabilities_bwd(plan.code, plan.rows, plan.vocabulary, ids, zb.ptr, self._kept.ptr + plan.nbytes,
                                                        *plan.planes(gb.ptr), out.ptr))
         return _device.download(out, z.shape, z.dtype)
 

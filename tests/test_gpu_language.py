@@ -193,3 +193,31 @@ def test_one_tensor_in_several_places():
             other[ids[0], n] += step
             moved.append(log_probabilities(layer_norm(embedding(other, ids), table[0], table[0], eps=1e-2), ids).data.sum())
         assert abs((moved[0] - moved[1]) / 2e-6 - first[ids[0], n]) < 1e-7
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32, np.float64])
+def test_results_without_a_graph(dtype):
+    """Arrays that no graph holds are sent for one call; operands of the same size do not take one another's place."""
+    rng = np.random.default_rng(3)
+    for rows, width in ((64, 8), (300, 1), (7, 33)):
+        x, w, ids = rng.standard_normal((rows, width)).astype(dtype), rng.standard_normal(width).astype(dtype), rng.integers(0, width, rows)
+        lists = rng.integers(0, width, (rows, width * x.itemsize // 4 or 1))
+        teacher = rng.standard_normal(lists.shape).astype(dtype)
+        for f in (lambda: layer_norm(x, w, w, eps=1e-3), lambda: embedding(x, ids % rows), lambda: log_probabilities(x, ids, entropy=True),
+                  lambda: log_probabilities(x, top=1)[1], lambda: distillation(x, lists, teacher), lambda: distillation(x, lists, teacher, temperature=3)):
+            with_graph = f().data.copy()
+            with mg.no_autodiff:
+                assert np.array_equal(f().data, with_graph)
+            with mg.mem_guard_off:
+                assert np.array_equal(f().data, with_graph)
+        g = rng.standard_normal(rows)
+        grads = []
+        for switch in (mg.mem_guard_on, mg.mem_guard_off):
+            with switch:
+                for f in (lambda t: layer_norm(t, w, w, eps=1e-3), lambda t: embedding(t, ids % rows), lambda t: log_probabilities(t, ids),
+                          lambda t: distillation(t, lists, teacher)):
+                    t = mg.Tensor(x.copy())
+                    y = f(t)
+                    y.backward(g if y.ndim == 1 else g[:, None] * np.ones(width))
+                    grads.append(t.grad)
+        assert all(np.array_equal(a, b) for a, b in zip(grads[:4], grads[4:]))

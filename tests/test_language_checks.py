@@ -133,6 +133,58 @@ print("sent once")
     assert "sent once" in run_on_standins(tmp_path, program)
 
 
+def test_operands_live_until_the_launch(tmp_path):
+    """What is sent for one call only (arrays that no graph holds, casts) is not given back, and so not given to the next who asks, before the call."""
+    program = """
+import weakref
+import numpy as np
+import mygrad_amd as mg
+from mygrad_amd import _device, _hip
+from mygrad_amd.nnet import distillation, embedding, layer_norm, log_probabilities
+lib, live, seen = _hip.lib(), weakref.WeakSet(), set()
+made = _device.DeviceBuffer.__init__
+def init(self, nbytes):
+    made(self, nbytes)
+    live.add(self)
+_device.DeviceBuffer.__init__ = init
+class Watched:
+    def __getattr__(self, name):
+        f = getattr(lib, name)
+        if not name.endswith(("_fwd", "_bwd")):
+            return f
+        def call(*args):
+            held = [(b.ptr, b.ptr + max(b.nbytes, 1)) for b in live if b._owned is not None]
+            for n, arg in enumerate(args):
+                assert not isinstance(arg, int) or arg < 1 << 20 or any(first <= arg < end for first, end in held), (name, n)
+            seen.add(name)
+            return f(*args)
+        return call
+_hip._lib = Watched()
+rng = np.random.default_rng(0)
+for dtype in (np.float16, np.float32, np.float64):
+    x, w, ids, lists = np.ones((6, 4), dtype), np.ones(4, dtype), np.zeros(6, int), np.zeros((6, 4), int)
+    teacher = np.ones((6, 4), np.float16)
+    calls = (lambda x: embedding(x, ids), lambda x: layer_norm(x, w, w, eps=1e-5), lambda x: log_probabilities(x, ids, entropy=True, top=2)[0],
+             lambda x: log_probabilities(x, top=2)[1], lambda x: distillation(x, lists, teacher))
+    for f in calls:
+        with mg.no_autodiff:
+            f(x)
+        f(x)
+        for switch in (mg.mem_guard_off, mg.mem_guard_on):
+            with switch:
+                t = mg.tensor(x)
+                y = f(t)
+                if not y.constant:
+                    y.backward(np.ones(y.shape, np.float64))
+                    assert t.grad.shape == x.shape
+                    y = f(t)
+                    y.backward(mg.device_tensor(np.ones(y.shape, y.dtype), constant=True))
+assert len(seen) == 8, seen
+print("live")
+"""
+    assert "live" in run_on_standins(tmp_path, program)
+
+
 # ------------------------------------------------------------------------------------------------------------------- the oracle
 def test_the_oracles_gradients_by_differences():
     rng = np.random.default_rng(0)
