@@ -1,7 +1,10 @@
 // Layer norm and its gradient for gfx950.
 //
 //   mu = mean x     d = x - mu     r = 1 / sqrt(mean(d^2) + eps)     n = d r     y = w n + b     (over the D values of a row)
-//   u = w grad      dx = r (u - mean(u) - n mean(u n))               dw = sum grad n             db = sum grad   (over the rows)
+//   u = r w grad    dx = u - mean(u) - n r mean(u d)                 dw = sum grad n             db = sum grad   (over the rows)
+//
+// Behind a row's end threads go on with x = 0 and grad = 0.  There n may be infinite (in a row of equal values far from zero, whose r is that of
+// eps alone), and grad n no number; u and d are numbers, and u d is 0.
 //
 // The mean is taken twice: x - mean is exact to a unit of itself where a row lies far from zero, so the mean of what is left, and the
 // variance around it, are those of the row to single precision whatever its offset.  The forward pass keeps both parts and r, three
@@ -91,18 +94,18 @@ __global__ void __launch_bounds__(kLong) layer_norm_dx_kernel(LayerNorm p, const
   const T *row = x + blockIdx.x * p.D, *g = grad + blockIdx.x * p.D;
   const Moments<C> m = kept[blockIdx.x];
   C sums[2] = {0, 0};
-  auto each = [&](long long d, int count, auto f) {  // behind the row's end g is 0
+  auto each = [&](long long d, int count, auto f) {  // u and x - mean; behind the row's end u is 0
     const Held xs = Piece<T>::load(row + d, count, T(0)), gs = Piece<T>::load(g + d, count, T(0));
     const Held weight = w ? Piece<T>::load(w + d, count, T(0)) : Held{};
 #pragma unroll
-    for (int n = 0; n < Piece<T>::V; ++n) f(n, (C)gs[n] * (w ? (C)weight[n] : C(1)), ((C)xs[n] - m.shift - m.mean) * m.r);
+    for (int n = 0; n < Piece<T>::V; ++n) f(n, (C)gs[n] * (w ? (C)weight[n] : C(1)) * m.r, (C)xs[n] - m.shift - m.mean);
   };
-  over_row<T>(p, [&](long long d, int count) { each(d, count, [&](int, C u, C n) { sums[0] += u, sums[1] += u * n; }); });
+  over_row<T>(p, [&](long long d, int count) { each(d, count, [&](int, C u, C t) { sums[0] += u, sums[1] += u * t; }); });
   block_add(sums, space);
-  const C first = sums[0] / (C)p.D, second = sums[1] / (C)p.D;
+  const C first = sums[0] / (C)p.D, second = m.r * (sums[1] / (C)p.D);
   over_row<T>(p, [&](long long d, int count) {
     Held out;
-    each(d, count, [&](int k, C u, C n) { out[k] = (T)(m.r * (u - first - n * second)); });
+    each(d, count, [&](int k, C u, C t) { out[k] = (T)(u - first - t * m.r * second); });
     Piece<T>::store(dx + blockIdx.x * p.D + d, count, out);
   });
 }
@@ -278,21 +281,21 @@ __global__ void __launch_bounds__(kThreads<WAVES>) layer_norm_rows_bwd_kernel(La
       for (int u = 0; u < N; ++u)
 #pragma unroll
         for (int n = 0; n < V; ++n) {
-          const C g = (C)gs[u][n], t = ((C)xs[u][n] - m.shift - m.mean) * m.r;  // behind the row's end g is 0
+          const C g = (C)gs[u][n], d = (C)xs[u][n] - m.shift - m.mean, t = d * m.r;
           v[u][n] = t;
-          u_of[u][n] = w ? g * (C)weight[u][n] : g;
-          first += u_of[u][n], second += u_of[u][n] * t;
+          u_of[u][n] = (w ? g * (C)weight[u][n] : g) * m.r;
+          first += u_of[u][n], second += u_of[u][n] * d;
           dw[u][n] += g * t, db[u][n] += g;
         }
       load(row + stride);  // the next row is on its way during the sums
       if (dx) {
         rows.add(first, second, lanes);
-        first /= (C)p.D, second /= (C)p.D;
+        first /= (C)p.D, second = m.r * (second / (C)p.D);
 #pragma unroll
         for (int u = 0; u < N; ++u) {
           Held out;
 #pragma unroll
-          for (int n = 0; n < V; ++n) out[n] = (T)(m.r * (u_of[u][n] - first - v[u][n] * second));
+          for (int n = 0; n < V; ++n) out[n] = (T)(u_of[u][n] - first - v[u][n] * second);
           const int d = d0 + u * step;
           if (here) Piece<T>::store(dx + row * p.D + d, p.D - d, out);
         }
@@ -304,20 +307,20 @@ __global__ void __launch_bounds__(kThreads<WAVES>) layer_norm_rows_bwd_kernel(La
       for (int u = 0; u < N; ++u)
 #pragma unroll
         for (int n = 0; n < V; ++n) {
-          const C g = (C)gs[u][n], t = ((C)xs[u][n] - m.shift - m.mean) * m.r, uw = w ? g * (C)weight[u][n] : g;
-          first += uw, second += uw * t;
-          dw[u][n] += g * t, db[u][n] += g;
+          const C g = (C)gs[u][n], d = (C)xs[u][n] - m.shift - m.mean, ur = (w ? g * (C)weight[u][n] : g) * m.r;
+          first += ur, second += ur * d;
+          dw[u][n] += g * (d * m.r), db[u][n] += g;
         }
       if (dx) {
         rows.add(first, second, lanes);
-        first /= (C)p.D, second /= (C)p.D;
+        first /= (C)p.D, second = m.r * (second / (C)p.D);
 #pragma unroll
         for (int u = 0; u < N; ++u) {
           Held out;
 #pragma unroll
           for (int n = 0; n < V; ++n) {
             const C g = (C)gs[u][n], t = ((C)xs[u][n] - m.shift - m.mean) * m.r;
-            out[n] = (T)(m.r * ((w ? g * (C)weight[u][n] : g) - first - t * second));
+            out[n] = (T)((w ? g * (C)weight[u][n] : g) * m.r - first - t * second);
           }
           const int d = d0 + u * step;
           if (here) Piece<T>::store(dx + row * p.D + d, p.D - d, out);

@@ -112,6 +112,26 @@ def test_rows_of_one_value_throughout(dtype):
         assert not y.data.any() and np.abs(x.grad).max() <= 400 * (dim / 16 + 16) * UNIT[dtype][0]
 
 
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("weight", [False, True])
+@pytest.mark.parametrize("dim", [1, 5, 20, 300, 1030, 2053, 4100, 9001, 16390, 40000, 40001])
+def test_gradients_of_rows_of_one_value_far_from_zero(dtype, weight, dim):
+    """What lies behind a row's end has no part in its sums, where the mean over the square root of eps (2^50) is beyond the type, too.  Norms are
+    exactly 0; a mean of v = w grad is off by (D / 16 + 16) u of the mean of |v|, and what comes of it by 4 u of its parts."""
+    u, r, chain, rng = *UNIT[dtype], dim / 16 + 16, np.random.default_rng(dim)
+    value, g = dtype(2.0**80 if dtype == np.float32 else 2.0**1000), rng.standard_normal((4, dim)).astype(dtype)
+    w = (1 + 0.3 * rng.standard_normal(dim)).astype(dtype) if weight else np.ones(dim, dtype)
+    x, tw, tb = mg.device_tensor(np.full((4, dim), value)), mg.device_tensor(w) if weight else None, mg.device_tensor(np.zeros(dim, dtype))
+    y = layer_norm(x, tw, tb, eps=2.0**-100)
+    y.backward(mg.device_tensor(g, constant=True))
+    v = g.astype(ora.WIDE) * w
+    size = np.abs(v).mean(-1, keepdims=True)
+    want = 2.0**50 * (v - v.mean(-1, keepdims=True))
+    assert not y.data.any() and (tw is None or not tw.grad.any())
+    assert outside(x.grad, want, 2.0**50 * ((chain + 4) * u * size + 4 * u * (np.abs(v) + size)) + r * np.abs(want)) == 0
+    assert outside(tb.grad, g.astype(ora.WIDE).sum(0), 20 * u * np.abs(g).sum(0)) == 0
+
+
 @pytest.mark.parametrize("dim", [64, 1000, 20000])
 def test_rows_that_are_no_numbers_stay_alone(dim):
     rng = np.random.default_rng(dim)
