@@ -476,8 +476,14 @@ int forward(const Embedding &p, const int32_t *ids, const void *weight, void *ou
   const bool past = (double)p.tokens * p.D * sizeof(T) > 6e7;
   auto kernel = many ? past ? embedding_kernel<T, 4, true> : embedding_kernel<T, 4, false>
                      : past ? embedding_kernel<T, 1, true> : embedding_kernel<T, 1, false>;
-  kernel<<<dim3((unsigned)ceil_div(p.tokens, groups * (many ? 4 : 1))), dim3(256), 0, runtime().stream>>>(p, lanes, ids, (const T *)weight, (T *)out);
-  MG_HIP(hipGetLastError());
+  // A launch has fewer than 2^32 threads; rows that a block takes four of at a time reach that with 2^26 - 3 tokens.
+  const long long at_once = groups * (many ? 4 : 1), most = ((1ll << 24) - 1) * at_once;
+  for (long long at = 0; at < p.tokens; at += most) {
+    Embedding part = p;
+    part.tokens = std::min(p.tokens - at, most);
+    kernel<<<dim3((unsigned)ceil_div(part.tokens, at_once)), dim3(256), 0, runtime().stream>>>(part, lanes, ids + at, (const T *)weight, (T *)out + at * p.D);
+    MG_HIP(hipGetLastError());
+  }
   return MG_OK;
 }
 

@@ -8,6 +8,12 @@
 
 namespace {
 int events_made = 0, blocks_refused = 0;
+hipError_t last_error = hipSuccess;
+struct {
+  dim3 grid, block;
+  size_t shared;
+  hipStream_t stream;
+} configuration;
 }
 
 extern "C" {
@@ -22,7 +28,10 @@ hipError_t hipGetDevicePropertiesR0600(hipDeviceProp_tR0600 *props, int) {
   return hipSuccess;
 }
 hipError_t hipGetSymbolAddress(void **ptr, const void *) { return *ptr = malloc(1 << 20), hipSuccess; }
-hipError_t hipGetLastError() { return hipSuccess; }
+hipError_t hipGetLastError() {
+  const hipError_t error = last_error;
+  return last_error = hipSuccess, error;
+}
 hipError_t hipStreamCreateWithFlags(hipStream_t *stream, unsigned) { return *stream = reinterpret_cast<hipStream_t>(1), hipSuccess; }
 hipError_t hipStreamDestroy(hipStream_t) { return hipSuccess; }
 hipError_t hipStreamSynchronize(hipStream_t) { return hipSuccess; }
@@ -38,7 +47,15 @@ hipError_t hipHostMalloc(void **ptr, size_t size, unsigned) { return *ptr = mall
 hipError_t hipHostFree(void *ptr) { return free(ptr), hipSuccess; }
 hipError_t hipMemcpy(void *dst, const void *src, size_t size, hipMemcpyKind) { return memcpy(dst, src, size), hipSuccess; }
 hipError_t hipMemcpyAsync(void *dst, const void *src, size_t size, hipMemcpyKind, hipStream_t) { return memcpy(dst, src, size), hipSuccess; }
-hipError_t hipLaunchKernel(const void *, dim3, dim3, void **, size_t, hipStream_t) { return hipSuccess; }
+hipError_t __hipPushCallConfiguration(dim3 grid, dim3 block, size_t shared, hipStream_t stream) { return configuration = {grid, block, shared, stream}, hipSuccess; }
+hipError_t __hipPopCallConfiguration(dim3 *grid, dim3 *block, size_t *shared, hipStream_t *stream) {
+  return *grid = configuration.grid, *block = configuration.block, *shared = configuration.shared, *stream = configuration.stream, hipSuccess;
+}
+// As the runtime, it refuses a launch of 2^32 threads or more along an axis.
+hipError_t hipLaunchKernel(const void *, dim3 grid, dim3 block, void **, size_t, hipStream_t) {
+  const auto fits = [](unsigned blocks, unsigned threads) { return (unsigned long long)blocks * threads < 1ull << 32; };
+  return last_error = fits(grid.x, block.x) && fits(grid.y, block.y) && fits(grid.z, block.z) ? hipSuccess : hipErrorInvalidConfiguration;
+}
 // STANDIN_FAIL_EVENT=n: the n-th event cannot be made
 hipError_t hipEventCreateWithFlags(hipEvent_t *event, unsigned) {
   const char *fail = getenv("STANDIN_FAIL_EVENT");

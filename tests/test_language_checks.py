@@ -185,6 +185,22 @@ print("live")
     assert "live" in run_on_standins(tmp_path, program)
 
 
+def test_as_many_tokens_as_are_allowed_fit_the_grids(tmp_path):
+    """A lookup of long rows takes a block of 256 threads for four tokens, and a launch has fewer than 2^32 threads."""
+    program = """
+from mygrad_amd import _device, _hip
+lib, p = _hip.lib(), _device.DeviceBuffer(1 << 16).ptr
+for dtype in (0, 1, 2):
+    for dim in (1, 700, 4096, 1 << 24):
+        for tokens in ((1 << 26) - 5, (1 << 26) - 4, (1 << 26) - 3, (1 << 26) - 1):
+            assert lib.mg_embedding_fwd(dtype, tokens, 3, dim, 1.0, p, p, p) == 0, (dtype, dim, tokens)
+        assert lib.mg_embedding_fwd(dtype, 1 << 26, 3, dim, 1.0, p, p, p) == -2
+    assert lib.mg_embedding_bwd(dtype, (1 << 26) - 1, 3, 1, 1.0, p, p, p) == 0
+print("they fit")
+"""
+    assert "they fit" in run_on_standins(tmp_path, program)
+
+
 # ------------------------------------------------------------------------------------------------------------------- the oracle
 def test_the_oracles_gradients_by_differences():
     rng = np.random.default_rng(0)
