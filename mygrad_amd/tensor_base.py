@@ -59,6 +59,29 @@ def device_tensor(x, *, dtype=None, constant=None):
     return Tensor(_device.DeviceArray(buf, arr.shape, arr.dtype), constant=constant, copy=False)
 
 
+class _References(list):
+    """Weak references to operations.
+
+    A tensor that is only ever read (a constant, weights that a model answers with) is never cleared, and would collect one dead reference
+    per operation.  Before there are more than ``most``, dead ones are dropped and ``most`` becomes twice the number of what is left: what is looked
+    through stays a fixed number for each operation, however many live.  (No set: dead references hash alike where their operations
+    lay in the same memory one after another.)
+    """
+
+    __slots__ = ("most",)
+
+    def __init__(self):
+        self.most = 32
+
+    def drop_dead(self):
+        self[:] = [ref for ref in self if ref() is not None]
+        self.most = max(32, 2 * len(self))
+
+    def clear(self):
+        self.most = 32
+        list.clear(self)
+
+
 class Tensor:
     """An N-dimensional array that remembers the operation that produced it."""
 
@@ -72,7 +95,7 @@ class Tensor:
         if isinstance(x, Tensor):
             x = x._value if copy is False else x.data
         self._creator = _creator
-        self._guards = []  # weak references to the operations that hold this tensor's value read-only
+        self._guards = _References()  # to the operations that hold this tensor's value read-only
         if isinstance(x, _device.DeviceArray) and copy is False and not ndmin and (dtype is None or np.dtype(dtype) == x.dtype):
             data = x  # a result that stays on the device until it is read
         elif copy is False:
@@ -94,7 +117,7 @@ class Tensor:
                 raise ValueError("Integer-valued tensors must be treated as constants.")
         self._constant = (not is_float) if constant is None else constant
         self._grad = None
-        self._ops = set()  # weak references to the operations this tensor feeds
+        self._ops = _References()  # to the operations this tensor feeds
         self._base = _base
 
     # ------------------------------------------------------------------ array-like surface
@@ -118,7 +141,7 @@ class Tensor:
         arr = dev.host()
         self._value = arr
         holders = [op for op in (ref() for ref in self._guards) if op is not None and op._guarded is not None]
-        self._guards = []
+        self._guards.clear()
         if holders:
             # the graph is alive: the host copy is held read-only like any other array of the
             # graph, which is also what keeps the device buffer a valid copy of it
@@ -261,11 +284,10 @@ class Tensor:
 
         ref_f = ReferenceType(f)
         for v in tensor_vars:
-            # a tensor that is only ever read (a constant, weights that a model answers with) is never cleared: without this it would
-            # collect one dead reference per operation, which hash alike where the operations lie in the same memory one after another
-            if len(v._ops) >= 32:
-                v._ops = {ref for ref in v._ops if ref() is not None}
-            v._ops.add(ref_f)
+            ops = v._ops
+            if len(ops) >= ops.most:
+                ops.drop_dead()
+            ops.append(ref_f)
 
         out = cls(op_out, constant=constant, copy=False, _creator=f)
 
@@ -276,11 +298,10 @@ class Tensor:
             # remembers who holds it, and locks the array on their behalf when it is read
             for t in (*tensor_vars, out):
                 if isinstance(t._value, _device.DeviceArray):
-                    # a device tensor that is never read on the host (a weight in a training loop)
-                    # would collect one dead reference per operation: drop them as the list grows
-                    if len(t._guards) >= 32:
-                        t._guards = [ref for ref in t._guards if ref() is not None]
-                    t._guards.append(ref_f)
+                    guards = t._guards
+                    if len(guards) >= guards.most:
+                        guards.drop_dead()
+                    guards.append(ref_f)
             if guarded:  # else nothing is to be released yet: what is read later sees to it (a finalizer costs 3 us)
                 finalize(f, _graph.release, guarded)
         _device.drop_pending()

@@ -250,6 +250,39 @@ print("dropped")
     assert "dropped" in run_on_standins(tmp_path, program)
 
 
+def test_a_tensor_that_feeds_many_live_operations(tmp_path):
+    """What is looked through for dead references grows with the number of operations, not with its square; dropping them goes on once there are some."""
+    program = """
+import weakref
+import numpy as np
+import mygrad_amd as mg
+from mygrad_amd import tensor_base
+from mygrad_amd.nnet import embedding
+looked = [0]
+class Counted(weakref.ref):
+    def __call__(self):
+        looked[0] += 1
+        return super().__call__()
+tensor_base.ReferenceType = Counted
+for weight in (mg.device_tensor(np.ones((4, 8), np.float32)), mg.tensor(np.ones((4, 8), np.float32))):
+    looked[0], live = 0, []
+    for n in range(3000):
+        live.append(embedding(weight, [n % 4]))
+    assert looked[0] <= 4 * 3000, looked  # the tensor's operations and those that hold it read-only, less than twice each
+    assert {out.creator for out in live} <= {ref() for ref in weight._ops}
+    looked[0] = 0
+    for n in range(9000):
+        embedding(weight, [1])
+    assert len(weight._ops) <= 6000 and len(weight._guards) <= 6000 and looked[0] <= 4 * 9000, (len(weight._ops), looked)
+    del live
+    for n in range(9000):
+        embedding(weight, [1])
+    assert len(weight._ops) <= 32 and len(weight._guards) <= 32
+print("counted")
+"""
+    assert "counted" in run_on_standins(tmp_path, program)
+
+
 def test_arrays_read_from_a_live_graph_are_released_with_it(tmp_path):
     """Where all operands lie on the device, nothing is held until somebody reads them; then until the operation is gone."""
     program = """
