@@ -32,7 +32,7 @@ class Distillation(Operation):
         if _graph.TRACK_GRAPH and not teacher.constant:
             raise ValueError("the teacher's logits have no gradient: they must be a constant")
         tokens = self._tokens = tokens if isinstance(tokens, TokenIds) else TokenIds(tokens)
-        key = z.shape, z.dtype, y.shape, y.dtype, tokens.shape, temperature
+        key = z.shape, z.dtype, y.shape, y.dtype, tokens.shape, temperature, type(temperature)
         found = _described.get(key)
         if found is None:
             found = self._describe(z, y, tokens, temperature)

@@ -98,6 +98,35 @@ def test_a_refused_call_leaves_arrays_writeable():
     w[0, 0] = z[0, 0] = 2
 
 
+def test_what_is_refused_does_not_hang_on_the_calls_before(tmp_path):
+    """Numbers of other types are equal to those of a call that was checked, and have its hash."""
+    program = """
+from decimal import Decimal
+from fractions import Fraction
+import numpy as np
+import mygrad_amd as mg
+from mygrad_amd.nnet import distillation, layer_norm, log_probabilities
+z, ids, teacher = np.ones((2, 9), np.float32), np.zeros((2, 3), int), np.ones((2, 3), np.float32)
+def refused(f):
+    try:
+        f()
+    except (TypeError, ValueError) as error:
+        return type(error)
+for once in range(2):
+    assert refused(lambda: distillation(z, ids, teacher, temperature=Decimal(2))) is ValueError
+    assert refused(lambda: distillation(z, ids, teacher, temperature=2 + 0j)) is ValueError
+    assert refused(lambda: layer_norm(z, eps=0.5 + 0j)) is TypeError
+    assert refused(lambda: log_probabilities(z, top=2.0)) is ValueError and refused(lambda: log_probabilities(z, entropy=1)) is TypeError
+    assert refused(lambda: log_probabilities(z, top=Fraction(2))) is ValueError
+    for fits in (2.0, 2, np.float32(2), Fraction(2)):
+        distillation(z, ids, teacher, temperature=fits)
+    layer_norm(z, eps=0.5)
+    log_probabilities(z, entropy=True, top=2)
+print("the same")
+"""
+    assert "the same" in run_on_standins(tmp_path, program)
+
+
 def test_one_upload_of_tokens_and_of_what_they_go_with(tmp_path):
     """Tokens are sent once, whoever takes them; what a backward pass needs is kept for those that have one."""
     program = """
