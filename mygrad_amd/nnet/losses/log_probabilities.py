@@ -181,6 +181,8 @@ def log_probabilities(logits, tokens=None, *, entropy: bool = False, top: int = 
         if not top:
             return out
     else:  # nothing that has a gradient
+        if constant is not None and not isinstance(constant, bool):
+            raise TypeError(f"`constant` must be a boolean value, got: {constant}")
         z = _device.value_of(logits if isinstance(logits, Tensor) else Tensor(logits, constant=True, copy=False))
         plan, out = _plan(z, None, entropy, top), None
         alternatives += plan.no_alternatives() if plan.empty else plan.run(z, None, False)[1]

@@ -127,6 +127,26 @@ print("the same")
     assert "the same" in run_on_standins(tmp_path, program)
 
 
+def test_alternatives_alone_refuse_a_constant_that_is_none(tmp_path):
+    program = """
+import numpy as np
+import mygrad_amd as mg
+from mygrad_amd.nnet import log_probabilities
+for kwargs in (dict(top=1), dict(top=1, entropy=True), dict(entropy=True)):
+    for rows in (0, 2):
+        for constant in (1, "no"):
+            try:
+                log_probabilities(np.ones((rows, 5)), constant=constant, **kwargs)
+            except TypeError:
+                continue
+            raise AssertionError((kwargs, rows, constant))
+        for constant in (None, True, False):
+            log_probabilities(np.ones((rows, 5)), constant=constant, **kwargs)
+print("refused")
+"""
+    assert "refused" in run_on_standins(tmp_path, program)
+
+
 def test_one_upload_of_tokens_and_of_what_they_go_with(tmp_path):
     """Tokens are sent once, whoever takes them; what a backward pass needs is kept for those that have one."""
     program = """
