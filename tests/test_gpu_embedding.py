@@ -140,6 +140,31 @@ def test_the_same_bits_every_time(count, vocabulary):
     assert all(np.array_equal(run, runs[0]) for run in runs)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("count,vocabulary,dim", [(70_000, 50_001, 5), (5_000, 600_000, 3), (300_001, 5_003, 7), (300_001, 300, 7), (600_001, 40, 3), (2_200_000, 1_000, 2),
+                                                  (40_000, 5_003, 2050), (66_000, 3_000, 1030)])
+def test_gradients_of_many_tokens(dtype, count, vocabulary, dim):
+    """Orders by two digits, chunks of 32 to 256 tokens, and runs that end in a chunk's first tokens, go on through several of its turns, or through several
+    chunks.  Sums of whole numbers are exact, and a result is rounded once."""
+    rng = np.random.default_rng([count, vocabulary])
+    lengths = rng.choice([1, 1, 2, 3, 15, 16, 17, 31, 32, 33, 47, 48, 49, 64, 65, 300], vocabulary)
+    lengths = lengths * max(1, count // int(lengths.sum())) + rng.integers(0, 18, vocabulary)
+    ids = np.full(count, -1)
+    there = np.repeat(rng.permutation(vocabulary), lengths)[:count]
+    ids[:there.size] = there
+    ids[rng.random(count) < 0.02] = -1
+    ids = rng.permutation(ids)
+    g = rng.integers(-2, 3, (count, dim)).astype(np.int8)
+    t = mg.device_tensor(np.zeros((vocabulary, dim), dtype))
+    embedding(t, ids).backward(mg.device_tensor(g.astype(dtype), constant=True))
+    order = np.argsort(ids, kind="stable")
+    order = order[ids[order] >= 0]
+    starts = np.flatnonzero(np.diff(ids[order], prepend=-1))
+    want = np.zeros((vocabulary, dim), np.int32)
+    want[ids[order][starts]] = np.add.reduceat(g[order], starts, 0, dtype=np.int32)
+    assert np.abs(want).max() < 2**15 and np.array_equal(t.grad, want.astype(dtype))
+
+
 def test_a_table_that_is_used_twice():
     rng = np.random.default_rng(0)
     weight, g = rng.standard_normal((7, 4)), rng.standard_normal((2, 5, 4))
