@@ -81,6 +81,31 @@ def test_lengths_of_rows(dtype, dim):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [2, 7, 9, 64, 130, 511, 513, 1000, 1531, 2049, 4100, 8193, 9001, 16390, 20003, 40000, 70001])
+def test_every_value_is_taken_once(dtype, dim):
+    """Rows of zeros but for one value at an edge of what threads hold, and gradients likewise, at the same place and at another: what is left out or taken
+    twice is all there is."""
+    piece = 16 // np.dtype(dtype).itemsize
+    every = piece * (8 if dim <= 4096 else 64 if dim <= 16384 else 512)
+    at = np.arange(0, dim, every)
+    at = np.concatenate((at, at - 1, [dim // piece * piece, dim // piece * piece - 1, dim - 1]))
+    at = np.unique(at[(at >= 0) & (at < dim)])
+    rows = np.arange(len(at))
+    x = np.zeros((len(at), dim), dtype)
+    x[rows, at] = 1
+    for other in (at, np.roll(at, 1)):
+        g = np.zeros((len(at), dim), dtype)
+        g[rows, other] = 1
+        tx, tb = mg.device_tensor(x), mg.device_tensor(np.zeros(dim, dtype))
+        y = layer_norm(tx, None, tb, eps=1e-8)
+        y.backward(mg.device_tensor(g, constant=True))
+        wanted = bars(dtype, x, None, None, g, 1e-8)
+        for have, (want, bar) in zip((y.data, tx.grad, tb.grad), (wanted[0], wanted[1], wanted[3])):
+            assert outside(have, want, bar) == 0
+        assert np.abs(wanted[0][0][rows, at]).min() > 100 * np.abs(wanted[0][1][rows, at]).max()  # the bar is small next to the value
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(64,), (1, 64), (2, 3, 4, 100), (4099, 24), (700, 515), (3000, 1024), (70000, 8), (2100, 4096)])
 def test_numbers_of_rows(dtype, shape):
     check(dtype, shape)

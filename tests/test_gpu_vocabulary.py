@@ -224,6 +224,57 @@ def test_more_rows_than_a_grid_has_blocks():
     assert not loss.data.any() and not t.grad.any()
 
 
+def edges(length, item):
+    """Both sides of where a row's pieces, steps and parts may end: every 8th piece of 16 bytes, every 64th of a long row, and what the last piece begins with."""
+    piece = 16 // item
+    every = piece * (8 if length <= 4096 else 64)
+    marks = np.arange(0, length, every)
+    marks = np.concatenate((marks, marks - 1, [length // piece * piece, length // piece * piece - 1, length - 1]))
+    return np.unique(marks[(marks >= 0) & (marks < length)])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocabulary", [*((3, n) for n in (1, 2, 3, 7, 8, 33, 65, 129, 257, 513, 1000, 1024, 2049, 4096, 4100, 8191, 8200, 16385, 32003, 50000, 131101)),
+                                             *((40, n) for n in (255, 511, 2047, 70001)), *((300, n) for n in (2047, 4099, 16001, 50001)),
+                                             *((4100, n) for n in (33, 250, 500, 1000, 2047, 2050, 4095, 8191))])
+def test_every_logit_is_taken_once(dtype, rows, vocabulary):
+    """K equal logits at the edges and all others so far below that their sum is less than half a unit: probabilities of 1 / K, and one that is left out or
+    taken twice is 1 / K of the sum.  K itself is exact; its logarithm and its inverse are off by 4 u."""
+    u, r = UNIT[dtype]
+    at = edges(vocabulary, np.dtype(dtype).itemsize)
+    count, z = len(at), np.full((rows, vocabulary), -100.0, dtype)
+    z[:, at] = 3.0
+    size, ids = float(np.log(count)), at[np.arange(rows) % count].astype(np.int32)
+    assert 1 / count > 100 * 8 * u * size  # the bars are small next to a logit's part
+    ids[::5] = 0 if at[0] == 0 else -1
+    own = ids >= 0
+    rng, top = np.random.default_rng(vocabulary), min(count, 128)
+    g = rng.standard_normal((2, rows)).astype(wide(dtype))
+    t = mg.device_tensor(z)
+    out, likeliest, which = log_probabilities(t, ids, entropy=True, top=top)
+    assert np.array_equal(which.data, np.tile(at[:top], (rows, 1)))
+    close("scores", out.data, np.stack((np.where(own, -size, 0), np.full(rows, size))), 8 * u * size + 1e-30)
+    close("likeliest", likeliest.data, np.full((rows, top), -size), 8 * u * size + 1e-30)
+    alone = log_probabilities(mg.device_tensor(z, constant=True), ids)  # by other kernels where rows are short
+    close("scores alone", alone.data, np.where(own, -size, 0), 8 * u * size + 1e-30)
+    out.backward(mg.device_tensor(g, constant=True))
+    want = np.zeros((rows, vocabulary))
+    want[:, at] = -(g[0] * own)[:, None] / count
+    want[np.arange(rows), ids] += g[0] * own
+    given = np.abs(g[0])[:, None] + np.abs(g[1])[:, None]
+    close("dz", t.grad, want, 8 * u * given * (want != 0) + 1e-30 * given + r * np.abs(want) + SMALLEST[dtype])
+    taught = at[np.unique(np.linspace(0, count - 1, 4).astype(int))] if count >= 4 else at[:1]
+    few = len(taught)
+    for per in (1.0, 2.0):
+        t = mg.device_tensor(z)
+        loss = distillation(t, np.tile(taught, (rows, 1)), np.full((rows, few), 2.0, dtype), temperature=1 / per)
+        loss.backward(mg.device_tensor(g[0], constant=True))
+        close("loss", loss.data, np.full(rows, size - np.log(few)), 16 * u * (size + np.log(few)) + 1e-30)
+        want[:], want[:, at] = 0, (g[0] * per / count)[:, None]
+        want[:, taught] -= (g[0] * per / few)[:, None]
+        close("dz of distillation", t.grad, want, 16 * u * per * given * (want != 0) + 1e-30 * given + r * np.abs(want) + 2 * SMALLEST[dtype])
+
+
 def test_leading_shapes():
     z = made(12, 50)
     flat = log_probabilities(z, np.arange(12), entropy=True, top=2)
