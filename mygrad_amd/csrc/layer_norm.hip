@@ -365,8 +365,8 @@ __global__ void __launch_bounds__(kThreads<WAVES>) layer_norm_rows_bwd_kernel(La
 struct Shape {
   int waves, pieces, lanes;
 };
-template <typename T>
-Shape shape_of(long long D, bool back) {
+template <typename T, bool BACK>
+Shape shape_of(long long D) {
   const long long pieces = ceil_div(D, Piece<T>::V);
   Shape s{0, 0, 64};
   if (pieces <= 64) {
@@ -378,14 +378,14 @@ Shape shape_of(long long D, bool back) {
     s = Shape{4, 2, 64};
   } else if (pieces <= 1024) {
     s = sizeof(T) == 2 ? Shape{16, 1, 64} : Shape{4, 4, 64};  // 85 us and 95 back in float16, 84 and 80 in float32
-  } else if (pieces <= (back && sizeof(T) == 2 ? 2048 : 4096)) {  // four pieces' sums of float16 do not fit: 265 us back, 190 by the kernels for longer rows
+  } else if (pieces <= (BACK && sizeof(T) == 2 ? 2048 : 4096)) {  // four pieces' sums of float16 do not fit: 265 us back, 190 by the kernels for longer rows
     s = Shape{16, pieces <= 2048 ? 2 : 4, 64};
   }
   return s;
 }
 
 // Calls f with a Shape's numbers of wavefronts and pieces as constants.
-template <typename T, typename F>
+template <typename T, bool BACK, typename F>
 void with_shape(const Shape &s, F f) {
   typedef std::integral_constant<int, 1> One;
   typedef std::integral_constant<int, 2> Two;
@@ -401,19 +401,21 @@ void with_shape(const Shape &s, F f) {
     if (s.waves == 4 && s.pieces == 4) f(Four{}, Four{});
   }
   if (s.waves == 16 && s.pieces == 2) f(Sixteen{}, Two{});
-  if (s.waves == 16 && s.pieces == 4) f(Sixteen{}, Four{});
+  if constexpr (!BACK || sizeof(T) > 2) {
+    if (s.waves == 16 && s.pieces == 4) f(Sixteen{}, Four{});
+  }
 }
 
 template <typename T, typename C>
 int forward(const LayerNorm &p, const void *x, const void *w, const void *b, void *y, void *kept) {
   ScopedTiming timed(TAG_LAYER_NORM);
   hipStream_t s = runtime().stream;
-  const Shape shape = shape_of<T>(p.D, false);
+  const Shape shape = shape_of<T, false>(p.D);
   if (shape.waves) {
     // eight blocks of 256 a compute unit, or as many threads in larger or smaller ones
     const long long most = (shape.waves == 1 ? 8 : 32 / shape.waves) * runtime().props.multiProcessorCount;
     const long long blocks = std::min<long long>(ceil_div(p.rows, shape.waves == 1 ? 256 / shape.lanes : 1), most);
-    with_shape<T>(shape, [&](auto waves, auto pieces) {
+    with_shape<T, false>(shape, [&](auto waves, auto pieces) {
       layer_norm_rows_kernel<T, C, waves, pieces><<<dim3((unsigned)blocks), dim3(kThreads<waves>), 0, s>>>(p, shape.lanes, (const T *)x, (const T *)w,
                                                                                                           (const T *)b, (T *)y, (Moments<C> *)kept);
     });
@@ -429,7 +431,7 @@ template <typename T, typename C>
 int backward(const LayerNorm &p, const void *x, const void *w, const void *kept, const void *grad, void *dx, void *dw, void *db) {
   hipStream_t s = runtime().stream;
   const bool columns = dw || db;
-  const Shape shape = shape_of<T>(p.D, true);
+  const Shape shape = shape_of<T, true>(p.D);
   void *space = nullptr;
   if (shape.waves) {
     // Each block's sums are written once and read once: four blocks of 256 a compute unit (or as many threads) where a thread has one piece, two
@@ -441,7 +443,7 @@ int backward(const LayerNorm &p, const void *x, const void *w, const void *kept,
     if (columns)
       if (const int rc = workspace((size_t)(2 * blocks * p.D) * sizeof(C), &space)) return rc;
     ScopedTiming timed(TAG_LAYER_NORM_BWD);
-    with_shape<T>(shape, [&](auto waves, auto pieces) {
+    with_shape<T, true>(shape, [&](auto waves, auto pieces) {
       layer_norm_rows_bwd_kernel<T, C, waves, pieces><<<dim3((unsigned)blocks), dim3(kThreads<waves>), 0, s>>>(
           p, shape.lanes, (const T *)x, (const T *)w, (const T *)grad, (const Moments<C> *)kept, (T *)dx, (C *)space);
     });
