@@ -34,9 +34,10 @@ int lanes_of(long long pieces) {
   return lanes;
 }
 
-// A group of threads takes AT_ONCE tokens, whose rows are on their way together.  Where they are more than 60 MB they are stored past the last-level
-// cache (PAST), which the table has a better use for.  The same table of 205 MB of halves each time, us alone, with a pass over the rows behind it, and with the gradient and passes
-// over both: 16384 rows of 2048 15, 32 and 155, past it 13, 32 and 150; 100000 rows 83, 213 and 459, 64, 165 and 411; 2000 rows 12, 22 and 95 either way.
+// A group of threads takes AT_ONCE tokens, whose rows are on their way together.  Where they are more than 40 MB they are stored past the last-level
+// cache (PAST), which the table has a better use for.  The same table of 205 MB of halves each time, us alone, with a pass over the rows behind it, and with the
+// gradient and passes over both, first as usual and then past it: rows of 16 MB 10.6, 21 and 95 either way, 32 MB 11, 24 and 109, 108; 48 MB 11.5, 24 and 126, 10.5, 24
+// and 123; 56 MB 12.8, 26 and 136, 10.6, 26 and 133; 80 MB 17, 35 and 169, 14, 35 and 163; 128 MB 26, 51 and 225, 21, 51 and 220; 410 MB 85, 205 and 456, 64, 142 and 405.
 template <typename T, int AT_ONCE, bool PAST>
 __global__ void __launch_bounds__(256) embedding_kernel(Embedding p, int lanes, const int32_t *__restrict__ ids, const T *__restrict__ weight,
                                                         T *__restrict__ out) {
@@ -473,7 +474,7 @@ int forward(const Embedding &p, const int32_t *ids, const void *weight, void *ou
   const int lanes = lanes_of(ceil_div(p.D, Piece<T>::V)), groups = 256 / lanes;
   // several rows a group where that leaves eight blocks a compute unit
   const bool many = p.tokens >= 4ll * groups * 8 * runtime().props.multiProcessorCount;
-  const bool past = (double)p.tokens * p.D * sizeof(T) > 6e7;
+  const bool past = (double)p.tokens * p.D * sizeof(T) > 4e7;
   auto kernel = many ? past ? embedding_kernel<T, 4, true> : embedding_kernel<T, 4, false>
                      : past ? embedding_kernel<T, 1, true> : embedding_kernel<T, 1, false>;
   // A launch has fewer than 2^32 threads; rows that a block takes four of at a time reach that with 2^26 - 3 tokens.
