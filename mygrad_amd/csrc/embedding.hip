@@ -1,10 +1,11 @@
 // Rows of a table by token, and the gradient of the table, for gfx950.
 //
-//   y[n] = scale W[ids[n]]  (zeros where ids[n] < 0)          dW[v] = scale * sum of grad[n] over the n with ids[n] = v, in their order
+//   y[n] = scale W[ids[n]]  (zeros where ids[n] < 0)          dW[v] = scale * sum of grad[n] over the n with ids[n] = v
 //
-// Both are bound by memory.  The gradient sorts the tokens, so that the rows to be added lie in a run, whatever the text: a run is cut
-// into chunks of a few rows that are summed side by side, and what a cut went through is joined in order.  Rows that no token names are zeros, which
-// all rows are filled with first.  Nothing is added by atomics: the same bits every time.
+// Both are bound by memory.  The gradient sorts the tokens, so that the rows to be added lie in a run, whatever the text: the sorted list is cut
+// into chunks of 16 to 256 tokens that are summed side by side, in the order of the tokens, and of a run that cuts go through the sums of chunks are joined in four
+// shares.  Where the cuts lie hangs on all tokens of the call, and with it the last bits of a row.  Rows that no token names are zeros, which
+// all rows are filled with first.  Nothing is added by atomics: the same call gives the same bits every time.
 #include "row_device.h"
 
 #include <algorithm>
@@ -267,7 +268,8 @@ __global__ void __launch_bounds__(1024) order_kernel(Owners p) {
   }
 }
 
-// More tokens than a block takes: for each digit the blocks count theirs, then each finds its places from all counts.
+// More tokens than a block takes: for each digit the blocks count theirs, then each finds its places from all counts.  These are read by every
+// block, the square of the blocks' number in all, which shows from millions of tokens on (2048 blocks for 2^23 tokens, 4 KB of counts each).
 constexpr int kTileK = 4;
 constexpr int kTile = 1024 * kTileK;
 

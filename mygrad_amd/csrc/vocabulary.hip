@@ -59,8 +59,9 @@ __device__ __forceinline__ uint64_t order_of(double z) {
 __device__ __forceinline__ float value_of(uint32_t order) { return __builtin_bit_cast(float, order >> 31 ? order & 0x7fffffffu : ~order); }
 __device__ __forceinline__ double value_of(uint64_t order) { return __builtin_bit_cast(double, order >> 63 ? order & ~(1ull << 63) : ~order); }
 
-// The exponential of a number that is not positive.  The result of float16 is rounded to 11 bits, so the instruction's own is enough
-// there: an argument rounded in single precision, |x| 2^-24 of the result.
+// The exponential of a number that is not positive.  For logits of float16 it is the instruction's own, of an argument rounded in single precision: off by
+// |x| 2^-24 of itself.  A gradient is rounded to 11 bits after that.  The results of the sums are not, but there the terms weigh it: s is off by |a| 2^-24 of
+// itself, where |a| is at most log V, which is what the rounding of t leaves of it, too.
 template <typename T>
 __device__ __forceinline__ float exponential(float x) {
   return sizeof(T) == 2 ? __builtin_amdgcn_exp2f(x * 1.4426950408889634f) : expf(x);
@@ -110,9 +111,9 @@ __device__ __forceinline__ C base_of(C m) {
 }
 
 // t and e^t as the sums take them.  In single precision t is held at -104 and above (a NaN stays one), where the exponential is less than half of
-// the smallest number, so zero.  With n = round(t log2 e), made by adding 1.5 2^23, 2^(t log2 e - n) is the instruction's, to a unit or two, and the
-// result is that times 2^n: nine instructions where the library's function has thirteen.  1021 x 32003 logits with entropies and alternatives take
-// 34 us so, 40 with that.
+// the smallest number, so zero.  A Cody-Waite reduction: with n = round(t log2 e), made by adding 1.5 2^23, and log2 e in two parts, 2^(t log2 e - n) is the
+// instruction's, to a unit or two, and the result is that times 2^n: nine instructions where the library's function has thirteen.  1021 x 32003 logits with
+// entropies and alternatives take 34 us so, 40 with that.
 template <typename T>
 __device__ __forceinline__ float term(float &t) {
   if constexpr (sizeof(T) == 2) {

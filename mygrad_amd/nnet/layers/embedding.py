@@ -157,8 +157,9 @@ def embedding(weight, tokens, *, scale: float = 1.0, constant: Optional[bool] = 
 
     ``weight`` is float16, float32 or float64.  ``tokens`` are whole numbers of any shape, less than ``vocabulary``; -1 stands for
     no token, whose row is zeros.  :class:`TokenIds` are checked and sent to the device once, any other array in each call.
-    The gradient of ``weight`` is an array of its shape; the rows of a token that occurs more than once are added in the order
-    of the tokens, in float32 (float64 for float64), and a result is rounded once.
+    The gradient of ``weight`` is an array of its shape; the rows of a token that occurs more than once are added in float32
+    (float64 for float64), and a result is rounded once.  The same call gives the same bits every time; in which order rows are added
+    hangs on all tokens of the call.
 
     >>> import mygrad_amd as mg
     >>> from mygrad_amd.nnet import embedding
