@@ -431,6 +431,13 @@ template <typename T, typename C>
 int backward(const LayerNorm &p, const void *x, const void *w, const void *kept, const void *grad, void *dx, void *dw, void *db) {
   hipStream_t s = runtime().stream;
   const bool columns = dw || db;
+  if (p.rows == 0) {  // sums of no rows
+    if (!columns) return MG_OK;
+    ScopedTiming timed(TAG_LAYER_NORM_BWD);
+    layer_norm_join_kernel<T, double><<<dim3((unsigned)ceil_div(p.D, 64), 2), dim3(1024), 0, s>>>(p.D, 0, nullptr, (T *)dw, (T *)db);
+    MG_HIP(hipGetLastError());
+    return MG_OK;
+  }
   const Shape shape = shape_of<T, true>(p.D);
   void *space = nullptr;
   if (shape.waves) {
@@ -507,14 +514,7 @@ int mg_layer_norm_bwd(int dtype, int64_t rows, int64_t D, const void *x, const v
   const int rc = check(dtype, rows, D, 0, "mg_layer_norm_bwd");
   if (rc) return rc;
   if (!dx && !dweight && !dbias) return fail(MG_ERR_BAD_ARG, "mg_layer_norm_bwd: no gradient is wanted");
-  if (rows == 0) {
-    const size_t bytes = (size_t)D * (dtype == MG_F64 ? 8 : dtype == MG_F32 ? 4 : 2);
-    for (void *out : {dweight, dbias})
-      if (out)
-        if (const int status = mg_memset_zero(out, bytes)) return status;
-    return MG_OK;
-  }
-  if (!x || !grad || !kept) return fail(MG_ERR_BAD_ARG, "null pointer in mg_layer_norm_bwd");
+  if (rows && (!x || !grad || !kept)) return fail(MG_ERR_BAD_ARG, "null pointer in mg_layer_norm_bwd");
   const LayerNorm p{rows, D, 0};
   if (dtype == MG_F64) return backward<double, double>(p, x, weight, kept, grad, dx, dweight, dbias);
   if (dtype == MG_F32) return backward<float, float>(p, x, weight, kept, grad, dx, dweight, dbias);

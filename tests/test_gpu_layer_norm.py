@@ -235,6 +235,23 @@ def test_memory_that_begins_anywhere(dtype, dim):
             assert (held[:shift] == 7).all() and (held[shift + want.size:] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [1, 33, 5000])
+def test_sums_over_no_rows_wherever_they_begin(dtype, dim):
+    from mygrad_amd import _device, _hip
+
+    item = np.dtype(dtype).itemsize
+    for shift in (0, 1, 3):
+        bufs = [_device.from_host(np.full(dim + 16, 7, dtype)).buf for _ in range(2)]
+        for given in ((0, 1), (0,), (1,)):
+            pdw, pdb = (bufs[n].ptr + shift * item if n in given else None for n in range(2))
+            _hip.check(_hip.lib().mg_layer_norm_bwd(_hip.storage_code(dtype), 0, dim, None, None, None, None, None, pdw, pdb))
+        for buf in bufs:
+            held = np.empty(dim + 16, dtype)
+            buf.download_into(held)
+            assert not held[shift:shift + dim].any() and (held[:shift] == 7).all() and (held[shift + dim:] == 7).all()
+
+
 def test_entry_points_refuse_bad_arguments():
     from mygrad_amd import _device, _hip
 
