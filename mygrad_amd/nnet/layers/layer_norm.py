@@ -103,7 +103,8 @@ def layer_norm(x, weight=None, bias=None, *, eps: float, constant: Optional[bool
 
     ``weight`` and ``bias`` are ``(dim,)`` in the dtype of ``x`` (float16, float32 or float64), or None; ``eps`` is a
     non-negative number and has no default.  Sums are carried in float32 (float64 for float64), the gradients of
-    ``weight`` and ``bias`` are joined in float64, and each result is rounded once.
+    ``weight`` and ``bias`` are joined in float64, and each result is rounded once.  A row whose squared deviations add up to more than
+    float32 (float64) holds, 3e38, is scaled by 0.
 
     >>> import mygrad_amd as mg
     >>> from mygrad_amd.nnet import layer_norm
